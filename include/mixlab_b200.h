@@ -311,6 +311,104 @@ MXB_API mxb_status mxb_mamba3_block_post_bwd(const mxb_mamba3_desc* d, float eps
                                      void* stream);
 
 /* ------------------------------------------------------------------------
+ * Serving: the Mamba-3 recurrence and the short convolution on a pool of states.
+ * The reference replays the whole prefix for every new token (train/generate.go:87-147);
+ * these keep what the recurrence needs of the past.
+ *
+ * The pool.  Each of its `slots` rows is one sequence's state:
+ *   h       [slots, D, N]        float32: h_t of the recurrence
+ *   phase   [slots, nheads, 2]   float32 (per-channel layout: [slots, D, N/2, 2]): cosine
+ *                                and sine of the angle phi_t, a unit vector
+ *   x_prev  [slots, D]           io_dtype: x of the last token
+ *   b_prev  [slots, nheads, N]   io_dtype (per-channel layout: [slots, G, N]): b of the last
+ *                                token, for each head that of its group
+ * A sequence that starts needs nothing in its row.  `slot` [S] int32 gives each sequence's
+ * row (NULL: sequence i has row i); rows of one call must be different.  A negative number
+ * or one beyond the pool is a padding entry: a prompt then runs from nothing and keeps no
+ * state, a single token is passed over and its row of y stays as it was.
+ *
+ * prefill: packed prompts.  rows = tokens of the call; sequence i is rows cu_seqlens[i] ..
+ * cu_seqlens[i+1] - 1 ([S+1] int32 on the device, not falling, within rows).  Where go_on[i]
+ * is nonzero (go_on NULL: nowhere) the sequence goes on from its state; the others start from
+ * nothing, whatever their row holds.  The row then holds the state behind the sequence's last
+ * token; that of a sequence without tokens stays as it was.  Rows of y that belong to no
+ * sequence stay as they were.
+ * decode_step: one token of each of S sequences (rows = S), all of which go on.
+ *
+ * desc: D channels, N states (even, <= 256), G groups; nheads > 0: head layout (dt, lambda,
+ * theta [rows, nheads], a_log [nheads]; nheads a multiple of G, D of nheads), 0: per-channel
+ * layout (dt, lambda [rows, D], theta [rows, D, N/2], a_log [D, N]).  x, y [rows, D], b, c
+ * [rows, G, N] in io_dtype.  h, phase and the workspace must be 16-byte aligned
+ * (MXB_ERR_ALIGNMENT).  flags: MXB_MAMBA3_RECURRENT_KERNELS, MXB_MAMBA3_SERIAL_WALK (never cut
+ * a sequence).  Every sum has a fixed order.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+  int32_t rows, S, slots, D, N, G, nheads, io_dtype, flags;
+} mxb_mamba3_serve_desc;
+typedef struct {
+  float *h, *phase;
+  void *x_prev, *b_prev;
+} mxb_mamba3_state;
+
+MXB_API size_t mxb_mamba3_prefill_workspace_bytes(const mxb_mamba3_serve_desc* d);
+MXB_API mxb_status mxb_mamba3_prefill(const mxb_mamba3_serve_desc* d, const void* x, const float* dt,
+                              const float* lambda, const float* theta, const float* a_log, const void* b,
+                              const void* c, const int32_t* cu_seqlens, const int32_t* slot,
+                              const uint8_t* go_on, const mxb_mamba3_state* state, void* y, void* workspace,
+                              size_t workspace_bytes, void* stream);
+MXB_API mxb_status mxb_mamba3_decode_step(const mxb_mamba3_serve_desc* d, const mxb_mamba3_state* state,
+                                  const void* x, const float* dt, const float* lambda, const float* theta,
+                                  const float* a_log, const void* b, const void* c, const int32_t* slot,
+                                  void* y, void* stream);
+
+/* The causal depthwise convolution in front of both scans (emitGatedDeltaNetShortConv1D,
+ * arch/blocks_gated_deltanet.go:345-368; causal_depthwise_conv1d, gpu/ir.cpp:1397-1425) on a
+ * pool of the last inputs, conv_state [slots, K-1, D] in io_dtype, oldest first:
+ *   y_t = act(sum_k w[:, k] x_{t-k} + bias)
+ * w(d, k) = w[d w_stride_d + k w_stride_k] float32, so that both blocks' weights ([D, K] and
+ * [K, D]) serve as they are; bias [D] may be NULL.  K <= 4.  cu_seqlens, slot, go_on and their
+ * rules as above. */
+enum { MXB_ACT_NONE = 0, MXB_ACT_SILU = 1 };
+typedef struct {
+  int32_t rows, S, slots, D, K, io_dtype, activation;
+  int64_t w_stride_d, w_stride_k;
+} mxb_short_conv_desc;
+MXB_API mxb_status mxb_short_conv_prefill(const mxb_short_conv_desc* d, const void* x, const float* w,
+                                  const float* bias, const int32_t* cu_seqlens, const int32_t* slot,
+                                  const uint8_t* go_on, void* conv_state, void* y, void* stream);
+MXB_API mxb_status mxb_short_conv_step(const mxb_short_conv_desc* d, void* conv_state, const void* x,
+                               const float* w, const float* bias, const int32_t* slot, void* y, void* stream);
+
+/* ------------------------------------------------------------------------
+ * The residual stream between two blocks (the RMSNorm in front of a block and the addition
+ * behind it, gpu/ir.cpp:2076, :2104), fused with an optional norm and SiLU gate of the block's
+ * output and a residual scale:
+ *   a = RMSNorm(y; post_norm) SiLU(z);  resid_out = resid + scale a;  n = RMSNorm(resid_out; norm)
+ * resid, resid_out [rows, D] in resid_dtype (io_dtype or MXB_F32); y, z, n [rows, D] in
+ * io_dtype; norm, post_norm, scale [D] float32.  post_norm, z, scale may be NULL (no norm, no
+ * gate, scale 1).  D <= 16384.  resid_out may be resid itself.  n is the norm of resid_out
+ * before it is rounded to resid_dtype.
+ * bwd: resid_out is what the forward returned, d_resid_out (may be NULL: zero) the gradient
+ * that reaches it from its other readers, dn that of n.  Every gradient: d_resid (resid_dtype),
+ * dy, dz (io_dtype), dnorm, dpost_norm, dscale [D] float32; dz, dpost_norm, dscale belong to
+ * operands that may be absent.  d_resid may be d_resid_out itself.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+  int64_t rows;
+  int32_t D, io_dtype, resid_dtype;
+  float eps;
+} mxb_residual_norm_desc;
+MXB_API size_t mxb_residual_norm_workspace_bytes(const mxb_residual_norm_desc* d);
+MXB_API mxb_status mxb_residual_norm_fwd(const mxb_residual_norm_desc* d, const void* resid, const void* y,
+                                 const float* norm, const float* post_norm, const void* z,
+                                 const float* scale, void* resid_out, void* n, void* stream);
+MXB_API mxb_status mxb_residual_norm_bwd(const mxb_residual_norm_desc* d, const void* resid_out, const void* y,
+                                 const float* norm, const float* post_norm, const void* z,
+                                 const float* scale, const void* d_resid_out, const void* dn, void* d_resid,
+                                 void* dy, void* dz, float* dnorm, float* dpost_norm, float* dscale,
+                                 void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * Data-parallel gradient exchange: the element-wise passes on either side of the
  * per-bucket all-reduce, over flat float32 buckets on the device (the collective
  * itself is the caller's: NCCL).  They fuse what the reference does op by op per

@@ -24,6 +24,7 @@ MXB_MAMBA3_BWD_USE_SAVED = 8
 MXB_MAMBA3_NO_TMA = 16
 MXB_MAMBA3_SERIAL_WALK = 32
 MXB_MAMBA3_WINDOW_PARALLEL = 64
+MXB_ACT_NONE, MXB_ACT_SILU = 0, 1
 
 
 class MxbError(RuntimeError):
@@ -38,6 +39,24 @@ class GdnDesc(C.Structure):
 
 class Mamba3Desc(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("B", "T", "D", "N", "G", "nheads", "io_dtype", "flags")]
+
+
+class Mamba3ServeDesc(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("rows", "S", "slots", "D", "N", "G", "nheads", "io_dtype", "flags")]
+
+
+class Mamba3StatePointers(C.Structure):
+    """mxb_mamba3_state: device pointers of a pool of recurrent states."""
+    _fields_ = [(n, C.c_void_p) for n in ("h", "phase", "x_prev", "b_prev")]
+
+
+class ShortConvDesc(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("rows", "S", "slots", "D", "K", "io_dtype", "activation")] + [
+        ("w_stride_d", C.c_int64), ("w_stride_k", C.c_int64)]
+
+
+class ResidualNormDesc(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("D", C.c_int32), ("io_dtype", C.c_int32), ("resid_dtype", C.c_int32), ("eps", C.c_float)]
 
 
 class IrOp(C.Structure):
@@ -81,6 +100,14 @@ EXPORTS = {
     "mxb_mamba3_block_bc_bwd": (C.c_int32, [C.POINTER(Mamba3Desc), C.c_float] + [_P] * 13 + [C.c_size_t, _P]),
     "mxb_mamba3_block_post_fwd": (C.c_int32, [C.POINTER(Mamba3Desc), C.c_float] + [_P] * 5),
     "mxb_mamba3_block_post_bwd": (C.c_int32, [C.POINTER(Mamba3Desc), C.c_float] + [_P] * 8 + [C.c_size_t, _P]),
+    "mxb_mamba3_prefill_workspace_bytes": (C.c_size_t, [C.POINTER(Mamba3ServeDesc)]),
+    "mxb_mamba3_prefill": (C.c_int32, [C.POINTER(Mamba3ServeDesc)] + [_P] * 10 + [C.POINTER(Mamba3StatePointers), _P, _P, C.c_size_t, _P]),
+    "mxb_mamba3_decode_step": (C.c_int32, [C.POINTER(Mamba3ServeDesc), C.POINTER(Mamba3StatePointers)] + [_P] * 10),
+    "mxb_short_conv_prefill": (C.c_int32, [C.POINTER(ShortConvDesc)] + [_P] * 9),
+    "mxb_short_conv_step": (C.c_int32, [C.POINTER(ShortConvDesc)] + [_P] * 7),
+    "mxb_residual_norm_workspace_bytes": (C.c_size_t, [C.POINTER(ResidualNormDesc)]),
+    "mxb_residual_norm_fwd": (C.c_int32, [C.POINTER(ResidualNormDesc)] + [_P] * 9),
+    "mxb_residual_norm_bwd": (C.c_int32, [C.POINTER(ResidualNormDesc)] + [_P] * 15 + [C.c_size_t, _P]),
     "mxb_dp_partial_floats": (C.c_size_t, []),
     "mxb_dp_sanitize": (C.c_int32, [_P, C.c_size_t, C.c_float, _P, _P]),
     "mxb_dp_finalize": (C.c_int32, [_P, C.c_size_t, C.c_float, C.c_float, _P, _P, _P]),

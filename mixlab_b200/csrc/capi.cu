@@ -12,6 +12,7 @@
 #include <vector>
 
 #include "common.cuh"
+#include "mamba3_serve.cuh"
 
 namespace mxb {
 
@@ -117,6 +118,13 @@ mxb_status gdn_block_pre_bwd(const mxb_gdn_desc*, const void*, const void*, cons
                              float*, float*, float*, float*, float*, void*, cudaStream_t);
 mxb_status gdn_block_post(const mxb_gdn_desc*, const void*, const void*, const float*, void*, const void*, void*, void*,
                           float*, void*, cudaStream_t);
+mxb_status short_conv(const mxb_short_conv_desc*, const void*, const float*, const float*, const int32_t*, const int32_t*,
+                      const unsigned char*, void*, void*, cudaStream_t);
+size_t residual_norm_scratch(const mxb_residual_norm_desc*);
+mxb_status residual_norm_fwd(const mxb_residual_norm_desc*, const void*, const void*, const float*, const float*, const void*,
+                             const float*, void*, void*, cudaStream_t);
+mxb_status residual_norm_bwd(const mxb_residual_norm_desc*, const void*, const void*, const float*, const float*, const void*,
+                             const float*, const void*, const void*, void*, void*, void*, float*, float*, float*, float*, cudaStream_t);
 bool mamba3_block_supported(const mxb_mamba3_desc*);
 size_t mamba3_block_workspace_bytes(const mxb_mamba3_desc*);
 mxb_status mamba3_block_conv(const mxb_mamba3_desc*, int, const void*, const float*, void*, const void*, void*, float*,
@@ -398,6 +406,142 @@ mxb_status mxb_mamba3_bwd(const mxb_mamba3_desc* d, const void* x, const float* 
   if (!workspace || workspace_bytes < need) return MXB_ERR_WORKSPACE;
   return mamba3_bwd(d, x, dt, lambda, theta, a_log, b, c, dy, dx, ddt, dlambda, dtheta, da_log, db, dc,
                     workspace, static_cast<cudaStream_t>(stream));
+}
+
+// ---------------------------------------------------------------- serving
+static mxb_status serve_params(const mxb_mamba3_serve_desc* d, ServeP* p) {
+  if (!d) return MXB_ERR_INVALID_ARGUMENT;
+  if (d->rows < 0 || d->S < 0 || d->slots < 0 || d->D <= 0 || d->N <= 0 || d->G <= 0 || d->nheads < 0) return MXB_ERR_INVALID_ARGUMENT;
+  if (d->io_dtype != MXB_F32 && d->io_dtype != MXB_BF16) return MXB_ERR_INVALID_ARGUMENT;
+  if (d->N % 2 || d->N > 256 || d->D % d->G) return MXB_ERR_UNSUPPORTED;
+  if (d->nheads > 0 && (d->D % d->nheads || d->nheads % d->G)) return MXB_ERR_UNSUPPORTED;
+  // (grids: heads and channels run along an axis of 65,535 blocks, sequences times heads along one of 2^31)
+  if (d->D > 65535 || d->S > (1 << 20) || (int64_t)d->S * d->D >= (int64_t)1 << 31) return MXB_ERR_UNSUPPORTED;
+  *p = ServeP{};
+  p->rows = d->rows; p->S = d->S; p->slots = d->slots; p->D = d->D; p->N = d->N; p->G = d->G; p->NH = d->nheads;
+  p->Kp = d->N / 2; p->P = d->nheads > 0 ? d->D / d->nheads : 1;
+  return MXB_OK;
+}
+static mxb_status serve_state(const mxb_mamba3_state* s, ServeP* p) {
+  if (!s) return MXB_ERR_INVALID_ARGUMENT;
+  if (p->slots > 0 && (!s->h || !s->phase || !s->x_prev || !s->b_prev)) return MXB_ERR_INVALID_ARGUMENT;
+  if (!aligned16(s->h) || !aligned16(s->phase)) return MXB_ERR_ALIGNMENT;
+  p->h = s->h; p->phase = reinterpret_cast<float2*>(s->phase); p->x_prev = s->x_prev; p->b_prev = s->b_prev;
+  return MXB_OK;
+}
+static mxb_status serve_operands(ServeP* p, const void* x, const float* dt, const float* lambda, const float* theta, const float* a_log,
+                                 const void* b, const void* c, const int32_t* slot, void* y) {
+  if (!x || !dt || !lambda || !theta || !a_log || !b || !c || !y) return MXB_ERR_INVALID_ARGUMENT;
+  if (!p->NH && !aligned16(a_log)) return MXB_ERR_ALIGNMENT;
+  p->x = x; p->dt = dt; p->lam = lambda; p->theta = theta; p->a_log = a_log; p->b = b; p->c = c; p->slot = slot; p->y = y;
+  return MXB_OK;
+}
+size_t mxb_mamba3_prefill_workspace_bytes(const mxb_mamba3_serve_desc* d) {
+  ServeP p;
+  return serve_params(d, &p) == MXB_OK ? m3walk_scratch(p, d->io_dtype == MXB_F32, d->flags, nullptr) : 0;
+}
+mxb_status mxb_mamba3_prefill(const mxb_mamba3_serve_desc* d, const void* x, const float* dt, const float* lambda, const float* theta,
+                              const float* a_log, const void* b, const void* c, const int32_t* cu_seqlens, const int32_t* slot,
+                              const uint8_t* go_on, const mxb_mamba3_state* state, void* y, void* workspace,
+                              size_t workspace_bytes, void* stream) {
+  ServeP p;
+  mxb_status s = serve_params(d, &p);
+  if (s != MXB_OK) return s;
+  if (p.rows == 0 || p.S == 0) return MXB_OK;
+  if (!cu_seqlens) return MXB_ERR_INVALID_ARGUMENT;
+  if ((s = serve_state(state, &p)) != MXB_OK) return s;
+  if ((s = serve_operands(&p, x, dt, lambda, theta, a_log, b, c, slot, y)) != MXB_OK) return s;
+  p.cu = cu_seqlens;
+  p.go = go_on;
+  const bool f32 = d->io_dtype == MXB_F32;
+  const size_t need = m3walk_scratch(p, f32, d->flags, nullptr);
+  if (need) {
+    if (!workspace || workspace_bytes < need) return MXB_ERR_WORKSPACE;
+    if (!aligned16(workspace)) return MXB_ERR_ALIGNMENT;
+    m3walk_scratch(p, f32, d->flags, static_cast<char*>(workspace));
+  }
+  return m3walk_prefill(p, f32, static_cast<cudaStream_t>(stream));
+}
+mxb_status mxb_mamba3_decode_step(const mxb_mamba3_serve_desc* d, const mxb_mamba3_state* state, const void* x, const float* dt,
+                                  const float* lambda, const float* theta, const float* a_log, const void* b, const void* c,
+                                  const int32_t* slot, void* y, void* stream) {
+  ServeP p;
+  mxb_status s = serve_params(d, &p);
+  if (s != MXB_OK) return s;
+  if (p.S == 0) return MXB_OK;
+  if ((s = serve_state(state, &p)) != MXB_OK) return s;
+  if ((s = serve_operands(&p, x, dt, lambda, theta, a_log, b, c, slot, y)) != MXB_OK) return s;
+  return m3serve_step(p, d->io_dtype == MXB_F32, static_cast<cudaStream_t>(stream));
+}
+
+static mxb_status check_conv_desc(const mxb_short_conv_desc* d) {
+  if (!d) return MXB_ERR_INVALID_ARGUMENT;
+  if (d->rows < 0 || d->S < 0 || d->slots < 0 || d->D <= 0 || d->K <= 0) return MXB_ERR_INVALID_ARGUMENT;
+  if (d->io_dtype != MXB_F32 && d->io_dtype != MXB_BF16) return MXB_ERR_INVALID_ARGUMENT;
+  if (d->activation != MXB_ACT_NONE && d->activation != MXB_ACT_SILU) return MXB_ERR_INVALID_ARGUMENT;
+  if (d->K > 4) return MXB_ERR_UNSUPPORTED;
+  return MXB_OK;
+}
+mxb_status mxb_short_conv_prefill(const mxb_short_conv_desc* d, const void* x, const float* w, const float* bias,
+                                  const int32_t* cu_seqlens, const int32_t* slot, const uint8_t* go_on, void* conv_state, void* y,
+                                  void* stream) {
+  const mxb_status s = check_conv_desc(d);
+  if (s != MXB_OK) return s;
+  if (d->rows == 0 || d->S == 0) return MXB_OK;
+  if (!x || !w || !y || !cu_seqlens || (!conv_state && d->slots > 0 && d->K > 1)) return MXB_ERR_INVALID_ARGUMENT;
+  return short_conv(d, x, w, bias, cu_seqlens, slot, go_on, conv_state, y, static_cast<cudaStream_t>(stream));
+}
+mxb_status mxb_short_conv_step(const mxb_short_conv_desc* d, void* conv_state, const void* x, const float* w, const float* bias,
+                               const int32_t* slot, void* y, void* stream) {
+  const mxb_status s = check_conv_desc(d);
+  if (s != MXB_OK) return s;
+  if (d->S > 65535) return MXB_ERR_UNSUPPORTED;
+  if (d->S == 0) return MXB_OK;
+  if (!x || !w || !y || (!conv_state && d->slots > 0 && d->K > 1)) return MXB_ERR_INVALID_ARGUMENT;
+  return short_conv(d, x, w, bias, nullptr, slot, nullptr, conv_state, y, static_cast<cudaStream_t>(stream));
+}
+
+// ---------------------------------------------------------------- residual stream
+static mxb_status check_norm_desc(const mxb_residual_norm_desc* d) {
+  if (!d) return MXB_ERR_INVALID_ARGUMENT;
+  if (d->rows < 0 || d->D <= 0 || !(d->eps >= 0.f)) return MXB_ERR_INVALID_ARGUMENT;
+  if (d->io_dtype != MXB_F32 && d->io_dtype != MXB_BF16) return MXB_ERR_INVALID_ARGUMENT;
+  if (d->resid_dtype != MXB_F32 && d->resid_dtype != d->io_dtype) return MXB_ERR_INVALID_ARGUMENT;
+  if (d->D > 16384) return MXB_ERR_UNSUPPORTED;
+  return MXB_OK;
+}
+size_t mxb_residual_norm_workspace_bytes(const mxb_residual_norm_desc* d) {
+  return check_norm_desc(d) == MXB_OK ? residual_norm_scratch(d) : 0;
+}
+mxb_status mxb_residual_norm_fwd(const mxb_residual_norm_desc* d, const void* resid, const void* y, const float* norm,
+                                 const float* post_norm, const void* z, const float* scale, void* resid_out, void* n, void* stream) {
+  const mxb_status s = check_norm_desc(d);
+  if (s != MXB_OK) return s;
+  if (d->rows == 0) return MXB_OK;
+  if (!resid || !y || !norm || !resid_out || !n) return MXB_ERR_INVALID_ARGUMENT;
+  return residual_norm_fwd(d, resid, y, norm, post_norm, z, scale, resid_out, n, static_cast<cudaStream_t>(stream));
+}
+mxb_status mxb_residual_norm_bwd(const mxb_residual_norm_desc* d, const void* resid_out, const void* y, const float* norm,
+                                 const float* post_norm, const void* z, const float* scale, const void* d_resid_out, const void* dn,
+                                 void* d_resid, void* dy, void* dz, float* dnorm, float* dpost_norm, float* dscale, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
+  const mxb_status s = check_norm_desc(d);
+  if (s != MXB_OK) return s;
+  if (!norm || !dnorm || (post_norm && !dpost_norm) || (scale && !dscale) || (z && !dz)) return MXB_ERR_INVALID_ARGUMENT;
+  if (d->rows == 0) {  // sums over no rows
+    for (float* g : {dnorm, post_norm ? dpost_norm : nullptr, scale ? dscale : nullptr})
+      if (g) {
+        const cudaError_t e = cudaMemsetAsync(g, 0, d->D * sizeof(float), static_cast<cudaStream_t>(stream));
+        if (e != cudaSuccess) { set_last_cuda_error((int)e); return MXB_ERR_CUDA; }
+      }
+    return MXB_OK;
+  }
+  if (!resid_out || !y || !dn || !d_resid || !dy) return MXB_ERR_INVALID_ARGUMENT;
+  if (!workspace || workspace_bytes < residual_norm_scratch(d)) return MXB_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return MXB_ERR_ALIGNMENT;
+  return residual_norm_bwd(d, resid_out, y, norm, post_norm, z, scale, d_resid_out, dn, d_resid, dy, z ? dz : nullptr, dnorm,
+                           post_norm ? dpost_norm : nullptr, scale ? dscale : nullptr, static_cast<float*>(workspace),
+                           static_cast<cudaStream_t>(stream));
 }
 
 // ---------------------------------------------------------------- IR op records

@@ -35,6 +35,8 @@ namespace {
   X(mxb_gdn_block_post_bwd) X(mxb_mamba3_fwd_workspace_bytes) X(mxb_mamba3_bwd_workspace_bytes) X(mxb_mamba3_fwd)     \
   X(mxb_mamba3_bwd) X(mxb_mamba3_block_workspace_bytes) X(mxb_mamba3_block_conv_fwd) X(mxb_mamba3_block_conv_bwd)     \
   X(mxb_mamba3_block_bc_fwd) X(mxb_mamba3_block_bc_bwd) X(mxb_mamba3_block_post_fwd) X(mxb_mamba3_block_post_bwd)     \
+  X(mxb_mamba3_prefill_workspace_bytes) X(mxb_mamba3_prefill) X(mxb_mamba3_decode_step) X(mxb_short_conv_prefill)    \
+  X(mxb_short_conv_step) X(mxb_residual_norm_workspace_bytes) X(mxb_residual_norm_fwd) X(mxb_residual_norm_bwd)       \
   X(mxb_ir_op_workspace_bytes) X(mxb_ir_op_forward)
 struct Abi {
 #define X(name) decltype(&::name) name = nullptr;
@@ -598,6 +600,174 @@ py::dict mamba3_block_post_backward(const Tensor& y, const Tensor& z, const Tens
   return r;
 }
 
+// ------------------------------------------------------------------ serving: state pools
+constexpr at::ScalarType I32 = at::kInt;
+struct PoolRows {  // which rows of a pool a call's sequences have, and (prompts) where they begin and which go on
+  int64_t S, slots;
+  const Opt &cu, &slot, &go_on;
+};
+void check_pool_rows(const PoolRows& r, at::Device dev) {
+  const int64_t S1 = r.S + 1;
+  check(r.cu, Shape(&S1, 1), I32, dev, "cu_seqlens");
+  check(r.slot, Shape(&r.S, 1), I32, dev, "slots");
+  check(r.go_on, Shape(&r.S, 1), at::kBool, dev, "go_on");
+  if (!r.slot && r.S > r.slots)
+    throw py::value_error("the state has " + std::to_string(r.slots) + " rows, " + std::to_string(r.S) + " sequences need as many or slots=");
+}
+int64_t sequences_of(const Tensor& cu) {
+  if (cu.dim() != 1 || cu.size(0) < 1) throw py::value_error("cu_seqlens must be [sequences + 1]");
+  return cu.size(0) - 1;
+}
+struct ServeCall {
+  mxb_mamba3_serve_desc d;
+  mxb_mamba3_state s;
+};
+ServeCall check_serve(at::Device dev, const std::vector<Tensor>& state, const Tensor& x, const Tensor& dt, const Tensor& lam,
+                      const Tensor& theta, const Tensor& a_log, const Tensor& b, const Tensor& c, const PoolRows& r, int64_t nheads,
+                      int64_t flags, const Opt& out) {
+  if (state.size() != 4) throw py::value_error("state must be a Mamba3State (h, phase, x_prev, b_prev)");
+  if (x.dim() != 2 || b.dim() != 3) throw py::value_error("x must be [rows,D] and b, c [rows,G,N]");
+  if (nheads < 0) throw py::value_error("nheads must not be negative");
+  const int64_t T = x.size(0), D = x.size(1), G = b.size(1), N = b.size(2);
+  const auto io = x.scalar_type();
+  const mxb_mamba3_serve_desc d{(int32_t)T, (int32_t)r.S, (int32_t)r.slots, (int32_t)D, (int32_t)N, (int32_t)G, (int32_t)nheads, io_code(x), (int32_t)flags};
+  const int64_t H = nheads > 0 ? nheads : D, per[] = {T, H, N / 2}, al[] = {H, N}, gn[] = {T, G, N};
+  check(x, x.sizes(), io, dev, "x");
+  check(dt, Shape(per, 2), F, dev, "dt");
+  check(lam, Shape(per, 2), F, dev, "lambda");
+  check(theta, Shape(per, nheads > 0 ? 2 : 3), F, dev, "theta");
+  check(a_log, Shape(al, nheads > 0 ? 1 : 2), F, dev, "a_log");
+  check(b, gn, io, dev, "b");
+  check(c, gn, io, dev, "c");
+  const int64_t hs[] = {r.slots, D, N}, ps[] = {r.slots, nheads, 2}, pc[] = {r.slots, D, N / 2, 2}, xs[] = {r.slots, D},
+                bs[] = {r.slots, nheads > 0 ? nheads : G, N};
+  check(state[0], hs, F, dev, "state.h");
+  check(state[1], nheads > 0 ? Shape(ps, 3) : Shape(pc, 4), F, dev, "state.phase");
+  check(state[2], xs, io, dev, "state.x_prev");
+  check(state[3], bs, io, dev, "state.b_prev");
+  check(out, x.sizes(), io, dev, "out");
+  check_pool_rows(r, dev);
+  return {d, {ptr<float>(state[0]), ptr<float>(state[1]), ptr(state[2]), ptr(state[3])}};
+}
+int64_t pool_size(const std::vector<Tensor>& state) {
+  if (state.empty() || state[0].dim() != 3) throw py::value_error("state.h must be [slots,D,N]");
+  return state[0].size(0);
+}
+Tensor mamba3_prefill(const Tensor& x, const Tensor& dt, const Tensor& lam, const Tensor& theta, const Tensor& a_log, const Tensor& b,
+                      const Tensor& c, const Tensor& cu, const std::vector<Tensor>& state, const Opt& slots, const Opt& go_on,
+                      int64_t nheads, const Opt& out, int64_t flags) {
+  const at::Device dev = cuda_device(x);
+  const Opt cu_(cu);
+  const ServeCall a = check_serve(dev, state, x, dt, lam, theta, a_log, b, c, {sequences_of(cu), pool_size(state), cu_, slots, go_on}, nheads, flags, out);
+  const On on(dev);
+  Tensor y = out ? *out : like(x);
+  const size_t need = abi.mxb_mamba3_prefill_workspace_bytes(&a.d);
+  auto go = [&](void* ws, size_t n, void* stream) {
+    return abi.mxb_mamba3_prefill(&a.d, ptr(x), ptr<float>(dt), ptr<float>(lam), ptr<float>(theta), ptr<float>(a_log), ptr(b), ptr(c),
+                                  ptr<int32_t>(cu), ptr<int32_t>(slots), reinterpret_cast<const uint8_t*>(ptr<bool>(go_on)), &a.s, ptr(y), ws, n, stream);
+  };
+  if (need) call_with_scratch(on, need, "mxb_mamba3_prefill", go);
+  else call("mxb_mamba3_prefill", go, nullptr, 0, on.stream);
+  return y;
+}
+Tensor mamba3_decode_step(const std::vector<Tensor>& state, const Tensor& x, const Tensor& dt, const Tensor& lam, const Tensor& theta,
+                          const Tensor& a_log, const Tensor& b, const Tensor& c, const Opt& slots, int64_t nheads, const Opt& out) {
+  const at::Device dev = cuda_device(x);
+  const Opt none;
+  const int64_t S = x.dim() ? x.size(0) : 0;
+  const ServeCall a = check_serve(dev, state, x, dt, lam, theta, a_log, b, c, {S, pool_size(state), none, slots, none}, nheads, 0, out);
+  const On on(dev);
+  Tensor y = out ? *out : like(x);
+  call("mxb_mamba3_decode_step", abi.mxb_mamba3_decode_step, &a.d, &a.s, ptr(x), ptr<float>(dt), ptr<float>(lam), ptr<float>(theta),
+       ptr<float>(a_log), ptr(b), ptr(c), ptr<int32_t>(slots), ptr(y), on.stream);
+  return y;
+}
+mxb_short_conv_desc check_short_conv(at::Device dev, const Tensor& state, const Tensor& x, const Tensor& w, const Opt& bias,
+                                     const PoolRows& r, const std::optional<std::string>& activation, const Opt& out) {
+  if (x.dim() != 2) throw py::value_error("x must be [rows,D]");
+  if (w.dim() != 2) throw py::value_error("w must be [D,K]");
+  const int64_t D = x.size(1), K = w.size(1), ss[] = {r.slots, K - 1, D};
+  const auto io = x.scalar_type();
+  if (activation && *activation != "silu") throw py::value_error("activation: None or \"silu\", not \"" + *activation + "\"");
+  check(x, x.sizes(), io, dev, "x");
+  if (!w.is_cuda()) not_cuda();
+  if (w.size(0) != D || K < 1) throw py::value_error("w: shape " + text(w.sizes()) + ", expected (" + std::to_string(D) + ", K)");
+  if (w.scalar_type() != F) throw py::type_error("w: dtype " + std::string(c10::toString(w.scalar_type())) + ", expected Float");
+  if (w.device() != dev) throw py::value_error("w: on " + w.device().str() + ", expected " + dev.str());
+  check(state, ss, io, dev, "conv_state");
+  check(bias, Shape(&D, 1), F, dev, "bias");
+  check(out, x.sizes(), io, dev, "out");
+  check_pool_rows(r, dev);
+  return {(int32_t)x.size(0), (int32_t)r.S, (int32_t)r.slots, (int32_t)D, (int32_t)K, io_code(x), activation ? MXB_ACT_SILU : MXB_ACT_NONE, w.stride(0), w.stride(1)};
+}
+Tensor short_conv_prefill(const Tensor& x, const Tensor& w, const Tensor& cu, const Tensor& state, const Opt& slots, const Opt& go_on,
+                          const Opt& bias, const std::optional<std::string>& activation, const Opt& out) {
+  const at::Device dev = cuda_device(x);
+  if (state.dim() != 3) throw py::value_error("conv_state must be [slots,K-1,D]");
+  const Opt cu_(cu);
+  const mxb_short_conv_desc d = check_short_conv(dev, state, x, w, bias, {sequences_of(cu), state.size(0), cu_, slots, go_on}, activation, out);
+  const On on(dev);
+  Tensor y = out ? *out : like(x);
+  call("mxb_short_conv_prefill", abi.mxb_short_conv_prefill, &d, ptr(x), ptr<float>(w), ptr<float>(bias), ptr<int32_t>(cu), ptr<int32_t>(slots),
+       reinterpret_cast<const uint8_t*>(ptr<bool>(go_on)), ptr(state), ptr(y), on.stream);
+  return y;
+}
+Tensor short_conv_step(const Tensor& state, const Tensor& x, const Tensor& w, const Opt& slots, const Opt& bias,
+                       const std::optional<std::string>& activation, const Opt& out) {
+  const at::Device dev = cuda_device(x);
+  if (state.dim() != 3) throw py::value_error("conv_state must be [slots,K-1,D]");
+  const Opt none;
+  const mxb_short_conv_desc d = check_short_conv(dev, state, x, w, bias, {x.dim() ? x.size(0) : 0, state.size(0), none, slots, none}, activation, out);
+  const On on(dev);
+  Tensor y = out ? *out : like(x);
+  call("mxb_short_conv_step", abi.mxb_short_conv_step, &d, ptr(state), ptr(x), ptr<float>(w), ptr<float>(bias), ptr<int32_t>(slots), ptr(y), on.stream);
+  return y;
+}
+
+// ------------------------------------------------------------------ residual stream
+mxb_residual_norm_desc check_norm(at::Device dev, const Tensor& resid, const Tensor& y, const Tensor& norm, const Opt& post, const Opt& z,
+                                  const Opt& scale, double eps) {
+  if (y.dim() < 1) throw py::value_error("y must be [..., D]");
+  const int64_t D = y.size(-1);
+  const auto io = y.scalar_type();
+  const mxb_residual_norm_desc d{D > 0 ? y.numel() / D : 0, (int32_t)D, io_code(y), io_code(resid), (float)eps};
+  check(y, y.sizes(), io, dev, "y");
+  check(resid, y.sizes(), resid.scalar_type(), dev, "resid");
+  if (resid.scalar_type() != io && resid.scalar_type() != F) throw py::type_error("resid: BFloat16 beside a Float y (one type, or a Float resid)");
+  check(norm, Shape(&D, 1), F, dev, "norm");
+  check(post, Shape(&D, 1), F, dev, "post_norm");
+  check(z, y.sizes(), io, dev, "z");
+  check(scale, Shape(&D, 1), F, dev, "scale");
+  return d;
+}
+py::tuple residual_norm(const Tensor& resid, const Tensor& y, const Tensor& norm, const Opt& post, const Opt& z, const Opt& scale, double eps) {
+  const at::Device dev = cuda_device(y);
+  const mxb_residual_norm_desc d = check_norm(dev, resid, y, norm, post, z, scale, eps);
+  const On on(dev);
+  Tensor r = like(resid), n = like(y);
+  call("mxb_residual_norm_fwd", abi.mxb_residual_norm_fwd, &d, ptr(resid), ptr(y), ptr<float>(norm), ptr<float>(post), ptr(z), ptr<float>(scale), ptr(r), ptr(n), on.stream);
+  return py::make_tuple(r, n);
+}
+py::dict residual_norm_backward(const Tensor& resid_out, const Tensor& y, const Tensor& norm, const Opt& d_resid_out, const Tensor& dn,
+                                const Opt& post, const Opt& z, const Opt& scale, double eps) {
+  const at::Device dev = cuda_device(y);
+  const mxb_residual_norm_desc d = check_norm(dev, resid_out, y, norm, post, z, scale, eps);
+  check(d_resid_out, y.sizes(), resid_out.scalar_type(), dev, "d_resid_out");
+  check(dn, y.sizes(), y.scalar_type(), dev, "dn");
+  const On on(dev);
+  Tensor dr = like(resid_out), dy = like(y), dw = like(norm);
+  Opt dz, dp, ds;
+  if (z) dz = like(*z);
+  if (post) dp = like(*post);
+  if (scale) ds = like(*scale);
+  call_with_scratch(on, abi.mxb_residual_norm_workspace_bytes(&d), "mxb_residual_norm_bwd", abi.mxb_residual_norm_bwd, &d, ptr(resid_out), ptr(y),
+                    ptr<float>(norm), ptr<float>(post), ptr(z), ptr<float>(scale), ptr(d_resid_out), ptr(dn), ptr(dr), ptr(dy), ptr(dz),
+                    ptr<float>(dw), ptr<float>(dp), ptr<float>(ds));
+  py::dict r;
+  r["d_resid"] = dr; r["dy"] = dy; r["dz"] = dz; r["dnorm"] = dw; r["dpost_norm"] = dp; r["dscale"] = ds;
+  return r;
+}
+
 // ------------------------------------------------------------------ IR op records
 Tensor ir_op_forward(int64_t op_type, const std::vector<Tensor>& inputs, const std::vector<int64_t>& int_params,
                      const std::vector<int64_t>& out_shape, const std::vector<double>& float_params) {
@@ -643,4 +813,10 @@ PYBIND11_MODULE(_front, m) {
   m.def("mamba3_block_bc_backward", &mamba3_block_bc_backward);
   m.def("mamba3_block_post", &mamba3_block_post);
   m.def("mamba3_block_post_backward", &mamba3_block_post_backward);
+  m.def("mamba3_prefill", &mamba3_prefill);
+  m.def("mamba3_decode_step", &mamba3_decode_step);
+  m.def("short_conv_prefill", &short_conv_prefill);
+  m.def("short_conv_step", &short_conv_step);
+  m.def("residual_norm", &residual_norm);
+  m.def("residual_norm_backward", &residual_norm_backward);
 }

@@ -1,0 +1,123 @@
+// Shared declarations of the Mamba-3 serving kernels: packed prompts and single tokens on a pool of recurrent states
+// (mamba3_step.cu: one token; mamba3_walk.cu: prompts step by step, both layouts).
+#pragma once
+
+#include "mamba3.cuh"
+
+namespace mxb {
+
+struct ServeP {
+  int rows, S, slots;       // tokens of the call, sequences, rows of the state pool
+  int D, N, G, NH, Kp, P;   // P: channels of a head (head layout)
+  const void *x, *b, *c;
+  const float *dt, *lam, *theta, *a_log;
+  const int* cu;            // prompts: [S + 1] first rows; nullptr: one token a sequence
+  const int* slot;          // [S] row of the pool, nullptr: the sequence's own number
+  const unsigned char* go;  // prompts: [S] goes on from its state; nullptr: none does
+  float* h;                 // [slots, D, N]
+  float2* phase;            // [slots, NH] or [slots, D, Kp]: cosine and sine of the angle
+  void *x_prev, *b_prev;    // [slots, D], [slots, NH or G, N]
+  void* y;
+  // prompts cut into segments of L steps
+  int L, pieces;
+  float* ends;      // [pieces, D, N]: what a segment adds to the state, then the state that it starts from
+  float* dsum;      // [pieces, NH or D]: sum of dt over the segment
+  int* turn;        // [pieces, NH or D Kp]: angle of the segment in 2^-32 turns
+  float* spoil;     // [pieces, D Kp]: NaN where the segment's angle is not finite, 0 elsewhere (channel layout)
+  float2* start;    // [pieces, NH]: cosine and sine of the angle that the segment starts at (head layout)
+  int slabs;        // head layout: CTAs that share a head's channels
+};
+
+// Angles are summed as 32-bit fractions of a turn, whose additions do not round and wrap by themselves.  dt theta as such a
+// fraction: the product and the division by 2 pi are carried out in two parts each, so that what is left is the rounding of dt.
+__device__ __forceinline__ int m3_turn(float dt, float theta) {
+  constexpr float kHi = 0.15915493667125702f, kLo = 6.420638243e-09f;  // 1 / (2 pi) in two floats
+  const float p = dt * theta, pl = fmaf(dt, theta, -p);
+  const float t = p * kHi, tl = fmaf(p, kHi, -t) + fmaf(p, kLo, pl * kHi);
+  return __float2int_rn((t - rintf(t)) * 4294967296.f) + __float2int_rn(tl * 4294967296.f);
+}
+// A sum of 0 x: 0, or NaN where x is not finite - an angle that is not finite has to reach every later step.
+__device__ __forceinline__ float m3_taint(float x, float sum) { return fmaf(x, 0.f, sum); }
+__device__ __forceinline__ float2 m3_unit(int turn, float taint) {  // cosine, sine
+  float s, c;
+  sincospif((float)turn * 4.656612873077393e-10f, &s, &c);
+  return make_float2(c + taint, s + taint);
+}
+__device__ __forceinline__ float2 m3_back(float2 v, float2 a) {  // R^T: v turned back by the angle of a
+  return make_float2(fmaf(a.x, v.x, a.y * v.y), fmaf(a.x, v.y, -a.y * v.x));
+}
+__device__ __forceinline__ float2 m3_on(float2 v, float2 a) {    // R: v turned on
+  return make_float2(fmaf(a.x, v.x, -a.y * v.y), fmaf(a.x, v.y, a.y * v.x));
+}
+// The product of two unit vectors, of unit length again (one step of Newton's method for 1 / sqrt).
+__device__ __forceinline__ float2 m3_turned(float2 u, float2 by) {
+  const float2 r = m3_on(u, by);
+  const float k = fmaf(-0.5f, fmaf(r.x, r.x, r.y * r.y), 1.5f);
+  return make_float2(r.x * k, r.y * k);
+}
+
+// A segment of a sequence: rows [first, last) of the sequence [begin, end); `base` is the piece of its first segment.
+struct Piece {
+  int seq, seg, segs, base, first, last, begin, end;
+  bool ok;
+};
+// The index-th piece: sequences one after the other, each cut every L rows.  Called by whole warps.  Whatever cu holds, rows
+// stay inside the call's.
+__device__ __forceinline__ Piece find_piece(const ServeP& p, int index) {
+  const int lane = threadIdx.x & 31;
+  Piece q{};
+  int before = 0;
+  for (int s0 = 0; s0 < p.S; s0 += 32) {
+    const int s = s0 + lane;
+    int a = 0, e = 0, n = 0;
+    if (s < p.S) {
+      a = min(max(__ldg(p.cu + s), 0), p.rows);
+      e = min(max(__ldg(p.cu + s + 1), a), p.rows);
+      n = (int)(((long long)e - a + p.L - 1) / p.L);
+    }
+    int incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    const unsigned m = __ballot_sync(0xffffffffu, before + incl > index);
+    if (m) {
+      const int src = __ffs(m) - 1;
+      q.seq = s0 + src;
+      q.begin = __shfl_sync(0xffffffffu, a, src);
+      q.end = __shfl_sync(0xffffffffu, e, src);
+      q.segs = __shfl_sync(0xffffffffu, n, src);
+      q.base = before + __shfl_sync(0xffffffffu, incl - n, src);
+      q.seg = index - q.base;
+      q.first = q.begin + q.seg * p.L;
+      q.last = (int)min((long long)q.first + p.L, (long long)q.end);
+      q.ok = true;
+      return q;
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return q;
+}
+// The sequence's row of the pool, -1 where it keeps no state.
+__device__ __forceinline__ int serve_slot(const ServeP& p, int seq) {
+  const int s = p.slot ? __ldg(p.slot + seq) : seq;
+  return s >= 0 && s < p.slots ? s : -1;
+}
+__device__ __forceinline__ bool serve_goes_on(const ServeP& p, int seq) { return p.go && __ldg(p.go + seq); }
+
+// (1 - lambda) dt of row t + 1, which weighs row t's outer product there; 0 behind the sequence's last row.
+__device__ __forceinline__ float serve_look(const ServeP& p, size_t at, bool in) {
+  return in ? (1.f - m3_sigmoid(__ldg(p.lam + at))) * m3_softplus(__ldg(p.dt + at)) : 0.f;
+}
+
+// Two neighbouring elements of a row (of b, c: N is even; a row may start at any element).
+template <typename IO>
+__device__ __forceinline__ float2 load_pair(const IO* p) { return make_float2(to_f32(p[0]), to_f32(p[1])); }
+
+mxb_status m3serve_step(const ServeP& p, bool f32, cudaStream_t st);
+size_t m3walk_scratch(ServeP& p, bool f32, int flags, char* base);
+mxb_status m3walk_prefill(const ServeP& p, bool f32, cudaStream_t st);
+mxb_status m3serve_tails(const ServeP& p, bool f32, bool x_too, cudaStream_t st);
+
+}  // namespace mxb

@@ -1,0 +1,577 @@
+// Mamba-3 scan of packed prompts on a pool of states, step by step: float32 and every shape, both parameter layouts (the
+// recurrence and the state are mamba3_step.cu's).
+//
+// What is carried from step to step is G_t = h_t + (1 - lam_{t+1}) dt_{t+1} Brot_t x_t (0 for the look-ahead behind the last
+// step), so that a step needs nothing of the one before:
+//     h_t = alpha_t G_{t-1} + lam_t dt_t Brot_t x_t;   y_t = <h_t, Crot_t>;   G_t = alpha_t G_{t-1} + e_t Brot_t x_t
+//     e_t = lam_t dt_t + (1 - lam_{t+1}) dt_{t+1}
+// A walk is one chain of steps, and prompts that are few and long would leave the GPU to a few of them.  Sequences longer than
+// L steps are cut into segments (serve_segment()): a first pass walks every segment but a sequence's last from a zero state,
+// a second one chains what they add, H <- decay H + added, and the walk that writes y starts from the results.
+//
+// Head layout: decay and angle are a head's own, so turning commutes with the decay and each segment counts its angle from
+// its own start; the state between two segments is the turned-on one, R(phi) h.  Channel layout: the two states of a pair
+// decay at rates of their own, so angles count from the sequence's start and a pass in front sums them by segments.
+#include <algorithm>
+#include <type_traits>
+
+#include "mamba3_serve.cuh"
+
+namespace mxb {
+namespace m3k {
+
+using bf16 = __nv_bfloat16;
+enum Mode { kOut, kEnds, kAngles };
+
+// ------------------------------------------------------------------ heads
+// A CTA per (segment, head, slab of channels): LN lanes along a row of states, NV pieces of 4 states a lane, R rows a thread,
+// all in registers.  16 steps at a time are made ready in shared memory: scalars by one warp, then b and c turned back and x.
+constexpr int kW = 16;
+constexpr int kRowsMost = 64;  // channels of a slab
+struct HeadSmem {
+  float alpha[kW], gs[kW], e[kW], gamma[kW];
+  float2 unit[kW];
+};
+template <typename IO, int NV, int R, Mode MODE>
+__global__ void __launch_bounds__(256) m3k_heads_kernel(ServeP p, int LN) {
+  begin_dependent();
+  extern __shared__ __align__(16) float smem[];
+  __shared__ HeadSmem sc;
+  __shared__ int s_turn;
+  __shared__ float s_taint, s_dt;
+  const int tid = threadIdx.x, hd = blockIdx.y / p.slabs, slab = blockIdx.y % p.slabs;
+  const Piece q = find_piece(p, blockIdx.x);
+  if (!q.ok || (MODE == kEnds && q.seg == q.segs - 1)) return;
+  const int ln = tid % LN, rg = tid / LN, rows_at_once = 256 / LN, npad = LN * 4 * NV;
+  const int per = (p.P + p.slabs - 1) / p.slabs, p0 = slab * per, np = min(per, p.P - p0);  // this CTA's channels of the head
+  const size_t chan = (size_t)hd * p.P + p0;
+  float *su = smem, *scv = su + kW * npad, *sx = scv + kW * npad, *sy = sx + kW * kRowsMost;
+  const int slot = serve_slot(p, q.seq), g = hd / (p.NH / p.G);
+  const bool from_state = MODE == kOut && q.segs == 1 && slot >= 0 && serve_goes_on(p, q.seq);
+  const size_t ph = (size_t)(slot < 0 ? 0 : slot) * p.NH + hd;
+  const float A = -expf(p.a_log[hd]);
+  float2 start = make_float2(1.f, 0.f);
+  if (MODE == kOut && q.segs > 1) start = p.start[(size_t)blockIdx.x * p.NH + hd];
+  else if (from_state) start = p.phase[ph];
+
+  auto row_of = [&](int r) { return rg + r * rows_at_once; };
+  auto n_of = [&](int k) { return (ln + k * LN) * 4; };
+  float G[R][NV][4];
+  const float look0 = from_state ? serve_look(p, (size_t)q.first * p.NH + hd, true) : 0.f;
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        const int row = row_of(r), n = n_of(k) + i;
+        float2 v = make_float2(0.f, 0.f);
+        if (row < np && n < p.N) {
+          if (MODE == kOut && q.segs > 1) {
+            v = *reinterpret_cast<const float2*>(p.ends + ((size_t)blockIdx.x * p.D + chan + row) * p.N + n);
+          } else if (from_state) {
+            v = m3_on(*reinterpret_cast<const float2*>(p.h + ((size_t)slot * p.D + chan + row) * p.N + n), start);
+            const float2 b = load_pair(static_cast<const IO*>(p.b_prev) + ph * p.N + n);
+            const float w = look0 * to_f32(static_cast<const IO*>(p.x_prev)[(size_t)slot * p.D + chan + row]);
+            v.x = fmaf(w, b.x, v.x);
+            v.y = fmaf(w, b.y, v.y);
+          }
+        }
+        G[r][k][i] = v.x;
+        G[r][k][i + 1] = v.y;
+      }
+  if (tid == 0) { s_turn = 0; s_taint = 0.f; s_dt = 0.f; }
+  for (int t0 = q.first; t0 < q.last; t0 += kW) {
+    __syncthreads();
+    if (tid < 32) {  // scalars of the steps; the angle runs on from block to block
+      const int t = t0 + tid;
+      const bool in = tid < kW && t < q.last;
+      const size_t at = (size_t)(in ? t : q.first) * p.NH + hd;
+      const float dt = m3_softplus(p.dt[at]), lam = m3_sigmoid(p.lam[at]), theta = p.theta[at];
+      const float look = serve_look(p, at + p.NH, in && t + 1 < q.end);
+      int turn = in ? m3_turn(dt, theta) : 0;
+      float taint = in ? m3_taint(dt * theta, 0.f) : 0.f, sum = in ? dt : 0.f;
+#pragma unroll
+      for (int o = 1; o < kW; o <<= 1) {
+        const int a = __shfl_up_sync(0xffffffffu, turn, o);
+        const float b = __shfl_up_sync(0xffffffffu, taint, o), c = __shfl_up_sync(0xffffffffu, sum, o);
+        if (tid >= o) { turn += a; taint += b; sum += c; }
+      }
+      turn += s_turn;
+      taint += s_taint;
+      sum += s_dt;
+      __syncwarp();
+      if (tid == kW - 1) { s_turn = turn; s_taint = taint; s_dt = sum; }
+      if (tid < kW) {
+        sc.alpha[tid] = in ? expf(A * dt) : 1.f;
+        sc.gamma[tid] = in ? lam * dt : 0.f;
+        sc.e[tid] = in ? lam * dt + look : 0.f;
+        sc.unit[tid] = m3_unit(turn, taint);
+      }
+    }
+    for (int i = tid; i < kW * np; i += 256) {
+      const int s = i / np, r = i - s * np;
+      sx[s * kRowsMost + r] = t0 + s < q.last ? to_f32(static_cast<const IO*>(p.x)[(size_t)(t0 + s) * p.D + chan + r]) : 0.f;
+    }
+    __syncthreads();
+    {  // 16 threads a step
+      const int s = tid / 16, j = tid % 16;
+      const bool in = t0 + s < q.last;
+      const size_t row = ((size_t)(in ? t0 + s : q.first) * p.G + g) * p.N;
+      const float2 a = sc.unit[s];
+      float dot = 0.f;
+      for (int k = j; k < npad / 2; k += 16) {
+        float2 u = make_float2(0.f, 0.f), c = u;
+        if (in && 2 * k < p.N) {
+          const float2 b = load_pair(static_cast<const IO*>(p.b) + row + 2 * k);
+          u = m3_back(b, a);
+          if (MODE == kOut) {
+            const float2 cr = load_pair(static_cast<const IO*>(p.c) + row + 2 * k);
+            dot = fmaf(b.x, cr.x, fmaf(b.y, cr.y, dot));  // <Brot, Crot> = <b, c>
+            c = m3_back(cr, a);
+          }
+        }
+        reinterpret_cast<float2*>(su + s * npad)[k] = u;
+        if (MODE == kOut) reinterpret_cast<float2*>(scv + s * npad)[k] = c;
+      }
+      if (MODE == kOut) {
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        if (j == 0) sc.gs[s] = sc.gamma[s] * dot + a.x * 0.f;  // (an angle that is not finite has to reach y here too)
+      }
+    }
+    __syncthreads();
+    const int steps = min(kW, q.last - t0);
+    for (int s = 0; s < steps; ++s) {
+      const float alpha = sc.alpha[s], e = sc.e[s];
+      float u[NV][4], c[NV][4], acc[R];
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const float4 a = *reinterpret_cast<const float4*>(su + s * npad + n_of(k));
+        u[k][0] = a.x; u[k][1] = a.y; u[k][2] = a.z; u[k][3] = a.w;
+        if (MODE == kOut) {
+          const float4 b = *reinterpret_cast<const float4*>(scv + s * npad + n_of(k));
+          c[k][0] = b.x; c[k][1] = b.y; c[k][2] = b.z; c[k][3] = b.w;
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int row = row_of(r);
+        const float x = row < np ? sx[s * kRowsMost + row] : 0.f, ex = e * x;
+        acc[r] = 0.f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float v = alpha * G[r][k][i];
+            if (MODE == kOut) acc[r] = fmaf(c[k][i], v, acc[r]);
+            G[r][k][i] = fmaf(ex, u[k][i], v);
+          }
+      }
+      if (MODE == kOut) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+          if (o < LN)
+#pragma unroll
+            for (int r = 0; r < R; ++r) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], o);
+        if (ln == 0)
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const int row = row_of(r);
+            if (row < np) sy[s * kRowsMost + row] = fmaf(sc.gs[s], sx[s * kRowsMost + row], acc[r]);
+          }
+      }
+    }
+    if (MODE == kOut) {
+      __syncthreads();
+      for (int i = tid; i < steps * np; i += 256) {
+        const int s = i / np, r = i - s * np;
+        static_cast<IO*>(p.y)[(size_t)(t0 + s) * p.D + chan + r] = from_f32<IO>(sy[s * kRowsMost + r]);
+      }
+    }
+  }
+  __syncthreads();
+  const float2 ran = m3_unit(s_turn, s_taint);
+  if (MODE == kEnds && tid == 0 && slab == 0) {
+    p.turn[(size_t)blockIdx.x * p.NH + hd] = s_turn;
+    p.dsum[(size_t)blockIdx.x * p.NH + hd] = s_dt + s_taint;
+  }
+  if (MODE == kOut && (q.seg != q.segs - 1 || slot < 0)) return;
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        const int row = row_of(r), n = n_of(k) + i;
+        if (row >= np || n >= p.N) continue;
+        const float2 v = make_float2(G[r][k][i], G[r][k][i + 1]);
+        if (MODE == kEnds) *reinterpret_cast<float2*>(p.ends + ((size_t)blockIdx.x * p.D + chan + row) * p.N + n) = m3_on(v, ran);
+        else *reinterpret_cast<float2*>(p.h + ((size_t)slot * p.D + chan + row) * p.N + n) = m3_back(v, start);
+      }
+  // (the slabs of a head all read the phase; with more than one it is written behind this launch)
+  if (MODE == kOut && tid == 0 && p.slabs == 1) p.phase[ph] = m3_turned(start, ran);
+}
+
+// What the segments of a sequence start from.  grid (pieces, blocks of pairs): the block of a sequence's first segment walks
+// over its segments, a thread per state pair of all channels.
+__global__ void __launch_bounds__(256) m3k_heads_chain_kernel(ServeP p, bool bf16_io) {
+  begin_dependent();
+  const Piece q = find_piece(p, blockIdx.x);
+  if (!q.ok || q.seg != 0 || q.segs == 1) return;
+  const size_t i = blockIdx.y * (size_t)256 + threadIdx.x, pairs = (size_t)p.D * p.Kp;
+  if (i >= pairs) return;
+  const int d = (int)(i / p.Kp), k = (int)(i % p.Kp), hd = d / p.P;
+  const int slot = serve_slot(p, q.seq);
+  float2 at = make_float2(1.f, 0.f), v = make_float2(0.f, 0.f);
+  if (slot >= 0 && serve_goes_on(p, q.seq)) {
+    const size_t ph = (size_t)slot * p.NH + hd;
+    at = p.phase[ph];
+    v = m3_on(reinterpret_cast<const float2*>(p.h)[((size_t)slot * p.D + d) * p.Kp + k], at);
+    const float w = serve_look(p, (size_t)q.begin * p.NH + hd, true) *
+                    (bf16_io ? to_f32(static_cast<const bf16*>(p.x_prev)[(size_t)slot * p.D + d]) : static_cast<const float*>(p.x_prev)[(size_t)slot * p.D + d]);
+    const float2 b = bf16_io ? load_pair(static_cast<const bf16*>(p.b_prev) + ph * p.N + 2 * k) : load_pair(static_cast<const float*>(p.b_prev) + ph * p.N + 2 * k);
+    v.x = fmaf(w, b.x, v.x);
+    v.y = fmaf(w, b.y, v.y);
+  }
+  const float A = -expf(p.a_log[hd]);
+  const bool first = k == 0 && d % p.P == 0;
+  float2* e = reinterpret_cast<float2*>(p.ends) + ((size_t)q.base * p.D + d) * p.Kp + k;
+  for (int s = 0; s < q.segs; ++s, e += pairs) {
+    const size_t sh = (size_t)(q.base + s) * p.NH + hd;
+    const float2 was = v;
+    if (s < q.segs - 1) {
+      const float2 add = *e, ran = m3_unit(p.turn[sh], m3_taint(p.dsum[sh], 0.f));  // (dsum carries the angle's taint)
+      const float L = expf(A * p.dsum[sh]);
+      const float2 r = m3_on(v, ran);
+      v.x = fmaf(L, r.x, add.x);
+      v.y = fmaf(L, r.y, add.y);
+      if (first) {
+        p.start[sh] = at;
+        at = m3_turned(at, ran);
+      }
+    } else if (first) {
+      p.start[sh] = at;
+    }
+    *e = was;
+  }
+}
+// The phase at a sequence's end where the heads are cut into slabs: summed again from dt theta.  grid (sequences, heads) x 256.
+__global__ void __launch_bounds__(256) m3k_heads_phase_kernel(ServeP p) {
+  begin_dependent();
+  __shared__ int s_turn[8];
+  __shared__ float s_taint[8];
+  const int seq = blockIdx.x, hd = blockIdx.y, slot = serve_slot(p, seq);
+  if (slot < 0) return;
+  const int a = min(max(p.cu[seq], 0), p.rows), e = min(max(p.cu[seq + 1], a), p.rows);
+  if (a == e) return;
+  int turn = 0;
+  float taint = 0.f;
+  for (int t = a + threadIdx.x; t < e; t += 256) {
+    const size_t at = (size_t)t * p.NH + hd;
+    const float dt = m3_softplus(p.dt[at]), theta = p.theta[at];
+    turn += m3_turn(dt, theta);
+    taint = m3_taint(dt * theta, taint);
+  }
+  turn = warp_sum(turn);
+  taint = warp_sum(taint);
+  if ((threadIdx.x & 31) == 0) { s_turn[threadIdx.x >> 5] = turn; s_taint[threadIdx.x >> 5] = taint; }
+  __syncthreads();
+  if (threadIdx.x) return;
+  turn = 0;
+  taint = 0.f;
+  for (int w = 0; w < 8; ++w) { turn += s_turn[w]; taint += s_taint[w]; }
+  const size_t ph = (size_t)slot * p.NH + hd;
+  const float2 from = serve_goes_on(p, seq) ? p.phase[ph] : make_float2(1.f, 0.f);
+  p.phase[ph] = m3_turned(from, m3_unit(turn, taint));
+}
+
+// ------------------------------------------------------------------ channels
+// LPC lanes a channel with PR state pairs each, 8 steps at a time: a lane works out softplus and sigmoid of its own steps and
+// hands them round; theta and the rows of b and c are requested before the first of the 8 steps.
+constexpr int kC = 8;
+template <typename IO, int PR, int LPC, Mode MODE>
+__global__ void __launch_bounds__(128) m3k_channels_kernel(ServeP p) {
+  begin_dependent();
+  constexpr int OWN = (kC + LPC - 1) / LPC, CPB = 128 / LPC;
+  const int lane = threadIdx.x & 31, sl = lane % LPC, base = lane - sl;
+  const int d_raw = blockIdx.y * CPB + threadIdx.x / LPC;
+  const bool live = d_raw < p.D;
+  const int d = live ? d_raw : p.D - 1;
+  const Piece q = find_piece(p, blockIdx.x);
+  if (!q.ok || (MODE != kOut && q.seg == q.segs - 1)) return;
+  const int slot = serve_slot(p, q.seq), g = d / (p.D / p.G);
+  const bool go = slot >= 0 && serve_goes_on(p, q.seq);
+  const size_t sd = (size_t)(slot < 0 ? 0 : slot) * p.D + d;
+  float G[PR][2], a[PR][2], taint[PR], dsum = 0.f;
+  int turn[PR];
+  auto kp = [&](int r) { return sl + r * LPC; };
+  auto has = [&](int r) { return kp(r) < p.Kp; };
+#pragma unroll
+  for (int r = 0; r < PR; ++r) {
+    G[r][0] = G[r][1] = a[r][0] = a[r][1] = taint[r] = 0.f;
+    turn[r] = 0;
+    if (!has(r)) continue;
+    const size_t pair = sd * p.Kp + kp(r);
+    float2 unit = make_float2(1.f, 0.f);
+    if (MODE != kAngles && go) {
+      unit = p.phase[pair];
+      turn[r] = __float2int_rn(atan2f(unit.y, unit.x) * 0.15915494309189535f * 4294967296.f);
+      taint[r] = m3_taint(unit.x, m3_taint(unit.y, 0.f));
+    }
+    if (MODE != kAngles) {
+      for (int s = 0; s < q.seg; ++s) {
+        const size_t at = (size_t)(q.base + s) * p.D * p.Kp + (size_t)d * p.Kp + kp(r);
+        turn[r] += p.turn[at];
+        taint[r] += p.spoil[at];
+      }
+      a[r][0] = -expf(p.a_log[(size_t)d * p.N + 2 * kp(r)]);
+      a[r][1] = -expf(p.a_log[(size_t)d * p.N + 2 * kp(r) + 1]);
+    }
+    if (MODE == kOut && q.segs > 1) {
+      const float2 v = reinterpret_cast<const float2*>(p.ends)[((size_t)blockIdx.x * p.D + d) * p.Kp + kp(r)];
+      G[r][0] = v.x;
+      G[r][1] = v.y;
+    } else if (MODE == kOut && go) {
+      const float2 v = reinterpret_cast<const float2*>(p.h)[pair];
+      const float2 b = m3_back(load_pair(static_cast<const IO*>(p.b_prev) + ((size_t)slot * p.G + g) * p.N + 2 * kp(r)), unit);
+      const float w = serve_look(p, (size_t)q.first * p.D + d, true) * to_f32(static_cast<const IO*>(p.x_prev)[sd]);
+      G[r][0] = fmaf(w, b.x, v.x);
+      G[r][1] = fmaf(w, b.y, v.y);
+    }
+  }
+  for (int t0 = q.first; t0 < q.last; t0 += kC) {
+    float theta[kC][PR];
+    float2 bv[kC][PR], cv[kC][PR];
+#pragma unroll
+    for (int s = 0; s < kC; ++s)
+#pragma unroll
+      for (int r = 0; r < PR; ++r) {
+        const size_t t = (size_t)min(t0 + s, q.last - 1);
+        const bool in = has(r) && t0 + s < q.last;
+        theta[s][r] = in ? __ldg(p.theta + (t * p.D + d) * p.Kp + kp(r)) : 0.f;
+        if (MODE != kAngles) bv[s][r] = in ? load_pair(static_cast<const IO*>(p.b) + (t * p.G + g) * p.N + 2 * kp(r)) : make_float2(0.f, 0.f);
+        if (MODE == kOut) cv[s][r] = in ? load_pair(static_cast<const IO*>(p.c) + (t * p.G + g) * p.N + 2 * kp(r)) : make_float2(0.f, 0.f);
+      }
+    float dts[OWN], gxs[OWN], exs[OWN], ys[kC];
+#pragma unroll
+    for (int o = 0; o < OWN; ++o) {
+      const int s = sl + o * LPC;
+      const bool in = s < kC && t0 + s < q.last;
+      const size_t at = (size_t)(in ? t0 + s : q.first) * p.D + d;
+      dts[o] = in ? m3_softplus(p.dt[at]) : 0.f;
+      gxs[o] = exs[o] = 0.f;
+      if (MODE != kAngles && in) {
+        const float x = to_f32(static_cast<const IO*>(p.x)[at]), gamma = m3_sigmoid(p.lam[at]) * dts[o];
+        gxs[o] = gamma * x;
+        exs[o] = (gamma + serve_look(p, at + p.D, t0 + s + 1 < q.end)) * x;
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < kC; ++s) {
+      const float dt = __shfl_sync(0xffffffffu, dts[s / LPC], base + s % LPC);
+      const float gx = MODE == kOut ? __shfl_sync(0xffffffffu, gxs[s / LPC], base + s % LPC) : 0.f;
+      const float ex = MODE != kAngles ? __shfl_sync(0xffffffffu, exs[s / LPC], base + s % LPC) : 0.f;
+      dsum += dt;
+      float acc = 0.f;
+#pragma unroll
+      for (int r = 0; r < PR; ++r) {
+        turn[r] += m3_turn(dt, theta[s][r]);
+        taint[r] = m3_taint(dt * theta[s][r], taint[r]);
+        if (MODE == kAngles) continue;
+        const float2 unit = m3_unit(turn[r], taint[r]);
+        const float2 u = m3_back(bv[s][r], unit);
+        const float v0 = expf(a[r][0] * dt) * G[r][0], v1 = expf(a[r][1] * dt) * G[r][1];
+        if (MODE == kOut) {
+          const float2 c = m3_back(cv[s][r], unit);
+          acc = fmaf(fmaf(gx, u.x, v0), c.x, fmaf(fmaf(gx, u.y, v1), c.y, acc));
+        }
+        G[r][0] = fmaf(ex, u.x, v0);
+        G[r][1] = fmaf(ex, u.y, v1);
+      }
+      ys[s] = acc;
+    }
+    if (MODE == kOut) {
+#pragma unroll
+      for (int s = 0; s < kC; ++s) {
+#pragma unroll
+        for (int o = LPC / 2; o > 0; o >>= 1) ys[s] += __shfl_xor_sync(0xffffffffu, ys[s], o);
+        if (live && sl == s % LPC && t0 + s < q.last) static_cast<IO*>(p.y)[(size_t)(t0 + s) * p.D + d] = from_f32<IO>(ys[s]);
+      }
+    }
+  }
+  if (!live) return;
+  if (MODE == kAngles) {
+    const size_t row = (size_t)blockIdx.x * p.D + d;
+    if (sl == 0) p.dsum[row] = dsum;
+#pragma unroll
+    for (int r = 0; r < PR; ++r)
+      if (has(r)) {
+        p.turn[row * p.Kp + kp(r)] = turn[r];
+        p.spoil[row * p.Kp + kp(r)] = taint[r];
+      }
+    return;
+  }
+  if (MODE == kOut && (q.seg != q.segs - 1 || slot < 0)) return;
+#pragma unroll
+  for (int r = 0; r < PR; ++r) {
+    if (!has(r)) continue;
+    const float2 v = make_float2(G[r][0], G[r][1]);
+    if (MODE == kEnds) {
+      reinterpret_cast<float2*>(p.ends)[((size_t)blockIdx.x * p.D + d) * p.Kp + kp(r)] = v;
+    } else {
+      reinterpret_cast<float2*>(p.h)[sd * p.Kp + kp(r)] = v;
+      p.phase[sd * p.Kp + kp(r)] = m3_unit(turn[r], taint[r]);
+    }
+  }
+}
+// What the segments of a sequence start from, as m3k_heads_chain_kernel.
+__global__ void __launch_bounds__(256) m3k_channels_chain_kernel(ServeP p, bool bf16_io) {
+  begin_dependent();
+  const Piece q = find_piece(p, blockIdx.x);
+  if (!q.ok || q.seg != 0 || q.segs == 1) return;
+  const size_t i = blockIdx.y * (size_t)256 + threadIdx.x, pairs = (size_t)p.D * p.Kp;
+  if (i >= pairs) return;
+  const int d = (int)(i / p.Kp), k = (int)(i % p.Kp), g = d / (p.D / p.G);
+  const int slot = serve_slot(p, q.seq);
+  float2 v = make_float2(0.f, 0.f);
+  if (slot >= 0 && serve_goes_on(p, q.seq)) {
+    const size_t sd = (size_t)slot * p.D + d, br = ((size_t)slot * p.G + g) * p.N + 2 * k;
+    v = reinterpret_cast<const float2*>(p.h)[sd * p.Kp + k];
+    const float w = serve_look(p, (size_t)q.begin * p.D + d, true) * (bf16_io ? to_f32(static_cast<const bf16*>(p.x_prev)[sd]) : static_cast<const float*>(p.x_prev)[sd]);
+    const float2 b = m3_back(bf16_io ? load_pair(static_cast<const bf16*>(p.b_prev) + br) : load_pair(static_cast<const float*>(p.b_prev) + br),
+                             p.phase[sd * p.Kp + k]);
+    v.x = fmaf(w, b.x, v.x);
+    v.y = fmaf(w, b.y, v.y);
+  }
+  const float a0 = -expf(p.a_log[(size_t)d * p.N + 2 * k]), a1 = -expf(p.a_log[(size_t)d * p.N + 2 * k + 1]);
+  float2* e = reinterpret_cast<float2*>(p.ends) + ((size_t)q.base * p.D + d) * p.Kp + k;
+  for (int s = 0; s < q.segs; ++s, e += pairs) {
+    const float2 was = v;
+    if (s < q.segs - 1) {
+      const float2 add = *e;
+      const float sum = p.dsum[(size_t)(q.base + s) * p.D + d];
+      v.x = fmaf(expf(a0 * sum), v.x, add.x);
+      v.y = fmaf(expf(a1 * sum), v.y, add.y);
+    }
+    *e = was;
+  }
+}
+
+// ------------------------------------------------------------------ host
+struct HeadShape { int LN, NV, R, slabs; };
+static HeadShape head_shape(const ServeP& p) {
+  HeadShape s{1, 1, 1, 1};
+  while (s.LN * 4 < p.N && s.LN < 32) s.LN *= 2;
+  while (s.LN * 4 * s.NV < p.N) s.NV *= 2;
+  const int at_once = 256 / s.LN, most = std::min(kRowsMost, at_once * (8 / s.NV));
+  s.slabs = (p.P + most - 1) / most;
+  const int per = (p.P + s.slabs - 1) / s.slabs;
+  while (s.R * at_once < per) s.R *= 2;
+  return s;
+}
+struct ChannelShape { int PR, LPC; };
+static ChannelShape channel_shape(const ServeP& p) {
+  ChannelShape s{1, 1};
+  while (s.LPC < p.Kp && s.LPC < 32) s.LPC *= 2;
+  while (s.LPC * s.PR < p.Kp) s.PR *= 2;
+  return s;
+}
+
+template <typename IO, Mode MODE>
+static void heads(const ServeP& p, cudaStream_t st) {
+  const HeadShape s = head_shape(p);
+  const size_t smem = sizeof(float) * (2 * kW * (size_t)s.LN * 4 * s.NV + 2 * kW * kRowsMost);
+  const dim3 grid(p.pieces, p.NH * s.slabs);
+  auto launch = [&](auto nv, auto r) {
+    constexpr int NV = decltype(nv)::value, R = decltype(r)::value;
+    MXB_LAUNCH(MODE == kOut ? "m3k_heads_kernel" : "m3k_heads_ends_kernel", st,
+               (launch_kernel(m3k_heads_kernel<IO, NV, R, MODE>, grid, 256, smem, st, p, s.LN)));
+  };
+  auto by_r = [&](auto nv) {
+    constexpr int NV = decltype(nv)::value;
+    if (s.R == 1) launch(nv, std::integral_constant<int, 1>{});
+    else if (s.R == 2) launch(nv, std::integral_constant<int, 2>{});
+    else if (s.R == 4 || NV == 2) launch(nv, std::integral_constant<int, 4>{});
+    else launch(nv, std::integral_constant<int, 8>{});
+  };
+  if (s.NV == 1) by_r(std::integral_constant<int, 1>{});
+  else by_r(std::integral_constant<int, 2>{});
+}
+template <typename IO, Mode MODE>
+static void channels(const ServeP& p, cudaStream_t st) {
+  const ChannelShape s = channel_shape(p);
+  const dim3 grid(p.pieces, (p.D + 128 / s.LPC - 1) / (128 / s.LPC));
+  auto launch = [&](auto kernel) {
+    MXB_LAUNCH(MODE == kOut ? "m3k_channels_kernel" : MODE == kEnds ? "m3k_channels_ends_kernel" : "m3k_channels_angles_kernel", st,
+               (launch_kernel(kernel, grid, 128, 0, st, p)));
+  };
+  switch (s.LPC * s.PR) {
+    case 1: launch(m3k_channels_kernel<IO, 1, 1, MODE>); break;
+    case 2: launch(m3k_channels_kernel<IO, 1, 2, MODE>); break;
+    case 4: launch(m3k_channels_kernel<IO, 1, 4, MODE>); break;
+    case 8: launch(m3k_channels_kernel<IO, 1, 8, MODE>); break;
+    case 16: launch(m3k_channels_kernel<IO, 1, 16, MODE>); break;
+    case 32: launch(m3k_channels_kernel<IO, 1, 32, MODE>); break;
+    case 64: launch(m3k_channels_kernel<IO, 2, 32, MODE>); break;
+    default: launch(m3k_channels_kernel<IO, 4, 32, MODE>); break;
+  }
+}
+template <typename IO>
+static mxb_status prefill(const ServeP& p, cudaStream_t st) {
+  const dim3 chain(p.pieces, (unsigned)(((size_t)p.D * p.Kp + 255) / 256));
+  const bool cut = p.ends != nullptr;
+  if (p.NH) {
+    if (cut) {
+      heads<IO, kEnds>(p, st);
+      MXB_LAUNCH("m3k_heads_chain_kernel", st, (launch_kernel(m3k_heads_chain_kernel, chain, 256, 0, st, p, sizeof(IO) == 2)));
+    }
+    heads<IO, kOut>(p, st);
+    if (p.slabs > 1) MXB_LAUNCH("m3k_heads_phase_kernel", st, (launch_kernel(m3k_heads_phase_kernel, dim3(p.S, p.NH), 256, 0, st, p)));
+  } else {
+    if (cut) {
+      channels<IO, kAngles>(p, st);
+      channels<IO, kEnds>(p, st);
+      MXB_LAUNCH("m3k_channels_chain_kernel", st, (launch_kernel(m3k_channels_chain_kernel, chain, 256, 0, st, p, sizeof(IO) == 2)));
+    }
+    channels<IO, kOut>(p, st);
+  }
+  const mxb_status s = check_launch("m3k_prefill");
+  return s == MXB_OK ? m3serve_tails(p, sizeof(IO) == 4, true, st) : s;
+}
+
+}  // namespace m3k
+
+// Steps of a segment: as many segments as CTAs that the GPU holds at once, and at least 64 steps each.  (The host does not know
+// the lengths; sequences of up to L steps are not cut.)
+static int walk_segment(const ServeP& p) {
+  const long long ctas = p.NH ? (long long)p.NH * p.slabs : [&] {
+    const int per = 128 / m3k::channel_shape(p).LPC;
+    return (long long)((p.D + per - 1) / per);
+  }();
+  const long long at_once = p.NH ? 148 * 3 : 148 * 8;
+  const long long L = (p.rows * ctas + at_once - 1) / at_once;
+  return (int)std::max<long long>(64, (L + 63) / 64 * 64);
+}
+// Sets the cut and lays out the scratch (base may be null: only its size is wanted).
+size_t m3walk_scratch(ServeP& p, bool f32, int flags, char* base) {
+  p.slabs = p.NH ? m3k::head_shape(p).slabs : 1;
+  p.L = flags & MXB_MAMBA3_SERIAL_WALK ? std::max(p.rows, 1) : walk_segment(p);
+  if (p.rows <= p.L) {
+    p.pieces = p.S;
+    return 0;
+  }
+  p.pieces = (p.rows + p.L - 1) / p.L + p.S;
+  Carver c(base);
+  p.ends = c.take<float>((size_t)p.pieces * p.D * p.N);
+  p.dsum = c.take<float>((size_t)p.pieces * (p.NH ? p.NH : p.D));
+  p.turn = c.take<int>((size_t)p.pieces * (p.NH ? p.NH : (size_t)p.D * p.Kp));
+  if (p.NH) p.start = c.take<float2>((size_t)p.pieces * p.NH);
+  else p.spoil = c.take<float>((size_t)p.pieces * p.D * p.Kp);
+  return c.bytes();
+}
+mxb_status m3walk_prefill(const ServeP& p, bool f32, cudaStream_t st) {
+  return f32 ? m3k::prefill<float>(p, st) : m3k::prefill<m3k::bf16>(p, st);
+}
+
+}  // namespace mxb

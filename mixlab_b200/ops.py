@@ -10,6 +10,7 @@ allocation, the cached workspace and the C ABI calls are native (csrc/front.cpp)
 from __future__ import annotations
 
 import ctypes as C
+from typing import NamedTuple
 
 import torch
 
@@ -162,3 +163,68 @@ def mamba3_block_post(y, z, post_norm, eps=1e-5):
 
 def mamba3_block_post_backward(y, z, post_norm, dout, eps=1e-5):
     return _native().mamba3_block_post_backward(y, z, post_norm, dout, eps)
+
+
+# ---------------------------------------------------------------- serving: state pools
+class Mamba3State(NamedTuple):
+    """The recurrent states of ``slots`` sequences, updated in place by ``mamba3_prefill`` and ``mamba3_decode_step``.
+
+    h [slots,D,N] float32; phase, cosine and sine of the running angle, float32 [slots,nheads,2] (per-channel layout
+    [slots,D,N/2,2]); x_prev [slots,D] and b_prev [slots,nheads,N] (per-channel layout [slots,G,N]), x and b of the last token,
+    the latter for each head that of its group."""
+    h: torch.Tensor
+    phase: torch.Tensor
+    x_prev: torch.Tensor
+    b_prev: torch.Tensor
+
+
+def mamba3_state(slots, D, N, G, *, nheads=0, dtype=torch.bfloat16, device="cuda") -> Mamba3State:
+    """A pool of states of sequences that have seen nothing."""
+    phase = torch.zeros((slots, nheads, 2) if nheads else (slots, D, N // 2, 2), device=device)
+    phase[..., 0] = 1.0
+    return Mamba3State(torch.zeros(slots, D, N, device=device), phase, torch.zeros(slots, D, dtype=dtype, device=device),
+                       torch.zeros(slots, nheads or G, N, dtype=dtype, device=device))
+
+
+def mamba3_prefill(x, dt, lam, theta, a_log, b, c, cu_seqlens, state, *, slots=None, go_on=None, nheads=0, out=None, flags=0):
+    """The scan of packed prompts: sequence i is rows cu_seqlens[i] .. cu_seqlens[i+1]-1 of x [rows,D], b, c [rows,G,N] and
+    of dt, lam, theta, which have ``mamba3_selective_scan``'s layouts with one row axis.  cu_seqlens [S+1] and slots [S], the
+    sequences' rows of ``state`` (None: 0, 1, ...; all different), are int32; go_on [S] bool tells which sequences go on
+    from their state (None: none), the others start from nothing.  Returns y [rows,D]; ``state`` then holds what
+    ``mamba3_decode_step`` or the next part of a prompt goes on from.  A sequence without tokens keeps its state; one whose slot
+    is negative or beyond the pool starts from nothing and keeps none; rows of no sequence are not written."""
+    return (_front or _native()).mamba3_prefill(x, dt, lam, theta, a_log, b, c, cu_seqlens, list(state), slots, go_on, nheads, out, flags)
+
+
+def mamba3_decode_step(state, x, dt, lam, theta, a_log, b, c, *, slots=None, nheads=0, out=None):
+    """One token of each of S sequences on ``state`` (updated in place): x [S,D], b, c [S,G,N], the others with S rows.  slots
+    [S] int32, all different (None: 0, 1, ...); a row whose slot is negative or beyond the pool is passed over and its row of
+    the result not written.  Returns y [S,D]."""
+    return (_front or _native()).mamba3_decode_step(list(state), x, dt, lam, theta, a_log, b, c, slots, nheads, out)
+
+
+def short_conv_prefill(x, w, cu_seqlens, conv_state, *, slots=None, go_on=None, bias=None, activation=None, out=None):
+    """Causal depthwise convolution of packed prompts: y_t = act(sum_k w[:,k] x_{t-k} + bias), x [rows,D], w [D,K] float32 of any
+    strides (a gated_deltanet block's [K,D] weights as ``conv.t()``), K <= 4, activation None or "silu".  conv_state
+    [slots,K-1,D], in x's type, holds each sequence's last K-1 inputs, oldest first: read where go_on, then written.
+    cu_seqlens, slots and go_on as for ``mamba3_prefill``."""
+    return (_front or _native()).short_conv_prefill(x, w, cu_seqlens, conv_state, slots, go_on, bias, activation, out)
+
+
+def short_conv_step(conv_state, x, w, *, slots=None, bias=None, activation=None, out=None):
+    """``short_conv_prefill`` for one token of each of S sequences, all of which go on: x [S,D] -> y [S,D]."""
+    return (_front or _native()).short_conv_step(conv_state, x, w, slots, bias, activation, out)
+
+
+# ---------------------------------------------------------------- residual stream
+def residual_norm(resid, y, norm, *, post_norm=None, z=None, scale=None, eps=1e-5):
+    """The residual stream between two blocks: with a = RMSNorm(y, post_norm, eps) SiLU(z), returns resid + scale a and its
+    RMSNorm with ``norm``, the next block's input.  resid, y, z [...,D] (resid in y's type or float32); norm, post_norm, scale
+    [D] float32; without post_norm, z or scale that step is left out.  D <= 16384."""
+    return (_front or _native()).residual_norm(resid, y, norm, post_norm, z, scale, eps)
+
+
+def residual_norm_backward(resid_out, y, norm, d_resid_out, dn, *, post_norm=None, z=None, scale=None, eps=1e-5):
+    """Gradients of ``residual_norm``: resid_out is what it returned, d_resid_out (None: zero) and dn the gradients of its two
+    results.  dict(d_resid, dy, dz, dnorm, dpost_norm, dscale), None for operands that were left out."""
+    return (_front or _native()).residual_norm_backward(resid_out, y, norm, d_resid_out, dn, post_norm, z, scale, eps)
