@@ -460,7 +460,7 @@ mxb_status mxb_mamba3_prefill(const mxb_mamba3_serve_desc* d, const void* x, con
     if (!aligned16(workspace)) return MXB_ERR_ALIGNMENT;
     m3walk_scratch(p, f32, d->flags, static_cast<char*>(workspace));
   }
-  return m3walk_prefill(p, f32, static_cast<cudaStream_t>(stream));
+  return m3walk_prefill(p, f32, d->flags, static_cast<cudaStream_t>(stream));
 }
 mxb_status mxb_mamba3_decode_step(const mxb_mamba3_serve_desc* d, const mxb_mamba3_state* state, const void* x, const float* dt,
                                   const float* lambda, const float* theta, const float* a_log, const void* b, const void* c,

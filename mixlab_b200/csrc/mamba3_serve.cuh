@@ -1,5 +1,6 @@
 // Shared declarations of the Mamba-3 serving kernels: packed prompts and single tokens on a pool of recurrent states
-// (mamba3_step.cu: one token; mamba3_walk.cu: prompts step by step, both layouts).
+// (mamba3_step.cu: one token; mamba3_walk.cu: prompts step by step, both layouts; mamba3_prompt.cu: prompts in chunks on the
+// tensor cores).
 #pragma once
 
 #include "mamba3.cuh"
@@ -26,6 +27,10 @@ struct ServeP {
   float* spoil;     // [pieces, D Kp]: NaN where the segment's angle is not finite, 0 elsewhere (channel layout)
   float2* start;    // [pieces, NH]: cosine and sine of the angle that the segment starts at (head layout)
   int slabs;        // head layout: CTAs that share a head's channels
+  // chunks on the tensor cores (mamba3_prompt.cu)
+  int chunks;       // at most: ceil(length / 64) of every sequence
+  float* scores;    // [chunks, G, 10 tiles, 2, 32 lanes, 8]
+  float* rec;       // [chunks, NH, 512]: scalars of a chunk's steps
 };
 
 // Angles are summed as 32-bit fractions of a turn, whose additions do not round and wrap by themselves.  dt theta as such a
@@ -56,46 +61,68 @@ __device__ __forceinline__ float2 m3_turned(float2 u, float2 by) {
   return make_float2(r.x * k, r.y * k);
 }
 
-// A segment of a sequence: rows [first, last) of the sequence [begin, end); `base` is the piece of its first segment.
+// A segment of a sequence: rows [first, last) of the sequence [begin, end); `base` is the piece of its first segment, `chunk` the
+// number of its own first chunk of 64 steps.
 struct Piece {
-  int seq, seg, segs, base, first, last, begin, end;
+  int seq, seg, segs, base, first, last, begin, end, chunk;
   bool ok;
 };
-// The index-th piece: sequences one after the other, each cut every L rows.  Called by whole warps.  Whatever cu holds, rows
-// stay inside the call's.
-__device__ __forceinline__ Piece find_piece(const ServeP& p, int index) {
+// The index-th piece: sequences one after the other, each cut every L rows; up to 32 sequences by falling length, so that the
+// long ones do not start last (32 heads of 16 sequences of 440 to 4377 rows: a third off the time).  Called by whole warps.
+// Whatever cu holds, rows stay inside the call's.
+__device__ __forceinline__ Piece find_piece(const ServeP& p, int index, int L) {
   const int lane = threadIdx.x & 31;
   Piece q{};
-  int before = 0;
+  int before = 0, chunks = 0;
   for (int s0 = 0; s0 < p.S; s0 += 32) {
     const int s = s0 + lane;
     int a = 0, e = 0, n = 0;
     if (s < p.S) {
       a = min(max(__ldg(p.cu + s), 0), p.rows);
       e = min(max(__ldg(p.cu + s + 1), a), p.rows);
-      n = (int)(((long long)e - a + p.L - 1) / p.L);
+      n = (int)(((long long)e - a + L - 1) / L);
     }
-    int incl = n;
+    int id = s;
+    if (p.S > 1 && p.S <= 32) {
+      const int len = s < p.S ? e - a : -1;
+      int rank = 0, from = 0;
+#pragma unroll 8
+      for (int j = 0; j < 32; ++j) {
+        const int other = __shfl_sync(0xffffffffu, len, j);
+        rank += other > len || (other == len && j < lane);
+      }
+#pragma unroll 8
+      for (int j = 0; j < 32; ++j)
+        if (__shfl_sync(0xffffffffu, rank, j) == lane) from = j;
+      id = from;
+      a = __shfl_sync(0xffffffffu, a, from);
+      e = __shfl_sync(0xffffffffu, e, from);
+      n = __shfl_sync(0xffffffffu, n, from);
+    }
+    int incl = n, cn = (e - a + 63) / 64;
+    const int own = cn;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
+      const int v = __shfl_up_sync(0xffffffffu, incl, o), c = __shfl_up_sync(0xffffffffu, cn, o);
+      if (lane >= o) { incl += v; cn += c; }
     }
     const unsigned m = __ballot_sync(0xffffffffu, before + incl > index);
     if (m) {
       const int src = __ffs(m) - 1;
-      q.seq = s0 + src;
+      q.seq = __shfl_sync(0xffffffffu, id, src);
       q.begin = __shfl_sync(0xffffffffu, a, src);
       q.end = __shfl_sync(0xffffffffu, e, src);
       q.segs = __shfl_sync(0xffffffffu, n, src);
       q.base = before + __shfl_sync(0xffffffffu, incl - n, src);
       q.seg = index - q.base;
-      q.first = q.begin + q.seg * p.L;
-      q.last = (int)min((long long)q.first + p.L, (long long)q.end);
+      q.first = q.begin + q.seg * L;
+      q.last = (int)min((long long)q.first + L, (long long)q.end);
+      q.chunk = chunks + __shfl_sync(0xffffffffu, cn - own, src) + (q.first - q.begin) / 64;
       q.ok = true;
       return q;
     }
     before += __shfl_sync(0xffffffffu, incl, 31);
+    chunks += __shfl_sync(0xffffffffu, cn, 31);
   }
   return q;
 }
@@ -115,9 +142,21 @@ __device__ __forceinline__ float serve_look(const ServeP& p, size_t at, bool in)
 template <typename IO>
 __device__ __forceinline__ float2 load_pair(const IO* p) { return make_float2(to_f32(p[0]), to_f32(p[1])); }
 
+// The last row of a head into the pool: x of its channels, b of its group.  By a CTA that alone reads them.
+template <typename IO>
+__device__ __forceinline__ void serve_tail(const ServeP& p, int row, int slot, int hd, int g, int threads) {
+  const IO *X = static_cast<const IO*>(p.x) + (size_t)row * p.D + (size_t)hd * p.P, *B = static_cast<const IO*>(p.b) + ((size_t)row * p.G + g) * p.N;
+  IO *XP = static_cast<IO*>(p.x_prev) + (size_t)slot * p.D + (size_t)hd * p.P, *BP = static_cast<IO*>(p.b_prev) + ((size_t)slot * p.NH + hd) * p.N;
+  for (int i = threadIdx.x; i < p.P; i += threads) XP[i] = X[i];
+  for (int i = threadIdx.x; i < p.N; i += threads) BP[i] = B[i];
+}
+
 mxb_status m3serve_step(const ServeP& p, bool f32, cudaStream_t st);
+bool m3prompt_supported(const ServeP& p, bool f32);
+mxb_status m3prompt_prepare(const ServeP& p, cudaStream_t st);
+mxb_status m3prompt_chunks(const ServeP& p, bool ends, cudaStream_t st);
 size_t m3walk_scratch(ServeP& p, bool f32, int flags, char* base);
-mxb_status m3walk_prefill(const ServeP& p, bool f32, cudaStream_t st);
+mxb_status m3walk_prefill(ServeP p, bool f32, int flags, cudaStream_t st);
 mxb_status m3serve_tails(const ServeP& p, bool f32, bool x_too, cudaStream_t st);
 
 }  // namespace mxb

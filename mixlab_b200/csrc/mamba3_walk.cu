@@ -39,8 +39,8 @@ __global__ void __launch_bounds__(256) m3k_heads_kernel(ServeP p, int LN) {
   __shared__ HeadSmem sc;
   __shared__ int s_turn;
   __shared__ float s_taint, s_dt;
-  const int tid = threadIdx.x, hd = blockIdx.y / p.slabs, slab = blockIdx.y % p.slabs;
-  const Piece q = find_piece(p, blockIdx.x);
+  const int heads = p.NH * p.slabs, piece = blockIdx.x / heads, tid = threadIdx.x, hd = blockIdx.x % heads / p.slabs, slab = blockIdx.x % p.slabs;
+  const Piece q = find_piece(p, piece, p.L);
   if (!q.ok || (MODE == kEnds && q.seg == q.segs - 1)) return;
   const int ln = tid % LN, rg = tid / LN, rows_at_once = 256 / LN, npad = LN * 4 * NV;
   const int per = (p.P + p.slabs - 1) / p.slabs, p0 = slab * per, np = min(per, p.P - p0);  // this CTA's channels of the head
@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(256) m3k_heads_kernel(ServeP p, int LN) {
   const size_t ph = (size_t)(slot < 0 ? 0 : slot) * p.NH + hd;
   const float A = -expf(p.a_log[hd]);
   float2 start = make_float2(1.f, 0.f);
-  if (MODE == kOut && q.segs > 1) start = p.start[(size_t)blockIdx.x * p.NH + hd];
+  if (MODE == kOut && q.segs > 1) start = p.start[(size_t)piece * p.NH + hd];
   else if (from_state) start = p.phase[ph];
 
   auto row_of = [&](int r) { return rg + r * rows_at_once; };
@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(256) m3k_heads_kernel(ServeP p, int LN) {
         float2 v = make_float2(0.f, 0.f);
         if (row < np && n < p.N) {
           if (MODE == kOut && q.segs > 1) {
-            v = *reinterpret_cast<const float2*>(p.ends + ((size_t)blockIdx.x * p.D + chan + row) * p.N + n);
+            v = *reinterpret_cast<const float2*>(p.ends + ((size_t)piece * p.D + chan + row) * p.N + n);
           } else if (from_state) {
             v = m3_on(*reinterpret_cast<const float2*>(p.h + ((size_t)slot * p.D + chan + row) * p.N + n), start);
             const float2 b = load_pair(static_cast<const IO*>(p.b_prev) + ph * p.N + n);
@@ -193,8 +193,8 @@ __global__ void __launch_bounds__(256) m3k_heads_kernel(ServeP p, int LN) {
   __syncthreads();
   const float2 ran = m3_unit(s_turn, s_taint);
   if (MODE == kEnds && tid == 0 && slab == 0) {
-    p.turn[(size_t)blockIdx.x * p.NH + hd] = s_turn;
-    p.dsum[(size_t)blockIdx.x * p.NH + hd] = s_dt + s_taint;
+    p.turn[(size_t)piece * p.NH + hd] = s_turn;
+    p.dsum[(size_t)piece * p.NH + hd] = s_dt + s_taint;
   }
   if (MODE == kOut && (q.seg != q.segs - 1 || slot < 0)) return;
 #pragma unroll
@@ -206,54 +206,67 @@ __global__ void __launch_bounds__(256) m3k_heads_kernel(ServeP p, int LN) {
         const int row = row_of(r), n = n_of(k) + i;
         if (row >= np || n >= p.N) continue;
         const float2 v = make_float2(G[r][k][i], G[r][k][i + 1]);
-        if (MODE == kEnds) *reinterpret_cast<float2*>(p.ends + ((size_t)blockIdx.x * p.D + chan + row) * p.N + n) = m3_on(v, ran);
+        if (MODE == kEnds) *reinterpret_cast<float2*>(p.ends + ((size_t)piece * p.D + chan + row) * p.N + n) = m3_on(v, ran);
         else *reinterpret_cast<float2*>(p.h + ((size_t)slot * p.D + chan + row) * p.N + n) = m3_back(v, start);
       }
-  // (the slabs of a head all read the phase; with more than one it is written behind this launch)
-  if (MODE == kOut && tid == 0 && p.slabs == 1) p.phase[ph] = m3_turned(start, ran);
+  // (the slabs of a head all read its phase and b_prev; with more than one they are written behind this launch)
+  if (MODE == kOut && p.slabs == 1) {
+    if (tid == 0) p.phase[ph] = m3_turned(start, ran);
+    serve_tail<IO>(p, q.end - 1, slot, hd, g, 256);
+  }
 }
 
-// What the segments of a sequence start from.  grid (pieces, blocks of pairs): the block of a sequence's first segment walks
-// over its segments, a thread per state pair of all channels.
+// What the segments of a sequence start from.  grid (pieces, blocks of pairs): the blocks of a sequence's first segment walk over
+// its segments, a thread per state pair of the channels; what kAhead segments add is requested at a time.
+constexpr int kAhead = 8;
 __global__ void __launch_bounds__(256) m3k_heads_chain_kernel(ServeP p, bool bf16_io) {
   begin_dependent();
-  const Piece q = find_piece(p, blockIdx.x);
-  if (!q.ok || q.seg != 0 || q.segs == 1) return;
-  const size_t i = blockIdx.y * (size_t)256 + threadIdx.x, pairs = (size_t)p.D * p.Kp;
-  if (i >= pairs) return;
-  const int d = (int)(i / p.Kp), k = (int)(i % p.Kp), hd = d / p.P;
+  const Piece q = find_piece(p, blockIdx.x, p.L);
+  if (!q.ok || q.seg != 0 || q.segs == 1 || q.base + q.segs > p.pieces) return;  // (more segments: lengths beyond the rows)
   const int slot = serve_slot(p, q.seq);
-  float2 at = make_float2(1.f, 0.f), v = make_float2(0.f, 0.f);
-  if (slot >= 0 && serve_goes_on(p, q.seq)) {
-    const size_t ph = (size_t)slot * p.NH + hd;
-    at = p.phase[ph];
-    v = m3_on(reinterpret_cast<const float2*>(p.h)[((size_t)slot * p.D + d) * p.Kp + k], at);
-    const float w = serve_look(p, (size_t)q.begin * p.NH + hd, true) *
-                    (bf16_io ? to_f32(static_cast<const bf16*>(p.x_prev)[(size_t)slot * p.D + d]) : static_cast<const float*>(p.x_prev)[(size_t)slot * p.D + d]);
-    const float2 b = bf16_io ? load_pair(static_cast<const bf16*>(p.b_prev) + ph * p.N + 2 * k) : load_pair(static_cast<const float*>(p.b_prev) + ph * p.N + 2 * k);
-    v.x = fmaf(w, b.x, v.x);
-    v.y = fmaf(w, b.y, v.y);
-  }
-  const float A = -expf(p.a_log[hd]);
-  const bool first = k == 0 && d % p.P == 0;
-  float2* e = reinterpret_cast<float2*>(p.ends) + ((size_t)q.base * p.D + d) * p.Kp + k;
-  for (int s = 0; s < q.segs; ++s, e += pairs) {
-    const size_t sh = (size_t)(q.base + s) * p.NH + hd;
-    const float2 was = v;
-    if (s < q.segs - 1) {
-      const float2 add = *e, ran = m3_unit(p.turn[sh], m3_taint(p.dsum[sh], 0.f));  // (dsum carries the angle's taint)
-      const float L = expf(A * p.dsum[sh]);
-      const float2 r = m3_on(v, ran);
-      v.x = fmaf(L, r.x, add.x);
-      v.y = fmaf(L, r.y, add.y);
-      if (first) {
-        p.start[sh] = at;
-        at = m3_turned(at, ran);
-      }
-    } else if (first) {
-      p.start[sh] = at;
+  const bool go = slot >= 0 && serve_goes_on(p, q.seq);
+  const size_t pairs = (size_t)p.D * p.Kp;
+  for (size_t i = blockIdx.y * (size_t)256 + threadIdx.x; i < pairs; i += gridDim.y * (size_t)256) {
+    const int d = (int)(i / p.Kp), k = (int)(i % p.Kp), hd = d / p.P;
+    float2 at = make_float2(1.f, 0.f), v = make_float2(0.f, 0.f);
+    if (go) {
+      const size_t ph = (size_t)slot * p.NH + hd;
+      at = p.phase[ph];
+      v = m3_on(reinterpret_cast<const float2*>(p.h)[((size_t)slot * p.D + d) * p.Kp + k], at);
+      const float w = serve_look(p, (size_t)q.begin * p.NH + hd, true) *
+                      (bf16_io ? to_f32(static_cast<const bf16*>(p.x_prev)[(size_t)slot * p.D + d]) : static_cast<const float*>(p.x_prev)[(size_t)slot * p.D + d]);
+      const float2 b = bf16_io ? load_pair(static_cast<const bf16*>(p.b_prev) + ph * p.N + 2 * k) : load_pair(static_cast<const float*>(p.b_prev) + ph * p.N + 2 * k);
+      v.x = fmaf(w, b.x, v.x);
+      v.y = fmaf(w, b.y, v.y);
     }
-    *e = was;
+    const float A = -expf(p.a_log[hd]);
+    const bool first = k == 0 && d % p.P == 0;
+    float2* e = reinterpret_cast<float2*>(p.ends) + ((size_t)q.base * p.D + d) * p.Kp + k;
+    for (int s0 = 0; s0 < q.segs; s0 += kAhead) {
+      const int n = min(kAhead, q.segs - s0), adds = min(kAhead, q.segs - 1 - s0);
+      float2 add[kAhead];
+      float sum[kAhead];
+      int turn[kAhead];
+#pragma unroll
+      for (int s = 0; s < kAhead; ++s) {
+        const size_t sh = (size_t)(q.base + s0 + s) * p.NH + hd;
+        add[s] = s < adds ? e[s * pairs] : make_float2(0.f, 0.f);
+        sum[s] = s < adds ? p.dsum[sh] : 0.f;
+        turn[s] = s < adds ? p.turn[sh] : 0;
+      }
+#pragma unroll
+      for (int s = 0; s < kAhead; ++s) {
+        if (s >= n) break;
+        e[s * pairs] = v;
+        if (first) p.start[(size_t)(q.base + s0 + s) * p.NH + hd] = at;
+        const float2 ran = m3_unit(turn[s], m3_taint(sum[s], 0.f)), r = m3_on(v, ran);  // (dsum carries the angle's taint)
+        const float L = expf(A * sum[s]);
+        v.x = fmaf(L, r.x, add[s].x);
+        v.y = fmaf(L, r.y, add[s].y);
+        if (first) at = m3_turned(at, ran);
+      }
+      e += kAhead * pairs;
+    }
   }
 }
 // The phase at a sequence's end where the heads are cut into slabs: summed again from dt theta.  grid (sequences, heads) x 256.
@@ -298,7 +311,7 @@ __global__ void __launch_bounds__(128) m3k_channels_kernel(ServeP p) {
   const int d_raw = blockIdx.y * CPB + threadIdx.x / LPC;
   const bool live = d_raw < p.D;
   const int d = live ? d_raw : p.D - 1;
-  const Piece q = find_piece(p, blockIdx.x);
+  const Piece q = find_piece(p, blockIdx.x, p.L);
   if (!q.ok || (MODE != kOut && q.seg == q.segs - 1)) return;
   const int slot = serve_slot(p, q.seq), g = d / (p.D / p.G);
   const bool go = slot >= 0 && serve_goes_on(p, q.seq);
@@ -428,37 +441,48 @@ __global__ void __launch_bounds__(128) m3k_channels_kernel(ServeP p) {
 // What the segments of a sequence start from, as m3k_heads_chain_kernel.
 __global__ void __launch_bounds__(256) m3k_channels_chain_kernel(ServeP p, bool bf16_io) {
   begin_dependent();
-  const Piece q = find_piece(p, blockIdx.x);
-  if (!q.ok || q.seg != 0 || q.segs == 1) return;
-  const size_t i = blockIdx.y * (size_t)256 + threadIdx.x, pairs = (size_t)p.D * p.Kp;
-  if (i >= pairs) return;
-  const int d = (int)(i / p.Kp), k = (int)(i % p.Kp), g = d / (p.D / p.G);
+  const Piece q = find_piece(p, blockIdx.x, p.L);
+  if (!q.ok || q.seg != 0 || q.segs == 1 || q.base + q.segs > p.pieces) return;  // (more segments: lengths beyond the rows)
   const int slot = serve_slot(p, q.seq);
-  float2 v = make_float2(0.f, 0.f);
-  if (slot >= 0 && serve_goes_on(p, q.seq)) {
-    const size_t sd = (size_t)slot * p.D + d, br = ((size_t)slot * p.G + g) * p.N + 2 * k;
-    v = reinterpret_cast<const float2*>(p.h)[sd * p.Kp + k];
-    const float w = serve_look(p, (size_t)q.begin * p.D + d, true) * (bf16_io ? to_f32(static_cast<const bf16*>(p.x_prev)[sd]) : static_cast<const float*>(p.x_prev)[sd]);
-    const float2 b = m3_back(bf16_io ? load_pair(static_cast<const bf16*>(p.b_prev) + br) : load_pair(static_cast<const float*>(p.b_prev) + br),
-                             p.phase[sd * p.Kp + k]);
-    v.x = fmaf(w, b.x, v.x);
-    v.y = fmaf(w, b.y, v.y);
-  }
-  const float a0 = -expf(p.a_log[(size_t)d * p.N + 2 * k]), a1 = -expf(p.a_log[(size_t)d * p.N + 2 * k + 1]);
-  float2* e = reinterpret_cast<float2*>(p.ends) + ((size_t)q.base * p.D + d) * p.Kp + k;
-  for (int s = 0; s < q.segs; ++s, e += pairs) {
-    const float2 was = v;
-    if (s < q.segs - 1) {
-      const float2 add = *e;
-      const float sum = p.dsum[(size_t)(q.base + s) * p.D + d];
-      v.x = fmaf(expf(a0 * sum), v.x, add.x);
-      v.y = fmaf(expf(a1 * sum), v.y, add.y);
+  const bool go = slot >= 0 && serve_goes_on(p, q.seq);
+  const size_t pairs = (size_t)p.D * p.Kp;
+  for (size_t i = blockIdx.y * (size_t)256 + threadIdx.x; i < pairs; i += gridDim.y * (size_t)256) {
+    const int d = (int)(i / p.Kp), k = (int)(i % p.Kp), g = d / (p.D / p.G);
+    float2 v = make_float2(0.f, 0.f);
+    if (go) {
+      const size_t sd = (size_t)slot * p.D + d, br = ((size_t)slot * p.G + g) * p.N + 2 * k;
+      v = reinterpret_cast<const float2*>(p.h)[sd * p.Kp + k];
+      const float w = serve_look(p, (size_t)q.begin * p.D + d, true) * (bf16_io ? to_f32(static_cast<const bf16*>(p.x_prev)[sd]) : static_cast<const float*>(p.x_prev)[sd]);
+      const float2 b = m3_back(bf16_io ? load_pair(static_cast<const bf16*>(p.b_prev) + br) : load_pair(static_cast<const float*>(p.b_prev) + br),
+                               p.phase[sd * p.Kp + k]);
+      v.x = fmaf(w, b.x, v.x);
+      v.y = fmaf(w, b.y, v.y);
     }
-    *e = was;
+    const float a0 = -expf(p.a_log[(size_t)d * p.N + 2 * k]), a1 = -expf(p.a_log[(size_t)d * p.N + 2 * k + 1]);
+    float2* e = reinterpret_cast<float2*>(p.ends) + ((size_t)q.base * p.D + d) * p.Kp + k;
+    for (int s0 = 0; s0 < q.segs; s0 += kAhead) {
+      const int n = min(kAhead, q.segs - s0), adds = min(kAhead, q.segs - 1 - s0);
+      float2 add[kAhead];
+      float sum[kAhead];
+#pragma unroll
+      for (int s = 0; s < kAhead; ++s) {
+        add[s] = s < adds ? e[s * pairs] : make_float2(0.f, 0.f);
+        sum[s] = s < adds ? p.dsum[(size_t)(q.base + s0 + s) * p.D + d] : 0.f;
+      }
+#pragma unroll
+      for (int s = 0; s < kAhead; ++s) {
+        if (s >= n) break;
+        e[s * pairs] = v;
+        v.x = fmaf(expf(a0 * sum[s]), v.x, add[s].x);
+        v.y = fmaf(expf(a1 * sum[s]), v.y, add[s].y);
+      }
+      e += kAhead * pairs;
+    }
   }
 }
 
 // ------------------------------------------------------------------ host
+static int serve_slabs(const ServeP& p) { return (p.P + kRowsMost - 1) / kRowsMost; }
 struct HeadShape { int LN, NV, R, slabs; };
 static HeadShape head_shape(const ServeP& p) {
   HeadShape s{1, 1, 1, 1};
@@ -482,7 +506,7 @@ template <typename IO, Mode MODE>
 static void heads(const ServeP& p, cudaStream_t st) {
   const HeadShape s = head_shape(p);
   const size_t smem = sizeof(float) * (2 * kW * (size_t)s.LN * 4 * s.NV + 2 * kW * kRowsMost);
-  const dim3 grid(p.pieces, p.NH * s.slabs);
+  const dim3 grid((unsigned)((size_t)p.pieces * p.NH * s.slabs));
   auto launch = [&](auto nv, auto r) {
     constexpr int NV = decltype(nv)::value, R = decltype(r)::value;
     MXB_LAUNCH(MODE == kOut ? "m3k_heads_kernel" : "m3k_heads_ends_kernel", st,
@@ -518,16 +542,24 @@ static void channels(const ServeP& p, cudaStream_t st) {
   }
 }
 template <typename IO>
-static mxb_status prefill(const ServeP& p, cudaStream_t st) {
-  const dim3 chain(p.pieces, (unsigned)(((size_t)p.D * p.Kp + 255) / 256));
+static mxb_status prefill(ServeP p, bool chunks, cudaStream_t st) {
+  // (a piece that is not a sequence's first has nothing to do: few blocks each where there are many)
+  const size_t blocks = ((size_t)p.D * p.Kp + 255) / 256;
+  const dim3 chain(p.pieces, (unsigned)std::min<size_t>(blocks, std::max<size_t>(148 * 32 / p.pieces, 1)));
   const bool cut = p.ends != nullptr;
   if (p.NH) {
+    p.slabs = chunks ? serve_slabs(p) : head_shape(p).slabs;
+    if (chunks)
+      if (const mxb_status s = m3prompt_prepare(p, st); s != MXB_OK) return s;
     if (cut) {
-      heads<IO, kEnds>(p, st);
+      if (!chunks) heads<IO, kEnds>(p, st);
+      else if (const mxb_status s = m3prompt_chunks(p, true, st); s != MXB_OK) return s;
       MXB_LAUNCH("m3k_heads_chain_kernel", st, (launch_kernel(m3k_heads_chain_kernel, chain, 256, 0, st, p, sizeof(IO) == 2)));
     }
-    heads<IO, kOut>(p, st);
-    if (p.slabs > 1) MXB_LAUNCH("m3k_heads_phase_kernel", st, (launch_kernel(m3k_heads_phase_kernel, dim3(p.S, p.NH), 256, 0, st, p)));
+    if (!chunks) heads<IO, kOut>(p, st);
+    else if (const mxb_status s = m3prompt_chunks(p, false, st); s != MXB_OK) return s;
+    if (p.slabs == 1) return check_launch("m3k_prefill");
+    MXB_LAUNCH("m3k_heads_phase_kernel", st, (launch_kernel(m3k_heads_phase_kernel, dim3(p.S, p.NH), 256, 0, st, p)));
   } else {
     if (cut) {
       channels<IO, kAngles>(p, st);
@@ -542,27 +574,31 @@ static mxb_status prefill(const ServeP& p, cudaStream_t st) {
 
 }  // namespace m3k
 
-// Steps of a segment: as many segments as CTAs that the GPU holds at once, and at least 64 steps each.  (The host does not know
-// the lengths; sequences of up to L steps are not cut.)
+// Steps of a segment: as many segments as CTAs that the GPU holds at once, and at least 64 steps each; a quarter longer where
+// several sequences can fill the GPU side by side, since a cut costs a pass of its own over what lies in front of it.  (The host
+// does not know the lengths; sequences of up to L steps are not cut.)
 static int walk_segment(const ServeP& p) {
-  const long long ctas = p.NH ? (long long)p.NH * p.slabs : [&] {
+  const long long ctas = p.NH ? (long long)p.NH * m3k::serve_slabs(p) : [&] {
     const int per = 128 / m3k::channel_shape(p).LPC;
     return (long long)((p.D + per - 1) / per);
   }();
-  const long long at_once = p.NH ? 148 * 3 : 148 * 8;
-  const long long L = (p.rows * ctas + at_once - 1) / at_once;
-  return (int)std::max<long long>(64, (L + 63) / 64 * 64);
+  const long long at_once = p.NH ? 148 * 2 : 148 * 8;
+  long long L = (p.rows * ctas + at_once - 1) / at_once;
+  if (p.S > 1) L += L / 4;
+  return (int)std::min<long long>(std::max<long long>(64, (L + 63) / 64 * 64), INT32_MAX);
 }
 // Sets the cut and lays out the scratch (base may be null: only its size is wanted).
 size_t m3walk_scratch(ServeP& p, bool f32, int flags, char* base) {
-  p.slabs = p.NH ? m3k::head_shape(p).slabs : 1;
   p.L = flags & MXB_MAMBA3_SERIAL_WALK ? std::max(p.rows, 1) : walk_segment(p);
-  if (p.rows <= p.L) {
-    p.pieces = p.S;
-    return 0;
-  }
-  p.pieces = (p.rows + p.L - 1) / p.L + p.S;
   Carver c(base);
+  if (!(flags & MXB_MAMBA3_RECURRENT_KERNELS) && m3prompt_supported(p, f32)) {
+    p.chunks = p.rows / 64 + std::min(p.S, p.rows);
+    p.rec = c.take<float>((size_t)p.chunks * p.NH * 512);
+    p.scores = c.take<float>((size_t)p.chunks * p.G * 10 * 512);
+  }
+  p.pieces = p.S;
+  if (p.rows <= p.L) return c.bytes();
+  p.pieces = (p.rows + p.L - 1) / p.L + p.S;
   p.ends = c.take<float>((size_t)p.pieces * p.D * p.N);
   p.dsum = c.take<float>((size_t)p.pieces * (p.NH ? p.NH : p.D));
   p.turn = c.take<int>((size_t)p.pieces * (p.NH ? p.NH : (size_t)p.D * p.Kp));
@@ -570,8 +606,10 @@ size_t m3walk_scratch(ServeP& p, bool f32, int flags, char* base) {
   else p.spoil = c.take<float>((size_t)p.pieces * p.D * p.Kp);
   return c.bytes();
 }
-mxb_status m3walk_prefill(const ServeP& p, bool f32, cudaStream_t st) {
-  return f32 ? m3k::prefill<float>(p, st) : m3k::prefill<m3k::bf16>(p, st);
+// The chunks on the tensor cores where they cover the call, the walks elsewhere.
+mxb_status m3walk_prefill(ServeP p, bool f32, int flags, cudaStream_t st) {
+  if (f32) return m3k::prefill<float>(p, false, st);
+  return m3k::prefill<m3k::bf16>(p, !(flags & MXB_MAMBA3_RECURRENT_KERNELS) && m3prompt_supported(p, f32), st);
 }
 
 }  // namespace mxb
