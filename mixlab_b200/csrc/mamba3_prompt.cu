@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(kThreads) m3p_prepare_kernel(ServeP p) {
   __shared__ float s_l[4], s_r[4], s_taint[4], s_ds[4];
   __shared__ int s_turn[4];
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  const Piece q = find_piece(p, blockIdx.x, Q);
+  const Piece q = find_piece<false, false>(p, blockIdx.x, Q);
   if (!q.ok) return;
   if ((int)blockIdx.y < p.G) {
     const int grp = blockIdx.y;
@@ -136,15 +136,26 @@ __global__ void __launch_bounds__(kThreads) m3p_prepare_kernel(ServeP p) {
     return;
   }
   const int i = tid & 63, t = q.first + i, h0 = ((int)blockIdx.y - p.G) * kRecHeads;
-  for (int hh = h0; hh < min(h0 + kRecHeads, p.NH); hh += 2) {
-    const int hd = min(hh + (w >> 1), p.NH - 1);  // (an odd number of heads: one twice, the same record)
-    const bool in = t < q.last;
-    const size_t a = (size_t)(in ? t : q.first) * p.NH + hd;
+  const bool in = t < q.last, next = in && t + 1 < q.end;
+  float dts[kRecHeads / 2][2], lams[kRecHeads / 2][2], thetas[kRecHeads / 2], logs[kRecHeads / 2];  // (requested before the first is used)
+#pragma unroll
+  for (int k = 0; k < kRecHeads / 2; ++k) {
+    const int hd = min(h0 + 2 * k + (w >> 1), p.NH - 1);
+    const size_t a = (size_t)(in ? t : q.first) * p.NH + hd, b = a + (next ? p.NH : 0);
+    dts[k][0] = p.dt[a]; dts[k][1] = p.dt[b];
+    lams[k][0] = p.lam[a]; lams[k][1] = p.lam[b];
+    thetas[k] = p.theta[a];
+    logs[k] = p.a_log[hd];
+  }
+#pragma unroll
+  for (int k = 0; k < kRecHeads / 2; ++k) {
+    if (h0 + 2 * k >= p.NH) break;
+    const int hd = min(h0 + 2 * k + (w >> 1), p.NH - 1);  // (an odd number of heads: one twice, the same record)
     // dt in 64 bits: an angle sums up tens of thousands of them, and their float32 roundings with it
-    const double raw = p.dt[a], dt64 = fmax(raw, 0.0) + log1p(exp(-fabs(raw)));
-    const float dt = (float)dt64, lam = m3_sigmoid(p.lam[a]), theta = p.theta[a];
-    const float look = serve_look(p, a + p.NH, in && t + 1 < q.end);
-    const float A2 = -expf(p.a_log[hd]) * 1.4426950408889634f;
+    const double raw = dts[k][0], dt64 = fmax(raw, 0.0) + log1p(exp(-fabs(raw)));
+    const float dt = (float)dt64, lam = m3_sigmoid(lams[k][0]), theta = thetas[k];
+    const float look = next ? (1.f - m3_sigmoid(lams[k][1])) * m3_softplus(dts[k][1]) : 0.f;
+    const float A2 = -expf(logs[k]) * 1.4426950408889634f;
     const double f = dt64 * theta * 0.15915494309189535;
     int turn = in ? (int)__double2ll_rn((f - rint(f)) * 4294967296.0) : 0;
     float taint = in ? m3_taint(dt * theta, 0.f) : 0.f, l = in ? dt * A2 : 0.f, r = l;

@@ -23,7 +23,8 @@ struct ServeP {
   int L, pieces;
   float* ends;      // [pieces, D, N]: what a segment adds to the state, then the state that it starts from
   float* dsum;      // [pieces, NH or D]: sum of dt over the segment
-  int* turn;        // [pieces, NH or D Kp]: angle of the segment in 2^-32 turns
+  int* turn;        // [pieces, NH or D Kp]: angle of the segment in 2^-32 turns (channel layout: then the one that it starts at)
+  float* ends2;     // [pieces, D, N]: what a segment adds by the sine of the angle that it starts at (channel layout)
   float* spoil;     // [pieces, D Kp]: NaN where the segment's angle is not finite, 0 elsewhere (channel layout)
   float2* start;    // [pieces, NH]: cosine and sine of the angle that the segment starts at (head layout)
   int slabs;        // head layout: CTAs that share a head's channels
@@ -48,6 +49,7 @@ __device__ __forceinline__ float2 m3_unit(int turn, float taint) {  // cosine, s
   sincospif((float)turn * 4.656612873077393e-10f, &s, &c);
   return make_float2(c + taint, s + taint);
 }
+__device__ __forceinline__ int serve_turn(float2 unit) { return __float2int_rn(atan2f(unit.y, unit.x) * 0.15915494309189535f * 4294967296.f); }
 __device__ __forceinline__ float2 m3_back(float2 v, float2 a) {  // R^T: v turned back by the angle of a
   return make_float2(fmaf(a.x, v.x, a.y * v.y), fmaf(a.x, v.y, -a.y * v.x));
 }
@@ -70,6 +72,8 @@ struct Piece {
 // The index-th piece: sequences one after the other, each cut every L rows; up to 32 sequences by falling length, so that the
 // long ones do not start last (32 heads of 16 sequences of 440 to 4377 rows: a third off the time).  Called by whole warps.
 // Whatever cu holds, rows stay inside the call's.
+// SEQUENCE: the first piece of the index-th sequence in that order.  SORT: false: sequences as they come (chunks are numbered so).
+template <bool SEQUENCE = false, bool SORT = true>
 __device__ __forceinline__ Piece find_piece(const ServeP& p, int index, int L) {
   const int lane = threadIdx.x & 31;
   Piece q{};
@@ -82,8 +86,16 @@ __device__ __forceinline__ Piece find_piece(const ServeP& p, int index, int L) {
       e = min(max(__ldg(p.cu + s + 1), a), p.rows);
       n = (int)(((long long)e - a + L - 1) / L);
     }
-    int id = s;
-    if (p.S > 1 && p.S <= 32) {
+    int id = s, cn = (e - a + 63) / 64, chunk = cn;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int c = __shfl_up_sync(0xffffffffu, chunk, o);
+      if (lane >= o) chunk += c;
+    }
+    const int all = __shfl_sync(0xffffffffu, chunk, 31);
+    chunk += chunks - cn;
+    chunks += all;
+    if (SORT && p.S > 1 && p.S <= 32) {
       const int len = s < p.S ? e - a : -1;
       int rank = 0, from = 0;
 #pragma unroll 8
@@ -98,15 +110,15 @@ __device__ __forceinline__ Piece find_piece(const ServeP& p, int index, int L) {
       a = __shfl_sync(0xffffffffu, a, from);
       e = __shfl_sync(0xffffffffu, e, from);
       n = __shfl_sync(0xffffffffu, n, from);
+      chunk = __shfl_sync(0xffffffffu, chunk, from);
     }
-    int incl = n, cn = (e - a + 63) / 64;
-    const int own = cn;
+    int incl = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, incl, o), c = __shfl_up_sync(0xffffffffu, cn, o);
-      if (lane >= o) { incl += v; cn += c; }
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
     }
-    const unsigned m = __ballot_sync(0xffffffffu, before + incl > index);
+    const unsigned m = __ballot_sync(0xffffffffu, SEQUENCE ? s == index : before + incl > index);
     if (m) {
       const int src = __ffs(m) - 1;
       q.seq = __shfl_sync(0xffffffffu, id, src);
@@ -114,15 +126,14 @@ __device__ __forceinline__ Piece find_piece(const ServeP& p, int index, int L) {
       q.end = __shfl_sync(0xffffffffu, e, src);
       q.segs = __shfl_sync(0xffffffffu, n, src);
       q.base = before + __shfl_sync(0xffffffffu, incl - n, src);
-      q.seg = index - q.base;
+      q.seg = SEQUENCE ? 0 : index - q.base;
       q.first = q.begin + q.seg * L;
       q.last = (int)min((long long)q.first + L, (long long)q.end);
-      q.chunk = chunks + __shfl_sync(0xffffffffu, cn - own, src) + (q.first - q.begin) / 64;
-      q.ok = true;
+      q.chunk = __shfl_sync(0xffffffffu, chunk, src) + (q.first - q.begin) / 64;
+      q.ok = q.segs > 0;
       return q;
     }
     before += __shfl_sync(0xffffffffu, incl, 31);
-    chunks += __shfl_sync(0xffffffffu, cn, 31);
   }
   return q;
 }

@@ -29,18 +29,20 @@ __device__ __forceinline__ void store_states(float* p, const float (&e)[V]) {
   else __stcs(reinterpret_cast<float2*>(p), make_float2(e[0], e[1]));
 }
 
-// Heads: a CTA per (sequence, head); LN lanes along a row of states with NV pieces of V each, 8 / NV rows a thread at a time.
-// b_prev has a row a head, so that the CTA which writes it is the only one that reads it.
-constexpr int kStepPieces = 8;
+// Heads: a CTA per (sequence, head); LN lanes along a row of states with NV pieces of V each, 8 / NV consecutive rows a thread at a
+// time.  The pieces are requested first; meanwhile two warps work out the scalars and turn b, c and the token before's b, two
+// more fetch x.  b_prev has a row a head, so that the CTA which writes it is the only one that reads it.
+constexpr int kStepPieces = 8, kStepRowsMost = 8 * 256;
 template <typename IO, int V, int NV>
 __global__ void __launch_bounds__(256) m3s_step_heads_kernel(ServeP p, int LN) {
   begin_dependent();
   constexpr int R = kStepPieces / NV;
   __shared__ __align__(16) float s_u[256], s_v[256], s_c[256];
-  const int seq = blockIdx.x / p.NH, hd = blockIdx.x % p.NH, tid = threadIdx.x;
+  __shared__ float s_x[kStepRowsMost], s_xp[kStepRowsMost], s_alpha;
+  const int seq = blockIdx.x / p.NH, hd = blockIdx.x % p.NH, tid = threadIdx.x, lane = tid & 31;
   const int slot = serve_slot(p, seq);
   if (slot < 0) return;
-  const int ln = tid % LN, rg = tid / LN, rows_at_once = 256 / LN, npad = LN * V * NV;
+  const int ln = tid % LN, rg = tid / LN, at_once = 256 / LN * R, npad = LN * V * NV;
   const size_t chan = (size_t)hd * p.P;  // first channel of the head
   float* hp = p.h + ((size_t)slot * p.D + chan) * p.N;
   float st[R][NV][V];
@@ -48,7 +50,7 @@ __global__ void __launch_bounds__(256) m3s_step_heads_kernel(ServeP p, int LN) {
   auto load = [&](int r0) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const int row = r0 + rg + r * rows_at_once;
+      const int row = r0 + rg * R + r;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         if (piece(k) < p.N && row < p.P) {
@@ -61,69 +63,94 @@ __global__ void __launch_bounds__(256) m3s_step_heads_kernel(ServeP p, int LN) {
     }
   };
   load(0);
-  const size_t sh = (size_t)seq * p.NH + hd, ph = (size_t)slot * p.NH + hd;
-  const float dt = m3_softplus(p.dt[sh]), lam = m3_sigmoid(p.lam[sh]), theta = p.theta[sh];
-  const float alpha = expf(-expf(p.a_log[hd]) * dt), look = (1.f - lam) * dt, gamma = lam * dt;
-  const float2 old = p.phase[ph];
-  const float2 now = m3_turned(old, m3_unit(m3_turn(dt, theta), m3_taint(dt * theta, 0.f)));
-  const int g = hd / (p.NH / p.G);
-  const IO *B = static_cast<const IO*>(p.b) + ((size_t)seq * p.G + g) * p.N, *C = static_cast<const IO*>(p.c) + ((size_t)seq * p.G + g) * p.N;
-  IO* BP = static_cast<IO*>(p.b_prev) + ph * p.N;
-  for (int k = tid; k < npad / 2; k += 256) {
-    float2 u = make_float2(0.f, 0.f), v = u, c = u;
-    if (2 * k < p.N) {
-      const float2 b = load_pair(B + 2 * k);
-      u = m3_back(b, now);
-      c = m3_back(load_pair(C + 2 * k), now);
-      v = m3_back(load_pair(BP + 2 * k), old);
-      BP[2 * k] = from_f32<IO>(b.x);
-      BP[2 * k + 1] = from_f32<IO>(b.y);
-    }
-    s_u[2 * k] = gamma * u.x; s_u[2 * k + 1] = gamma * u.y;
-    s_v[2 * k] = look * v.x; s_v[2 * k + 1] = look * v.y;
-    s_c[2 * k] = c.x; s_c[2 * k + 1] = c.y;
-  }
-  __syncthreads();  // (also behind every thread's read of the phase)
-  if (tid == 0) p.phase[ph] = now;
   const IO* X = static_cast<const IO*>(p.x) + (size_t)seq * p.D + chan;
   IO* XP = static_cast<IO*>(p.x_prev) + (size_t)slot * p.D + chan;
   IO* Y = static_cast<IO*>(p.y) + (size_t)seq * p.D + chan;
-  for (int r0 = 0; r0 < p.P; r0 += R * rows_at_once) {
-    if (r0) load(r0);
-    float xv[R], acc[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int row = r0 + rg + r * rows_at_once;
-      const bool live = row < p.P;
-      xv[r] = live ? to_f32(X[row]) : 0.f;
-      const float xp = live ? to_f32(XP[row]) : 0.f;
-      acc[r] = 0.f;
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const int n = piece(k) + i;
-          st[r][k][i] = fmaf(xv[r], s_u[n], alpha * fmaf(xp, s_v[n], st[r][k][i]));
-          acc[r] = fmaf(st[r][k][i], s_c[n], acc[r]);
-        }
-        if (piece(k) < p.N && live) store_states<V>(hp + (size_t)row * p.N + piece(k), st[r][k]);
-      }
+  auto load_x = [&](int r0, int first, int threads) {  // (one thread reads and then writes a channel's x_prev)
+    for (int i = tid - first; i < min(at_once, p.P - r0); i += threads) {
+      const IO x = X[r0 + i];
+      s_xp[i] = to_f32(XP[r0 + i]);
+      s_x[i] = to_f32(x);
+      XP[r0 + i] = x;
     }
+  };
+  const size_t sh = (size_t)seq * p.NH + hd, ph = (size_t)slot * p.NH + hd;
+  if (tid < 64) {
+    const float dt = m3_softplus(p.dt[sh]), lam = m3_sigmoid(p.lam[sh]), theta = p.theta[sh];
+    const float look = (1.f - lam) * dt, gamma = lam * dt;
+    const float2 old = p.phase[ph];
+    const float2 now = m3_turned(old, m3_unit(m3_turn(dt, theta), m3_taint(dt * theta, 0.f)));
+    const int g = hd / (p.NH / p.G);
+    const IO *B = static_cast<const IO*>(p.b) + ((size_t)seq * p.G + g) * p.N, *C = static_cast<const IO*>(p.c) + ((size_t)seq * p.G + g) * p.N;
+    IO* BP = static_cast<IO*>(p.b_prev) + ph * p.N;
+    for (int k = tid; k < npad / 2; k += 64) {
+      float2 u = make_float2(0.f, 0.f), v = u, c = u;
+      if (2 * k < p.N) {
+        const float2 b = load_pair(B + 2 * k);
+        u = m3_back(b, now);
+        c = m3_back(load_pair(C + 2 * k), now);
+        v = m3_back(load_pair(BP + 2 * k), old);
+        BP[2 * k] = from_f32<IO>(b.x);
+        BP[2 * k + 1] = from_f32<IO>(b.y);
+      }
+      reinterpret_cast<float2*>(s_u)[k] = make_float2(gamma * u.x, gamma * u.y);
+      reinterpret_cast<float2*>(s_v)[k] = make_float2(look * v.x, look * v.y);
+      reinterpret_cast<float2*>(s_c)[k] = c;
+    }
+    asm volatile("bar.sync 1, 64;" ::: "memory");  // (both warps have read the phase)
+    if (tid == 0) {
+      s_alpha = expf(-expf(p.a_log[hd]) * dt);
+      p.phase[ph] = now;
+    }
+  } else {
+    load_x(0, 64, 192);
+  }
+  __syncthreads();
+  const float alpha = s_alpha;
+  for (int r0 = 0; r0 < p.P; r0 += at_once) {
+    if (r0) {
+      __syncthreads();
+      load(r0);
+      load_x(r0, 0, 256);
+      __syncthreads();
+    }
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-      if (o < LN)
+    for (int k = 0; k < NV; ++k) {
+      float u[V], v[V], c[V];
 #pragma unroll
-        for (int r = 0; r < R; ++r) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], o);
-    __syncwarp();  // x_prev is written behind the reads of all lanes of its row
-    if (ln == 0)
+      for (int j = 0; j < V; j += 2) {
+        const int n = (piece(k) + j) / 2;
+        const float2 a = reinterpret_cast<const float2*>(s_u)[n], b = reinterpret_cast<const float2*>(s_v)[n], d = reinterpret_cast<const float2*>(s_c)[n];
+        u[j] = a.x; u[j + 1] = a.y; v[j] = b.x; v[j + 1] = b.y; c[j] = d.x; c[j + 1] = d.y;
+      }
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const int row = r0 + rg + r * rows_at_once;
-        if (row < p.P) {
-          Y[row] = from_f32<IO>(acc[r]);
-          XP[row] = from_f32<IO>(xv[r]);
+        const int i = rg * R + r, row = r0 + i;
+        const float x = s_x[i], xp = s_xp[i];  // (behind the head's last channel whatever stands there: its rows go nowhere)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          st[r][k][j] = fmaf(x, u[j], alpha * fmaf(xp, v[j], st[r][k][j]));
+          acc[r] = fmaf(st[r][k][j], c[j], acc[r]);
         }
+        if (piece(k) < p.N && row < p.P) store_states<V>(hp + (size_t)row * p.N + piece(k), st[r][k]);
       }
+    }
+    if (LN == 32) {  // lane l gets row l & 7
+      colsum8(acc, lane);
+      const int row = r0 + rg * R + lane;
+      if (lane < R && row < p.P) Y[row] = from_f32<IO>(acc[0]);
+    } else {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1)
+        if (o < LN)
+#pragma unroll
+          for (int r = 0; r < R; ++r) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], o);
+      if (ln == 0)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          if (r0 + rg * R + r < p.P) Y[r0 + rg * R + r] = from_f32<IO>(acc[r]);
+    }
   }
 }
 

@@ -16,12 +16,13 @@
 #include <type_traits>
 
 #include "mamba3_serve.cuh"
+#include "packed.cuh"
 
 namespace mxb {
 namespace m3k {
 
 using bf16 = __nv_bfloat16;
-enum Mode { kOut, kEnds, kAngles };
+enum Mode { kOut, kEnds };
 
 // ------------------------------------------------------------------ heads
 // A CTA per (segment, head, slab of channels): LN lanes along a row of states, NV pieces of 4 states a lane, R rows a thread,
@@ -216,13 +217,13 @@ __global__ void __launch_bounds__(256) m3k_heads_kernel(ServeP p, int LN) {
   }
 }
 
-// What the segments of a sequence start from.  grid (pieces, blocks of pairs): the blocks of a sequence's first segment walk over
-// its segments, a thread per state pair of the channels; what kAhead segments add is requested at a time.
+// What the segments of a sequence start from.  grid (sequences, blocks of pairs): a thread per state pair of the channels walks
+// over the segments; what kAhead segments add is requested at a time.
 constexpr int kAhead = 8;
 __global__ void __launch_bounds__(256) m3k_heads_chain_kernel(ServeP p, bool bf16_io) {
   begin_dependent();
-  const Piece q = find_piece(p, blockIdx.x, p.L);
-  if (!q.ok || q.seg != 0 || q.segs == 1 || q.base + q.segs > p.pieces) return;  // (more segments: lengths beyond the rows)
+  const Piece q = find_piece<true>(p, blockIdx.x, p.L);
+  if (!q.ok || q.segs == 1 || q.base + q.segs > p.pieces) return;  // (more segments: lengths beyond the rows)
   const int slot = serve_slot(p, q.seq);
   const bool go = slot >= 0 && serve_goes_on(p, q.seq);
   const size_t pairs = (size_t)p.D * p.Kp;
@@ -301,8 +302,64 @@ __global__ void __launch_bounds__(256) m3k_heads_phase_kernel(ServeP p) {
 
 // ------------------------------------------------------------------ channels
 // LPC lanes a channel with PR state pairs each, 8 steps at a time: a lane works out softplus and sigmoid of its own steps and
-// hands them round; theta and the rows of b and c are requested before the first of the 8 steps.
+// hands them round; theta and the rows of b and c come by cp.async 8 steps ahead, each lane's own elements into its own places
+// in shared memory (no barrier, and no registers while they are under way).
+//
+// What bounds it is the issue of instructions, a sine, a cosine and two exponentials a state pair and step (4003 steps x 448
+// channels of 16 states: 14 M of them).  So two steps' angles go through packed polynomials, the two states of a pair are
+// packed, and y of 8 steps is added over 8 lanes by halving exchanges.
 constexpr int kC = 8;
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// Cosine and sine of two angles in 2^-32 turns: the nearest quarter turn by integers, Taylor polynomials of degree 9 and 10 on
+// what is left, at most pi / 4 (truncation below 2e-9, roundings below 1.2e-7 as in mamba3_windows.cu).
+__device__ __forceinline__ void unit2(int t0, int t1, float2& u0, float2& u1) {
+  const int k0 = (t0 + 0x20000000) >> 30, k1 = (t1 + 0x20000000) >> 30;
+  const f2 r = mul2(pack2((float)(t0 - (k0 << 30)), (float)(t1 - (k1 << 30))), dup2(1.4629180792671596e-9f));  // 2 pi / 2^32
+  const f2 r2 = mul2(r, r);
+  f2 ps = dup2(2.7557319223985893e-6f);
+  ps = mad2(ps, r2, dup2(-1.9841269841269841e-4f));
+  ps = mad2(ps, r2, dup2(8.3333333333333333e-3f));
+  ps = mad2(ps, r2, dup2(-1.6666666666666667e-1f));
+  ps = mad2(mul2(ps, r2), r, r);
+  f2 pc = dup2(-2.7557319223985888e-7f);
+  pc = mad2(pc, r2, dup2(2.4801587301587302e-5f));
+  pc = mad2(pc, r2, dup2(-1.3888888888888889e-3f));
+  pc = mad2(pc, r2, dup2(4.1666666666666667e-2f));
+  pc = mad2(pc, r2, dup2(-0.5f));
+  pc = mad2(pc, r2, dup2(1.f));
+  const float2 s = unpack2(ps), c = unpack2(pc);
+  auto quarter = [](float s, float c, int k) {
+    const float a = (k & 1) ? c : s, b = (k & 1) ? s : c;
+    return make_float2(__int_as_float(__float_as_int(b) ^ (((k + 1) & 2) << 30)), __int_as_float(__float_as_int(a) ^ ((k & 2) << 30)));
+  };
+  u0 = quarter(s.x, c.x, k0);
+  u1 = quarter(s.y, c.y, k1);
+}
+// m3_turn with dt theta rounded once, as dt is.
+__device__ __forceinline__ int turn_of(float p) {
+  constexpr float kHi = 0.15915493667125702f, kLo = 6.420638243e-09f;
+  const float t = p * kHi, tl = fmaf(p, kLo, fmaf(p, kHi, -t));
+  return __float2int_rn(((t - rintf(t)) + tl) * 4294967296.f);
+}
+// What a lane has requested of 8 steps.
+template <typename IO, int PR, Mode MODE>
+struct Ahead {
+  using Two = std::conditional_t<sizeof(IO) == 4, float2, uint32_t>;  // a pair of b or c
+  float theta[kC][PR][128];
+  Two b[kC][PR][128], c[MODE == kOut ? kC : 1][PR][128];
+};
+template <int BYTES>
+__device__ __forceinline__ void copy_ahead(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ float2 pair_of(float2 v) { return v; }
+__device__ __forceinline__ float2 pair_of(uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }
+
 template <typename IO, int PR, int LPC, Mode MODE>
 __global__ void __launch_bounds__(128) m3k_channels_kernel(ServeP p) {
   begin_dependent();
@@ -312,171 +369,281 @@ __global__ void __launch_bounds__(128) m3k_channels_kernel(ServeP p) {
   const bool live = d_raw < p.D;
   const int d = live ? d_raw : p.D - 1;
   const Piece q = find_piece(p, blockIdx.x, p.L);
-  if (!q.ok || (MODE != kOut && q.seg == q.segs - 1)) return;
+  if (!q.ok || (MODE == kEnds && q.seg == q.segs - 1)) return;
   const int slot = serve_slot(p, q.seq), g = d / (p.D / p.G);
-  const bool go = slot >= 0 && serve_goes_on(p, q.seq);
-  const size_t sd = (size_t)(slot < 0 ? 0 : slot) * p.D + d;
-  float G[PR][2], a[PR][2], taint[PR], dsum = 0.f;
-  int turn[PR];
-  auto kp = [&](int r) { return sl + r * LPC; };
-  auto has = [&](int r) { return kp(r) < p.Kp; };
+  const bool from_state = MODE == kOut && q.segs == 1 && slot >= 0 && serve_goes_on(p, q.seq);
+  const size_t sd = (size_t)(slot < 0 ? 0 : slot) * p.D + d, row = (size_t)blockIdx.x * p.D + d;
+  f2 G[PR], H[MODE == kEnds ? PR : 1];  // the state; kEnds: its factors of the cosine and of the sine of the angle at the start
+  float a[PR][2], taint[PR], dsum = 0.f;
+  int turn[PR], kp[PR];
+  bool has[PR];
 #pragma unroll
   for (int r = 0; r < PR; ++r) {
-    G[r][0] = G[r][1] = a[r][0] = a[r][1] = taint[r] = 0.f;
+    kp[r] = sl + r * LPC;
+    has[r] = kp[r] < p.Kp;
+    G[r] = 0;
+    if (MODE == kEnds) H[MODE == kEnds ? r : 0] = 0;
+    a[r][0] = a[r][1] = taint[r] = 0.f;
     turn[r] = 0;
-    if (!has(r)) continue;
-    const size_t pair = sd * p.Kp + kp(r);
-    float2 unit = make_float2(1.f, 0.f);
-    if (MODE != kAngles && go) {
-      unit = p.phase[pair];
-      turn[r] = __float2int_rn(atan2f(unit.y, unit.x) * 0.15915494309189535f * 4294967296.f);
-      taint[r] = m3_taint(unit.x, m3_taint(unit.y, 0.f));
-    }
-    if (MODE != kAngles) {
-      for (int s = 0; s < q.seg; ++s) {
-        const size_t at = (size_t)(q.base + s) * p.D * p.Kp + (size_t)d * p.Kp + kp(r);
-        turn[r] += p.turn[at];
-        taint[r] += p.spoil[at];
-      }
-      a[r][0] = -expf(p.a_log[(size_t)d * p.N + 2 * kp(r)]);
-      a[r][1] = -expf(p.a_log[(size_t)d * p.N + 2 * kp(r) + 1]);
-    }
+    if (!has[r]) continue;
+    a[r][0] = -expf(p.a_log[(size_t)d * p.N + 2 * kp[r]]) * 1.4426950408889634f;
+    a[r][1] = -expf(p.a_log[(size_t)d * p.N + 2 * kp[r] + 1]) * 1.4426950408889634f;
     if (MODE == kOut && q.segs > 1) {
-      const float2 v = reinterpret_cast<const float2*>(p.ends)[((size_t)blockIdx.x * p.D + d) * p.Kp + kp(r)];
-      G[r][0] = v.x;
-      G[r][1] = v.y;
-    } else if (MODE == kOut && go) {
-      const float2 v = reinterpret_cast<const float2*>(p.h)[pair];
-      const float2 b = m3_back(load_pair(static_cast<const IO*>(p.b_prev) + ((size_t)slot * p.G + g) * p.N + 2 * kp(r)), unit);
+      const float2 v = reinterpret_cast<const float2*>(p.ends)[row * p.Kp + kp[r]];
+      G[r] = pack2(v.x, v.y);
+      turn[r] = p.turn[row * p.Kp + kp[r]];
+      taint[r] = p.spoil[row * p.Kp + kp[r]];
+    } else if (from_state) {
+      const float2 unit = p.phase[sd * p.Kp + kp[r]], v = reinterpret_cast<const float2*>(p.h)[sd * p.Kp + kp[r]];
+      turn[r] = serve_turn(unit);
+      taint[r] = m3_taint(unit.x, m3_taint(unit.y, 0.f));
+      const float2 b = m3_back(load_pair(static_cast<const IO*>(p.b_prev) + ((size_t)slot * p.G + g) * p.N + 2 * kp[r]), unit);
       const float w = serve_look(p, (size_t)q.first * p.D + d, true) * to_f32(static_cast<const IO*>(p.x_prev)[sd]);
-      G[r][0] = fmaf(w, b.x, v.x);
-      G[r][1] = fmaf(w, b.y, v.y);
+      G[r] = pack2(fmaf(w, b.x, v.x), fmaf(w, b.y, v.y));
     }
   }
-  for (int t0 = q.first; t0 < q.last; t0 += kC) {
-    float theta[kC][PR];
-    float2 bv[kC][PR], cv[kC][PR];
-#pragma unroll
-    for (int s = 0; s < kC; ++s)
+  extern __shared__ __align__(16) unsigned char raw[];
+  using Block = Ahead<IO, PR, MODE>;
+  Block* ahead = reinterpret_cast<Block*>(raw);
+  const float* theta_at = p.theta + ((size_t)q.first * p.D + d) * p.Kp + sl;
+  const IO *b_at = static_cast<const IO*>(p.b) + ((size_t)q.first * p.G + g) * p.N + 2 * sl, *c_at = static_cast<const IO*>(p.c) + ((size_t)q.first * p.G + g) * p.N + 2 * sl;
+  const size_t theta_row = (size_t)p.D * p.Kp, bc_row = (size_t)p.G * p.N;
+  const bool pairs = ((reinterpret_cast<uintptr_t>(p.b) | reinterpret_cast<uintptr_t>(p.c)) & (2 * sizeof(IO) - 1)) == 0;
+  const size_t bc_bytes = bc_row * sizeof(IO), theta_bytes = theta_row * sizeof(float);
+  auto request = [&](int t0, Block& to) {  // zeros for steps behind the last and lanes without a pair
+    const int steps = min(kC, q.last - t0);
+    const char *th = reinterpret_cast<const char*>(theta_at), *b = reinterpret_cast<const char*>(b_at), *c = reinterpret_cast<const char*>(c_at);
+    if (pairs && steps == kC) {
 #pragma unroll
       for (int r = 0; r < PR; ++r) {
-        const size_t t = (size_t)min(t0 + s, q.last - 1);
-        const bool in = has(r) && t0 + s < q.last;
-        theta[s][r] = in ? __ldg(p.theta + (t * p.D + d) * p.Kp + kp(r)) : 0.f;
-        if (MODE != kAngles) bv[s][r] = in ? load_pair(static_cast<const IO*>(p.b) + (t * p.G + g) * p.N + 2 * kp(r)) : make_float2(0.f, 0.f);
-        if (MODE == kOut) cv[s][r] = in ? load_pair(static_cast<const IO*>(p.c) + (t * p.G + g) * p.N + 2 * kp(r)) : make_float2(0.f, 0.f);
+        if (!has[r]) continue;
+        const char *th_r = th + r * LPC * sizeof(float), *b_r = b + 2 * r * LPC * sizeof(IO), *c_r = c + 2 * r * LPC * sizeof(IO);
+#pragma unroll
+        for (int s = 0; s < kC; ++s, th_r += theta_bytes, b_r += bc_bytes, c_r += bc_bytes) {
+          copy_ahead<4>(&to.theta[s][r][threadIdx.x], th_r);
+          copy_ahead<2 * sizeof(IO)>(&to.b[s][r][threadIdx.x], b_r);
+          if (MODE == kOut) copy_ahead<2 * sizeof(IO)>(&to.c[s][r][threadIdx.x], c_r);
+        }
       }
-    float dts[OWN], gxs[OWN], exs[OWN], ys[kC];
+    } else {
+#pragma unroll 1
+      for (int s = 0; s < kC; ++s)
+#pragma unroll 1
+        for (int r = 0; r < PR; ++r) {
+          const bool in = sl + r * LPC < p.Kp && s < steps;
+          const IO *bs = reinterpret_cast<const IO*>(b + s * bc_bytes) + 2 * r * LPC, *cs = reinterpret_cast<const IO*>(c + s * bc_bytes) + 2 * r * LPC;
+          IO *db = reinterpret_cast<IO*>(&to.b[s][r][threadIdx.x]), *dc = reinterpret_cast<IO*>(&to.c[MODE == kOut ? s : 0][r][threadIdx.x]);
+          to.theta[s][r][threadIdx.x] = in ? reinterpret_cast<const float*>(th + s * theta_bytes)[r * LPC] : 0.f;
+          for (int k = 0; k < 2; ++k) {
+            db[k] = in ? bs[k] : from_f32<IO>(0.f);
+            if (MODE == kOut) dc[k] = in ? cs[k] : from_f32<IO>(0.f);
+          }
+        }
+    }
+    theta_at += kC * theta_row;
+    b_at += kC * bc_row;
+    c_at += kC * bc_row;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if (!has[PR - 1]) {  // (a lane without a pair reads zeros)
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll 1
+      for (int s = 0; s < kC; ++s)
+        for (int r = 0; r < PR; ++r) {
+          ahead[k].theta[s][r][threadIdx.x] = 0.f;
+          ahead[k].b[s][r][threadIdx.x] = {};
+          if (MODE == kOut) ahead[k].c[s][r][threadIdx.x] = {};
+        }
+  }
+  // dt, lambda, x of this lane's steps of a block: as read, and what is made of them
+  struct Raw { float dt[OWN], lam[OWN], x[OWN]; } next;
+  struct Made { float dt[OWN], gamma[OWN], look[OWN], x[OWN]; } own;
+  auto request_scalars = [&](int t0) {
 #pragma unroll
     for (int o = 0; o < OWN; ++o) {
-      const int s = sl + o * LPC;
-      const bool in = s < kC && t0 + s < q.last;
-      const size_t at = (size_t)(in ? t0 + s : q.first) * p.D + d;
-      dts[o] = in ? m3_softplus(p.dt[at]) : 0.f;
-      gxs[o] = exs[o] = 0.f;
-      if (MODE != kAngles && in) {
-        const float x = to_f32(static_cast<const IO*>(p.x)[at]), gamma = m3_sigmoid(p.lam[at]) * dts[o];
-        gxs[o] = gamma * x;
-        exs[o] = (gamma + serve_look(p, at + p.D, t0 + s + 1 < q.end)) * x;
-      }
+      const int t = t0 + sl + o * LPC;
+      const bool in = sl + o * LPC < kC && t < q.end;  // (the step behind the segment's last counts, for its weight of that one)
+      const size_t at = (size_t)(in ? t : q.first) * p.D + d;
+      next.dt[o] = in ? p.dt[at] : -INFINITY;
+      next.lam[o] = in ? p.lam[at] : 0.f;
+      next.x[o] = in ? to_f32(static_cast<const IO*>(p.x)[at]) : 0.f;
     }
+  };
+  auto make_scalars = [&](int t0) {
+    Made m;
 #pragma unroll
-    for (int s = 0; s < kC; ++s) {
-      const float dt = __shfl_sync(0xffffffffu, dts[s / LPC], base + s % LPC);
-      const float gx = MODE == kOut ? __shfl_sync(0xffffffffu, gxs[s / LPC], base + s % LPC) : 0.f;
-      const float ex = MODE != kAngles ? __shfl_sync(0xffffffffu, exs[s / LPC], base + s % LPC) : 0.f;
-      dsum += dt;
-      float acc = 0.f;
+    for (int o = 0; o < OWN; ++o) {
+      const float dt = m3_softplus(next.dt[o]), lam = m3_sigmoid(next.lam[o]);
+      const bool in = t0 + sl + o * LPC < q.last;
+      m.look[o] = (1.f - lam) * dt;
+      m.dt[o] = in ? dt : 0.f;
+      m.gamma[o] = in ? lam * dt : 0.f;
+      m.x[o] = in ? next.x[o] : 0.f;
+    }
+    return m;
+  };
+  request(q.first, ahead[0]);
+  request_scalars(q.first);
+  own = make_scalars(q.first);
+  request_scalars(q.first + kC);
+  int buf = 0;
+  for (int t0 = q.first; t0 < q.last; t0 += kC, buf ^= 1) {
+    const int steps = min(kC, q.last - t0);
+    if (t0 + kC < q.last) {
+      request(t0 + kC, ahead[buf ^ 1]);
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+    } else {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+    }
+    const Made behind = make_scalars(t0 + kC);
+    if (t0 + kC < q.last) request_scalars(t0 + 2 * kC);
+    float dts[OWN], gxs[OWN], exs[OWN], ys[kC];
+#pragma unroll
+    for (int o = 0; o < OWN; ++o) {  // e: lambda dt and what the step behind gives this one
+      const float a = __shfl_sync(0xffffffffu, own.look[o], base + (sl + 1) % LPC);
+      const float b = o + 1 < OWN ? __shfl_sync(0xffffffffu, own.look[o + 1 < OWN ? o + 1 : 0], base) : __shfl_sync(0xffffffffu, behind.look[0], base);
+      dts[o] = own.dt[o];
+      gxs[o] = own.gamma[o] * own.x[o];
+      exs[o] = (own.gamma[o] + (sl + 1 < (LPC < kC ? LPC : kC) ? a : b)) * own.x[o];
+    }
+    own = behind;
+    const Block& now = ahead[buf];
+#pragma unroll
+    for (int s = 0; s < kC; s += 2) {  // two steps' angles together
+      float dt[2], gx[2], ex[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        dt[k] = __shfl_sync(0xffffffffu, dts[(s + k) / LPC], base + (s + k) % LPC);
+        gx[k] = MODE == kOut ? __shfl_sync(0xffffffffu, gxs[(s + k) / LPC], base + (s + k) % LPC) : 0.f;
+        ex[k] = __shfl_sync(0xffffffffu, exs[(s + k) / LPC], base + (s + k) % LPC);
+        dsum += dt[k];
+      }
+      float acc[2] = {0.f, 0.f};
 #pragma unroll
       for (int r = 0; r < PR; ++r) {
-        turn[r] += m3_turn(dt, theta[s][r]);
-        taint[r] = m3_taint(dt * theta[s][r], taint[r]);
-        if (MODE == kAngles) continue;
-        const float2 unit = m3_unit(turn[r], taint[r]);
-        const float2 u = m3_back(bv[s][r], unit);
-        const float v0 = expf(a[r][0] * dt) * G[r][0], v1 = expf(a[r][1] * dt) * G[r][1];
-        if (MODE == kOut) {
-          const float2 c = m3_back(cv[s][r], unit);
-          acc = fmaf(fmaf(gx, u.x, v0), c.x, fmaf(fmaf(gx, u.y, v1), c.y, acc));
+        const float p0 = dt[0] * now.theta[s][r][threadIdx.x], p1 = dt[1] * now.theta[s + 1][r][threadIdx.x];
+        const int t1 = turn[r] + turn_of(p0), t2 = t1 + turn_of(p1);
+        const float n1 = m3_taint(p0, taint[r]), n2 = m3_taint(p1, n1);
+        float2 unit[2];
+        unit2(t1, t2, unit[0], unit[1]);
+        acc[0] += n1;  // (an angle that is not finite: y by hand, the state at the block's end)
+        acc[1] += n2;
+        turn[r] = t2;
+        taint[r] = n2;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float2 b = pair_of(now.b[s + k][r][threadIdx.x]);
+          const f2 v = mul2(pack2(ex2(a[r][0] * dt[k]), ex2(a[r][1] * dt[k])), G[r]), e2 = dup2(ex[k]);
+          if (MODE == kOut) {
+            const float2 u2 = m3_back(b, unit[k]), c = m3_back(pair_of(now.c[MODE == kOut ? s + k : 0][r][threadIdx.x]), unit[k]);
+            const f2 u = pack2(u2.x, u2.y);
+            acc[k] += sum2(mul2(mad2(dup2(gx[k]), u, v), pack2(c.x, c.y)));
+            G[r] = mad2(e2, u, v);
+          } else {
+            const float2 u = m3_back(b, unit[k]);
+            const int h = MODE == kEnds ? r : 0;
+            const f2 w = mul2(pack2(ex2(a[r][0] * dt[k]), ex2(a[r][1] * dt[k])), H[h]);
+            G[r] = mad2(e2, pack2(u.x, u.y), v);
+            H[h] = mad2(e2, pack2(u.y, -u.x), w);
+          }
         }
-        G[r][0] = fmaf(ex, u.x, v0);
-        G[r][1] = fmaf(ex, u.y, v1);
       }
-      ys[s] = acc;
+      ys[s] = acc[0];
+      ys[s + 1] = acc[1];
     }
+#pragma unroll
+    for (int r = 0; r < PR; ++r) G[r] = add2(G[r], dup2(taint[r]));
     if (MODE == kOut) {
+      if (LPC >= 8) {  // lane sl gets the sum of step sl & 7
+        colsum8_step<4, 4>(ys, lane);
+        colsum8_step<2, 2>(ys, lane);
+        colsum8_step<1, 1>(ys, lane);
 #pragma unroll
-      for (int s = 0; s < kC; ++s) {
+        for (int o = 8; o < LPC; o <<= 1) ys[0] += __shfl_xor_sync(0xffffffffu, ys[0], o);
+        if (live && sl < steps && sl < kC) static_cast<IO*>(p.y)[(size_t)(t0 + sl) * p.D + d] = from_f32<IO>(ys[0]);
+      } else {
 #pragma unroll
-        for (int o = LPC / 2; o > 0; o >>= 1) ys[s] += __shfl_xor_sync(0xffffffffu, ys[s], o);
-        if (live && sl == s % LPC && t0 + s < q.last) static_cast<IO*>(p.y)[(size_t)(t0 + s) * p.D + d] = from_f32<IO>(ys[s]);
+        for (int s = 0; s < kC; ++s) {
+#pragma unroll
+          for (int o = LPC / 2; o > 0; o >>= 1) ys[s] += __shfl_xor_sync(0xffffffffu, ys[s], o);
+          if (live && sl == s % LPC && s < steps) static_cast<IO*>(p.y)[(size_t)(t0 + s) * p.D + d] = from_f32<IO>(ys[s]);
+        }
       }
     }
   }
   if (!live) return;
-  if (MODE == kAngles) {
-    const size_t row = (size_t)blockIdx.x * p.D + d;
-    if (sl == 0) p.dsum[row] = dsum;
-#pragma unroll
-    for (int r = 0; r < PR; ++r)
-      if (has(r)) {
-        p.turn[row * p.Kp + kp(r)] = turn[r];
-        p.spoil[row * p.Kp + kp(r)] = taint[r];
-      }
-    return;
-  }
+  if (MODE == kEnds && sl == 0) p.dsum[row] = dsum;
   if (MODE == kOut && (q.seg != q.segs - 1 || slot < 0)) return;
 #pragma unroll
   for (int r = 0; r < PR; ++r) {
-    if (!has(r)) continue;
-    const float2 v = make_float2(G[r][0], G[r][1]);
+    if (!has[r]) continue;
+    const float2 v = unpack2(G[r]);
     if (MODE == kEnds) {
-      reinterpret_cast<float2*>(p.ends)[((size_t)blockIdx.x * p.D + d) * p.Kp + kp(r)] = v;
+      const size_t at = row * p.Kp + kp[r];
+      reinterpret_cast<float2*>(p.ends)[at] = v;
+      reinterpret_cast<float2*>(p.ends2)[at] = unpack2(H[MODE == kEnds ? r : 0]);
+      p.turn[at] = turn[r];
+      p.spoil[at] = taint[r];
     } else {
-      reinterpret_cast<float2*>(p.h)[sd * p.Kp + kp(r)] = v;
-      p.phase[sd * p.Kp + kp(r)] = m3_unit(turn[r], taint[r]);
+      reinterpret_cast<float2*>(p.h)[sd * p.Kp + kp[r]] = v;
+      p.phase[sd * p.Kp + kp[r]] = m3_unit(turn[r], taint[r]);
     }
   }
 }
-// What the segments of a sequence start from, as m3k_heads_chain_kernel.
+// What the segments of a sequence start from, as m3k_heads_chain_kernel: the state and the angle.
 __global__ void __launch_bounds__(256) m3k_channels_chain_kernel(ServeP p, bool bf16_io) {
   begin_dependent();
-  const Piece q = find_piece(p, blockIdx.x, p.L);
-  if (!q.ok || q.seg != 0 || q.segs == 1 || q.base + q.segs > p.pieces) return;  // (more segments: lengths beyond the rows)
+  const Piece q = find_piece<true>(p, blockIdx.x, p.L);
+  if (!q.ok || q.segs == 1 || q.base + q.segs > p.pieces) return;  // (more segments: lengths beyond the rows)
   const int slot = serve_slot(p, q.seq);
   const bool go = slot >= 0 && serve_goes_on(p, q.seq);
   const size_t pairs = (size_t)p.D * p.Kp;
   for (size_t i = blockIdx.y * (size_t)256 + threadIdx.x; i < pairs; i += gridDim.y * (size_t)256) {
     const int d = (int)(i / p.Kp), k = (int)(i % p.Kp), g = d / (p.D / p.G);
     float2 v = make_float2(0.f, 0.f);
+    int angle = 0;
+    float taint = 0.f;
     if (go) {
       const size_t sd = (size_t)slot * p.D + d, br = ((size_t)slot * p.G + g) * p.N + 2 * k;
+      const float2 unit = p.phase[sd * p.Kp + k];
+      angle = serve_turn(unit);
+      taint = m3_taint(unit.x, m3_taint(unit.y, 0.f));
       v = reinterpret_cast<const float2*>(p.h)[sd * p.Kp + k];
       const float w = serve_look(p, (size_t)q.begin * p.D + d, true) * (bf16_io ? to_f32(static_cast<const bf16*>(p.x_prev)[sd]) : static_cast<const float*>(p.x_prev)[sd]);
-      const float2 b = m3_back(bf16_io ? load_pair(static_cast<const bf16*>(p.b_prev) + br) : load_pair(static_cast<const float*>(p.b_prev) + br),
-                               p.phase[sd * p.Kp + k]);
+      const float2 b = m3_back(bf16_io ? load_pair(static_cast<const bf16*>(p.b_prev) + br) : load_pair(static_cast<const float*>(p.b_prev) + br), unit);
       v.x = fmaf(w, b.x, v.x);
       v.y = fmaf(w, b.y, v.y);
     }
     const float a0 = -expf(p.a_log[(size_t)d * p.N + 2 * k]), a1 = -expf(p.a_log[(size_t)d * p.N + 2 * k + 1]);
-    float2* e = reinterpret_cast<float2*>(p.ends) + ((size_t)q.base * p.D + d) * p.Kp + k;
+    size_t at = (size_t)q.base * pairs + i;
     for (int s0 = 0; s0 < q.segs; s0 += kAhead) {
       const int n = min(kAhead, q.segs - s0), adds = min(kAhead, q.segs - 1 - s0);
-      float2 add[kAhead];
-      float sum[kAhead];
+      float2 c[kAhead], s[kAhead];
+      float sum[kAhead], spoil[kAhead];
+      int turn[kAhead];
 #pragma unroll
-      for (int s = 0; s < kAhead; ++s) {
-        add[s] = s < adds ? e[s * pairs] : make_float2(0.f, 0.f);
-        sum[s] = s < adds ? p.dsum[(size_t)(q.base + s0 + s) * p.D + d] : 0.f;
+      for (int j = 0; j < kAhead; ++j) {
+        const bool in = j < adds;
+        c[j] = in ? reinterpret_cast<const float2*>(p.ends)[at + j * pairs] : make_float2(0.f, 0.f);
+        s[j] = in ? reinterpret_cast<const float2*>(p.ends2)[at + j * pairs] : make_float2(0.f, 0.f);
+        sum[j] = in ? p.dsum[(size_t)(q.base + s0 + j) * p.D + d] : 0.f;
+        turn[j] = in ? p.turn[at + j * pairs] : 0;
+        spoil[j] = in ? p.spoil[at + j * pairs] : 0.f;
       }
 #pragma unroll
-      for (int s = 0; s < kAhead; ++s) {
-        if (s >= n) break;
-        e[s * pairs] = v;
-        v.x = fmaf(expf(a0 * sum[s]), v.x, add[s].x);
-        v.y = fmaf(expf(a1 * sum[s]), v.y, add[s].y);
+      for (int j = 0; j < kAhead; ++j) {
+        if (j >= n) break;
+        reinterpret_cast<float2*>(p.ends)[at + j * pairs] = v;
+        p.turn[at + j * pairs] = angle;
+        p.spoil[at + j * pairs] = taint;
+        const float2 unit = m3_unit(angle, taint);
+        v.x = fmaf(expf(a0 * sum[j]), v.x, fmaf(unit.x, c[j].x, unit.y * s[j].x));
+        v.y = fmaf(expf(a1 * sum[j]), v.y, fmaf(unit.x, c[j].y, unit.y * s[j].y));
+        angle += turn[j];
+        taint += spoil[j];
       }
-      e += kAhead * pairs;
+      at += kAhead * pairs;
     }
   }
 }
@@ -523,29 +690,35 @@ static void heads(const ServeP& p, cudaStream_t st) {
   else by_r(std::integral_constant<int, 2>{});
 }
 template <typename IO, Mode MODE>
-static void channels(const ServeP& p, cudaStream_t st) {
+static mxb_status channels(const ServeP& p, cudaStream_t st) {
   const ChannelShape s = channel_shape(p);
   const dim3 grid(p.pieces, (p.D + 128 / s.LPC - 1) / (128 / s.LPC));
-  auto launch = [&](auto kernel) {
-    MXB_LAUNCH(MODE == kOut ? "m3k_channels_kernel" : MODE == kEnds ? "m3k_channels_ends_kernel" : "m3k_channels_angles_kernel", st,
-               (launch_kernel(kernel, grid, 128, 0, st, p)));
+  mxb_status status = MXB_OK;
+  auto launch = [&](auto pr, auto lpc) {
+    constexpr int PR = decltype(pr)::value, LPC = decltype(lpc)::value;
+    constexpr int smem = 2 * (int)sizeof(Ahead<IO, PR, MODE>);
+    status = MXB_ALLOW_SMEM(smem, m3k_channels_kernel<IO, PR, LPC, MODE>);
+    if (status != MXB_OK) return;
+    MXB_LAUNCH(MODE == kOut ? "m3k_channels_kernel" : "m3k_channels_ends_kernel", st,
+               (launch_kernel(m3k_channels_kernel<IO, PR, LPC, MODE>, grid, 128, smem, st, p)));
   };
+  constexpr std::integral_constant<int, 1> one;
   switch (s.LPC * s.PR) {
-    case 1: launch(m3k_channels_kernel<IO, 1, 1, MODE>); break;
-    case 2: launch(m3k_channels_kernel<IO, 1, 2, MODE>); break;
-    case 4: launch(m3k_channels_kernel<IO, 1, 4, MODE>); break;
-    case 8: launch(m3k_channels_kernel<IO, 1, 8, MODE>); break;
-    case 16: launch(m3k_channels_kernel<IO, 1, 16, MODE>); break;
-    case 32: launch(m3k_channels_kernel<IO, 1, 32, MODE>); break;
-    case 64: launch(m3k_channels_kernel<IO, 2, 32, MODE>); break;
-    default: launch(m3k_channels_kernel<IO, 4, 32, MODE>); break;
+    case 1: launch(one, one); break;
+    case 2: launch(one, std::integral_constant<int, 2>{}); break;
+    case 4: launch(one, std::integral_constant<int, 4>{}); break;
+    case 8: launch(one, std::integral_constant<int, 8>{}); break;
+    case 16: launch(one, std::integral_constant<int, 16>{}); break;
+    case 32: launch(one, std::integral_constant<int, 32>{}); break;
+    case 64: launch(std::integral_constant<int, 2>{}, std::integral_constant<int, 32>{}); break;
+    default: launch(std::integral_constant<int, 4>{}, std::integral_constant<int, 32>{}); break;
   }
+  return status;
 }
 template <typename IO>
 static mxb_status prefill(ServeP p, bool chunks, cudaStream_t st) {
-  // (a piece that is not a sequence's first has nothing to do: few blocks each where there are many)
-  const size_t blocks = ((size_t)p.D * p.Kp + 255) / 256;
-  const dim3 chain(p.pieces, (unsigned)std::min<size_t>(blocks, std::max<size_t>(148 * 32 / p.pieces, 1)));
+  const size_t blocks = ((size_t)p.D * p.Kp + 255) / 256;  // (most of many sequences are not cut: few blocks each)
+  const dim3 chain(p.S, (unsigned)std::min<size_t>(blocks, std::max<size_t>(148 * 4 / p.S, 1)));
   const bool cut = p.ends != nullptr;
   if (p.NH) {
     p.slabs = chunks ? serve_slabs(p) : head_shape(p).slabs;
@@ -562,11 +735,10 @@ static mxb_status prefill(ServeP p, bool chunks, cudaStream_t st) {
     MXB_LAUNCH("m3k_heads_phase_kernel", st, (launch_kernel(m3k_heads_phase_kernel, dim3(p.S, p.NH), 256, 0, st, p)));
   } else {
     if (cut) {
-      channels<IO, kAngles>(p, st);
-      channels<IO, kEnds>(p, st);
+      if (const mxb_status s = channels<IO, kEnds>(p, st); s != MXB_OK) return s;
       MXB_LAUNCH("m3k_channels_chain_kernel", st, (launch_kernel(m3k_channels_chain_kernel, chain, 256, 0, st, p, sizeof(IO) == 2)));
     }
-    channels<IO, kOut>(p, st);
+    if (const mxb_status s = channels<IO, kOut>(p, st); s != MXB_OK) return s;
   }
   const mxb_status s = check_launch("m3k_prefill");
   return s == MXB_OK ? m3serve_tails(p, sizeof(IO) == 4, true, st) : s;
@@ -582,7 +754,7 @@ static int walk_segment(const ServeP& p) {
     const int per = 128 / m3k::channel_shape(p).LPC;
     return (long long)((p.D + per - 1) / per);
   }();
-  const long long at_once = p.NH ? 148 * 2 : 148 * 8;
+  const long long at_once = p.NH ? 148 * 2 : 148 * 16;
   long long L = (p.rows * ctas + at_once - 1) / at_once;
   if (p.S > 1) L += L / 4;
   return (int)std::min<long long>(std::max<long long>(64, (L + 63) / 64 * 64), INT32_MAX);
@@ -603,7 +775,10 @@ size_t m3walk_scratch(ServeP& p, bool f32, int flags, char* base) {
   p.dsum = c.take<float>((size_t)p.pieces * (p.NH ? p.NH : p.D));
   p.turn = c.take<int>((size_t)p.pieces * (p.NH ? p.NH : (size_t)p.D * p.Kp));
   if (p.NH) p.start = c.take<float2>((size_t)p.pieces * p.NH);
-  else p.spoil = c.take<float>((size_t)p.pieces * p.D * p.Kp);
+  else {
+    p.ends2 = c.take<float>((size_t)p.pieces * p.D * p.N);
+    p.spoil = c.take<float>((size_t)p.pieces * p.D * p.Kp);
+  }
   return c.bytes();
 }
 // The chunks on the tensor cores where they cover the call, the walks elsewhere.

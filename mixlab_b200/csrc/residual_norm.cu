@@ -4,7 +4,8 @@
 //     d  = dr' + k (t - r' k^2 mean(t r'))          the gradient of r' from both its readers; dr = d
 //     s  = d scale post_norm SiLU(z)
 //     dy = j (s - y j^2 mean(s y)), j = 1 / rms(y)  (s itself without post_norm)
-//     dz = d scale post_norm y j SiLU'(z),  dnorm = sum dn r' k,  dpost_norm = sum d scale y j SiLU(z),  dscale = sum d a
+//     dz = d scale post_norm y j SiLU'(z),  dnorm = sum dn r' k,  dpost_norm = scale A,  dscale = post_norm A,
+//     A = sum d y j SiLU(z) over the rows
 //
 // HBM streams.  A row is read once, held by TPR threads in 8 (beyond 8192 columns 16) registers a tensor, and its sums go
 // through the lanes and, for TPR > 32, shared memory; narrow rows share a CTA.  Column sums of the gradients: every group of
@@ -14,6 +15,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "packed.cuh"
 
 namespace mxb {
 namespace rnorm {
@@ -29,55 +31,93 @@ struct NormP {
   void *resid_out, *n;
   const void *d_resid, *dn;           // d_resid may be null
   void *dr, *dy, *dz;
-  float* part;                        // [groups][3][D]
+  float* part;                        // [groups][2][D]: dnorm, A
 };
 
-// 8 consecutive columns from c0, those below D: V says that whole pieces may be read.
+// 8 consecutive columns from c0, those below D, as four packed pairs.  V says that whole pieces may be read.
+__device__ __forceinline__ void unpack8(const uint4& v, f2 (&e)[4]) {  // eight bf16
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) e[i] = pack2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+}
 template <typename T, bool V>
-__device__ __forceinline__ void load8(const T* row, int c0, int D, float (&e)[8]) {
+__device__ __forceinline__ void load8(const T* row, int c0, int D, f2 (&e)[4]) {
   if constexpr (V) {
     if (c0 < D) {
       if constexpr (sizeof(T) == 4) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const float4 a = *reinterpret_cast<const float4*>(row + c0 + 4 * i);
-          e[4 * i] = a.x; e[4 * i + 1] = a.y; e[4 * i + 2] = a.z; e[4 * i + 3] = a.w;
+          e[2 * i] = pack2(a.x, a.y);
+          e[2 * i + 1] = pack2(a.z, a.w);
         }
       } else {
-        const uint4 v = *reinterpret_cast<const uint4*>(row + c0);
-        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { e[2 * i] = __low2float(h[i]); e[2 * i + 1] = __high2float(h[i]); }
+        unpack8(*reinterpret_cast<const uint4*>(row + c0), e);
       }
       return;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = 0.f;
+    for (int i = 0; i < 4; ++i) e[i] = 0;
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = c0 + i < D ? to_f32(row[c0 + i]) : 0.f;
+    for (int i = 0; i < 4; ++i) {
+      const int c = c0 + 2 * i;
+      e[i] = pack2(c < D ? to_f32(row[c]) : 0.f, c + 1 < D ? to_f32(row[c + 1]) : 0.f);
+    }
   }
 }
 template <typename T, bool V>
-__device__ __forceinline__ void store8(T* row, int c0, int D, const float (&e)[8]) {
+__device__ __forceinline__ void store8(T* row, int c0, int D, const f2 (&e)[4]) {
   if constexpr (V) {
     if (c0 >= D) return;
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) *reinterpret_cast<float4*>(row + c0 + 4 * i) = make_float4(e[4 * i], e[4 * i + 1], e[4 * i + 2], e[4 * i + 3]);
+      for (int i = 0; i < 2; ++i) {
+        const float2 a = unpack2(e[2 * i]), b = unpack2(e[2 * i + 1]);
+        *reinterpret_cast<float4*>(row + c0 + 4 * i) = make_float4(a.x, a.y, b.x, b.y);
+      }
     } else {
       uint4 v;
       __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&v);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(e[2 * i], e[2 * i + 1]);
+      for (int i = 0; i < 4; ++i) { const float2 a = unpack2(e[i]); h[i] = __floats2bfloat162_rn(a.x, a.y); }
       *reinterpret_cast<uint4*>(row + c0) = v;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (c0 + i < D) row[c0 + i] = from_f32<T>(e[i]);
+    for (int i = 0; i < 4; ++i) {
+      const float2 a = unpack2(e[i]);
+      const int c = c0 + 2 * i;
+      if (c < D) row[c] = from_f32<T>(a.x);
+      if (c + 1 < D) row[c + 1] = from_f32<T>(a.y);
+    }
   }
 }
+// A piece of a row as it is in memory, requested ahead of its use (whole pieces only; else read when it is used).
+template <typename T, bool V>
+struct Ahead {
+  static constexpr int W = sizeof(T) == 4 ? 2 : 1;
+  uint4 raw[V ? W : 1];
+  __device__ __forceinline__ void load(const T* row, int c0, int D) {
+    if constexpr (V) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) raw[i] = c0 < D ? reinterpret_cast<const uint4*>(row + c0)[i] : make_uint4(0, 0, 0, 0);
+    }
+  }
+  __device__ __forceinline__ void get(const T* row, int c0, int D, f2 (&e)[4]) const {
+    if constexpr (!V) {
+      load8<T, false>(row, c0, D, e);
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        e[2 * i] = pack2(__uint_as_float(raw[i].x), __uint_as_float(raw[i].y));
+        e[2 * i + 1] = pack2(__uint_as_float(raw[i].z), __uint_as_float(raw[i].w));
+      }
+    } else {
+      unpack8(raw[0], e);
+    }
+  }
+};
 // Sums of M values over the TPR threads of a row; every thread gets them.  red: shared, M floats a warp.  All threads of the
 // CTA call it.
 template <int TPR, int M>
@@ -103,7 +143,18 @@ __device__ __forceinline__ void row_sum(float (&v)[M], float* red) {
     }
   }
 }
-__device__ __forceinline__ float sigmoid_of(float z) { return 1.f / (1.f + expf(-z)); }
+// (bf16 tensors: the hardware's exponential and division, good to a few 2^-22 where results keep 2^-9)
+template <typename IO>
+__device__ __forceinline__ float sigmoid_of(float z) { return sizeof(IO) == 4 ? 1.f / (1.f + expf(-z)) : __fdividef(1.f, 1.f + __expf(-z)); }
+
+// z -> SiLU(z) and, where wanted, its slope
+template <typename IO>
+__device__ __forceinline__ void gate_of(f2 z, f2& gate, f2& slope) {
+  const float2 v = unpack2(z);
+  const f2 sg = pack2(sigmoid_of<IO>(v.x), sigmoid_of<IO>(v.y));
+  gate = mul2(z, sg);
+  slope = mad2(gate, add2(dup2(1.f), sg ^ 0x8000000080000000ull), sg);
+}
 
 template <int TPR>
 constexpr int kThreads = TPR > 256 ? TPR : 256;
@@ -115,205 +166,233 @@ __global__ void __launch_bounds__(kThreads<TPR>) rnorm_fwd_kernel(NormP p) {
   constexpr int GROUPS = kThreads<TPR> / TPR;
   const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
   const float inv = 1.f / (float)p.D;
+  // the next row of each tensor is under way while one is worked on
+  Ahead<RES, V> a_r[E];
+  Ahead<IO, V> a_y[E], a_z[E];
+  auto offset = [&](size_t r0) { return (r0 + group < p.rows ? r0 + group : r0) * p.D; };
+  auto request = [&](size_t r0) {
+    const size_t off = offset(r0);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int c = (lane + e * TPR) * 8;
+      a_y[e].load(static_cast<const IO*>(p.y) + off, c, p.D);
+      a_r[e].load(static_cast<const RES*>(p.resid) + off, c, p.D);
+      if (p.z) a_z[e].load(static_cast<const IO*>(p.z) + off, c, p.D);
+    }
+  };
+  request((size_t)blockIdx.x * GROUPS);
   for (size_t r0 = (size_t)blockIdx.x * GROUPS; r0 < p.rows; r0 += (size_t)gridDim.x * GROUPS) {
     const bool live = r0 + group < p.rows;
-    const size_t off = (live ? r0 + group : r0) * p.D;
-    float r[E][8], a[E][8];
+    const size_t off = offset(r0);
+    f2 r[E][4], a[E][4];
+    f2 sum = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int c = (lane + e * TPR) * 8;
-      load8<IO, V>(static_cast<const IO*>(p.y) + off, c, p.D, a[e]);
-      load8<RES, V>(static_cast<const RES*>(p.resid) + off, c, p.D, r[e]);
-    }
-    if (p.z) {
-      float s[1] = {0.f};
-      float zs[E][8];
+      a_y[e].get(static_cast<const IO*>(p.y) + off, c, p.D, a[e]);
+      a_r[e].get(static_cast<const RES*>(p.resid) + off, c, p.D, r[e]);
 #pragma unroll
-      for (int e = 0; e < E; ++e) load8<IO, V>(static_cast<const IO*>(p.z) + off, (lane + e * TPR) * 8, p.D, zs[e]);
+      for (int i = 0; i < 4; ++i) fma2(sum, a[e][i], a[e][i]);
+      if (p.z) {
+        f2 z[4], gate, slope;
+        a_z[e].get(static_cast<const IO*>(p.z) + off, c, p.D, z);
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          s[0] = fmaf(a[e][i], a[e][i], s[0]);
-          a[e][i] *= zs[e][i] * sigmoid_of(zs[e][i]);
+        for (int i = 0; i < 4; ++i) {
+          gate_of<IO>(z[i], gate, slope);
+          a[e][i] = mul2(a[e][i], gate);
         }
-      if (p.post) {
-        row_sum<TPR>(s, red);
-        const float j = rsqrtf(s[0] * inv + p.eps);
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) a[e][i] *= j;
       }
-    } else if (p.post) {
-      float s[1] = {0.f};
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s[0] = fmaf(a[e][i], a[e][i], s[0]);
-      row_sum<TPR>(s, red);
-      const float j = rsqrtf(s[0] * inv + p.eps);
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) a[e][i] *= j;
     }
-    float s[1] = {0.f};
+    if (r0 + (size_t)gridDim.x * GROUPS < p.rows) request(r0 + (size_t)gridDim.x * GROUPS);
+    float s[1], j = 1.f;
+    if (p.post) {
+      s[0] = sum2(sum);
+      row_sum<TPR>(s, red);
+      j = rsqrtf(s[0] * inv + p.eps);
+    }
+    sum = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int c = (lane + e * TPR) * 8;
-      float w[8];
+      f2 w[4];
       if (p.post) {
         load8<float, V>(p.post, c, p.D, w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) a[e][i] *= w[i];
+        for (int i = 0; i < 4; ++i) a[e][i] = mul2(mul2(a[e][i], dup2(j)), w[i]);
       }
       if (p.scale) {
         load8<float, V>(p.scale, c, p.D, w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) a[e][i] *= w[i];
+        for (int i = 0; i < 4; ++i) a[e][i] = mul2(a[e][i], w[i]);
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        r[e][i] += a[e][i];
-        s[0] = fmaf(r[e][i], r[e][i], s[0]);
+      for (int i = 0; i < 4; ++i) {
+        r[e][i] = add2(r[e][i], a[e][i]);
+        fma2(sum, r[e][i], r[e][i]);
       }
       if (live) store8<RES, V>(static_cast<RES*>(p.resid_out) + off, c, p.D, r[e]);
     }
+    s[0] = sum2(sum);
     row_sum<TPR>(s, red);
     const float k = rsqrtf(s[0] * inv + p.eps);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int c = (lane + e * TPR) * 8;
-      float w[8];
+      f2 w[4];
       load8<float, V>(p.norm, c, p.D, w);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] *= r[e][i] * k;
+      for (int i = 0; i < 4; ++i) w[i] = mul2(w[i], mul2(r[e][i], dup2(k)));
       if (live) store8<IO, V>(static_cast<IO*>(p.n) + off, c, p.D, w);
     }
   }
 }
 
 template <typename IO, typename RES, int TPR, int E, bool V>
-__global__ void __launch_bounds__(kThreads<TPR>) rnorm_bwd_kernel(NormP p) {
+__global__ void __launch_bounds__(kThreads<TPR>, TPR > 256 ? 1 : 2) rnorm_bwd_kernel(NormP p) {
   begin_dependent();
   __shared__ float red[kThreads<TPR> / 32 * 3];
   constexpr int GROUPS = kThreads<TPR> / TPR;
   const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
   const float inv = 1.f / (float)p.D;
-  float dnorm[E][8], dpost[E][8], dscale[E][8];
+  f2 dnorm[E][4], both[E][4];
 #pragma unroll
   for (int e = 0; e < E; ++e)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) dnorm[e][i] = dpost[e][i] = dscale[e][i] = 0.f;
+    for (int i = 0; i < 4; ++i) dnorm[e][i] = both[e][i] = 0;
+  // the next row of each tensor is under way while one is worked on
+  Ahead<RES, V> a_r[E], a_d[E];
+  Ahead<IO, V> a_g[E], a_y[E], a_z[E];
+  auto offset = [&](size_t r0) { return (r0 + group < p.rows ? r0 + group : r0) * p.D; };
+  auto request = [&](size_t r0) {
+    const size_t off = offset(r0);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int c = (lane + e * TPR) * 8;
+      a_r[e].load(static_cast<const RES*>(p.resid) + off, c, p.D);
+      a_g[e].load(static_cast<const IO*>(p.dn) + off, c, p.D);
+      a_y[e].load(static_cast<const IO*>(p.y) + off, c, p.D);
+      if (p.d_resid) a_d[e].load(static_cast<const RES*>(p.d_resid) + off, c, p.D);
+      if (p.z) a_z[e].load(static_cast<const IO*>(p.z) + off, c, p.D);
+    }
+  };
+  request((size_t)blockIdx.x * GROUPS);
   for (size_t r0 = (size_t)blockIdx.x * GROUPS; r0 < p.rows; r0 += (size_t)gridDim.x * GROUPS) {
     const bool live = r0 + group < p.rows;
-    const size_t off = (live ? r0 + group : r0) * p.D;
-    float r[E][8], y[E][8], g[E][8], d[E][8], s[3] = {0.f, 0.f, 0.f};
+    const size_t off = offset(r0);
+    f2 r[E][4], y[E][4], g[E][4], d[E][4], z[E][4], s0 = 0, s1 = 0, s2 = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int c = (lane + e * TPR) * 8;
-      load8<RES, V>(static_cast<const RES*>(p.resid) + off, c, p.D, r[e]);
-      load8<IO, V>(static_cast<const IO*>(p.dn) + off, c, p.D, g[e]);
-      load8<IO, V>(static_cast<const IO*>(p.y) + off, c, p.D, y[e]);
+      a_r[e].get(static_cast<const RES*>(p.resid) + off, c, p.D, r[e]);
+      a_g[e].get(static_cast<const IO*>(p.dn) + off, c, p.D, g[e]);
+      a_y[e].get(static_cast<const IO*>(p.y) + off, c, p.D, y[e]);
       if (p.d_resid) {
-        load8<RES, V>(static_cast<const RES*>(p.d_resid) + off, c, p.D, d[e]);
+        a_d[e].get(static_cast<const RES*>(p.d_resid) + off, c, p.D, d[e]);
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) d[e][i] = 0.f;
+        for (int i = 0; i < 4; ++i) d[e][i] = 0;
       }
+      if (p.z) a_z[e].get(static_cast<const IO*>(p.z) + off, c, p.D, z[e]);
     }
+    if (r0 + (size_t)gridDim.x * GROUPS < p.rows) request(r0 + (size_t)gridDim.x * GROUPS);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      float w[8];
+      f2 w[4];
       load8<float, V>(p.norm, (lane + e * TPR) * 8, p.D, w);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        s[0] = fmaf(r[e][i], r[e][i], s[0]);
-        s[1] = fmaf(g[e][i] * w[i], r[e][i], s[1]);
-        s[2] = fmaf(y[e][i], y[e][i], s[2]);
+      for (int i = 0; i < 4; ++i) {
+        fma2(s0, r[e][i], r[e][i]);
+        fma2(s1, mul2(g[e][i], w[i]), r[e][i]);
+        fma2(s2, y[e][i], y[e][i]);
       }
     }
+    float s[3] = {sum2(s0), sum2(s1), sum2(s2)};
     row_sum<TPR>(s, red);
     const float k = rsqrtf(s[0] * inv + p.eps), k2 = k * k * s[1] * inv, j = p.post ? rsqrtf(s[2] * inv + p.eps) : 1.f;
-    float q[1] = {0.f};
+    const f2 kk = dup2(k), mk2 = dup2(-k2), jj = dup2(j);
+    f2 qs = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int c = (lane + e * TPR) * 8;
-      float w[8], z[8];
+      f2 w[4], f[4];
       load8<float, V>(p.norm, c, p.D, w);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (live) dnorm[e][i] = fmaf(g[e][i], r[e][i] * k, dnorm[e][i]);
-        d[e][i] = fmaf(k, fmaf(-r[e][i], k2, g[e][i] * w[i]), d[e][i]);
+      for (int i = 0; i < 4; ++i) {
+        if (live) fma2(dnorm[e][i], g[e][i], mul2(r[e][i], kk));
+        d[e][i] = mad2(kk, mad2(r[e][i], mk2, mul2(g[e][i], w[i])), d[e][i]);
       }
       if (live) store8<RES, V>(static_cast<RES*>(p.dr) + off, c, p.D, d[e]);
-      // g <- d scale post SiLU(z): what reaches y j, and on the way the sums over the rows and dz
+      if (p.post) {
+        load8<float, V>(p.post, c, p.D, f);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) g[e][i] = d[e][i];
-      float post[8], gate[8], slope[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) { post[i] = 1.f; gate[i] = 1.f; slope[i] = 0.f; }
-      if (p.post) load8<float, V>(p.post, c, p.D, post);
-      if (p.z) {
-        load8<IO, V>(static_cast<const IO*>(p.z) + off, c, p.D, z);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float sg = sigmoid_of(z[i]);
-          gate[i] = z[i] * sg;
-          slope[i] = fmaf(gate[i], 1.f - sg, sg);
-        }
+        for (int i = 0; i < 4; ++i) f[i] = dup2(1.f);
       }
       if (p.scale) {
         load8<float, V>(p.scale, c, p.D, w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (live) dscale[e][i] = fmaf(d[e][i], y[e][i] * j * post[i] * gate[i], dscale[e][i]);
-          g[e][i] *= w[i];
+        for (int i = 0; i < 4; ++i) f[i] = mul2(f[i], w[i]);
+      }
+      // g <- d scale post SiLU(z): what reaches y j; on the way A and dz
+      if (p.z) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          f2 gate, slope;
+          gate_of<IO>(z[e][i], gate, slope);
+          const f2 dy = mul2(mul2(d[e][i], y[e][i]), jj);
+          if (live) fma2(both[e][i], dy, gate);
+          z[e][i] = mul2(slope, mul2(dy, f[i]));
+          g[e][i] = mul2(mul2(d[e][i], f[i]), gate);
+          fma2(qs, g[e][i], y[e][i]);
+        }
+        if (live) store8<IO, V>(static_cast<IO*>(p.dz) + off, c, p.D, z[e]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (live) fma2(both[e][i], mul2(d[e][i], y[e][i]), jj);
+          g[e][i] = mul2(d[e][i], f[i]);
+          fma2(qs, g[e][i], y[e][i]);
         }
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float t = g[e][i] * y[e][i] * j;
-        if (live) dpost[e][i] = fmaf(t, gate[i], dpost[e][i]);
-        slope[i] *= t * post[i];
-        g[e][i] *= post[i] * gate[i];
-        q[0] = fmaf(g[e][i], y[e][i], q[0]);
-      }
-      if (p.z && live) store8<IO, V>(static_cast<IO*>(p.dz) + off, c, p.D, slope);
     }
+    float q[1] = {sum2(qs)};
     if (p.post) row_sum<TPR>(q, red);
-    const float j2 = p.post ? j * j * q[0] * inv : 0.f;
+    const f2 mj2 = dup2(p.post ? -j * j * q[0] * inv : 0.f);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) g[e][i] = j * fmaf(-y[e][i], j2, g[e][i]);
+      for (int i = 0; i < 4; ++i) g[e][i] = mul2(jj, mad2(y[e][i], mj2, g[e][i]));
       if (live) store8<IO, V>(static_cast<IO*>(p.dy) + off, (lane + e * TPR) * 8, p.D, g[e]);
     }
   }
-  float* part = p.part + ((size_t)blockIdx.x * GROUPS + group) * 3 * p.D;
+  float* part = p.part + ((size_t)blockIdx.x * GROUPS + group) * 2 * p.D;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int c = (lane + e * TPR) * 8;
     store8<float, false>(part, c, p.D, dnorm[e]);
-    if (p.post) store8<float, false>(part + p.D, c, p.D, dpost[e]);
-    if (p.scale) store8<float, false>(part + 2 * p.D, c, p.D, dscale[e]);
+    store8<float, false>(part + p.D, c, p.D, both[e]);
   }
 }
-// Sums of the partial rows.  grid (column blocks, 3): dnorm, dpost_norm, dscale; a null result is skipped.
+// Sums of the partial rows.  grid (column blocks, 1 or 2): dnorm; A, and from it dpost_norm and dscale.
 struct SumP {
   const float* part;
   int rows, D;
-  float* out[3];
+  float *dnorm, *dpost, *dscale;
+  const float *post, *scale;
 };
 template <bool TALL>
 __global__ void __launch_bounds__(kSumThreads<TALL>) rnorm_sum_kernel(SumP p) {
   begin_dependent();
-  float* out = p.out[blockIdx.y];
-  if (!out) return;
   const int c0 = blockIdx.x * kSumCols<TALL>, mine = c0 + threadIdx.x % kSumCols<TALL>;
-  col_sum<TALL>(p.part + blockIdx.y * (size_t)p.D + mine, p.rows, 3 * (size_t)p.D, mine < p.D, [&](int c, float t) {
-    if (c0 + c < p.D) out[c0 + c] = t;
+  col_sum<TALL>(p.part + blockIdx.y * (size_t)p.D + mine, p.rows, 2 * (size_t)p.D, mine < p.D, [&](int c, float t) {
+    c += c0;
+    if (c >= p.D) return;
+    if (blockIdx.y == 0) {
+      p.dnorm[c] = t;
+    } else {
+      if (p.dpost) p.dpost[c] = p.scale ? t * p.scale[c] : t;
+      if (p.dscale) p.dscale[c] = p.post ? t * p.post[c] : t;
+    }
   });
 }
 
@@ -324,10 +403,10 @@ static int threads_per_row(int D) {  // the smallest power of two with 8 columns
   return t;
 }
 static int groups_of(int tpr) { return tpr > 256 ? 1 : 256 / tpr; }
-// CTAs: the gradients' column sums want few of them, a few a SM; the forward pass has a CTA for every group of rows.
+// CTAs: what the GPU holds at once.
 static int ctas(size_t rows, int D, bool bwd) {
   const int tpr = threads_per_row(D), g = groups_of(tpr);
-  const size_t want = (rows + g - 1) / g, most = bwd ? 148 * (tpr > 256 ? 1 : 2) : 1u << 30;
+  const size_t want = (rows + g - 1) / g, most = std::max(148, 148 * (bwd ? 2 : 4) * 256 / std::max(tpr, 256));
   return (int)std::min(want, most);
 }
 template <typename F>
@@ -363,12 +442,13 @@ static mxb_status run(const NormP& p, float* const (&sums)[3], cudaStream_t st) 
     }
   });
   if (bwd) {
-    SumP s{p.part, parts, p.D, {sums[0], sums[1], sums[2]}};
+    const SumP s{p.part, parts, p.D, sums[0], sums[1], sums[2], p.post, p.scale};
+    const int kinds = sums[1] || sums[2] ? 2 : 1;
     auto launch = [&](auto tall) {
       constexpr bool T = decltype(tall)::value;
-      MXB_LAUNCH("rnorm_sum_kernel", st, (launch_kernel(rnorm_sum_kernel<T>, dim3((p.D + kSumCols<T> - 1) / kSumCols<T>, 3), kSumThreads<T>, 0, st, s)));
+      MXB_LAUNCH("rnorm_sum_kernel", st, (launch_kernel(rnorm_sum_kernel<T>, dim3((p.D + kSumCols<T> - 1) / kSumCols<T>, kinds), kSumThreads<T>, 0, st, s)));
     };
-    if (col_sum_tall(3 * (size_t)p.D)) launch(std::true_type{});
+    if (col_sum_tall(kinds * (size_t)p.D)) launch(std::true_type{});
     else launch(std::false_type{});
   }
   return check_launch(bwd ? "rnorm_bwd" : "rnorm_fwd");
@@ -391,7 +471,7 @@ static mxb_status by_type(const mxb_residual_norm_desc* d, const NormP& p, float
 
 size_t residual_norm_scratch(const mxb_residual_norm_desc* d) {
   const int tpr = rnorm::threads_per_row(d->D);
-  return (size_t)rnorm::ctas(d->rows, d->D, true) * rnorm::groups_of(tpr) * 3 * d->D * sizeof(float);
+  return (size_t)rnorm::ctas(d->rows, d->D, true) * rnorm::groups_of(tpr) * 2 * d->D * sizeof(float);
 }
 mxb_status residual_norm_fwd(const mxb_residual_norm_desc* d, const void* resid, const void* y, const float* norm, const float* post,
                              const void* z, const float* scale, void* resid_out, void* n, cudaStream_t st) {

@@ -4,9 +4,10 @@
 // first) where the sequence goes on, and is 0 where it starts; the pool then takes the sequence's own last K-1 inputs.
 //
 // An HBM stream in 16-byte pieces (single elements where D or a pointer does not allow them): a thread owns C channels and
-// walks down a run of rows with the last K-1 inputs in registers, eight rows requested at a time.  The first K-1 rows of a
+// walks down a run of rows with the last K-1 inputs in registers, four rows requested at a time.  The first K-1 rows of a
 // sequence all belong to the run of its first row, so that one thread alone reads and then writes a sequence's pool entry.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -14,7 +15,7 @@ namespace mxb {
 namespace sconv {
 
 using bf16 = __nv_bfloat16;
-constexpr int kThreads = 128, kAhead = 8;
+constexpr int kThreads = 128, kAhead = 4;
 
 struct ConvP {
   int rows, S, slots, D, K, silu, run, wvec;
@@ -54,6 +55,17 @@ __device__ __forceinline__ void store_c(IO* p, const float (&e)[C]) {
     *reinterpret_cast<uint4*>(p) = v;
   }
 }
+// C channels of a row as they are in memory.
+template <typename IO, int C>
+struct Piece {
+  using V = std::conditional_t<C == 1, IO, uint4>;
+  V raw;
+  __device__ __forceinline__ void load(const IO* p) { raw = *reinterpret_cast<const V*>(p); }
+  __device__ __forceinline__ void get(float (&e)[C]) const {
+    if constexpr (C == 1) e[0] = to_f32(raw);
+    else load_c<IO, C>(reinterpret_cast<const IO*>(&raw), e);
+  }
+};
 // (K is known when compiled: a tap that is not there must not meet an infinite input with a weight of 0.)
 template <typename IO, int C, int K>
 struct Taps {
@@ -119,7 +131,7 @@ __device__ __forceinline__ void store_hist(const ConvP& p, int slot, int ch, con
 
 // grid (ceil(D / C / 128), runs)
 template <typename IO, int C, int K>
-__global__ void __launch_bounds__(kThreads) sconv_prefill_kernel(ConvP p) {
+__global__ void __launch_bounds__(kThreads, 4) sconv_prefill_kernel(ConvP p) {
   begin_dependent();
   using T = Taps<IO, C, K>;
   const int lane = threadIdx.x & 31, ch = (blockIdx.x * kThreads + threadIdx.x) * C;
@@ -177,16 +189,24 @@ __global__ void __launch_bounds__(kThreads) sconv_prefill_kernel(ConvP p) {
         }
       }
     }
-    for (; t < stop; t += kAhead) {
-      float v[kAhead][C];
+    // four rows are requested while the four before are worked on
+    Piece<IO, C> next[kAhead], now[kAhead];
+    auto request = [&](int at) {
 #pragma unroll
-      for (int r = 0; r < kAhead; ++r) load_c<IO, C>(x + (size_t)min(t + r, stop - 1) * p.D, v[r]);
+      for (int r = 0; r < kAhead; ++r) next[r].load(x + (size_t)min(at + r, stop - 1) * p.D);
+    };
+    request(t);
+    for (; t < stop; t += kAhead) {
+#pragma unroll
+      for (int r = 0; r < kAhead; ++r) now[r] = next[r];
+      if (t + kAhead < stop) request(t + kAhead);
 #pragma unroll
       for (int r = 0; r < kAhead; ++r) {
-        float o[C];
-        taps.apply(v[r], h, o);
+        float v[C], o[C];
+        now[r].get(v);
+        taps.apply(v, h, o);
         if (t + r < stop) store_c<IO, C>(y + (size_t)(t + r) * p.D, o);
-        push(h, v[r]);
+        push(h, v);
       }
     }
   }
@@ -213,9 +233,9 @@ template <typename IO, int C, int K>
 static mxb_status launch_k(ConvP p, cudaStream_t st) {
   const unsigned cols = (p.D / C + kThreads - 1) / kThreads;
   if (p.cu) {
-    // up to 64 rows a run while that gives four CTAs an SM
-    int run = 64;
-    while (run > 8 && (size_t)cols * ((p.rows + run - 1) / run) < 148 * 4) run /= 2;
+    // CTAs for whole rounds of what the GPU holds at once (four an SM by the kernel's registers), runs of 8 to 128 rows
+    const size_t at_once = 148 * 4, work = (size_t)cols * p.rows, rounds = (work + at_once * 128 - 1) / (at_once * 128);
+    int run = (int)std::max<size_t>(8, (work + at_once * rounds - 1) / (at_once * rounds));
     while ((p.rows + run - 1) / run > 65535) run *= 2;
     p.run = run;
     MXB_LAUNCH("sconv_prefill_kernel", st, (launch_kernel(sconv_prefill_kernel<IO, C, K>, dim3(cols, (p.rows + run - 1) / run), kThreads, 0, st, p)));
