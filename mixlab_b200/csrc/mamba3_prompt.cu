@@ -137,29 +137,46 @@ __global__ void __launch_bounds__(kThreads) m3p_prepare_kernel(ServeP p) {
   }
   const int i = tid & 63, t = q.first + i, h0 = ((int)blockIdx.y - p.G) * kRecHeads;
   const bool in = t < q.last, next = in && t + 1 < q.end;
-  float dts[kRecHeads / 2][2], lams[kRecHeads / 2][2], thetas[kRecHeads / 2], logs[kRecHeads / 2];  // (requested before the first is used)
+  // dt, lambda and theta of the eight heads by rows (a head by itself: a sector of 32 bytes for each of its 4), with the step behind
+  constexpr int PITCH = kRecHeads + 1;
+  float(*in_)[Q + 1][PITCH] = reinterpret_cast<float(*)[Q + 1][PITCH]>(tb);
+  static_assert(sizeof(float) * 3 * (Q + 1) * PITCH <= sizeof(tb), "the tile of b is free here");
+#pragma unroll
+  for (int j = 0; j < (Q + 1) * kRecHeads; j += kThreads) {
+    const int e = j + tid, r = e / kRecHeads, hd = h0 + e % kRecHeads;
+    if (r > Q) break;
+    const bool there = q.first + r < (r < Q ? q.last : q.end) && hd < p.NH;
+    const size_t at = (size_t)(there ? q.first + r : q.first) * p.NH + min(hd, p.NH - 1);
+    in_[0][r][e % kRecHeads] = there ? p.dt[at] : 0.f;
+    in_[1][r][e % kRecHeads] = there ? p.lam[at] : 0.f;
+    in_[2][r][e % kRecHeads] = there ? p.theta[at] : 0.f;
+  }
+  __syncthreads();
+  // what needs no other step, of all heads before the first exchange: eight chains side by side
+  float dts[kRecHeads / 2], gammas[kRecHeads / 2], looks[kRecHeads / 2], taints[kRecHeads / 2], rates[kRecHeads / 2];
+  int turns[kRecHeads / 2];
 #pragma unroll
   for (int k = 0; k < kRecHeads / 2; ++k) {
-    const int hd = min(h0 + 2 * k + (w >> 1), p.NH - 1);
-    const size_t a = (size_t)(in ? t : q.first) * p.NH + hd, b = a + (next ? p.NH : 0);
-    dts[k][0] = p.dt[a]; dts[k][1] = p.dt[b];
-    lams[k][0] = p.lam[a]; lams[k][1] = p.lam[b];
-    thetas[k] = p.theta[a];
-    logs[k] = p.a_log[hd];
+    const int c = 2 * k + (w >> 1);
+    // dt in 64 bits: an angle sums up tens of thousands of them, and their float32 roundings with it
+    const double raw = in_[0][i][c], dt64 = fmax(raw, 0.0) + log1p(exp(-fabs(raw)));
+    const float dt = (float)dt64, theta = in_[2][i][c];
+    const double f = dt64 * theta * 0.15915494309189535;
+    turns[k] = in ? (int)__double2ll_rn((f - rint(f)) * 4294967296.0) : 0;
+    taints[k] = in ? m3_taint(dt * theta, 0.f) : 0.f;
+    dts[k] = in ? dt : 0.f;
+    gammas[k] = in ? m3_sigmoid(in_[1][i][c]) * dt : 0.f;
+    looks[k] = next ? (1.f - m3_sigmoid(in_[1][i + 1][c])) * m3_softplus(in_[0][i + 1][c]) : 0.f;
+    rates[k] = -expf(p.a_log[min(h0 + c, p.NH - 1)]) * 1.4426950408889634f;
   }
 #pragma unroll
   for (int k = 0; k < kRecHeads / 2; ++k) {
     if (h0 + 2 * k >= p.NH) break;
-    const int hd = min(h0 + 2 * k + (w >> 1), p.NH - 1);  // (an odd number of heads: one twice, the same record)
-    // dt in 64 bits: an angle sums up tens of thousands of them, and their float32 roundings with it
-    const double raw = dts[k][0], dt64 = fmax(raw, 0.0) + log1p(exp(-fabs(raw)));
-    const float dt = (float)dt64, lam = m3_sigmoid(lams[k][0]), theta = thetas[k];
-    const float look = next ? (1.f - m3_sigmoid(lams[k][1])) * m3_softplus(dts[k][1]) : 0.f;
-    const float A2 = -expf(logs[k]) * 1.4426950408889634f;
-    const double f = dt64 * theta * 0.15915494309189535;
-    int turn = in ? (int)__double2ll_rn((f - rint(f)) * 4294967296.0) : 0;
-    float taint = in ? m3_taint(dt * theta, 0.f) : 0.f, l = in ? dt * A2 : 0.f, r = l;
-    const float own = l, ds = warp_sum(in ? dt : 0.f);
+    const int hd = h0 + 2 * k + (w >> 1);
+    const float dt = dts[k], look = looks[k], gamma = gammas[k];
+    int turn = turns[k];
+    float taint = taints[k], l = dt * rates[k], r = l;
+    const float own = l, ds = warp_sum(dt);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int b = __shfl_up_sync(0xffffffffu, turn, o);
@@ -174,16 +191,18 @@ __global__ void __launch_bounds__(kThreads) m3p_prepare_kernel(ServeP p) {
     if (w & 1) { turn += s_turn[w0]; taint += s_taint[w0]; l += s_l[w0]; }
     else r += s_r[w + 1];
     Rec* rec = reinterpret_cast<Rec*>(p.rec) + (size_t)blockIdx.x * p.NH + hd;
-    const float gamma = in ? lam * dt : 0.f, e = in ? gamma + look : 0.f, g = e * exp2f(r - own);  // (r: from the sum behind row j)
+    const float e = gamma + look, g = e * exp2f(r - own);  // (r: from the sum behind row j)
     const float2 unit = m3_unit(turn, taint);
-    rec->co[i] = unit.x;
-    rec->si[i] = unit.y;
-    rec->L[i] = l;
-    rec->e[i] = e;
-    rec->gam[i] = gamma;
-    rec->gc[i] = g * unit.x;
-    rec->gs[i] = g * unit.y;
-    if (i == 63) {
+    if (hd < p.NH) {  // (the last of an odd number has no partner)
+      rec->co[i] = unit.x;
+      rec->si[i] = unit.y;
+      rec->L[i] = l;
+      rec->e[i] = e;
+      rec->gam[i] = gamma;
+      rec->gc[i] = g * unit.x;
+      rec->gs[i] = g * unit.y;
+    }
+    if (i == 63 && hd < p.NH) {
       rec->turn = turn;
       rec->taint = taint;
       rec->dsum = s_ds[w0] + s_ds[w0 + 1];
@@ -346,7 +365,8 @@ __global__ void __launch_bounds__(2 * kThreads, 2) m3p_chunks_kernel(ServeP p) {
 #pragma unroll
           for (int l = i; l < i + 2; ++l) {
             const float2 v = unpack(a[l]);
-            float2 zc = make_float2(c.x * v.x, c.y * v.y), zs = make_float2(sn.x * v.x, sn.y * v.y);
+            const f2 vv = pack2(v.x, v.y);
+            float2 zc = unpack2(mul2(pack2(c.x, c.y), vv)), zs = unpack2(mul2(pack2(sn.x, sn.y), vv));
             xc[l] = pack(zc.x, zc.y);
             xs[l] = pack(zs.x, zs.y);
             for (int u = 0; u < part; ++u) {
@@ -492,10 +512,10 @@ __global__ void __launch_bounds__(2 * kThreads, 2) m3p_chunks_kernel(ServeP p) {
         const float c0 = rec.co[i0] * f0, s0 = rec.si[i0] * f0, c1 = rec.co[i0 + 8] * f1, s1 = rec.si[i0 + 8] * f1;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          y[m][c][0] = fmaf(c0, y[m][c][0], s0 * z[m][c][0]);
-          y[m][c][1] = fmaf(c0, y[m][c][1], s0 * z[m][c][1]);
-          y[m][c][2] = fmaf(c1, y[m][c][2], s1 * z[m][c][2]);
-          y[m][c][3] = fmaf(c1, y[m][c][3], s1 * z[m][c][3]);
+          float *a = y[m][c], *b = z[m][c];
+          const float2 u = unpack2(mad2(dup2(c0), pack2(a[0], a[1]), mul2(dup2(s0), pack2(b[0], b[1])))),
+                       v = unpack2(mad2(dup2(c1), pack2(a[2], a[3]), mul2(dup2(s1), pack2(b[2], b[3]))));
+          a[0] = u.x; a[1] = u.y; a[2] = v.x; a[3] = v.y;
         }
       }
 #pragma unroll
@@ -537,11 +557,15 @@ __global__ void __launch_bounds__(2 * kThreads, 2) m3p_chunks_kernel(ServeP p) {
       }
     }
     {
-      const float decay = exp2f(rec.Lq);
+      const f2 decay = dup2(exp2f(rec.Lq));
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) h[t][c] *= decay;
+        for (int c = 0; c < 4; c += 2) {
+          const float2 v = unpack2(mul2(decay, pack2(h[t][c], h[t][c + 1])));
+          h[t][c] = v.x;
+          h[t][c + 1] = v.y;
+        }
     }
     // h += (g cos x) (x) b - (g sin x) (x) J b, part after part of the weighted x
     const uint32_t sb = smem_at(s.b[k & 1]) + r16 * (U * 16);
@@ -640,10 +664,12 @@ static mxb_status launch(const ServeP& p, bool ends, cudaStream_t st) {
 
 }  // namespace m3p
 
-// Whole 16-byte pieces of x, b and c rows, and a state that fits a CTA's registers.
+// Whole 16-byte pieces of rows, a state that fits the registers of four warps, and more rows than the walk makes ready at once:
+// up to 16 it takes 7 us, with half of the launches, where the chunks take 14 to 27.
+bool m3prompt_shape(const ServeP& p, bool f32) { return !f32 && p.NH > 0 && p.N % 8 == 0 && p.N <= 128 && p.P % 8 == 0 && p.rows > 16; }
 bool m3prompt_supported(const ServeP& p, bool f32) {
   auto al = [](const void* q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };
-  return !f32 && p.NH > 0 && p.N % 8 == 0 && p.N <= 128 && p.P % 8 == 0 && al(p.x) && al(p.b) && al(p.c) && reinterpret_cast<uintptr_t>(p.y) % 4 == 0;
+  return m3prompt_shape(p, f32) && al(p.x) && al(p.b) && al(p.c) && reinterpret_cast<uintptr_t>(p.y) % 4 == 0;
 }
 mxb_status m3prompt_prepare(const ServeP& p, cudaStream_t st) {
   const dim3 grid(p.chunks, p.G + (p.NH + m3p::kRecHeads - 1) / m3p::kRecHeads);
