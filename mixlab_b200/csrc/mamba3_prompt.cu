@@ -24,8 +24,6 @@
 // Roundings to bf16: G as operand, g x and M once each; y itself.  The state is a float32 result of its own, so that one
 // rounding of g x is too much where it still reaches the segment's end: there (decay to the end above 2^-11, above 2^-3) the
 // remainder of the rounding is multiplied as well, and the remainder of that: 16 and 24 bits of g x, while b is exact.
-//
-// x that is not finite reaches up to 15 rows in front of its own, where it meets a weight of 0.
 #include <algorithm>
 #include <type_traits>
 
@@ -518,17 +516,51 @@ __global__ void __launch_bounds__(2 * kThreads, 2) m3p_chunks_kernel(ServeP p) {
           a[0] = u.x; a[1] = u.y; a[2] = v.x; a[3] = v.y;
         }
       }
+      // M x, below the diagonal's tiles and on them.  There, rows in front of a step meet its x with a weight of 0, which an x that
+      // is not finite does not leave at 0: with one in the chunk its tiles on the diagonal are summed term by term.
+      uint32_t xv[4][4];
+      __nv_bfloat162 odd = __floats2bfloat162_rn(0.f, 0.f);
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
-        uint32_t b[4];
-        ms::ldsm_t(b, xb + at<8>(16 * kk + r16, 2 * w + hi));
+        ms::ldsm_t(xv[kk], xb + at<8>(16 * kk + r16, 2 * w + hi));
 #pragma unroll
-        for (int m = kk; m < 4; ++m) {
+        for (int m = kk + 1; m < 4; ++m) {
           const uint4 v = s.m[k & 1][(m * (m + 1) / 2 + kk) * 32 + lane];
           const uint32_t a[4] = {v.x, v.y, v.z, v.w};
-          ms::mma(y[m][0], a, b[0], b[1]);
-          ms::mma(y[m][1], a, b[2], b[3]);
+          ms::mma(y[m][0], a, xv[kk][0], xv[kk][1]);
+          ms::mma(y[m][1], a, xv[kk][2], xv[kk][3]);
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) odd = __hfma2(*reinterpret_cast<__nv_bfloat162*>(&xv[kk][i]), __floats2bfloat162_rn(0.f, 0.f), odd);
+      }
+      if (!__any_sync(0xffffffffu, *reinterpret_cast<uint32_t*>(&odd) << 1 & 0xfffefffeu)) {
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const uint4 v = s.m[k & 1][m * (m + 3) / 2 * 32 + lane];
+          const uint32_t a[4] = {v.x, v.y, v.z, v.w};
+          ms::mma(y[m][0], a, xv[m][0], xv[m][1]);
+          ms::mma(y[m][1], a, xv[m][2], xv[m][3]);
+        }
+      } else {
+#pragma unroll 1
+        for (int j = 0; j < 16; ++j)
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            const bf16* row = reinterpret_cast<const bf16*>(&s.m[k & 1][m * (m + 3) / 2 * 32 + (lane & 28) + (j & 7) / 2]) + (j / 8) * 4 + (j & 1);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              uint32_t v;
+              asm("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(xb + at<8>(16 * m + j, 2 * w + c) + (lane & 3) * 4) : "memory");
+              const float2 xj = unpack(v);
+#pragma unroll
+              for (int low = 0; low < 2; ++low)
+                if (j <= lane / 4 + 8 * low) {
+                  const float weight = __bfloat162float(row[2 * low]);
+                  y[m][c][2 * low] = fmaf(weight, xj.x, y[m][c][2 * low]);
+                  y[m][c][2 * low + 1] = fmaf(weight, xj.y, y[m][c][2 * low + 1]);
+                }
+            }
+          }
       }
       // Four lanes hold a row's 2 x 8 channels in pairs, for rows 8 apart: they exchange until each has 8 channels of one row.
       const int ql = lane % 4, left = q.last - t0 - lane / 4 - 8 * (ql >> 1), ch = 16 * w + 8 * (ql & 1);

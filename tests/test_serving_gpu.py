@@ -191,6 +191,32 @@ def test_angle_that_is_not_finite(shape):
         assert bool(torch.isnan(state.phase).all()) and bool(torch.isnan(state.h).all())
 
 
+@pytest.mark.parametrize("shape", [(128, 128, 1, 2), (64, 64, 1, 1), (24, 16, 1, 0)], ids=str)
+@pytest.mark.parametrize("io", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("name", ["x", "dt", "lam", "theta", "b", "c"])
+def test_what_is_not_finite_reaches_no_earlier_row(name, io, shape):
+    """A step with an infinity or a NaN leaves the rows in front of it, and the other sequences, what they were."""
+    D, N, G, nheads = shape
+    lens, first = [50, 167, 50], 50
+    a = scan_inputs(267, D, N, G, nheads, io, 19)
+    for flags in (0, WALK):
+        ys = []
+        for value, step in ((None, 0), (float("inf"), 9), (float("nan"), 100), (-float("inf"), 127), (float("nan"), 166)):
+            b = {k: v.clone() for k, v in a.items()}
+            if value is not None:
+                b[name][first + step].view(-1)[0] = value
+            state = ops.mamba3_state(3, D, N, G, nheads=nheads, dtype=io)
+            ys.append(ops.mamba3_prefill(*(t.cuda() for t in args_of(b)), cu_of(lens), state, nheads=nheads, flags=flags))
+            if value is None:
+                continue
+            assert_close(ys[-1][:first + step].cpu(), ys[0][:first + step].cpu().double(), TOL[io], f"in front of step {step}")
+            assert torch.equal(ys[-1][217:], ys[0][217:])
+            reached = value != value or name in "xbc"  # (dt, lam of -inf weigh 0)
+            assert not reached or not bool(torch.isfinite(ys[-1][first + step].float()).all())
+            if name == "x":
+                assert bool(torch.isfinite(ys[-1][:, 1:].float()).all())  # the other channels
+
+
 def test_pool_beyond_32_bit_offsets():
     """Rows of a pool of 2.2 billion elements, the first and the last: 64-bit offsets."""
     D, N, G, nheads, slots = 2048, 128, 1, 32, 8300
