@@ -315,52 +315,61 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// Cosine and sine of two angles in 2^-32 turns: the nearest quarter turn by integers, Taylor polynomials of degree 9 and 10 on
-// what is left, at most pi / 4 (truncation below 2e-9, roundings below 1.2e-7 as in mamba3_windows.cu).
+// Cosine and sine of two angles in 2^-32 turns: the nearest half turn by integers, minimax polynomials of degree 9 and 10 on what
+// is left, at most pi / 2 (fitted by least squares with Lawson's weights: 4.6e-9 and 2.4e-10; with the roundings 2.2e-7, 4e-8 in
+// the mean).  A nearest quarter turn would halve the roundings, and costs a dozen selections more.
 __device__ __forceinline__ void unit2(int t0, int t1, float2& u0, float2& u1) {
-  const int k0 = (t0 + 0x20000000) >> 30, k1 = (t1 + 0x20000000) >> 30;
-  const f2 r = mul2(pack2((float)(t0 - (k0 << 30)), (float)(t1 - (k1 << 30))), dup2(1.4629180792671596e-9f));  // 2 pi / 2^32
+  const int half0 = (t0 + 0x40000000) & 0x80000000, half1 = (t1 + 0x40000000) & 0x80000000;
+  const f2 r = mul2(pack2((float)(t0 ^ half0), (float)(t1 ^ half1)), dup2(1.4629180792671596e-9f));  // 2 pi / 2^32
   const f2 r2 = mul2(r, r);
-  f2 ps = dup2(2.7557319223985893e-6f);
-  ps = mad2(ps, r2, dup2(-1.9841269841269841e-4f));
-  ps = mad2(ps, r2, dup2(8.3333333333333333e-3f));
-  ps = mad2(ps, r2, dup2(-1.6666666666666667e-1f));
+  f2 ps = dup2(2.600054585855105e-06f);
+  ps = mad2(ps, r2, dup2(-0.00019806614727713168f));
+  ps = mad2(ps, r2, dup2(0.008333017118275166f));
+  ps = mad2(ps, r2, dup2(-0.16666656732559204f));
   ps = mad2(mul2(ps, r2), r, r);
-  f2 pc = dup2(-2.7557319223985888e-7f);
-  pc = mad2(pc, r2, dup2(2.4801587301587302e-5f));
-  pc = mad2(pc, r2, dup2(-1.3888888888888889e-3f));
-  pc = mad2(pc, r2, dup2(4.1666666666666667e-2f));
+  f2 pc = dup2(-2.6077103143506974e-07f);
+  pc = mad2(pc, r2, dup2(2.4761886379565112e-05f));
+  pc = mad2(pc, r2, dup2(-0.00138884037733078f));
+  pc = mad2(pc, r2, dup2(0.04166664183139801f));
   pc = mad2(pc, r2, dup2(-0.5f));
   pc = mad2(pc, r2, dup2(1.f));
   const float2 s = unpack2(ps), c = unpack2(pc);
-  auto quarter = [](float s, float c, int k) {
-    const float a = (k & 1) ? c : s, b = (k & 1) ? s : c;
-    return make_float2(__int_as_float(__float_as_int(b) ^ (((k + 1) & 2) << 30)), __int_as_float(__float_as_int(a) ^ ((k & 2) << 30)));
-  };
-  u0 = quarter(s.x, c.x, k0);
-  u1 = quarter(s.y, c.y, k1);
+  auto by = [](float v, int half) { return __int_as_float(__float_as_int(v) ^ half); };
+  u0 = make_float2(by(c.x, half0), by(s.x, half0));
+  u1 = make_float2(by(c.y, half1), by(s.y, half1));
 }
-// m3_turn with dt theta rounded once, as dt is.
-__device__ __forceinline__ int turn_of(float p) {
-  constexpr float kHi = 0.15915493667125702f, kLo = 6.420638243e-09f;
-  const float t = p * kHi, tl = fmaf(p, kLo, fmaf(p, kHi, -t));
-  return __float2int_rn(((t - rintf(t)) + tl) * 4294967296.f);
+// m3_turn of two steps, with dt theta rounded once, as dt is.  (The nearest whole turn by adding 1.5 x 2^23: good for up to 2^22
+// turns a step, where a float32 is no angle any more.)
+__device__ __forceinline__ void turn2(f2 p, int& t0, int& t1) {
+  const f2 hi = dup2(0.15915493667125702f), t = mul2(p, hi), low = mad2(p, dup2(-6.420638243e-09f), mad2(p, dup2(-0.15915493667125702f), t));
+  const f2 whole = add2(add2(t, dup2(12582912.f)), dup2(-12582912.f));
+  const float2 f = unpack2(mul2(mad2(low, dup2(-1.f), mad2(whole, dup2(-1.f), t)), dup2(4294967296.f)));
+  t0 = __float2int_rn(f.x);
+  t1 = __float2int_rn(f.y);
 }
-// What a lane has requested of 8 steps.
-template <typename IO, int PR, Mode MODE>
+// What the lanes have requested of 8 steps.  WHOLE: a warp's channels are of one group and their pairs fill its lanes, so that its
+// rows of theta, b and c are 16-byte pieces that the warp shares; otherwise every lane requests its own elements.
+template <typename IO, int PR, int LPC, Mode MODE, bool WHOLE>
 struct Ahead {
   using Two = std::conditional_t<sizeof(IO) == 4, float2, uint32_t>;  // a pair of b or c
+  static constexpr int kRow = PR * (WHOLE ? 4 * LPC : 128), kR = WHOLE ? LPC : 128;  // pairs of a step; of r
   float theta[kC][PR][128];
-  Two b[kC][PR][128], c[MODE == kOut ? kC : 1][PR][128];
+  Two b[kC][kRow], c[MODE == kOut ? kC : 1][kRow];
 };
+// What a step is made of, two steps side by side: dt, e x, gamma x of each; a channel's 8 steps (padded: other banks).
+struct __align__(16) Two { float dt[2], ex[2], gx[2], pad[2]; };
+struct __align__(16) Steps { Two two[kC / 2]; float pad[4]; };
 template <int BYTES>
 __device__ __forceinline__ void copy_ahead(void* dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "n"(BYTES) : "memory");
 }
+__device__ __forceinline__ void copy_ahead_16(void* dst, const void* src, bool in) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
 __device__ __forceinline__ float2 pair_of(float2 v) { return v; }
 __device__ __forceinline__ float2 pair_of(uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }
 
-template <typename IO, int PR, int LPC, Mode MODE>
+template <typename IO, int PR, int LPC, Mode MODE, bool WHOLE>
 __global__ void __launch_bounds__(128) m3k_channels_kernel(ServeP p) {
   begin_dependent();
   constexpr int OWN = (kC + LPC - 1) / LPC, CPB = 128 / LPC;
@@ -380,7 +389,7 @@ __global__ void __launch_bounds__(128) m3k_channels_kernel(ServeP p) {
 #pragma unroll
   for (int r = 0; r < PR; ++r) {
     kp[r] = sl + r * LPC;
-    has[r] = kp[r] < p.Kp;
+    has[r] = WHOLE || kp[r] < p.Kp;
     G[r] = 0;
     if (MODE == kEnds) H[MODE == kEnds ? r : 0] = 0;
     a[r][0] = a[r][1] = taint[r] = 0.f;
@@ -403,15 +412,57 @@ __global__ void __launch_bounds__(128) m3k_channels_kernel(ServeP p) {
     }
   }
   extern __shared__ __align__(16) unsigned char raw[];
-  using Block = Ahead<IO, PR, MODE>;
+  using Block = Ahead<IO, PR, LPC, MODE, WHOLE>;
   Block* ahead = reinterpret_cast<Block*>(raw);
+  Steps& made = reinterpret_cast<Steps*>(ahead + 2)[threadIdx.x / LPC];
+  const int bc_at = WHOLE ? (threadIdx.x / 32) * PR * LPC + sl : threadIdx.x;  // this lane's first pair in a row of b or c
   const float* theta_at = p.theta + ((size_t)q.first * p.D + d) * p.Kp + sl;
   const IO *b_at = static_cast<const IO*>(p.b) + ((size_t)q.first * p.G + g) * p.N + 2 * sl, *c_at = static_cast<const IO*>(p.c) + ((size_t)q.first * p.G + g) * p.N + 2 * sl;
   const size_t theta_row = (size_t)p.D * p.Kp, bc_row = (size_t)p.G * p.N;
   const bool pairs = ((reinterpret_cast<uintptr_t>(p.b) | reinterpret_cast<uintptr_t>(p.c)) & (2 * sizeof(IO) - 1)) == 0;
   const size_t bc_bytes = bc_row * sizeof(IO), theta_bytes = theta_row * sizeof(float);
+  // WHOLE: this lane's 16-byte pieces, the first of theta and what follows it; pieces of a step's row of b or c
+  const int warp_d = min((int)(blockIdx.y * CPB + (threadIdx.x & 96) / LPC), p.D - 32 / LPC);
+  const int theta_s = lane / 8 / PR, theta_r = lane / 8 % PR, theta_i = lane % 8 * 4;
+  const float* theta_16 = p.theta + ((size_t)(q.first + theta_s) * p.D + warp_d) * p.Kp + theta_r * 32 + theta_i;
+  constexpr int PB = 2 * LPC * PR * (int)sizeof(IO) / 16 + !WHOLE, ALL = kC * PB, PJ = (ALL + 31) / 32;
+  const char *b_16[PJ], *c_16[PJ];
+  if constexpr (WHOLE)
+#pragma unroll
+    for (int j = 0; j < PJ; ++j) {
+      const int i = lane + 32 * j;
+      b_16[j] = reinterpret_cast<const char*>(b_at - 2 * sl) + i / PB * bc_bytes + i % PB * 16;
+      c_16[j] = reinterpret_cast<const char*>(c_at - 2 * sl) + i / PB * bc_bytes + i % PB * 16;
+    }
+  auto request_whole = [&](int left, Block& to, auto all) {  // of as many steps as are left, or all 8
+    constexpr bool FULL = decltype(all)::value;
+    float* dst = &to.theta[theta_s][theta_r][(threadIdx.x & 96) + theta_i];
+#pragma unroll
+    for (int j = 0; j < 2 * PR; ++j) {
+      const int s = j * 4 / PR;
+      const bool in = FULL || theta_s + s < left;
+      copy_ahead_16(dst + s * PR * 128, in ? theta_16 + s * theta_row : p.theta, in);
+    }
+#pragma unroll
+    for (int j = 0; j < PJ; ++j) {
+      const int i = lane + 32 * j, s = i / PB, to_pair = (threadIdx.x / 32) * PR * LPC + i % PB * (8 / (int)sizeof(IO));
+      if (ALL < 32 && i >= ALL) break;
+      const bool in = FULL || s < left;
+      copy_ahead_16(&to.b[s][to_pair], in ? b_16[j] : static_cast<const char*>(p.b), in);
+      if (MODE == kOut) copy_ahead_16(&to.c[MODE == kOut ? s : 0][to_pair], in ? c_16[j] : static_cast<const char*>(p.c), in);
+      b_16[j] += kC * bc_bytes;
+      c_16[j] += kC * bc_bytes;
+    }
+    theta_16 += kC * theta_row;
+  };
   auto request = [&](int t0, Block& to) {  // zeros for steps behind the last and lanes without a pair
     const int steps = min(kC, q.last - t0);
+    if constexpr (WHOLE) {
+      if (steps == kC) request_whole(kC, to, std::true_type{});
+      else request_whole(steps, to, std::false_type{});
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      return;
+    }
     const char *th = reinterpret_cast<const char*>(theta_at), *b = reinterpret_cast<const char*>(b_at), *c = reinterpret_cast<const char*>(c_at);
     if (pairs && steps == kC) {
 #pragma unroll
@@ -421,8 +472,8 @@ __global__ void __launch_bounds__(128) m3k_channels_kernel(ServeP p) {
 #pragma unroll
         for (int s = 0; s < kC; ++s, th_r += theta_bytes, b_r += bc_bytes, c_r += bc_bytes) {
           copy_ahead<4>(&to.theta[s][r][threadIdx.x], th_r);
-          copy_ahead<2 * sizeof(IO)>(&to.b[s][r][threadIdx.x], b_r);
-          if (MODE == kOut) copy_ahead<2 * sizeof(IO)>(&to.c[s][r][threadIdx.x], c_r);
+          copy_ahead<2 * sizeof(IO)>(&to.b[s][bc_at + r * Block::kR], b_r);
+          if (MODE == kOut) copy_ahead<2 * sizeof(IO)>(&to.c[s][bc_at + r * Block::kR], c_r);
         }
       }
     } else {
@@ -432,7 +483,7 @@ __global__ void __launch_bounds__(128) m3k_channels_kernel(ServeP p) {
         for (int r = 0; r < PR; ++r) {
           const bool in = sl + r * LPC < p.Kp && s < steps;
           const IO *bs = reinterpret_cast<const IO*>(b + s * bc_bytes) + 2 * r * LPC, *cs = reinterpret_cast<const IO*>(c + s * bc_bytes) + 2 * r * LPC;
-          IO *db = reinterpret_cast<IO*>(&to.b[s][r][threadIdx.x]), *dc = reinterpret_cast<IO*>(&to.c[MODE == kOut ? s : 0][r][threadIdx.x]);
+          IO *db = reinterpret_cast<IO*>(&to.b[s][bc_at + r * Block::kR]), *dc = reinterpret_cast<IO*>(&to.c[MODE == kOut ? s : 0][bc_at + r * Block::kR]);
           to.theta[s][r][threadIdx.x] = in ? reinterpret_cast<const float*>(th + s * theta_bytes)[r * LPC] : 0.f;
           for (int k = 0; k < 2; ++k) {
             db[k] = in ? bs[k] : from_f32<IO>(0.f);
@@ -445,36 +496,39 @@ __global__ void __launch_bounds__(128) m3k_channels_kernel(ServeP p) {
     c_at += kC * bc_row;
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  if (!has[PR - 1]) {  // (a lane without a pair reads zeros)
+  if (!WHOLE && !has[PR - 1]) {  // (a lane without a pair reads zeros)
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll 1
       for (int s = 0; s < kC; ++s)
         for (int r = 0; r < PR; ++r) {
           ahead[k].theta[s][r][threadIdx.x] = 0.f;
-          ahead[k].b[s][r][threadIdx.x] = {};
-          if (MODE == kOut) ahead[k].c[s][r][threadIdx.x] = {};
+          ahead[k].b[s][bc_at + r * Block::kR] = {};
+          if (MODE == kOut) ahead[k].c[MODE == kOut ? s : 0][bc_at + r * Block::kR] = {};
         }
   }
   // dt, lambda, x of this lane's steps of a block: as read, and what is made of them
   struct Raw { float dt[OWN], lam[OWN], x[OWN]; } next;
   struct Made { float dt[OWN], gamma[OWN], look[OWN], x[OWN]; } own;
+  const float *dt_at = p.dt + (size_t)(q.first + sl) * p.D + d, *lam_at = p.lam + (size_t)(q.first + sl) * p.D + d;
+  const IO* x_at = static_cast<const IO*>(p.x) + (size_t)(q.first + sl) * p.D + d;
   auto request_scalars = [&](int t0) {
 #pragma unroll
-    for (int o = 0; o < OWN; ++o) {
-      const int t = t0 + sl + o * LPC;
-      const bool in = sl + o * LPC < kC && t < q.end;  // (the step behind the segment's last counts, for its weight of that one)
-      const size_t at = (size_t)(in ? t : q.first) * p.D + d;
-      next.dt[o] = in ? p.dt[at] : -INFINITY;
-      next.lam[o] = in ? p.lam[at] : 0.f;
-      next.x[o] = in ? to_f32(static_cast<const IO*>(p.x)[at]) : 0.f;
+    for (int o = 0; o < OWN; ++o) {  // (the step behind the segment's last counts, for its weight of that one)
+      const bool in = sl + o * LPC < kC && t0 + sl + o * LPC < q.end;
+      next.dt[o] = in ? dt_at[(size_t)o * LPC * p.D] : -INFINITY;
+      next.lam[o] = in ? lam_at[(size_t)o * LPC * p.D] : 0.f;
+      next.x[o] = in ? to_f32(x_at[(size_t)o * LPC * p.D]) : 0.f;
     }
+    dt_at += (size_t)kC * p.D;
+    lam_at += (size_t)kC * p.D;
+    x_at += (size_t)kC * p.D;
   };
   auto make_scalars = [&](int t0) {
     Made m;
 #pragma unroll
     for (int o = 0; o < OWN; ++o) {
-      const float dt = m3_softplus(next.dt[o]), lam = m3_sigmoid(next.lam[o]);
+      const float dt = fmaxf(next.dt[o], 0.f) + log1pf(expf(-fabsf(next.dt[o]))), lam = __fdividef(1.f, 1.f + expf(-next.lam[o]));
       const bool in = t0 + sl + o * LPC < q.last;
       m.look[o] = (1.f - lam) * dt;
       m.dt[o] = in ? dt : 0.f;
@@ -487,44 +541,51 @@ __global__ void __launch_bounds__(128) m3k_channels_kernel(ServeP p) {
   request_scalars(q.first);
   own = make_scalars(q.first);
   request_scalars(q.first + kC);
+  IO* y_at = static_cast<IO*>(p.y) + (size_t)(q.first + sl) * p.D + d;  // (of 8 lanes and more)
   int buf = 0;
   for (int t0 = q.first; t0 < q.last; t0 += kC, buf ^= 1) {
     const int steps = min(kC, q.last - t0);
+    __syncwarp();  // (what the warp shares has been read)
+    const Made behind = make_scalars(t0 + kC);
+    if (MODE == kEnds)
+#pragma unroll
+      for (int o = 0; o < OWN; ++o) dsum += own.dt[o];
+#pragma unroll
+    for (int o = 0; o < OWN; ++o) {  // e: lambda dt and what the step behind gives this one
+      const int s = sl + o * LPC;
+      const float a = __shfl_sync(0xffffffffu, own.look[o], base + (sl + 1) % LPC);
+      const float b = o + 1 < OWN ? __shfl_sync(0xffffffffu, own.look[o + 1 < OWN ? o + 1 : 0], base) : __shfl_sync(0xffffffffu, behind.look[0], base);
+      if (LPC > kC && sl >= kC) continue;
+      Two& to = made.two[s / 2];
+      to.dt[s & 1] = own.dt[o];
+      to.ex[s & 1] = (own.gamma[o] + (sl + 1 < (LPC < kC ? LPC : kC) ? a : b)) * own.x[o];
+      if (MODE == kOut) to.gx[s & 1] = own.gamma[o] * own.x[o];
+    }
+    own = behind;
     if (t0 + kC < q.last) {
+      request_scalars(t0 + 2 * kC);
       request(t0 + kC, ahead[buf ^ 1]);
       asm volatile("cp.async.wait_group 1;" ::: "memory");
     } else {
       asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
-    const Made behind = make_scalars(t0 + kC);
-    if (t0 + kC < q.last) request_scalars(t0 + 2 * kC);
-    float dts[OWN], gxs[OWN], exs[OWN], ys[kC];
-#pragma unroll
-    for (int o = 0; o < OWN; ++o) {  // e: lambda dt and what the step behind gives this one
-      const float a = __shfl_sync(0xffffffffu, own.look[o], base + (sl + 1) % LPC);
-      const float b = o + 1 < OWN ? __shfl_sync(0xffffffffu, own.look[o + 1 < OWN ? o + 1 : 0], base) : __shfl_sync(0xffffffffu, behind.look[0], base);
-      dts[o] = own.dt[o];
-      gxs[o] = own.gamma[o] * own.x[o];
-      exs[o] = (own.gamma[o] + (sl + 1 < (LPC < kC ? LPC : kC) ? a : b)) * own.x[o];
-    }
-    own = behind;
+    __syncwarp();
     const Block& now = ahead[buf];
+    float ys[kC];
 #pragma unroll
     for (int s = 0; s < kC; s += 2) {  // two steps' angles together
-      float dt[2], gx[2], ex[2];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        dt[k] = __shfl_sync(0xffffffffu, dts[(s + k) / LPC], base + (s + k) % LPC);
-        gx[k] = MODE == kOut ? __shfl_sync(0xffffffffu, gxs[(s + k) / LPC], base + (s + k) % LPC) : 0.f;
-        ex[k] = __shfl_sync(0xffffffffu, exs[(s + k) / LPC], base + (s + k) % LPC);
-        dsum += dt[k];
-      }
+      const float4 of = *reinterpret_cast<const float4*>(&made.two[s / 2]);
+      const float2 gxs = MODE == kOut ? *reinterpret_cast<const float2*>(made.two[s / 2].gx) : make_float2(0.f, 0.f);
+      const float dt[2] = {of.x, of.y}, ex[2] = {of.z, of.w}, gx[2] = {gxs.x, gxs.y};
       float acc[2] = {0.f, 0.f};
 #pragma unroll
       for (int r = 0; r < PR; ++r) {
-        const float p0 = dt[0] * now.theta[s][r][threadIdx.x], p1 = dt[1] * now.theta[s + 1][r][threadIdx.x];
-        const int t1 = turn[r] + turn_of(p0), t2 = t1 + turn_of(p1);
-        const float n1 = m3_taint(p0, taint[r]), n2 = m3_taint(p1, n1);
+        const f2 angles = mul2(pack2(dt[0], dt[1]), pack2(now.theta[s][r][threadIdx.x], now.theta[s + 1][r][threadIdx.x]));
+        int t1, t2;
+        turn2(angles, t1, t2);
+        t1 += turn[r];
+        t2 += t1;
+        const float n1 = m3_taint(unpack2(angles).x, taint[r]), n2 = m3_taint(unpack2(angles).y, n1);
         float2 unit[2];
         unit2(t1, t2, unit[0], unit[1]);
         acc[0] += n1;  // (an angle that is not finite: y by hand, the state at the block's end)
@@ -533,17 +594,19 @@ __global__ void __launch_bounds__(128) m3k_channels_kernel(ServeP p) {
         taint[r] = n2;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const float2 b = pair_of(now.b[s + k][r][threadIdx.x]);
-          const f2 v = mul2(pack2(ex2(a[r][0] * dt[k]), ex2(a[r][1] * dt[k])), G[r]), e2 = dup2(ex[k]);
+          const float2 b = pair_of(now.b[s + k][bc_at + r * Block::kR]);
+          const float2 decay = unpack2(mul2(pack2(a[r][0], a[r][1]), dup2(dt[k])));
+          const f2 kept = pack2(ex2(decay.x), ex2(decay.y)), v = mul2(kept, G[r]), e2 = dup2(ex[k]);
           if (MODE == kOut) {
-            const float2 u2 = m3_back(b, unit[k]), c = m3_back(pair_of(now.c[MODE == kOut ? s + k : 0][r][threadIdx.x]), unit[k]);
+            const float2 u2 = m3_back(b, unit[k]), c = m3_back(pair_of(now.c[MODE == kOut ? s + k : 0][bc_at + r * Block::kR]), unit[k]);
             const f2 u = pack2(u2.x, u2.y);
-            acc[k] += sum2(mul2(mad2(dup2(gx[k]), u, v), pack2(c.x, c.y)));
+            const float2 h = unpack2(mad2(dup2(gx[k]), u, v));
+            acc[k] = fmaf(h.x, c.x, fmaf(h.y, c.y, acc[k]));
             G[r] = mad2(e2, u, v);
           } else {
             const float2 u = m3_back(b, unit[k]);
             const int h = MODE == kEnds ? r : 0;
-            const f2 w = mul2(pack2(ex2(a[r][0] * dt[k]), ex2(a[r][1] * dt[k])), H[h]);
+            const f2 w = mul2(kept, H[h]);
             G[r] = mad2(e2, pack2(u.x, u.y), v);
             H[h] = mad2(e2, pack2(u.y, -u.x), w);
           }
@@ -561,7 +624,8 @@ __global__ void __launch_bounds__(128) m3k_channels_kernel(ServeP p) {
         colsum8_step<1, 1>(ys, lane);
 #pragma unroll
         for (int o = 8; o < LPC; o <<= 1) ys[0] += __shfl_xor_sync(0xffffffffu, ys[0], o);
-        if (live && sl < steps && sl < kC) static_cast<IO*>(p.y)[(size_t)(t0 + sl) * p.D + d] = from_f32<IO>(ys[0]);
+        if (live && sl < steps && sl < kC) *y_at = from_f32<IO>(ys[0]);
+        y_at += (size_t)kC * p.D;
       } else {
 #pragma unroll
         for (int s = 0; s < kC; ++s) {
@@ -572,6 +636,7 @@ __global__ void __launch_bounds__(128) m3k_channels_kernel(ServeP p) {
       }
     }
   }
+  if (MODE == kEnds) dsum = group_sum<LPC>(dsum);
   if (!live) return;
   if (MODE == kEnds && sl == 0) p.dsum[row] = dsum;
   if (MODE == kOut && (q.seg != q.segs - 1 || slot < 0)) return;
@@ -693,25 +758,34 @@ template <typename IO, Mode MODE>
 static mxb_status channels(const ServeP& p, cudaStream_t st) {
   const ChannelShape s = channel_shape(p);
   const dim3 grid(p.pieces, (p.D + 128 / s.LPC - 1) / (128 / s.LPC));
+  // (pairs that fill the lanes, warps that lie in one group, rows of whole 16-byte pieces)
+  const bool whole = p.Kp == s.LPC * s.PR && p.D / p.G % (32 / s.LPC) == 0 && p.N * sizeof(IO) % 16 == 0 &&
+                     ((reinterpret_cast<uintptr_t>(p.theta) | reinterpret_cast<uintptr_t>(p.b) | reinterpret_cast<uintptr_t>(p.c)) & 15) == 0;
   mxb_status status = MXB_OK;
-  auto launch = [&](auto pr, auto lpc) {
+  auto launch = [&](auto pr, auto lpc, auto all) {
     constexpr int PR = decltype(pr)::value, LPC = decltype(lpc)::value;
-    constexpr int smem = 2 * (int)sizeof(Ahead<IO, PR, MODE>);
-    status = MXB_ALLOW_SMEM(smem, m3k_channels_kernel<IO, PR, LPC, MODE>);
+    constexpr bool WHOLE = decltype(all)::value;
+    constexpr int smem = 2 * (int)sizeof(Ahead<IO, PR, LPC, MODE, WHOLE>) + 128 / LPC * (int)sizeof(Steps);
+    status = MXB_ALLOW_SMEM(smem, m3k_channels_kernel<IO, PR, LPC, MODE, WHOLE>);
     if (status != MXB_OK) return;
     MXB_LAUNCH(MODE == kOut ? "m3k_channels_kernel" : "m3k_channels_ends_kernel", st,
-               (launch_kernel(m3k_channels_kernel<IO, PR, LPC, MODE>, grid, 128, smem, st, p)));
+               (launch_kernel(m3k_channels_kernel<IO, PR, LPC, MODE, WHOLE>, grid, 128, smem, st, p)));
+  };
+  auto by_whole = [&](auto pr, auto lpc) {
+    if constexpr (2 * decltype(pr)::value * decltype(lpc)::value * sizeof(IO) % 16 == 0)
+      if (whole) return launch(pr, lpc, std::true_type{});
+    launch(pr, lpc, std::false_type{});
   };
   constexpr std::integral_constant<int, 1> one;
   switch (s.LPC * s.PR) {
-    case 1: launch(one, one); break;
-    case 2: launch(one, std::integral_constant<int, 2>{}); break;
-    case 4: launch(one, std::integral_constant<int, 4>{}); break;
-    case 8: launch(one, std::integral_constant<int, 8>{}); break;
-    case 16: launch(one, std::integral_constant<int, 16>{}); break;
-    case 32: launch(one, std::integral_constant<int, 32>{}); break;
-    case 64: launch(std::integral_constant<int, 2>{}, std::integral_constant<int, 32>{}); break;
-    default: launch(std::integral_constant<int, 4>{}, std::integral_constant<int, 32>{}); break;
+    case 1: by_whole(one, one); break;
+    case 2: by_whole(one, std::integral_constant<int, 2>{}); break;
+    case 4: by_whole(one, std::integral_constant<int, 4>{}); break;
+    case 8: by_whole(one, std::integral_constant<int, 8>{}); break;
+    case 16: by_whole(one, std::integral_constant<int, 16>{}); break;
+    case 32: by_whole(one, std::integral_constant<int, 32>{}); break;
+    case 64: by_whole(std::integral_constant<int, 2>{}, std::integral_constant<int, 32>{}); break;
+    default: by_whole(std::integral_constant<int, 4>{}, std::integral_constant<int, 32>{}); break;
   }
   return status;
 }

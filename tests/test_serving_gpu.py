@@ -66,7 +66,8 @@ def check_state(state, want, io, tol, used):
 
 # (D, N, G, nheads)
 SHAPES = [(128, 128, 1, 2), (256, 128, 2, 4), (64, 64, 1, 1), (96, 16, 1, 3), (80, 38, 2, 2), (24, 2, 1, 1), (256, 256, 1, 2), (160, 128, 1, 1),
-          (512, 96, 1, 8), (48, 16, 4, 0), (40, 16, 1, 0), (9, 6, 3, 0), (20, 80, 2, 0), (8, 256, 1, 0), (128, 2, 1, 0), (36, 64, 1, 0)]
+          (512, 96, 1, 8), (48, 16, 4, 0), (40, 16, 1, 0), (9, 6, 3, 0), (20, 80, 2, 0), (8, 256, 1, 0), (128, 2, 1, 0), (36, 64, 1, 0),
+          (24, 4, 1, 0), (32, 8, 2, 0), (12, 8, 3, 0), (6, 32, 2, 0), (5, 128, 1, 0)]
 LENS = {"one token": [1], "one": [37], "ragged": [64, 0, 1, 130, 65, 0, 63, 2], "longer": [3, 333, 64], "empty ends": [0, 5, 0]}
 
 
