@@ -223,7 +223,7 @@ struct Smem {
 constexpr int kStart = 128, kReady = 88, kMultiply = 168;
 static_assert(kReady + kMultiply <= 2 * kStart, "what one half takes the other has to give");
 // Barriers between the two halves: a chunk's b, c, x, M are there and the chunk is done with (by its parity), its weighted x is
-// there, a part of that is done with.
+// there, a part of that has been read.
 enum { kFull = 1, kEmpty = 3, kAmong = 5, kWeighted = 6, kPart = 7 };
 __device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 __device__ __forceinline__ void bar_arrive(int id, int n) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(n) : "memory"); }
@@ -244,12 +244,14 @@ __global__ void __launch_bounds__(2 * kThreads, 2) m3p_chunks_kernel(ServeP p) {
   const int p0 = slab * kPS, np = min(kPS, p.P - p0);
   const size_t chan = (size_t)hd * p.P + p0;
   const int slot = serve_slot(p, q.seq), grp = hd / (p.NH / p.G);
+  const bool goes_on = serve_goes_on(p, q.seq);
   const bool keeps = ENDS || (q.seg == q.segs - 1 && slot >= 0);  // the state at the end is somebody's
   const Rec* recs = reinterpret_cast<const Rec*>(p.rec) + (size_t)q.chunk * p.NH + hd;
 
   // chunks from which on one, two parts of g x are not enough: by the decay from their end to the segment's
   int from2 = chunks, from3 = chunks;
-  if (keeps) {
+  auto find_parts = [&] {
+    if (!keeps) return;
     float rem = 0.f;
     for (int k0 = chunks - 1; k0 >= 0 && !(rem <= -11.f); k0 -= 32) {
       const int k = k0 - lane;
@@ -265,7 +267,7 @@ __global__ void __launch_bounds__(2 * kThreads, 2) m3p_chunks_kernel(ServeP p) {
       from3 -= __popc(__ballot_sync(0xffffffffu, k >= 0 && !(behind <= -3.f)));
       rem += __shfl_sync(0xffffffffu, v, 31);
     }
-  }
+  };
 
   if (threadIdx.x >= kThreads) {
     // ---------------------------------------------------------------- the warps that bring operands
@@ -349,7 +351,9 @@ __global__ void __launch_bounds__(2 * kThreads, 2) m3p_chunks_kernel(ServeP p) {
       m[lane] = make_uint4(out[0], out[1], out[2], out[3]);
     };
     auto fetch_rec = [&](int k) { cp16(smem_at(s.rec[k % 3]) + tid * 16, reinterpret_cast<const char*>(recs + (size_t)k * p.NH) + tid * 16, true); };
-    auto weigh_x = [&](int k, int part) {  // this warp's 16 channels; part 1, 2: what rounding has left, and what rounding that has
+    // this warp's 16 channels; part 1, 2: what rounding has left, and what rounding that has
+    auto weigh_x = [&](int k, auto nth) {
+      constexpr int part = decltype(nth)::value;
       const Rec& rec = s.rec[k % 3];
       const uint32_t xb = smem_at(s.x[k & 1]);
 #pragma unroll
@@ -367,6 +371,7 @@ __global__ void __launch_bounds__(2 * kThreads, 2) m3p_chunks_kernel(ServeP p) {
             float2 zc = unpack2(mul2(pack2(c.x, c.y), vv)), zs = unpack2(mul2(pack2(sn.x, sn.y), vv));
             xc[l] = pack(zc.x, zc.y);
             xs[l] = pack(zs.x, zs.y);
+#pragma unroll
             for (int u = 0; u < part; ++u) {
               const float2 d = unpack(xc[l]), e = unpack(xs[l]);
               zc.x -= d.x; zc.y -= d.y; zs.x -= e.x; zs.y -= e.y;
@@ -396,13 +401,19 @@ __global__ void __launch_bounds__(2 * kThreads, 2) m3p_chunks_kernel(ServeP p) {
       cp_commit();
       if (k + 1 < chunks) fetch_rec(k + 1);
       cp_commit();
+      if (k == 0) find_parts();
       if (k >= 1) {  // the chunk that is being multiplied: its weighted x, part after part
         const int parts = k - 1 >= from3 ? 3 : k - 1 >= from2 ? 2 : 1;
-        weigh_x(k - 1, 0);
+        weigh_x(k - 1, std::integral_constant<int, 0>{});
         bar_arrive(kWeighted, 2 * kThreads);
-        for (int part = 1; part < parts; ++part) {
+        if (parts > 1) {
           bar_sync(kPart, 2 * kThreads);
-          weigh_x(k - 1, part);
+          weigh_x(k - 1, std::integral_constant<int, 1>{});
+          bar_arrive(kWeighted, 2 * kThreads);
+        }
+        if (parts > 2) {
+          bar_sync(kPart, 2 * kThreads);
+          weigh_x(k - 1, std::integral_constant<int, 2>{});
           bar_arrive(kWeighted, 2 * kThreads);
         }
       }
@@ -439,34 +450,50 @@ __global__ void __launch_bounds__(2 * kThreads, 2) m3p_chunks_kernel(ServeP p) {
 
   // ------------------------------------------------------------------ the warps that multiply
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kMultiply));
-  const bool from_state = !ENDS && q.segs == 1 && slot >= 0 && serve_goes_on(p, q.seq);
+  const bool from_state = !ENDS && q.segs == 1 && slot >= 0 && goes_on;
   const size_t ph = (size_t)(slot < 0 ? 0 : slot) * p.NH + hd;
   float2 start = make_float2(1.f, 0.f);
   if (!ENDS && q.segs > 1) start = p.start[(size_t)piece * p.NH + hd];
   else if (from_state) start = p.phase[ph];
-  // h[t]: channels 16 w + lane / 4 (+ 8), states 8 t + 2 (lane % 4) + {0, 1}
+  // h[t]: channels 16 w + lane / 4 (+ 8), states 8 t + 2 (lane % 4) + {0, 1}.  One address a row, all elements requested before
+  // the first is used, and little code: a warp runs through it once.
   float h[NT][4];
-  const float look0 = from_state ? serve_look(p, (size_t)q.first * p.NH + hd, true) : 0.f;
+  const int row0 = 16 * w + lane / 4, n0 = 2 * (lane % 4);
+  const bool rows_in[2] = {row0 < np, row0 + 8 < np};
+  auto load_h = [&](const float* from) {
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int row = 16 * w + lane / 4 + 8 * k, n = 8 * t + 2 * (lane % 4);
-      float2 v = make_float2(0.f, 0.f);
-      if (row < np && n < p.N) {
-        if (!ENDS && q.segs > 1) {
-          v = *reinterpret_cast<const float2*>(p.ends + ((size_t)piece * p.D + chan + row) * p.N + n);
-        } else if (from_state) {
-          v = m3_on(*reinterpret_cast<const float2*>(p.h + ((size_t)slot * p.D + chan + row) * p.N + n), start);
-          const float2 b = load_pair(static_cast<const bf16*>(p.b_prev) + ph * p.N + n);
-          const float k0 = look0 * to_f32(static_cast<const bf16*>(p.x_prev)[(size_t)slot * p.D + chan + row]);
-          v.x = fmaf(k0, b.x, v.x);
-          v.y = fmaf(k0, b.y, v.y);
-        }
+      for (int k = 0; k < 2; ++k) {
+        const bool in = rows_in[k] && 8 * t < p.N;
+        const float2 v = in ? *reinterpret_cast<const float2*>(from + (size_t)8 * k * p.N + 8 * t) : make_float2(0.f, 0.f);
+        h[t][2 * k] = v.x;
+        h[t][2 * k + 1] = v.y;
       }
-      h[t][2 * k] = v.x;
-      h[t][2 * k + 1] = v.y;
+  };
+  if (!ENDS && q.segs > 1) {
+    load_h(p.ends + ((size_t)piece * p.D + chan + row0) * p.N + n0);
+  } else if (from_state) {
+    load_h(p.h + ((size_t)slot * p.D + chan + row0) * p.N + n0);
+    const bf16 *b_prev = static_cast<const bf16*>(p.b_prev) + ph * p.N + n0, *x_prev = static_cast<const bf16*>(p.x_prev) + (size_t)slot * p.D + chan + row0;
+    uint32_t b[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) b[t] = 8 * t < p.N ? *reinterpret_cast<const uint32_t*>(b_prev + 8 * t) : 0u;
+    const float look0 = serve_look(p, (size_t)q.first * p.NH + hd, true);
+    const float k0 = rows_in[0] ? look0 * to_f32(x_prev[0]) : 0.f, k1 = rows_in[1] ? look0 * to_f32(x_prev[8]) : 0.f;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const float2 v = unpack(b[t]), h0 = m3_on(make_float2(h[t][0], h[t][1]), start), h1 = m3_on(make_float2(h[t][2], h[t][3]), start);
+      h[t][0] = fmaf(k0, v.x, h0.x);
+      h[t][1] = fmaf(k0, v.y, h0.y);
+      h[t][2] = fmaf(k1, v.x, h1.x);
+      h[t][3] = fmaf(k1, v.y, h1.y);
     }
+  } else {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) h[t][0] = h[t][1] = h[t][2] = h[t][3] = 0.f;
+  }
+  find_parts();
 
   int turn = 0;
   float taint = 0.f, dsum = 0.f;
@@ -612,6 +639,7 @@ __global__ void __launch_bounds__(2 * kThreads, 2) m3p_chunks_kernel(ServeP p) {
         xc[kk][0] = a.x; xc[kk][1] = a.y; xc[kk][2] = a.z; xc[kk][3] = a.w;
         xs[kk][0] = b.x; xs[kk][1] = b.y; xs[kk][2] = b.z; xs[kk][3] = b.w;
       }
+      if (part + 1 < parts) bar_arrive(kPart, 2 * kThreads);  // (this part is in registers: the next is made ready meanwhile)
       uint32_t b[2][4];
       auto load_b = [&](int i) { ms::ldsm_t(b[i & 1], sb + (i % 4) * (16 * U * 16) + (((2 * (i / 4) + hi) ^ (lane & 7)) << 4)); };
       load_b(0);
@@ -635,7 +663,6 @@ __global__ void __launch_bounds__(2 * kThreads, 2) m3p_chunks_kernel(ServeP p) {
             h[2 * t + i][c + 1] -= v[i][c];
           }
       }
-      if (part + 1 < parts) bar_arrive(kPart, 2 * kThreads);
     }
     turn += rec.turn;
     taint += rec.taint;
@@ -648,17 +675,14 @@ __global__ void __launch_bounds__(2 * kThreads, 2) m3p_chunks_kernel(ServeP p) {
     p.dsum[(size_t)piece * p.NH + hd] = dsum + taint;
   }
   if (!keeps) return;
-  const float2 ran = m3_unit(turn, taint);
+  const float2 ran = m3_unit(turn, taint), by = ENDS ? ran : make_float2(start.x, -start.y);  // (R turns on, and back by the conjugate)
+  float* to = (ENDS ? p.ends + ((size_t)piece * p.D + chan + row0) * p.N : p.h + ((size_t)slot * p.D + chan + row0) * p.N) + n0;
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int row = 16 * w + lane / 4 + 8 * k, c = 8 * t + 2 * (lane % 4);
-      if (row >= np || c >= p.N) continue;
-      const float2 v = make_float2(h[t][2 * k], h[t][2 * k + 1]);
-      if (ENDS) *reinterpret_cast<float2*>(p.ends + ((size_t)piece * p.D + chan + row) * p.N + c) = m3_on(v, ran);
-      else *reinterpret_cast<float2*>(p.h + ((size_t)slot * p.D + chan + row) * p.N + c) = m3_back(v, start);
-    }
+    for (int k = 0; k < 2; ++k)
+      if (rows_in[k] && 8 * t < p.N)
+        *reinterpret_cast<float2*>(to + (size_t)8 * k * p.N + 8 * t) = m3_on(make_float2(h[t][2 * k], h[t][2 * k + 1]), by);
   // (the slabs of a head all read its phase and b_prev; with more than one they are written behind this launch)
   if (!ENDS && p.slabs == 1) {  // (every thread has read them: barriers lie between)
     if (tid == 0) p.phase[ph] = m3_turned(start, ran);
