@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(kThreads) m3p_prepare_kernel(ServeP p) {
   __shared__ float s_l[4], s_r[4], s_taint[4], s_ds[4];
   __shared__ int s_turn[4];
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  const Piece q = find_piece<false, false>(p, blockIdx.x, Q);
+  const Piece q = find_piece<kPieces, false>(p, blockIdx.x, Q);
   if (!q.ok) return;
   if ((int)blockIdx.y < p.G) {
     const int grp = blockIdx.y;
@@ -236,9 +236,10 @@ __global__ void __launch_bounds__(2 * kThreads, 2) m3p_chunks_kernel(ServeP p) {
   Smem<N>& s = *reinterpret_cast<Smem<N>*>(raw);
   constexpr int U = N / 8, NT = N / 8, KK = N / 16;
   const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) & 3, tid = threadIdx.x & (kThreads - 1);
-  const int per = p.NH * p.slabs, piece = blockIdx.x / per, hd = blockIdx.x % per / p.slabs, slab = blockIdx.x % p.slabs;  // (heads first)
-  const Piece q = find_piece(p, piece, p.L);
-  if (!q.ok || (ENDS && q.seg == q.segs - 1)) return;
+  const int per = p.NH * p.slabs, hd = blockIdx.x % per / p.slabs, slab = blockIdx.x % p.slabs;  // (heads first)
+  const Piece q = find_piece<ENDS ? kInner : kPieces>(p, blockIdx.x / per, p.L);
+  const int piece = q.base + q.seg;
+  if (!q.ok || piece >= p.pieces) return;
   const int chunks = (q.last - q.first + Q - 1) / Q;
   if (q.chunk + chunks > p.chunks) return;  // (lengths that add up to more than the rows)
   const int p0 = slab * kPS, np = min(kPS, p.P - p0);
@@ -701,7 +702,7 @@ template <int N>
 static mxb_status launch(const ServeP& p, bool ends, cudaStream_t st) {
   const int smem = (int)sizeof(Smem<N>);
   auto go = [&](auto kernel, const char* name) {
-    MXB_LAUNCH(name, st, (launch_kernel(kernel, dim3((unsigned)((size_t)p.pieces * p.NH * p.slabs)), 2 * kThreads, smem, st, p)));
+    MXB_LAUNCH(name, st, (launch_kernel(kernel, dim3((unsigned)((size_t)(ends ? p.rows / p.L : p.pieces) * p.NH * p.slabs)), 2 * kThreads, smem, st, p)));
     return check_launch(name);
   };
   static std::atomic<bool> looked_up{false};

@@ -70,70 +70,72 @@ struct Piece {
   bool ok;
 };
 // The index-th piece: sequences one after the other, each cut every L rows; up to 32 sequences by falling length, so that the
-// long ones do not start last (32 heads of 16 sequences of 440 to 4377 rows: a third off the time).  Called by whole warps.
-// Whatever cu holds, rows stay inside the call's.
-// SEQUENCE: the first piece of the index-th sequence in that order.  SORT: false: sequences as they come (chunks are numbered so).
-template <bool SEQUENCE = false, bool SORT = true>
+// long ones do not start last (32 heads of 16 sequences of 440 to 4377 rows: a third off the time).  Called by whole warps, which
+// look through 32 sequences at a time and add up those in front.  Whatever cu holds, rows stay inside the call's.
+// kInner: the index-th of the pieces that are not their sequence's last (at most rows / L of them); kCut: the first piece of the
+// index-th sequence that is cut.  SORT: false: sequences as they come (chunks are numbered so).
+enum Find { kPieces, kInner, kCut };
+template <Find WHAT = kPieces, bool SORT = true>
 __device__ __forceinline__ Piece find_piece(const ServeP& p, int index, int L) {
   const int lane = threadIdx.x & 31;
+  constexpr unsigned kAll = 0xffffffffu;
+  auto scan = [&](int v) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(kAll, v, o);
+      if (lane >= o) v += u;
+    }
+    return v;
+  };
+  auto wanted = [](int n) { return WHAT == kPieces ? n : WHAT == kInner ? max(n - 1, 0) : n > 1; };
   Piece q{};
-  int before = 0, chunks = 0;
+  int before = 0, base = 0, chunks = 0;  // wanted pieces, pieces, chunks in front
   for (int s0 = 0; s0 < p.S; s0 += 32) {
     const int s = s0 + lane;
-    int a = 0, e = 0, n = 0;
+    int a = 0, e = 0;
     if (s < p.S) {
       a = min(max(__ldg(p.cu + s), 0), p.rows);
       e = min(max(__ldg(p.cu + s + 1), a), p.rows);
-      n = (int)(((long long)e - a + L - 1) / L);
     }
-    int id = s, cn = (e - a + 63) / 64, chunk = cn;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int c = __shfl_up_sync(0xffffffffu, chunk, o);
-      if (lane >= o) chunk += c;
+    int n = (int)(((unsigned)(e - a) + (unsigned)L - 1u) / (unsigned)L);
+    const int cn = (e - a + 63) / 64, these = __reduce_add_sync(kAll, wanted(n));
+    if (index >= before + these) {
+      before += these;
+      base += WHAT == kPieces ? these : __reduce_add_sync(kAll, n);
+      chunks += __reduce_add_sync(kAll, cn);
+      continue;
     }
-    const int all = __shfl_sync(0xffffffffu, chunk, 31);
-    chunk += chunks - cn;
-    chunks += all;
+    int id = s, chunk = chunks + scan(cn) - cn;
     if (SORT && p.S > 1 && p.S <= 32) {
       const int len = s < p.S ? e - a : -1;
       int rank = 0, from = 0;
 #pragma unroll 8
       for (int j = 0; j < 32; ++j) {
-        const int other = __shfl_sync(0xffffffffu, len, j);
+        const int other = __shfl_sync(kAll, len, j);
         rank += other > len || (other == len && j < lane);
       }
 #pragma unroll 8
       for (int j = 0; j < 32; ++j)
-        if (__shfl_sync(0xffffffffu, rank, j) == lane) from = j;
+        if (__shfl_sync(kAll, rank, j) == lane) from = j;
       id = from;
-      a = __shfl_sync(0xffffffffu, a, from);
-      e = __shfl_sync(0xffffffffu, e, from);
-      n = __shfl_sync(0xffffffffu, n, from);
-      chunk = __shfl_sync(0xffffffffu, chunk, from);
+      a = __shfl_sync(kAll, a, from);
+      e = __shfl_sync(kAll, e, from);
+      n = __shfl_sync(kAll, n, from);
+      chunk = __shfl_sync(kAll, chunk, from);
     }
-    int incl = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
-    }
-    const unsigned m = __ballot_sync(0xffffffffu, SEQUENCE ? s == index : before + incl > index);
-    if (m) {
-      const int src = __ffs(m) - 1;
-      q.seq = __shfl_sync(0xffffffffu, id, src);
-      q.begin = __shfl_sync(0xffffffffu, a, src);
-      q.end = __shfl_sync(0xffffffffu, e, src);
-      q.segs = __shfl_sync(0xffffffffu, n, src);
-      q.base = before + __shfl_sync(0xffffffffu, incl - n, src);
-      q.seg = SEQUENCE ? 0 : index - q.base;
-      q.first = q.begin + q.seg * L;
-      q.last = (int)min((long long)q.first + L, (long long)q.end);
-      q.chunk = __shfl_sync(0xffffffffu, chunk, src) + (q.first - q.begin) / 64;
-      q.ok = q.segs > 0;
-      return q;
-    }
-    before += __shfl_sync(0xffffffffu, incl, 31);
+    const int all = scan(n), mine = WHAT == kPieces ? all : scan(wanted(n));
+    const int src = __ffs(__ballot_sync(kAll, before + mine > index)) - 1;
+    q.seq = __shfl_sync(kAll, id, src);
+    q.begin = __shfl_sync(kAll, a, src);
+    q.end = __shfl_sync(kAll, e, src);
+    q.segs = __shfl_sync(kAll, n, src);
+    q.base = (WHAT == kPieces ? before : base) + __shfl_sync(kAll, all - n, src);
+    q.seg = WHAT == kCut ? 0 : index - before - __shfl_sync(kAll, mine - wanted(n), src);
+    q.first = q.begin + q.seg * L;
+    q.last = (int)min((long long)q.first + L, (long long)q.end);
+    q.chunk = __shfl_sync(kAll, chunk, src) + (q.first - q.begin) / 64;
+    q.ok = true;
+    return q;
   }
   return q;
 }

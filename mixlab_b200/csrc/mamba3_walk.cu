@@ -40,9 +40,10 @@ __global__ void __launch_bounds__(256) m3k_heads_kernel(ServeP p, int LN) {
   __shared__ HeadSmem sc;
   __shared__ int s_turn;
   __shared__ float s_taint, s_dt;
-  const int heads = p.NH * p.slabs, piece = blockIdx.x / heads, tid = threadIdx.x, hd = blockIdx.x % heads / p.slabs, slab = blockIdx.x % p.slabs;
-  const Piece q = find_piece(p, piece, p.L);
-  if (!q.ok || (MODE == kEnds && q.seg == q.segs - 1)) return;
+  const int heads = p.NH * p.slabs, tid = threadIdx.x, hd = blockIdx.x % heads / p.slabs, slab = blockIdx.x % p.slabs;
+  const Piece q = find_piece<MODE == kEnds ? kInner : kPieces>(p, blockIdx.x / heads, p.L);
+  const int piece = q.base + q.seg;
+  if (!q.ok || piece >= p.pieces) return;
   const int ln = tid % LN, rg = tid / LN, rows_at_once = 256 / LN, npad = LN * 4 * NV;
   const int per = (p.P + p.slabs - 1) / p.slabs, p0 = slab * per, np = min(per, p.P - p0);  // this CTA's channels of the head
   const size_t chan = (size_t)hd * p.P + p0;
@@ -222,8 +223,8 @@ __global__ void __launch_bounds__(256) m3k_heads_kernel(ServeP p, int LN) {
 constexpr int kAhead = 8;
 __global__ void __launch_bounds__(256) m3k_heads_chain_kernel(ServeP p, bool bf16_io) {
   begin_dependent();
-  const Piece q = find_piece<true>(p, blockIdx.x, p.L);
-  if (!q.ok || q.segs == 1 || q.base + q.segs > p.pieces) return;  // (more segments: lengths beyond the rows)
+  const Piece q = find_piece<kCut>(p, blockIdx.x, p.L);
+  if (!q.ok || q.base + q.segs > p.pieces) return;  // (more segments: lengths beyond the rows)
   const int slot = serve_slot(p, q.seq);
   const bool go = slot >= 0 && serve_goes_on(p, q.seq);
   const size_t pairs = (size_t)p.D * p.Kp;
@@ -377,11 +378,12 @@ __global__ void __launch_bounds__(128) m3k_channels_kernel(ServeP p) {
   const int d_raw = blockIdx.y * CPB + threadIdx.x / LPC;
   const bool live = d_raw < p.D;
   const int d = live ? d_raw : p.D - 1;
-  const Piece q = find_piece(p, blockIdx.x, p.L);
-  if (!q.ok || (MODE == kEnds && q.seg == q.segs - 1)) return;
+  const Piece q = find_piece<MODE == kEnds ? kInner : kPieces>(p, blockIdx.x, p.L);
+  const int piece = q.base + q.seg;
+  if (!q.ok || piece >= p.pieces) return;
   const int slot = serve_slot(p, q.seq), g = d / (p.D / p.G);
   const bool from_state = MODE == kOut && q.segs == 1 && slot >= 0 && serve_goes_on(p, q.seq);
-  const size_t sd = (size_t)(slot < 0 ? 0 : slot) * p.D + d, row = (size_t)blockIdx.x * p.D + d;
+  const size_t sd = (size_t)(slot < 0 ? 0 : slot) * p.D + d, row = (size_t)piece * p.D + d;
   f2 G[PR], H[MODE == kEnds ? PR : 1];  // the state; kEnds: its factors of the cosine and of the sine of the angle at the start
   float a[PR][2], taint[PR], dsum = 0.f;
   int turn[PR], kp[PR];
@@ -659,8 +661,8 @@ __global__ void __launch_bounds__(128) m3k_channels_kernel(ServeP p) {
 // What the segments of a sequence start from, as m3k_heads_chain_kernel: the state and the angle.
 __global__ void __launch_bounds__(256) m3k_channels_chain_kernel(ServeP p, bool bf16_io) {
   begin_dependent();
-  const Piece q = find_piece<true>(p, blockIdx.x, p.L);
-  if (!q.ok || q.segs == 1 || q.base + q.segs > p.pieces) return;  // (more segments: lengths beyond the rows)
+  const Piece q = find_piece<kCut>(p, blockIdx.x, p.L);
+  if (!q.ok || q.base + q.segs > p.pieces) return;  // (more segments: lengths beyond the rows)
   const int slot = serve_slot(p, q.seq);
   const bool go = slot >= 0 && serve_goes_on(p, q.seq);
   const size_t pairs = (size_t)p.D * p.Kp;
@@ -738,7 +740,7 @@ template <typename IO, Mode MODE>
 static void heads(const ServeP& p, cudaStream_t st) {
   const HeadShape s = head_shape(p);
   const size_t smem = sizeof(float) * (2 * kW * (size_t)s.LN * 4 * s.NV + 2 * kW * kRowsMost);
-  const dim3 grid((unsigned)((size_t)p.pieces * p.NH * s.slabs));
+  const dim3 grid((unsigned)((size_t)(MODE == kEnds ? p.rows / p.L : p.pieces) * p.NH * s.slabs));
   auto launch = [&](auto nv, auto r) {
     constexpr int NV = decltype(nv)::value, R = decltype(r)::value;
     MXB_LAUNCH(MODE == kOut ? "m3k_heads_kernel" : "m3k_heads_ends_kernel", st,
@@ -757,7 +759,7 @@ static void heads(const ServeP& p, cudaStream_t st) {
 template <typename IO, Mode MODE>
 static mxb_status channels(const ServeP& p, cudaStream_t st) {
   const ChannelShape s = channel_shape(p);
-  const dim3 grid(p.pieces, (p.D + 128 / s.LPC - 1) / (128 / s.LPC));
+  const dim3 grid(MODE == kEnds ? p.rows / p.L : p.pieces, (p.D + 128 / s.LPC - 1) / (128 / s.LPC));
   // (pairs that fill the lanes, warps that lie in one group, rows of whole 16-byte pieces)
   const bool whole = p.Kp == s.LPC * s.PR && p.D / p.G % (32 / s.LPC) == 0 && p.N * sizeof(IO) % 16 == 0 &&
                      ((reinterpret_cast<uintptr_t>(p.theta) | reinterpret_cast<uintptr_t>(p.b) | reinterpret_cast<uintptr_t>(p.c)) & 15) == 0;
@@ -791,8 +793,9 @@ static mxb_status channels(const ServeP& p, cudaStream_t st) {
 }
 template <typename IO>
 static mxb_status prefill(ServeP p, bool chunks, cudaStream_t st) {
-  const size_t blocks = ((size_t)p.D * p.Kp + 255) / 256;  // (most of many sequences are not cut: few blocks each)
-  const dim3 chain(p.S, (unsigned)std::min<size_t>(blocks, std::max<size_t>(148 * 4 / p.S, 1)));
+  const size_t blocks = ((size_t)p.D * p.Kp + 255) / 256;
+  const int cuts = std::max(std::min(p.S, (int)(p.rows / ((long long)p.L + 1))), 1);  // sequences that can be longer than L
+  const dim3 chain(cuts, (unsigned)std::min<size_t>(blocks, std::max<size_t>(148 * 4 / cuts, 1)));
   const bool cut = p.ends != nullptr;
   if (p.NH) {
     p.slabs = chunks ? serve_slabs(p) : head_shape(p).slabs;
