@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(256) m3k_heads_kernel(ServeP p, int LN) {
 
   auto row_of = [&](int r) { return rg + r * rows_at_once; };
   auto n_of = [&](int k) { return (ln + k * LN) * 4; };
-  float G[R][NV][4];
+  f2 G[R][NV][2];
   const float look0 = from_state ? serve_look(p, (size_t)q.first * p.NH + hd, true) : 0.f;
 #pragma unroll
   for (int r = 0; r < R; ++r)
@@ -79,20 +79,47 @@ __global__ void __launch_bounds__(256) m3k_heads_kernel(ServeP p, int LN) {
             v.y = fmaf(w, b.y, v.y);
           }
         }
-        G[r][k][i] = v.x;
-        G[r][k][i + 1] = v.y;
+        G[r][k][i / 2] = pack2(v.x, v.y);
       }
   if (tid == 0) { s_turn = 0; s_taint = 0.f; s_dt = 0.f; }
+  // What 16 steps are made of, as read; requested while the 16 in front are walked.
+  constexpr int XR = kW * kRowsMost / 256, NB = NV == 4 ? 8 : 4;
+  struct { float dt, lam, theta, dt1, lam1, x[XR]; float2 b[NB], c[MODE == kOut ? NB : 1]; } raw;
+  const int bs = tid / 16, bj = tid % 16;  // 16 threads a step
+  auto request = [&](int t0) {
+    if (tid < kW) {
+      const int t = t0 + tid;
+      const bool in = t < q.last, next = in && t + 1 < q.end;
+      const size_t at = (size_t)(in ? t : q.first) * p.NH + hd;
+      raw.dt = p.dt[at];
+      raw.lam = p.lam[at];
+      raw.theta = p.theta[at];
+      raw.dt1 = next ? p.dt[at + p.NH] : -INFINITY;
+      raw.lam1 = next ? p.lam[at + p.NH] : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < XR; ++k) {
+      const int i = tid + k * 256, s = i / kRowsMost, r = i % kRowsMost;
+      raw.x[k] = r < np && t0 + s < q.last ? to_f32(static_cast<const IO*>(p.x)[(size_t)(t0 + s) * p.D + chan + r]) : 0.f;
+    }
+    const bool in = t0 + bs < q.last;
+    const size_t row = ((size_t)(in ? t0 + bs : q.first) * p.G + g) * p.N;
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+      const int n = 2 * (bj + 16 * k);
+      raw.b[k] = in && n < p.N ? load_pair(static_cast<const IO*>(p.b) + row + n) : make_float2(0.f, 0.f);
+      if (MODE == kOut) raw.c[MODE == kOut ? k : 0] = in && n < p.N ? load_pair(static_cast<const IO*>(p.c) + row + n) : make_float2(0.f, 0.f);
+    }
+  };
+  request(q.first);
   for (int t0 = q.first; t0 < q.last; t0 += kW) {
     __syncthreads();
     if (tid < 32) {  // scalars of the steps; the angle runs on from block to block
-      const int t = t0 + tid;
-      const bool in = tid < kW && t < q.last;
-      const size_t at = (size_t)(in ? t : q.first) * p.NH + hd;
-      const float dt = m3_softplus(p.dt[at]), lam = m3_sigmoid(p.lam[at]), theta = p.theta[at];
-      const float look = serve_look(p, at + p.NH, in && t + 1 < q.end);
-      int turn = in ? m3_turn(dt, theta) : 0;
-      float taint = in ? m3_taint(dt * theta, 0.f) : 0.f, sum = in ? dt : 0.f;
+      const bool in = tid < kW && t0 + tid < q.last;
+      const float dt = m3_softplus(raw.dt), lam = m3_sigmoid(raw.lam);
+      const float look = (1.f - m3_sigmoid(raw.lam1)) * m3_softplus(raw.dt1);
+      int turn = in ? m3_turn(dt, raw.theta) : 0;
+      float taint = in ? m3_taint(dt * raw.theta, 0.f) : 0.f, sum = in ? dt : 0.f;
 #pragma unroll
       for (int o = 1; o < kW; o <<= 1) {
         const int a = __shfl_up_sync(0xffffffffu, turn, o);
@@ -111,64 +138,59 @@ __global__ void __launch_bounds__(256) m3k_heads_kernel(ServeP p, int LN) {
         sc.unit[tid] = m3_unit(turn, taint);
       }
     }
-    for (int i = tid; i < kW * np; i += 256) {
-      const int s = i / np, r = i - s * np;
-      sx[s * kRowsMost + r] = t0 + s < q.last ? to_f32(static_cast<const IO*>(p.x)[(size_t)(t0 + s) * p.D + chan + r]) : 0.f;
-    }
+#pragma unroll
+    for (int k = 0; k < XR; ++k) sx[tid + k * 256] = raw.x[k];
     __syncthreads();
-    {  // 16 threads a step
-      const int s = tid / 16, j = tid % 16;
-      const bool in = t0 + s < q.last;
-      const size_t row = ((size_t)(in ? t0 + s : q.first) * p.G + g) * p.N;
-      const float2 a = sc.unit[s];
+    {
+      const float2 a = sc.unit[bs];
       float dot = 0.f;
-      for (int k = j; k < npad / 2; k += 16) {
-        float2 u = make_float2(0.f, 0.f), c = u;
-        if (in && 2 * k < p.N) {
-          const float2 b = load_pair(static_cast<const IO*>(p.b) + row + 2 * k);
-          u = m3_back(b, a);
-          if (MODE == kOut) {
-            const float2 cr = load_pair(static_cast<const IO*>(p.c) + row + 2 * k);
-            dot = fmaf(b.x, cr.x, fmaf(b.y, cr.y, dot));  // <Brot, Crot> = <b, c>
-            c = m3_back(cr, a);
-          }
+#pragma unroll
+      for (int k = 0; k < NB; ++k) {
+        const int pair = bj + 16 * k;
+        if (2 * pair >= npad) break;
+        reinterpret_cast<float2*>(su + bs * npad)[pair] = m3_back(raw.b[k], a);
+        if (MODE == kOut) {
+          const float2 b = raw.b[k], c = raw.c[MODE == kOut ? k : 0];
+          dot = fmaf(b.x, c.x, fmaf(b.y, c.y, dot));  // <Brot, Crot> = <b, c>
+          reinterpret_cast<float2*>(scv + bs * npad)[pair] = m3_back(c, a);
         }
-        reinterpret_cast<float2*>(su + s * npad)[k] = u;
-        if (MODE == kOut) reinterpret_cast<float2*>(scv + s * npad)[k] = c;
       }
       if (MODE == kOut) {
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-        if (j == 0) sc.gs[s] = sc.gamma[s] * dot + a.x * 0.f;  // (an angle that is not finite has to reach y here too)
+        if (bj == 0) sc.gs[bs] = sc.gamma[bs] * dot + a.x * 0.f;  // (an angle that is not finite has to reach y here too)
       }
     }
     __syncthreads();
+    request(t0 + kW);
     const int steps = min(kW, q.last - t0);
     for (int s = 0; s < steps; ++s) {
       const float alpha = sc.alpha[s], e = sc.e[s];
-      float u[NV][4], c[NV][4], acc[R];
+      f2 u[NV][2], c[NV][2];
+      float acc[R];
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const float4 a = *reinterpret_cast<const float4*>(su + s * npad + n_of(k));
-        u[k][0] = a.x; u[k][1] = a.y; u[k][2] = a.z; u[k][3] = a.w;
+        const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(su + s * npad + n_of(k));
+        u[k][0] = a.x; u[k][1] = a.y;
         if (MODE == kOut) {
-          const float4 b = *reinterpret_cast<const float4*>(scv + s * npad + n_of(k));
-          c[k][0] = b.x; c[k][1] = b.y; c[k][2] = b.z; c[k][3] = b.w;
+          const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(scv + s * npad + n_of(k));
+          c[k][0] = b.x; c[k][1] = b.y;
         }
       }
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         const int row = row_of(r);
-        const float x = row < np ? sx[s * kRowsMost + row] : 0.f, ex = e * x;
-        acc[r] = 0.f;
+        const f2 ex = dup2(row < np ? e * sx[s * kRowsMost + row] : 0.f), keep = dup2(alpha);
+        f2 sum = 0;
 #pragma unroll
         for (int k = 0; k < NV; ++k)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float v = alpha * G[r][k][i];
-            if (MODE == kOut) acc[r] = fmaf(c[k][i], v, acc[r]);
-            G[r][k][i] = fmaf(ex, u[k][i], v);
+          for (int i = 0; i < 2; ++i) {
+            const f2 v = mul2(keep, G[r][k][i]);
+            if (MODE == kOut) sum = mad2(c[k][i], v, sum);
+            G[r][k][i] = mad2(ex, u[k][i], v);
           }
+        acc[r] = sum2(sum);
       }
       if (MODE == kOut) {
 #pragma unroll
@@ -207,7 +229,7 @@ __global__ void __launch_bounds__(256) m3k_heads_kernel(ServeP p, int LN) {
       for (int i = 0; i < 4; i += 2) {
         const int row = row_of(r), n = n_of(k) + i;
         if (row >= np || n >= p.N) continue;
-        const float2 v = make_float2(G[r][k][i], G[r][k][i + 1]);
+        const float2 v = unpack2(G[r][k][i / 2]);
         if (MODE == kEnds) *reinterpret_cast<float2*>(p.ends + ((size_t)piece * p.D + chan + row) * p.N + n) = m3_on(v, ran);
         else *reinterpret_cast<float2*>(p.h + ((size_t)slot * p.D + chan + row) * p.N + n) = m3_back(v, start);
       }
@@ -717,15 +739,16 @@ __global__ void __launch_bounds__(256) m3k_channels_chain_kernel(ServeP p, bool 
 
 // ------------------------------------------------------------------ host
 static int serve_slabs(const ServeP& p) { return (p.P + kRowsMost - 1) / kRowsMost; }
+// Lanes along a row: as few as keep a row's 4 NV states (NV up to 4) in registers, for a step's sum over lanes costs a row LN's
+// logarithm in exchanges, but enough that narrow heads still give all threads a row.
 struct HeadShape { int LN, NV, R, slabs; };
 static HeadShape head_shape(const ServeP& p) {
-  HeadShape s{1, 1, 1, 1};
-  while (s.LN * 4 < p.N && s.LN < 32) s.LN *= 2;
+  HeadShape s{4, 1, 1, 1};
+  while (s.LN * 4 < p.N && (s.LN < 8 || s.LN * 16 < p.N || (256 / s.LN > p.P && s.LN < (p.N > 128 ? 16 : 32)))) s.LN *= 2;
   while (s.LN * 4 * s.NV < p.N) s.NV *= 2;
-  const int at_once = 256 / s.LN, most = std::min(kRowsMost, at_once * (8 / s.NV));
-  s.slabs = (p.P + most - 1) / most;
+  s.slabs = (p.P + kRowsMost - 1) / kRowsMost;
   const int per = (p.P + s.slabs - 1) / s.slabs;
-  while (s.R * at_once < per) s.R *= 2;
+  while (s.R * (256 / s.LN) < per) s.R *= 2;
   return s;
 }
 struct ChannelShape { int PR, LPC; };
@@ -746,15 +769,17 @@ static void heads(const ServeP& p, cudaStream_t st) {
     MXB_LAUNCH(MODE == kOut ? "m3k_heads_kernel" : "m3k_heads_ends_kernel", st,
                (launch_kernel(m3k_heads_kernel<IO, NV, R, MODE>, grid, 256, smem, st, p, s.LN)));
   };
+  constexpr std::integral_constant<int, 1> one;
+  constexpr std::integral_constant<int, 2> two;
+  constexpr std::integral_constant<int, 4> four;
   auto by_r = [&](auto nv) {
-    constexpr int NV = decltype(nv)::value;
-    if (s.R == 1) launch(nv, std::integral_constant<int, 1>{});
-    else if (s.R == 2) launch(nv, std::integral_constant<int, 2>{});
-    else if (s.R == 4 || NV == 2) launch(nv, std::integral_constant<int, 4>{});
-    else launch(nv, std::integral_constant<int, 8>{});
+    if (s.R == 1) launch(nv, one);
+    else launch(nv, two);
   };
-  if (s.NV == 1) by_r(std::integral_constant<int, 1>{});
-  else by_r(std::integral_constant<int, 2>{});
+  if (s.NV == 1) by_r(one);
+  else if (s.NV == 2) by_r(two);
+  else if (s.R == 4) launch(four, four);
+  else by_r(four);
 }
 template <typename IO, Mode MODE>
 static mxb_status channels(const ServeP& p, cudaStream_t st) {
