@@ -21,6 +21,11 @@
 // this way.  (Turning b and c instead halves two of the three products, but the turning, with its passes through shared memory,
 // took more time than that.)
 //
+// Bound: shared memory.  16 prompts, 32768 rows, 32 heads of 64 channels and 128 states, half of them from states: scalars and
+// scores 35 us, chunks 307 us at 67 % of the shared-memory pipe and 43 % of the tensor pipe's time, 336 us in all (the products
+// alone at that rate 131, the bytes 49).  Two CTAs of eight warps an SM; one CTA of 12 or 16 warps, with the fragments of b and c
+// for 32 channels a warp or products and state in warps of their own, took 359 to 374 us where this took 322.
+//
 // Roundings to bf16: G as operand, g x and M once each; y itself.  The state is a float32 result of its own, so that one
 // rounding of g x is too much where it still reaches the segment's end: there (decay to the end above 2^-11, above 2^-3) the
 // remainder of the rounding is multiplied as well, and the remainder of that: 16 and 24 bits of g x, while b is exact.
@@ -722,7 +727,8 @@ static mxb_status launch(const ServeP& p, bool ends, cudaStream_t st) {
 }  // namespace m3p
 
 // Whole 16-byte pieces of rows, a state that fits the registers of four warps, and more rows than the walk makes ready at once:
-// up to 16 it takes 7 us, with half of the launches, where the chunks take 14 to 27.
+// one prompt of 16 rows of 32 heads 23 us by the walk, of 17 rows 24 by the chunks and 25 by the walk, of 64 rows 26 and 45, of
+// 512 rows 48 and 83 (timer and cold caches included); 16 prompts of 2048 rows 376 and 2491.
 bool m3prompt_shape(const ServeP& p, bool f32) { return !f32 && p.NH > 0 && p.N % 8 == 0 && p.N <= 128 && p.P % 8 == 0 && p.rows > 16; }
 bool m3prompt_supported(const ServeP& p, bool f32) {
   auto al = [](const void* q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };

