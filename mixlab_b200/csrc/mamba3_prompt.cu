@@ -94,8 +94,9 @@ __global__ void __launch_bounds__(kThreads) m3p_prepare_kernel(ServeP p) {
   begin_dependent();
   constexpr int U = N / 8;
   __shared__ uint4 tb[Q * U], tc[Q * U];
-  __shared__ float s_l[4], s_r[4], s_taint[4], s_ds[4];
-  __shared__ int s_turn[4];
+  constexpr int K2 = kRecHeads / 2;
+  __shared__ float s_l[K2][4], s_r[K2][4], s_taint[K2][4], s_ds[K2][4];
+  __shared__ int s_turn[K2][4];
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const Piece q = find_piece<kPieces, false>(p, blockIdx.x, Q);
   if (!q.ok) return;
@@ -156,10 +157,10 @@ __global__ void __launch_bounds__(kThreads) m3p_prepare_kernel(ServeP p) {
   }
   __syncthreads();
   // what needs no other step, of all heads before the first exchange: eight chains side by side
-  float dts[kRecHeads / 2], gammas[kRecHeads / 2], looks[kRecHeads / 2], taints[kRecHeads / 2], rates[kRecHeads / 2];
-  int turns[kRecHeads / 2];
+  float dts[K2], gammas[K2], looks[K2], taints[K2], rates[K2];
+  int turns[K2];
 #pragma unroll
-  for (int k = 0; k < kRecHeads / 2; ++k) {
+  for (int k = 0; k < K2; ++k) {
     const int c = 2 * k + (w >> 1);
     // dt in 64 bits: an angle sums up tens of thousands of them, and their float32 roundings with it
     const double raw = in_[0][i][c], dt64 = fmax(raw, 0.0) + log1p(exp(-fabs(raw)));
@@ -172,46 +173,51 @@ __global__ void __launch_bounds__(kThreads) m3p_prepare_kernel(ServeP p) {
     looks[k] = next ? (1.f - m3_sigmoid(in_[1][i + 1][c])) * m3_softplus(in_[0][i + 1][c]) : 0.f;
     rates[k] = -expf(p.a_log[min(h0 + c, p.NH - 1)]) * 1.4426950408889634f;
   }
+  float l[K2], r[K2], own[K2], ds[K2];
 #pragma unroll
-  for (int k = 0; k < kRecHeads / 2; ++k) {
-    if (h0 + 2 * k >= p.NH) break;
+  for (int k = 0; k < K2; ++k) {
+    own[k] = l[k] = r[k] = dts[k] * rates[k];
+    ds[k] = dts[k];
+  }
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1)  // (four heads' chains of sums beside each other)
+#pragma unroll
+    for (int k = 0; k < K2; ++k) {
+      const int b = __shfl_up_sync(0xffffffffu, turns[k], o);
+      const float c = __shfl_up_sync(0xffffffffu, taints[k], o), d = __shfl_up_sync(0xffffffffu, l[k], o), e = __shfl_down_sync(0xffffffffu, r[k], o);
+      ds[k] += __shfl_xor_sync(0xffffffffu, ds[k], o);
+      if (lane >= o) { turns[k] += b; taints[k] += c; l[k] += d; }
+      if (lane + o < 32) r[k] += e;
+    }
+#pragma unroll
+  for (int k = 0; k < K2; ++k) {
+    if (lane == 31) { s_turn[k][w] = turns[k]; s_taint[k][w] = taints[k]; s_l[k][w] = l[k]; s_ds[k][w] = ds[k]; }
+    if (lane == 0) s_r[k][w] = r[k];
+  }
+  __syncthreads();
+  const int w0 = w & 2;
+#pragma unroll
+  for (int k = 0; k < K2; ++k) {
     const int hd = h0 + 2 * k + (w >> 1);
-    const float dt = dts[k], look = looks[k], gamma = gammas[k];
-    int turn = turns[k];
-    float taint = taints[k], l = dt * rates[k], r = l;
-    const float own = l, ds = warp_sum(dt);
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int b = __shfl_up_sync(0xffffffffu, turn, o);
-      const float c = __shfl_up_sync(0xffffffffu, taint, o), d = __shfl_up_sync(0xffffffffu, l, o), e = __shfl_down_sync(0xffffffffu, r, o);
-      if (lane >= o) { turn += b; taint += c; l += d; }
-      if (lane + o < 32) r += e;
-    }
-    if (lane == 31) { s_turn[w] = turn; s_taint[w] = taint; s_l[w] = l; s_ds[w] = ds; }
-    if (lane == 0) s_r[w] = r;
-    __syncthreads();
-    const int w0 = w & 2;
-    if (w & 1) { turn += s_turn[w0]; taint += s_taint[w0]; l += s_l[w0]; }
-    else r += s_r[w + 1];
+    if (hd >= p.NH) break;
+    if (w & 1) { turns[k] += s_turn[k][w0]; taints[k] += s_taint[k][w0]; l[k] += s_l[k][w0]; }
+    else r[k] += s_r[k][w + 1];
     Rec* rec = reinterpret_cast<Rec*>(p.rec) + (size_t)blockIdx.x * p.NH + hd;
-    const float e = gamma + look, g = e * exp2f(r - own);  // (r: from the sum behind row j)
-    const float2 unit = m3_unit(turn, taint);
-    if (hd < p.NH) {  // (the last of an odd number has no partner)
-      rec->co[i] = unit.x;
-      rec->si[i] = unit.y;
-      rec->L[i] = l;
-      rec->e[i] = e;
-      rec->gam[i] = gamma;
-      rec->gc[i] = g * unit.x;
-      rec->gs[i] = g * unit.y;
+    const float e = gammas[k] + looks[k], g = e * exp2f(r[k] - own[k]);  // (r: from the sum behind row j)
+    const float2 unit = m3_unit(turns[k], taints[k]);
+    rec->co[i] = unit.x;
+    rec->si[i] = unit.y;
+    rec->L[i] = l[k];
+    rec->e[i] = e;
+    rec->gam[i] = gammas[k];
+    rec->gc[i] = g * unit.x;
+    rec->gs[i] = g * unit.y;
+    if (i == 63) {
+      rec->turn = turns[k];
+      rec->taint = taints[k];
+      rec->dsum = s_ds[k][w0] + s_ds[k][w0 + 1];
+      rec->Lq = l[k];
     }
-    if (i == 63 && hd < p.NH) {
-      rec->turn = turn;
-      rec->taint = taint;
-      rec->dsum = s_ds[w0] + s_ds[w0 + 1];
-      rec->Lq = l;
-    }
-    __syncthreads();  // (the sums are used again)
   }
 }
 
