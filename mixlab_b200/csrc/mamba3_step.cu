@@ -4,8 +4,8 @@
 // The state keeps cosine and sine of phi, and the token before as its x and its (unturned) b.
 //
 // The state is read once and written once, in 16-byte pieces; everything else is small.  Bound: HBM for large batches, launch
-// and one chain of load -> sum -> store for small ones.  Heads, 64 channels and 128 states, bf16: 256 tokens of 32 heads 101 us
-// (546 MB: 83 % of the measured copy rate), one token 6.9 us; 61 tokens of 448 channels of 16 states, float32, 9.4 us.
+// and one chain of load -> sum -> store for small ones.  Heads, 64 channels and 128 states, bf16: 256 tokens of 32 heads 96 us
+// (546 MB: 87 % of the measured copy rate), one token 6.9 us; 61 tokens of 448 channels of 16 states, float32, 9.4 us.
 #include "mamba3_serve.cuh"
 
 namespace mxb {
@@ -33,9 +33,11 @@ __device__ __forceinline__ void store_states(float* p, const float (&e)[V]) {
 // Heads: a CTA per (sequence, head); LN lanes along a row of states with NV pieces of V each, 8 / NV consecutive rows a thread at a
 // time.  The pieces are requested first; meanwhile two warps work out the scalars and turn b, c and the token before's b, two
 // more fetch x.  b_prev has a row a head, so that the CTA which writes it is the only one that reads it.
+// Four CTAs an SM (64 registers): 96 us for the 256 tokens, 101 with the three that 80 registers allow; stores that do not stream
+// take 35 us more.
 constexpr int kStepPieces = 8, kStepRowsMost = 8 * 256;
 template <typename IO, int V, int NV>
-__global__ void __launch_bounds__(256) m3s_step_heads_kernel(ServeP p, int LN) {
+__global__ void __launch_bounds__(256, 4) m3s_step_heads_kernel(ServeP p, int LN) {
   begin_dependent();
   constexpr int R = kStepPieces / NV;
   __shared__ __align__(16) float s_u[256], s_v[256], s_c[256];
@@ -77,26 +79,35 @@ __global__ void __launch_bounds__(256) m3s_step_heads_kernel(ServeP p, int LN) {
   };
   const size_t sh = (size_t)seq * p.NH + hd, ph = (size_t)slot * p.NH + hd;
   if (tid < 64) {
+    // (b, c and the token before's b are requested in front of the angle: a CTA's chain of loads is what it lives for)
+    const int g = hd / (p.NH / p.G);
+    const IO *B = static_cast<const IO*>(p.b) + ((size_t)seq * p.G + g) * p.N, *C = static_cast<const IO*>(p.c) + ((size_t)seq * p.G + g) * p.N;
+    IO* BP = static_cast<IO*>(p.b_prev) + ph * p.N;
+    float2 bs[2], cs[2], bps[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int n = 2 * (tid + 64 * j);
+      const bool in = n < p.N;
+      bs[j] = in ? load_pair(B + n) : make_float2(0.f, 0.f);
+      cs[j] = in ? load_pair(C + n) : make_float2(0.f, 0.f);
+      bps[j] = in ? load_pair(BP + n) : make_float2(0.f, 0.f);
+    }
     const float dt = m3_softplus(p.dt[sh]), lam = m3_sigmoid(p.lam[sh]), theta = p.theta[sh];
     const float look = (1.f - lam) * dt, gamma = lam * dt;
     const float2 old = p.phase[ph];
     const float2 now = m3_turned(old, m3_unit(m3_turn(dt, theta), m3_taint(dt * theta, 0.f)));
-    const int g = hd / (p.NH / p.G);
-    const IO *B = static_cast<const IO*>(p.b) + ((size_t)seq * p.G + g) * p.N, *C = static_cast<const IO*>(p.c) + ((size_t)seq * p.G + g) * p.N;
-    IO* BP = static_cast<IO*>(p.b_prev) + ph * p.N;
-    for (int k = tid; k < npad / 2; k += 64) {
-      float2 u = make_float2(0.f, 0.f), v = u, c = u;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int k = tid + 64 * j;
+      if (k >= npad / 2) break;
+      const float2 u = m3_back(bs[j], now), v = m3_back(bps[j], old);
       if (2 * k < p.N) {
-        const float2 b = load_pair(B + 2 * k);
-        u = m3_back(b, now);
-        c = m3_back(load_pair(C + 2 * k), now);
-        v = m3_back(load_pair(BP + 2 * k), old);
-        BP[2 * k] = from_f32<IO>(b.x);
-        BP[2 * k + 1] = from_f32<IO>(b.y);
+        BP[2 * k] = from_f32<IO>(bs[j].x);
+        BP[2 * k + 1] = from_f32<IO>(bs[j].y);
       }
       reinterpret_cast<float2*>(s_u)[k] = make_float2(gamma * u.x, gamma * u.y);
       reinterpret_cast<float2*>(s_v)[k] = make_float2(look * v.x, look * v.y);
-      reinterpret_cast<float2*>(s_c)[k] = c;
+      reinterpret_cast<float2*>(s_c)[k] = m3_back(cs[j], now);
     }
     asm volatile("bar.sync 1, 64;" ::: "memory");  // (both warps have read the phase)
     if (tid == 0) {
