@@ -22,7 +22,7 @@
 // took more time than that.)
 //
 // Bound: shared memory.  16 prompts, 32768 rows, 32 heads of 64 channels and 128 states, half of them from states: scalars and
-// scores 35 us, chunks 307 us at 67 % of the shared-memory pipe and 43 % of the tensor pipe's time, 336 us in all (the products
+// scores 33 us, chunks 306 us at 70 % of the shared-memory pipe and 45 % of the tensor pipe's time, 334 us in all (the products
 // alone at that rate 131, the bytes 49).  Two CTAs of eight warps an SM; one CTA of 12 or 16 warps, with the fragments of b and c
 // for 32 channels a warp or products and state in warps of their own, took 359 to 374 us where this took 322.
 //
