@@ -9,7 +9,7 @@
 //
 // HBM streams: 8191 rows of 2048 columns, bf16 with a float32 stream, gate and scale, 42 us (235 MB: 86 % of the measured copy
 // rate); every gradient of 32768 rows in bf16 222 us (1.07 GB: 74 %), 8 of them in the column sums' own launch; one row 6.2 us, of
-// which the call on the host is most.  A row is read once, held by TPR threads in 8 (beyond 8192 columns 16) registers a tensor, and its sums go
+// which the call on the host is most.  A row is read once, held by TPR threads in 8 to 32 registers a tensor, and its sums go
 // through the lanes and, for TPR > 32, shared memory; narrow rows share a CTA.  Column sums of the gradients: every group of
 // TPR threads walks over rows with its columns' sums in registers and leaves a partial row; a second launch adds those in a
 // fixed order.  Everything is computed in float32 whatever the tensors' types.
@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(kThreads<TPR>) rnorm_fwd_kernel(NormP p) {
 }
 
 template <typename IO, typename RES, int TPR, int E, bool V>
-__global__ void __launch_bounds__(kThreads<TPR>, TPR > 256 ? 1 : 2) rnorm_bwd_kernel(NormP p) {
+__global__ void __launch_bounds__(kThreads<TPR>, TPR > 256 || E > 1 ? 1 : 2) rnorm_bwd_kernel(NormP p) {
   begin_dependent();
   __shared__ float red[kThreads<TPR> / 32 * 3];
   constexpr int GROUPS = kThreads<TPR> / TPR;
@@ -261,7 +261,8 @@ __global__ void __launch_bounds__(kThreads<TPR>, TPR > 256 ? 1 : 2) rnorm_bwd_ke
   for (int e = 0; e < E; ++e)
 #pragma unroll
     for (int i = 0; i < 4; ++i) dnorm[e][i] = both[e][i] = 0;
-  // the next row of each tensor is under way while one is worked on
+  // the next row of each tensor is under way while one is worked on (where there are registers for it)
+  constexpr bool EARLY = TPR <= 256;
   Ahead<RES, V> a_r[E], a_d[E];
   Ahead<IO, V> a_g[E], a_y[E], a_z[E];
   auto offset = [&](size_t r0) { return (r0 + group < p.rows ? r0 + group : r0) * p.D; };
@@ -277,11 +278,12 @@ __global__ void __launch_bounds__(kThreads<TPR>, TPR > 256 ? 1 : 2) rnorm_bwd_ke
       if (p.z) a_z[e].load(static_cast<const IO*>(p.z) + off, c, p.D);
     }
   };
-  request((size_t)blockIdx.x * GROUPS);
+  if (EARLY) request((size_t)blockIdx.x * GROUPS);
   for (size_t r0 = (size_t)blockIdx.x * GROUPS; r0 < p.rows; r0 += (size_t)gridDim.x * GROUPS) {
     const bool live = r0 + group < p.rows;
     const size_t off = offset(r0);
     f2 r[E][4], y[E][4], g[E][4], d[E][4], z[E][4], s0 = 0, s1 = 0, s2 = 0;
+    if (!EARLY) request(r0);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int c = (lane + e * TPR) * 8;
@@ -296,7 +298,7 @@ __global__ void __launch_bounds__(kThreads<TPR>, TPR > 256 ? 1 : 2) rnorm_bwd_ke
       }
       if (p.z) a_z[e].get(static_cast<const IO*>(p.z) + off, c, p.D, z[e]);
     }
-    if (r0 + (size_t)gridDim.x * GROUPS < p.rows) request(r0 + (size_t)gridDim.x * GROUPS);
+    if (EARLY && r0 + (size_t)gridDim.x * GROUPS < p.rows) request(r0 + (size_t)gridDim.x * GROUPS);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       f2 w[4];
@@ -404,30 +406,52 @@ static int threads_per_row(int D) {  // the smallest power of two with 8 columns
   while (8 * t < D && t < 1024) t *= 2;
   return t;
 }
+// Threads of a row, pieces of 8 columns a thread.  The gradients hold six tensors' pieces and the columns' sums: beyond 2048 columns
+// one CTA of fewer threads with more registers (16384 rows of 4096 columns in bf16 250 us, with 512 threads 326; 8192 of 8192 375,
+// with 1024 threads 747), up to there two CTAs (32768 rows of 2048 218 us; with half of the threads a row 279).
+struct RowShape { int tpr, e; };
+static RowShape row_shape(int D, bool bwd) {
+  const int t = threads_per_row(D);
+  if (!bwd) return {t, D > 8192 ? 2 : 1};
+  if (D <= 2048) return {t, 1};
+  if (D <= 4096) return {t / 2, 2};
+  return {512, D > 8192 ? 4 : 2};
+}
 static int groups_of(int tpr) { return tpr > 256 ? 1 : 256 / tpr; }
 // CTAs: what the GPU holds at once, 4 an SM forwards and, by registers, 2 backwards (8191 rows of 2048 columns 42.6 us, 49.7 with
-// half of them, 43.0 with twice as many; gradients of 32768 rows 213, 309, 218).
+// half of them, 43.0 with twice as many), or one with two pieces a thread.
 static int ctas(size_t rows, int D, bool bwd) {
-  const int tpr = threads_per_row(D), g = groups_of(tpr);
-  const size_t want = (rows + g - 1) / g, most = std::max(148, 148 * (bwd ? 2 : 4) * 256 / std::max(tpr, 256));
+  const RowShape s = row_shape(D, bwd);
+  const int g = groups_of(s.tpr);
+  const size_t want = (rows + g - 1) / g, most = std::max(148, 148 * (!bwd ? 4 : s.e == 1 ? 2 : 1) * 256 / std::max(s.tpr, 256));
   return (int)std::min(want, most);
 }
 template <typename F>
-static void by_shape(int D, F&& f) {
-  auto call = [&](auto t) {
-    if (D > 8192) f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 2>{});
-    else f(t, std::integral_constant<int, 1>{});
-  };
-  switch (threads_per_row(D)) {
-    case 4: call(std::integral_constant<int, 4>{}); break;
-    case 8: call(std::integral_constant<int, 8>{}); break;
-    case 16: call(std::integral_constant<int, 16>{}); break;
-    case 32: call(std::integral_constant<int, 32>{}); break;
-    case 64: call(std::integral_constant<int, 64>{}); break;
-    case 128: call(std::integral_constant<int, 128>{}); break;
-    case 256: call(std::integral_constant<int, 256>{}); break;
-    case 512: call(std::integral_constant<int, 512>{}); break;
-    default: call(std::integral_constant<int, 1024>{}); break;
+static void by_shape(int D, bool bwd, F&& f) {
+  const RowShape s = row_shape(D, bwd);
+  constexpr std::integral_constant<int, 1> one;
+  constexpr std::integral_constant<int, 2> two;
+  if (bwd && s.e > 1) {
+    switch (s.tpr) {
+      case 256: f(std::integral_constant<int, 256>{}, two); break;
+      default:
+        if (s.e == 2) f(std::integral_constant<int, 512>{}, two);
+        else f(std::integral_constant<int, 512>{}, std::integral_constant<int, 4>{});
+    }
+    return;
+  }
+  switch (s.tpr) {
+    case 4: f(std::integral_constant<int, 4>{}, one); break;
+    case 8: f(std::integral_constant<int, 8>{}, one); break;
+    case 16: f(std::integral_constant<int, 16>{}, one); break;
+    case 32: f(std::integral_constant<int, 32>{}, one); break;
+    case 64: f(std::integral_constant<int, 64>{}, one); break;
+    case 128: f(std::integral_constant<int, 128>{}, one); break;
+    case 256: f(std::integral_constant<int, 256>{}, one); break;
+    case 512: f(std::integral_constant<int, 512>{}, one); break;
+    default:
+      if (s.e == 1) f(std::integral_constant<int, 1024>{}, one);
+      else f(std::integral_constant<int, 1024>{}, two);
   }
 }
 template <typename IO, typename RES, bool V>
@@ -435,14 +459,16 @@ static mxb_status run(const NormP& p, float* const (&sums)[3], cudaStream_t st) 
   const bool bwd = p.dn != nullptr;
   const int n = ctas(p.rows, p.D, bwd);
   int parts = 0;
-  by_shape(p.D, [&](auto tpr, auto e) {
+  by_shape(p.D, bwd, [&](auto tpr, auto e) {
     constexpr int TPR = decltype(tpr)::value, E = decltype(e)::value;
-    if (bwd) {
-      parts = n * (kThreads<TPR> / TPR);
-      MXB_LAUNCH("rnorm_bwd_kernel", st, (launch_kernel(rnorm_bwd_kernel<IO, RES, TPR, E, V>, n, kThreads<TPR>, 0, st, p)));
-    } else {
-      MXB_LAUNCH("rnorm_fwd_kernel", st, (launch_kernel(rnorm_fwd_kernel<IO, RES, TPR, E, V>, n, kThreads<TPR>, 0, st, p)));
-    }
+    // (row_shape(): which there are)
+    if constexpr (E == 1 ? TPR <= 256 : TPR <= 512)
+      if (bwd) {
+        parts = n * (kThreads<TPR> / TPR);
+        MXB_LAUNCH("rnorm_bwd_kernel", st, (launch_kernel(rnorm_bwd_kernel<IO, RES, TPR, E, V>, n, kThreads<TPR>, 0, st, p)));
+      }
+    if constexpr (E == 1 || TPR > 512)
+      if (!bwd) MXB_LAUNCH("rnorm_fwd_kernel", st, (launch_kernel(rnorm_fwd_kernel<IO, RES, TPR, E, V>, n, kThreads<TPR>, 0, st, p)));
   });
   if (bwd) {
     const SumP s{p.part, parts, p.D, sums[0], sums[1], sums[2], p.post, p.scale};
@@ -474,7 +500,7 @@ static mxb_status by_type(const mxb_residual_norm_desc* d, const NormP& p, float
 }  // namespace rnorm
 
 size_t residual_norm_scratch(const mxb_residual_norm_desc* d) {
-  const int tpr = rnorm::threads_per_row(d->D);
+  const int tpr = rnorm::row_shape(d->D, true).tpr;
   return (size_t)rnorm::ctas(d->rows, d->D, true) * rnorm::groups_of(tpr) * 2 * d->D * sizeof(float);
 }
 mxb_status residual_norm_fwd(const mxb_residual_norm_desc* d, const void* resid, const void* y, const float* norm, const float* post,

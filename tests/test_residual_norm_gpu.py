@@ -49,7 +49,7 @@ def oracle_grads(a, d=True, eps=1e-5):
 
 
 OPTIONS = [(False, False, False), (True, False, False), (False, True, True), (True, True, True), (True, False, True)]
-SIZES = [(1, 1), (3, 7), (5, 64), (1, 449), (700, 40), (33, 1000), (9, 2048), (2, 5000), (3, 8200), (2, 16384)]
+SIZES = [(1, 1), (3, 7), (5, 64), (1, 449), (700, 40), (33, 1000), (9, 2048), (300, 2600), (400, 4096), (2, 5000), (3, 8200), (2, 16384)]
 
 
 @pytest.mark.parametrize("io,res", [(F32, F32), (BF16, F32), (BF16, BF16)], ids=["f32", "bf16 on f32", "bf16"])
