@@ -6,12 +6,13 @@
 //     h_t = alpha_t G_{t-1} + lam_t dt_t Brot_t x_t;   y_t = <h_t, Crot_t>;   G_t = alpha_t G_{t-1} + e_t Brot_t x_t
 //     e_t = lam_t dt_t + (1 - lam_{t+1}) dt_{t+1}
 // A walk is one chain of steps, and prompts that are few and long would leave the GPU to a few of them.  Sequences longer than
-// L steps are cut into segments (serve_segment()): a first pass walks every segment but a sequence's last from a zero state,
+// L steps are cut into segments (walk_segment()): a first pass walks every segment but a sequence's last from a zero state,
 // a second one chains what they add, H <- decay H + added, and the walk that writes y starts from the results.
 //
 // Head layout: decay and angle are a head's own, so turning commutes with the decay and each segment counts its angle from
 // its own start; the state between two segments is the turned-on one, R(phi) h.  Channel layout: the two states of a pair
-// decay at rates of their own, so angles count from the sequence's start and a pass in front sums them by segments.
+// decay at rates of their own, so angles count from the sequence's start: the first pass leaves what a segment adds as the factors
+// of cosine and sine of its first angle, which the chain knows.
 #include <algorithm>
 #include <type_traits>
 
@@ -242,7 +243,7 @@ __global__ void __launch_bounds__(256) m3k_heads_kernel(ServeP p, int LN) {
   }
 }
 
-// What the segments of a sequence start from.  grid (sequences, blocks of pairs): a thread per state pair of the channels walks
+// What the segments of a sequence start from.  grid (sequences that can be longer than L, blocks of pairs): a thread per state pair of the channels walks
 // over the segments; what kAhead segments add is requested at a time.
 constexpr int kAhead = 8;
 __global__ void __launch_bounds__(256) m3k_heads_chain_kernel(ServeP p, bool bf16_io) {
@@ -327,8 +328,8 @@ __global__ void __launch_bounds__(256) m3k_heads_phase_kernel(ServeP p) {
 
 // ------------------------------------------------------------------ channels
 // LPC lanes a channel with PR state pairs each, 8 steps at a time: a lane works out softplus and sigmoid of its own steps and
-// hands them round; theta and the rows of b and c come by cp.async 8 steps ahead, each lane's own elements into its own places
-// in shared memory (no barrier, and no registers while they are under way).
+// hands them round through shared memory; theta and the rows of b and c come by cp.async 8 steps ahead, by 16-byte pieces that a
+// warp shares or each lane's own elements into its own places (no barrier of the CTA, no registers while they are under way).
 //
 // What bounds it is the issue of instructions, a sine, a cosine and two exponentials a state pair and step (4003 steps x 448
 // channels of 16 states: 14 M of them, 62 instructions each in the first pass over what is cut, 44 us, and 80 in the second, 52 us).  So two steps' angles go through packed polynomials, the two states of a pair are
