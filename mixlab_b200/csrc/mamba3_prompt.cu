@@ -488,14 +488,14 @@ __global__ void __launch_bounds__(2 * kThreads, 2) m3p_chunks_kernel(ServeP p) {
   } else if (from_state) {
     load_h(p.h + ((size_t)slot * p.D + chan + row0) * p.N + n0);
     const bf16 *b_prev = static_cast<const bf16*>(p.b_prev) + ph * p.N + n0, *x_prev = static_cast<const bf16*>(p.x_prev) + (size_t)slot * p.D + chan + row0;
-    uint32_t b[NT];
+    float2 b[NT];  // (by elements: the pool's b may start at any)
 #pragma unroll
-    for (int t = 0; t < NT; ++t) b[t] = 8 * t < p.N ? *reinterpret_cast<const uint32_t*>(b_prev + 8 * t) : 0u;
+    for (int t = 0; t < NT; ++t) b[t] = 8 * t < p.N ? load_pair(b_prev + 8 * t) : make_float2(0.f, 0.f);
     const float look0 = serve_look(p, (size_t)q.first * p.NH + hd, true);
     const float k0 = rows_in[0] ? look0 * to_f32(x_prev[0]) : 0.f, k1 = rows_in[1] ? look0 * to_f32(x_prev[8]) : 0.f;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const float2 v = unpack(b[t]), h0 = m3_on(make_float2(h[t][0], h[t][1]), start), h1 = m3_on(make_float2(h[t][2], h[t][3]), start);
+      const float2 v = b[t], h0 = m3_on(make_float2(h[t][0], h[t][1]), start), h1 = m3_on(make_float2(h[t][2], h[t][3]), start);
       h[t][0] = fmaf(k0, v.x, h0.x);
       h[t][1] = fmaf(k0, v.y, h0.y);
       h[t][2] = fmaf(k1, v.x, h1.x);

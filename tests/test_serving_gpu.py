@@ -314,6 +314,32 @@ def test_unaligned_operands_give_the_same():
         ops.mamba3_decode_step(ops.Mamba3State(odd(s.h), *s[1:]), *(t if i == 4 else t[:1].contiguous() for i, t in enumerate(dev)), nheads=nheads)
 
 
+@pytest.mark.parametrize("shape", [(128, 128, 1, 2), (128, 40, 2, 2), (64, 64, 1, 1), (24, 16, 1, 0), (36, 64, 1, 0)], ids=str)
+@pytest.mark.parametrize("io", [F32, BF16], ids=["f32", "bf16"])
+def test_pool_rows_may_start_at_any_element(io, shape):
+    """x_prev and b_prev as views that start at an odd element, beside operands on 16 bytes, of prompts that go on from them:
+    short ones, one that is cut, and single tokens.  The same kernels on the same values: the same bits."""
+    D, N, G, nheads = shape
+    lens = [40, 1, 900, 130]
+    a = [t.cuda() for t in args_of(scan_inputs(sum(lens), D, N, G, nheads, io, 27))]
+    pool = gpu_state(pool_inputs(4, D, N, G, nheads, io, 28))
+
+    def odd(t):
+        raw = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")
+        raw[1:] = t.flatten()
+        return raw[1:].view(t.shape)
+
+    results = []
+    for move in (torch.clone, odd):
+        for flags in (0, WALK):
+            state = ops.Mamba3State(pool.h.clone(), pool.phase.clone(), move(pool.x_prev), move(pool.b_prev))
+            y = ops.mamba3_prefill(*a, cu_of(lens), state, go_on=torch.ones(4, dtype=torch.bool, device="cuda"), nheads=nheads, flags=flags)
+            y1 = ops.mamba3_decode_step(state, *(t if i == 4 else t[:4].contiguous() for i, t in enumerate(a)), nheads=nheads)
+            results.append([y, y1, *state])
+    for got, want in zip(results[2:], results[:2]):
+        assert all(torch.equal(t, u) for t, u in zip(got, want))
+
+
 def test_a_layer_serves_prompts_then_tokens():
     """The operators as a layer uses them: prompts through norm, projections, convolution, scan and gate, then five tokens
     each; the same rows in one go by the oracle in float64."""
