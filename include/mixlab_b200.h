@@ -334,6 +334,7 @@ MXB_API mxb_status mxb_mamba3_block_post_bwd(const mxb_mamba3_desc* d, float eps
  * token; that of a sequence without tokens stays as it was.  Rows of y that belong to no
  * sequence stay as they were.
  * decode_step: one token of each of S sequences (rows = S), all of which go on.
+ * y shares no memory with an operand or the pool; that of decode_step may be x itself.
  *
  * desc: D channels, N states (even, <= 256), G groups; nheads > 0: head layout (dt, lambda,
  * theta [rows, nheads], a_log [nheads]; nheads a multiple of G, D of nheads), 0: per-channel
@@ -366,8 +367,8 @@ MXB_API mxb_status mxb_mamba3_decode_step(const mxb_mamba3_serve_desc* d, const 
  * pool of the last inputs, conv_state [slots, K-1, D] in io_dtype, oldest first:
  *   y_t = act(sum_k w[:, k] x_{t-k} + bias)
  * w(d, k) = w[d w_stride_d + k w_stride_k] float32, so that both blocks' weights ([D, K] and
- * [K, D]) serve as they are; bias [D] may be NULL.  K <= 4.  cu_seqlens, slot, go_on and their
- * rules as above. */
+ * [K, D]) serve as they are; bias [D] may be NULL.  K <= 4.  cu_seqlens, slot, go_on, y and
+ * their rules as above. */
 enum { MXB_ACT_NONE = 0, MXB_ACT_SILU = 1 };
 typedef struct {
   int32_t rows, S, slots, D, K, io_dtype, activation;

@@ -85,6 +85,28 @@ void check(const Opt& t, Shape shape, at::ScalarType dtype, at::Device dev, cons
   if (t) check(*t, shape, dtype, dev, name);
 }
 
+// `out` shares no memory with what the call reads or updates besides: a prompt's rows are read again after rows of the result are
+// written, by other CTAs too.  `itself`: the one that it may be as a whole (a token's inputs are read before its results are written).
+struct Named {
+  const Tensor* t;  // may be null
+  const char* name;
+};
+const Tensor* at_of(const Opt& t) { return t ? &*t : nullptr; }
+void check_apart(const Tensor& out, const Tensor* itself, std::initializer_list<Named> others) {
+  auto range = [](const Tensor& t) {
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    const char* from = static_cast<const char*>(t.data_ptr());
+    return std::make_pair(from, t.numel() ? from + (last + 1) * (int64_t)t.element_size() : from);
+  };
+  const auto a = range(out);
+  for (const Named& o : others) {
+    if (!o.t) continue;
+    const auto b = range(*o.t);
+    if (a.first < b.second && b.first < a.second && !(o.t == itself && a == b)) throw py::value_error(std::string("out: overlaps ") + o.name);
+  }
+}
+
 template <typename T = void>
 T* ptr(const Tensor& t) { return static_cast<T*>(t.data_ptr()); }
 template <typename T = void>
@@ -647,6 +669,11 @@ ServeCall check_serve(at::Device dev, const std::vector<Tensor>& state, const Te
   check(state[3], bs, io, dev, "state.b_prev");
   check(out, x.sizes(), io, dev, "out");
   check_pool_rows(r, dev);
+  if (out)
+    check_apart(*out, r.cu ? nullptr : &x,
+                {{&x, "x"}, {&dt, "dt"}, {&lam, "lambda"}, {&theta, "theta"}, {&a_log, "a_log"}, {&b, "b"}, {&c, "c"}, {&state[0], "state.h"},
+                 {&state[1], "state.phase"}, {&state[2], "state.x_prev"}, {&state[3], "state.b_prev"}, {at_of(r.cu), "cu_seqlens"},
+                 {at_of(r.slot), "slots"}, {at_of(r.go_on), "go_on"}});
   return {d, {ptr<float>(state[0]), ptr<float>(state[1]), ptr(state[2]), ptr(state[3])}};
 }
 int64_t pool_size(const std::vector<Tensor>& state) {
@@ -698,6 +725,9 @@ mxb_short_conv_desc check_short_conv(at::Device dev, const Tensor& state, const 
   check(bias, Shape(&D, 1), F, dev, "bias");
   check(out, x.sizes(), io, dev, "out");
   check_pool_rows(r, dev);
+  if (out)
+    check_apart(*out, r.cu ? nullptr : &x,
+                {{&x, "x"}, {&w, "w"}, {at_of(bias), "bias"}, {&state, "conv_state"}, {at_of(r.cu), "cu_seqlens"}, {at_of(r.slot), "slots"}, {at_of(r.go_on), "go_on"}});
   return {(int32_t)x.size(0), (int32_t)r.S, (int32_t)r.slots, (int32_t)D, (int32_t)K, io_code(x), activation ? MXB_ACT_SILU : MXB_ACT_NONE, w.stride(0), w.stride(1)};
 }
 Tensor short_conv_prefill(const Tensor& x, const Tensor& w, const Tensor& cu, const Tensor& state, const Opt& slots, const Opt& go_on,

@@ -192,14 +192,15 @@ def mamba3_prefill(x, dt, lam, theta, a_log, b, c, cu_seqlens, state, *, slots=N
     sequences' rows of ``state`` (None: 0, 1, ...; all different), are int32; go_on [S] bool tells which sequences go on
     from their state (None: none), the others start from nothing.  Returns y [rows,D]; ``state`` then holds what
     ``mamba3_decode_step`` or the next part of a prompt goes on from.  A sequence without tokens keeps its state; one whose slot
-    is negative or beyond the pool starts from nothing and keeps none; rows of no sequence are not written."""
+    is negative or beyond the pool starts from nothing and keeps none; rows of no sequence are not written.  ``out`` must not
+    overlap an operand or the state."""
     return (_front or _native()).mamba3_prefill(x, dt, lam, theta, a_log, b, c, cu_seqlens, list(state), slots, go_on, nheads, out, flags)
 
 
 def mamba3_decode_step(state, x, dt, lam, theta, a_log, b, c, *, slots=None, nheads=0, out=None):
     """One token of each of S sequences on ``state`` (updated in place): x [S,D], b, c [S,G,N], the others with S rows.  slots
     [S] int32, all different (None: 0, 1, ...); a row whose slot is negative or beyond the pool is passed over and its row of
-    the result not written.  Returns y [S,D]."""
+    the result not written.  Returns y [S,D]; ``out`` may be x itself, and must not overlap an operand or the state otherwise."""
     return (_front or _native()).mamba3_decode_step(list(state), x, dt, lam, theta, a_log, b, c, slots, nheads, out)
 
 
@@ -207,12 +208,13 @@ def short_conv_prefill(x, w, cu_seqlens, conv_state, *, slots=None, go_on=None, 
     """Causal depthwise convolution of packed prompts: y_t = act(sum_k w[:,k] x_{t-k} + bias), x [rows,D], w [D,K] float32 of any
     strides (a gated_deltanet block's [K,D] weights as ``conv.t()``), K <= 4, activation None or "silu".  conv_state
     [slots,K-1,D], in x's type, holds each sequence's last K-1 inputs, oldest first: read where go_on, then written.
-    cu_seqlens, slots and go_on as for ``mamba3_prefill``."""
+    cu_seqlens, slots, go_on and out as for ``mamba3_prefill``."""
     return (_front or _native()).short_conv_prefill(x, w, cu_seqlens, conv_state, slots, go_on, bias, activation, out)
 
 
 def short_conv_step(conv_state, x, w, *, slots=None, bias=None, activation=None, out=None):
-    """``short_conv_prefill`` for one token of each of S sequences, all of which go on: x [S,D] -> y [S,D]."""
+    """``short_conv_prefill`` for one token of each of S sequences, all of which go on: x [S,D] -> y [S,D].  ``out`` may be x
+    itself."""
     return (_front or _native()).short_conv_step(conv_state, x, w, slots, bias, activation, out)
 
 

@@ -495,3 +495,41 @@ def test_refusals():
             ops.short_conv_prefill(a[0], torch.zeros(D, 4).cuda(), cu, conv, **kw)
     with pytest.raises(_lib.MxbError):
         ops.short_conv_step(torch.zeros(8, 4, D, dtype=BF16).cuda(), a[0], torch.zeros(D, 5).cuda())
+
+
+@pytest.mark.parametrize("io", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(128, 64, 2, 2), (64, 16, 1, 0)], ids=str)
+def test_results_on_top_of_operands(shape, io):
+    """A prompt's result anywhere on an operand or the state is refused, a token's too, but for x as a whole: that gives what a
+    result of its own gives."""
+    D, N, G, nheads = shape
+    a = [t.cuda() for t in args_of(scan_inputs(40, D, N, G, nheads, io, 29))]
+    cu, w = cu_of([40]), torch.randn(D, 3).cuda()
+    new = lambda: ops.mamba3_state(40, D, N, G, nheads=nheads, dtype=io)  # noqa: E731
+    conv = lambda: torch.ones(40, 2, D, dtype=io).cuda()  # noqa: E731
+    s, k = new(), conv()
+    raw = torch.randn(41 * D + 1, generator=torch.Generator().manual_seed(30)).to(io).cuda()
+    x, apart = raw[:40 * D].view(40, D), torch.empty(40, D, dtype=io, device="cuda")
+    tops = [raw[o:o + 40 * D].view(40, D) for o in (1, D)] + [t.flatten()[:40 * D].view(40, D) for t in (s.x_prev,)]
+    if io == F32:
+        tops += [s.h.flatten()[:40 * D].view(40, D)]
+    for out in tops + [x]:
+        with pytest.raises(ValueError, match="out: overlaps"):
+            ops.mamba3_prefill(x, *a[1:], cu, s, nheads=nheads, out=out)
+        if out is x:
+            break
+        with pytest.raises(ValueError, match="out: overlaps"):
+            ops.mamba3_decode_step(s, x, *a[1:], nheads=nheads, out=out)
+    for out in tops[:2] + [k[:20].view(40, D), x]:
+        with pytest.raises(ValueError, match="out: overlaps"):
+            ops.short_conv_prefill(x, w, cu, k, out=out)
+        if out is x:
+            break
+        with pytest.raises(ValueError, match="out: overlaps"):
+            ops.short_conv_step(k, x, w, out=out)
+    ops.mamba3_prefill(raw[D + 1:].view(40, D), *a[1:], cu, s, nheads=nheads, out=apart)  # (beside each other)
+    want = ops.mamba3_decode_step(new(), x, *a[1:], nheads=nheads), ops.short_conv_step(conv(), x, w)
+    y = x.clone()
+    assert torch.equal(ops.mamba3_decode_step(new(), y, *a[1:], nheads=nheads, out=y), want[0])
+    y = x.clone()
+    assert torch.equal(ops.short_conv_step(conv(), y, w, out=y), want[1])
