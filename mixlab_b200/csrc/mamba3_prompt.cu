@@ -732,10 +732,16 @@ static mxb_status launch(const ServeP& p, bool ends, cudaStream_t st) {
 
 }  // namespace m3p
 
-// Whole 16-byte pieces of rows, a state that fits the registers of four warps, and more rows than the walk makes ready at once:
-// one prompt of 16 rows of 32 heads 23 us by the walk, of 17 rows 24 by the chunks and 25 by the walk, of 64 rows 26 and 45, of
-// 512 rows 48 and 83 (timer and cold caches included); 16 prompts of 2048 rows 376 and 2491.
-bool m3prompt_shape(const ServeP& p, bool f32) { return !f32 && p.NH > 0 && p.N % 8 == 0 && p.N <= 128 && p.P % 8 == 0 && p.rows > 16; }
+// Whole 16-byte pieces of rows, a state that fits the registers of four warps, and rows enough for chunks of 64 to be worth
+// it: more than 16 in the call and more than 4 a sequence (the host knows their mean only).  us, chunks / walk, 128 states:
+//   one prompt of 16 rows, 32 heads          14 / 14     of 24 rows 17 / 18     of 64 rows 17 / 35
+//   256 prompts of 32 heads, 1 row each     437 / 290    4 rows 438 / 328       8 rows 439 / 378    16 rows 440 / 476
+//   64 prompts of 8 heads, 1 row each        35 / 20     4 rows  40 / 26        8 rows  40 / 30     24 rows  41 / 48
+// Tokens beside one prompt are what the line is not drawn further out for: 8 heads, 255 of them beside 512 rows (3 a sequence)
+// 138 / 127, 63 beside 256 rows (5 a sequence) 48 / 72, 15 beside 128 (9 a sequence) 30 / 53.
+static bool m3prompt_shape(const ServeP& p, bool f32) {
+  return !f32 && p.NH > 0 && p.N % 8 == 0 && p.N <= 128 && p.P % 8 == 0 && p.rows > 16 && p.rows > 4 * (long long)p.S;
+}
 bool m3prompt_supported(const ServeP& p, bool f32) {
   auto al = [](const void* q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };
   return m3prompt_shape(p, f32) && al(p.x) && al(p.b) && al(p.c) && reinterpret_cast<uintptr_t>(p.y) % 4 == 0;

@@ -165,7 +165,6 @@ __device__ __forceinline__ void serve_tail(const ServeP& p, int row, int slot, i
 }
 
 mxb_status m3serve_step(const ServeP& p, bool f32, cudaStream_t st);
-bool m3prompt_shape(const ServeP& p, bool f32);
 bool m3prompt_supported(const ServeP& p, bool f32);
 mxb_status m3prompt_prepare(const ServeP& p, cudaStream_t st);
 mxb_status m3prompt_chunks(const ServeP& p, bool ends, cudaStream_t st);

@@ -6,6 +6,7 @@ Tolerances, relative in the 2-norm and in the largest element.  float32 results:
 the rounding of y itself and, on the tensor-core kernels, one each of the weights and of the state that y is read from, each at
 most half a step, 2^-8: together at most 3 x 2^-8 = 1.2e-2.  States are float32 whatever the inputs' type and keep the float32
 bound; x_prev and b_prev are copies."""
+import ctypes as C
 import math
 
 import pytest
@@ -533,3 +534,28 @@ def test_results_on_top_of_operands(shape, io):
     assert torch.equal(ops.mamba3_decode_step(new(), y, *a[1:], nheads=nheads, out=y), want[0])
     y = x.clone()
     assert torch.equal(ops.short_conv_step(conv(), y, w, out=y), want[1])
+
+
+@pytest.mark.parametrize("lens,chunks", [([16], False), ([17], True), ([1] * 64, False), ([4] * 64, False), ([5] * 64, True), ([1] * 63 + [512], True),
+                                         ([64] * 16, True)], ids=["16", "17", "64 of 1", "64 of 4", "64 of 5", "63 of 1 and one of 512", "16 of 64"])
+def test_short_prompts_go_step_by_step(lens, chunks):
+    """bf16 prompts of few rows each go step by step, where only y is rounded (half a step of bf16, and the float32 bound beside it);
+    the others in chunks."""
+    D, N, G, nheads, S = 128, 64, 1, 2, len(lens)
+    a = scan_inputs(sum(lens), D, N, G, nheads, BF16, 31)
+    pool = pool_inputs(S, D, N, G, nheads, BF16, 32)
+    want = list(double(pool))
+    y_want = serving.mamba3_prefill(want, *double(args_of(a)), lens, list(range(S)), [True] * S, nheads)
+    state, lib = gpu_state(pool), _lib.lib()
+    args = [t.cuda() for t in args_of(a)], cu_of(lens), torch.ones(S, dtype=torch.bool, device="cuda")
+    lib.mxb_trace_enable(1)
+    y = ops.mamba3_prefill(*args[0], args[1], state, go_on=args[2], nheads=nheads)
+    torch.cuda.synchronize()
+    buf = C.create_string_buffer(4096)
+    lib.mxb_trace_summary(buf, len(buf))
+    lib.mxb_trace_enable(0)
+    assert (b"m3p_chunks_kernel" in buf.value) == chunks and (b"m3k_heads_kernel" in buf.value) != chunks, buf.value
+    if not chunks:
+        assert bool(((y.cpu().double() - y_want).abs() <= 2.0 ** -8 * y_want.abs() + TOL[F32] * y_want.abs().max()).all())
+    assert_close(y.cpu(), y_want, TOL[BF16])
+    check_state(state, want, BF16, 2 * TOL[F32], list(range(S)))
