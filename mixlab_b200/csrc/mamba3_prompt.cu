@@ -696,10 +696,9 @@ __global__ void __launch_bounds__(2 * kThreads, 2) m3p_chunks_kernel(ServeP p) {
       if (rows_in[k] && 8 * t < p.N)
         *reinterpret_cast<float2*>(to + (size_t)8 * k * p.N + 8 * t) = m3_on(make_float2(h[t][2 * k], h[t][2 * k + 1]), by);
   // (the slabs of a head all read its phase and b_prev; with more than one they are written behind this launch)
-  if (!ENDS && p.slabs == 1) {  // (every thread has read them: barriers lie between)
-    if (tid == 0) p.phase[ph] = m3_turned(start, ran);
-    serve_tail<bf16>(p, q.end - 1, slot, hd, grp, kThreads);
-  }
+  // (every thread has read them: barriers lie between)
+  if (!ENDS && tid == 0 && slab == 0) *serve_phase_end(p, q.seq, ph, hd) = m3_turned(start, ran);
+  if (!ENDS && p.slabs == 1) serve_tail<bf16>(p, q.end - 1, slot, hd, grp, kThreads);
 }
 
 // The split of the registers waits for good where the kernel starts with fewer than it counts on: looked up once.

@@ -28,6 +28,7 @@ struct ServeP {
   float* spoil;     // [pieces, D Kp]: NaN where the segment's angle is not finite, 0 elsewhere (channel layout)
   float2* start;    // [pieces, NH]: cosine and sine of the angle that the segment starts at (head layout)
   int slabs;        // head layout: CTAs that share a head's channels
+  float2* phase_end;  // [S, NH]: with several slabs, the phase behind a sequence's last step (into the pool with its last row)
   // chunks on the tensor cores (mamba3_prompt.cu)
   int chunks;       // at most: ceil(length / 64) of every sequence
   float* scores;    // [chunks, G, 10 tiles, 2, 32 lanes, 8]
@@ -145,6 +146,11 @@ __device__ __forceinline__ int serve_slot(const ServeP& p, int seq) {
   return s >= 0 && s < p.slots ? s : -1;
 }
 __device__ __forceinline__ bool serve_goes_on(const ServeP& p, int seq) { return p.go && __ldg(p.go + seq); }
+
+// Where the phase behind a sequence's last step goes; ph: its place in the pool.
+__device__ __forceinline__ float2* serve_phase_end(const ServeP& p, int seq, size_t ph, int hd) {
+  return p.slabs > 1 ? p.phase_end + (size_t)seq * p.NH + hd : p.phase + ph;
+}
 
 // (1 - lambda) dt of row t + 1, which weighs row t's outer product there; 0 behind the sequence's last row.
 __device__ __forceinline__ float serve_look(const ServeP& p, size_t at, bool in) {

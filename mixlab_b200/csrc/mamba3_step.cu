@@ -211,7 +211,8 @@ __global__ void __launch_bounds__(256) m3s_step_channels_kernel(ServeP p, int LN
   }
 }
 
-// The last token of every sequence into the pool: x too, or only b.  grid: sequences.
+// The last token of every sequence into the pool: x too, or only b; and the phase, where a head's slabs have left it beside the
+// pool.  grid: sequences.
 template <typename IO>
 __global__ void __launch_bounds__(256) m3s_tails_kernel(ServeP p, int x_too) {
   begin_dependent();
@@ -227,6 +228,8 @@ __global__ void __launch_bounds__(256) m3s_tails_kernel(ServeP p, int x_too) {
   const IO* B = static_cast<const IO*>(p.b) + row * p.G * p.N;
   IO* BP = static_cast<IO*>(p.b_prev) + (size_t)slot * copies * p.N;
   for (int i = threadIdx.x; i < copies * p.N; i += 256) BP[i] = B[(i / p.N / rep) * p.N + i % p.N];
+  if (p.phase_end)
+    for (int i = threadIdx.x; i < p.NH; i += 256) p.phase[(size_t)slot * p.NH + i] = p.phase_end[(size_t)seq * p.NH + i];
   if (x_too)
     for (int i = threadIdx.x; i < p.D; i += 256) static_cast<IO*>(p.x_prev)[(size_t)slot * p.D + i] = static_cast<const IO*>(p.x)[row * p.D + i];
 }

@@ -237,10 +237,8 @@ __global__ void __launch_bounds__(256) m3k_heads_kernel(ServeP p, int LN) {
         else *reinterpret_cast<float2*>(p.h + ((size_t)slot * p.D + chan + row) * p.N + n) = m3_back(v, start);
       }
   // (the slabs of a head all read its phase and b_prev; with more than one they are written behind this launch)
-  if (MODE == kOut && p.slabs == 1) {
-    if (tid == 0) p.phase[ph] = m3_turned(start, ran);
-    serve_tail<IO>(p, q.end - 1, slot, hd, g, 256);
-  }
+  if (MODE == kOut && tid == 0 && slab == 0) *serve_phase_end(p, q.seq, ph, hd) = m3_turned(start, ran);
+  if (MODE == kOut && p.slabs == 1) serve_tail<IO>(p, q.end - 1, slot, hd, g, 256);
 }
 
 // What the segments of a sequence start from.  grid (sequences that can be longer than L, blocks of pairs): a thread per state pair of the channels walks
@@ -295,35 +293,6 @@ __global__ void __launch_bounds__(256) m3k_heads_chain_kernel(ServeP p, bool bf1
       e += kAhead * pairs;
     }
   }
-}
-// The phase at a sequence's end where the heads are cut into slabs: summed again from dt theta.  grid (sequences, heads) x 256.
-__global__ void __launch_bounds__(256) m3k_heads_phase_kernel(ServeP p) {
-  begin_dependent();
-  __shared__ int s_turn[8];
-  __shared__ float s_taint[8];
-  const int seq = blockIdx.x, hd = blockIdx.y, slot = serve_slot(p, seq);
-  if (slot < 0) return;
-  const int a = min(max(p.cu[seq], 0), p.rows), e = min(max(p.cu[seq + 1], a), p.rows);
-  if (a == e) return;
-  int turn = 0;
-  float taint = 0.f;
-  for (int t = a + threadIdx.x; t < e; t += 256) {
-    const size_t at = (size_t)t * p.NH + hd;
-    const float dt = m3_softplus(p.dt[at]), theta = p.theta[at];
-    turn += m3_turn(dt, theta);
-    taint = m3_taint(dt * theta, taint);
-  }
-  turn = warp_sum(turn);
-  taint = warp_sum(taint);
-  if ((threadIdx.x & 31) == 0) { s_turn[threadIdx.x >> 5] = turn; s_taint[threadIdx.x >> 5] = taint; }
-  __syncthreads();
-  if (threadIdx.x) return;
-  turn = 0;
-  taint = 0.f;
-  for (int w = 0; w < 8; ++w) { turn += s_turn[w]; taint += s_taint[w]; }
-  const size_t ph = (size_t)slot * p.NH + hd;
-  const float2 from = serve_goes_on(p, seq) ? p.phase[ph] : make_float2(1.f, 0.f);
-  p.phase[ph] = m3_turned(from, m3_unit(turn, taint));
 }
 
 // ------------------------------------------------------------------ channels
@@ -839,7 +808,6 @@ static mxb_status prefill(ServeP p, bool chunks, cudaStream_t st) {
     if (!chunks) heads<IO, kOut>(p, st);
     else if (const mxb_status s = m3prompt_chunks(p, false, st); s != MXB_OK) return s;
     if (p.slabs == 1) return check_launch("m3k_prefill");
-    MXB_LAUNCH("m3k_heads_phase_kernel", st, (launch_kernel(m3k_heads_phase_kernel, dim3(p.S, p.NH), 256, 0, st, p)));
   } else {
     if (cut) {
       if (const mxb_status s = channels<IO, kEnds>(p, st); s != MXB_OK) return s;
@@ -877,6 +845,7 @@ size_t m3walk_scratch(ServeP& p, bool f32, int flags, char* base) {
     p.rec = c.take<float>((size_t)p.chunks * p.NH * 512);
     p.scores = c.take<float>((size_t)p.chunks * p.G * 10 * 512);
   }
+  if (p.NH && m3k::serve_slabs(p) > 1) p.phase_end = c.take<float2>((size_t)p.S * p.NH);
   p.pieces = p.S;
   if (p.rows <= p.L) return c.bytes();
   p.pieces = (p.rows + p.L - 1) / p.L + p.S;

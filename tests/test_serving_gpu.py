@@ -559,3 +559,44 @@ def test_short_prompts_go_step_by_step(lens, chunks):
         assert bool(((y.cpu().double() - y_want).abs() <= 2.0 ** -8 * y_want.abs() + TOL[F32] * y_want.abs().max()).all())
     assert_close(y.cpu(), y_want, TOL[BF16])
     check_state(state, want, BF16, 2 * TOL[F32], list(range(S)))
+
+
+@pytest.mark.parametrize("D", [64, 128, 320], ids=lambda D: f"head of {D}")
+def test_angle_of_a_long_prompt(D):
+    """The phase behind 16384 bf16 steps that all turn the same way, by 8 radians each, whole and in two parts, for heads of one,
+    two and five slabs.  Each step is rounded to half of 2^-32 turns, 16384 x 2^-33 x 2 pi = 1.2e-5 in all; the phase goes through at
+    most 148 segments' products of unit vectors, off by at most four roundings of 2^-24 each: 3.6e-5."""
+    T, N = 16384, 16
+    a = scan_inputs(T, D, N, 1, 1, BF16, 33)
+    a["dt"].fill_(2.5)
+    a["theta"].fill_(3.1)
+    angle = (T * torch.nn.functional.softplus(a["dt"][0].double()) * a["theta"][0].double()).item()
+    want = torch.tensor([math.cos(angle), math.sin(angle)], dtype=torch.float64)
+    dev = [t.cuda() for t in args_of(a)]
+    for cuts in ((0, T), (0, 7001, T)):
+        state = ops.mamba3_state(1, D, N, 1, nheads=1)
+        for lo, hi in zip(cuts, cuts[1:]):
+            ops.mamba3_prefill(*(t if i == 4 else t[lo:hi].contiguous() for i, t in enumerate(dev)), cu_of([hi - lo]), state, nheads=1,
+                               go_on=torch.tensor([lo > 0]).cuda())
+        assert (state.phase.cpu().double() - want).abs().max() <= 1.2e-5 + 3.6e-5
+
+
+@pytest.mark.parametrize("shape", [(128, 64, 1, 1), (160, 128, 1, 1), (320, 32, 2, 2), (130, 6, 1, 1)], ids=str)
+@pytest.mark.parametrize("io", [F32, BF16], ids=["f32", "bf16"])
+def test_wide_heads_of_cut_sequences(shape, io):
+    """Heads of more than 64 channels (several CTAs a head) whose sequences are cut in segments, beside others; a padding entry."""
+    D, N, G, nheads = shape
+    lens, slots = [5, 700, 0, 391, 64, 200], [3, 0, 2, 1, 5, -1]
+    a = scan_inputs(sum(lens), D, N, G, nheads, io, 34)
+    pool = pool_inputs(6, D, N, G, nheads, io, 35)
+    go_on = [True, True, True, False, True, True]
+    want = list(double(pool))
+    y_want = serving.mamba3_prefill(want, *double(args_of(a)), lens, slots, go_on, nheads)
+    for flags in (0, WALK, WALK | SERIAL):
+        state = gpu_state(pool)
+        y = ops.mamba3_prefill(*(t.cuda() for t in args_of(a)), cu_of(lens), state, slots=torch.tensor(slots).int().cuda(),
+                               go_on=torch.tensor(go_on).cuda(), nheads=nheads, flags=flags)
+        assert_close(y.cpu(), y_want, TOL[io], f"y flags {flags}")
+        check_state(state, want, io, 2 * TOL[F32], [0, 1, 3, 5])  # (700 steps: the bound of the angles grows with them)
+        for t, w in zip(state, pool):
+            assert torch.equal(t[[2, 4]].cpu(), w[[2, 4]])
