@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(2 * kThreads, 2) m3p_chunks_kernel(ServeP p) {
   const int per = p.NH * p.slabs, hd = blockIdx.x % per / p.slabs, slab = blockIdx.x % p.slabs;  // (heads first)
   const Piece q = find_piece<ENDS ? kInner : kPieces>(p, blockIdx.x / per, p.L);
   const int piece = q.base + q.seg;
-  if (!q.ok || piece >= p.pieces) return;
+  if (!q.ok || !cut_fits(p, q)) return;
   const int chunks = (q.last - q.first + Q - 1) / Q;
   if (q.chunk + chunks > p.chunks) return;  // (lengths that add up to more than the rows)
   const int p0 = slab * kPS, np = min(kPS, p.P - p0);

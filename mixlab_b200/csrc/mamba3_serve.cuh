@@ -19,14 +19,14 @@ struct ServeP {
   float2* phase;            // [slots, NH] or [slots, D, Kp]: cosine and sine of the angle
   void *x_prev, *b_prev;    // [slots, D], [slots, NH or G, N]
   void* y;
-  // prompts cut into segments of L steps
-  int L, pieces;
-  float* ends;      // [pieces, D, N]: what a segment adds to the state, then the state that it starts from
-  float* dsum;      // [pieces, NH or D]: sum of dt over the segment
-  int* turn;        // [pieces, NH or D Kp]: angle of the segment in 2^-32 turns (channel layout: then the one that it starts at)
-  float* ends2;     // [pieces, D, N]: what a segment adds by the sine of the angle that it starts at (channel layout)
-  float* spoil;     // [pieces, D Kp]: NaN where the segment's angle is not finite, 0 elsewhere (channel layout)
-  float2* start;    // [pieces, NH]: cosine and sine of the angle that the segment starts at (head layout)
+  // prompts cut into segments of L steps: at most so many segments in all, and of sequences that have more than one
+  int L, pieces, cuts;
+  float* ends;      // [cuts, D, N]: what a segment adds to the state, then the state that it starts from
+  float* dsum;      // [cuts, NH or D]: sum of dt over the segment
+  int* turn;        // [cuts, NH or D Kp]: angle of the segment in 2^-32 turns (channel layout: then the one that it starts at)
+  float* ends2;     // [cuts, D, N]: what a segment adds by the sine of the angle that it starts at (channel layout)
+  float* spoil;     // [cuts, D Kp]: NaN where the segment's angle is not finite, 0 elsewhere (channel layout)
+  float2* start;    // [cuts, NH]: cosine and sine of the angle that the segment starts at (head layout)
   int slabs;        // head layout: CTAs that share a head's channels
   float2* phase_end;  // [S, NH]: with several slabs, the phase behind a sequence's last step (into the pool with its last row)
   // chunks on the tensor cores (mamba3_prompt.cu)
@@ -64,12 +64,14 @@ __device__ __forceinline__ float2 m3_turned(float2 u, float2 by) {
   return make_float2(r.x * k, r.y * k);
 }
 
-// A segment of a sequence: rows [first, last) of the sequence [begin, end); `base` is the piece of its first segment, `chunk` the
-// number of its own first chunk of 64 steps.
+// A segment of a sequence: rows [first, last) of the sequence [begin, end); `base` counts the segments of cut sequences in front of
+// its own (what ends and the arrays beside it are numbered by), `chunk` is the number of its own first chunk of 64 steps.
 struct Piece {
   int seq, seg, segs, base, first, last, begin, end, chunk;
   bool ok;
 };
+// Whether a cut sequence's segments have their places (they do not where lengths add up to more than the rows).
+__device__ __forceinline__ bool cut_fits(const ServeP& p, const Piece& q) { return q.segs == 1 || q.base + q.segs <= p.cuts; }
 // The index-th piece: sequences one after the other, each cut every L rows; up to 32 sequences by falling length, so that the
 // long ones do not start last (32 heads of 16 sequences of 440 to 4377 rows: a third off the time).  Called by whole warps, which
 // look through 32 sequences at a time and add up those in front.  Whatever cu holds, rows stay inside the call's.
@@ -89,8 +91,9 @@ __device__ __forceinline__ Piece find_piece(const ServeP& p, int index, int L) {
     return v;
   };
   auto wanted = [](int n) { return WHAT == kPieces ? n : WHAT == kInner ? max(n - 1, 0) : n > 1; };
+  auto cut = [](int n) { return n > 1 ? n : 0; };
   Piece q{};
-  int before = 0, base = 0, chunks = 0;  // wanted pieces, pieces, chunks in front
+  int before = 0, base = 0, chunks = 0;  // wanted pieces, pieces of cut sequences, chunks in front
   for (int s0 = 0; s0 < p.S; s0 += 32) {
     const int s = s0 + lane;
     int a = 0, e = 0;
@@ -102,7 +105,7 @@ __device__ __forceinline__ Piece find_piece(const ServeP& p, int index, int L) {
     const int cn = (e - a + 63) / 64, these = __reduce_add_sync(kAll, wanted(n));
     if (index >= before + these) {
       before += these;
-      base += WHAT == kPieces ? these : __reduce_add_sync(kAll, n);
+      base += __reduce_add_sync(kAll, cut(n));
       chunks += __reduce_add_sync(kAll, cn);
       continue;
     }
@@ -124,13 +127,13 @@ __device__ __forceinline__ Piece find_piece(const ServeP& p, int index, int L) {
       n = __shfl_sync(kAll, n, from);
       chunk = __shfl_sync(kAll, chunk, from);
     }
-    const int all = scan(n), mine = WHAT == kPieces ? all : scan(wanted(n));
+    const int cuts = scan(cut(n)), mine = scan(wanted(n));
     const int src = __ffs(__ballot_sync(kAll, before + mine > index)) - 1;
     q.seq = __shfl_sync(kAll, id, src);
     q.begin = __shfl_sync(kAll, a, src);
     q.end = __shfl_sync(kAll, e, src);
     q.segs = __shfl_sync(kAll, n, src);
-    q.base = (WHAT == kPieces ? before : base) + __shfl_sync(kAll, all - n, src);
+    q.base = base + __shfl_sync(kAll, cuts - cut(n), src);
     q.seg = WHAT == kCut ? 0 : index - before - __shfl_sync(kAll, mine - wanted(n), src);
     q.first = q.begin + q.seg * L;
     q.last = (int)min((long long)q.first + L, (long long)q.end);

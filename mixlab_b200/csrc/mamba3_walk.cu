@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(256) m3k_heads_kernel(ServeP p, int LN) {
   const int heads = p.NH * p.slabs, tid = threadIdx.x, hd = blockIdx.x % heads / p.slabs, slab = blockIdx.x % p.slabs;
   const Piece q = find_piece<MODE == kEnds ? kInner : kPieces>(p, blockIdx.x / heads, p.L);
   const int piece = q.base + q.seg;
-  if (!q.ok || piece >= p.pieces) return;
+  if (!q.ok || !cut_fits(p, q)) return;
   const int ln = tid % LN, rg = tid / LN, rows_at_once = 256 / LN, npad = LN * 4 * NV;
   const int per = (p.P + p.slabs - 1) / p.slabs, p0 = slab * per, np = min(per, p.P - p0);  // this CTA's channels of the head
   const size_t chan = (size_t)hd * p.P + p0;
@@ -247,7 +247,7 @@ constexpr int kAhead = 8;
 __global__ void __launch_bounds__(256) m3k_heads_chain_kernel(ServeP p, bool bf16_io) {
   begin_dependent();
   const Piece q = find_piece<kCut>(p, blockIdx.x, p.L);
-  if (!q.ok || q.base + q.segs > p.pieces) return;  // (more segments: lengths beyond the rows)
+  if (!q.ok || !cut_fits(p, q)) return;
   const int slot = serve_slot(p, q.seq);
   const bool go = slot >= 0 && serve_goes_on(p, q.seq);
   const size_t pairs = (size_t)p.D * p.Kp;
@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(128) m3k_channels_kernel(ServeP p) {
   const int d = live ? d_raw : p.D - 1;
   const Piece q = find_piece<MODE == kEnds ? kInner : kPieces>(p, blockIdx.x, p.L);
   const int piece = q.base + q.seg;
-  if (!q.ok || piece >= p.pieces) return;
+  if (!q.ok || !cut_fits(p, q)) return;
   const int slot = serve_slot(p, q.seq), g = d / (p.D / p.G);
   const bool from_state = MODE == kOut && q.segs == 1 && slot >= 0 && serve_goes_on(p, q.seq);
   const size_t sd = (size_t)(slot < 0 ? 0 : slot) * p.D + d, row = (size_t)piece * p.D + d;
@@ -656,7 +656,7 @@ __global__ void __launch_bounds__(128) m3k_channels_kernel(ServeP p) {
 __global__ void __launch_bounds__(256) m3k_channels_chain_kernel(ServeP p, bool bf16_io) {
   begin_dependent();
   const Piece q = find_piece<kCut>(p, blockIdx.x, p.L);
-  if (!q.ok || q.base + q.segs > p.pieces) return;  // (more segments: lengths beyond the rows)
+  if (!q.ok || !cut_fits(p, q)) return;
   const int slot = serve_slot(p, q.seq);
   const bool go = slot >= 0 && serve_goes_on(p, q.seq);
   const size_t pairs = (size_t)p.D * p.Kp;
@@ -710,6 +710,7 @@ __global__ void __launch_bounds__(256) m3k_channels_chain_kernel(ServeP p, bool 
 }
 
 // ------------------------------------------------------------------ host
+static int longer_than_L(const ServeP& p) { return std::min(p.S, (int)(p.rows / ((long long)p.L + 1))); }  // at most so many sequences
 static int serve_slabs(const ServeP& p) { return (p.P + kRowsMost - 1) / kRowsMost; }
 // Lanes along a row: as few as keep a row's 4 NV states (NV up to 4) in registers, for a step's sum over lanes costs a row LN's
 // logarithm in exchanges, but enough that narrow heads still give all threads a row.  (Rows of 128 states over 32 lanes: 2046 us
@@ -793,7 +794,7 @@ static mxb_status channels(const ServeP& p, cudaStream_t st) {
 template <typename IO>
 static mxb_status prefill(ServeP p, bool chunks, cudaStream_t st) {
   const size_t blocks = ((size_t)p.D * p.Kp + 255) / 256;
-  const int cuts = std::max(std::min(p.S, (int)(p.rows / ((long long)p.L + 1))), 1);  // sequences that can be longer than L
+  const int cuts = std::max(longer_than_L(p), 1);
   const dim3 chain(cuts, (unsigned)std::min<size_t>(blocks, std::max<size_t>(148 * 4 / cuts, 1)));
   const bool cut = p.ends != nullptr;
   if (p.NH) {
@@ -848,14 +849,16 @@ size_t m3walk_scratch(ServeP& p, bool f32, int flags, char* base) {
   if (p.NH && m3k::serve_slabs(p) > 1) p.phase_end = c.take<float2>((size_t)p.S * p.NH);
   p.pieces = p.S;
   if (p.rows <= p.L) return c.bytes();
-  p.pieces = (p.rows + p.L - 1) / p.L + p.S;
-  p.ends = c.take<float>((size_t)p.pieces * p.D * p.N);
-  p.dsum = c.take<float>((size_t)p.pieces * (p.NH ? p.NH : p.D));
-  p.turn = c.take<int>((size_t)p.pieces * (p.NH ? p.NH : (size_t)p.D * p.Kp));
-  if (p.NH) p.start = c.take<float2>((size_t)p.pieces * p.NH);
+  // (a sequence's segments but the last are L rows each)
+  p.cuts = p.rows / p.L + m3k::longer_than_L(p);
+  p.pieces = p.rows / p.L + p.S;
+  p.ends = c.take<float>((size_t)p.cuts * p.D * p.N);
+  p.dsum = c.take<float>((size_t)p.cuts * (p.NH ? p.NH : p.D));
+  p.turn = c.take<int>((size_t)p.cuts * (p.NH ? p.NH : (size_t)p.D * p.Kp));
+  if (p.NH) p.start = c.take<float2>((size_t)p.cuts * p.NH);
   else {
-    p.ends2 = c.take<float>((size_t)p.pieces * p.D * p.N);
-    p.spoil = c.take<float>((size_t)p.pieces * p.D * p.Kp);
+    p.ends2 = c.take<float>((size_t)p.cuts * p.D * p.N);
+    p.spoil = c.take<float>((size_t)p.cuts * p.D * p.Kp);
   }
   return c.bytes();
 }

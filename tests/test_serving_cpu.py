@@ -90,3 +90,17 @@ def test_oracle_is_the_scan(nheads):
     w, pool = r(D, 3), torch.zeros(1, 2, D, dtype=torch.float64)
     parts = [serving.short_conv(pool, x[q], w, None, [len(x[q])], [0], [i > 0], False) for i, q in enumerate((slice(0, 1), slice(1, T)))]
     assert torch.allclose(torch.cat(parts), mamba3_block.depthwise_conv(x[None], w)[0])
+
+
+@pytest.mark.parametrize("nheads,D,N", [(32, 2048, 128), (0, 448, 16), (2, 256, 64)])
+def test_scratch_of_many_sequences(nheads, D, N):
+    """What a cut needs goes by the sequences that can be longer than a segment, not by all: many short ones beside a long one
+    take no state's room each.  (Step by step: nothing; in chunks their scores and scalars, a chunk's 2 KB a head and 20 KB; heads
+    of several slabs 8 bytes each.)"""
+    need = lambda S, flags: mixlab_b200.lib().mxb_mamba3_prefill_workspace_bytes(  # noqa: E731
+        C.byref(_serve(rows=32768, S=S, slots=S, D=D, N=N, nheads=nheads, flags=flags)))
+    walk = _lib.MXB_MAMBA3_RECURRENT_KERNELS
+    small, large = 512, 4096  # (more than the segments that there can be)
+    assert need(small, walk) > D * N * 4  # a cut it is
+    assert need(large, walk) - need(small, walk) <= 8 * nheads * (large - small) * (nheads > 0 and D // nheads > 64) + 256
+    assert need(large, 0) - need(small, 0) <= (2048 * nheads + 20480 + 8 * nheads) * (large - small) + 1024
