@@ -173,10 +173,13 @@ __global__ void __launch_bounds__(kThreads) m3p_prepare_kernel(ServeP p) {
     looks[k] = next ? (1.f - m3_sigmoid(in_[1][i + 1][c])) * m3_softplus(in_[0][i + 1][c]) : 0.f;
     rates[k] = -expf(p.a_log[min(h0 + c, p.NH - 1)]) * 1.4426950408889634f;
   }
-  float l[K2], r[K2], own[K2], ds[K2];
+  // A step's decay, in powers of two.  Beyond 2^-160, which is 0 as a float32, it counts as that: what follows such a step is
+  // weighed by differences of the sums from the chunk's start on, which a step of some thousands would leave few bits.
+  float l[K2], r[K2], ds[K2];
 #pragma unroll
   for (int k = 0; k < K2; ++k) {
-    own[k] = l[k] = r[k] = dts[k] * rates[k];
+    const float fall = in ? dts[k] * rates[k] : 0.f;
+    l[k] = r[k] = fall < -160.f ? -160.f : fall;
     ds[k] = dts[k];
   }
 #pragma unroll
@@ -193,6 +196,8 @@ __global__ void __launch_bounds__(kThreads) m3p_prepare_kernel(ServeP p) {
   for (int k = 0; k < K2; ++k) {
     if (lane == 31) { s_turn[k][w] = turns[k]; s_taint[k][w] = taints[k]; s_l[k][w] = l[k]; s_ds[k][w] = ds[k]; }
     if (lane == 0) s_r[k][w] = r[k];
+    const float behind = __shfl_down_sync(0xffffffffu, r[k], 1);
+    r[k] = lane < 31 ? behind : 0.f;  // of the steps behind this one
   }
   __syncthreads();
   const int w0 = w & 2;
@@ -203,7 +208,7 @@ __global__ void __launch_bounds__(kThreads) m3p_prepare_kernel(ServeP p) {
     if (w & 1) { turns[k] += s_turn[k][w0]; taints[k] += s_taint[k][w0]; l[k] += s_l[k][w0]; }
     else r[k] += s_r[k][w + 1];
     Rec* rec = reinterpret_cast<Rec*>(p.rec) + (size_t)blockIdx.x * p.NH + hd;
-    const float e = gammas[k] + looks[k], g = e * exp2f(r[k] - own[k]);  // (r: from the sum behind row j)
+    const float e = gammas[k] + looks[k], g = e * exp2f(r[k]);
     const float2 unit = m3_unit(turns[k], taints[k]);
     rec->co[i] = unit.x;
     rec->si[i] = unit.y;

@@ -600,3 +600,24 @@ def test_wide_heads_of_cut_sequences(shape, io):
         check_state(state, want, io, 2 * TOL[F32], [0, 1, 3, 5])  # (700 steps: the bound of the angles grows with them)
         for t, w in zip(state, pool):
             assert torch.equal(t[[2, 4]].cpu(), w[[2, 4]])
+
+
+@pytest.mark.parametrize("raw", [200.0, 3e5])
+@pytest.mark.parametrize("io", [F32, BF16], ids=["f32", "bf16"])
+def test_steps_that_forget_everything(io, raw):
+    """Steps with a decay of thousands and millions of powers of two, among slow ones: what follows them is as exact as elsewhere."""
+    D, N, G, nheads, lens = 128, 64, 1, 2, [150, 70]
+    a = scan_inputs(sum(lens), D, N, G, nheads, io, 36)
+    a["dt"] -= 4.0
+    a["a_log"].fill_(math.log(16.0))
+    steps = [20, 100, 150 + 33]
+    a["dt"][steps] = raw
+    want = list(double(pool_inputs(2, D, N, G, nheads, io, 37)))
+    pool = [t.float() for t in want]
+    y_want = serving.mamba3_prefill(want, *double(args_of(a)), lens, [0, 1], [True, True], nheads)
+    for flags in (0, WALK):
+        state = gpu_state([t.to(w.dtype) for t, w in zip(pool, (torch.zeros((), dtype=F32), torch.zeros((), dtype=F32), a["x"], a["x"]))])
+        y = ops.mamba3_prefill(*(t.cuda() for t in args_of(a)), cu_of(lens), state, go_on=torch.ones(2, dtype=torch.bool, device="cuda"), nheads=nheads, flags=flags)
+        for lo, hi in zip([0] + steps, steps + [sum(lens)]):
+            assert_close(y[lo:hi].cpu(), y_want[lo:hi], TOL[io], f"rows {lo} to {hi}, flags {flags}")
+        check_state(state, want, io, TOL[F32], [0, 1])
