@@ -339,9 +339,11 @@ MXB_API mxb_status mxb_mamba3_block_post_bwd(const mxb_mamba3_desc* d, float eps
  * desc: D channels, N states (even, <= 256), G groups; nheads > 0: head layout (dt, lambda,
  * theta [rows, nheads], a_log [nheads]; nheads a multiple of G, D of nheads), 0: per-channel
  * layout (dt, lambda [rows, D], theta [rows, D, N/2], a_log [D, N]).  x, y [rows, D], b, c
- * [rows, G, N] in io_dtype.  h, phase and the workspace must be 16-byte aligned
- * (MXB_ERR_ALIGNMENT).  flags: MXB_MAMBA3_RECURRENT_KERNELS, MXB_MAMBA3_SERIAL_WALK (never cut
- * a sequence).  Every sum has a fixed order.
+ * [rows, G, N] in io_dtype.  h, phase, the workspace and, in the per-channel layout, a_log must
+ * be 16-byte aligned (MXB_ERR_ALIGNMENT); everything else may start at any element.  At most
+ * 2^31 - 2^20 rows, 2^20 sequences, 65,535 channels, and fewer than 2^31 sequences times channels
+ * (MXB_ERR_UNSUPPORTED).  flags: MXB_MAMBA3_RECURRENT_KERNELS, MXB_MAMBA3_SERIAL_WALK (never cut a
+ * sequence).  Every sum has a fixed order.
  * ---------------------------------------------------------------------- */
 typedef struct {
   int32_t rows, S, slots, D, N, G, nheads, io_dtype, flags;
@@ -367,8 +369,8 @@ MXB_API mxb_status mxb_mamba3_decode_step(const mxb_mamba3_serve_desc* d, const 
  * pool of the last inputs, conv_state [slots, K-1, D] in io_dtype, oldest first:
  *   y_t = act(sum_k w[:, k] x_{t-k} + bias)
  * w(d, k) = w[d w_stride_d + k w_stride_k] float32, so that both blocks' weights ([D, K] and
- * [K, D]) serve as they are; bias [D] may be NULL.  K <= 4.  cu_seqlens, slot, go_on, y and
- * their rules as above. */
+ * [K, D]) serve as they are; bias [D] may be NULL.  K <= 4; at most 2^31 - 2^20 rows, sequences
+ * and channels, 65,535 tokens of a step.  cu_seqlens, slot, go_on, y and their rules as above. */
 enum { MXB_ACT_NONE = 0, MXB_ACT_SILU = 1 };
 typedef struct {
   int32_t rows, S, slots, D, K, io_dtype, activation;

@@ -409,6 +409,8 @@ mxb_status mxb_mamba3_bwd(const mxb_mamba3_desc* d, const void* x, const float* 
 }
 
 // ---------------------------------------------------------------- serving
+// Rows, sequences and channels are counted in 32 bits, and kernels count a little beyond the last.
+constexpr int32_t kMostRows = INT32_MAX - (1 << 20);
 static mxb_status serve_params(const mxb_mamba3_serve_desc* d, ServeP* p) {
   if (!d) return MXB_ERR_INVALID_ARGUMENT;
   if (d->rows < 0 || d->S < 0 || d->slots < 0 || d->D <= 0 || d->N <= 0 || d->G <= 0 || d->nheads < 0) return MXB_ERR_INVALID_ARGUMENT;
@@ -416,7 +418,7 @@ static mxb_status serve_params(const mxb_mamba3_serve_desc* d, ServeP* p) {
   if (d->N % 2 || d->N > 256 || d->D % d->G) return MXB_ERR_UNSUPPORTED;
   if (d->nheads > 0 && (d->D % d->nheads || d->nheads % d->G)) return MXB_ERR_UNSUPPORTED;
   // (grids: heads and channels run along an axis of 65,535 blocks, sequences times heads along one of 2^31)
-  if (d->D > 65535 || d->S > (1 << 20) || (int64_t)d->S * d->D >= (int64_t)1 << 31) return MXB_ERR_UNSUPPORTED;
+  if (d->rows > kMostRows || d->D > 65535 || d->S > (1 << 20) || (int64_t)d->S * d->D >= (int64_t)1 << 31) return MXB_ERR_UNSUPPORTED;
   *p = ServeP{};
   p->rows = d->rows; p->S = d->S; p->slots = d->slots; p->D = d->D; p->N = d->N; p->G = d->G; p->NH = d->nheads;
   p->Kp = d->N / 2; p->P = d->nheads > 0 ? d->D / d->nheads : 1;
@@ -479,7 +481,7 @@ static mxb_status check_conv_desc(const mxb_short_conv_desc* d) {
   if (d->rows < 0 || d->S < 0 || d->slots < 0 || d->D <= 0 || d->K <= 0) return MXB_ERR_INVALID_ARGUMENT;
   if (d->io_dtype != MXB_F32 && d->io_dtype != MXB_BF16) return MXB_ERR_INVALID_ARGUMENT;
   if (d->activation != MXB_ACT_NONE && d->activation != MXB_ACT_SILU) return MXB_ERR_INVALID_ARGUMENT;
-  if (d->K > 4) return MXB_ERR_UNSUPPORTED;
+  if (d->K > 4 || d->rows > kMostRows || d->S > kMostRows || d->D > kMostRows) return MXB_ERR_UNSUPPORTED;
   return MXB_OK;
 }
 mxb_status mxb_short_conv_prefill(const mxb_short_conv_desc* d, const void* x, const float* w, const float* bias,

@@ -107,6 +107,12 @@ void check_apart(const Tensor& out, const Tensor* itself, std::initializer_list<
   }
 }
 
+// A size that a descriptor counts in 32 bits.
+int32_t i32(int64_t n, const char* name) {
+  if (n > INT32_MAX || n < INT32_MIN) throw py::value_error(std::string(name) + ": " + std::to_string(n) + " is beyond 32 bits");
+  return (int32_t)n;
+}
+
 template <typename T = void>
 T* ptr(const Tensor& t) { return static_cast<T*>(t.data_ptr()); }
 template <typename T = void>
@@ -652,7 +658,8 @@ ServeCall check_serve(at::Device dev, const std::vector<Tensor>& state, const Te
   if (nheads < 0) throw py::value_error("nheads must not be negative");
   const int64_t T = x.size(0), D = x.size(1), G = b.size(1), N = b.size(2);
   const auto io = x.scalar_type();
-  const mxb_mamba3_serve_desc d{(int32_t)T, (int32_t)r.S, (int32_t)r.slots, (int32_t)D, (int32_t)N, (int32_t)G, (int32_t)nheads, io_code(x), (int32_t)flags};
+  const mxb_mamba3_serve_desc d{i32(T, "rows"), i32(r.S, "sequences"), i32(r.slots, "slots"), i32(D, "D"), i32(N, "N"), i32(G, "G"), i32(nheads, "nheads"),
+                                io_code(x), i32(flags, "flags")};
   const int64_t H = nheads > 0 ? nheads : D, per[] = {T, H, N / 2}, al[] = {H, N}, gn[] = {T, G, N};
   check(x, x.sizes(), io, dev, "x");
   check(dt, Shape(per, 2), F, dev, "dt");
@@ -728,7 +735,7 @@ mxb_short_conv_desc check_short_conv(at::Device dev, const Tensor& state, const 
   if (out)
     check_apart(*out, r.cu ? nullptr : &x,
                 {{&x, "x"}, {&w, "w"}, {at_of(bias), "bias"}, {&state, "conv_state"}, {at_of(r.cu), "cu_seqlens"}, {at_of(r.slot), "slots"}, {at_of(r.go_on), "go_on"}});
-  return {(int32_t)x.size(0), (int32_t)r.S, (int32_t)r.slots, (int32_t)D, (int32_t)K, io_code(x), activation ? MXB_ACT_SILU : MXB_ACT_NONE, w.stride(0), w.stride(1)};
+  return {i32(x.size(0), "rows"), i32(r.S, "sequences"), i32(r.slots, "slots"), i32(D, "D"), i32(K, "K"), io_code(x), activation ? MXB_ACT_SILU : MXB_ACT_NONE, w.stride(0), w.stride(1)};
 }
 Tensor short_conv_prefill(const Tensor& x, const Tensor& w, const Tensor& cu, const Tensor& state, const Opt& slots, const Opt& go_on,
                           const Opt& bias, const std::optional<std::string>& activation, const Opt& out) {
@@ -760,7 +767,7 @@ mxb_residual_norm_desc check_norm(at::Device dev, const Tensor& resid, const Ten
   if (y.dim() < 1) throw py::value_error("y must be [..., D]");
   const int64_t D = y.size(-1);
   const auto io = y.scalar_type();
-  const mxb_residual_norm_desc d{D > 0 ? y.numel() / D : 0, (int32_t)D, io_code(y), io_code(resid), (float)eps};
+  const mxb_residual_norm_desc d{D > 0 ? y.numel() / D : 0, i32(D, "D"), io_code(y), io_code(resid), (float)eps};
   check(y, y.sizes(), io, dev, "y");
   check(resid, y.sizes(), resid.scalar_type(), dev, "resid");
   if (resid.scalar_type() != io && resid.scalar_type() != F) throw py::type_error("resid: BFloat16 beside a Float y (one type, or a Float resid)");

@@ -104,3 +104,13 @@ def test_scratch_of_many_sequences(nheads, D, N):
     assert need(small, walk) > D * N * 4  # a cut it is
     assert need(large, walk) - need(small, walk) <= 8 * nheads * (large - small) * (nheads > 0 and D // nheads > 64) + 256
     assert need(large, 0) - need(small, 0) <= (2048 * nheads + 20480 + 8 * nheads) * (large - small) + 1024
+
+
+def test_sizes_near_32_bits_are_refused():
+    most = (1 << 31) - 1
+    conv = lambda rows=8, S=2, D=64: _lib.ShortConvDesc(rows, S, 4, D, 4, 2, 0, 4, 1)  # noqa: E731
+    lib = mixlab_b200.lib()
+    assert _prefill(_serve(rows=most)) == -2 and mixlab_b200.lib().mxb_mamba3_prefill_workspace_bytes(C.byref(_serve(rows=most))) == 0
+    for d in (conv(rows=most), conv(S=most), conv(D=most)):
+        assert lib.mxb_short_conv_prefill(C.byref(d), FAKE, FAKE, None, FAKE, None, None, FAKE, FAKE, None) == -2
+        assert lib.mxb_short_conv_step(C.byref(d), FAKE, FAKE, FAKE, None, None, FAKE, None) == -2

@@ -621,3 +621,12 @@ def test_steps_that_forget_everything(io, raw):
         for lo, hi in zip([0] + steps, steps + [sum(lens)]):
             assert_close(y[lo:hi].cpu(), y_want[lo:hi], TOL[io], f"rows {lo} to {hi}, flags {flags}")
         check_state(state, want, io, TOL[F32], [0, 1])
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """2^32 + 8 rows or columns are not taken for 8."""
+    big = torch.empty((1 << 32) + 8, 1, dtype=BF16, device="cuda")
+    with pytest.raises(ValueError, match="beyond 32 bits"):
+        ops.short_conv_prefill(big, torch.ones(1, 1).cuda(), cu_of([8]), torch.empty(1, 0, 1, dtype=BF16, device="cuda"))
+    with pytest.raises(ValueError, match="beyond 32 bits"):
+        ops.residual_norm(big.t(), big.t(), torch.empty((1 << 32) + 8, device="cuda"))
