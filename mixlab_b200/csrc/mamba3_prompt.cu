@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(2 * kThreads, 2) m3p_chunks_kernel(ServeP p) {
   const int per = p.NH * p.slabs, hd = blockIdx.x % per / p.slabs, slab = blockIdx.x % p.slabs;  // (heads first)
   const Piece q = find_piece<ENDS ? kInner : kPieces>(p, blockIdx.x / per, p.L);
   const int piece = q.base + q.seg;
-  if (!q.ok || !cut_fits(p, q)) return;
+  if (!q.ok || piece >= p.cuts) return;
   const int chunks = (q.last - q.first + Q - 1) / Q;
   if (q.chunk + chunks > p.chunks) return;  // (lengths that add up to more than the rows)
   const int p0 = slab * kPS, np = min(kPS, p.P - p0);
@@ -493,14 +493,14 @@ __global__ void __launch_bounds__(2 * kThreads, 2) m3p_chunks_kernel(ServeP p) {
   } else if (from_state) {
     load_h(p.h + ((size_t)slot * p.D + chan + row0) * p.N + n0);
     const bf16 *b_prev = static_cast<const bf16*>(p.b_prev) + ph * p.N + n0, *x_prev = static_cast<const bf16*>(p.x_prev) + (size_t)slot * p.D + chan + row0;
-    float2 b[NT];  // (by elements: the pool's b may start at any)
+    uint32_t b[NT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) b[t] = 8 * t < p.N ? load_pair(b_prev + 8 * t) : make_float2(0.f, 0.f);
+    for (int t = 0; t < NT; ++t) b[t] = 8 * t < p.N ? *reinterpret_cast<const uint32_t*>(b_prev + 8 * t) : 0u;
     const float look0 = serve_look(p, (size_t)q.first * p.NH + hd, true);
     const float k0 = rows_in[0] ? look0 * to_f32(x_prev[0]) : 0.f, k1 = rows_in[1] ? look0 * to_f32(x_prev[8]) : 0.f;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const float2 v = b[t], h0 = m3_on(make_float2(h[t][0], h[t][1]), start), h1 = m3_on(make_float2(h[t][2], h[t][3]), start);
+      const float2 v = unpack(b[t]), h0 = m3_on(make_float2(h[t][0], h[t][1]), start), h1 = m3_on(make_float2(h[t][2], h[t][3]), start);
       h[t][0] = fmaf(k0, v.x, h0.x);
       h[t][1] = fmaf(k0, v.y, h0.y);
       h[t][2] = fmaf(k1, v.x, h1.x);
@@ -702,8 +702,12 @@ __global__ void __launch_bounds__(2 * kThreads, 2) m3p_chunks_kernel(ServeP p) {
         *reinterpret_cast<float2*>(to + (size_t)8 * k * p.N + 8 * t) = m3_on(make_float2(h[t][2 * k], h[t][2 * k + 1]), by);
   // (the slabs of a head all read its phase and b_prev; with more than one they are written behind this launch)
   // (every thread has read them: barriers lie between)
-  if (!ENDS && tid == 0 && slab == 0) *serve_phase_end(p, q.seq, ph, hd) = m3_turned(start, ran);
-  if (!ENDS && p.slabs == 1) serve_tail<bf16>(p, q.end - 1, slot, hd, grp, kThreads);
+  if (!ENDS && p.slabs == 1) {
+    if (tid == 0) p.phase[ph] = m3_turned(start, ran);
+    serve_tail<bf16>(p, q.end - 1, slot, hd, grp, kThreads);
+  } else if (!ENDS && tid == 0 && slab == 0) {
+    p.phase_end[(size_t)q.seq * p.NH + hd] = m3_turned(start, ran);
+  }
 }
 
 // The split of the registers waits for good where the kernel starts with fewer than it counts on: looked up once.
@@ -736,19 +740,20 @@ static mxb_status launch(const ServeP& p, bool ends, cudaStream_t st) {
 
 }  // namespace m3p
 
-// Whole 16-byte pieces of rows, a state that fits the registers of four warps, and rows enough for chunks of 64 to be worth
-// it: more than 16 in the call and more than 4 a sequence (the host knows their mean only).  us, chunks / walk, 128 states:
-//   one prompt of 16 rows, 32 heads          14 / 14     of 24 rows 17 / 18     of 64 rows 17 / 35
-//   256 prompts of 32 heads, 1 row each     437 / 290    4 rows 438 / 328       8 rows 439 / 378    16 rows 440 / 476
-//   64 prompts of 8 heads, 1 row each        35 / 20     4 rows  40 / 26        8 rows  40 / 30     24 rows  41 / 48
+// Whole 16-byte pieces of rows, a b_prev of whole pairs (read by elements, 256 short prompts take 437 us for 412), a state that
+// fits the registers of four warps, and rows enough for chunks of 64 to be worth it: more than 16 in the call and more than 4 a
+// sequence (the host knows their mean only).  us, chunks / walk, 128 states:
+//   one prompt of 16 rows, 32 heads          14 / 14     of 24 rows 16 / 18     of 64 rows 16 / 35
+//   256 prompts of 32 heads, 1 row each     410 / 288    4 rows 412 / 326       8 rows 412 / 375    16 rows 414 / 474
+//   64 prompts of 8 heads, 1 row each        33 / 20     4 rows  38 / 26        8 rows  38 / 30     24 rows  39 / 48
 // Tokens beside one prompt are what the line is not drawn further out for: 8 heads, 255 of them beside 512 rows (3 a sequence)
-// 138 / 127, 63 beside 256 rows (5 a sequence) 48 / 72, 15 beside 128 (9 a sequence) 30 / 53.
+// 134 / 129, 63 beside 256 rows (5 a sequence) 46 / 71, 15 beside 128 (9 a sequence) 29 / 54.
 static bool m3prompt_shape(const ServeP& p, bool f32) {
   return !f32 && p.NH > 0 && p.N % 8 == 0 && p.N <= 128 && p.P % 8 == 0 && p.rows > 16 && p.rows > 4 * (long long)p.S;
 }
 bool m3prompt_supported(const ServeP& p, bool f32) {
   auto al = [](const void* q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };
-  return m3prompt_shape(p, f32) && al(p.x) && al(p.b) && al(p.c) && reinterpret_cast<uintptr_t>(p.y) % 4 == 0;
+  return m3prompt_shape(p, f32) && al(p.x) && al(p.b) && al(p.c) && (reinterpret_cast<uintptr_t>(p.y) | reinterpret_cast<uintptr_t>(p.b_prev)) % 4 == 0;
 }
 mxb_status m3prompt_prepare(const ServeP& p, cudaStream_t st) {
   const dim3 grid(p.chunks, p.G + (p.NH + m3p::kRecHeads - 1) / m3p::kRecHeads);

@@ -19,7 +19,8 @@ struct ServeP {
   float2* phase;            // [slots, NH] or [slots, D, Kp]: cosine and sine of the angle
   void *x_prev, *b_prev;    // [slots, D], [slots, NH or G, N]
   void* y;
-  // prompts cut into segments of L steps: at most so many segments in all, and of sequences that have more than one
+  // prompts cut into segments of L steps; at most `pieces` segments, and fewer than `cuts` of sequences that have more than one
+  // (what counts beyond belongs to lengths that add up to more than the rows, and is left)
   int L, pieces, cuts;
   float* ends;      // [cuts, D, N]: what a segment adds to the state, then the state that it starts from
   float* dsum;      // [cuts, NH or D]: sum of dt over the segment
@@ -70,8 +71,6 @@ struct Piece {
   int seq, seg, segs, base, first, last, begin, end, chunk;
   bool ok;
 };
-// Whether a cut sequence's segments have their places (they do not where lengths add up to more than the rows).
-__device__ __forceinline__ bool cut_fits(const ServeP& p, const Piece& q) { return q.segs == 1 || q.base + q.segs <= p.cuts; }
 // The index-th piece: sequences one after the other, each cut every L rows; up to 32 sequences by falling length, so that the
 // long ones do not start last (32 heads of 16 sequences of 440 to 4377 rows: a third off the time).  Called by whole warps, which
 // look through 32 sequences at a time and add up those in front.  Whatever cu holds, rows stay inside the call's.
@@ -149,11 +148,6 @@ __device__ __forceinline__ int serve_slot(const ServeP& p, int seq) {
   return s >= 0 && s < p.slots ? s : -1;
 }
 __device__ __forceinline__ bool serve_goes_on(const ServeP& p, int seq) { return p.go && __ldg(p.go + seq); }
-
-// Where the phase behind a sequence's last step goes; ph: its place in the pool.
-__device__ __forceinline__ float2* serve_phase_end(const ServeP& p, int seq, size_t ph, int hd) {
-  return p.slabs > 1 ? p.phase_end + (size_t)seq * p.NH + hd : p.phase + ph;
-}
 
 // (1 - lambda) dt of row t + 1, which weighs row t's outer product there; 0 behind the sequence's last row.
 __device__ __forceinline__ float serve_look(const ServeP& p, size_t at, bool in) {

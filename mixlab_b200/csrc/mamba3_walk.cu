@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(256) m3k_heads_kernel(ServeP p, int LN) {
   const int heads = p.NH * p.slabs, tid = threadIdx.x, hd = blockIdx.x % heads / p.slabs, slab = blockIdx.x % p.slabs;
   const Piece q = find_piece<MODE == kEnds ? kInner : kPieces>(p, blockIdx.x / heads, p.L);
   const int piece = q.base + q.seg;
-  if (!q.ok || !cut_fits(p, q)) return;
+  if (!q.ok || piece >= p.cuts) return;
   const int ln = tid % LN, rg = tid / LN, rows_at_once = 256 / LN, npad = LN * 4 * NV;
   const int per = (p.P + p.slabs - 1) / p.slabs, p0 = slab * per, np = min(per, p.P - p0);  // this CTA's channels of the head
   const size_t chan = (size_t)hd * p.P + p0;
@@ -237,8 +237,12 @@ __global__ void __launch_bounds__(256) m3k_heads_kernel(ServeP p, int LN) {
         else *reinterpret_cast<float2*>(p.h + ((size_t)slot * p.D + chan + row) * p.N + n) = m3_back(v, start);
       }
   // (the slabs of a head all read its phase and b_prev; with more than one they are written behind this launch)
-  if (MODE == kOut && tid == 0 && slab == 0) *serve_phase_end(p, q.seq, ph, hd) = m3_turned(start, ran);
-  if (MODE == kOut && p.slabs == 1) serve_tail<IO>(p, q.end - 1, slot, hd, g, 256);
+  if (MODE == kOut && p.slabs == 1) {
+    if (tid == 0) p.phase[ph] = m3_turned(start, ran);
+    serve_tail<IO>(p, q.end - 1, slot, hd, g, 256);
+  } else if (MODE == kOut && tid == 0 && slab == 0) {
+    p.phase_end[(size_t)q.seq * p.NH + hd] = m3_turned(start, ran);
+  }
 }
 
 // What the segments of a sequence start from.  grid (sequences that can be longer than L, blocks of pairs): a thread per state pair of the channels walks
@@ -247,7 +251,7 @@ constexpr int kAhead = 8;
 __global__ void __launch_bounds__(256) m3k_heads_chain_kernel(ServeP p, bool bf16_io) {
   begin_dependent();
   const Piece q = find_piece<kCut>(p, blockIdx.x, p.L);
-  if (!q.ok || !cut_fits(p, q)) return;
+  if (!q.ok || q.base + q.segs > p.cuts) return;
   const int slot = serve_slot(p, q.seq);
   const bool go = slot >= 0 && serve_goes_on(p, q.seq);
   const size_t pairs = (size_t)p.D * p.Kp;
@@ -374,7 +378,7 @@ __global__ void __launch_bounds__(128) m3k_channels_kernel(ServeP p) {
   const int d = live ? d_raw : p.D - 1;
   const Piece q = find_piece<MODE == kEnds ? kInner : kPieces>(p, blockIdx.x, p.L);
   const int piece = q.base + q.seg;
-  if (!q.ok || !cut_fits(p, q)) return;
+  if (!q.ok || piece >= p.cuts) return;
   const int slot = serve_slot(p, q.seq), g = d / (p.D / p.G);
   const bool from_state = MODE == kOut && q.segs == 1 && slot >= 0 && serve_goes_on(p, q.seq);
   const size_t sd = (size_t)(slot < 0 ? 0 : slot) * p.D + d, row = (size_t)piece * p.D + d;
@@ -656,7 +660,7 @@ __global__ void __launch_bounds__(128) m3k_channels_kernel(ServeP p) {
 __global__ void __launch_bounds__(256) m3k_channels_chain_kernel(ServeP p, bool bf16_io) {
   begin_dependent();
   const Piece q = find_piece<kCut>(p, blockIdx.x, p.L);
-  if (!q.ok || !cut_fits(p, q)) return;
+  if (!q.ok || q.base + q.segs > p.cuts) return;
   const int slot = serve_slot(p, q.seq);
   const bool go = slot >= 0 && serve_goes_on(p, q.seq);
   const size_t pairs = (size_t)p.D * p.Kp;
@@ -848,9 +852,9 @@ size_t m3walk_scratch(ServeP& p, bool f32, int flags, char* base) {
   }
   if (p.NH && m3k::serve_slabs(p) > 1) p.phase_end = c.take<float2>((size_t)p.S * p.NH);
   p.pieces = p.S;
+  p.cuts = 1;
   if (p.rows <= p.L) return c.bytes();
-  // (a sequence's segments but the last are L rows each)
-  p.cuts = p.rows / p.L + m3k::longer_than_L(p);
+  p.cuts += p.rows / p.L + m3k::longer_than_L(p);  // (a sequence's segments but the last are L rows each)
   p.pieces = p.rows / p.L + p.S;
   p.ends = c.take<float>((size_t)p.cuts * p.D * p.N);
   p.dsum = c.take<float>((size_t)p.cuts * (p.NH ? p.NH : p.D));

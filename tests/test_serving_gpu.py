@@ -319,7 +319,8 @@ def test_unaligned_operands_give_the_same():
 @pytest.mark.parametrize("io", [F32, BF16], ids=["f32", "bf16"])
 def test_pool_rows_may_start_at_any_element(io, shape):
     """x_prev and b_prev as views that start at an odd element, beside operands on 16 bytes, of prompts that go on from them:
-    short ones, one that is cut, and single tokens.  The same kernels on the same values: the same bits."""
+    short ones, one that is cut, and single tokens.  The same kernels on the same values give the same bits; bf16 prompts that
+    would run in chunks go step by step then."""
     D, N, G, nheads = shape
     lens = [40, 1, 900, 130]
     a = [t.cuda() for t in args_of(scan_inputs(sum(lens), D, N, G, nheads, io, 27))]
@@ -337,8 +338,15 @@ def test_pool_rows_may_start_at_any_element(io, shape):
             y = ops.mamba3_prefill(*a, cu_of(lens), state, go_on=torch.ones(4, dtype=torch.bool, device="cuda"), nheads=nheads, flags=flags)
             y1 = ops.mamba3_decode_step(state, *(t if i == 4 else t[:4].contiguous() for i, t in enumerate(a)), nheads=nheads)
             results.append([y, y1, *state])
-    for got, want in zip(results[2:], results[:2]):
-        assert all(torch.equal(t, u) for t, u in zip(got, want))
+    for flags, got, want in zip((0, WALK), results[2:], results[:2]):
+        if flags or io == F32 or not nheads:
+            assert all(torch.equal(t, u) for t, u in zip(got, want))
+            continue
+        for t, u in zip(got[:2], want):
+            assert_close(t, u.double(), TOL[BF16])
+        for t, u in zip(got[2:4], want[2:]):  # (900 steps: the bound of the angles grows with them)
+            assert_close(t, u.double(), 3 * TOL[F32])
+        assert torch.equal(got[4], want[4]) and torch.equal(got[5], want[5])
 
 
 def test_a_layer_serves_prompts_then_tokens():
