@@ -3,6 +3,8 @@
 Tolerances: float32 results carry a few roundings of 2^-24 and one 2^-24 more for every doubling of the sums' length (pairs, by
 lanes): 1e-6 covers 16; column sums over up to 3000 rows one after the other in a CTA, at most rows / CTAs x 2^-24 more: 1e-5.
 bf16 results are rounded once: 2^-8."""
+import ctypes as C
+
 import pytest
 import torch
 
@@ -137,6 +139,44 @@ def test_gradients_in_a_graph_and_on_a_stream():
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(got[k], t) for k, t in want.items())
+
+
+@pytest.mark.parametrize("io,res", [(F32, F32), (BF16, F32), (BF16, BF16)], ids=["f32", "bf16 on f32", "bf16"])
+@pytest.mark.parametrize("rows,D", [(700, 2048), (1300, 1000), (660, 1999), (330, 5000), (310, 8200), (300, 16384)])
+def test_several_rows_a_thread(rows, D, io, res):
+    """More rows than the GPU holds at once: a CTA walks over two or three, with the next one under way, and adds up their columns."""
+    a = inputs(rows, D, io, res, True, True, True, 9)
+    dev, f = on(a, lambda t: t.cuda()), on(a, lambda t: t.double())
+    r, n = call(dev)
+    r_want, n_want = serving.residual_norm(f["resid"], f["y"], f["norm"], f["post_norm"], f["z"], f["scale"])
+    assert_close(r.cpu(), r_want, TOL[res], "resid")
+    assert_close(n.cpu(), n_want, TOL[io], "n")
+    got, want = back(dev), oracle_grads(a)
+    for k, w in want.items():
+        assert_close(got[k].cpu(), w, TOL[io] if k in ("dy", "dz") else TOL[res] if k == "d_resid" else 1e-5, k)
+
+
+@pytest.mark.parametrize("rows,D", [(700, 2048), (5, 64), (9, 449), (300, 4096)])
+@pytest.mark.parametrize("io,res", [(F32, F32), (BF16, F32), (BF16, BF16)], ids=["f32", "bf16 on f32", "bf16"])
+def test_stream_in_place(rows, D, io, res):
+    """resid_out on resid, d_resid on d_resid_out: the bits of separate arrays."""
+    a = on(inputs(rows, D, io, res, True, True, True, 10), lambda t: t.cuda())
+    lib, p = _lib.lib(), lambda t: C.c_void_p(t.data_ptr())
+    code = lambda t: _lib.MXB_F32 if t == F32 else _lib.MXB_BF16  # noqa: E731
+    d = _lib.ResidualNormDesc(rows, D, code(io), code(res), 1e-5)
+    stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    want_r, want_n = call(a)
+    r, n = a["resid"].clone(), torch.empty_like(a["y"])
+    assert lib.mxb_residual_norm_fwd(C.byref(d), p(r), p(a["y"]), p(a["norm"]), p(a["post_norm"]), p(a["z"]), p(a["scale"]), p(r), p(n), stream) == 0
+    assert torch.equal(r, want_r) and torch.equal(n, want_n)
+    want = back(a)
+    g = {k: torch.empty_like(v) for k, v in want.items()}
+    g["d_resid"] = a["d"].clone()
+    ws = torch.empty(lib.mxb_residual_norm_workspace_bytes(C.byref(d)), dtype=torch.uint8, device="cuda")
+    assert lib.mxb_residual_norm_bwd(C.byref(d), p(a["resid"]), p(a["y"]), p(a["norm"]), p(a["post_norm"]), p(a["z"]), p(a["scale"]), p(g["d_resid"]),
+                                     p(a["dn"]), p(g["d_resid"]), p(g["dy"]), p(g["dz"]), p(g["dnorm"]), p(g["dpost_norm"]), p(g["dscale"]), p(ws),
+                                     ws.numel(), stream) == 0
+    assert all(torch.equal(g[k], want[k]) for k in want)
 
 
 def test_refusals():
