@@ -638,3 +638,35 @@ def test_sizes_beyond_32_bits_are_refused():
         ops.short_conv_prefill(big, torch.ones(1, 1).cuda(), cu_of([8]), torch.empty(1, 0, 1, dtype=BF16, device="cuda"))
     with pytest.raises(ValueError, match="beyond 32 bits"):
         ops.residual_norm(big.t(), big.t(), torch.empty((1 << 32) + 8, device="cuda"))
+
+
+@pytest.mark.parametrize("nheads,D,N", [(2, 128, 64), (0, 48, 16)])
+def test_a_served_layer_is_the_trained_one(nheads, D, N):
+    """A Mamba-3 layer by the stages of training over [1, T] and by those of serving, prompt and tokens: float32, the bound of
+    prompts on either side."""
+    E, G, K, T, cut = 40, 1, 4, 90, 83
+    g = torch.Generator().manual_seed(38)
+    r = lambda *s: torch.randn(*s, generator=g).cuda()  # noqa: E731
+    H = nheads or D
+    n, w, post, next_norm, scale = r(T, E), r(D, K) / 2, 1 + 0.1 * r(D), 1 + 0.1 * r(E), 0.5 + 0.1 * r(E)
+    W = {k: r(E, c) / E ** 0.5 for k, c in dict(x=D, z=D, b=N, c=N, dt=H, lam=H, theta=H if nheads else D * N // 2).items()}
+    W_o, h, a_log = r(D, E) / D ** 0.5, r(T, E), torch.rand(*((nheads,) if nheads else (D, N)), generator=g).cuda()
+    p = {k: n @ v for k, v in W.items()}
+    p["dt"], p["theta"] = p["dt"] - 2, p["theta"] if nheads else p["theta"].view(T, D, N // 2)
+    b, c = ops.mamba3_block_bc(p["b"][None], p["c"][None], 1 + 0.1 * r(N), 1 + 0.1 * r(N), 0.1 * r(N), 0.1 * r(N), G, N)
+    b, c = b.view(1, T, G, N), c.view(1, T, G, N)
+
+    def behind(y, rows):
+        o = ops.mamba3_block_post(y[None], p["z"][rows][None].contiguous(), post)[0] @ W_o
+        return torch.stack(ops.residual_norm(h[rows], o, next_norm, scale=scale))
+
+    x = ops.mamba3_block_conv(p["x"][None], w)
+    y = ops.mamba3_selective_scan(x, p["dt"][None], p["lam"][None], p["theta"][None], a_log, b, c, nheads=nheads)
+    want = behind(y[0], slice(0, T))
+    state, conv, rows = ops.mamba3_state(1, D, N, G, nheads=nheads, dtype=F32), torch.zeros(1, K - 1, D).cuda(), slice(0, cut)
+    part = lambda q: [t[q].contiguous() for t in (p["dt"], p["lam"], p["theta"])] + [a_log, b[0, q].contiguous(), c[0, q].contiguous()]  # noqa: E731
+    got = [behind(ops.mamba3_prefill(ops.short_conv_prefill(p["x"][rows], w, cu_of([cut]), conv), *part(rows), cu_of([cut]), state, nheads=nheads), rows)]
+    for t in range(cut, T):
+        q = slice(t, t + 1)
+        got.append(behind(ops.mamba3_decode_step(state, ops.short_conv_step(conv, p["x"][q], w), *part(q), nheads=nheads), q))
+    assert_close(torch.cat(got, 1), want.double(), 2 * TOL[F32])
