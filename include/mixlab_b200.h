@@ -389,8 +389,9 @@ MXB_API mxb_status mxb_short_conv_step(const mxb_short_conv_desc* d, void* conv_
  *   a = RMSNorm(y; post_norm) SiLU(z);  resid_out = resid + scale a;  n = RMSNorm(resid_out; norm)
  * resid, resid_out [rows, D] in resid_dtype (io_dtype or MXB_F32); y, z, n [rows, D] in
  * io_dtype; norm, post_norm, scale [D] float32.  post_norm, z, scale may be NULL (no norm, no
- * gate, scale 1).  D <= 16384.  resid_out may be resid itself.  n is the norm of resid_out
- * before it is rounded to resid_dtype.
+ * gate, scale 1).  D <= 16384.  resid_out may be resid itself.  n is the norm of resid_out before
+ * it is rounded to resid_dtype.  (The gated_deltanet and Mamba-3 blocks have a projection between
+ * their gate and the addition: there y is its result, and norm and gate are the block's post stage.)
  * bwd: resid_out is what the forward returned, d_resid_out (may be NULL: zero) the gradient
  * that reaches it from its other readers, dn that of n.  Every gradient: d_resid (resid_dtype),
  * dy, dz (io_dtype), dnorm, dpost_norm, dscale [D] float32; dz, dpost_norm, dscale belong to

@@ -4,8 +4,8 @@
 // The state keeps cosine and sine of phi, and the token before as its x and its (unturned) b.
 //
 // The state is read once and written once, in 16-byte pieces; everything else is small.  Bound: HBM for large batches, launch
-// and one chain of load -> sum -> store for small ones.  Heads, 64 channels and 128 states, bf16: 256 tokens of 32 heads 96 us
-// (546 MB: 87 % of the measured copy rate), one token 6.9 us; 61 tokens of 448 channels of 16 states, float32, 9.4 us.
+// and one chain of load -> sum -> store for small ones.  Heads, 64 channels and 128 states, bf16: 256 tokens of 32 heads 96 to
+// 98 us (546 MB: 86 % of the measured copy rate), one token 6.7 us; 61 tokens of 448 channels of 16 states, float32, 8.7 us.
 #include "mamba3_serve.cuh"
 
 namespace mxb {

@@ -29,7 +29,9 @@ enum Mode { kOut, kEnds };
 // A CTA per (segment, head, slab of channels): LN lanes along a row of states, NV pieces of 4 states a lane, R rows a thread,
 // all in registers.  16 steps at a time are made ready in shared memory: scalars by one warp, then b and c turned back and x; what
 // they are made of is requested 16 steps earlier.  Bound: shared memory and the issue of instructions.  Float32, 8 heads of 64
-// channels, 128 states: 16 prompts of 2048 rows 931 us, one of 16384 rows 417 us (cut in 37), one of 37 rows 33 us.
+// channels, 128 states: 16 prompts of 2048 rows 911 us, one of 16384 rows 407 us (cut in 37), one of 37 rows 24 us.
+// Angles sum dt as float32 (each rounded by 2^-24 of itself, as in the scan over [B, T] batches): n steps that turn by a radian are
+// off by about n 2^-24 at most.
 constexpr int kW = 16;
 constexpr int kRowsMost = 64;  // channels of a slab
 struct HeadSmem {
@@ -245,8 +247,8 @@ __global__ void __launch_bounds__(256) m3k_heads_kernel(ServeP p, int LN) {
   }
 }
 
-// What the segments of a sequence start from.  grid (sequences that can be longer than L, blocks of pairs): a thread per state pair of the channels walks
-// over the segments; what kAhead segments add is requested at a time.
+// What the segments of a sequence start from.  grid (sequences that can be longer than L, blocks of pairs): a thread per state
+// pair of the channels walks over the segments; what kAhead segments add is requested at a time.
 constexpr int kAhead = 8;
 __global__ void __launch_bounds__(256) m3k_heads_chain_kernel(ServeP p, bool bf16_io) {
   begin_dependent();
@@ -305,8 +307,9 @@ __global__ void __launch_bounds__(256) m3k_heads_chain_kernel(ServeP p, bool bf1
 // warp shares or each lane's own elements into its own places (no barrier of the CTA, no registers while they are under way).
 //
 // What bounds it is the issue of instructions, a sine, a cosine and two exponentials a state pair and step (4003 steps x 448
-// channels of 16 states: 14 M of them, 62 instructions each in the first pass over what is cut, 44 us, and 80 in the second, 52 us).  So two steps' angles go through packed polynomials, the two states of a pair are
-// packed, and y of 8 steps is added over 8 lanes by halving exchanges.
+// channels of 16 states: 14 M of them, 62 instructions each in the first pass over what is cut, 44 us, and 80 in the second, 52
+// us).  So two steps' angles go through packed polynomials, the two states of a pair are packed, and y of 8 steps is added over 8
+// lanes by halving exchanges.
 constexpr int kC = 8;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -315,8 +318,9 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 // Cosine and sine of two angles in 2^-32 turns: the nearest half turn by integers, minimax polynomials of degree 9 and 10 on what
-// is left, at most pi / 2 (fitted by least squares with Lawson's weights: 4.6e-9 and 2.4e-10; with the roundings 2.2e-7, 4e-8 in
-// the mean).  A nearest quarter turn would halve the roundings, and costs a dozen selections more.
+// is left, at most pi / 2 (fitted by least squares with Lawson's weights; with the coefficients rounded to float32 1.7e-8 and
+// 5.0e-9, with the roundings of a call 2.2e-7, 4e-8 in the mean).  A nearest quarter turn would halve the roundings, and costs a
+// dozen selections more.
 __device__ __forceinline__ void unit2(int t0, int t1, float2& u0, float2& u1) {
   const int half0 = (t0 + 0x40000000) & 0x80000000, half1 = (t1 + 0x40000000) & 0x80000000;
   const f2 r = mul2(pack2((float)(t0 ^ half0), (float)(t1 ^ half1)), dup2(1.4629180792671596e-9f));  // 2 pi / 2^32
@@ -337,8 +341,9 @@ __device__ __forceinline__ void unit2(int t0, int t1, float2& u0, float2& u1) {
   u0 = make_float2(by(c.x, half0), by(s.x, half0));
   u1 = make_float2(by(c.y, half1), by(s.y, half1));
 }
-// m3_turn of two steps, with dt theta rounded once, as dt is.  (The nearest whole turn by adding 1.5 x 2^23: good for up to 2^22
-// turns a step, where a float32 is no angle any more.)
+// m3_turn of two steps, with dt theta rounded once, as dt is.  (With this, the decays by ex2.approx and lambda by the fast
+// division y of float32 prompts of 4003 rows is 3.7e-7 off in the mean; elementary operations with angles in 64 bits: 1.2e-7.  The
+// nearest whole turn by adding 1.5 x 2^23: good for up to 2^22 turns a step, where a float32 is no angle any more.)
 __device__ __forceinline__ void turn2(f2 p, int& t0, int& t1) {
   const f2 hi = dup2(0.15915493667125702f), t = mul2(p, hi), low = mad2(p, dup2(-6.420638243e-09f), mad2(p, dup2(-0.15915493667125702f), t));
   const f2 whole = add2(add2(t, dup2(12582912.f)), dup2(-12582912.f));
@@ -826,11 +831,13 @@ static mxb_status prefill(ServeP p, bool chunks, cudaStream_t st) {
 
 }  // namespace m3k
 
-// Steps of a segment: as many segments as CTAs that the GPU holds at once, and at least 64 steps each; a quarter longer where
-// several sequences can fill the GPU side by side, since a cut costs a pass of its own over what lies in front of it.  (The host
-// does not know the lengths; sequences of up to L steps are not cut.)  Half and twice as many segments, us: a prompt of 16381 rows
-// of 8 heads in chunks 99 and 111 for 87; float32 599 and 480 for 417; 4003 rows of 448 channels 111 (half) for 97.  Without the
-// quarter: 16 prompts of 32 heads, 32768 rows, 422 us for 319 (the passes after the scalars); three of 700 rows, 8 heads, float32, 85 for 103.
+// Steps of a segment: as many segments as the CTAs that the GPU holds at once (heads), or twice that (channels: seven CTAs an SM
+// by registers), and at least 64 steps each; a quarter longer where several sequences can fill the GPU side by side, since a cut
+// costs a pass of its own over what lies in front of it.  (The host does not know the lengths; sequences of up to L steps are not
+// cut.)  Half and twice as many segments, us: a prompt of 16381 rows of 8 heads in chunks 99 and 111 for 87; float32 599 and 480
+// for 417; channels, 7 prompts of 4003 rows of 448 channels of 16 states 99 and 97 for 97, in bf16 108 and 99 for 99, one of 16384
+// rows 318 and 323 for 315, 4 of 2048 rows of 256 channels of 32 states 223 and 184 for 204.  Without the quarter, heads: 16
+// prompts of 32 heads, 32768 rows, 422 us for 319 (the passes after the scalars); three of 700 rows, 8 heads, float32, 85 for 103.
 static int walk_segment(const ServeP& p) {
   const long long ctas = p.NH ? (long long)p.NH * m3k::serve_slabs(p) : [&] {
     const int per = 128 / m3k::channel_shape(p).LPC;

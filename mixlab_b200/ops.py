@@ -222,7 +222,10 @@ def short_conv_step(conv_state, x, w, *, slots=None, bias=None, activation=None,
 def residual_norm(resid, y, norm, *, post_norm=None, z=None, scale=None, eps=1e-5):
     """The residual stream between two blocks: with a = RMSNorm(y, post_norm, eps) SiLU(z), returns resid + scale a and its
     RMSNorm with ``norm``, the next block's input.  resid, y, z [...,D] (resid in y's type or float32); norm, post_norm, scale
-    [D] float32; without post_norm, z or scale that step is left out.  D <= 16384."""
+    [D] float32; without post_norm, z or scale that step is left out.  D <= 16384.
+
+    The gated_deltanet and Mamba-3 blocks have their output projection between the gate and the addition: there y is the
+    projection's result, with ``scale`` alone, behind ``mamba3_block_post`` or ``gdn_block_post``."""
     return (_front or _native()).residual_norm(resid, y, norm, post_norm, z, scale, eps)
 
 
