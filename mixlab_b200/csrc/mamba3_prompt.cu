@@ -27,10 +27,10 @@
 // for 32 channels a warp or products and state in warps of their own, took 359 to 374 us where this took 322.
 //
 // Roundings to bf16: G as operand, g x and M once each; y itself.  (In the mean y is 2.4e-3 of itself off, 1.7e-3 by its own
-// rounding alone, 2.6e-3 where the state decays slowly; splitting G and M in two parts each would double the products that y is made of.)  The state is a float32 result
-// of its own, so that one rounding of g x is too much where it still reaches the segment's end: there (decay to the end above
-// 2^-11, above 2^-3) the remainder of the rounding is multiplied as well, and the remainder of that: 16 and 24 bits of g x, while
-// b is exact.
+// rounding alone, 2.6e-3 where the state decays slowly; splitting G and M in two parts each would double the products that y is
+// made of.)  The state is a float32 result of its own, so that one rounding of g x is too much where it still reaches the
+// segment's end: there (decay to the end above 2^-11, above 2^-3) the remainder of the rounding is multiplied as well, and the
+// remainder of that: 16 and 24 bits of g x, while b is exact.
 #include <algorithm>
 #include <type_traits>
 
