@@ -413,6 +413,48 @@ MXB_API mxb_status mxb_residual_norm_bwd(const mxb_residual_norm_desc* d, const 
                                  void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------
+ * The token rows in front of the residual stream, and their gradient:
+ *   out_t = scale W[token_t];   dW_v = scale * sum over token_t = v of d_out_t, in the order of t
+ * tokens [tokens] int32 or int64 (token_bytes 4 or 8); a token outside 0..V-1 is padding: a row of
+ * zeros, and no part in dW.  fwd: weight [V, D] in io_dtype, out [tokens, D] in out_dtype.  bwd:
+ * d_out [tokens, D] in io_dtype, dweight [V, D] in out_dtype; adds != 0: the sums are added to what
+ * dweight holds (a matrix that the output head shares), else every row of it is written.  Sums are
+ * float32, in a fixed order, and rounded once.  bwd: fewer than 2^31 tokens.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+  int64_t tokens;
+  int32_t V, D, token_bytes, io_dtype, out_dtype;
+  float scale;
+} mxb_embedding_desc;
+MXB_API mxb_status mxb_embedding_fwd(const mxb_embedding_desc* d, const void* tokens, const void* weight, void* out,
+                                     void* stream);
+MXB_API size_t mxb_embedding_bwd_workspace_bytes(const mxb_embedding_desc* d);
+MXB_API mxb_status mxb_embedding_bwd(const mxb_embedding_desc* d, const void* tokens, const void* d_out, void* dweight,
+                                     int32_t adds, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * The layer norm over the residual stream, with the addition in front of it:
+ *   h = resid + x (x without resid);  n = (h - mean h) / sqrt(var h + eps) weight + bias
+ * resid, stream [rows, D] in resid_dtype (io_dtype or MXB_F32), n in io_dtype, x in io_dtype, or in
+ * resid_dtype where resid is NULL (stream then is not written); weight, bias [D] float32, bias may be
+ * NULL.  D <= 16384.  stream may be resid itself.  n is the norm of h before it is rounded.
+ * bwd: x is the stream in resid_dtype, dn [rows, D] in io_dtype the gradient of n, d_resid (resid_dtype,
+ * may be NULL: zero) the gradient that reaches the stream from its other readers; dx (resid_dtype, may be
+ * d_resid itself), dweight, dbias [D] float32.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+  int64_t rows;
+  int32_t D, io_dtype, resid_dtype;
+  float eps;
+} mxb_layer_norm_desc;
+MXB_API mxb_status mxb_layer_norm_fwd(const mxb_layer_norm_desc* d, const void* resid, const void* x, const float* weight,
+                                      const float* bias, void* stream_out, void* n, void* stream);
+MXB_API size_t mxb_layer_norm_bwd_workspace_bytes(const mxb_layer_norm_desc* d);
+MXB_API mxb_status mxb_layer_norm_bwd(const mxb_layer_norm_desc* d, const void* x, const float* weight, const void* d_resid,
+                                      const void* dn, void* dx, float* dweight, float* dbias, void* workspace,
+                                      size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * Data-parallel gradient exchange: the element-wise passes on either side of the
  * per-bucket all-reduce, over flat float32 buckets on the device (the collective
  * itself is the caller's: NCCL).  They fuse what the reference does op by op per

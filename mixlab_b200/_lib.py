@@ -59,6 +59,14 @@ class ResidualNormDesc(C.Structure):
     _fields_ = [("rows", C.c_int64), ("D", C.c_int32), ("io_dtype", C.c_int32), ("resid_dtype", C.c_int32), ("eps", C.c_float)]
 
 
+class EmbeddingDesc(C.Structure):
+    _fields_ = [("tokens", C.c_int64)] + [(n, C.c_int32) for n in ("V", "D", "token_bytes", "io_dtype", "out_dtype")] + [("scale", C.c_float)]
+
+
+class LayerNormDesc(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("D", C.c_int32), ("io_dtype", C.c_int32), ("resid_dtype", C.c_int32), ("eps", C.c_float)]
+
+
 class IrOp(C.Structure):
     """mxb_ir_op: an IR op record (mlx_ir_program_add_op) after name resolution."""
     _fields_ = [("op_type", C.c_int32), ("inputs", C.POINTER(C.c_void_p)), ("n_inputs", C.c_int32),
@@ -108,6 +116,12 @@ EXPORTS = {
     "mxb_residual_norm_workspace_bytes": (C.c_size_t, [C.POINTER(ResidualNormDesc)]),
     "mxb_residual_norm_fwd": (C.c_int32, [C.POINTER(ResidualNormDesc)] + [_P] * 9),
     "mxb_residual_norm_bwd": (C.c_int32, [C.POINTER(ResidualNormDesc)] + [_P] * 15 + [C.c_size_t, _P]),
+    "mxb_embedding_fwd": (C.c_int32, [C.POINTER(EmbeddingDesc)] + [_P] * 4),
+    "mxb_embedding_bwd_workspace_bytes": (C.c_size_t, [C.POINTER(EmbeddingDesc)]),
+    "mxb_embedding_bwd": (C.c_int32, [C.POINTER(EmbeddingDesc)] + [_P] * 3 + [C.c_int32, _P, C.c_size_t, _P]),
+    "mxb_layer_norm_fwd": (C.c_int32, [C.POINTER(LayerNormDesc)] + [_P] * 7),
+    "mxb_layer_norm_bwd_workspace_bytes": (C.c_size_t, [C.POINTER(LayerNormDesc)]),
+    "mxb_layer_norm_bwd": (C.c_int32, [C.POINTER(LayerNormDesc)] + [_P] * 8 + [C.c_size_t, _P]),
     "mxb_dp_partial_floats": (C.c_size_t, []),
     "mxb_dp_sanitize": (C.c_int32, [_P, C.c_size_t, C.c_float, _P, _P]),
     "mxb_dp_finalize": (C.c_int32, [_P, C.c_size_t, C.c_float, C.c_float, _P, _P, _P]),

@@ -125,6 +125,13 @@ mxb_status residual_norm_fwd(const mxb_residual_norm_desc*, const void*, const v
                              const float*, void*, void*, cudaStream_t);
 mxb_status residual_norm_bwd(const mxb_residual_norm_desc*, const void*, const void*, const float*, const float*, const void*,
                              const float*, const void*, const void*, void*, void*, void*, float*, float*, float*, float*, cudaStream_t);
+mxb_status embedding_fwd(const mxb_embedding_desc*, const void*, const void*, void*, cudaStream_t);
+size_t embedding_bwd_scratch(const mxb_embedding_desc*);
+mxb_status embedding_bwd(const mxb_embedding_desc*, const void*, const void*, void*, int, void*, cudaStream_t);
+size_t layer_norm_scratch(const mxb_layer_norm_desc*);
+mxb_status layer_norm_fwd(const mxb_layer_norm_desc*, const void*, const void*, const float*, const float*, void*, void*, cudaStream_t);
+mxb_status layer_norm_bwd(const mxb_layer_norm_desc*, const void*, const float*, const void*, const void*, void*, float*, float*, float*,
+                          cudaStream_t);
 bool mamba3_block_supported(const mxb_mamba3_desc*);
 size_t mamba3_block_workspace_bytes(const mxb_mamba3_desc*);
 mxb_status mamba3_block_conv(const mxb_mamba3_desc*, int, const void*, const float*, void*, const void*, void*, float*,
@@ -544,6 +551,73 @@ mxb_status mxb_residual_norm_bwd(const mxb_residual_norm_desc* d, const void* re
   return residual_norm_bwd(d, resid_out, y, norm, post_norm, z, scale, d_resid_out, dn, d_resid, dy, z ? dz : nullptr, dnorm,
                            post_norm ? dpost_norm : nullptr, scale ? dscale : nullptr, static_cast<float*>(workspace),
                            static_cast<cudaStream_t>(stream));
+}
+
+// ---------------------------------------------------------------- the ends of a training step
+static mxb_status zeros(void* p, size_t bytes, void* stream) {
+  const cudaError_t e = cudaMemsetAsync(p, 0, bytes, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) { set_last_cuda_error((int)e); return MXB_ERR_CUDA; }
+  return MXB_OK;
+}
+static bool element_type(int32_t t) { return t == MXB_F32 || t == MXB_BF16; }
+static size_t element_bytes(int32_t t) { return t == MXB_F32 ? 4 : 2; }
+static mxb_status check_embedding_desc(const mxb_embedding_desc* d, bool bwd) {
+  if (!d || d->tokens < 0 || d->V <= 0 || d->D <= 0 || (d->token_bytes != 4 && d->token_bytes != 8)) return MXB_ERR_INVALID_ARGUMENT;
+  if (!element_type(d->io_dtype) || !element_type(d->out_dtype)) return MXB_ERR_INVALID_ARGUMENT;
+  if (bwd && d->tokens > INT32_MAX - 4096) return MXB_ERR_UNSUPPORTED;
+  return MXB_OK;
+}
+mxb_status mxb_embedding_fwd(const mxb_embedding_desc* d, const void* tokens, const void* weight, void* out, void* stream) {
+  const mxb_status s = check_embedding_desc(d, false);
+  if (s != MXB_OK) return s;
+  if (d->tokens == 0) return MXB_OK;
+  if (!tokens || !weight || !out) return MXB_ERR_INVALID_ARGUMENT;
+  return embedding_fwd(d, tokens, weight, out, static_cast<cudaStream_t>(stream));
+}
+size_t mxb_embedding_bwd_workspace_bytes(const mxb_embedding_desc* d) {
+  return check_embedding_desc(d, true) == MXB_OK ? embedding_bwd_scratch(d) : 0;
+}
+mxb_status mxb_embedding_bwd(const mxb_embedding_desc* d, const void* tokens, const void* d_out, void* dweight, int32_t adds, void* workspace,
+                             size_t workspace_bytes, void* stream) {
+  const mxb_status s = check_embedding_desc(d, true);
+  if (s != MXB_OK) return s;
+  if (!dweight) return MXB_ERR_INVALID_ARGUMENT;
+  if (d->tokens == 0) return adds ? MXB_OK : zeros(dweight, (size_t)d->V * d->D * element_bytes(d->out_dtype), stream);
+  if (!tokens || !d_out) return MXB_ERR_INVALID_ARGUMENT;
+  if (!workspace || workspace_bytes < embedding_bwd_scratch(d)) return MXB_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return MXB_ERR_ALIGNMENT;
+  return embedding_bwd(d, tokens, d_out, dweight, adds != 0, workspace, static_cast<cudaStream_t>(stream));
+}
+static mxb_status check_layer_norm_desc(const mxb_layer_norm_desc* d) {
+  if (!d || d->rows < 0 || d->D <= 0 || !(d->eps >= 0.f) || !element_type(d->io_dtype)) return MXB_ERR_INVALID_ARGUMENT;
+  if (d->resid_dtype != MXB_F32 && d->resid_dtype != d->io_dtype) return MXB_ERR_INVALID_ARGUMENT;
+  if (d->D > 16384) return MXB_ERR_UNSUPPORTED;
+  return MXB_OK;
+}
+mxb_status mxb_layer_norm_fwd(const mxb_layer_norm_desc* d, const void* resid, const void* x, const float* weight, const float* bias,
+                              void* stream_out, void* n, void* stream) {
+  const mxb_status s = check_layer_norm_desc(d);
+  if (s != MXB_OK) return s;
+  if (d->rows == 0) return MXB_OK;
+  if (!x || !weight || !n || (resid && !stream_out)) return MXB_ERR_INVALID_ARGUMENT;
+  return layer_norm_fwd(d, resid, x, weight, bias, stream_out, n, static_cast<cudaStream_t>(stream));
+}
+size_t mxb_layer_norm_bwd_workspace_bytes(const mxb_layer_norm_desc* d) {
+  return check_layer_norm_desc(d) == MXB_OK ? layer_norm_scratch(d) : 0;
+}
+mxb_status mxb_layer_norm_bwd(const mxb_layer_norm_desc* d, const void* x, const float* weight, const void* d_resid, const void* dn, void* dx,
+                              float* dweight, float* dbias, void* workspace, size_t workspace_bytes, void* stream) {
+  mxb_status s = check_layer_norm_desc(d);
+  if (s != MXB_OK) return s;
+  if (!weight || !dweight || !dbias) return MXB_ERR_INVALID_ARGUMENT;
+  if (d->rows == 0) {  // sums over no rows
+    s = zeros(dweight, d->D * sizeof(float), stream);
+    return s == MXB_OK ? zeros(dbias, d->D * sizeof(float), stream) : s;
+  }
+  if (!x || !dn || !dx) return MXB_ERR_INVALID_ARGUMENT;
+  if (!workspace || workspace_bytes < layer_norm_scratch(d)) return MXB_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return MXB_ERR_ALIGNMENT;
+  return layer_norm_bwd(d, x, weight, d_resid, dn, dx, dweight, dbias, static_cast<float*>(workspace), static_cast<cudaStream_t>(stream));
 }
 
 // ---------------------------------------------------------------- IR op records

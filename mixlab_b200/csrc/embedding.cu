@@ -1,0 +1,455 @@
+// Rows of the token matrix and their gradient:
+//     y_t = s W[i_t],    dW_v = s sum over the t with i_t = v of dy_t, in the order of t
+// A token outside 0 .. V-1 is padding: its row of y is zero and it has no part in dW.
+//
+// Both are HBM streams.  The gradient sorts the positions by token (stable, so that a token's positions stand in their own order
+// and the sums do not depend on how blocks run), cuts the sorted list into runs of equal length, whatever the tokens' counts are,
+// and adds up the rows of each run; a token that lies in several runs leaves a partial row in each, which a last launch adds
+// in the order of the runs.  Sums are float32 and rounded once.
+#include <algorithm>
+#include <type_traits>
+
+#include "common.cuh"
+#include "row_pieces.cuh"
+
+namespace mxb {
+namespace embed {
+
+using bf16 = __nv_bfloat16;
+
+template <typename TOK>
+__device__ __forceinline__ int token_of(const TOK* tokens, size_t t, int V) {  // V: padding
+  const TOK v = tokens[t];
+  return v >= 0 && v < (TOK)V ? (int)v : V;
+}
+// (a 32-bit token is never above what V can be)
+template <>
+__device__ __forceinline__ int token_of<int32_t>(const int32_t* tokens, size_t t, int V) {
+  const int32_t v = tokens[t];
+  return v >= 0 && v < V ? v : V;
+}
+
+// ------------------------------------------------------------------ forward
+struct FwdP {
+  const void* tokens;
+  const void* weight;
+  void* out;
+  size_t N;
+  int V, D;
+  float scale;
+};
+// TPR threads a row, a group of them takes R rows at a time.
+template <typename TOK, typename IN, typename OUT, int R, bool V>
+__global__ void __launch_bounds__(256) embedding_fwd_kernel(FwdP p, int tpr) {
+  begin_dependent();
+  const int groups = 256 / tpr, lane = threadIdx.x & (tpr - 1), group = threadIdx.x / tpr;
+  const f2 s = dup2(p.scale);
+  for (size_t t0 = ((size_t)blockIdx.x * groups + group) * R; t0 < p.N; t0 += (size_t)gridDim.x * groups * R) {
+    int tok[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) tok[r] = t0 + r < p.N ? token_of(static_cast<const TOK*>(p.tokens), t0 + r, p.V) : p.V;
+    for (int c = lane * 8; c < p.D; c += tpr * 8) {
+      f2 e[R][4];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        if (tok[r] < p.V) {
+          load8<IN, V>(static_cast<const IN*>(p.weight) + (size_t)tok[r] * p.D, c, p.D, e[r]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) e[r][i] = 0;
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        if (t0 + r >= p.N) continue;
+        if (tok[r] < p.V)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) e[r][i] = mul2(e[r][i], s);
+        store8<OUT, V>(static_cast<OUT*>(p.out) + (t0 + r) * p.D, c, p.D, e[r]);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ sorting the positions by token
+// Least significant digit first, at most 10 bits a pass.  A block takes kTile consecutive entries.
+constexpr int kTile = 2048, kSortThreads = 256, kWarps = kSortThreads / 32, kEach = kTile / kSortThreads, kMaxDigits = 1024;
+struct SortP {
+  const void* tokens;
+  const int32_t *key_in, *pos_in;  // null in the first pass
+  int32_t *key_out, *pos_out;
+  int32_t* hist;                   // [digits][tiles]
+  int N, V, shift, digits, tiles;
+};
+template <typename TOK>
+__device__ __forceinline__ int key_at(const SortP& p, int i) {
+  return p.key_in ? p.key_in[i] : token_of(static_cast<const TOK*>(p.tokens), i, p.V);
+}
+template <typename TOK>
+__global__ void __launch_bounds__(kSortThreads) embedding_count_kernel(SortP p) {
+  begin_dependent();
+  __shared__ int32_t count[kMaxDigits];
+  for (int d = threadIdx.x; d < p.digits; d += kSortThreads) count[d] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int64_t i = (int64_t)blockIdx.x * kTile + k * kSortThreads + threadIdx.x;
+    if (i < p.N) atomicAdd(&count[(key_at<TOK>(p, (int)i) >> p.shift) & (p.digits - 1)], 1);
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < p.digits; d += kSortThreads) p.hist[(size_t)d * p.tiles + blockIdx.x] = count[d];
+}
+// The counts become the places of each digit's first entry of each tile, without the digits in front: those are added where the
+// places are used, from the row ends that this leaves in total[digit].
+__global__ void __launch_bounds__(256) embedding_scan_kernel(int32_t* hist, int32_t* total, int tiles) {
+  begin_dependent();
+  __shared__ int32_t warps[8];
+  int32_t* row = hist + (size_t)blockIdx.x * tiles;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int32_t before = 0;
+  for (int t0 = 0; t0 < tiles; t0 += 256) {
+    const int t = t0 + threadIdx.x;
+    const int32_t v = t < tiles ? row[t] : 0;
+    int32_t s = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int32_t u = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += u;
+    }
+    if (lane == 31) warps[warp] = s;
+    __syncthreads();
+    int32_t base = before, all = before;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      if (w < warp) base += warps[w];
+      all += warps[w];
+    }
+    if (t < tiles) row[t] = base + s - v;
+    before = all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) total[blockIdx.x] = before;
+}
+// Each entry to its place: digits in front, tiles in front, warps in front, entries in front in the warp.
+template <typename TOK>
+__global__ void __launch_bounds__(kSortThreads) embedding_place_kernel(SortP p, const int32_t* total) {
+  begin_dependent();
+  __shared__ int32_t place[kMaxDigits];
+  __shared__ uint16_t mine[kWarps][kMaxDigits];
+  __shared__ int32_t sums[kWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int d = threadIdx.x; d < kWarps * p.digits; d += kSortThreads) mine[d / p.digits][d % p.digits] = 0;
+  // places of the digits: an exclusive sum of the totals, each thread four of them (kMaxDigits / kSortThreads)
+  int32_t v[4], sum = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int d = threadIdx.x * 4 + k;
+    v[k] = d < p.digits ? total[d] : 0;
+    sum += v[k];
+  }
+  int32_t s = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int32_t u = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += u;
+  }
+  if (lane == 31) sums[warp] = s;
+  __syncthreads();
+  s -= sum;
+  for (int w = 0; w < warp; ++w) s += sums[w];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int d = threadIdx.x * 4 + k;
+    if (d < p.digits) place[d] = s + p.hist[(size_t)d * p.tiles + blockIdx.x];
+    s += v[k];
+  }
+  // a warp takes 32 consecutive entries at a time, kEach times
+  const int64_t first = (int64_t)blockIdx.x * kTile + warp * (32 * kEach) + lane;
+  int key[kEach], rank[kEach];
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int64_t i = first + 32 * k;
+    const bool in = i < p.N;
+    key[k] = in ? key_at<TOK>(p, (int)i) : -1;
+    const int d = in ? (key[k] >> p.shift) & (p.digits - 1) : kMaxDigits;
+    const uint32_t peers = __match_any_sync(0xffffffffu, d);
+    rank[k] = 0;
+    if (in) rank[k] = mine[warp][d] + __popc(peers & ((1u << lane) - 1u));
+    __syncwarp();
+    if (in && (peers >> lane) == 1u) mine[warp][d] = (uint16_t)(rank[k] + 1);  // the last of its digit in the warp
+    __syncwarp();
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < p.digits; d += kSortThreads) {
+    int before = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const int n = mine[w][d];
+      mine[w][d] = (uint16_t)before;
+      before += n;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int64_t i = first + 32 * k;
+    if (i >= p.N) continue;
+    const int d = (key[k] >> p.shift) & (p.digits - 1), to = place[d] + mine[warp][d] + rank[k];
+    p.key_out[to] = key[k];
+    p.pos_out[to] = p.pos_in ? p.pos_in[i] : (int)i;
+  }
+}
+
+// ------------------------------------------------------------------ sums
+struct SumP {
+  const int32_t *key, *pos;  // sorted; padding (key V) stands at the end
+  const void* d_out;
+  void* dweight;
+  float* part;               // [runs][2][D]: 0 of a token that began before the run, 1 of one that goes on behind it
+  int N, V, D, run, runs, adds;
+  float scale;
+};
+template <typename OUT, bool V>
+__device__ __forceinline__ void put_row(const SumP& p, int row, int c, f2 (&acc)[4]) {
+  OUT* to = static_cast<OUT*>(p.dweight) + (size_t)row * p.D;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc[i] = mul2(acc[i], dup2(p.scale));
+  if (p.adds) {
+    f2 old[4];
+    load8<OUT, V>(to, c, p.D, old);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = add2(old[i], acc[i]);
+  }
+  store8<OUT, V>(to, c, p.D, acc);
+}
+// Blocks 0 .. ceil(runs / groups) - 1 add up the runs, those behind write zeros to the rows of tokens that do not occur.
+constexpr int kZeroRows = 32;
+template <typename IN, typename OUT, bool V>
+__global__ void __launch_bounds__(256) embedding_bwd_kernel(SumP p, int tpr, int sum_blocks) {
+  begin_dependent();
+  const int groups = 256 / tpr, lane = threadIdx.x & (tpr - 1), group = threadIdx.x / tpr;
+  if ((int)blockIdx.x >= sum_blocks) {
+    __shared__ uint32_t there;
+    const int64_t r0 = (int64_t)(blockIdx.x - sum_blocks) * kZeroRows;
+    if (threadIdx.x < kZeroRows) {  // whether row r0 + lane occurs: the first sorted entry that is not below it
+      const int64_t row = r0 + threadIdx.x;
+      int lo = 0, hi = p.N;
+      while (lo < hi) {
+        const int mid = lo + (hi - lo) / 2;
+        if (p.key[mid] < row) lo = mid + 1;
+        else hi = mid;
+      }
+      const uint32_t b = __ballot_sync(0xffffffffu, row >= p.V || (lo < p.N && p.key[lo] == row));
+      if (threadIdx.x == 0) there = b;
+    }
+    __syncthreads();
+    f2 zero[4] = {0, 0, 0, 0};
+    for (int r = group; r < kZeroRows; r += groups) {
+      if (there >> r & 1u) continue;
+      OUT* to = static_cast<OUT*>(p.dweight) + (size_t)(r0 + r) * p.D;
+      for (int c = lane * 8; c < p.D; c += tpr * 8) store8<OUT, V>(to, c, p.D, zero);
+    }
+    return;
+  }
+  const int64_t run = (int64_t)blockIdx.x * groups + group, i0 = run * p.run;
+  if (i0 >= p.N) return;
+  const int n = (int)min((int64_t)p.run, p.N - i0);
+  const int32_t *key = p.key + i0, *pos = p.pos + i0;
+  const int before = i0 > 0 ? key[-1] : -1, behind = i0 + n < p.N ? key[n] : -1;
+  constexpr int AHEAD = 8;
+  for (int c = lane * 8; c < p.D; c += tpr * 8) {
+    f2 acc[4] = {0, 0, 0, 0};
+    bool began = key[0] != before;  // the token that is being added up began in this run
+    for (int j0 = 0; j0 < n; j0 += AHEAD) {
+      f2 e[AHEAD][4];
+      int k[AHEAD + 1];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        k[j] = j0 + j < n ? key[j0 + j] : p.V;
+        if (k[j] < p.V) load8<IN, V>(static_cast<const IN*>(p.d_out) + (size_t)pos[j0 + j] * p.D, c, p.D, e[j]);
+      }
+      k[AHEAD] = j0 + AHEAD < n ? key[j0 + AHEAD] : p.V;
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        if (j0 + j >= n || k[j] >= p.V) continue;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] = add2(acc[i], e[j][i]);
+        const bool last = j0 + j + 1 == n;
+        if (k[j + 1] == k[j] && !last) continue;
+        const bool goes_on = last && behind == k[j];
+        if (began && !goes_on) put_row<OUT, V>(p, k[j], c, acc);
+        else store8<float, V>(p.part + ((size_t)run * 2 + (began ? 1 : 0)) * p.D, c, p.D, acc);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] = 0;
+        began = true;
+      }
+    }
+  }
+}
+// Tokens that lie in more than one run: the block of the run where one begins adds up its partial rows, each of its warps those of
+// consecutive runs, then the warps' sums one after the other.  grid (runs - 1, pieces of 256 columns).
+template <typename OUT, bool V>
+__global__ void __launch_bounds__(256) embedding_join_kernel(SumP p) {
+  begin_dependent();
+  __shared__ f2 sums[8][32][4];
+  const int run = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t begin = (int64_t)run * p.run, end = begin + p.run;
+  const int tok = p.key[end];  // (there is a run behind this one)
+  if (tok >= p.V || p.key[end - 1] != tok) return;
+  if (run > 0 && p.key[begin] == tok && p.key[begin - 1] == tok) return;  // it began before
+  int lo = (int)end, hi = p.N;  // the first entry behind the token's
+  while (lo < hi) {
+    const int mid = lo + (hi - lo) / 2;
+    if (p.key[mid] <= tok) lo = mid + 1;
+    else hi = mid;
+  }
+  const int n = (lo - 1) / p.run - run;  // partial rows besides the first
+  const int c = (blockIdx.y * 32 + lane) * 8, each = (n + 7) / 8, from = run + 1 + warp * each, to = min(from + each, run + 1 + n);
+  f2 acc[4] = {0, 0, 0, 0};
+  if (c < p.D) {
+    if (warp == 0) load8<float, V>(p.part + ((size_t)run * 2 + 1) * p.D, c, p.D, acc);
+    for (int r0 = from; r0 < to; r0 += 8) {
+      f2 e[8][4];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (r0 + j < to) load8<float, V>(p.part + (size_t)(r0 + j) * 2 * p.D, c, p.D, e[j]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (r0 + j < to)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[i] = add2(acc[i], e[j][i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sums[warp][lane][i] = acc[i];
+  __syncthreads();
+  if (warp != 0 || c >= p.D) return;
+  for (int w = 1; w < 8; ++w)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = add2(acc[i], sums[w][lane][i]);
+  put_row<OUT, V>(p, tok, c, acc);
+}
+
+// ------------------------------------------------------------------ host
+static int threads_per_row(int D) {  // a power of two, 8 columns a thread, 4 to 256
+  int t = 4;
+  while (8 * t < D && t < 256) t *= 2;
+  return t;
+}
+// Entries of a run: enough runs to give every SM eight blocks, 8 to 64 entries.
+static int run_length(int64_t N, int D) {
+  const int64_t groups = 256 / threads_per_row(D), want = N / (148 * 8 * groups);
+  return (int)std::min<int64_t>(64, std::max<int64_t>(8, (want + 7) / 8 * 8));
+}
+struct Scratch {
+  int32_t *key[2], *pos[2], *hist, *total;
+  float* part;
+  size_t bytes;
+  int passes, bits, run, runs, tiles;
+};
+static Scratch carve(const mxb_embedding_desc* d, void* base) {
+  Scratch s{};
+  Carver c(base);
+  const int64_t N = d->tokens;
+  int bits = 1;
+  while ((int64_t)1 << bits <= d->V) ++bits;  // keys are 0 .. V
+  s.passes = (bits + 9) / 10;
+  s.bits = (bits + s.passes - 1) / s.passes;
+  s.run = run_length(N, d->D);
+  s.runs = (int)((N + s.run - 1) / s.run);
+  s.tiles = (int)((N + kTile - 1) / kTile);
+  for (int i = 0; i < 2; ++i) {
+    s.key[i] = c.take<int32_t>(N);
+    s.pos[i] = c.take<int32_t>(N);
+  }
+  s.hist = c.take<int32_t>(((size_t)1 << s.bits) * s.tiles);
+  s.total = c.take<int32_t>((size_t)1 << s.bits);
+  s.part = c.take<float>((size_t)s.runs * 2 * d->D);
+  s.bytes = c.bytes();
+  return s;
+}
+template <typename F>
+static void with_token(const mxb_embedding_desc* d, F&& f) {
+  if (d->token_bytes == 8) f(int64_t{});
+  else f(int32_t{});
+}
+template <typename F>
+static void with_type(int32_t type, F&& f) {
+  if (type == MXB_F32) f(float{});
+  else f(bf16{});
+}
+static bool whole_pieces(int D, const void* a, const void* b) {
+  return D % 8 == 0 && ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) == 0;
+}
+
+}  // namespace embed
+
+using namespace embed;
+
+mxb_status embedding_fwd(const mxb_embedding_desc* d, const void* tokens, const void* weight, void* out, cudaStream_t st) {
+  const FwdP p{tokens, weight, out, (size_t)d->tokens, d->V, d->D, d->scale};
+  const int tpr = threads_per_row(d->D), groups = 256 / tpr;
+  auto launch = [&](auto tok, auto in, auto o, auto rows, auto whole) {
+    constexpr int R = decltype(rows)::value;
+    const int64_t want = (d->tokens + groups * R - 1) / (groups * R);
+    MXB_LAUNCH("embedding_fwd_kernel", st,
+               (launch_kernel(embedding_fwd_kernel<decltype(tok), decltype(in), decltype(o), R, decltype(whole)::value>,
+                              (unsigned)std::min<int64_t>(want, 148 * 8), 256, 0, st, p, tpr)));
+  };
+  const bool whole = whole_pieces(d->D, weight, out), many = d->tokens >= (int64_t)148 * 8 * groups;
+  with_token(d, [&](auto tok) {
+    with_type(d->io_dtype, [&](auto in) {
+      with_type(d->out_dtype, [&](auto o) {
+        auto rows = [&](auto w) {
+          if (many) launch(tok, in, o, std::integral_constant<int, 4>{}, w);
+          else launch(tok, in, o, std::integral_constant<int, 1>{}, w);
+        };
+        if (whole) rows(std::true_type{});
+        else rows(std::false_type{});
+      });
+    });
+  });
+  return check_launch("embedding_fwd");
+}
+
+size_t embedding_bwd_scratch(const mxb_embedding_desc* d) { return carve(d, nullptr).bytes; }
+
+mxb_status embedding_bwd(const mxb_embedding_desc* d, const void* tokens, const void* d_out, void* dweight, int adds, void* workspace,
+                         cudaStream_t st) {
+  const Scratch s = carve(d, workspace);
+  SortP q{tokens, nullptr, nullptr, nullptr, nullptr, s.hist, (int)d->tokens, d->V, 0, 1 << s.bits, s.tiles};
+  int at = 0;
+  for (int pass = 0; pass < s.passes; ++pass, at ^= 1) {
+    q.shift = pass * s.bits;
+    q.key_out = s.key[at];
+    q.pos_out = s.pos[at];
+    with_token(d, [&](auto tok) {
+      using TOK = decltype(tok);
+      MXB_LAUNCH("embedding_count_kernel", st, (launch_kernel(embedding_count_kernel<TOK>, s.tiles, kSortThreads, 0, st, q)));
+      MXB_LAUNCH("embedding_scan_kernel", st, (launch_kernel(embedding_scan_kernel, 1 << s.bits, 256, 0, st, s.hist, s.total, s.tiles)));
+      MXB_LAUNCH("embedding_place_kernel", st, (launch_kernel(embedding_place_kernel<TOK>, s.tiles, kSortThreads, 0, st, q, s.total)));
+    });
+    q.key_in = q.key_out;
+    q.pos_in = q.pos_out;
+  }
+  const SumP p{q.key_in, q.pos_in, d_out, dweight, s.part, (int)d->tokens, d->V, d->D, s.run, s.runs, adds, d->scale};
+  const int tpr = threads_per_row(d->D), groups = 256 / tpr, sums = (s.runs + groups - 1) / groups;
+  const int zeros = adds ? 0 : (int)(((int64_t)d->V + kZeroRows - 1) / kZeroRows);
+  with_type(d->io_dtype, [&](auto in) {
+    with_type(d->out_dtype, [&](auto o) {
+      auto launch = [&](auto whole) {
+        constexpr bool W = decltype(whole)::value;
+        MXB_LAUNCH("embedding_bwd_kernel", st,
+                   (launch_kernel(embedding_bwd_kernel<decltype(in), decltype(o), W>, sums + zeros, 256, 0, st, p, tpr, sums)));
+        if (s.runs > 1)
+          MXB_LAUNCH("embedding_join_kernel", st,
+                     (launch_kernel(embedding_join_kernel<decltype(o), W>, dim3(s.runs - 1, (d->D + 255) / 256), 256, 0, st, p)));
+      };
+      if (whole_pieces(d->D, d_out, dweight)) launch(std::true_type{});
+      else launch(std::false_type{});
+    });
+  });
+  return check_launch("embedding_bwd");
+}
+
+}  // namespace mxb

@@ -37,6 +37,8 @@ namespace {
   X(mxb_mamba3_block_bc_fwd) X(mxb_mamba3_block_bc_bwd) X(mxb_mamba3_block_post_fwd) X(mxb_mamba3_block_post_bwd)     \
   X(mxb_mamba3_prefill_workspace_bytes) X(mxb_mamba3_prefill) X(mxb_mamba3_decode_step) X(mxb_short_conv_prefill)    \
   X(mxb_short_conv_step) X(mxb_residual_norm_workspace_bytes) X(mxb_residual_norm_fwd) X(mxb_residual_norm_bwd)       \
+  X(mxb_embedding_fwd) X(mxb_embedding_bwd_workspace_bytes) X(mxb_embedding_bwd) X(mxb_layer_norm_fwd)                \
+  X(mxb_layer_norm_bwd_workspace_bytes) X(mxb_layer_norm_bwd)                                                         \
   X(mxb_ir_op_workspace_bytes) X(mxb_ir_op_forward)
 struct Abi {
 #define X(name) decltype(&::name) name = nullptr;
@@ -805,6 +807,107 @@ py::dict residual_norm_backward(const Tensor& resid_out, const Tensor& y, const 
   return r;
 }
 
+// ------------------------------------------------------------------ the ends of a training step
+// A dtype argument: None, or one of the two element types.
+at::ScalarType dtype_or(const py::object& dtype, at::ScalarType otherwise) {
+  if (dtype.is_none()) return otherwise;
+  if (!THPDtype_Check(dtype.ptr())) throw py::type_error("dtype: torch.float32, torch.bfloat16 or None expected");
+  const at::ScalarType t = reinterpret_cast<THPDtype*>(dtype.ptr())->scalar_type;
+  if (t != at::kFloat && t != at::kBFloat16) throw py::type_error(std::string("dtype: ") + c10::toString(t) + " (float32 or bfloat16)");
+  return t;
+}
+int32_t code_of(at::ScalarType t) { return t == at::kFloat ? MXB_F32 : MXB_BF16; }
+// Token numbers, int32 or int64: bytes of one.
+int32_t check_tokens(const Tensor& t, Shape shape, at::Device dev, const char* name) {
+  if (!t.is_cuda()) not_cuda();
+  const bool wide = t.scalar_type() == at::kLong;
+  if (!wide && t.scalar_type() != at::kInt) throw py::type_error(std::string(name) + ": dtype " + c10::toString(t.scalar_type()) + ", expected Int or Long");
+  check(t, shape, t.scalar_type(), dev, name);
+  return wide ? 8 : 4;
+}
+Tensor embedding(const Tensor& tokens, const Tensor& weight, double scale, const py::object& dtype) {
+  const at::Device dev = cuda_device(weight);
+  const int32_t io = io_code(weight);
+  if (weight.dim() != 2) throw py::value_error("weight must be [V,D]");
+  check(weight, weight.sizes(), weight.scalar_type(), dev, "weight");
+  const int32_t bytes = check_tokens(tokens, tokens.sizes(), dev, "tokens");
+  const at::ScalarType to = dtype_or(dtype, weight.scalar_type());
+  const mxb_embedding_desc d{tokens.numel(), i32(weight.size(0), "V"), i32(weight.size(1), "D"), bytes, io, code_of(to), (float)scale};
+  std::vector<int64_t> shape = tokens.sizes().vec();
+  shape.push_back(weight.size(1));
+  const On on(dev);
+  Tensor out = make(shape, to, on.dev);
+  call("mxb_embedding_fwd", abi.mxb_embedding_fwd, &d, ptr(tokens), ptr(weight), ptr(out), on.stream);
+  return out;
+}
+Tensor embedding_backward(const Tensor& tokens, const Tensor& d_out, int64_t V, double scale, const py::object& dtype, const Opt& dweight) {
+  const at::Device dev = cuda_device(d_out);
+  const int32_t io = io_code(d_out);
+  if (d_out.dim() < 1) throw py::value_error("d_out must be [...,D]");
+  const int64_t D = d_out.size(-1), vd[] = {V, D};
+  check(d_out, d_out.sizes(), d_out.scalar_type(), dev, "d_out");
+  const int32_t bytes = check_tokens(tokens, d_out.sizes().slice(0, d_out.dim() - 1), dev, "tokens");
+  const at::ScalarType to = dtype_or(dtype, dweight ? dweight->scalar_type() : d_out.scalar_type());
+  if (V <= 0) throw py::value_error("V must be positive");
+  if (dweight) {
+    if (to != at::kFloat && to != at::kBFloat16) io_code(*dweight);  // (throws)
+    check(dweight, vd, to, dev, "dweight");
+    check_apart(*dweight, nullptr, {{&d_out, "d_out"}, {&tokens, "tokens"}});
+  }
+  const mxb_embedding_desc d{tokens.numel(), i32(V, "V"), i32(D, "D"), bytes, io, code_of(to), (float)scale};
+  const On on(dev);
+  Tensor dw = dweight ? *dweight : make(vd, to, on.dev);
+  call_with_scratch(on, abi.mxb_embedding_bwd_workspace_bytes(&d), "mxb_embedding_bwd", abi.mxb_embedding_bwd, &d, ptr(tokens), ptr(d_out), ptr(dw),
+                    (int32_t)dweight.has_value());
+  return dw;
+}
+// x (the stream's type where there is none beside it), weight and bias.
+mxb_layer_norm_desc check_layer_norm(at::Device dev, const Tensor& x, at::ScalarType io, at::ScalarType res, const Tensor& weight, const Opt& bias,
+                                     double eps) {
+  if (x.dim() < 1) throw py::value_error("x must be [...,D]");
+  const int64_t D = x.size(-1);
+  check(x, x.sizes(), x.scalar_type(), dev, "x");
+  check(weight, Shape(&D, 1), F, dev, "weight");
+  check(bias, Shape(&D, 1), F, dev, "bias");
+  return {D > 0 ? x.numel() / D : 0, i32(D, "D"), code_of(io), code_of(res), (float)eps};
+}
+py::object layer_norm(const Tensor& x, const Tensor& weight, const Opt& bias, const Opt& resid, double eps, const py::object& dtype) {
+  const at::Device dev = cuda_device(x);
+  io_code(x);
+  const at::ScalarType to = dtype_or(dtype, x.scalar_type());
+  if (resid && to != x.scalar_type()) throw py::type_error("dtype: with resid the norm has x's type");
+  if (to == F && x.scalar_type() != F) throw py::type_error("dtype: Float for a BFloat16 x (x's type, or BFloat16 for a Float x)");
+  if (resid) io_code(*resid);
+  const at::ScalarType res = resid ? resid->scalar_type() : x.scalar_type();
+  if (resid && res != to && res != F) throw py::type_error("resid: BFloat16 beside a Float x (one type, or a Float resid)");
+  const mxb_layer_norm_desc d = check_layer_norm(dev, x, to, res, weight, bias, eps);
+  check(resid, x.sizes(), res, dev, "resid");
+  const On on(dev);
+  Tensor n = make(x.sizes(), to, on.dev);
+  Opt stream;
+  if (resid) stream = like(*resid);
+  call("mxb_layer_norm_fwd", abi.mxb_layer_norm_fwd, &d, ptr(resid), ptr(x), ptr<float>(weight), ptr<float>(bias), ptr(stream), ptr(n), on.stream);
+  return resid ? py::object(py::make_tuple(*stream, n)) : py::cast(n);
+}
+py::dict layer_norm_backward(const Tensor& x, const Tensor& weight, const Tensor& dn, const Opt& d_resid, double eps) {
+  const at::Device dev = cuda_device(x);
+  io_code(x);
+  if (!dn.is_cuda()) not_cuda();
+  io_code(dn);
+  if (dn.scalar_type() != x.scalar_type() && x.scalar_type() != F) throw py::type_error("dn: Float beside a BFloat16 x (one type, or a Float x)");
+  const Opt none;
+  const mxb_layer_norm_desc d = check_layer_norm(dev, x, dn.scalar_type(), x.scalar_type(), weight, none, eps);
+  check(dn, x.sizes(), dn.scalar_type(), dev, "dn");
+  check(d_resid, x.sizes(), x.scalar_type(), dev, "d_resid");
+  const On on(dev);
+  Tensor dx = like(x), dw = like(weight), db = like(weight);
+  call_with_scratch(on, abi.mxb_layer_norm_bwd_workspace_bytes(&d), "mxb_layer_norm_bwd", abi.mxb_layer_norm_bwd, &d, ptr(x), ptr<float>(weight),
+                    ptr(d_resid), ptr(dn), ptr(dx), ptr<float>(dw), ptr<float>(db));
+  py::dict r;
+  r["dx"] = dx; r["dweight"] = dw; r["dbias"] = db;
+  return r;
+}
+
 // ------------------------------------------------------------------ IR op records
 Tensor ir_op_forward(int64_t op_type, const std::vector<Tensor>& inputs, const std::vector<int64_t>& int_params,
                      const std::vector<int64_t>& out_shape, const std::vector<double>& float_params) {
@@ -856,4 +959,8 @@ PYBIND11_MODULE(_front, m) {
   m.def("short_conv_step", &short_conv_step);
   m.def("residual_norm", &residual_norm);
   m.def("residual_norm_backward", &residual_norm_backward);
+  m.def("embedding", &embedding);
+  m.def("embedding_backward", &embedding_backward);
+  m.def("layer_norm", &layer_norm);
+  m.def("layer_norm_backward", &layer_norm_backward);
 }

@@ -233,3 +233,31 @@ def residual_norm_backward(resid_out, y, norm, d_resid_out, dn, *, post_norm=Non
     """Gradients of ``residual_norm``: resid_out is what it returned, d_resid_out (None: zero) and dn the gradients of its two
     results.  dict(d_resid, dy, dz, dnorm, dpost_norm, dscale), None for operands that were left out."""
     return (_front or _native()).residual_norm_backward(resid_out, y, norm, d_resid_out, dn, post_norm, z, scale, eps)
+
+
+# ---------------------------------------------------------------- the ends of a training step
+def embedding(tokens, weight, *, scale=1.0, dtype=None):
+    """The residual stream's first value: rows of weight [V,D] by tokens [...] (int32 or int64), times scale, in ``dtype`` (None: the
+    weight's; float32 or bfloat16).  A token outside 0 .. V-1 is padding: a row of zeros."""
+    return (_front or _native()).embedding(tokens, weight, scale, dtype)
+
+
+def embedding_backward(tokens, d_out, V, *, scale=1.0, dtype=None, dweight=None):
+    """Gradient of ``embedding`` by its weight: [V,D] in ``dtype`` (None: d_out's), the rows of d_out [...,D] summed by token in their
+    own order in float32, times scale; padding has no part.  ``dweight``: a gradient [V,D] that the sums are added to in place
+    (a matrix that the output head shares) and that is returned."""
+    return (_front or _native()).embedding_backward(tokens, d_out, V, scale, dtype, dweight)
+
+
+def layer_norm(x, weight, bias=None, *, resid=None, eps=1e-5, dtype=None):
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last axis; x [...,D], weight, bias [D] float32, the result in ``dtype``
+    (None: x's; bfloat16 for a float32 x).  With ``resid`` [...,D] (x's type or float32) the residual stream between two blocks:
+    returns resid + x, in resid's type, and its norm in x's.  D <= 16384."""
+    return (_front or _native()).layer_norm(x, weight, bias, resid, eps, dtype)
+
+
+def layer_norm_backward(x, weight, dn, *, d_resid=None, eps=1e-5):
+    """Gradients of ``layer_norm``: x is what was normalised (with ``resid``: the stream that it returned), dn the gradient of the norm
+    (x's type, or bfloat16 beside a float32 x), d_resid (x's type; None: zero) the gradient that reaches x from its other readers.
+    dict(dx, dweight, dbias), dx in x's type, the others float32."""
+    return (_front or _native()).layer_norm_backward(x, weight, dn, d_resid, eps)
