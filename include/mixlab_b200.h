@@ -455,6 +455,32 @@ MXB_API mxb_status mxb_layer_norm_bwd(const mxb_layer_norm_desc* d, const void* 
                                       size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------
+ * The output head and its loss without the logits in memory, and every gradient:
+ *   z_tv = x_t . W_v;  lse_t = log sum_v exp z_tv;  loss_t = lse_t - z_t,target_t
+ *   g_tv = (d_loss_t + d_lse_t) exp(z_tv - lse_t) - d_loss_t [v = target_t];  dx = g W;  dW = g^T x
+ * x, dx [rows, D], weight, dweight [V, D] in io_dtype; targets [rows] int32 or int64 (target_bytes 4 or
+ * 8); loss, lse, d_loss, d_lse [rows] float32, d_lse may be NULL (zero), lse in the backward is what the
+ * forward returned.  A row whose target is outside 0..V-1 has no part: its loss, lse and dx are zero and
+ * its x may hold anything; the same holds in the backward for a row whose d_loss and d_lse are zero.
+ * bf16: products of bf16 on the tensor cores added up in float32, g rounded to bf16 for the last two.  float32:
+ * operands in three bf16 parts, the error of float32 products.  The backward keeps g for a piece of the
+ * vocabulary at a time, at most 512 MB or 256 columns.  bf16 weights with D a multiple of 8 must lie on
+ * 16 bytes; everything else may start at any element.  The workspace's first word is the kernels'
+ * error word (mxb_gdn_device_status).
+ * ---------------------------------------------------------------------- */
+typedef struct {
+  int64_t rows;
+  int32_t V, D, target_bytes, io_dtype;
+} mxb_linear_ce_desc;
+MXB_API size_t mxb_linear_ce_fwd_workspace_bytes(const mxb_linear_ce_desc* d);
+MXB_API size_t mxb_linear_ce_bwd_workspace_bytes(const mxb_linear_ce_desc* d);
+MXB_API mxb_status mxb_linear_ce_fwd(const mxb_linear_ce_desc* d, const void* x, const void* weight, const void* targets,
+                                     float* loss, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+MXB_API mxb_status mxb_linear_ce_bwd(const mxb_linear_ce_desc* d, const void* x, const void* weight, const void* targets,
+                                     const float* lse, const float* d_loss, const float* d_lse, void* dx, void* dweight,
+                                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * Data-parallel gradient exchange: the element-wise passes on either side of the
  * per-bucket all-reduce, over flat float32 buckets on the device (the collective
  * itself is the caller's: NCCL).  They fuse what the reference does op by op per

@@ -67,6 +67,10 @@ class LayerNormDesc(C.Structure):
     _fields_ = [("rows", C.c_int64), ("D", C.c_int32), ("io_dtype", C.c_int32), ("resid_dtype", C.c_int32), ("eps", C.c_float)]
 
 
+class LinearCeDesc(C.Structure):
+    _fields_ = [("rows", C.c_int64)] + [(n, C.c_int32) for n in ("V", "D", "target_bytes", "io_dtype")]
+
+
 class IrOp(C.Structure):
     """mxb_ir_op: an IR op record (mlx_ir_program_add_op) after name resolution."""
     _fields_ = [("op_type", C.c_int32), ("inputs", C.POINTER(C.c_void_p)), ("n_inputs", C.c_int32),
@@ -122,6 +126,10 @@ EXPORTS = {
     "mxb_layer_norm_fwd": (C.c_int32, [C.POINTER(LayerNormDesc)] + [_P] * 7),
     "mxb_layer_norm_bwd_workspace_bytes": (C.c_size_t, [C.POINTER(LayerNormDesc)]),
     "mxb_layer_norm_bwd": (C.c_int32, [C.POINTER(LayerNormDesc)] + [_P] * 8 + [C.c_size_t, _P]),
+    "mxb_linear_ce_fwd_workspace_bytes": (C.c_size_t, [C.POINTER(LinearCeDesc)]),
+    "mxb_linear_ce_bwd_workspace_bytes": (C.c_size_t, [C.POINTER(LinearCeDesc)]),
+    "mxb_linear_ce_fwd": (C.c_int32, [C.POINTER(LinearCeDesc)] + [_P] * 6 + [C.c_size_t, _P]),
+    "mxb_linear_ce_bwd": (C.c_int32, [C.POINTER(LinearCeDesc)] + [_P] * 9 + [C.c_size_t, _P]),
     "mxb_dp_partial_floats": (C.c_size_t, []),
     "mxb_dp_sanitize": (C.c_int32, [_P, C.c_size_t, C.c_float, _P, _P]),
     "mxb_dp_finalize": (C.c_int32, [_P, C.c_size_t, C.c_float, C.c_float, _P, _P, _P]),

@@ -132,6 +132,10 @@ size_t layer_norm_scratch(const mxb_layer_norm_desc*);
 mxb_status layer_norm_fwd(const mxb_layer_norm_desc*, const void*, const void*, const float*, const float*, void*, void*, cudaStream_t);
 mxb_status layer_norm_bwd(const mxb_layer_norm_desc*, const void*, const float*, const void*, const void*, void*, float*, float*, float*,
                           cudaStream_t);
+size_t linear_ce_scratch(const mxb_linear_ce_desc*, bool bwd);
+mxb_status linear_ce_fwd(const mxb_linear_ce_desc*, const void*, const void*, const void*, float*, float*, void*, cudaStream_t);
+mxb_status linear_ce_bwd(const mxb_linear_ce_desc*, const void*, const void*, const void*, const float*, const float*, const float*, void*, void*,
+                         void*, cudaStream_t);
 bool mamba3_block_supported(const mxb_mamba3_desc*);
 size_t mamba3_block_workspace_bytes(const mxb_mamba3_desc*);
 mxb_status mamba3_block_conv(const mxb_mamba3_desc*, int, const void*, const float*, void*, const void*, void*, float*,
@@ -618,6 +622,49 @@ mxb_status mxb_layer_norm_bwd(const mxb_layer_norm_desc* d, const void* x, const
   if (!workspace || workspace_bytes < layer_norm_scratch(d)) return MXB_ERR_WORKSPACE;
   if (!aligned16(workspace)) return MXB_ERR_ALIGNMENT;
   return layer_norm_bwd(d, x, weight, d_resid, dn, dx, dweight, dbias, static_cast<float*>(workspace), static_cast<cudaStream_t>(stream));
+}
+
+static mxb_status check_linear_ce_desc(const mxb_linear_ce_desc* d) {
+  if (!d || d->rows < 0 || d->V <= 0 || d->D <= 0 || (d->target_bytes != 4 && d->target_bytes != 8) || !element_type(d->io_dtype))
+    return MXB_ERR_INVALID_ARGUMENT;
+  // the kernels count tiles of 256 x 128 and rows of tiles in 32 bits
+  if (d->rows > INT32_MAX / 2 || d->V > INT32_MAX - 512 || d->D > INT32_MAX / 16) return MXB_ERR_UNSUPPORTED;
+  const int64_t m = (d->rows + 255) / 256, n = ((int64_t)d->V + 127) / 128, k = ((int64_t)d->D + 127) / 128;
+  if (m * n > INT32_MAX / 2 || m * k > INT32_MAX / 256 || n * k > INT32_MAX / 256) return MXB_ERR_UNSUPPORTED;
+  return MXB_OK;
+}
+static mxb_status check_linear_ce(const mxb_linear_ce_desc* d, const void* weight, const void* ws, size_t bytes, size_t need) {
+  if (!ws || bytes < need) return MXB_ERR_WORKSPACE;
+  if (!aligned16(ws) || (d->io_dtype == MXB_BF16 && d->D % 8 == 0 && !aligned16(weight))) return MXB_ERR_ALIGNMENT;
+  return MXB_OK;
+}
+size_t mxb_linear_ce_fwd_workspace_bytes(const mxb_linear_ce_desc* d) {
+  return check_linear_ce_desc(d) == MXB_OK ? linear_ce_scratch(d, false) : 0;
+}
+size_t mxb_linear_ce_bwd_workspace_bytes(const mxb_linear_ce_desc* d) {
+  return check_linear_ce_desc(d) == MXB_OK ? linear_ce_scratch(d, true) : 0;
+}
+mxb_status mxb_linear_ce_fwd(const mxb_linear_ce_desc* d, const void* x, const void* weight, const void* targets, float* loss, float* lse,
+                             void* workspace, size_t workspace_bytes, void* stream) {
+  mxb_status s = check_linear_ce_desc(d);
+  if (s != MXB_OK) return s;
+  if (d->rows == 0) return MXB_OK;
+  if (!x || !weight || !targets || !loss || !lse) return MXB_ERR_INVALID_ARGUMENT;
+  s = check_linear_ce(d, weight, workspace, workspace_bytes, linear_ce_scratch(d, false));
+  if (s != MXB_OK) return s;
+  return linear_ce_fwd(d, x, weight, targets, loss, lse, workspace, static_cast<cudaStream_t>(stream));
+}
+mxb_status mxb_linear_ce_bwd(const mxb_linear_ce_desc* d, const void* x, const void* weight, const void* targets, const float* lse,
+                             const float* d_loss, const float* d_lse, void* dx, void* dweight, void* workspace, size_t workspace_bytes,
+                             void* stream) {
+  mxb_status s = check_linear_ce_desc(d);
+  if (s != MXB_OK) return s;
+  if (!dweight) return MXB_ERR_INVALID_ARGUMENT;
+  if (d->rows == 0) return zeros(dweight, (size_t)d->V * d->D * element_bytes(d->io_dtype), stream);  // sums over no tokens
+  if (!x || !weight || !targets || !lse || !d_loss || !dx) return MXB_ERR_INVALID_ARGUMENT;
+  s = check_linear_ce(d, weight, workspace, workspace_bytes, linear_ce_scratch(d, true));
+  if (s != MXB_OK) return s;
+  return linear_ce_bwd(d, x, weight, targets, lse, d_loss, d_lse, dx, dweight, workspace, static_cast<cudaStream_t>(stream));
 }
 
 // ---------------------------------------------------------------- IR op records

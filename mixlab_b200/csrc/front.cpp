@@ -38,7 +38,8 @@ namespace {
   X(mxb_mamba3_prefill_workspace_bytes) X(mxb_mamba3_prefill) X(mxb_mamba3_decode_step) X(mxb_short_conv_prefill)    \
   X(mxb_short_conv_step) X(mxb_residual_norm_workspace_bytes) X(mxb_residual_norm_fwd) X(mxb_residual_norm_bwd)       \
   X(mxb_embedding_fwd) X(mxb_embedding_bwd_workspace_bytes) X(mxb_embedding_bwd) X(mxb_layer_norm_fwd)                \
-  X(mxb_layer_norm_bwd_workspace_bytes) X(mxb_layer_norm_bwd)                                                         \
+  X(mxb_layer_norm_bwd_workspace_bytes) X(mxb_layer_norm_bwd) X(mxb_linear_ce_fwd_workspace_bytes)                    \
+  X(mxb_linear_ce_bwd_workspace_bytes) X(mxb_linear_ce_fwd) X(mxb_linear_ce_bwd)                                      \
   X(mxb_ir_op_workspace_bytes) X(mxb_ir_op_forward)
 struct Abi {
 #define X(name) decltype(&::name) name = nullptr;
@@ -908,6 +909,42 @@ py::dict layer_norm_backward(const Tensor& x, const Tensor& weight, const Tensor
   return r;
 }
 
+mxb_linear_ce_desc check_linear_ce(at::Device dev, const Tensor& x, const Tensor& weight, const Tensor& targets) {
+  if (x.dim() < 1) throw py::value_error("x must be [...,D]");
+  const int32_t io = io_code(x);
+  const int64_t D = x.size(-1);
+  check(x, x.sizes(), x.scalar_type(), dev, "x");
+  if (!weight.is_cuda()) not_cuda();
+  if (weight.dim() != 2) throw py::value_error("weight: shape " + text(weight.sizes()) + ", expected (V, " + std::to_string(D) + ")");
+  const int64_t V = weight.size(0), vd[] = {V, D};
+  check(weight, vd, x.scalar_type(), dev, "weight");
+  const int32_t bytes = check_tokens(targets, x.sizes().slice(0, x.dim() - 1), dev, "targets");
+  return {targets.numel(), i32(V, "V"), i32(D, "D"), bytes, io};
+}
+py::tuple linear_ce(const Tensor& x, const Tensor& weight, const Tensor& targets) {
+  const at::Device dev = cuda_device(x);
+  const mxb_linear_ce_desc d = check_linear_ce(dev, x, weight, targets);
+  const On on(dev);
+  Tensor loss = make(targets.sizes(), F, on.dev), lse = make(targets.sizes(), F, on.dev);
+  call_with_scratch(on, abi.mxb_linear_ce_fwd_workspace_bytes(&d), "mxb_linear_ce_fwd", abi.mxb_linear_ce_fwd, &d, ptr(x), ptr(weight), ptr(targets),
+                    ptr<float>(loss), ptr<float>(lse));
+  return py::make_tuple(loss, lse);
+}
+py::dict linear_ce_backward(const Tensor& x, const Tensor& weight, const Tensor& targets, const Tensor& lse, const Tensor& d_loss, const Opt& d_lse) {
+  const at::Device dev = cuda_device(x);
+  const mxb_linear_ce_desc d = check_linear_ce(dev, x, weight, targets);
+  check(lse, targets.sizes(), F, dev, "lse");
+  check(d_loss, targets.sizes(), F, dev, "d_loss");
+  check(d_lse, targets.sizes(), F, dev, "d_lse");
+  const On on(dev);
+  Tensor dx = like(x), dw = like(weight);
+  call_with_scratch(on, abi.mxb_linear_ce_bwd_workspace_bytes(&d), "mxb_linear_ce_bwd", abi.mxb_linear_ce_bwd, &d, ptr(x), ptr(weight), ptr(targets),
+                    ptr<float>(lse), ptr<float>(d_loss), ptr<float>(d_lse), ptr(dx), ptr(dw));
+  py::dict r;
+  r["dx"] = dx; r["dweight"] = dw;
+  return r;
+}
+
 // ------------------------------------------------------------------ IR op records
 Tensor ir_op_forward(int64_t op_type, const std::vector<Tensor>& inputs, const std::vector<int64_t>& int_params,
                      const std::vector<int64_t>& out_shape, const std::vector<double>& float_params) {
@@ -963,4 +1000,6 @@ PYBIND11_MODULE(_front, m) {
   m.def("embedding_backward", &embedding_backward);
   m.def("layer_norm", &layer_norm);
   m.def("layer_norm_backward", &layer_norm_backward);
+  m.def("linear_ce", &linear_ce);
+  m.def("linear_ce_backward", &linear_ce_backward);
 }

@@ -1,0 +1,881 @@
+// The output head and its loss, without the logits in memory:
+//     z_tv = x_t . W_v,   lse_t = log sum_v exp z_tv,   loss_t = lse_t - z_t,i_t
+// and its gradients: with a_t, c_t the gradients of loss_t and lse_t,
+//     g_tv = (a_t + c_t) exp(z_tv - lse_t) - a_t [v = i_t],   dx = g W,   dW = g^T x
+// Tokens whose target is outside 0 .. V-1 (in the backward pass also those whose a and c are zero) have no part: a first launch
+// moves the rows of the others together, so that they are neither computed nor read (they may hold anything).
+//
+// Products on the tensor cores, 256 x 256 a pair of CTAs, fed by TMA through a ring of shared-memory stages; two accumulators
+// in TMEM, so that one is read while the other is filled.  Forward: the accumulator is reduced to the maximum and the sum of
+// exponentials of each row over the tile's columns, 8 bytes a row and tile.  Backward, in pieces of the vocabulary: z again, g in
+// bf16 to a workspace of bounded size, then dx += g W and dW = g^T x from it.
+// float32 tensors: every operand is split into three bf16 parts (24 bits and more), and six products of parts, those above
+// 2^-24, are added up: the first in an accumulator of its own, as the others are 2^-8 and less of it.
+#include <cuda.h>
+
+#include <algorithm>
+#include <cstring>
+#include <type_traits>
+
+#include "common.cuh"
+#include "packed.cuh"
+#include "umma_tiles.cuh"
+
+namespace mxb {
+namespace lce {
+
+using bf16 = __nv_bfloat16;
+constexpr float kLog2e = 1.4426950408889634f;
+
+// ------------------------------------------------------------------ tokens that count
+constexpr int kCountRows = 1024;  // rows whose tokens one block counts
+struct PackP {
+  const void* targets;
+  const void* x;
+  const float *lse, *d_loss, *d_lse;  // backward; d_lse may be null
+  const int32_t* counts;              // of every kCountRows rows (where there are as many)
+  int32_t *live, *idx, *tgt;          // how many; their rows; their targets
+  float *a, *both, *lse2;             // their gradients of loss and of both, lse in powers of two
+  bf16* xc;                           // [parts][pad][Dp]
+  void* dx;                           // backward: rows of the other tokens become zero
+  float *loss, *lse_out;              // forward: likewise
+  int32_t* status;
+  size_t N, pad;
+  int V, D, Dp, wide, f32;            // wide: targets of 64 bits
+};
+__device__ __forceinline__ int target_of(const PackP& p, size_t t) {  // -1: none
+  const int64_t v = p.wide ? static_cast<const int64_t*>(p.targets)[t] : static_cast<const int32_t*>(p.targets)[t];
+  return v >= 0 && v < p.V ? (int)v : -1;
+}
+__device__ __forceinline__ bool counts(const PackP& p, size_t t) {
+  if (target_of(p, t) < 0) return false;
+  if (!p.d_loss) return true;
+  return !(p.d_loss[t] == 0.f) || (p.d_lse && !(p.d_lse[t] == 0.f));
+}
+__device__ __forceinline__ int block_sum(int v, int32_t* red) {  // 256 threads
+  v = __reduce_add_sync(0xffffffffu, v);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  int s = 0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) s += red[w];
+  return s;
+}
+// How many of the tokens in front of t count.
+__device__ __forceinline__ int counted_before(const PackP& p, size_t t, int32_t* red) {
+  const size_t blocks = t / kCountRows;
+  int n = 0;
+  for (size_t b = threadIdx.x; b < blocks; b += 256) n += p.counts[b];
+  for (size_t i = blocks * kCountRows + threadIdx.x; i < t; i += 256) n += counts(p, i);
+  return block_sum(n, red);
+}
+__global__ void __launch_bounds__(256) lce_count_kernel(PackP p, int32_t* out) {
+  begin_dependent();
+  __shared__ int32_t red[8];
+  int n = 0;
+  for (int k = 0; k < kCountRows / 256; ++k) {
+    const size_t t = (size_t)blockIdx.x * kCountRows + k * 256 + threadIdx.x;
+    n += t < p.N && counts(p, t);
+  }
+  n = block_sum(n, red);
+  if (threadIdx.x == 0) out[blockIdx.x] = n;
+}
+// A value in bf16 parts, the first the nearest to it, each other the nearest to what is left.
+template <int PARTS>
+__device__ __forceinline__ void split(float v, bf16 (&part)[PARTS]) {
+#pragma unroll
+  for (int k = 0; k < PARTS; ++k) {
+    part[k] = __float2bfloat16_rn(v);
+    // (what is left of an infinity or a NaN would be a NaN)
+    v = k + 1 < PARTS ? (isfinite(v) ? v - __bfloat162float(part[k]) : 0.f) : 0.f;
+  }
+}
+// Row `from` of a matrix with D columns (null: zeros) to row `to` of its packed form, by one warp.
+template <typename T>
+__device__ __forceinline__ void pack_row(const T* from, bf16* to, size_t part_stride, int D, int Dp, int lane) {
+  constexpr int PARTS = sizeof(T) == 4 ? 3 : 1;
+  const bool whole = D % 8 == 0 && (reinterpret_cast<uintptr_t>(from) & 15) == 0;  // (Dp is a multiple of 8)
+  for (int c = lane * 8; c < Dp; c += 256) {
+    if (PARTS == 1 && whole) {
+      *reinterpret_cast<uint4*>(to + c) = from ? *reinterpret_cast<const uint4*>(from + c) : make_uint4(0, 0, 0, 0);
+      continue;
+    }
+    float v[8];
+    if (whole && from && sizeof(T) == 4) {
+      const float4 lo = *reinterpret_cast<const float4*>(from + c), hi = *reinterpret_cast<const float4*>(from + c + 4);
+      v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w; v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = from && c + i < D ? to_f32(from[c + i]) : 0.f;
+    }
+    bf16 e[PARTS][8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      bf16 part[PARTS];
+      split<PARTS>(v[i], part);
+#pragma unroll
+      for (int k = 0; k < PARTS; ++k) e[k][i] = part[k];
+    }
+#pragma unroll
+    for (int k = 0; k < PARTS; ++k) *reinterpret_cast<uint4*>(to + k * part_stride + c) = *reinterpret_cast<uint4*>(e[k]);
+  }
+}
+// Blocks of eight rows, a warp each; 32 blocks behind them fill up the last tile of 256 rows with zeros.
+template <typename T>
+__global__ void __launch_bounds__(256) lce_pack_kernel(PackP p, int row_blocks) {
+  begin_dependent();
+  __shared__ int32_t red[8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if ((int)blockIdx.x >= row_blocks) {
+    const int live = counted_before(p, p.N, red), k = ((int)blockIdx.x - row_blocks) * 8 + warp;
+    const size_t j = (size_t)live + k;
+    if (blockIdx.x == row_blocks && threadIdx.x == 0) {
+      *p.live = live;
+      *p.status = 0;
+    }
+    if (j >= ((size_t)live + 255) / 256 * 256) return;
+    pack_row<T>(nullptr, p.xc + j * p.Dp, p.pad * p.Dp, p.D, p.Dp, lane);
+    if (lane == 0) {
+      p.tgt[j] = -1;
+      if (p.d_loss) p.a[j] = p.both[j] = p.lse2[j] = 0.f;
+    }
+    return;
+  }
+  const size_t r0 = (size_t)blockIdx.x * 8, r = r0 + warp;
+  const int before = counted_before(p, r0, red);
+  bool mine = r < p.N && counts(p, r);
+  __syncthreads();  // (the sum has been read)
+  if (lane == 0) red[warp] = mine;
+  __syncthreads();
+  if (r >= p.N) return;
+  if (!mine) {
+    if (p.d_loss) {
+      T* to = static_cast<T*>(p.dx) + r * p.D;
+      for (int c = lane; c < p.D; c += 32) to[c] = from_f32<T>(0.f);
+    } else if (lane == 0) {
+      p.loss[r] = p.lse_out[r] = 0.f;
+    }
+    return;
+  }
+  size_t j = before;
+  for (int w = 0; w < warp; ++w) j += red[w];
+  if (lane == 0) {
+    p.idx[j] = (int32_t)r;
+    p.tgt[j] = target_of(p, r);
+    if (p.d_loss) {
+      const float a = p.d_loss[r];
+      p.a[j] = a;
+      p.both[j] = p.d_lse ? a + p.d_lse[r] : a;
+      p.lse2[j] = p.lse[r] * kLog2e;
+    }
+  }
+  pack_row<T>(static_cast<const T*>(p.x) + r * p.D, p.xc + j * p.Dp, p.pad * p.Dp, p.D, p.Dp, lane);
+}
+// Rows of a piece of W.
+template <typename T>
+__global__ void __launch_bounds__(256) lce_pack_weight_kernel(const T* w, bf16* to, int rows, size_t pad, int D, int Dp) {
+  begin_dependent();
+  const int r = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (r < rows) pack_row<T>(w + (size_t)r * D, to + (size_t)r * Dp, pad * Dp, D, Dp, threadIdx.x & 31);
+}
+
+// ------------------------------------------------------------------ the products
+enum Mode { kStats, kGrad, kDx, kDw };
+// A stage of the ring: PARTS tiles of A, 128 rows a CTA, and of B, BN / 2 rows a CTA, 64 deep.
+template <int MODE, bool F32>
+struct Cfg {
+  static constexpr int BN = F32 ? 128 : 256, PARTS = F32 ? 3 : 1, COLS = BN / 2;  // COLS: of a thread of the epilogue
+  static constexpr int A = 128 * 128, B = BN / 2 * 128, STAGE = PARTS * (A + B);
+  static constexpr int STAGES = F32 ? (MODE == kGrad ? 2 : 3) : 6;
+  static constexpr int STAGING = MODE == kGrad ? 8 * 4096 : 0;  // a box of 32 rows x 64 columns a warp
+  static constexpr bool A_MN = MODE == kDw, B_MN = MODE == kDx || MODE == kDw;
+  static constexpr int SMEM = 1024 + STAGES * STAGE + STAGING + 256 + (MODE == kStats ? 128 + 4 * 128 * 8 : 0);
+};
+constexpr int kThreads = 320, kSegment = 32;  // blocks of 64 that a float32 accumulator takes before it is added up in registers
+struct GemmP {
+  const int32_t* live;
+  int32_t* status;
+  int M, N, K;            // the extent that counts tokens is *live
+  int b_row0;             // first row of B in its map (the vocabulary's piece)
+  int splits;             // of K
+  int group;              // tiles of M that are walked through together
+  int v0, V;              // first row of the vocabulary's piece, rows in all
+  size_t pad;             // rows of what is indexed by token
+  float2* part;           // kStats: [tiles of the vocabulary][pad] maximum and sum
+  float* hit;             //   logit of the target
+  const int32_t *tgt, *idx;
+  const float *a, *both, *lse2;
+  float* sums;            // kDx, kDw: float32 [splits][rows][D], null: straight to out
+  int adds;               //   to what is there
+  size_t sums_stride;
+  void* out;              // rows by idx (kDx) or from v0 (kDw)
+  int D, whole;           // whole: out's rows may be written in pieces of 16 bytes
+};
+struct Maps { CUtensorMap a, b, g; };
+
+// A wait that gives up: on its own limit, or when another role of the CTA has.
+struct Wait {
+  volatile int32_t* bad;
+  __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) const {
+    for (uint32_t i = 0; i < 1000000u; ++i) {
+      if (tc::mbar_try_wait(bar, parity)) return true;
+      if ((i & 63u) == 63u && *bad) return false;
+    }
+    *bad = 1;
+    return false;
+  }
+};
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A maximum (-infinity: nothing yet) and the sum of exponentials from it, and another such pair.
+__device__ __forceinline__ void add_sum(float2& a, float2 b) {
+  const float t = fmaxf(a.x, b.x);
+  a.y = (a.x == -INFINITY ? 0.f : a.y * ex2((a.x - t) * kLog2e)) + (b.x == -INFINITY ? 0.f : b.y * ex2((b.x - t) * kLog2e));
+  a.x = t;
+}
+
+// What all roles walk through: tiles of 256 x BN, group tiles of M at a time so that both operands' tiles stay in L2.
+struct Walk {
+  int m_tiles, n_tiles, kblocks, items;
+  __device__ __forceinline__ Walk(const GemmP& p, int mode, int BN) {
+    const int live = *p.live;
+    const int M = mode == kDw ? p.M : live, K = mode == kDw ? live : p.K;
+    m_tiles = (M + 255) / 256;
+    n_tiles = (p.N + BN - 1) / BN;
+    kblocks = (K + 63) / 64;
+    items = m_tiles * n_tiles * p.splits;
+  }
+  __device__ __forceinline__ void item(const GemmP& p, int i, int& m, int& n, int& split, int& k0, int& k1) const {
+    const int tiles = m_tiles * n_tiles;
+    split = i / tiles;
+    i -= split * tiles;
+    const int g = i / (p.group * n_tiles), rest = i - g * p.group * n_tiles, gm = min(p.group, m_tiles - g * p.group);
+    m = g * p.group + rest % gm;
+    n = rest / gm;
+    k0 = (int)((int64_t)kblocks * split / p.splits);
+    k1 = (int)((int64_t)kblocks * (split + 1) / p.splits);
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void store_row(T* to, int c, int D, bool whole, const float* v) {  // 8 columns from c
+  if (whole) {
+    if (c >= D) return;
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(to + c) = make_float4(v[0], v[1], v[2], v[3]);
+      *reinterpret_cast<float4*>(to + c + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      *reinterpret_cast<uint4*>(to + c) = tc::pack8(v);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (c + i < D) to[c + i] = from_f32<T>(v[i]);
+}
+
+template <int MODE, bool F32>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gemm_kernel(const GemmP p, const __grid_constant__ Maps maps) {
+  using C = Cfg<MODE, F32>;
+  begin_dependent();
+  extern __shared__ uint8_t raw[];
+  const uint32_t base = (tc::smem_u32(raw) + 1023u) & ~1023u;
+  uint8_t* sm = raw + (base - tc::smem_u32(raw));
+  uint8_t* staging = sm + C::STAGES * C::STAGE;
+  uint64_t* full = reinterpret_cast<uint64_t*>(staging + C::STAGING);
+  uint64_t *empty = full + C::STAGES, *acc_full = empty + C::STAGES, *acc_empty = acc_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  volatile int32_t* bad = reinterpret_cast<volatile int32_t*>(tmem_slot + 1);
+  // kStats: what the warps of a tile's second half found, for those of the first: a ring of four tiles, a barrier a slot and warp.
+  // (When a warp writes for tile t + 4, tile t + 3's accumulator has been filled, so tile t + 1's has been read by all warps, which
+  // are done with tile t.)
+  uint64_t* halves_full = reinterpret_cast<uint64_t*>(staging + C::STAGING + 256);  // [4][4]
+  float2* halves = reinterpret_cast<float2*>(halves_full + 16);                     // [4][128]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = tc::cluster_rank();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      tc::mbar_init(full + s, 1);
+      tc::mbar_init(empty + s, 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      tc::mbar_init(acc_full + s, 1);
+      tc::mbar_init(acc_empty + s, 16);
+    }
+    if (MODE == kStats)
+      for (int s = 0; s < 16; ++s) tc::mbar_init(halves_full + s, 1);
+    *bad = 0;
+    tc::mbar_fence_init();
+  }
+  if (warp == 9) {
+    tc::tmem_alloc_pair(tmem_slot, 512);
+    tc::tmem_relinquish_pair();
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::cluster_sync();
+  tc::fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  const Walk walk(p, MODE, C::BN);
+  const Wait wait{bad};
+  // blocks of K behind which an accumulator is handed over
+  constexpr int SEG = F32 ? kSegment : 1 << 30;
+
+  if (warp == 8) {
+    // ---- copies: each CTA its half of A and B, counted by the barrier of the CTA that issues the products
+    if (tc::elect_one()) {
+      int s = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int i = pair; ok && i < walk.items; i += pairs) {
+        int m, n, split, k0, k1;
+        walk.item(p, i, m, n, split, k0, k1);
+        for (int kb = k0; kb < k1; ++kb) {
+          if (!(ok = wait(empty + s, phase ^ 1u))) break;
+          if (rank == 0) tc::mbar_expect_tx(full + s, 2 * C::STAGE);
+          const uint32_t bar = tc::in_cta(tc::smem_u32(full + s), 0);
+          uint32_t to = base + s * C::STAGE;
+#pragma unroll
+          for (int part = 0; part < C::PARTS; ++part, to += C::A) {
+            const int m0 = m * 256 + (int)rank * 128;
+            if (C::A_MN) {
+              tc::tma_load_3d_pair(to, &maps.a, m0, kb * 64, part, bar);
+              tc::tma_load_3d_pair(to + 8192, &maps.a, m0 + 64, kb * 64, part, bar);
+            } else {
+              tc::tma_load_3d_pair(to, &maps.a, kb * 64, m0, part, bar);
+            }
+          }
+#pragma unroll
+          for (int part = 0; part < C::PARTS; ++part, to += C::B) {
+            const int n0 = n * C::BN + (int)rank * (C::BN / 2);
+            if (C::B_MN) {
+#pragma unroll
+              for (int x = 0; x < C::BN / 128; ++x) tc::tma_load_3d_pair(to + x * 8192, &maps.b, n0 + 64 * x, p.b_row0 + kb * 64, part, bar);
+            } else {
+              tc::tma_load_3d_pair(to, &maps.b, kb * 64, p.b_row0 + n0, part, bar);
+            }
+          }
+          if (++s == C::STAGES) { s = 0; phase ^= 1u; }
+        }
+      }
+    }
+  } else if (warp == 9) {
+    // ---- products, by one thread of the pair
+    if (rank == 0 && tc::elect_one()) {
+      constexpr uint32_t idesc = tc::make_idesc_bf16(256, C::BN, C::A_MN, C::B_MN);
+      constexpr uint32_t a_step = C::A_MN ? 2048 : 32, b_step = C::B_MN ? 2048 : 32;
+      int s = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int i = pair; ok && i < walk.items; i += pairs) {
+        int m, n, split, k0, k1;
+        walk.item(p, i, m, n, split, k0, k1);
+        for (int ks = k0; ok && ks < k1; ks += SEG) {
+          if (!(ok = wait(acc_empty + acc, acc_phase ^ 1u))) break;
+          tc::fence_after_sync();
+          const uint32_t d = tmem + acc * 256;
+          const int ke = min(ks + min(SEG, k1 - ks), k1);
+          for (int kb = ks; kb < ke; ++kb) {
+            if (!(ok = wait(full + s, phase))) break;
+            tc::fence_after_sync();
+            const uint32_t sa = base + s * C::STAGE, sb = sa + C::PARTS * C::A;
+            auto product = [&](int pa, int pb, uint32_t to, bool first) {
+              const uint64_t da = tc::make_smem_desc(sa + pa * C::A, C::A_MN ? 8192 : 16, 1024, tc::kSwizzle128);
+              const uint64_t db = tc::make_smem_desc(sb + pb * C::B, C::B_MN ? 8192 : 16, 1024, tc::kSwizzle128);
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                tc::mma_pair(to, da + (uint64_t)((k * a_step) >> 4), db + (uint64_t)((k * b_step) >> 4), idesc, !(first && k == 0));
+            };
+            product(0, 0, d, kb == ks);
+            if (F32) {
+              product(2, 0, d + 128, kb == ks);
+              product(0, 2, d + 128, false);
+              product(1, 1, d + 128, false);
+              product(1, 0, d + 128, false);
+              product(0, 1, d + 128, false);
+            }
+            tc::mma_commit_pair(empty + s);
+            if (++s == C::STAGES) { s = 0; phase ^= 1u; }
+          }
+          if (!ok) break;
+          tc::mma_commit_pair(acc_full + acc);
+          if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+        }
+      }
+    }
+  } else {
+    // ---- epilogue: a thread has a row of the CTA's 128 and half of the tile's columns
+    const int half = warp >> 2, quarter = warp & 3, mine = quarter * 32 + lane;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const int live = *p.live;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    for (int i = pair; ok && i < walk.items; i += pairs) {
+      int m, n, split, k0, k1;
+      walk.item(p, i, m, n, split, k0, k1);
+      float v[C::COLS];
+      if (k0 == k1 || F32)
+#pragma unroll
+        for (int c = 0; c < C::COLS; ++c) v[c] = 0.f;
+      for (int ks = k0; ks < k1; ks += min(SEG, k1 - ks)) {
+        if (!(ok = wait(acc_full + acc, acc_phase))) break;
+        __syncwarp();
+        tc::fence_after_sync();
+        const uint32_t d = tmem + lanes + acc * 256 + half * C::COLS;
+        if constexpr (!F32) {
+#pragma unroll
+          for (int c = 0; c < C::COLS; c += 32) {
+            uint32_t(&r)[32] = reinterpret_cast<uint32_t(&)[32]>(v[c]);
+            tc::tmem_ld_32x32b_x32(d + c, r);
+          }
+          tc::tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int c = 0; c < C::COLS; c += 32) {
+            uint32_t big[32], small[32];
+            tc::tmem_ld_32x32b_x32(d + c, big);
+            tc::tmem_ld_32x32b_x32(d + 128 + c, small);
+            tc::tmem_ld_wait();
+#pragma unroll
+            for (int x = 0; x < 32; ++x) v[c + x] += __uint_as_float(big[x]) + __uint_as_float(small[x]);
+          }
+        }
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive_cluster(tc::in_cta(tc::smem_u32(acc_empty + acc), 0));
+        if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+      }
+      if (!ok) break;
+      const int row = m * 256 + (int)rank * 128 + mine, c0 = n * C::BN + half * C::COLS;
+      if constexpr (MODE == kStats || MODE == kGrad) {
+        const int here = p.V - p.v0 - c0;  // columns from c0 that are in the vocabulary
+        const int at = p.tgt[row] - p.v0 - c0;
+        const bool hit = at >= 0 && at < C::COLS;
+        if constexpr (MODE == kStats) {
+          if (here < C::COLS)
+#pragma unroll
+            for (int c = 0; c < C::COLS; ++c) v[c] = c < here ? v[c] : -INFINITY;
+          float top = v[0];
+#pragma unroll
+          for (int c = 1; c < C::COLS; ++c) top = fmaxf(top, v[c]);
+          // (an infinite maximum would make NaNs of the infinities: the exponentials are then 0 or infinite)
+          const float back = fabsf(top) == INFINITY ? 0.f : -top * kLog2e, shift = top == INFINITY ? 0.f : top;
+          float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+          for (int c = 0; c < C::COLS; c += 2) {
+            s0 += ex2(fmaf(v[c], kLog2e, back));
+            s1 += ex2(fmaf(v[c + 1], kLog2e, back));
+          }
+          float sum = s0 + s1;
+          if (__any_sync(0xffffffffu, hit)) {
+            float z = 0.f;
+#pragma unroll
+            for (int c = 0; c < C::COLS; ++c) z = c == at ? v[c] : z;
+            if (hit && row < live) p.hit[row] = z;
+          }
+          const int turn = i / pairs, slot = turn & 3;
+          float2* buf = halves + slot * 128;
+          uint64_t* there = halves_full + slot * 4 + quarter;
+          if (half == 1) {
+            buf[mine] = make_float2(shift, sum);
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(there);
+          } else {
+            if (!(ok = wait(there, (uint32_t)(turn >> 2) & 1u))) break;
+            const float2 o = buf[mine];
+            if (row < live) {
+              float2 both{shift, sum};
+              add_sum(both, o);
+              p.part[((size_t)(p.v0 / C::BN) + n) * p.pad + row] = both;
+            }
+          }
+        } else {
+          const float both = p.both[row], back = -p.lse2[row];
+#pragma unroll
+          for (int c = 0; c < C::COLS; ++c) v[c] = both * ex2(fmaf(v[c], kLog2e, back));
+          if (row >= live || here < C::COLS)
+#pragma unroll
+            for (int c = 0; c < C::COLS; ++c) v[c] = row < live && c < here ? v[c] : 0.f;
+          if (__any_sync(0xffffffffu, hit)) {
+            const float a = hit ? p.a[row] : 0.f;
+#pragma unroll
+            for (int c = 0; c < C::COLS; ++c) v[c] = c == at ? v[c] - a : v[c];
+          }
+          // to the workspace in boxes of 32 rows x 64 columns, by this warp's part of shared memory (128-byte swizzle)
+          uint8_t* box = staging + warp * 4096;
+          const int r0 = m * 256 + (int)rank * 128 + quarter * 32;
+#pragma unroll
+          for (int x = 0; x < C::COLS / 64; ++x)
+#pragma unroll
+            for (int part = 0; part < C::PARTS; ++part) {
+              if (lane == 0) tc::bulk_wait_read<0>();
+              __syncwarp();
+#pragma unroll
+              for (int u = 0; u < 8; ++u) {
+                float* e = v + x * 64 + u * 8;
+                const uint4 w = tc::pack8(e);
+                *reinterpret_cast<uint4*>(box + lane * 128 + ((u ^ (lane & 7)) << 4)) = w;
+                if (part + 1 < C::PARTS) {
+                  float lo[8];
+                  tc::unpack8(w, lo);
+#pragma unroll
+                  for (int y = 0; y < 8; ++y) e[y] -= lo[y];
+                }
+              }
+              tc::fence_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                tc::tma_store_3d(&maps.g, tc::smem_u32(box), c0 + x * 64, r0, part);
+                tc::bulk_commit();
+              }
+            }
+        }
+      } else {
+        const bool in = row < (MODE == kDx ? live : p.M);
+        if (in) {
+          if (p.sums) {
+            float* to = p.sums + split * p.sums_stride + (size_t)row * p.D;
+            const bool four = p.D % 4 == 0;
+#pragma unroll
+            for (int c = 0; c < C::COLS; c += 4) {
+              const int col = c0 + c;
+              if (four) {
+                if (col < p.D) {
+                  float4 o = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+                  if (p.adds) {
+                    const float4 old = *reinterpret_cast<const float4*>(to + col);
+                    o.x += old.x; o.y += old.y; o.z += old.z; o.w += old.w;
+                  }
+                  *reinterpret_cast<float4*>(to + col) = o;
+                }
+              } else {
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                  if (col + x < p.D) to[col + x] = p.adds ? to[col + x] + v[c + x] : v[c + x];
+              }
+            }
+          } else {
+            using T = std::conditional_t<F32, float, bf16>;
+            T* to = static_cast<T*>(p.out) + (MODE == kDx ? (size_t)p.idx[row] : (size_t)p.v0 + row) * p.D;
+#pragma unroll
+            for (int c = 0; c < C::COLS; c += 8) store_row<T>(to, c0 + c, p.D, p.whole, v + c);
+          }
+        }
+      }
+    }
+    if (MODE == kGrad && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+  __syncwarp();
+  __syncthreads();
+  if (threadIdx.x == 0 && *bad) atomicExch(p.status, 11);
+  __syncwarp();
+  tc::fence_before_sync();
+  tc::cluster_sync();  // (neither CTA leaves while the other's products read its shared memory or arrive at its barriers)
+  tc::fence_after_sync();
+  if (warp == 9) tc::tmem_dealloc_pair(tmem, 512);
+}
+
+// lse and loss of each row from its tiles' maxima and sums: eight warps take every eighth tile, then warp 0 theirs in order.
+struct JoinP {
+  const float2* part;
+  const float* hit;
+  const int32_t *live, *idx;
+  float *loss, *lse;
+  size_t pad;
+  int tiles;
+};
+__global__ void __launch_bounds__(256) lce_join_kernel(JoinP p) {
+  begin_dependent();
+  __shared__ float2 red[8][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row = blockIdx.x * 32 + lane;
+  const bool in = row < *p.live;
+  float2 all{-INFINITY, 0.f};
+  if (in)
+    for (int t = warp; t < p.tiles; t += 8) add_sum(all, p.part[(size_t)t * p.pad + row]);
+  red[warp][lane] = all;
+  __syncthreads();
+  if (warp != 0 || !in) return;
+  for (int w = 1; w < 8; ++w) add_sum(all, red[w][lane]);
+  const float lse = all.x + logf(all.y);
+  const int to = p.idx[row];
+  p.lse[to] = lse;
+  p.loss[to] = lse - p.hit[row];
+}
+// Rows of float32 sums over the splits, in order, to their places in the tensor's type.
+struct FinishP {
+  const float* sums;
+  const int32_t *live, *idx;  // idx null: rows from row0, all of them
+  void* out;
+  size_t stride, row0;
+  int rows, D, splits;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) lce_finish_kernel(FinishP p) {
+  begin_dependent();
+  const int rows = p.idx ? *p.live : p.rows;
+  for (int r = blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.x * 8) {
+    T* to = static_cast<T*>(p.out) + (p.idx ? (size_t)p.idx[r] : p.row0 + r) * p.D;
+    const float* from = p.sums + (size_t)r * p.D;
+    for (int c = threadIdx.x & 31; c < p.D; c += 32) {
+      float s = from[c];
+      for (int k = 1; k < p.splits; ++k) s += from[k * p.stride + c];
+      to[c] = from_f32<T>(s);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ host
+static bool make_map(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows, uint64_t parts, uint64_t pitch, uint64_t part_pitch,
+                     uint32_t box_rows) {
+  typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                             const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static const Encode encode = []() -> Encode {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess)
+      return nullptr;
+    return reinterpret_cast<Encode>(f);
+  }();
+  const cuuint64_t dims[3] = {cols, rows, parts}, strides[2] = {pitch * 2, part_pitch * 2};
+  const cuuint32_t box[3] = {64, box_rows, 1}, step[3] = {1, 1, 1};
+  return encode && encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+constexpr int kPairs = 74;
+// Bytes of g that are kept at a time.
+constexpr size_t kGradBytes = (size_t)512 << 20;
+constexpr size_t kPackBytes = (size_t)256 << 20;
+
+struct Plan {
+  bool f32, pack_w;
+  int parts, Dp, piece, pieces, BN;
+  size_t N, pad;
+  int dx_splits, dw_splits;
+  bool dx_sums;
+  // workspace
+  int32_t *status, *live, *counts, *idx, *tgt;
+  float *a, *both, *lse2, *hit, *dx_part, *dw_part;
+  float2* part;
+  bf16 *xc, *wc, *g;
+  size_t bytes;
+};
+static int splits_of(int64_t tiles, int64_t kblocks) {
+  return (int)std::max<int64_t>(1, std::min<int64_t>(kPairs / std::max<int64_t>(tiles, 1), kblocks / 8));
+}
+// bwd: the backward pass.  weight only says whether it can be read as it is.
+static Plan plan(const mxb_linear_ce_desc* d, const void* weight, bool bwd, void* base) {
+  Plan q{};
+  q.f32 = d->io_dtype == MXB_F32;
+  q.parts = q.f32 ? 3 : 1;
+  q.BN = q.f32 ? 128 : 256;
+  q.Dp = (d->D + 7) / 8 * 8;
+  q.N = d->rows;
+  q.pad = std::max<size_t>((q.N + 255) / 256 * 256, 256);
+  // (a base off 16 bytes: as many bytes of workspace are asked for whatever the pointer, so that the query needs none)
+  q.pack_w = q.f32 || d->D % 8 != 0 || (reinterpret_cast<uintptr_t>(weight) & 15) != 0;
+  const int64_t all = ((int64_t)d->V + 255) / 256 * 256;
+  int64_t most = bwd ? (int64_t)(kGradBytes / (q.pad * q.parts * 2)) : all;
+  most = std::min<int64_t>(most, (int64_t)(kPackBytes / ((size_t)q.Dp * q.parts * 2)));
+  q.piece = (int)std::min<int64_t>(all, std::max<int64_t>(256, most / 256 * 256));
+  if (!bwd && !q.pack_w) q.piece = (int)all;
+  q.pieces = (int)((d->V + (int64_t)q.piece - 1) / q.piece);
+  const int64_t m_tiles = q.pad / 256, d_tiles = (d->D + q.BN - 1) / q.BN;
+  q.dx_splits = splits_of(m_tiles * d_tiles, q.piece / 64);
+  q.dx_sums = q.pieces > 1 || q.dx_splits > 1;
+  q.dw_splits = splits_of(q.piece / 256 * d_tiles, (int64_t)((q.N + 63) / 64));
+  Carver c(base);
+  q.status = c.take<int32_t>(64);  // (the device's error word leads the workspace)
+  q.live = c.take<int32_t>(1);
+  q.counts = c.take<int32_t>(q.N / kCountRows + 1);
+  q.idx = c.take<int32_t>(q.pad);
+  q.tgt = c.take<int32_t>(q.pad);
+  q.xc = c.take<bf16>((size_t)q.parts * q.pad * q.Dp);
+  // the packed piece of W: asked for where D alone says so; a base off 16 bytes is refused instead
+  if (q.f32 || d->D % 8 != 0) q.wc = c.take<bf16>((size_t)q.parts * q.piece * q.Dp);
+  if (!bwd) {
+    q.hit = c.take<float>(q.pad);
+    q.part = c.take<float2>(((size_t)d->V + q.BN - 1) / q.BN * q.pad);
+  } else {
+    q.a = c.take<float>(q.pad);
+    q.both = c.take<float>(q.pad);
+    q.lse2 = c.take<float>(q.pad);
+    q.g = c.take<bf16>((size_t)q.parts * q.pad * q.piece);
+    if (q.dx_sums) q.dx_part = c.take<float>((size_t)q.dx_splits * q.pad * d->D);
+    if (q.dw_splits > 1) q.dw_part = c.take<float>((size_t)q.dw_splits * q.piece * d->D);
+  }
+  q.bytes = c.bytes();
+  return q;
+}
+
+template <int MODE, bool F32>
+static mxb_status launch_gemm(const GemmP& p, const Maps& maps, int64_t items, cudaStream_t st) {
+  using C = Cfg<MODE, F32>;
+  if (MXB_ALLOW_SMEM(C::SMEM, lce_gemm_kernel<MODE, F32>) != MXB_OK) return MXB_ERR_CUDA;
+  static const char* const names[] = {"lce_stats_kernel", "lce_grad_kernel", "lce_dx_kernel", "lce_dw_kernel"};
+  const unsigned ctas = 2 * (unsigned)std::min<int64_t>(items, kPairs);
+  MXB_LAUNCH(names[MODE], st, (launch_kernel(lce_gemm_kernel<MODE, F32>, ctas, kThreads, C::SMEM, st, p, maps)));
+  return check_launch(names[MODE]);
+}
+template <typename T>
+static mxb_status pack(const mxb_linear_ce_desc* d, PackP& p, cudaStream_t st) {
+  if (p.N >= kCountRows)
+    MXB_LAUNCH("lce_count_kernel", st, (launch_kernel(lce_count_kernel, (unsigned)(p.N / kCountRows), 256, 0, st, p, const_cast<int32_t*>(p.counts))));
+  const int blocks = (int)((p.N + 7) / 8);
+  MXB_LAUNCH("lce_pack_kernel", st, (launch_kernel(lce_pack_kernel<T>, blocks + 32, 256, 0, st, p, blocks)));
+  return check_launch("lce_pack_kernel");
+}
+
+template <bool F32>
+static mxb_status run(const mxb_linear_ce_desc* d, const Plan& q, PackP& pk, const void* weight, void* dweight, cudaStream_t st) {
+  using T = std::conditional_t<F32, float, bf16>;
+  const bool bwd = pk.d_loss != nullptr;
+  mxb_status s = pack<T>(d, pk, st);
+  if (s != MXB_OK) return s;
+  const size_t pad = q.pad;
+  const int D = d->D, BN = q.BN;
+  const int64_t m_tiles = pad / 256, d_tiles = (D + BN - 1) / BN;
+  for (int piece = 0; piece < q.pieces; ++piece) {
+    const int v0 = piece * q.piece, rows = (int)std::min<int64_t>(q.piece, (int64_t)d->V - v0);
+    const void* w = weight;
+    uint64_t w_rows = d->V, w_part = (uint64_t)d->V * D;
+    int w_row0 = v0;
+    if (q.pack_w) {
+      MXB_LAUNCH("lce_pack_weight_kernel", st,
+                 (launch_kernel(lce_pack_weight_kernel<T>, (unsigned)((rows + 7) / 8), 256, 0, st, static_cast<const T*>(weight) + (size_t)v0 * D, q.wc,
+                                rows, (size_t)q.piece, D, q.Dp)));
+      w = q.wc;
+      w_rows = rows;
+      w_part = (uint64_t)q.piece * q.Dp;
+      w_row0 = 0;
+    }
+    GemmP p{};
+    p.live = q.live;
+    p.status = q.status;
+    p.tgt = q.tgt;
+    p.idx = q.idx;
+    p.v0 = v0;
+    p.V = d->V;
+    p.pad = pad;
+    p.D = D;
+    p.splits = 1;
+    p.group = 8;
+    Maps maps;
+    std::memset(&maps, 0, sizeof maps);
+    bool ok = make_map(&maps.a, q.xc, q.Dp, pad, q.parts, q.Dp, pad * q.Dp, 128) && make_map(&maps.b, w, q.Dp, w_rows, q.parts, q.Dp, w_part, BN / 2);
+    if (bwd) ok = ok && make_map(&maps.g, q.g, q.piece, pad, q.parts, q.piece, pad * q.piece, 32);
+    if (!ok) return MXB_ERR_UNSUPPORTED;
+    p.N = rows;
+    p.K = D;
+    p.b_row0 = w_row0;
+    p.part = q.part;
+    p.hit = q.hit;
+    p.a = q.a;
+    p.both = q.both;
+    p.lse2 = q.lse2;
+    const int64_t tiles = m_tiles * ((rows + BN - 1) / BN);
+    s = bwd ? launch_gemm<kGrad, F32>(p, maps, tiles, st) : launch_gemm<kStats, F32>(p, maps, tiles, st);
+    if (s != MXB_OK) return s;
+    if (bwd) {
+      // dx: sums over the piece, in the order of the pieces
+      GemmP x = p;
+      x.N = D;
+      x.K = rows;
+      x.b_row0 = w_row0;
+      x.splits = q.dx_splits;
+      x.sums = q.dx_part;
+      x.sums_stride = pad * D;
+      x.adds = piece > 0;
+      x.out = pk.dx;
+      x.whole = D % 8 == 0 && (reinterpret_cast<uintptr_t>(pk.dx) & 15) == 0;
+      if (!make_map(&maps.a, q.g, q.piece, pad, q.parts, q.piece, pad * q.piece, 128) || !make_map(&maps.b, w, q.Dp, w_rows, q.parts, q.Dp, w_part, 64))
+        return MXB_ERR_UNSUPPORTED;
+      s = launch_gemm<kDx, F32>(x, maps, m_tiles * d_tiles * q.dx_splits, st);
+      if (s != MXB_OK) return s;
+      // dW: sums over the tokens
+      GemmP y = p;
+      y.M = rows;
+      y.N = D;
+      y.b_row0 = 0;
+      y.splits = q.dw_splits;
+      y.sums = q.dw_part;
+      y.sums_stride = (size_t)q.piece * D;
+      y.out = dweight;
+      y.whole = D % 8 == 0 && (reinterpret_cast<uintptr_t>(dweight) & 15) == 0;
+      if (!make_map(&maps.a, q.g, q.piece, pad, q.parts, q.piece, pad * q.piece, 64) || !make_map(&maps.b, q.xc, q.Dp, pad, q.parts, q.Dp, pad * q.Dp, 64))
+        return MXB_ERR_UNSUPPORTED;
+      s = launch_gemm<kDw, F32>(y, maps, (int64_t)((rows + 255) / 256) * d_tiles * q.dw_splits, st);
+      if (s != MXB_OK) return s;
+      if (q.dw_part) {
+        const FinishP f{q.dw_part, q.live, nullptr, dweight, y.sums_stride, (size_t)v0, rows, D, q.dw_splits};
+        MXB_LAUNCH("lce_finish_kernel", st, (launch_kernel(lce_finish_kernel<T>, (unsigned)std::min<int64_t>((rows + 7) / 8, 148 * 8), 256, 0, st, f)));
+      }
+    }
+  }
+  if (bwd) {
+    if (q.dx_part) {
+      const FinishP f{q.dx_part, q.live, q.idx, pk.dx, pad * D, 0, 0, D, q.dx_splits};
+      MXB_LAUNCH("lce_finish_kernel", st, (launch_kernel(lce_finish_kernel<T>, (unsigned)std::min<int64_t>((pad + 7) / 8, 148 * 8), 256, 0, st, f)));
+    }
+    return check_launch("linear_ce_bwd");
+  }
+  const JoinP j{q.part, q.hit, q.live, q.idx, pk.loss, pk.lse_out, pad, (d->V + BN - 1) / BN};
+  MXB_LAUNCH("lce_join_kernel", st, (launch_kernel(lce_join_kernel, (unsigned)(pad / 32), 256, 0, st, j)));
+  return check_launch("linear_ce_fwd");
+}
+static PackP pack_args(const mxb_linear_ce_desc* d, const Plan& q, const void* x, const void* targets) {
+  PackP p{};
+  p.targets = targets;
+  p.x = x;
+  p.counts = q.counts;
+  p.live = q.live;
+  p.idx = q.idx;
+  p.tgt = q.tgt;
+  p.a = q.a;
+  p.both = q.both;
+  p.lse2 = q.lse2;
+  p.xc = q.xc;
+  p.status = q.status;
+  p.N = q.N;
+  p.pad = q.pad;
+  p.V = d->V;
+  p.D = d->D;
+  p.Dp = q.Dp;
+  p.wide = d->target_bytes == 8;
+  p.f32 = q.f32;
+  return p;
+}
+
+}  // namespace lce
+
+size_t linear_ce_scratch(const mxb_linear_ce_desc* d, bool bwd) { return lce::plan(d, nullptr, bwd, nullptr).bytes; }
+
+mxb_status linear_ce_fwd(const mxb_linear_ce_desc* d, const void* x, const void* weight, const void* targets, float* loss, float* lse,
+                         void* workspace, cudaStream_t st) {
+  const lce::Plan q = lce::plan(d, weight, false, workspace);
+  lce::PackP p = lce::pack_args(d, q, x, targets);
+  p.loss = loss;
+  p.lse_out = lse;
+  return q.f32 ? lce::run<true>(d, q, p, weight, nullptr, st) : lce::run<false>(d, q, p, weight, nullptr, st);
+}
+mxb_status linear_ce_bwd(const mxb_linear_ce_desc* d, const void* x, const void* weight, const void* targets, const float* lse, const float* d_loss,
+                         const float* d_lse, void* dx, void* dweight, void* workspace, cudaStream_t st) {
+  const lce::Plan q = lce::plan(d, weight, true, workspace);
+  lce::PackP p = lce::pack_args(d, q, x, targets);
+  p.lse = lse;
+  p.d_loss = d_loss;
+  p.d_lse = d_lse;
+  p.dx = dx;
+  return q.f32 ? lce::run<true>(d, q, p, weight, dweight, st) : lce::run<false>(d, q, p, weight, dweight, st);
+}
+
+}  // namespace mxb

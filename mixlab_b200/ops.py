@@ -261,3 +261,17 @@ def layer_norm_backward(x, weight, dn, *, d_resid=None, eps=1e-5):
     (x's type, or bfloat16 beside a float32 x), d_resid (x's type; None: zero) the gradient that reaches x from its other readers.
     dict(dx, dweight, dbias), dx in x's type, the others float32."""
     return (_front or _native()).layer_norm_backward(x, weight, dn, d_resid, eps)
+
+
+def linear_cross_entropy(x, weight, targets):
+    """The output head and its loss without the logits in memory: with z = x weight^T, returns loss = lse - z[target] and
+    lse = log sum exp z, float32 [...].  x [...,D], weight [V,D] (float32 or bfloat16), targets [...] (int32 or int64).  A token whose
+    target is outside 0 .. V-1 has no part: its loss and lse are zero, its x may hold anything."""
+    return (_front or _native()).linear_ce(x, weight, targets)
+
+
+def linear_cross_entropy_backward(x, weight, targets, lse, d_loss, *, d_lse=None):
+    """Gradients of ``linear_cross_entropy`` by x and weight, in their types: lse is what it returned, d_loss and d_lse (None: zero)
+    float32 [...] the gradients of its two results - 1 / tokens, or 1 where the gradients are numerators that the gradient exchange
+    divides.  Tokens without a target, or whose gradients are zero, have no part.  dict(dx, dweight)."""
+    return (_front or _native()).linear_ce_backward(x, weight, targets, lse, d_loss, d_lse)

@@ -37,10 +37,37 @@ def test_layer_norm_refusals():
     assert n > 0 and bwd(desc(), None, 0) == -3 and bwd(desc(), FAKE, n - 1) == -3 and bwd(desc(), ODD, n) == -5 and bwd(desc(), FAKE, n, None) == -1
 
 
+def test_linear_cross_entropy_refusals():
+    lib = mixlab_b200.lib()
+    desc = lambda **kw: _lib.LinearCeDesc(*dict(dict(rows=8, V=16, D=8, target_bytes=4, io=2), **kw).values())  # noqa: E731
+    fwd = lambda d, ws, n, w=FAKE, x=FAKE: lib.mxb_linear_ce_fwd(C.byref(d), x, w, FAKE, FAKE, FAKE, ws, n, None)  # noqa: E731
+    bwd = lambda d, ws, n, w=FAKE, dw=FAKE: lib.mxb_linear_ce_bwd(C.byref(d), FAKE, w, FAKE, FAKE, FAKE, None, FAKE, dw, ws, n, None)  # noqa: E731
+    for kw, want in [(dict(rows=-1), -1), (dict(V=0), -1), (dict(D=0), -1), (dict(target_bytes=1), -1), (dict(io=3), -1), (dict(rows=1 << 40), -2),
+                     (dict(rows=1 << 29, V=1 << 30), -2), (dict(D=1 << 30), -2)]:
+        assert fwd(desc(**kw), FAKE, 1 << 60) == want and bwd(desc(**kw), FAKE, 1 << 60) == want, kw
+        assert lib.mxb_linear_ce_fwd_workspace_bytes(C.byref(desc(**kw))) == 0 == lib.mxb_linear_ce_bwd_workspace_bytes(C.byref(desc(**kw)))
+    for call, n in ((fwd, lib.mxb_linear_ce_fwd_workspace_bytes(C.byref(desc()))), (bwd, lib.mxb_linear_ce_bwd_workspace_bytes(C.byref(desc())))):
+        assert n > 0 and call(desc(), None, 0) == -3 and call(desc(), FAKE, n - 1) == -3 and call(desc(), ODD, n) == -5
+        assert call(desc(), FAKE, n, w=C.c_void_p(4098)) == -5 and call(desc(), FAKE, n, w=None) == -1
+    assert lib.mxb_linear_ce_bwd_workspace_bytes(C.byref(desc(rows=0))) > 0  # (nothing is divided by the rows)
+    assert fwd(desc(rows=0), None, 0, x=None) == 0 and bwd(desc(), FAKE, 1 << 40, dw=None) == -1
+
+
+def test_the_backward_keeps_a_piece_of_the_vocabulary():
+    """Its workspace is far below the logits' size, whatever the vocabulary."""
+    lib = mixlab_b200.lib()
+    for V in (50001, 400001):
+        d = _lib.LinearCeDesc(32768, V, 1024, 8, _lib.MXB_BF16)
+        assert lib.mxb_linear_ce_bwd_workspace_bytes(C.byref(d)) < (800 << 20)
+    d = _lib.LinearCeDesc(1 << 21, 50001, 64, 8, _lib.MXB_BF16)  # (so many tokens that a piece is one tile)
+    assert lib.mxb_linear_ce_bwd_workspace_bytes(C.byref(d)) < (3 << 30)
+
+
 def test_cpu_tensors_are_refused():
     t, tok = torch.zeros(4, 64), torch.zeros(4).long()
     for call in (lambda: ops.embedding(tok, t), lambda: ops.embedding_backward(tok, t, 9), lambda: ops.layer_norm(t, torch.ones(64)),
-                 lambda: ops.layer_norm_backward(t, torch.ones(64), t)):
+                 lambda: ops.layer_norm_backward(t, torch.ones(64), t), lambda: ops.linear_cross_entropy(t, torch.zeros(9, 64), tok),
+                 lambda: ops.linear_cross_entropy_backward(t, torch.zeros(9, 64), tok, torch.zeros(4), torch.zeros(4))):
         with pytest.raises(ValueError, match="CUDA tensors only"):
             call()
 
@@ -51,6 +78,9 @@ _OPERANDS = {  # operator: its tensor operands (shape, dtype), the other argumen
     "embedding_backward": (dict(d_out=((2, 6, 24), BF16), tokens=((2, 6), "int32"), dweight=((11, 24), F32)), dict(V=11)),
     "layer_norm": (dict(x=((2, 6, 24), BF16), weight=((24,), F32), bias=((24,), F32), resid=((2, 6, 24), F32)), {}),
     "layer_norm_backward": (dict(x=((2, 6, 24), F32), weight=((24,), F32), dn=((2, 6, 24), BF16), d_resid=((2, 6, 24), F32)), {}),
+    "linear_cross_entropy": (dict(x=((2, 6, 24), BF16), weight=((11, 24), BF16), targets=((2, 6), "int64")), {}),
+    "linear_cross_entropy_backward": (dict(x=((2, 6, 24), BF16), weight=((11, 24), BF16), targets=((2, 6), "int32"), lse=((2, 6), F32),
+                                           d_loss=((2, 6), F32), d_lse=((2, 6), F32)), {}),
 }
 
 
@@ -74,7 +104,7 @@ def test_every_operand_is_checked(op):
             refused(name, TypeError, lambda s, _: torch.empty(s, dtype=torch.float16, device="cuda:0"))
             msg = refused(name, ValueError, lambda s, _: torch.empty(*s[:-1], 2 * s[-1], dtype=own, device="cuda:0")[..., ::2])
             assert "contiguous" in msg, (name, msg)
-            if name != first and (op, name) != ("embedding", "tokens"):
+            if name != first and (op, name) != ("embedding", "tokens") and (op[:6], name) != ("linear", "weight"):
                 refused(name, ValueError, lambda s, _: torch.empty(s[0] + 1, *s[1:], dtype=own, device="cuda:0"))
             if name != first:
                 assert "cuda:1" in refused(name, ValueError, lambda s, _: torch.empty(s, dtype=own, device="cuda:1"))
