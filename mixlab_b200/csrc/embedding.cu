@@ -11,6 +11,7 @@
 
 #include "common.cuh"
 #include "row_pieces.cuh"
+#include "tcgen05.cuh"
 
 namespace mxb {
 namespace embed {
@@ -48,12 +49,12 @@ __global__ void __launch_bounds__(256) embedding_fwd_kernel(FwdP p, int tpr) {
     int tok[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) tok[r] = t0 + r < p.N ? token_of(static_cast<const TOK*>(p.tokens), t0 + r, p.V) : p.V;
-    for (int c = lane * 8; c < p.D; c += tpr * 8) {
+    for (int c = 0; c < p.D; c += tpr * 8) {
       f2 e[R][4];
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         if (tok[r] < p.V) {
-          load8<IN, V>(static_cast<const IN*>(p.weight) + (size_t)tok[r] * p.D, c, p.D, e[r]);
+          load_cols<IN, V>(static_cast<const IN*>(p.weight) + (size_t)tok[r] * p.D, c, lane, tpr, p.D, e[r]);
         } else {
 #pragma unroll
           for (int i = 0; i < 4; ++i) e[r][i] = 0;
@@ -65,7 +66,7 @@ __global__ void __launch_bounds__(256) embedding_fwd_kernel(FwdP p, int tpr) {
         if (tok[r] < p.V)
 #pragma unroll
           for (int i = 0; i < 4; ++i) e[r][i] = mul2(e[r][i], s);
-        store8<OUT, V>(static_cast<OUT*>(p.out) + (t0 + r) * p.D, c, p.D, e[r]);
+        store_cols<OUT, V>(static_cast<OUT*>(p.out) + (t0 + r) * p.D, c, lane, tpr, p.D, e[r]);
       }
     }
   }
@@ -79,6 +80,7 @@ struct SortP {
   const int32_t *key_in, *pos_in;  // null in the first pass
   int32_t *key_out, *pos_out;
   int32_t* hist;                   // [digits][tiles]
+  uint32_t* rows;                  // the first pass: a bit for each token that occurs
   int N, V, shift, digits, tiles;
 };
 template <typename TOK>
@@ -90,6 +92,8 @@ __global__ void __launch_bounds__(kSortThreads) embedding_count_kernel(SortP p) 
   begin_dependent();
   __shared__ int32_t count[kMaxDigits];
   for (int d = threadIdx.x; d < p.digits; d += kSortThreads) count[d] = 0;
+  if (!p.key_in)
+    for (int64_t w = (int64_t)blockIdx.x * kSortThreads + threadIdx.x; w <= p.V / 32; w += (int64_t)gridDim.x * kSortThreads) p.rows[w] = 0;
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < kEach; ++k) {
@@ -197,12 +201,121 @@ __global__ void __launch_bounds__(kSortThreads) embedding_place_kernel(SortP p, 
     const int d = (key[k] >> p.shift) & (p.digits - 1), to = place[d] + mine[warp][d] + rank[k];
     p.key_out[to] = key[k];
     p.pos_out[to] = p.pos_in ? p.pos_in[i] : (int)i;
+    if (!p.key_in) atomicOr(p.rows + key[k] / 32, 1u << (key[k] & 31));
+  }
+}
+
+// The whole sort in one launch for up to kClusterEntries entries: a cluster of CTAs, each with an equal share of the entries, that read
+// each other's digit counts through distributed shared memory.  (2047 entries, five launches: 19.8 us for the gradient, of which
+// 15 are the sort's three.)
+constexpr int kClusterThreads = 1024, kClusterEach = 8, kClusterMost = 8, kClusterEntries = kClusterThreads * kClusterEach * kClusterMost;
+__device__ __forceinline__ int32_t of_cta(const int32_t* p, uint32_t rank) {
+  int32_t v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(tc::in_cta(tc::smem_u32(p), rank)) : "memory");
+  return v;
+}
+struct ClusterP {
+  const void* tokens;
+  int32_t *key[2], *pos[2];
+  uint32_t* rows;
+  int N, V, bits, passes, share;  // share: entries of a CTA
+};
+template <typename TOK>
+__global__ void __launch_bounds__(kClusterThreads) embedding_sort_kernel(ClusterP p) {
+  begin_dependent();
+  extern __shared__ uint16_t mine[];  // [32 warps][digits]
+  __shared__ int32_t hist[kMaxDigits], place[kMaxDigits], sums[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, digits = 1 << p.bits, ctas = gridDim.x, rank = tc::cluster_rank();
+  const int each = (p.share + kClusterThreads - 1) / kClusterThreads;  // rounds of 32 consecutive entries a warp
+  const int begin = rank * p.share, end = min(begin + p.share, p.N), first = begin + warp * 32 * each + lane;
+  for (int64_t w = (int64_t)rank * kClusterThreads + threadIdx.x; w <= p.V / 32; w += (int64_t)ctas * kClusterThreads) p.rows[w] = 0;
+  for (int pass = 0; pass < p.passes; ++pass) {
+    const int shift = pass * p.bits;
+    const bool odd = pass & 1;
+    const int32_t *key_in = odd ? p.key[0] : p.key[1], *pos_in = odd ? p.pos[0] : p.pos[1];
+    int32_t *key_out = odd ? p.key[1] : p.key[0], *pos_out = odd ? p.pos[1] : p.pos[0];
+    for (int d = threadIdx.x; d < 16 * digits; d += kClusterThreads) reinterpret_cast<uint32_t*>(mine)[d] = 0;
+    int key[kClusterEach], pos[kClusterEach], at[kClusterEach];
+#pragma unroll
+    for (int k = 0; k < kClusterEach; ++k) {
+      const int i = first + 32 * k;
+      key[k] = -1;
+      if (k < each && i < end) {
+        key[k] = pass ? key_in[i] : token_of(static_cast<const TOK*>(p.tokens), i, p.V);
+        pos[k] = pass ? pos_in[i] : i;
+      }
+    }
+    __syncthreads();
+    uint16_t* own = mine + warp * digits;
+#pragma unroll
+    for (int k = 0; k < kClusterEach; ++k) {
+      if (k >= each) break;
+      const bool in = key[k] >= 0;
+      const int d = in ? key[k] >> shift & digits - 1 : kMaxDigits;
+      const uint32_t peers = __match_any_sync(0xffffffffu, d);
+      at[k] = 0;
+      if (in) at[k] = own[d] + __popc(peers & ((1u << lane) - 1u));
+      __syncwarp();
+      if (in && (peers >> lane) == 1u) own[d] = (uint16_t)(at[k] + 1);  // the last of its digit in the warp
+      __syncwarp();
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < digits; d += kClusterThreads) {
+      int before = 0;
+#pragma unroll 8
+      for (int w = 0; w < 32; ++w) {
+        const int n = mine[w * digits + d];
+        mine[w * digits + d] = (uint16_t)before;
+        before += n;
+      }
+      hist[d] = before;
+    }
+    tc::cluster_sync();
+    // places of the digits: those in front (an exclusive sum over the cluster's totals), CTAs in front
+    int before = 0, total = 0;
+    if ((int)threadIdx.x < digits)
+      for (int r = 0; r < ctas; ++r) {
+        const int n = of_cta(hist + threadIdx.x, r);
+        if (r < rank) before += n;
+        total += n;
+      }
+    int s = total;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += u;
+    }
+    if (lane == 31) sums[warp] = s;
+    __syncthreads();
+    if (warp == 0) {
+      int v = sums[lane];
+      const int own_sum = v;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
+      }
+      sums[lane] = v - own_sum;
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < digits) place[threadIdx.x] = sums[warp] + s - total + before;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kClusterEach; ++k) {
+      if (k >= each || key[k] < 0) continue;
+      const int d = key[k] >> shift & digits - 1, to = place[d] + own[d] + at[k];
+      key_out[to] = key[k];
+      pos_out[to] = pos[k];
+      if (pass == 0) atomicOr(p.rows + key[k] / 32, 1u << (key[k] & 31));
+    }
+    tc::cluster_sync();  // (the entries are in place, the counts have been read)
   }
 }
 
 // ------------------------------------------------------------------ sums
 struct SumP {
   const int32_t *key, *pos;  // sorted; padding (key V) stands at the end
+  const uint32_t* rows;      // a bit for each row of dW: its token occurs
   const void* d_out;
   void* dweight;
   float* part;               // [runs][2][D]: 0 of a token that began before the run, 1 of one that goes on behind it
@@ -210,17 +323,17 @@ struct SumP {
   float scale;
 };
 template <typename OUT, bool V>
-__device__ __forceinline__ void put_row(const SumP& p, int row, int c, f2 (&acc)[4]) {
+__device__ __forceinline__ void put_row(const SumP& p, int row, int c, int lane, int tpr, f2 (&acc)[4]) {
   OUT* to = static_cast<OUT*>(p.dweight) + (size_t)row * p.D;
 #pragma unroll
   for (int i = 0; i < 4; ++i) acc[i] = mul2(acc[i], dup2(p.scale));
   if (p.adds) {
     f2 old[4];
-    load8<OUT, V>(to, c, p.D, old);
+    load_cols<OUT, V>(to, c, lane, tpr, p.D, old);
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] = add2(old[i], acc[i]);
   }
-  store8<OUT, V>(to, c, p.D, acc);
+  store_cols<OUT, V>(to, c, lane, tpr, p.D, acc);
 }
 // Blocks 0 .. ceil(runs / groups) - 1 add up the runs, those behind write zeros to the rows of tokens that do not occur.
 constexpr int kZeroRows = 32;
@@ -229,25 +342,13 @@ __global__ void __launch_bounds__(256) embedding_bwd_kernel(SumP p, int tpr, int
   begin_dependent();
   const int groups = 256 / tpr, lane = threadIdx.x & (tpr - 1), group = threadIdx.x / tpr;
   if ((int)blockIdx.x >= sum_blocks) {
-    __shared__ uint32_t there;
-    const int64_t r0 = (int64_t)(blockIdx.x - sum_blocks) * kZeroRows;
-    if (threadIdx.x < kZeroRows) {  // whether row r0 + lane occurs: the first sorted entry that is not below it
-      const int64_t row = r0 + threadIdx.x;
-      int lo = 0, hi = p.N;
-      while (lo < hi) {
-        const int mid = lo + (hi - lo) / 2;
-        if (p.key[mid] < row) lo = mid + 1;
-        else hi = mid;
-      }
-      const uint32_t b = __ballot_sync(0xffffffffu, row >= p.V || (lo < p.N && p.key[lo] == row));
-      if (threadIdx.x == 0) there = b;
-    }
-    __syncthreads();
+    const int64_t word = blockIdx.x - sum_blocks, r0 = word * kZeroRows;
+    const uint32_t there = p.rows[word];
     f2 zero[4] = {0, 0, 0, 0};
     for (int r = group; r < kZeroRows; r += groups) {
-      if (there >> r & 1u) continue;
+      if (there >> r & 1u || r0 + r >= p.V) continue;
       OUT* to = static_cast<OUT*>(p.dweight) + (size_t)(r0 + r) * p.D;
-      for (int c = lane * 8; c < p.D; c += tpr * 8) store8<OUT, V>(to, c, p.D, zero);
+      for (int c = 0; c < p.D; c += tpr * 8) store_cols<OUT, V>(to, c, lane, tpr, p.D, zero);
     }
     return;
   }
@@ -257,28 +358,30 @@ __global__ void __launch_bounds__(256) embedding_bwd_kernel(SumP p, int tpr, int
   const int32_t *key = p.key + i0, *pos = p.pos + i0;
   const int before = i0 > 0 ? key[-1] : -1, behind = i0 + n < p.N ? key[n] : -1;
   constexpr int AHEAD = 8;
-  for (int c = lane * 8; c < p.D; c += tpr * 8) {
+  for (int c = 0; c < p.D; c += tpr * 8) {
     f2 acc[4] = {0, 0, 0, 0};
     bool began = key[0] != before;  // the token that is being added up began in this run
     for (int j0 = 0; j0 < n; j0 += AHEAD) {
-      f2 e[AHEAD][4];
+      Cols<IN, V> e[AHEAD];
       int k[AHEAD + 1];
 #pragma unroll
       for (int j = 0; j < AHEAD; ++j) {
         k[j] = j0 + j < n ? key[j0 + j] : p.V;
-        if (k[j] < p.V) load8<IN, V>(static_cast<const IN*>(p.d_out) + (size_t)pos[j0 + j] * p.D, c, p.D, e[j]);
+        if (k[j] < p.V) e[j].load(static_cast<const IN*>(p.d_out) + (size_t)pos[j0 + j] * p.D, c, lane, tpr, p.D);
       }
       k[AHEAD] = j0 + AHEAD < n ? key[j0 + AHEAD] : p.V;
 #pragma unroll
       for (int j = 0; j < AHEAD; ++j) {
         if (j0 + j >= n || k[j] >= p.V) continue;
+        f2 row[4];
+        e[j].get(row);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = add2(acc[i], e[j][i]);
+        for (int i = 0; i < 4; ++i) acc[i] = add2(acc[i], row[i]);
         const bool last = j0 + j + 1 == n;
         if (k[j + 1] == k[j] && !last) continue;
         const bool goes_on = last && behind == k[j];
-        if (began && !goes_on) put_row<OUT, V>(p, k[j], c, acc);
-        else store8<float, V>(p.part + ((size_t)run * 2 + (began ? 1 : 0)) * p.D, c, p.D, acc);
+        if (began && !goes_on) put_row<OUT, V>(p, k[j], c, lane, tpr, acc);
+        else store_cols<float, V>(p.part + ((size_t)run * 2 + (began ? 1 : 0)) * p.D, c, lane, tpr, p.D, acc);
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[i] = 0;
         began = true;
@@ -304,30 +407,28 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(SumP p) {
     else hi = mid;
   }
   const int n = (lo - 1) / p.run - run;  // partial rows besides the first
-  const int c = (blockIdx.y * 32 + lane) * 8, each = (n + 7) / 8, from = run + 1 + warp * each, to = min(from + each, run + 1 + n);
+  const int c = blockIdx.y * 256, each = (n + 7) / 8, from = run + 1 + warp * each, to = min(from + each, run + 1 + n);
   f2 acc[4] = {0, 0, 0, 0};
-  if (c < p.D) {
-    if (warp == 0) load8<float, V>(p.part + ((size_t)run * 2 + 1) * p.D, c, p.D, acc);
-    for (int r0 = from; r0 < to; r0 += 8) {
-      f2 e[8][4];
+  if (warp == 0) load_cols<float, V>(p.part + ((size_t)run * 2 + 1) * p.D, c, lane, 32, p.D, acc);
+  for (int r0 = from; r0 < to; r0 += 8) {
+    f2 e[8][4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (r0 + j < to) load8<float, V>(p.part + (size_t)(r0 + j) * 2 * p.D, c, p.D, e[j]);
+    for (int j = 0; j < 8; ++j)
+      if (r0 + j < to) load_cols<float, V>(p.part + (size_t)(r0 + j) * 2 * p.D, c, lane, 32, p.D, e[j]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (r0 + j < to)
+    for (int j = 0; j < 8; ++j)
+      if (r0 + j < to)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[i] = add2(acc[i], e[j][i]);
-    }
+        for (int i = 0; i < 4; ++i) acc[i] = add2(acc[i], e[j][i]);
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) sums[warp][lane][i] = acc[i];
   __syncthreads();
-  if (warp != 0 || c >= p.D) return;
+  if (warp != 0) return;
   for (int w = 1; w < 8; ++w)
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] = add2(acc[i], sums[w][lane][i]);
-  put_row<OUT, V>(p, tok, c, acc);
+  put_row<OUT, V>(p, tok, c, lane, 32, acc);
 }
 
 // ------------------------------------------------------------------ host
@@ -336,13 +437,14 @@ static int threads_per_row(int D) {  // a power of two, 8 columns a thread, 4 to
   while (8 * t < D && t < 256) t *= 2;
   return t;
 }
-// Entries of a run: enough runs to give every SM eight blocks, 8 to 64 entries.
+// Entries of a run: enough runs to give every SM four blocks, 8 to 64 entries.
 static int run_length(int64_t N, int D) {
-  const int64_t groups = 256 / threads_per_row(D), want = N / (148 * 8 * groups);
+  const int64_t groups = 256 / threads_per_row(D), want = N / (148 * 4 * groups);
   return (int)std::min<int64_t>(64, std::max<int64_t>(8, (want + 7) / 8 * 8));
 }
 struct Scratch {
   int32_t *key[2], *pos[2], *hist, *total;
+  uint32_t* rows;
   float* part;
   size_t bytes;
   int passes, bits, run, runs, tiles;
@@ -362,6 +464,7 @@ static Scratch carve(const mxb_embedding_desc* d, void* base) {
     s.key[i] = c.take<int32_t>(N);
     s.pos[i] = c.take<int32_t>(N);
   }
+  s.rows = c.take<uint32_t>((size_t)d->V / 32 + 1);
   s.hist = c.take<int32_t>(((size_t)1 << s.bits) * s.tiles);
   s.total = c.take<int32_t>((size_t)1 << s.bits);
   s.part = c.take<float>((size_t)s.runs * 2 * d->D);
@@ -417,22 +520,51 @@ size_t embedding_bwd_scratch(const mxb_embedding_desc* d) { return carve(d, null
 mxb_status embedding_bwd(const mxb_embedding_desc* d, const void* tokens, const void* d_out, void* dweight, int adds, void* workspace,
                          cudaStream_t st) {
   const Scratch s = carve(d, workspace);
-  SortP q{tokens, nullptr, nullptr, nullptr, nullptr, s.hist, (int)d->tokens, d->V, 0, 1 << s.bits, s.tiles};
-  int at = 0;
-  for (int pass = 0; pass < s.passes; ++pass, at ^= 1) {
-    q.shift = pass * s.bits;
-    q.key_out = s.key[at];
-    q.pos_out = s.pos[at];
+  const int last = (s.passes - 1) & 1;  // where the sorted entries are
+  if (d->tokens <= kClusterEntries) {
+    // about four entries a thread
+    int ctas = 1;
+    while (ctas < kClusterMost && (int64_t)ctas * kClusterThreads * 4 < d->tokens) ctas *= 2;
+    const ClusterP q{tokens, {s.key[0], s.key[1]}, {s.pos[0], s.pos[1]}, s.rows, (int)d->tokens, d->V, s.bits, s.passes, (int)((d->tokens + ctas - 1) / ctas)};
+    mxb_status st_ = MXB_OK;
     with_token(d, [&](auto tok) {
       using TOK = decltype(tok);
-      MXB_LAUNCH("embedding_count_kernel", st, (launch_kernel(embedding_count_kernel<TOK>, s.tiles, kSortThreads, 0, st, q)));
-      MXB_LAUNCH("embedding_scan_kernel", st, (launch_kernel(embedding_scan_kernel, 1 << s.bits, 256, 0, st, s.hist, s.total, s.tiles)));
-      MXB_LAUNCH("embedding_place_kernel", st, (launch_kernel(embedding_place_kernel<TOK>, s.tiles, kSortThreads, 0, st, q, s.total)));
+      const int smem = 32 * 2 << s.bits;
+      st_ = MXB_ALLOW_SMEM(64 * kMaxDigits, embedding_sort_kernel<TOK>);
+      if (st_ != MXB_OK) return;
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = ctas;
+      cfg.blockDim = kClusterThreads;
+      cfg.dynamicSmemBytes = smem;
+      cfg.stream = st;
+      cudaLaunchAttribute attr[2] = {};
+      attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attr[0].val.programmaticStreamSerializationAllowed = 1;
+      attr[1].id = cudaLaunchAttributeClusterDimension;
+      attr[1].val.clusterDim.x = ctas;
+      attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 2;
+      MXB_LAUNCH("embedding_sort_kernel", st, (cudaLaunchKernelEx(&cfg, embedding_sort_kernel<TOK>, q)));
     });
-    q.key_in = q.key_out;
-    q.pos_in = q.pos_out;
+    if (st_ != MXB_OK) return st_;
+  } else {
+    SortP q{tokens, nullptr, nullptr, nullptr, nullptr, s.hist, s.rows, (int)d->tokens, d->V, 0, 1 << s.bits, s.tiles};
+    for (int pass = 0; pass < s.passes; ++pass) {
+      q.shift = pass * s.bits;
+      q.key_out = s.key[pass & 1];
+      q.pos_out = s.pos[pass & 1];
+      with_token(d, [&](auto tok) {
+        using TOK = decltype(tok);
+        MXB_LAUNCH("embedding_count_kernel", st, (launch_kernel(embedding_count_kernel<TOK>, s.tiles, kSortThreads, 0, st, q)));
+        MXB_LAUNCH("embedding_scan_kernel", st, (launch_kernel(embedding_scan_kernel, 1 << s.bits, 256, 0, st, s.hist, s.total, s.tiles)));
+        MXB_LAUNCH("embedding_place_kernel", st, (launch_kernel(embedding_place_kernel<TOK>, s.tiles, kSortThreads, 0, st, q, s.total)));
+      });
+      q.key_in = q.key_out;
+      q.pos_in = q.pos_out;
+    }
   }
-  const SumP p{q.key_in, q.pos_in, d_out, dweight, s.part, (int)d->tokens, d->V, d->D, s.run, s.runs, adds, d->scale};
+  const SumP p{s.key[last], s.pos[last], s.rows, d_out, dweight, s.part, (int)d->tokens, d->V, d->D, s.run, s.runs, adds, d->scale};
   const int tpr = threads_per_row(d->D), groups = 256 / tpr, sums = (s.runs + groups - 1) / groups;
   const int zeros = adds ? 0 : (int)(((int64_t)d->V + kZeroRows - 1) / kZeroRows);
   with_type(d->io_dtype, [&](auto in) {

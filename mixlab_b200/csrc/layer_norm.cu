@@ -36,15 +36,40 @@ constexpr int kThreads = TPR > 256 ? TPR : 256;
 
 // h - m in the columns that there are, zero behind them.
 template <bool V>
-__device__ __forceinline__ void centre(f2 (&h)[4], int c, int D, f2 minus_m) {
+__device__ __forceinline__ void centre(f2 (&h)[4], int base, int lane, int tpr, int D, f2 minus_m) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     h[i] = add2(h[i], minus_m);
     if (V) {
-      if (c >= D) h[i] = 0;
+      if (base + lane * 8 >= D) h[i] = 0;
     } else {
       const float2 v = unpack2(h[i]);
-      h[i] = pack2(c + 2 * i < D ? v.x : 0.f, c + 2 * i + 1 < D ? v.y : 0.f);
+      const int c = col_of<false>(base, lane, tpr, 2 * i);
+      h[i] = pack2(c < D ? v.x : 0.f, c + tpr < D ? v.y : 0.f);
+    }
+  }
+}
+// Sums of M values over the TPR threads of a row.  One barrier: whoever calls it alternates between two places in shared memory, so
+// that the barrier of one sum stands between the reads of the last and the writes of the next.
+template <int TPR, int M>
+__device__ __forceinline__ void row_total(float (&v)[M], float* red) {
+#pragma unroll
+  for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int m = 0; m < M; ++m) v[m] += __shfl_xor_sync(0xffffffffu, v[m], o);
+  if constexpr (TPR > 32) {
+    constexpr int W = TPR / 32;
+    const int warp = threadIdx.x >> 5;
+    if ((threadIdx.x & 31) == 0)
+#pragma unroll
+      for (int m = 0; m < M; ++m) red[warp * M + m] = v[m];
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) s += red[(warp / W * W + w) * M + m];
+      v[m] = s;
     }
   }
 }
@@ -53,21 +78,21 @@ __device__ __forceinline__ void centre(f2 (&h)[4], int c, int D, f2 minus_m) {
 template <typename IO, typename RES, int TPR, int E, bool V>
 __global__ void __launch_bounds__(kThreads<TPR>) lnorm_fwd_kernel(NormP p) {
   begin_dependent();
-  __shared__ float red[kThreads<TPR> / 32];
+  __shared__ float red[2][kThreads<TPR> / 32];
   constexpr int GROUPS = kThreads<TPR> / TPR;
   const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
   const float inv = 1.f / (float)p.D;
   const RES* stream = static_cast<const RES*>(p.resid ? p.resid : p.x);
-  Ahead<RES, V> a_h[E];
-  Ahead<IO, V> a_x[E];
+  Cols<RES, V> a_h[E];
+  Cols<IO, V> a_x[E];
   auto offset = [&](size_t r0) { return (r0 + group < p.rows ? r0 + group : r0) * p.D; };
   auto request = [&](size_t r0) {
     const size_t off = offset(r0);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int c = (lane + e * TPR) * 8;
-      a_h[e].load(stream + off, c, p.D);
-      if (p.resid) a_x[e].load(static_cast<const IO*>(p.x) + off, c, p.D);
+      const int c = e * TPR * 8;
+      a_h[e].load(stream + off, c, lane, TPR, p.D);
+      if (p.resid) a_x[e].load(static_cast<const IO*>(p.x) + off, c, lane, TPR, p.D);
     }
   };
   request((size_t)blockIdx.x * GROUPS);
@@ -77,11 +102,11 @@ __global__ void __launch_bounds__(kThreads<TPR>) lnorm_fwd_kernel(NormP p) {
     f2 h[E][4], sum = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int c = (lane + e * TPR) * 8;
-      a_h[e].get(stream + off, c, p.D, h[e]);
+      const int c = e * TPR * 8;
+      a_h[e].get(h[e]);
       if (p.resid) {
         f2 x[4];
-        a_x[e].get(static_cast<const IO*>(p.x) + off, c, p.D, x);
+        a_x[e].get(x);
 #pragma unroll
         for (int i = 0; i < 4; ++i) h[e][i] = add2(h[e][i], x[i]);
       }
@@ -90,29 +115,29 @@ __global__ void __launch_bounds__(kThreads<TPR>) lnorm_fwd_kernel(NormP p) {
     }
     if (r0 + (size_t)gridDim.x * GROUPS < p.rows) request(r0 + (size_t)gridDim.x * GROUPS);
     float s[1] = {sum2(sum)};
-    row_sum<TPR>(s, red);
+    row_total<TPR>(s, red[0]);
     const f2 minus_m = dup2(-s[0] * inv);
     sum = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int c = (lane + e * TPR) * 8;
-      if (p.resid && live) store8<RES, V>(static_cast<RES*>(p.stream) + off, c, p.D, h[e]);
-      centre<V>(h[e], c, p.D, minus_m);
+      const int c = e * TPR * 8;
+      if (p.resid && live) store_cols<RES, V>(static_cast<RES*>(p.stream) + off, c, lane, TPR, p.D, h[e]);
+      centre<V>(h[e], c, lane, TPR, p.D, minus_m);
 #pragma unroll
       for (int i = 0; i < 4; ++i) fma2(sum, h[e][i], h[e][i]);
     }
     s[0] = sum2(sum);
-    row_sum<TPR>(s, red);
+    row_total<TPR>(s, red[1]);
     const f2 k = dup2(rsqrtf(s[0] * inv + p.eps));
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int c = (lane + e * TPR) * 8;
+      const int c = e * TPR * 8;
       f2 w[4], b[4] = {0, 0, 0, 0};
-      load8<float, V>(p.weight, c, p.D, w);
-      if (p.bias) load8<float, V>(p.bias, c, p.D, b);
+      load_cols<float, V>(p.weight, c, lane, TPR, p.D, w);
+      if (p.bias) load_cols<float, V>(p.bias, c, lane, TPR, p.D, b);
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = mad2(mul2(h[e][i], k), w[i], b[i]);
-      if (live) store8<IO, V>(static_cast<IO*>(p.n) + off, c, p.D, w);
+      if (live) store_cols<IO, V>(static_cast<IO*>(p.n) + off, c, lane, TPR, p.D, w);
     }
   }
 }
@@ -120,7 +145,7 @@ __global__ void __launch_bounds__(kThreads<TPR>) lnorm_fwd_kernel(NormP p) {
 template <typename IO, typename RES, int TPR, int E, bool V>
 __global__ void __launch_bounds__(kThreads<TPR>, TPR > 256 || E > 1 ? 1 : 2) lnorm_bwd_kernel(NormP p) {
   begin_dependent();
-  __shared__ float red[kThreads<TPR> / 32 * 3];
+  __shared__ float red[kThreads<TPR> / 32], red3[kThreads<TPR> / 32 * 3];
   constexpr int GROUPS = kThreads<TPR> / TPR;
   const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
   const float inv = 1.f / (float)p.D;
@@ -129,17 +154,17 @@ __global__ void __launch_bounds__(kThreads<TPR>, TPR > 256 || E > 1 ? 1 : 2) lno
   for (int e = 0; e < E; ++e)
 #pragma unroll
     for (int i = 0; i < 4; ++i) dw[e][i] = db[e][i] = 0;
-  Ahead<RES, V> a_h[E], a_d[E];
-  Ahead<IO, V> a_g[E];
+  Cols<RES, V> a_h[E], a_d[E];
+  Cols<IO, V> a_g[E];
   auto offset = [&](size_t r0) { return (r0 + group < p.rows ? r0 + group : r0) * p.D; };
   auto request = [&](size_t r0) {
     const size_t off = offset(r0);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int c = (lane + e * TPR) * 8;
-      a_h[e].load(static_cast<const RES*>(p.x) + off, c, p.D);
-      a_g[e].load(static_cast<const IO*>(p.dn) + off, c, p.D);
-      if (p.d_resid) a_d[e].load(static_cast<const RES*>(p.d_resid) + off, c, p.D);
+      const int c = e * TPR * 8;
+      a_h[e].load(static_cast<const RES*>(p.x) + off, c, lane, TPR, p.D);
+      a_g[e].load(static_cast<const IO*>(p.dn) + off, c, lane, TPR, p.D);
+      if (p.d_resid) a_d[e].load(static_cast<const RES*>(p.d_resid) + off, c, lane, TPR, p.D);
     }
   };
   request((size_t)blockIdx.x * GROUPS);
@@ -149,11 +174,11 @@ __global__ void __launch_bounds__(kThreads<TPR>, TPR > 256 || E > 1 ? 1 : 2) lno
     f2 h[E][4], g[E][4], d[E][4], sum = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int c = (lane + e * TPR) * 8;
-      a_h[e].get(static_cast<const RES*>(p.x) + off, c, p.D, h[e]);
-      a_g[e].get(static_cast<const IO*>(p.dn) + off, c, p.D, g[e]);
+      const int c = e * TPR * 8;
+      a_h[e].get(h[e]);
+      a_g[e].get(g[e]);
       if (p.d_resid) {
-        a_d[e].get(static_cast<const RES*>(p.d_resid) + off, c, p.D, d[e]);
+        a_d[e].get(d[e]);
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) d[e][i] = 0;
@@ -163,15 +188,15 @@ __global__ void __launch_bounds__(kThreads<TPR>, TPR > 256 || E > 1 ? 1 : 2) lno
     }
     if (r0 + (size_t)gridDim.x * GROUPS < p.rows) request(r0 + (size_t)gridDim.x * GROUPS);
     float m[1] = {sum2(sum)};
-    row_sum<TPR>(m, red);
+    row_total<TPR>(m, red);
     const f2 minus_m = dup2(-m[0] * inv);
     f2 s0 = 0, s1 = 0, s2 = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int c = (lane + e * TPR) * 8;
-      centre<V>(h[e], c, p.D, minus_m);
+      const int c = e * TPR * 8;
+      centre<V>(h[e], c, lane, TPR, p.D, minus_m);
       f2 w[4];
-      load8<float, V>(p.weight, c, p.D, w);
+      load_cols<float, V>(p.weight, c, lane, TPR, p.D, w);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const f2 t = mul2(g[e][i], w[i]);
@@ -181,14 +206,14 @@ __global__ void __launch_bounds__(kThreads<TPR>, TPR > 256 || E > 1 ? 1 : 2) lno
       }
     }
     float s[3] = {sum2(s0), sum2(s1), sum2(s2)};
-    row_sum<TPR>(s, red);
+    row_total<TPR>(s, red3);
     const float k = rsqrtf(s[0] * inv + p.eps);
     const f2 kk = dup2(k), mt = dup2(-s[1] * inv), mtu = dup2(-k * k * s[2] * inv);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int c = (lane + e * TPR) * 8;
+      const int c = e * TPR * 8;
       f2 w[4];
-      load8<float, V>(p.weight, c, p.D, w);
+      load_cols<float, V>(p.weight, c, lane, TPR, p.D, w);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (live) {
@@ -197,15 +222,15 @@ __global__ void __launch_bounds__(kThreads<TPR>, TPR > 256 || E > 1 ? 1 : 2) lno
         }
         d[e][i] = mad2(kk, mad2(h[e][i], mtu, mad2(g[e][i], w[i], mt)), d[e][i]);
       }
-      if (live) store8<RES, V>(static_cast<RES*>(p.dx) + off, c, p.D, d[e]);
+      if (live) store_cols<RES, V>(static_cast<RES*>(p.dx) + off, c, lane, TPR, p.D, d[e]);
     }
   }
   float* part = p.part + ((size_t)blockIdx.x * GROUPS + group) * 2 * p.D;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const int c = (lane + e * TPR) * 8;
-    store8<float, false>(part, c, p.D, dw[e]);
-    store8<float, false>(part + p.D, c, p.D, db[e]);
+    const int c = e * TPR * 8;
+    store_cols<float, V>(part, c, lane, TPR, p.D, dw[e]);
+    store_cols<float, V>(part + p.D, c, lane, TPR, p.D, db[e]);
   }
 }
 // Sums of the partial rows.  grid (column blocks, 2): dw, db.

@@ -35,7 +35,7 @@ struct PackP {
   const float *lse, *d_loss, *d_lse;  // backward; d_lse may be null
   const int32_t* counts;              // of every kCountRows rows (where there are as many)
   int32_t *live, *idx, *tgt;          // how many; their rows; their targets
-  float *a, *both, *lse2;             // their gradients of loss and of both, lse in powers of two
+  float *a, *both, *lse2;             // their gradients of loss and of both, lse (bf16: in powers of two)
   bf16* xc;                           // [parts][pad][Dp]
   void* dx;                           // backward: rows of the other tokens become zero
   float *loss, *lse_out;              // forward: likewise
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(256) lce_pack_kernel(PackP p, int row_blocks) 
       const float a = p.d_loss[r];
       p.a[j] = a;
       p.both[j] = p.d_lse ? a + p.d_lse[r] : a;
-      p.lse2[j] = p.lse[r] * kLog2e;
+      p.lse2[j] = sizeof(T) == 4 ? p.lse[r] : p.lse[r] * kLog2e;
     }
   }
   pack_row<T>(static_cast<const T*>(p.x) + r * p.D, p.xc + j * p.Dp, p.pad * p.Dp, p.D, p.Dp, lane);
@@ -192,7 +192,7 @@ struct Cfg {
   static constexpr bool A_MN = MODE == kDw, B_MN = MODE == kDx || MODE == kDw;
   static constexpr int SMEM = 1024 + STAGES * STAGE + STAGING + 256 + (MODE == kStats ? 128 + 4 * 128 * 8 : 0);
 };
-constexpr int kThreads = 320, kSegment = 32;  // blocks of 64 that a float32 accumulator takes before it is added up in registers
+constexpr int kThreads = 320, kSegment = 4;  // blocks of 64 that a float32 accumulator takes before it is added up in registers
 struct GemmP {
   const int32_t* live;
   int32_t* status;
@@ -498,9 +498,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
             }
           }
         } else {
+          // (float32: the logit's distance from lse first, which leaves the exponent the error of that distance alone)
           const float both = p.both[row], back = -p.lse2[row];
 #pragma unroll
-          for (int c = 0; c < C::COLS; ++c) v[c] = both * ex2(fmaf(v[c], kLog2e, back));
+          for (int c = 0; c < C::COLS; ++c) v[c] = both * ex2(F32 ? (v[c] + back) * kLog2e : fmaf(v[c], kLog2e, back));
           if (row >= live || here < C::COLS)
 #pragma unroll
             for (int c = 0; c < C::COLS; ++c) v[c] = row < live && c < here ? v[c] : 0.f;

@@ -233,7 +233,10 @@ def test_layer_norm_at_any_element_and_in_place(D):
     d = _lib.LayerNormDesc(rows, D, _lib.MXB_F32, _lib.MXB_F32, 1e-5)
     p, st = lambda t: C.c_void_p(t.data_ptr()), C.c_void_p(torch.cuda.current_stream().cuda_stream)  # noqa: E731
     assert lib.mxb_layer_norm_fwd(C.byref(d), None, p(x), p(w), None, None, p(n[1:]), st) == 0
-    assert n[0] == 9 and n[-1] == 9 and torch.equal(n[1:-1].view(rows, D), ops.layer_norm(x.clone(), w))
+    # (single elements a thread add up in another order than whole pieces: the same bounds, not the same bits)
+    want = step_ends.layer_norm(x.double().cpu(), w.double().cpu())[1]
+    near(n[1:-1].view(rows, D), want, norm_slack(x.double().cpu(), w.double().cpu(), None, 1e-5), (F32, "norm"))
+    assert n[0] == 9 and n[-1] == 9
     # the stream and its gradient in place
     r, y = rnd(g, rows, D).cuda(), rnd(g, rows, D).cuda()
     want_h, want_n = ops.layer_norm(y, w, resid=r)
