@@ -80,7 +80,7 @@ struct SortP {
   const int32_t *key_in, *pos_in;  // null in the first pass
   int32_t *key_out, *pos_out;
   int32_t* hist;                   // [digits][tiles]
-  uint32_t* rows;                  // the first pass: a bit for each token that occurs
+  uint32_t* rows;                  // the first pass sets it to zero
   int N, V, shift, digits, tiles;
 };
 template <typename TOK>
@@ -201,8 +201,19 @@ __global__ void __launch_bounds__(kSortThreads) embedding_place_kernel(SortP p, 
     const int d = (key[k] >> p.shift) & (p.digits - 1), to = place[d] + mine[warp][d] + rank[k];
     p.key_out[to] = key[k];
     p.pos_out[to] = p.pos_in ? p.pos_in[i] : (int)i;
-    if (!p.key_in) atomicOr(p.rows + key[k] / 32, 1u << (key[k] & 31));
   }
+}
+
+// A bit for each token that occurs, by its first entry in sorted order.  (By every entry, words of frequent tokens are updated so
+// often that the updates, one after the other, took 20 us of 32768 tokens.)
+__device__ __forceinline__ void mark_first(const int32_t* key, int i, uint32_t* rows) {
+  const int k = key[i];
+  if (i == 0 || key[i - 1] != k) atomicOr(rows + k / 32, 1u << (k & 31));
+}
+__global__ void __launch_bounds__(256) embedding_mark_kernel(const int32_t* key, int N, uint32_t* rows) {
+  begin_dependent();
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < N) mark_first(key, (int)i, rows);
 }
 
 // The whole sort in one launch for up to kClusterEntries entries: a cluster of CTAs, each with an equal share of the entries, that read
@@ -262,23 +273,32 @@ __global__ void __launch_bounds__(kClusterThreads) embedding_sort_kernel(Cluster
     __syncthreads();
     for (int d = threadIdx.x; d < digits; d += kClusterThreads) {
       int before = 0;
-#pragma unroll 8
-      for (int w = 0; w < 32; ++w) {
-        const int n = mine[w * digits + d];
-        mine[w * digits + d] = (uint16_t)before;
-        before += n;
+#pragma unroll
+      for (int w0 = 0; w0 < 32; w0 += 16) {
+        int n[16];
+#pragma unroll
+        for (int w = 0; w < 16; ++w) n[w] = mine[(w0 + w) * digits + d];
+#pragma unroll
+        for (int w = 0; w < 16; ++w) {
+          mine[(w0 + w) * digits + d] = (uint16_t)before;
+          before += n[w];
+        }
       }
       hist[d] = before;
     }
     tc::cluster_sync();
     // places of the digits: those in front (an exclusive sum over the cluster's totals), CTAs in front
     int before = 0, total = 0;
-    if ((int)threadIdx.x < digits)
-      for (int r = 0; r < ctas; ++r) {
-        const int n = of_cta(hist + threadIdx.x, r);
-        if (r < rank) before += n;
-        total += n;
+    if ((int)threadIdx.x < digits) {
+      int n[kClusterMost];
+#pragma unroll
+      for (int r = 0; r < kClusterMost; ++r) n[r] = r < ctas ? of_cta(hist + threadIdx.x, r) : 0;
+#pragma unroll
+      for (int r = 0; r < kClusterMost; ++r) {
+        if (r < rank) before += n[r];
+        total += n[r];
       }
+    }
     int s = total;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -306,10 +326,11 @@ __global__ void __launch_bounds__(kClusterThreads) embedding_sort_kernel(Cluster
       const int d = key[k] >> shift & digits - 1, to = place[d] + own[d] + at[k];
       key_out[to] = key[k];
       pos_out[to] = pos[k];
-      if (pass == 0) atomicOr(p.rows + key[k] / 32, 1u << (key[k] & 31));
     }
     tc::cluster_sync();  // (the entries are in place, the counts have been read)
   }
+  const int32_t* key = p.passes & 1 ? p.key[0] : p.key[1];
+  for (int i = rank * kClusterThreads + threadIdx.x; i < p.N; i += ctas * kClusterThreads) mark_first(key, i, p.rows);
 }
 
 // ------------------------------------------------------------------ sums
@@ -338,7 +359,7 @@ __device__ __forceinline__ void put_row(const SumP& p, int row, int c, int lane,
 // Blocks 0 .. ceil(runs / groups) - 1 add up the runs, those behind write zeros to the rows of tokens that do not occur.
 constexpr int kZeroRows = 32;
 template <typename IN, typename OUT, bool V>
-__global__ void __launch_bounds__(256) embedding_bwd_kernel(SumP p, int tpr, int sum_blocks) {
+__global__ void __launch_bounds__(256, V ? 4 : 2) embedding_bwd_kernel(SumP p, int tpr, int sum_blocks) {
   begin_dependent();
   const int groups = 256 / tpr, lane = threadIdx.x & (tpr - 1), group = threadIdx.x / tpr;
   if ((int)blockIdx.x >= sum_blocks) {
@@ -352,35 +373,48 @@ __global__ void __launch_bounds__(256) embedding_bwd_kernel(SumP p, int tpr, int
     }
     return;
   }
+  // the runs' entries, the one in front and the one behind (-1: none)
+  extern __shared__ int32_t entries[];  // [groups][run + 2] tokens, [groups][run] positions
+  const int64_t begin = (int64_t)blockIdx.x * groups * p.run;
+  for (int k = threadIdx.x; k < groups * (p.run + 2); k += 256) {
+    const int64_t i = begin + (int64_t)(k / (p.run + 2)) * p.run + k % (p.run + 2) - 1;
+    entries[k] = i >= 0 && i < p.N ? p.key[i] : -1;
+  }
+  for (int k = threadIdx.x; k < groups * p.run; k += 256) entries[groups * (p.run + 2) + k] = begin + k < p.N ? p.pos[begin + k] : 0;
+  __syncthreads();
   const int64_t run = (int64_t)blockIdx.x * groups + group, i0 = run * p.run;
   if (i0 >= p.N) return;
   const int n = (int)min((int64_t)p.run, p.N - i0);
-  const int32_t *key = p.key + i0, *pos = p.pos + i0;
-  const int before = i0 > 0 ? key[-1] : -1, behind = i0 + n < p.N ? key[n] : -1;
-  constexpr int AHEAD = 8;
+  const int32_t *key = entries + group * (p.run + 2) + 1, *pos = entries + groups * (p.run + 2) + group * p.run;
+  constexpr int R = sizeof(IN) == 4 ? 2 : 4;  // rows in a batch; the next batch is under way while one is added up
   for (int c = 0; c < p.D; c += tpr * 8) {
     f2 acc[4] = {0, 0, 0, 0};
-    bool began = key[0] != before;  // the token that is being added up began in this run
-    for (int j0 = 0; j0 < n; j0 += AHEAD) {
-      Cols<IN, V> e[AHEAD];
-      int k[AHEAD + 1];
+    bool began = key[0] != key[-1];  // the token that is being added up began in this run
+    Cols<IN, V> next[R];
+    auto request = [&](int j0) {
 #pragma unroll
-      for (int j = 0; j < AHEAD; ++j) {
-        k[j] = j0 + j < n ? key[j0 + j] : p.V;
-        if (k[j] < p.V) e[j].load(static_cast<const IN*>(p.d_out) + (size_t)pos[j0 + j] * p.D, c, lane, tpr, p.D);
-      }
-      k[AHEAD] = j0 + AHEAD < n ? key[j0 + AHEAD] : p.V;
+      for (int j = 0; j < R; ++j)
+        if (j0 + j < n && key[j0 + j] < p.V) next[j].load(static_cast<const IN*>(p.d_out) + (size_t)pos[j0 + j] * p.D, c, lane, tpr, p.D);
+    };
+    request(0);
+    for (int j0 = 0; j0 < n; j0 += R) {
+      Cols<IN, V> e[R];
 #pragma unroll
-      for (int j = 0; j < AHEAD; ++j) {
-        if (j0 + j >= n || k[j] >= p.V) continue;
+      for (int j = 0; j < R; ++j) e[j] = next[j];
+      request(j0 + R);
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        const int at = j0 + j;
+        if (at >= n) break;
+        const int k = key[at];
+        if (k >= p.V) break;
         f2 row[4];
         e[j].get(row);
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[i] = add2(acc[i], row[i]);
-        const bool last = j0 + j + 1 == n;
-        if (k[j + 1] == k[j] && !last) continue;
-        const bool goes_on = last && behind == k[j];
-        if (began && !goes_on) put_row<OUT, V>(p, k[j], c, lane, tpr, acc);
+        if (key[at + 1] == k && at + 1 < n) continue;
+        // the token's last entry, or the run's
+        if (began && key[at + 1] != k) put_row<OUT, V>(p, k, c, lane, tpr, acc);
         else store_cols<float, V>(p.part + ((size_t)run * 2 + (began ? 1 : 0)) * p.D, c, lane, tpr, p.D, acc);
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[i] = 0;
@@ -389,38 +423,68 @@ __global__ void __launch_bounds__(256) embedding_bwd_kernel(SumP p, int tpr, int
     }
   }
 }
-// Tokens that lie in more than one run: the block of the run where one begins adds up its partial rows, each of its warps those of
-// consecutive runs, then the warps' sums one after the other.  grid (runs - 1, pieces of 256 columns).
+// Tokens that lie in more than one run: the warp of the run where one begins adds up its partial rows in the order of the runs; those
+// of a token in more than kLong runs are added by all warps of its block, each those of consecutive runs, then the warps' sums in
+// order.  (A block's eight runs hold the beginning of one such token at most.)  grid (blocks of eight runs, pieces of 256 columns).
+constexpr int kLong = 8;
+template <bool V>
+__device__ __forceinline__ void add_rows(const SumP& p, int from, int to, int c, int lane, f2 (&acc)[4]) {
+  for (int r0 = from; r0 < to; r0 += 4) {
+    Cols<float, V> e[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (r0 + j < to) e[j].load(p.part + (size_t)(r0 + j) * 2 * p.D, c, lane, 32, p.D);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (r0 + j >= to) break;
+      f2 row[4];
+      e[j].get(row);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] = add2(acc[i], row[i]);
+    }
+  }
+}
 template <typename OUT, bool V>
 __global__ void __launch_bounds__(256) embedding_join_kernel(SumP p) {
   begin_dependent();
   __shared__ f2 sums[8][32][4];
-  const int run = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ int long_run, long_rows, long_tok;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, run = blockIdx.x * 8 + warp, c = blockIdx.y * 256;
+  if (threadIdx.x == 0) long_run = -1;
+  __syncthreads();
   const int64_t begin = (int64_t)run * p.run, end = begin + p.run;
-  const int tok = p.key[end];  // (there is a run behind this one)
-  if (tok >= p.V || p.key[end - 1] != tok) return;
-  if (run > 0 && p.key[begin] == tok && p.key[begin - 1] == tok) return;  // it began before
-  int lo = (int)end, hi = p.N;  // the first entry behind the token's
-  while (lo < hi) {
-    const int mid = lo + (hi - lo) / 2;
-    if (p.key[mid] <= tok) lo = mid + 1;
-    else hi = mid;
+  if (end < p.N) {
+    const int tok = p.key[end];
+    const bool starts = tok < p.V && p.key[end - 1] == tok && !(run > 0 && p.key[begin] == tok && p.key[begin - 1] == tok);
+    if (starts) {
+      int lo = (int)end, hi = p.N;  // the first entry behind the token's
+      if (end + p.run < p.N && p.key[end + p.run] != tok) hi = (int)end + p.run;
+      while (lo < hi) {
+        const int mid = lo + (hi - lo) / 2;
+        if (p.key[mid] <= tok) lo = mid + 1;
+        else hi = mid;
+      }
+      const int n = (lo - 1) / p.run - run;  // partial rows besides the first
+      if (n > kLong) {
+        if (lane == 0) {
+          long_run = run;
+          long_rows = n;
+          long_tok = tok;
+        }
+      } else {
+        f2 acc[4];
+        load_cols<float, V>(p.part + ((size_t)run * 2 + 1) * p.D, c, lane, 32, p.D, acc);
+        add_rows<V>(p, run + 1, run + 1 + n, c, lane, acc);
+        put_row<OUT, V>(p, tok, c, lane, 32, acc);
+      }
+    }
   }
-  const int n = (lo - 1) / p.run - run;  // partial rows besides the first
-  const int c = blockIdx.y * 256, each = (n + 7) / 8, from = run + 1 + warp * each, to = min(from + each, run + 1 + n);
+  __syncthreads();
+  if (long_run < 0) return;
   f2 acc[4] = {0, 0, 0, 0};
-  if (warp == 0) load_cols<float, V>(p.part + ((size_t)run * 2 + 1) * p.D, c, lane, 32, p.D, acc);
-  for (int r0 = from; r0 < to; r0 += 8) {
-    f2 e[8][4];
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (r0 + j < to) load_cols<float, V>(p.part + (size_t)(r0 + j) * 2 * p.D, c, lane, 32, p.D, e[j]);
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (r0 + j < to)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = add2(acc[i], e[j][i]);
-  }
+  if (warp == 0) load_cols<float, V>(p.part + ((size_t)long_run * 2 + 1) * p.D, c, lane, 32, p.D, acc);
+  const int each = (long_rows + 7) / 8, from = long_run + 1 + warp * each, to = min(from + each, long_run + 1 + long_rows);
+  add_rows<V>(p, from, to, c, lane, acc);
 #pragma unroll
   for (int i = 0; i < 4; ++i) sums[warp][lane][i] = acc[i];
   __syncthreads();
@@ -428,7 +492,7 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(SumP p) {
   for (int w = 1; w < 8; ++w)
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] = add2(acc[i], sums[w][lane][i]);
-  put_row<OUT, V>(p, tok, c, lane, 32, acc);
+  put_row<OUT, V>(p, long_tok, c, lane, 32, acc);
 }
 
 // ------------------------------------------------------------------ host
@@ -437,10 +501,10 @@ static int threads_per_row(int D) {  // a power of two, 8 columns a thread, 4 to
   while (8 * t < D && t < 256) t *= 2;
   return t;
 }
-// Entries of a run: enough runs to give every SM four blocks, 8 to 64 entries.
+// Entries of a run: enough runs to give every SM eight blocks, 8 to 32 entries.
 static int run_length(int64_t N, int D) {
-  const int64_t groups = 256 / threads_per_row(D), want = N / (148 * 4 * groups);
-  return (int)std::min<int64_t>(64, std::max<int64_t>(8, (want + 7) / 8 * 8));
+  const int64_t groups = 256 / threads_per_row(D), want = N / (148 * 8 * groups);
+  return (int)std::min<int64_t>(32, std::max<int64_t>(8, (want + 7) / 8 * 8));
 }
 struct Scratch {
   int32_t *key[2], *pos[2], *hist, *total;
@@ -481,9 +545,7 @@ static void with_type(int32_t type, F&& f) {
   if (type == MXB_F32) f(float{});
   else f(bf16{});
 }
-static bool whole_pieces(int D, const void* a, const void* b) {
-  return D % 8 == 0 && ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) == 0;
-}
+static uintptr_t address(const void* p) { return reinterpret_cast<uintptr_t>(p); }
 
 }  // namespace embed
 
@@ -499,7 +561,7 @@ mxb_status embedding_fwd(const mxb_embedding_desc* d, const void* tokens, const 
                (launch_kernel(embedding_fwd_kernel<decltype(tok), decltype(in), decltype(o), R, decltype(whole)::value>,
                               (unsigned)std::min<int64_t>(want, 148 * 8), 256, 0, st, p, tpr)));
   };
-  const bool whole = whole_pieces(d->D, weight, out), many = d->tokens >= (int64_t)148 * 8 * groups;
+  const bool whole = whole_pieces(address(weight) | address(out), d->D), many = d->tokens >= (int64_t)148 * 8 * groups;
   with_token(d, [&](auto tok) {
     with_type(d->io_dtype, [&](auto in) {
       with_type(d->out_dtype, [&](auto o) {
@@ -563,6 +625,8 @@ mxb_status embedding_bwd(const mxb_embedding_desc* d, const void* tokens, const 
       q.key_in = q.key_out;
       q.pos_in = q.pos_out;
     }
+    MXB_LAUNCH("embedding_mark_kernel", st,
+               (launch_kernel(embedding_mark_kernel, (unsigned)((d->tokens + 255) / 256), 256, 0, st, s.key[last], (int)d->tokens, s.rows)));
   }
   const SumP p{s.key[last], s.pos[last], s.rows, d_out, dweight, s.part, (int)d->tokens, d->V, d->D, s.run, s.runs, adds, d->scale};
   const int tpr = threads_per_row(d->D), groups = 256 / tpr, sums = (s.runs + groups - 1) / groups;
@@ -572,12 +636,13 @@ mxb_status embedding_bwd(const mxb_embedding_desc* d, const void* tokens, const 
       auto launch = [&](auto whole) {
         constexpr bool W = decltype(whole)::value;
         MXB_LAUNCH("embedding_bwd_kernel", st,
-                   (launch_kernel(embedding_bwd_kernel<decltype(in), decltype(o), W>, sums + zeros, 256, 0, st, p, tpr, sums)));
+                   (launch_kernel(embedding_bwd_kernel<decltype(in), decltype(o), W>, sums + zeros, 256, groups * (2 * s.run + 2) * sizeof(int32_t), st,
+                                  p, tpr, sums)));
         if (s.runs > 1)
           MXB_LAUNCH("embedding_join_kernel", st,
-                     (launch_kernel(embedding_join_kernel<decltype(o), W>, dim3(s.runs - 1, (d->D + 255) / 256), 256, 0, st, p)));
+                     (launch_kernel(embedding_join_kernel<decltype(o), W>, dim3((s.runs + 6) / 8, (d->D + 255) / 256), 256, 0, st, p)));
       };
-      if (whole_pieces(d->D, d_out, dweight)) launch(std::true_type{});
+      if (whole_pieces(address(d_out) | address(dweight), d->D)) launch(std::true_type{});
       else launch(std::false_type{});
     });
   });

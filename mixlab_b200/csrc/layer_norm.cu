@@ -319,7 +319,7 @@ static mxb_status by_alignment(const NormP& p, float* dweight, float* dbias, cud
   for (const void* q : {p.resid, p.x, (const void*)p.weight, (const void*)p.bias, (const void*)p.stream, (const void*)p.n, p.d_resid, p.dn,
                         (const void*)p.dx})
     at |= reinterpret_cast<uintptr_t>(q);
-  return at % 16 == 0 && p.D % 8 == 0 ? run<IO, RES, true>(p, dweight, dbias, st) : run<IO, RES, false>(p, dweight, dbias, st);
+  return whole_pieces(at, p.D) ? run<IO, RES, true>(p, dweight, dbias, st) : run<IO, RES, false>(p, dweight, dbias, st);
 }
 static mxb_status by_type(const mxb_layer_norm_desc* d, const NormP& p, float* dweight, float* dbias, cudaStream_t st) {
   if (d->io_dtype == MXB_F32) return by_alignment<float, float>(p, dweight, dbias, st);

@@ -90,6 +90,19 @@ struct Ahead {
     }
   }
 };
+// Eight floats in one access (32 bytes, on 32 bytes): two of 16 would write each sector of 32 bytes in halves.
+__device__ __forceinline__ void load_floats(const float* p, uint32_t (&r)[8]) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "l"(p)
+               : "memory");
+}
+__device__ __forceinline__ void store_floats(float* p, const f2 (&e)[4]) {
+  asm volatile("st.global.v4.b64 [%0], {%1, %2, %3, %4};" ::"l"(p), "l"(e[0]), "l"(e[1]), "l"(e[2]), "l"(e[3]) : "memory");
+}
+// Whether every tensor of D columns may be read and written in such pieces, by the addresses' bits.
+inline bool whole_pieces(uintptr_t bits, int D) { return bits % 32 == 0 && D % 8 == 0; }
+
 // Eight columns of a row by each of its `tpr` threads, from column `base` on.  Whole pieces (V): eight neighbours a thread.  Else
 // thread `lane` takes base + lane + j tpr, so that a warp's accesses lie side by side (eight neighbours a thread in single
 // elements: gradients of a layer norm of 4001 x 449 in float32 23 us).
@@ -97,7 +110,12 @@ template <bool V>
 __device__ __forceinline__ int col_of(int base, int lane, int tpr, int j) { return V ? base + lane * 8 + j : base + lane + j * tpr; }
 template <typename T, bool V>
 __device__ __forceinline__ void load_cols(const T* row, int base, int lane, int tpr, int D, f2 (&e)[4]) {
-  if constexpr (V) {
+  if constexpr (V && sizeof(T) == 4) {
+    uint32_t r[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (base + lane * 8 < D) load_floats(row + base + lane * 8, r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+  } else if constexpr (V) {
     load8<T, true>(row, base + lane * 8, D, e);
   } else {
     float v[8];
@@ -112,7 +130,9 @@ __device__ __forceinline__ void load_cols(const T* row, int base, int lane, int 
 }
 template <typename T, bool V>
 __device__ __forceinline__ void store_cols(T* row, int base, int lane, int tpr, int D, const f2 (&e)[4]) {
-  if constexpr (V) {
+  if constexpr (V && sizeof(T) == 4) {
+    if (base + lane * 8 < D) store_floats(row + base + lane * 8, e);
+  } else if constexpr (V) {
     store8<T, true>(row, base + lane * 8, D, e);
   } else {
 #pragma unroll
@@ -127,14 +147,21 @@ __device__ __forceinline__ void store_cols(T* row, int base, int lane, int tpr, 
 // ... as they are in memory, requested ahead of their use.
 template <typename T, bool V>
 struct Cols {
-  static constexpr int W = V ? (sizeof(T) == 4 ? 2 : 1) : 1;
-  uint4 raw[W];
+  static constexpr int W = V ? 2 * sizeof(T) : 1;  // words
+  uint32_t raw[W];
   T one[V ? 1 : 8];
   __device__ __forceinline__ void load(const T* row, int base, int lane, int tpr, int D) {
     if constexpr (V) {
       const int c = base + lane * 8;
 #pragma unroll
-      for (int i = 0; i < W; ++i) raw[i] = c < D ? reinterpret_cast<const uint4*>(row + c)[i] : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < W; ++i) raw[i] = 0;
+      if (c >= D) return;
+      if constexpr (sizeof(T) == 4) {
+        load_floats(row + c, raw);
+      } else {
+        const uint4 v = *reinterpret_cast<const uint4*>(row + c);
+        raw[0] = v.x; raw[1] = v.y; raw[2] = v.z; raw[3] = v.w;
+      }
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -149,12 +176,9 @@ struct Cols {
       for (int i = 0; i < 4; ++i) e[i] = pack2(to_f32(one[2 * i]), to_f32(one[2 * i + 1]));
     } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        e[2 * i] = pack2(__uint_as_float(raw[i].x), __uint_as_float(raw[i].y));
-        e[2 * i + 1] = pack2(__uint_as_float(raw[i].z), __uint_as_float(raw[i].w));
-      }
+      for (int i = 0; i < 4; ++i) e[i] = pack2(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1]));
     } else {
-      unpack8(raw[0], e);
+      unpack8(make_uint4(raw[0], raw[1], raw[2], raw[3]), e);
     }
   }
 };
