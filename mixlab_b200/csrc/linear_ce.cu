@@ -121,11 +121,13 @@ __device__ __forceinline__ void pack_row(const T* from, bf16* to, size_t part_st
     for (int k = 0; k < PARTS; ++k) *reinterpret_cast<uint4*>(to + k * part_stride + c) = *reinterpret_cast<uint4*>(e[k]);
   }
 }
-// Blocks of eight rows, a warp each; 32 blocks behind them fill up the last tile of 256 rows with zeros.
+// Blocks of 32 rows, four a warp; 32 blocks of eight behind them fill up the last tile of 256 rows with zeros.
+constexpr int kPackRows = 32;
 template <typename T>
 __global__ void __launch_bounds__(256) lce_pack_kernel(PackP p, int row_blocks) {
   begin_dependent();
   __shared__ int32_t red[8];
+  __shared__ uint32_t counted;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if ((int)blockIdx.x >= row_blocks) {
     const int live = counted_before(p, p.N, red), k = ((int)blockIdx.x - row_blocks) * 8 + warp;
@@ -142,35 +144,40 @@ __global__ void __launch_bounds__(256) lce_pack_kernel(PackP p, int row_blocks) 
     }
     return;
   }
-  const size_t r0 = (size_t)blockIdx.x * 8, r = r0 + warp;
+  const size_t r0 = (size_t)blockIdx.x * kPackRows;
+  if (warp == 0) {
+    const uint32_t b = __ballot_sync(0xffffffffu, r0 + lane < p.N && counts(p, r0 + lane));
+    if (lane == 0) counted = b;
+  }
   const int before = counted_before(p, r0, red);
-  bool mine = r < p.N && counts(p, r);
-  __syncthreads();  // (the sum has been read)
-  if (lane == 0) red[warp] = mine;
-  __syncthreads();
-  if (r >= p.N) return;
-  if (!mine) {
-    if (p.d_loss) {
-      T* to = static_cast<T*>(p.dx) + r * p.D;
-      for (int c = lane; c < p.D; c += 32) to[c] = from_f32<T>(0.f);
-    } else if (lane == 0) {
-      p.loss[r] = p.lse_out[r] = 0.f;
+  const uint32_t mask = counted;
+#pragma unroll
+  for (int k = 0; k < kPackRows / 8; ++k) {
+    const int i = warp * (kPackRows / 8) + k;
+    const size_t r = r0 + i;
+    if (r >= p.N) return;
+    if (!(mask >> i & 1u)) {
+      if (p.d_loss) {
+        T* to = static_cast<T*>(p.dx) + r * p.D;
+        for (int c = lane; c < p.D; c += 32) to[c] = from_f32<T>(0.f);
+      } else if (lane == 0) {
+        p.loss[r] = p.lse_out[r] = 0.f;
+      }
+      continue;
     }
-    return;
-  }
-  size_t j = before;
-  for (int w = 0; w < warp; ++w) j += red[w];
-  if (lane == 0) {
-    p.idx[j] = (int32_t)r;
-    p.tgt[j] = target_of(p, r);
-    if (p.d_loss) {
-      const float a = p.d_loss[r];
-      p.a[j] = a;
-      p.both[j] = p.d_lse ? a + p.d_lse[r] : a;
-      p.lse2[j] = sizeof(T) == 4 ? p.lse[r] : p.lse[r] * kLog2e;
+    const size_t j = (size_t)before + __popc(mask & ((1u << i) - 1u));
+    if (lane == 0) {
+      p.idx[j] = (int32_t)r;
+      p.tgt[j] = target_of(p, r);
+      if (p.d_loss) {
+        const float a = p.d_loss[r];
+        p.a[j] = a;
+        p.both[j] = p.d_lse ? a + p.d_lse[r] : a;
+        p.lse2[j] = sizeof(T) == 4 ? p.lse[r] : p.lse[r] * kLog2e;
+      }
     }
+    pack_row<T>(static_cast<const T*>(p.x) + r * p.D, p.xc + j * p.Dp, p.pad * p.Dp, p.D, p.Dp, lane);
   }
-  pack_row<T>(static_cast<const T*>(p.x) + r * p.D, p.xc + j * p.Dp, p.pad * p.Dp, p.D, p.Dp, lane);
 }
 // Rows of a piece of W.
 template <typename T>
@@ -183,12 +190,14 @@ __global__ void __launch_bounds__(256) lce_pack_weight_kernel(const T* w, bf16* 
 // ------------------------------------------------------------------ the products
 enum Mode { kStats, kGrad, kDx, kDw };
 // A stage of the ring: PARTS tiles of A, 128 rows a CTA, and of B, BN / 2 rows a CTA, 64 deep.
-template <int MODE, bool F32>
+// BN, columns of a tile: 128 where two accumulators of float32 products lie side by side, or where all columns are that few.
+template <int MODE, bool F32, int BN_>
 struct Cfg {
-  static constexpr int BN = F32 ? 128 : 256, PARTS = F32 ? 3 : 1, COLS = BN / 2;  // COLS: of a thread of the epilogue
+  static constexpr int BN = BN_, PARTS = F32 ? 3 : 1, COLS = BN / 2;  // COLS: of a thread of the epilogue
   static constexpr int A = 128 * 128, B = BN / 2 * 128, STAGE = PARTS * (A + B);
   static constexpr int STAGES = F32 ? (MODE == kGrad ? 2 : 3) : 6;
-  static constexpr int STAGING = MODE == kGrad ? 8 * 4096 : 0;  // a box of 32 rows x 64 columns a warp
+  static constexpr bool BOXES = MODE == kGrad || (MODE == kDw && !F32);  // results leave in boxes of 32 rows x 64 columns a warp
+  static constexpr int STAGING = BOXES ? 8 * 4096 : 0;
   static constexpr bool A_MN = MODE == kDw, B_MN = MODE == kDx || MODE == kDw;
   static constexpr int SMEM = 1024 + STAGES * STAGE + STAGING + 256 + (MODE == kStats ? 128 + 4 * 128 * 8 : 0);
 };
@@ -198,7 +207,6 @@ struct GemmP {
   int32_t* status;
   int M, N, K;            // the extent that counts tokens is *live
   int b_row0;             // first row of B in its map (the vocabulary's piece)
-  int splits;             // of K
   int group;              // tiles of M that are walked through together
   int v0, V;              // first row of the vocabulary's piece, rows in all
   size_t pad;             // rows of what is indexed by token
@@ -206,9 +214,9 @@ struct GemmP {
   float* hit;             //   logit of the target
   const int32_t *tgt, *idx;
   const float *a, *both, *lse2;
-  float* sums;            // kDx, kDw: float32 [splits][rows][D], null: straight to out
+  float* sums;            // kDx: float32 sums of all pieces, by tiles (tile_at()), null: straight to out
   int adds;               //   to what is there
-  size_t sums_stride;
+  float* shares;          // kDx, kDw: tiles of which a pair has a share of K, two a pair
   void* out;              // rows by idx (kDx) or from v0 (kDw)
   int D, whole;           // whole: out's rows may be written in pieces of 16 bytes
 };
@@ -239,28 +247,63 @@ __device__ __forceinline__ void add_sum(float2& a, float2 b) {
   a.x = t;
 }
 
-// What all roles walk through: tiles of 256 x BN, group tiles of M at a time so that both operands' tiles stay in L2.
+// What all roles walk through: tiles of 256 x BN, group tiles of M at a time so that both operands' tiles stay in L2.  A pair takes
+// every pairs-th tile.  Where tiles stand for long sums (kDx, kDw) and the last round has fewer tiles than pairs, those are cut along K
+// into equal shares for all pairs, of one or two tiles each, and left as float32 shares that lce_shares_kernel adds up in order.
+// (Gradients of 28672 tokens, pieces of 8192 words: 448 and 128 tiles for 74 pairs; without the cut the last round of seven, or of
+// two, runs on a few of them.)
+struct Item {
+  int m, n, k0, k1;
+  int share;  // -1: the whole tile
+};
 struct Walk {
-  int m_tiles, n_tiles, kblocks, items;
-  __device__ __forceinline__ Walk(const GemmP& p, int mode, int BN) {
+  int m_tiles, n_tiles, kblocks, tiles, whole, rest, sharers, pairs, group;
+  __device__ __forceinline__ Walk(const GemmP& p, int mode, int BN, int pairs_) {
     const int live = *p.live;
     const int M = mode == kDw ? p.M : live, K = mode == kDw ? live : p.K;
+    pairs = pairs_;
+    group = p.group;
     m_tiles = (M + 255) / 256;
     n_tiles = (p.N + BN - 1) / BN;
     kblocks = (K + 63) / 64;
-    items = m_tiles * n_tiles * p.splits;
+    tiles = m_tiles * n_tiles;
+    rest = mode == kStats || mode == kGrad || kblocks < 16 ? 0 : tiles % pairs;
+    whole = tiles - rest;
+    sharers = (int)min((int64_t)pairs, (int64_t)rest * kblocks / 8);  // (at least two a tile)
   }
-  __device__ __forceinline__ void item(const GemmP& p, int i, int& m, int& n, int& split, int& k0, int& k1) const {
-    const int tiles = m_tiles * n_tiles;
-    split = i / tiles;
-    i -= split * tiles;
-    const int g = i / (p.group * n_tiles), rest = i - g * p.group * n_tiles, gm = min(p.group, m_tiles - g * p.group);
-    m = g * p.group + rest % gm;
-    n = rest / gm;
-    k0 = (int)((int64_t)kblocks * split / p.splits);
-    k1 = (int)((int64_t)kblocks * (split + 1) / p.splits);
+  __device__ __forceinline__ int64_t first_unit(int pair) const { return (int64_t)rest * kblocks * pair / sharers; }
+  __device__ __forceinline__ void place(int i, Item& t) const {
+    const int g = i / (group * n_tiles), in = i - g * group * n_tiles, gm = min(group, m_tiles - g * group);
+    t.m = g * group + in % gm;
+    t.n = in / gm;
+  }
+  // The pair's j-th item; false: there is none.
+  __device__ __forceinline__ bool item(int pair, int j, Item& t) const {
+    const int64_t i = (int64_t)j * pairs + pair;
+    if (i < whole) {
+      place((int)i, t);
+      t.k0 = 0;
+      t.k1 = kblocks;
+      t.share = -1;
+      return true;
+    }
+    if (pair >= sharers) return false;
+    const int64_t from = first_unit(pair), to = first_unit(pair + 1);
+    const int tile = (int)(from / kblocks), second = j - (whole + pairs - 1 - pair) / pairs;
+    const int64_t cut = (int64_t)(tile + 1) * kblocks;
+    if (second > 1 || (second == 1 && to <= cut)) return false;
+    place(whole + tile + second, t);
+    t.k0 = second ? 0 : (int)(from - (int64_t)tile * kblocks);
+    t.k1 = (int)((second ? to : min(to, cut)) - (int64_t)(tile + second) * kblocks);
+    t.share = pair * 2 + second;
+    return true;
   }
 };
+// Float32 tiles as the epilogue has them: element (row, c .. c + 3) of a CTA's 128 rows, 16 bytes of 32 rows side by side.
+template <int BN>
+__device__ __forceinline__ size_t tile_at(size_t tile, int rank, int row, int c) {
+  return ((tile * 2 + rank) * (BN / 4) + c / 4) * 512 + row * 4;
+}
 
 template <typename T>
 __device__ __forceinline__ void store_row(T* to, int c, int D, bool whole, const float* v) {  // 8 columns from c
@@ -279,9 +322,40 @@ __device__ __forceinline__ void store_row(T* to, int c, int D, bool whole, const
     if (c + i < D) to[c + i] = from_f32<T>(v[i]);
 }
 
-template <int MODE, bool F32>
+// A warp's 32 rows x COLS columns to a bf16 tensor in boxes of 64 columns, by its part of shared memory (128-byte swizzle); what a
+// bf16 leaves of a value goes to the next of PARTS.
+template <int COLS, int PARTS>
+__device__ __forceinline__ void leave_in_boxes(const void* map, uint8_t* box, float (&v)[COLS], int c0, int r0, int lane) {
+#pragma unroll
+  for (int x = 0; x < COLS / 64; ++x)
+#pragma unroll
+    for (int part = 0; part < PARTS; ++part) {
+      if (lane == 0) tc::bulk_wait_read<0>();
+      __syncwarp();
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        float* e = v + x * 64 + u * 8;
+        const uint4 w = tc::pack8(e);
+        *reinterpret_cast<uint4*>(box + lane * 128 + ((u ^ (lane & 7)) << 4)) = w;
+        if (part + 1 < PARTS) {
+          float lo[8];
+          tc::unpack8(w, lo);
+#pragma unroll
+          for (int y = 0; y < 8; ++y) e[y] -= lo[y];
+        }
+      }
+      tc::fence_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        tc::tma_store_3d(map, tc::smem_u32(box), c0 + x * 64, r0, part);
+        tc::bulk_commit();
+      }
+    }
+}
+
+template <int MODE, bool F32, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gemm_kernel(const GemmP p, const __grid_constant__ Maps maps) {
-  using C = Cfg<MODE, F32>;
+  using C = Cfg<MODE, F32, BN>;
   begin_dependent();
   extern __shared__ uint8_t raw[];
   const uint32_t base = (tc::smem_u32(raw) + 1023u) & ~1023u;
@@ -323,7 +397,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
   tc::cluster_sync();
   tc::fence_after_sync();
   const uint32_t tmem = *tmem_slot;
-  const Walk walk(p, MODE, C::BN);
+  const Walk walk(p, MODE, C::BN, pairs);
+  Item t;
   const Wait wait{bad};
   // blocks of K behind which an accumulator is handed over
   constexpr int SEG = F32 ? kSegment : 1 << 30;
@@ -334,17 +409,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
       int s = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int i = pair; ok && i < walk.items; i += pairs) {
-        int m, n, split, k0, k1;
-        walk.item(p, i, m, n, split, k0, k1);
-        for (int kb = k0; kb < k1; ++kb) {
+      for (int j = 0; ok && walk.item(pair, j, t); ++j) {
+        for (int kb = t.k0; kb < t.k1; ++kb) {
           if (!(ok = wait(empty + s, phase ^ 1u))) break;
           if (rank == 0) tc::mbar_expect_tx(full + s, 2 * C::STAGE);
           const uint32_t bar = tc::in_cta(tc::smem_u32(full + s), 0);
           uint32_t to = base + s * C::STAGE;
 #pragma unroll
           for (int part = 0; part < C::PARTS; ++part, to += C::A) {
-            const int m0 = m * 256 + (int)rank * 128;
+            const int m0 = t.m * 256 + (int)rank * 128;
             if (C::A_MN) {
               tc::tma_load_3d_pair(to, &maps.a, m0, kb * 64, part, bar);
               tc::tma_load_3d_pair(to + 8192, &maps.a, m0 + 64, kb * 64, part, bar);
@@ -354,7 +427,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
           }
 #pragma unroll
           for (int part = 0; part < C::PARTS; ++part, to += C::B) {
-            const int n0 = n * C::BN + (int)rank * (C::BN / 2);
+            const int n0 = t.n * C::BN + (int)rank * (C::BN / 2);
             if (C::B_MN) {
 #pragma unroll
               for (int x = 0; x < C::BN / 128; ++x) tc::tma_load_3d_pair(to + x * 8192, &maps.b, n0 + 64 * x, p.b_row0 + kb * 64, part, bar);
@@ -374,10 +447,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
       int s = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
-      for (int i = pair; ok && i < walk.items; i += pairs) {
-        int m, n, split, k0, k1;
-        walk.item(p, i, m, n, split, k0, k1);
-        for (int ks = k0; ok && ks < k1; ks += SEG) {
+      for (int j = 0; ok && walk.item(pair, j, t); ++j) {
+        const int k1 = t.k1;
+        for (int ks = t.k0; ok && ks < k1; ks += SEG) {
           if (!(ok = wait(acc_empty + acc, acc_phase ^ 1u))) break;
           tc::fence_after_sync();
           const uint32_t d = tmem + acc * 256;
@@ -418,9 +490,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
-    for (int i = pair; ok && i < walk.items; i += pairs) {
-      int m, n, split, k0, k1;
-      walk.item(p, i, m, n, split, k0, k1);
+    for (int j = 0; ok && walk.item(pair, j, t); ++j) {
+      const int m = t.m, n = t.n, k0 = t.k0, k1 = t.k1;
       float v[C::COLS];
       if (k0 == k1 || F32)
 #pragma unroll
@@ -481,7 +552,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
             for (int c = 0; c < C::COLS; ++c) z = c == at ? v[c] : z;
             if (hit && row < live) p.hit[row] = z;
           }
-          const int turn = i / pairs, slot = turn & 3;
+          const int slot = j & 3;
           float2* buf = halves + slot * 128;
           uint64_t* there = halves_full + slot * 4 + quarter;
           if (half == 1) {
@@ -489,7 +560,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(there);
           } else {
-            if (!(ok = wait(there, (uint32_t)(turn >> 2) & 1u))) break;
+            if (!(ok = wait(there, (uint32_t)(j >> 2) & 1u))) break;
             const float2 o = buf[mine];
             if (row < live) {
               float2 both{shift, sum};
@@ -510,69 +581,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
 #pragma unroll
             for (int c = 0; c < C::COLS; ++c) v[c] = c == at ? v[c] - a : v[c];
           }
-          // to the workspace in boxes of 32 rows x 64 columns, by this warp's part of shared memory (128-byte swizzle)
-          uint8_t* box = staging + warp * 4096;
-          const int r0 = m * 256 + (int)rank * 128 + quarter * 32;
-#pragma unroll
-          for (int x = 0; x < C::COLS / 64; ++x)
-#pragma unroll
-            for (int part = 0; part < C::PARTS; ++part) {
-              if (lane == 0) tc::bulk_wait_read<0>();
-              __syncwarp();
-#pragma unroll
-              for (int u = 0; u < 8; ++u) {
-                float* e = v + x * 64 + u * 8;
-                const uint4 w = tc::pack8(e);
-                *reinterpret_cast<uint4*>(box + lane * 128 + ((u ^ (lane & 7)) << 4)) = w;
-                if (part + 1 < C::PARTS) {
-                  float lo[8];
-                  tc::unpack8(w, lo);
-#pragma unroll
-                  for (int y = 0; y < 8; ++y) e[y] -= lo[y];
-                }
-              }
-              tc::fence_async_smem();
-              __syncwarp();
-              if (lane == 0) {
-                tc::tma_store_3d(&maps.g, tc::smem_u32(box), c0 + x * 64, r0, part);
-                tc::bulk_commit();
-              }
-            }
+          leave_in_boxes<C::COLS, C::PARTS>(&maps.g, staging + warp * 4096, v, c0, m * 256 + (int)rank * 128 + quarter * 32, lane);
         }
-      } else {
-        const bool in = row < (MODE == kDx ? live : p.M);
-        if (in) {
-          if (p.sums) {
-            float* to = p.sums + split * p.sums_stride + (size_t)row * p.D;
-            const bool four = p.D % 4 == 0;
+      } else if (t.share >= 0 || (MODE == kDx && p.sums)) {
+        const bool add = t.share < 0 && p.adds;
+        float* to = (t.share >= 0 ? p.shares : p.sums) +
+                    tile_at<C::BN>(t.share >= 0 ? (size_t)t.share : (size_t)m * walk.n_tiles + n, rank, mine, half * C::COLS);
 #pragma unroll
-            for (int c = 0; c < C::COLS; c += 4) {
-              const int col = c0 + c;
-              if (four) {
-                if (col < p.D) {
-                  float4 o = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
-                  if (p.adds) {
-                    const float4 old = *reinterpret_cast<const float4*>(to + col);
-                    o.x += old.x; o.y += old.y; o.z += old.z; o.w += old.w;
-                  }
-                  *reinterpret_cast<float4*>(to + col) = o;
-                }
-              } else {
+        for (int c = 0; c < C::COLS; c += 32) {
+          float4 old[8];
 #pragma unroll
-                for (int x = 0; x < 4; ++x)
-                  if (col + x < p.D) to[col + x] = p.adds ? to[col + x] + v[c + x] : v[c + x];
-              }
-            }
-          } else {
-            using T = std::conditional_t<F32, float, bf16>;
-            T* to = static_cast<T*>(p.out) + (MODE == kDx ? (size_t)p.idx[row] : (size_t)p.v0 + row) * p.D;
+          for (int x = 0; x < 8; ++x) old[x] = add ? *reinterpret_cast<const float4*>(to + (c / 4 + x) * 512) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int c = 0; c < C::COLS; c += 8) store_row<T>(to, c0 + c, p.D, p.whole, v + c);
+          for (int x = 0; x < 8; ++x) {
+            const float* e = v + c + 4 * x;
+            *reinterpret_cast<float4*>(to + (c / 4 + x) * 512) = make_float4(old[x].x + e[0], old[x].y + e[1], old[x].z + e[2], old[x].w + e[3]);
           }
         }
+      } else if (C::BOXES && p.whole) {
+        leave_in_boxes<C::COLS, 1>(&maps.g, staging + warp * 4096, v, c0, p.v0 + m * 256 + (int)rank * 128 + quarter * 32, lane);
+      } else if (row < (MODE == kDx ? live : p.M)) {
+        using T = std::conditional_t<F32, float, bf16>;
+        T* to = static_cast<T*>(p.out) + (MODE == kDx ? (size_t)p.idx[row] : (size_t)p.v0 + row) * p.D;
+#pragma unroll
+        for (int c = 0; c < C::COLS; c += 8) store_row<T>(to, c0 + c, p.D, p.whole, v + c);
       }
     }
-    if (MODE == kGrad && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if (C::BOXES && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   __syncwarp();
   __syncthreads();
@@ -611,25 +646,82 @@ __global__ void __launch_bounds__(256) lce_join_kernel(JoinP p) {
   p.lse[to] = lse;
   p.loss[to] = lse - p.hit[row];
 }
-// Rows of float32 sums over the splits, in order, to their places in the tensor's type.
-struct FinishP {
-  const float* sums;
-  const int32_t *live, *idx;  // idx null: rows from row0, all of them
-  void* out;
-  size_t stride, row0;
-  int rows, D, splits;
-};
-template <typename T>
-__global__ void __launch_bounds__(256) lce_finish_kernel(FinishP p) {
+// Tiles that were cut along K: their shares in order.  grid (at most pairs - 1 tiles, 2 CTAs' rows x pieces of 64 columns).
+template <int MODE, bool F32, int BN>
+__global__ void __launch_bounds__(256) lce_shares_kernel(const GemmP p, int pairs) {
+  using C = Cfg<MODE, F32, BN>;
+  using T = std::conditional_t<F32, float, bf16>;
   begin_dependent();
-  const int rows = p.idx ? *p.live : p.rows;
-  for (int r = blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.x * 8) {
-    T* to = static_cast<T*>(p.out) + (p.idx ? (size_t)p.idx[r] : p.row0 + r) * p.D;
-    const float* from = p.sums + (size_t)r * p.D;
-    for (int c = threadIdx.x & 31; c < p.D; c += 32) {
-      float s = from[c];
-      for (int k = 1; k < p.splits; ++k) s += from[k * p.stride + c];
-      to[c] = from_f32<T>(s);
+  const Walk walk(p, MODE, C::BN, pairs);
+  const int tile = blockIdx.x;
+  if (tile >= walk.rest) return;
+  Item t;
+  walk.place(walk.whole + tile, t);
+  const int rank = blockIdx.y & 1, mine = threadIdx.x & 127, c0 = (blockIdx.y >> 1) * 64 + (threadIdx.x >> 7) * 32;
+  // the pairs that have a unit of it: from the last that begins at or before its first unit on
+  const int64_t from = (int64_t)tile * walk.kblocks, to = from + walk.kblocks, all = (int64_t)walk.rest * walk.kblocks;
+  int pair = (int)(from * walk.sharers / all);
+  while (pair > 0 && walk.first_unit(pair) > from) --pair;
+  while (walk.first_unit(pair + 1) <= from) ++pair;
+  float v[32];
+#pragma unroll
+  for (int c = 0; c < 32; ++c) v[c] = 0.f;
+  for (; pair < walk.sharers && walk.first_unit(pair) < to; ++pair) {
+    const int second = (int)(walk.first_unit(pair) / walk.kblocks) != tile;
+    const float* e = p.shares + tile_at<C::BN>((size_t)pair * 2 + second, rank, mine, c0);
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const float4 o = *reinterpret_cast<const float4*>(e + x * 512);
+      v[4 * x] += o.x; v[4 * x + 1] += o.y; v[4 * x + 2] += o.z; v[4 * x + 3] += o.w;
+    }
+  }
+  if (MODE == kDx && p.sums) {
+    float* e = p.sums + tile_at<C::BN>((size_t)t.m * walk.n_tiles + t.n, rank, mine, c0);
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      float4 o = make_float4(v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]);
+      if (p.adds) {
+        const float4 old = *reinterpret_cast<const float4*>(e + x * 512);
+        o.x += old.x; o.y += old.y; o.z += old.z; o.w += old.w;
+      }
+      *reinterpret_cast<float4*>(e + x * 512) = o;
+    }
+    return;
+  }
+  const int row = t.m * 256 + rank * 128 + mine;
+  if (row >= (MODE == kDx ? *p.live : p.M)) return;
+  T* out = static_cast<T*>(p.out) + (MODE == kDx ? (size_t)p.idx[row] : (size_t)p.v0 + row) * p.D;
+#pragma unroll
+  for (int c = 0; c < 32; c += 8) store_row<T>(out, t.n * C::BN + c0 + c, p.D, p.whole, v + c);
+}
+// dx from its sums by tiles, in the tensor's type.  grid (128 rows, pieces of 64 columns).
+template <bool F32, int BN>
+__global__ void __launch_bounds__(256) lce_finish_kernel(const GemmP p, int n_tiles) {
+  using T = std::conditional_t<F32, float, bf16>;
+  begin_dependent();
+  __shared__ float box[128][65];
+  const int m0 = blockIdx.x * 128, col = blockIdx.y * 64, live = *p.live;
+  if (m0 >= live) return;
+  const float* from = p.sums + tile_at<BN>((size_t)(blockIdx.x >> 1) * n_tiles + col / BN, blockIdx.x & 1, threadIdx.x & 127, col % BN);
+#pragma unroll
+  for (int x = 0; x < 8; ++x) {
+    const int c4 = x * 2 + (threadIdx.x >> 7);
+    const float4 v = *reinterpret_cast<const float4*>(from + c4 * 512);
+    float* to = &box[threadIdx.x & 127][c4 * 4];
+    to[0] = v.x; to[1] = v.y; to[2] = v.z; to[3] = v.w;
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  for (int r = threadIdx.x >> 5; r < 128 && m0 + r < live; r += 8) {
+    T* to = static_cast<T*>(p.out) + (size_t)p.idx[m0 + r] * p.D + col;
+    if (p.whole) {  // two columns a lane
+      if (col + 2 * lane >= p.D) continue;
+      if constexpr (F32) *reinterpret_cast<float2*>(to + 2 * lane) = make_float2(box[r][2 * lane], box[r][2 * lane + 1]);
+      else *reinterpret_cast<uint32_t*>(to + 2 * lane) = tc::pack_bf16(box[r][2 * lane], box[r][2 * lane + 1]);
+    } else {
+#pragma unroll
+      for (int c = lane; c < 64; c += 32)
+        if (col + c < p.D) to[c] = from_f32<T>(box[r][c]);
     }
   }
 }
@@ -659,26 +751,23 @@ constexpr size_t kPackBytes = (size_t)256 << 20;
 
 struct Plan {
   bool f32, pack_w;
-  int parts, Dp, piece, pieces, BN;
+  int parts, Dp, piece, pieces;
+  int BN, BD;  // columns of a tile: of logits, of gradients
   size_t N, pad;
-  int dx_splits, dw_splits;
-  bool dx_sums;
   // workspace
   int32_t *status, *live, *counts, *idx, *tgt;
-  float *a, *both, *lse2, *hit, *dx_part, *dw_part;
+  float *a, *both, *lse2, *hit, *sums, *shares;
   float2* part;
   bf16 *xc, *wc, *g;
   size_t bytes;
 };
-static int splits_of(int64_t tiles, int64_t kblocks) {
-  return (int)std::max<int64_t>(1, std::min<int64_t>(kPairs / std::max<int64_t>(tiles, 1), kblocks / 8));
-}
 // bwd: the backward pass.  weight only says whether it can be read as it is.
 static Plan plan(const mxb_linear_ce_desc* d, const void* weight, bool bwd, void* base) {
   Plan q{};
   q.f32 = d->io_dtype == MXB_F32;
   q.parts = q.f32 ? 3 : 1;
   q.BN = q.f32 ? 128 : 256;
+  q.BD = q.f32 || d->D <= 128 ? 128 : 256;
   q.Dp = (d->D + 7) / 8 * 8;
   q.N = d->rows;
   q.pad = std::max<size_t>((q.N + 255) / 256 * 256, 256);
@@ -690,10 +779,7 @@ static Plan plan(const mxb_linear_ce_desc* d, const void* weight, bool bwd, void
   q.piece = (int)std::min<int64_t>(all, std::max<int64_t>(256, most / 256 * 256));
   if (!bwd && !q.pack_w) q.piece = (int)all;
   q.pieces = (int)((d->V + (int64_t)q.piece - 1) / q.piece);
-  const int64_t m_tiles = q.pad / 256, d_tiles = (d->D + q.BN - 1) / q.BN;
-  q.dx_splits = splits_of(m_tiles * d_tiles, q.piece / 64);
-  q.dx_sums = q.pieces > 1 || q.dx_splits > 1;
-  q.dw_splits = splits_of(q.piece / 256 * d_tiles, (int64_t)((q.N + 63) / 64));
+  const int64_t m_tiles = q.pad / 256, d_tiles = (d->D + q.BD - 1) / q.BD;
   Carver c(base);
   q.status = c.take<int32_t>(64);  // (the device's error word leads the workspace)
   q.live = c.take<int32_t>(1);
@@ -711,40 +797,48 @@ static Plan plan(const mxb_linear_ce_desc* d, const void* weight, bool bwd, void
     q.both = c.take<float>(q.pad);
     q.lse2 = c.take<float>(q.pad);
     q.g = c.take<bf16>((size_t)q.parts * q.pad * q.piece);
-    if (q.dx_sums) q.dx_part = c.take<float>((size_t)q.dx_splits * q.pad * d->D);
-    if (q.dw_splits > 1) q.dw_part = c.take<float>((size_t)q.dw_splits * q.piece * d->D);
+    if (q.pieces > 1) q.sums = c.take<float>((size_t)m_tiles * d_tiles * 256 * q.BD);
+    q.shares = c.take<float>((size_t)kPairs * 2 * 256 * q.BD);
   }
   q.bytes = c.bytes();
   return q;
 }
 
-template <int MODE, bool F32>
-static mxb_status launch_gemm(const GemmP& p, const Maps& maps, int64_t items, cudaStream_t st) {
-  using C = Cfg<MODE, F32>;
-  if (MXB_ALLOW_SMEM(C::SMEM, lce_gemm_kernel<MODE, F32>) != MXB_OK) return MXB_ERR_CUDA;
+// tiles, and blocks of 64 of K, at most (the tokens that count may be fewer)
+template <int MODE, bool F32, int BN>
+static mxb_status launch_gemm(const GemmP& p, const Maps& maps, int64_t tiles, int64_t kblocks, cudaStream_t st) {
+  using C = Cfg<MODE, F32, BN>;
+  if (MXB_ALLOW_SMEM(C::SMEM, lce_gemm_kernel<MODE, F32, BN>) != MXB_OK) return MXB_ERR_CUDA;
   static const char* const names[] = {"lce_stats_kernel", "lce_grad_kernel", "lce_dx_kernel", "lce_dw_kernel"};
-  const unsigned ctas = 2 * (unsigned)std::min<int64_t>(items, kPairs);
-  MXB_LAUNCH(names[MODE], st, (launch_kernel(lce_gemm_kernel<MODE, F32>, ctas, kThreads, C::SMEM, st, p, maps)));
+  constexpr bool cut = MODE == kDx || MODE == kDw;
+  const int pairs = (int)std::min<int64_t>(cut && kblocks >= 16 ? std::max<int64_t>(tiles, tiles * kblocks / 8) : tiles, kPairs);
+  MXB_LAUNCH(names[MODE], st, (launch_kernel(lce_gemm_kernel<MODE, F32, BN>, 2 * pairs, kThreads, C::SMEM, st, p, maps)));
+  if constexpr (cut)
+    if (kblocks >= 16 && pairs > 1)
+      MXB_LAUNCH("lce_shares_kernel", st,
+                 (launch_kernel(lce_shares_kernel<MODE, F32, BN>, dim3((unsigned)std::min<int64_t>(tiles, pairs - 1), 2 * C::BN / 64), 256, 0, st, p, pairs)));
   return check_launch(names[MODE]);
 }
 template <typename T>
 static mxb_status pack(const mxb_linear_ce_desc* d, PackP& p, cudaStream_t st) {
   if (p.N >= kCountRows)
     MXB_LAUNCH("lce_count_kernel", st, (launch_kernel(lce_count_kernel, (unsigned)(p.N / kCountRows), 256, 0, st, p, const_cast<int32_t*>(p.counts))));
-  const int blocks = (int)((p.N + 7) / 8);
+  const int blocks = (int)((p.N + kPackRows - 1) / kPackRows);
   MXB_LAUNCH("lce_pack_kernel", st, (launch_kernel(lce_pack_kernel<T>, blocks + 32, 256, 0, st, p, blocks)));
   return check_launch("lce_pack_kernel");
 }
 
-template <bool F32>
+template <bool F32, int BD>
 static mxb_status run(const mxb_linear_ce_desc* d, const Plan& q, PackP& pk, const void* weight, void* dweight, cudaStream_t st) {
   using T = std::conditional_t<F32, float, bf16>;
   const bool bwd = pk.d_loss != nullptr;
   mxb_status s = pack<T>(d, pk, st);
   if (s != MXB_OK) return s;
   const size_t pad = q.pad;
-  const int D = d->D, BN = q.BN;
-  const int64_t m_tiles = pad / 256, d_tiles = (D + BN - 1) / BN;
+  const int D = d->D;
+  constexpr int BN = F32 ? 128 : 256;
+  GemmP last{};  // of the last piece's dx
+  const int64_t m_tiles = pad / 256, d_tiles = (D + BD - 1) / BD;
   for (int piece = 0; piece < q.pieces; ++piece) {
     const int v0 = piece * q.piece, rows = (int)std::min<int64_t>(q.piece, (int64_t)d->V - v0);
     const void* w = weight;
@@ -768,7 +862,6 @@ static mxb_status run(const mxb_linear_ce_desc* d, const Plan& q, PackP& pk, con
     p.V = d->V;
     p.pad = pad;
     p.D = D;
-    p.splits = 1;
     p.group = 8;
     Maps maps;
     std::memset(&maps, 0, sizeof maps);
@@ -784,7 +877,7 @@ static mxb_status run(const mxb_linear_ce_desc* d, const Plan& q, PackP& pk, con
     p.both = q.both;
     p.lse2 = q.lse2;
     const int64_t tiles = m_tiles * ((rows + BN - 1) / BN);
-    s = bwd ? launch_gemm<kGrad, F32>(p, maps, tiles, st) : launch_gemm<kStats, F32>(p, maps, tiles, st);
+    s = bwd ? launch_gemm<kGrad, F32, BN>(p, maps, tiles, 0, st) : launch_gemm<kStats, F32, BN>(p, maps, tiles, 0, st);
     if (s != MXB_OK) return s;
     if (bwd) {
       // dx: sums over the piece, in the order of the pieces
@@ -792,46 +885,44 @@ static mxb_status run(const mxb_linear_ce_desc* d, const Plan& q, PackP& pk, con
       x.N = D;
       x.K = rows;
       x.b_row0 = w_row0;
-      x.splits = q.dx_splits;
-      x.sums = q.dx_part;
-      x.sums_stride = pad * D;
+      x.sums = q.sums;
+      x.shares = q.shares;
       x.adds = piece > 0;
       x.out = pk.dx;
       x.whole = D % 8 == 0 && (reinterpret_cast<uintptr_t>(pk.dx) & 15) == 0;
       if (!make_map(&maps.a, q.g, q.piece, pad, q.parts, q.piece, pad * q.piece, 128) || !make_map(&maps.b, w, q.Dp, w_rows, q.parts, q.Dp, w_part, 64))
         return MXB_ERR_UNSUPPORTED;
-      s = launch_gemm<kDx, F32>(x, maps, m_tiles * d_tiles * q.dx_splits, st);
+      s = launch_gemm<kDx, F32, BD>(x, maps, m_tiles * d_tiles, (rows + 63) / 64, st);
       if (s != MXB_OK) return s;
+      last = x;
       // dW: sums over the tokens
       GemmP y = p;
       y.M = rows;
       y.N = D;
       y.b_row0 = 0;
-      y.splits = q.dw_splits;
-      y.sums = q.dw_part;
-      y.sums_stride = (size_t)q.piece * D;
+      y.shares = q.shares;
       y.out = dweight;
       y.whole = D % 8 == 0 && (reinterpret_cast<uintptr_t>(dweight) & 15) == 0;
       if (!make_map(&maps.a, q.g, q.piece, pad, q.parts, q.piece, pad * q.piece, 64) || !make_map(&maps.b, q.xc, q.Dp, pad, q.parts, q.Dp, pad * q.Dp, 64))
         return MXB_ERR_UNSUPPORTED;
-      s = launch_gemm<kDw, F32>(y, maps, (int64_t)((rows + 255) / 256) * d_tiles * q.dw_splits, st);
+      if (!F32 && y.whole && !make_map(&maps.g, dweight, D, d->V, 1, D, (uint64_t)d->V * D, 32)) return MXB_ERR_UNSUPPORTED;
+      s = launch_gemm<kDw, F32, BD>(y, maps, (int64_t)((rows + 255) / 256) * d_tiles, (int64_t)((q.N + 63) / 64), st);
       if (s != MXB_OK) return s;
-      if (q.dw_part) {
-        const FinishP f{q.dw_part, q.live, nullptr, dweight, y.sums_stride, (size_t)v0, rows, D, q.dw_splits};
-        MXB_LAUNCH("lce_finish_kernel", st, (launch_kernel(lce_finish_kernel<T>, (unsigned)std::min<int64_t>((rows + 7) / 8, 148 * 8), 256, 0, st, f)));
-      }
     }
   }
   if (bwd) {
-    if (q.dx_part) {
-      const FinishP f{q.dx_part, q.live, q.idx, pk.dx, pad * D, 0, 0, D, q.dx_splits};
-      MXB_LAUNCH("lce_finish_kernel", st, (launch_kernel(lce_finish_kernel<T>, (unsigned)std::min<int64_t>((pad + 7) / 8, 148 * 8), 256, 0, st, f)));
-    }
+    if (q.sums)
+      MXB_LAUNCH("lce_finish_kernel", st,
+                 (launch_kernel(lce_finish_kernel<F32, BD>, dim3((unsigned)(pad / 128), (unsigned)((D + 63) / 64)), 256, 0, st, last, (int)d_tiles)));
     return check_launch("linear_ce_bwd");
   }
   const JoinP j{q.part, q.hit, q.live, q.idx, pk.loss, pk.lse_out, pad, (d->V + BN - 1) / BN};
   MXB_LAUNCH("lce_join_kernel", st, (launch_kernel(lce_join_kernel, (unsigned)(pad / 32), 256, 0, st, j)));
   return check_launch("linear_ce_fwd");
+}
+static mxb_status by_shape(const mxb_linear_ce_desc* d, const Plan& q, PackP& p, const void* weight, void* dweight, cudaStream_t st) {
+  if (q.f32) return run<true, 128>(d, q, p, weight, dweight, st);
+  return q.BD == 128 ? run<false, 128>(d, q, p, weight, dweight, st) : run<false, 256>(d, q, p, weight, dweight, st);
 }
 static PackP pack_args(const mxb_linear_ce_desc* d, const Plan& q, const void* x, const void* targets) {
   PackP p{};
@@ -866,7 +957,7 @@ mxb_status linear_ce_fwd(const mxb_linear_ce_desc* d, const void* x, const void*
   lce::PackP p = lce::pack_args(d, q, x, targets);
   p.loss = loss;
   p.lse_out = lse;
-  return q.f32 ? lce::run<true>(d, q, p, weight, nullptr, st) : lce::run<false>(d, q, p, weight, nullptr, st);
+  return lce::by_shape(d, q, p, weight, nullptr, st);
 }
 mxb_status linear_ce_bwd(const mxb_linear_ce_desc* d, const void* x, const void* weight, const void* targets, const float* lse, const float* d_loss,
                          const float* d_lse, void* dx, void* dweight, void* workspace, cudaStream_t st) {
@@ -876,7 +967,7 @@ mxb_status linear_ce_bwd(const mxb_linear_ce_desc* d, const void* x, const void*
   p.d_loss = d_loss;
   p.d_lse = d_lse;
   p.dx = dx;
-  return q.f32 ? lce::run<true>(d, q, p, weight, dweight, st) : lce::run<false>(d, q, p, weight, dweight, st);
+  return lce::by_shape(d, q, p, weight, dweight, st);
 }
 
 }  // namespace mxb
