@@ -15,6 +15,7 @@
 
 #include <algorithm>
 #include <cstring>
+#include <numeric>
 #include <type_traits>
 
 #include "common.cuh"
@@ -41,11 +42,19 @@ struct PackP {
   float *loss, *lse_out;              // forward: likewise
   int32_t* status;
   size_t N, pad;
-  int V, D, Dp, wide, f32;            // wide: targets of 64 bits
+  int V, D, Dp, wide;                 // wide: targets of 64 bits
+  int each;                           // rows of a warp of the pack kernel
+  const void* w;                      // first rows of W to pack in the same launch (w_rows; 0: none)
+  bf16* wc;
+  size_t w_pad;
+  int w_rows;
 };
+__device__ __forceinline__ int target_at(const void* targets, int wide, int V, size_t t) {  // -1: none
+  const int64_t v = wide ? static_cast<const int64_t*>(targets)[t] : static_cast<const int32_t*>(targets)[t];
+  return v >= 0 && v < V ? (int)v : -1;
+}
 __device__ __forceinline__ int target_of(const PackP& p, size_t t) {  // -1: none
-  const int64_t v = p.wide ? static_cast<const int64_t*>(p.targets)[t] : static_cast<const int32_t*>(p.targets)[t];
-  return v >= 0 && v < p.V ? (int)v : -1;
+  return target_at(p.targets, p.wide, p.V, t);
 }
 __device__ __forceinline__ bool counts(const PackP& p, size_t t) {
   if (target_of(p, t) < 0) return false;
@@ -64,7 +73,7 @@ __device__ __forceinline__ int block_sum(int v, int32_t* red) {  // 256 threads
 }
 // How many of the tokens in front of t count.
 __device__ __forceinline__ int counted_before(const PackP& p, size_t t, int32_t* red) {
-  const size_t blocks = t / kCountRows;
+  const size_t blocks = p.counts ? t / kCountRows : 0;
   int n = 0;
   for (size_t b = threadIdx.x; b < blocks; b += 256) n += p.counts[b];
   for (size_t i = blocks * kCountRows + threadIdx.x; i < t; i += 256) n += counts(p, i);
@@ -121,8 +130,8 @@ __device__ __forceinline__ void pack_row(const T* from, bf16* to, size_t part_st
     for (int k = 0; k < PARTS; ++k) *reinterpret_cast<uint4*>(to + k * part_stride + c) = *reinterpret_cast<uint4*>(e[k]);
   }
 }
-// Blocks of 32 rows, four a warp; 32 blocks of eight behind them fill up the last tile of 256 rows with zeros.
-constexpr int kPackRows = 32;
+// Blocks of eight warps with p.each rows each; 32 blocks behind them fill up the last tile of 256 rows with zeros, those behind them
+// pack rows of W.
 template <typename T>
 __global__ void __launch_bounds__(256) lce_pack_kernel(PackP p, int row_blocks) {
   begin_dependent();
@@ -130,6 +139,11 @@ __global__ void __launch_bounds__(256) lce_pack_kernel(PackP p, int row_blocks) 
   __shared__ uint32_t counted;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if ((int)blockIdx.x >= row_blocks) {
+    if ((int)blockIdx.x >= row_blocks + 32) {
+      const int r = ((int)blockIdx.x - row_blocks - 32) * 8 + warp;
+      if (r < p.w_rows) pack_row<T>(static_cast<const T*>(p.w) + (size_t)r * p.D, p.wc + (size_t)r * p.Dp, p.w_pad * p.Dp, p.D, p.Dp, lane);
+      return;
+    }
     const int live = counted_before(p, p.N, red), k = ((int)blockIdx.x - row_blocks) * 8 + warp;
     const size_t j = (size_t)live + k;
     if (blockIdx.x == row_blocks && threadIdx.x == 0) {
@@ -144,16 +158,15 @@ __global__ void __launch_bounds__(256) lce_pack_kernel(PackP p, int row_blocks) 
     }
     return;
   }
-  const size_t r0 = (size_t)blockIdx.x * kPackRows;
+  const size_t r0 = (size_t)blockIdx.x * 8 * p.each;
   if (warp == 0) {
-    const uint32_t b = __ballot_sync(0xffffffffu, r0 + lane < p.N && counts(p, r0 + lane));
+    const uint32_t b = __ballot_sync(0xffffffffu, lane < 8 * p.each && r0 + lane < p.N && counts(p, r0 + lane));
     if (lane == 0) counted = b;
   }
   const int before = counted_before(p, r0, red);
   const uint32_t mask = counted;
-#pragma unroll
-  for (int k = 0; k < kPackRows / 8; ++k) {
-    const int i = warp * (kPackRows / 8) + k;
+  for (int k = 0; k < p.each; ++k) {
+    const int i = warp * p.each + k;
     const size_t r = r0 + i;
     if (r >= p.N) return;
     if (!(mask >> i & 1u)) {
@@ -195,21 +208,27 @@ template <int MODE, bool F32, int BN_>
 struct Cfg {
   static constexpr int BN = BN_, PARTS = F32 ? 3 : 1, COLS = BN / 2;  // COLS: of a thread of the epilogue
   static constexpr int A = 128 * 128, B = BN / 2 * 128, STAGE = PARTS * (A + B);
-  static constexpr int STAGES = F32 ? (MODE == kGrad ? 2 : 3) : 6;
-  static constexpr bool BOXES = MODE == kGrad || (MODE == kDw && !F32);  // results leave in boxes of 32 rows x 64 columns a warp
+  static constexpr int STAGES = F32 ? 3 : 6;
+  // results leave in boxes of 32 rows x 64 columns a warp (float32: shared memory is better spent on a third stage)
+  static constexpr bool BOXES = (MODE == kGrad || MODE == kDw) && !F32;
   static constexpr int STAGING = BOXES ? 8 * 4096 : 0;
   static constexpr bool A_MN = MODE == kDw, B_MN = MODE == kDx || MODE == kDw;
   static constexpr int SMEM = 1024 + STAGES * STAGE + STAGING + 256 + (MODE == kStats ? 128 + 4 * 128 * 8 : 0);
 };
 constexpr int kThreads = 320, kSegment = 4;  // blocks of 64 that a float32 accumulator takes before it is added up in registers
 struct GemmP {
-  const int32_t* live;
+  const int32_t* live;    // null: rows tokens, none left out
+  const void* targets;    //   their targets (wide: of 64 bits)
+  int32_t* flags;         //   what *status gets, by blocks
+  int rows, wide;
   int32_t* status;
   int M, N, K;            // the extent that counts tokens is *live
   int b_row0;             // first row of B in its map (the vocabulary's piece)
   int group;              // tiles of M that are walked through together
   int v0, V;              // first row of the vocabulary's piece, rows in all
+  bf16* g;
   size_t pad;             // rows of what is indexed by token
+  int piece;              // columns of g
   float2* part;           // kStats: [tiles of the vocabulary][pad] maximum and sum
   float* hit;             //   logit of the target
   const int32_t *tgt, *idx;
@@ -221,6 +240,7 @@ struct GemmP {
   int D, whole;           // whole: out's rows may be written in pieces of 16 bytes
 };
 struct Maps { CUtensorMap a, b, g; };
+__device__ __forceinline__ int live_of(const GemmP& p) { return p.live ? *p.live : p.rows; }
 
 // A wait that gives up: on its own limit, or when another role of the CTA has.
 struct Wait {
@@ -259,7 +279,7 @@ struct Item {
 struct Walk {
   int m_tiles, n_tiles, kblocks, tiles, whole, rest, sharers, pairs, group;
   __device__ __forceinline__ Walk(const GemmP& p, int mode, int BN, int pairs_) {
-    const int live = *p.live;
+    const int live = live_of(p);
     const int M = mode == kDw ? p.M : live, K = mode == kDw ? live : p.K;
     pairs = pairs_;
     group = p.group;
@@ -322,35 +342,22 @@ __device__ __forceinline__ void store_row(T* to, int c, int D, bool whole, const
     if (c + i < D) to[c + i] = from_f32<T>(v[i]);
 }
 
-// A warp's 32 rows x COLS columns to a bf16 tensor in boxes of 64 columns, by its part of shared memory (128-byte swizzle); what a
-// bf16 leaves of a value goes to the next of PARTS.
-template <int COLS, int PARTS>
-__device__ __forceinline__ void leave_in_boxes(const void* map, uint8_t* box, float (&v)[COLS], int c0, int r0, int lane) {
+// A warp's 32 rows x COLS columns to a bf16 tensor in boxes of 64 columns, by its part of shared memory (128-byte swizzle).
+template <int COLS>
+__device__ __forceinline__ void leave_in_boxes(const void* map, uint8_t* box, const float (&v)[COLS], int c0, int r0, int lane) {
 #pragma unroll
-  for (int x = 0; x < COLS / 64; ++x)
+  for (int x = 0; x < COLS / 64; ++x) {
+    if (lane == 0) tc::bulk_wait_read<0>();
+    __syncwarp();
 #pragma unroll
-    for (int part = 0; part < PARTS; ++part) {
-      if (lane == 0) tc::bulk_wait_read<0>();
-      __syncwarp();
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        float* e = v + x * 64 + u * 8;
-        const uint4 w = tc::pack8(e);
-        *reinterpret_cast<uint4*>(box + lane * 128 + ((u ^ (lane & 7)) << 4)) = w;
-        if (part + 1 < PARTS) {
-          float lo[8];
-          tc::unpack8(w, lo);
-#pragma unroll
-          for (int y = 0; y < 8; ++y) e[y] -= lo[y];
-        }
-      }
-      tc::fence_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        tc::tma_store_3d(map, tc::smem_u32(box), c0 + x * 64, r0, part);
-        tc::bulk_commit();
-      }
+    for (int u = 0; u < 8; ++u) *reinterpret_cast<uint4*>(box + lane * 128 + ((u ^ (lane & 7)) << 4)) = tc::pack8(v + x * 64 + u * 8);
+    tc::fence_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tc::tma_store_3d(map, tc::smem_u32(box), c0 + x * 64, r0, 0);
+      tc::bulk_commit();
     }
+  }
 }
 
 template <int MODE, bool F32, int BN>
@@ -486,7 +493,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
     // ---- epilogue: a thread has a row of the CTA's 128 and half of the tile's columns
     const int half = warp >> 2, quarter = warp & 3, mine = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    const int live = *p.live;
+    const int live = live_of(p);
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
@@ -528,8 +535,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
       const int row = m * 256 + (int)rank * 128 + mine, c0 = n * C::BN + half * C::COLS;
       if constexpr (MODE == kStats || MODE == kGrad) {
         const int here = p.V - p.v0 - c0;  // columns from c0 that are in the vocabulary
-        const int at = p.tgt[row] - p.v0 - c0;
-        const bool hit = at >= 0 && at < C::COLS;
+        const int target = MODE != kStats || p.live ? p.tgt[row] : row < live ? target_at(p.targets, p.wide, p.V, row) : -1;
+        const int at = target - p.v0 - c0;
+        const bool hit = target >= 0 && at >= 0 && at < C::COLS;
         if constexpr (MODE == kStats) {
           if (here < C::COLS)
 #pragma unroll
@@ -581,7 +589,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
 #pragma unroll
             for (int c = 0; c < C::COLS; ++c) v[c] = c == at ? v[c] - a : v[c];
           }
-          leave_in_boxes<C::COLS, C::PARTS>(&maps.g, staging + warp * 4096, v, c0, m * 256 + (int)rank * 128 + quarter * 32, lane);
+          if constexpr (C::BOXES) {
+            leave_in_boxes<C::COLS>(&maps.g, staging + warp * 4096, v, c0, m * 256 + (int)rank * 128 + quarter * 32, lane);
+          } else {
+            bf16* to = p.g + (size_t)row * p.piece + n * C::BN + half * C::COLS;
+#pragma unroll
+            for (int part = 0; part < C::PARTS; ++part, to += p.pad * p.piece)
+#pragma unroll
+              for (int c = 0; c < C::COLS; c += 8) {  // what a part leaves of a value goes to the next
+                const uint4 w = tc::pack8(v + c);
+                *reinterpret_cast<uint4*>(to + c) = w;
+                float lo[8];
+                tc::unpack8(w, lo);
+#pragma unroll
+                for (int y = 0; y < 8; ++y) v[c + y] -= lo[y];
+              }
+          }
         }
       } else if (t.share >= 0 || (MODE == kDx && p.sums)) {
         const bool add = t.share < 0 && p.adds;
@@ -599,7 +622,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
           }
         }
       } else if (C::BOXES && p.whole) {
-        leave_in_boxes<C::COLS, 1>(&maps.g, staging + warp * 4096, v, c0, p.v0 + m * 256 + (int)rank * 128 + quarter * 32, lane);
+        leave_in_boxes<C::COLS>(&maps.g, staging + warp * 4096, v, c0, p.v0 + m * 256 + (int)rank * 128 + quarter * 32, lane);
       } else if (row < (MODE == kDx ? live : p.M)) {
         using T = std::conditional_t<F32, float, bf16>;
         T* to = static_cast<T*>(p.out) + (MODE == kDx ? (size_t)p.idx[row] : (size_t)p.v0 + row) * p.D;
@@ -611,7 +634,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
   }
   __syncwarp();
   __syncthreads();
-  if (threadIdx.x == 0 && *bad) atomicExch(p.status, 11);
+  if (threadIdx.x == 0) {
+    if (MODE == kStats && p.flags) p.flags[blockIdx.x] = *bad ? 11 : 0;
+    else if (*bad) atomicExch(p.status, 11);
+  }
   __syncwarp();
   tc::fence_before_sync();
   tc::cluster_sync();  // (neither CTA leaves while the other's products read its shared memory or arrive at its barriers)
@@ -624,61 +650,86 @@ struct JoinP {
   const float2* part;
   const float* hit;
   const int32_t *live, *idx;
+  const void* targets;   // where live is null: rows in their own places
+  const int32_t* flags;
+  int32_t* status;
   float *loss, *lse;
   size_t pad;
-  int tiles;
+  int tiles, rows, wide, V, blocks;
 };
 __global__ void __launch_bounds__(256) lce_join_kernel(JoinP p) {
   begin_dependent();
   __shared__ float2 red[8][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row = blockIdx.x * 32 + lane;
-  const bool in = row < *p.live;
+  const bool in = row < (p.live ? *p.live : p.rows);
+  if (!p.live && blockIdx.x == 0) {
+    const int any = __syncthreads_or((int)threadIdx.x < p.blocks && p.flags[threadIdx.x]);
+    if (threadIdx.x == 0) *p.status = any ? 11 : 0;
+  }
   float2 all{-INFINITY, 0.f};
   if (in)
-    for (int t = warp; t < p.tiles; t += 8) add_sum(all, p.part[(size_t)t * p.pad + row]);
+    for (int t0 = warp; t0 < p.tiles; t0 += 32) {
+      float2 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = t0 + 8 * k < p.tiles ? p.part[(size_t)(t0 + 8 * k) * p.pad + row] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) add_sum(all, v[k]);
+    }
   red[warp][lane] = all;
   __syncthreads();
   if (warp != 0 || !in) return;
   for (int w = 1; w < 8; ++w) add_sum(all, red[w][lane]);
   const float lse = all.x + logf(all.y);
-  const int to = p.idx[row];
-  p.lse[to] = lse;
-  p.loss[to] = lse - p.hit[row];
+  const bool counts = p.live || target_at(p.targets, p.wide, p.V, row) >= 0;
+  const int to = p.live ? p.idx[row] : row;
+  p.lse[to] = counts ? lse : 0.f;
+  p.loss[to] = counts ? lse - p.hit[row] : 0.f;
 }
-// Tiles that were cut along K: their shares in order.  grid (at most pairs - 1 tiles, 2 CTAs' rows x pieces of 64 columns).
-template <int MODE, bool F32, int BN>
-__global__ void __launch_bounds__(256) lce_shares_kernel(const GemmP p, int pairs) {
-  using C = Cfg<MODE, F32, BN>;
+// Tiles that were cut along K, of dx and of dW: their shares in order, up to four at a time.  grid (at most pairs - 1 tiles, 2 CTAs' rows x
+// pieces of 16 columns, 2).
+template <bool F32, int BN>
+__global__ void __launch_bounds__(256) lce_shares_kernel(const GemmP px, const GemmP py, int pairs_x, int pairs_y) {
   using T = std::conditional_t<F32, float, bf16>;
   begin_dependent();
-  const Walk walk(p, MODE, C::BN, pairs);
+  const bool is_dx = blockIdx.z == 0;
+  const GemmP& p = is_dx ? px : py;
+  const Walk walk(p, is_dx ? kDx : kDw, BN, is_dx ? pairs_x : pairs_y);
   const int tile = blockIdx.x;
   if (tile >= walk.rest) return;
   Item t;
   walk.place(walk.whole + tile, t);
-  const int rank = blockIdx.y & 1, mine = threadIdx.x & 127, c0 = (blockIdx.y >> 1) * 64 + (threadIdx.x >> 7) * 32;
+  const int rank = blockIdx.y & 1, mine = threadIdx.x & 127, c0 = (blockIdx.y >> 1) * 16 + (threadIdx.x >> 7) * 8;
   // the pairs that have a unit of it: from the last that begins at or before its first unit on
   const int64_t from = (int64_t)tile * walk.kblocks, to = from + walk.kblocks, all = (int64_t)walk.rest * walk.kblocks;
   int pair = (int)(from * walk.sharers / all);
   while (pair > 0 && walk.first_unit(pair) > from) --pair;
   while (walk.first_unit(pair + 1) <= from) ++pair;
-  float v[32];
+  const int first_second = (int)(walk.first_unit(pair) / walk.kblocks) != tile;  // (only the first can have begun with another tile)
+  int end = (int)((to - 1) * walk.sharers / all);
+  while (end > 0 && walk.first_unit(end) >= to) --end;
+  while (end + 1 < walk.sharers && walk.first_unit(end + 1) < to) ++end;
+  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  const size_t in = tile_at<BN>(0, rank, mine, c0), stride = tile_at<BN>(1, 0, 0, 0);
+  for (int q = pair; q <= end; q += 4) {
+    float4 e[4][2];
 #pragma unroll
-  for (int c = 0; c < 32; ++c) v[c] = 0.f;
-  for (; pair < walk.sharers && walk.first_unit(pair) < to; ++pair) {
-    const int second = (int)(walk.first_unit(pair) / walk.kblocks) != tile;
-    const float* e = p.shares + tile_at<C::BN>((size_t)pair * 2 + second, rank, mine, c0);
+    for (int k = 0; k < 4; ++k)
+      if (q + k <= end) {
+        const float* at = p.shares + in + ((size_t)(q + k) * 2 + (q + k == pair ? first_second : 0)) * stride;
+        e[k][0] = *reinterpret_cast<const float4*>(at);
+        e[k][1] = *reinterpret_cast<const float4*>(at + 512);
+      }
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
-      const float4 o = *reinterpret_cast<const float4*>(e + x * 512);
-      v[4 * x] += o.x; v[4 * x + 1] += o.y; v[4 * x + 2] += o.z; v[4 * x + 3] += o.w;
-    }
+    for (int k = 0; k < 4; ++k)
+      if (q + k <= end)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) { v[4 * x] += e[k][x].x; v[4 * x + 1] += e[k][x].y; v[4 * x + 2] += e[k][x].z; v[4 * x + 3] += e[k][x].w; }
   }
-  if (MODE == kDx && p.sums) {
-    float* e = p.sums + tile_at<C::BN>((size_t)t.m * walk.n_tiles + t.n, rank, mine, c0);
+  if (is_dx && p.sums) {
+    float* e = p.sums + tile_at<BN>((size_t)t.m * walk.n_tiles + t.n, rank, mine, c0);
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
+    for (int x = 0; x < 2; ++x) {
       float4 o = make_float4(v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]);
       if (p.adds) {
         const float4 old = *reinterpret_cast<const float4*>(e + x * 512);
@@ -689,10 +740,9 @@ __global__ void __launch_bounds__(256) lce_shares_kernel(const GemmP p, int pair
     return;
   }
   const int row = t.m * 256 + rank * 128 + mine;
-  if (row >= (MODE == kDx ? *p.live : p.M)) return;
-  T* out = static_cast<T*>(p.out) + (MODE == kDx ? (size_t)p.idx[row] : (size_t)p.v0 + row) * p.D;
-#pragma unroll
-  for (int c = 0; c < 32; c += 8) store_row<T>(out, t.n * C::BN + c0 + c, p.D, p.whole, v + c);
+  if (row >= (is_dx ? *p.live : p.M)) return;
+  T* out = static_cast<T*>(p.out) + (is_dx ? (size_t)p.idx[row] : (size_t)p.v0 + row) * p.D;
+  store_row<T>(out, t.n * BN + c0, p.D, p.whole, v);
 }
 // dx from its sums by tiles, in the tensor's type.  grid (128 rows, pieces of 64 columns).
 template <bool F32, int BN>
@@ -746,23 +796,23 @@ static bool make_map(CUtensorMap* m, const void* base, uint64_t cols, uint64_t r
 
 constexpr int kPairs = 74;
 // Bytes of g that are kept at a time.
-constexpr size_t kGradBytes = (size_t)512 << 20;
+constexpr size_t kGradBytes = (size_t)640 << 20;
 constexpr size_t kPackBytes = (size_t)256 << 20;
 
 struct Plan {
-  bool f32, pack_w;
+  bool f32, pack_w, direct;
   int parts, Dp, piece, pieces;
   int BN, BD;  // columns of a tile: of logits, of gradients
   size_t N, pad;
   // workspace
-  int32_t *status, *live, *counts, *idx, *tgt;
-  float *a, *both, *lse2, *hit, *sums, *shares;
+  int32_t *status, *live, *counts, *idx, *tgt, *flags;
+  float *a, *both, *lse2, *hit, *sums, *shares[2];
   float2* part;
   bf16 *xc, *wc, *g;
   size_t bytes;
 };
-// bwd: the backward pass.  weight only says whether it can be read as it is.
-static Plan plan(const mxb_linear_ce_desc* d, const void* weight, bool bwd, void* base) {
+// bwd: the backward pass.  x and weight only say whether they can be read as they are.
+static Plan plan(const mxb_linear_ce_desc* d, const void* x, const void* weight, bool bwd, void* base) {
   Plan q{};
   q.f32 = d->io_dtype == MXB_F32;
   q.parts = q.f32 ? 3 : 1;
@@ -776,13 +826,20 @@ static Plan plan(const mxb_linear_ce_desc* d, const void* weight, bool bwd, void
   const int64_t all = ((int64_t)d->V + 255) / 256 * 256;
   int64_t most = bwd ? (int64_t)(kGradBytes / (q.pad * q.parts * 2)) : all;
   most = std::min<int64_t>(most, (int64_t)(kPackBytes / ((size_t)q.Dp * q.parts * 2)));
+  // whole rounds of dW's tiles where a piece is that large: nothing of it is cut into shares then
+  const int64_t d_tiles = (d->D + q.BD - 1) / q.BD, round = kPairs / std::gcd<int64_t, int64_t>(kPairs, d_tiles);
+  if (bwd && most < all && most / 256 >= round) most = most / 256 / round * round * 256;
   q.piece = (int)std::min<int64_t>(all, std::max<int64_t>(256, most / 256 * 256));
+  // few tokens: a tile of 256 rows costs as much with all of them as with some (512 tokens, 32768 words of 1024: 46 us with their
+  // rows moved together first, PLACEHOLDER without)
+  q.direct = !bwd && !q.pack_w && q.N <= 1024 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
   if (!bwd && !q.pack_w) q.piece = (int)all;
   q.pieces = (int)((d->V + (int64_t)q.piece - 1) / q.piece);
-  const int64_t m_tiles = q.pad / 256, d_tiles = (d->D + q.BD - 1) / q.BD;
+  const int64_t m_tiles = q.pad / 256;
   Carver c(base);
   q.status = c.take<int32_t>(64);  // (the device's error word leads the workspace)
   q.live = c.take<int32_t>(1);
+  q.flags = c.take<int32_t>(2 * kPairs);
   q.counts = c.take<int32_t>(q.N / kCountRows + 1);
   q.idx = c.take<int32_t>(q.pad);
   q.tgt = c.take<int32_t>(q.pad);
@@ -798,7 +855,7 @@ static Plan plan(const mxb_linear_ce_desc* d, const void* weight, bool bwd, void
     q.lse2 = c.take<float>(q.pad);
     q.g = c.take<bf16>((size_t)q.parts * q.pad * q.piece);
     if (q.pieces > 1) q.sums = c.take<float>((size_t)m_tiles * d_tiles * 256 * q.BD);
-    q.shares = c.take<float>((size_t)kPairs * 2 * 256 * q.BD);
+    for (float*& s : q.shares) s = c.take<float>((size_t)kPairs * 2 * 256 * q.BD);
   }
   q.bytes = c.bytes();
   return q;
@@ -806,25 +863,26 @@ static Plan plan(const mxb_linear_ce_desc* d, const void* weight, bool bwd, void
 
 // tiles, and blocks of 64 of K, at most (the tokens that count may be fewer)
 template <int MODE, bool F32, int BN>
-static mxb_status launch_gemm(const GemmP& p, const Maps& maps, int64_t tiles, int64_t kblocks, cudaStream_t st) {
+static mxb_status launch_gemm(const GemmP& p, const Maps& maps, int pairs, cudaStream_t st) {
   using C = Cfg<MODE, F32, BN>;
   if (MXB_ALLOW_SMEM(C::SMEM, lce_gemm_kernel<MODE, F32, BN>) != MXB_OK) return MXB_ERR_CUDA;
   static const char* const names[] = {"lce_stats_kernel", "lce_grad_kernel", "lce_dx_kernel", "lce_dw_kernel"};
-  constexpr bool cut = MODE == kDx || MODE == kDw;
-  const int pairs = (int)std::min<int64_t>(cut && kblocks >= 16 ? std::max<int64_t>(tiles, tiles * kblocks / 8) : tiles, kPairs);
   MXB_LAUNCH(names[MODE], st, (launch_kernel(lce_gemm_kernel<MODE, F32, BN>, 2 * pairs, kThreads, C::SMEM, st, p, maps)));
-  if constexpr (cut)
-    if (kblocks >= 16 && pairs > 1)
-      MXB_LAUNCH("lce_shares_kernel", st,
-                 (launch_kernel(lce_shares_kernel<MODE, F32, BN>, dim3((unsigned)std::min<int64_t>(tiles, pairs - 1), 2 * C::BN / 64), 256, 0, st, p, pairs)));
   return check_launch(names[MODE]);
 }
+// Pairs for so many tiles, whose sums may be cut (tiles and blocks of 64 of K at most: the tokens that count may be fewer).
+static int pairs_for(int64_t tiles, int64_t kblocks) {
+  return (int)std::min<int64_t>(kblocks >= 16 ? std::max<int64_t>(tiles, tiles * kblocks / 8) : tiles, kPairs);
+}
 template <typename T>
-static mxb_status pack(const mxb_linear_ce_desc* d, PackP& p, cudaStream_t st) {
-  if (p.N >= kCountRows)
-    MXB_LAUNCH("lce_count_kernel", st, (launch_kernel(lce_count_kernel, (unsigned)(p.N / kCountRows), 256, 0, st, p, const_cast<int32_t*>(p.counts))));
-  const int blocks = (int)((p.N + kPackRows - 1) / kPackRows);
-  MXB_LAUNCH("lce_pack_kernel", st, (launch_kernel(lce_pack_kernel<T>, blocks + 32, 256, 0, st, p, blocks)));
+static mxb_status pack(PackP& p, int32_t* counts, cudaStream_t st) {
+  if (p.N > 4 * kCountRows) {  // (up to there every block counts for itself)
+    p.counts = counts;
+    MXB_LAUNCH("lce_count_kernel", st, (launch_kernel(lce_count_kernel, (unsigned)(p.N / kCountRows), 256, 0, st, p, counts)));
+  }
+  p.each = p.N > 148 * 32 ? 4 : 1;
+  const int blocks = (int)((p.N + 8 * p.each - 1) / (8 * p.each));
+  MXB_LAUNCH("lce_pack_kernel", st, (launch_kernel(lce_pack_kernel<T>, blocks + 32 + (p.w_rows + 7) / 8, 256, 0, st, p, blocks)));
   return check_launch("lce_pack_kernel");
 }
 
@@ -832,12 +890,22 @@ template <bool F32, int BD>
 static mxb_status run(const mxb_linear_ce_desc* d, const Plan& q, PackP& pk, const void* weight, void* dweight, cudaStream_t st) {
   using T = std::conditional_t<F32, float, bf16>;
   const bool bwd = pk.d_loss != nullptr;
-  mxb_status s = pack<T>(d, pk, st);
-  if (s != MXB_OK) return s;
+  mxb_status s = MXB_OK;
+  if (!q.direct) {
+    if (q.pack_w) {
+      pk.w = weight;
+      pk.wc = q.wc;
+      pk.w_pad = q.piece;
+      pk.w_rows = (int)std::min<int64_t>(q.piece, d->V);
+    }
+    s = pack<T>(pk, q.counts, st);
+    if (s != MXB_OK) return s;
+  }
   const size_t pad = q.pad;
   const int D = d->D;
   constexpr int BN = F32 ? 128 : 256;
   GemmP last{};  // of the last piece's dx
+  int blocks = 0;
   const int64_t m_tiles = pad / 256, d_tiles = (D + BD - 1) / BD;
   for (int piece = 0; piece < q.pieces; ++piece) {
     const int v0 = piece * q.piece, rows = (int)std::min<int64_t>(q.piece, (int64_t)d->V - v0);
@@ -845,17 +913,24 @@ static mxb_status run(const mxb_linear_ce_desc* d, const Plan& q, PackP& pk, con
     uint64_t w_rows = d->V, w_part = (uint64_t)d->V * D;
     int w_row0 = v0;
     if (q.pack_w) {
-      MXB_LAUNCH("lce_pack_weight_kernel", st,
-                 (launch_kernel(lce_pack_weight_kernel<T>, (unsigned)((rows + 7) / 8), 256, 0, st, static_cast<const T*>(weight) + (size_t)v0 * D, q.wc,
-                                rows, (size_t)q.piece, D, q.Dp)));
+      if (piece > 0)
+        MXB_LAUNCH("lce_pack_weight_kernel", st,
+                   (launch_kernel(lce_pack_weight_kernel<T>, (unsigned)((rows + 7) / 8), 256, 0, st, static_cast<const T*>(weight) + (size_t)v0 * D,
+                                  q.wc, rows, (size_t)q.piece, D, q.Dp)));
       w = q.wc;
       w_rows = rows;
       w_part = (uint64_t)q.piece * q.Dp;
       w_row0 = 0;
     }
     GemmP p{};
-    p.live = q.live;
+    p.live = q.direct ? nullptr : q.live;
+    p.targets = pk.targets;
+    p.wide = pk.wide;
+    p.rows = (int)q.N;
+    p.flags = q.direct ? q.flags : nullptr;
     p.status = q.status;
+    p.g = q.g;
+    p.piece = q.piece;
     p.tgt = q.tgt;
     p.idx = q.idx;
     p.v0 = v0;
@@ -865,7 +940,7 @@ static mxb_status run(const mxb_linear_ce_desc* d, const Plan& q, PackP& pk, con
     p.group = 8;
     Maps maps;
     std::memset(&maps, 0, sizeof maps);
-    bool ok = make_map(&maps.a, q.xc, q.Dp, pad, q.parts, q.Dp, pad * q.Dp, 128) && make_map(&maps.b, w, q.Dp, w_rows, q.parts, q.Dp, w_part, BN / 2);
+    bool ok = (q.direct ? make_map(&maps.a, pk.x, D, q.N, 1, D, q.N * D, 128) : make_map(&maps.a, q.xc, q.Dp, pad, q.parts, q.Dp, pad * q.Dp, 128)) && make_map(&maps.b, w, q.Dp, w_rows, q.parts, q.Dp, w_part, BN / 2);
     if (bwd) ok = ok && make_map(&maps.g, q.g, q.piece, pad, q.parts, q.piece, pad * q.piece, 32);
     if (!ok) return MXB_ERR_UNSUPPORTED;
     p.N = rows;
@@ -877,7 +952,9 @@ static mxb_status run(const mxb_linear_ce_desc* d, const Plan& q, PackP& pk, con
     p.both = q.both;
     p.lse2 = q.lse2;
     const int64_t tiles = m_tiles * ((rows + BN - 1) / BN);
-    s = bwd ? launch_gemm<kGrad, F32, BN>(p, maps, tiles, 0, st) : launch_gemm<kStats, F32, BN>(p, maps, tiles, 0, st);
+    const int pairs = (int)std::min<int64_t>(tiles, kPairs);
+    s = bwd ? launch_gemm<kGrad, F32, BN>(p, maps, pairs, st) : launch_gemm<kStats, F32, BN>(p, maps, pairs, st);
+    blocks = 2 * pairs;
     if (s != MXB_OK) return s;
     if (bwd) {
       // dx: sums over the piece, in the order of the pieces
@@ -886,13 +963,15 @@ static mxb_status run(const mxb_linear_ce_desc* d, const Plan& q, PackP& pk, con
       x.K = rows;
       x.b_row0 = w_row0;
       x.sums = q.sums;
-      x.shares = q.shares;
+      x.shares = q.shares[0];
       x.adds = piece > 0;
       x.out = pk.dx;
       x.whole = D % 8 == 0 && (reinterpret_cast<uintptr_t>(pk.dx) & 15) == 0;
       if (!make_map(&maps.a, q.g, q.piece, pad, q.parts, q.piece, pad * q.piece, 128) || !make_map(&maps.b, w, q.Dp, w_rows, q.parts, q.Dp, w_part, 64))
         return MXB_ERR_UNSUPPORTED;
-      s = launch_gemm<kDx, F32, BD>(x, maps, m_tiles * d_tiles, (rows + 63) / 64, st);
+      const int64_t x_tiles = m_tiles * d_tiles, x_blocks = (rows + 63) / 64, y_tiles = (int64_t)((rows + 255) / 256) * d_tiles, y_blocks = (q.N + 63) / 64;
+      const int x_pairs = pairs_for(x_tiles, x_blocks), y_pairs = pairs_for(y_tiles, y_blocks);
+      s = launch_gemm<kDx, F32, BD>(x, maps, x_pairs, st);
       if (s != MXB_OK) return s;
       last = x;
       // dW: sums over the tokens
@@ -900,14 +979,19 @@ static mxb_status run(const mxb_linear_ce_desc* d, const Plan& q, PackP& pk, con
       y.M = rows;
       y.N = D;
       y.b_row0 = 0;
-      y.shares = q.shares;
+      y.shares = q.shares[1];
       y.out = dweight;
       y.whole = D % 8 == 0 && (reinterpret_cast<uintptr_t>(dweight) & 15) == 0;
       if (!make_map(&maps.a, q.g, q.piece, pad, q.parts, q.piece, pad * q.piece, 64) || !make_map(&maps.b, q.xc, q.Dp, pad, q.parts, q.Dp, pad * q.Dp, 64))
         return MXB_ERR_UNSUPPORTED;
       if (!F32 && y.whole && !make_map(&maps.g, dweight, D, d->V, 1, D, (uint64_t)d->V * D, 32)) return MXB_ERR_UNSUPPORTED;
-      s = launch_gemm<kDw, F32, BD>(y, maps, (int64_t)((rows + 255) / 256) * d_tiles, (int64_t)((q.N + 63) / 64), st);
+      s = launch_gemm<kDw, F32, BD>(y, maps, y_pairs, st);
       if (s != MXB_OK) return s;
+      // (how many tiles of dx there are, the device knows)
+      const int64_t x_cut = x_blocks >= 16 ? std::min<int64_t>(x_tiles, x_pairs - 1) : 0, y_cut = y_blocks >= 16 ? y_tiles % y_pairs : 0;
+      if (x_cut || y_cut)
+        MXB_LAUNCH("lce_shares_kernel", st,
+                   (launch_kernel(lce_shares_kernel<F32, BD>, dim3((unsigned)std::max(x_cut, y_cut), 2 * BD / 16, 2), 256, 0, st, x, y, x_pairs, y_pairs)));
     }
   }
   if (bwd) {
@@ -916,7 +1000,8 @@ static mxb_status run(const mxb_linear_ce_desc* d, const Plan& q, PackP& pk, con
                  (launch_kernel(lce_finish_kernel<F32, BD>, dim3((unsigned)(pad / 128), (unsigned)((D + 63) / 64)), 256, 0, st, last, (int)d_tiles)));
     return check_launch("linear_ce_bwd");
   }
-  const JoinP j{q.part, q.hit, q.live, q.idx, pk.loss, pk.lse_out, pad, (d->V + BN - 1) / BN};
+  const JoinP j{q.part, q.hit, q.direct ? nullptr : q.live, q.idx, pk.targets, q.flags, q.status, pk.loss, pk.lse_out, pad, (d->V + BN - 1) / BN, (int)q.N,
+                pk.wide, d->V, blocks};
   MXB_LAUNCH("lce_join_kernel", st, (launch_kernel(lce_join_kernel, (unsigned)(pad / 32), 256, 0, st, j)));
   return check_launch("linear_ce_fwd");
 }
@@ -928,7 +1013,6 @@ static PackP pack_args(const mxb_linear_ce_desc* d, const Plan& q, const void* x
   PackP p{};
   p.targets = targets;
   p.x = x;
-  p.counts = q.counts;
   p.live = q.live;
   p.idx = q.idx;
   p.tgt = q.tgt;
@@ -943,17 +1027,16 @@ static PackP pack_args(const mxb_linear_ce_desc* d, const Plan& q, const void* x
   p.D = d->D;
   p.Dp = q.Dp;
   p.wide = d->target_bytes == 8;
-  p.f32 = q.f32;
   return p;
 }
 
 }  // namespace lce
 
-size_t linear_ce_scratch(const mxb_linear_ce_desc* d, bool bwd) { return lce::plan(d, nullptr, bwd, nullptr).bytes; }
+size_t linear_ce_scratch(const mxb_linear_ce_desc* d, bool bwd) { return lce::plan(d, nullptr, nullptr, bwd, nullptr).bytes; }
 
 mxb_status linear_ce_fwd(const mxb_linear_ce_desc* d, const void* x, const void* weight, const void* targets, float* loss, float* lse,
                          void* workspace, cudaStream_t st) {
-  const lce::Plan q = lce::plan(d, weight, false, workspace);
+  const lce::Plan q = lce::plan(d, x, weight, false, workspace);
   lce::PackP p = lce::pack_args(d, q, x, targets);
   p.loss = loss;
   p.lse_out = lse;
@@ -961,7 +1044,7 @@ mxb_status linear_ce_fwd(const mxb_linear_ce_desc* d, const void* x, const void*
 }
 mxb_status linear_ce_bwd(const mxb_linear_ce_desc* d, const void* x, const void* weight, const void* targets, const float* lse, const float* d_loss,
                          const float* d_lse, void* dx, void* dweight, void* workspace, cudaStream_t st) {
-  const lce::Plan q = lce::plan(d, weight, true, workspace);
+  const lce::Plan q = lce::plan(d, x, weight, true, workspace);
   lce::PackP p = lce::pack_args(d, q, x, targets);
   p.lse = lse;
   p.d_loss = d_loss;

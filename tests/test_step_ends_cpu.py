@@ -58,7 +58,7 @@ def test_the_backward_keeps_a_piece_of_the_vocabulary():
     lib = mixlab_b200.lib()
     for V in (50001, 400001):
         d = _lib.LinearCeDesc(32768, V, 1024, 8, _lib.MXB_BF16)
-        assert lib.mxb_linear_ce_bwd_workspace_bytes(C.byref(d)) < (800 << 20)
+        assert lib.mxb_linear_ce_bwd_workspace_bytes(C.byref(d)) < (1 << 30)
     d = _lib.LinearCeDesc(1 << 21, 50001, 64, 8, _lib.MXB_BF16)  # (so many tokens that a piece is one tile)
     assert lib.mxb_linear_ce_bwd_workspace_bytes(C.byref(d)) < (3 << 30)
 
