@@ -10,7 +10,9 @@
 // exponentials of each row over the tile's columns, 8 bytes a row and tile.  Backward, in pieces of the vocabulary: z again, g in
 // bf16 to a workspace of bounded size, then dx += g W and dW = g^T x from it.
 // float32 tensors: every operand is split into three bf16 parts (24 bits and more), and six products of parts, those above
-// 2^-24, are added up: the first in an accumulator of its own, as the others are 2^-8 and less of it.
+// 2^-24, are added up.  An accumulator in TMEM is cut, not rounded, with every product added to it, so it takes the products
+// of 128 terms, small ones first, and is handed over: the sums of those are float32 in registers (2048 tokens, 5003 words of 448: gradients
+// off by 7e-7, with accumulators of 2048 terms by 3.6e-6).
 #include <cuda.h>
 
 #include <algorithm>
@@ -203,19 +205,19 @@ __global__ void __launch_bounds__(256) lce_pack_weight_kernel(const T* w, bf16* 
 // ------------------------------------------------------------------ the products
 enum Mode { kStats, kGrad, kDx, kDw };
 // A stage of the ring: PARTS tiles of A, 128 rows a CTA, and of B, BN / 2 rows a CTA, 64 deep.
-// BN, columns of a tile: 128 where two accumulators of float32 products lie side by side, or where all columns are that few.
+// BN, columns of a tile.
 template <int MODE, bool F32, int BN_>
 struct Cfg {
   static constexpr int BN = BN_, PARTS = F32 ? 3 : 1, COLS = BN / 2;  // COLS: of a thread of the epilogue
   static constexpr int A = 128 * 128, B = BN / 2 * 128, STAGE = PARTS * (A + B);
-  static constexpr int STAGES = F32 ? 3 : 6;
-  // results leave in boxes of 32 rows x 64 columns a warp (float32: shared memory is better spent on a third stage)
-  static constexpr bool BOXES = (MODE == kGrad || MODE == kDw) && !F32;
+  static constexpr int STAGES = !F32 ? 6 : BN == 128 ? 3 : 2;
+  static constexpr bool BOXES = MODE == kDw && !F32;  // results leave in boxes of 32 rows x 64 columns a warp
   static constexpr int STAGING = BOXES ? 8 * 4096 : 0;
   static constexpr bool A_MN = MODE == kDw, B_MN = MODE == kDx || MODE == kDw;
-  static constexpr int SMEM = 1024 + STAGES * STAGE + STAGING + 256 + (MODE == kStats ? 128 + 4 * 128 * 8 : 0);
+  static constexpr int ACCS = 512 / BN, RING = 2 * ACCS;  // accumulators in TMEM; kStats: slots for what halves of a tile exchange
+  static constexpr int SMEM = 1024 + STAGES * STAGE + STAGING + 256 + (MODE == kStats ? RING * (4 * 8 + 128 * 8) : 0);
 };
-constexpr int kThreads = 320, kSegment = 4;  // blocks of 64 that a float32 accumulator takes before it is added up in registers
+constexpr int kThreads = 320;
 struct GemmP {
   const int32_t* live;    // null: rows tokens, none left out
   const void* targets;    //   their targets (wide: of 64 bits)
@@ -228,7 +230,7 @@ struct GemmP {
   int v0, V;              // first row of the vocabulary's piece, rows in all
   bf16* g;
   size_t pad;             // rows of what is indexed by token
-  int piece;              // columns of g
+  int piece, blocks;      // columns of g, blocks of 128 rows of one of its parts
   float2* part;           // kStats: [tiles of the vocabulary][pad] maximum and sum
   float* hit;             //   logit of the target
   const int32_t *tgt, *idx;
@@ -277,7 +279,8 @@ struct Item {
   int share;  // -1: the whole tile
 };
 struct Walk {
-  int m_tiles, n_tiles, kblocks, tiles, whole, rest, sharers, pairs, group;
+  int m_tiles, n_tiles, kblocks, tiles, whole, rest, pairs, group;
+  int units, share;  // blocks of K of all tiles that are cut; a pair's
   __device__ __forceinline__ Walk(const GemmP& p, int mode, int BN, int pairs_) {
     const int live = live_of(p);
     const int M = mode == kDw ? p.M : live, K = mode == kDw ? live : p.K;
@@ -289,9 +292,10 @@ struct Walk {
     tiles = m_tiles * n_tiles;
     rest = mode == kStats || mode == kGrad || kblocks < 16 ? 0 : tiles % pairs;
     whole = tiles - rest;
-    sharers = (int)min((int64_t)pairs, (int64_t)rest * kblocks / 8);  // (at least two a tile)
+    units = rest * kblocks;  // (2^31 at most: check_linear_ce_desc())
+    const int sharers = min(pairs, units / 8);  // more than there are tiles: a share is a tile's sum at most
+    share = sharers ? (units + sharers - 1) / sharers : 0;
   }
-  __device__ __forceinline__ int64_t first_unit(int pair) const { return (int64_t)rest * kblocks * pair / sharers; }
   __device__ __forceinline__ void place(int i, Item& t) const {
     const int g = i / (group * n_tiles), in = i - g * group * n_tiles, gm = min(group, m_tiles - g * group);
     t.m = g * group + in % gm;
@@ -307,9 +311,9 @@ struct Walk {
       t.share = -1;
       return true;
     }
-    if (pair >= sharers) return false;
-    const int64_t from = first_unit(pair), to = first_unit(pair + 1);
-    const int tile = (int)(from / kblocks), second = j - (whole + pairs - 1 - pair) / pairs;
+    const int64_t from = (int64_t)pair * share, to = min(from + share, (int64_t)units);
+    if (from >= units) return false;
+    const int tile = (int)from / kblocks, second = j - (whole + pairs - 1 - pair) / pairs;
     const int64_t cut = (int64_t)(tile + 1) * kblocks;
     if (second > 1 || (second == 1 && to <= cut)) return false;
     place(whole + tile + second, t);
@@ -319,6 +323,10 @@ struct Walk {
     return true;
   }
 };
+// g lies in blocks of 128 rows, in those by eight columns, 16 bytes a row: a warp of the epilogue writes whole lines straight from its
+// registers, and a copy of such blocks is an operand of the products without a swizzle, with the contraction along columns (dx) or
+// rows (dW).  (float32, 2048 tokens, 5003 words of 448: 52 us; rows of the matrix, 16 bytes a lane, 70.)
+__device__ __forceinline__ size_t g_at(const GemmP& p, int block, int col) { return ((size_t)block * (p.piece / 8) + col / 8) * 1024; }
 // Float32 tiles as the epilogue has them: element (row, c .. c + 3) of a CTA's 128 rows, 16 bytes of 32 rows side by side.
 template <int BN>
 __device__ __forceinline__ size_t tile_at(size_t tile, int rank, int row, int c) {
@@ -363,20 +371,19 @@ __device__ __forceinline__ void leave_in_boxes(const void* map, uint8_t* box, co
 template <int MODE, bool F32, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gemm_kernel(const GemmP p, const __grid_constant__ Maps maps) {
   using C = Cfg<MODE, F32, BN>;
-  begin_dependent();
   extern __shared__ uint8_t raw[];
   const uint32_t base = (tc::smem_u32(raw) + 1023u) & ~1023u;
   uint8_t* sm = raw + (base - tc::smem_u32(raw));
   uint8_t* staging = sm + C::STAGES * C::STAGE;
   uint64_t* full = reinterpret_cast<uint64_t*>(staging + C::STAGING);
-  uint64_t *empty = full + C::STAGES, *acc_full = empty + C::STAGES, *acc_empty = acc_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  uint64_t *empty = full + C::STAGES, *acc_full = empty + C::STAGES, *acc_empty = acc_full + C::ACCS;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + C::ACCS);
   volatile int32_t* bad = reinterpret_cast<volatile int32_t*>(tmem_slot + 1);
-  // kStats: what the warps of a tile's second half found, for those of the first: a ring of four tiles, a barrier a slot and warp.
-  // (When a warp writes for tile t + 4, tile t + 3's accumulator has been filled, so tile t + 1's has been read by all warps, which
-  // are done with tile t.)
-  uint64_t* halves_full = reinterpret_cast<uint64_t*>(staging + C::STAGING + 256);  // [4][4]
-  float2* halves = reinterpret_cast<float2*>(halves_full + 16);                     // [4][128]
+  // kStats: what the warps of a tile's second half found, for those of the first: a ring of slots by tiles, a barrier a slot and warp.
+  // (When a warp writes for tile t + 2 ACCS, that tile's accumulator has been filled, so tile t + ACCS's has been read by all warps,
+  // which are done with the tiles in front of it.)
+  uint64_t* halves_full = reinterpret_cast<uint64_t*>(staging + C::STAGING + 256);  // [RING][4]
+  float2* halves = reinterpret_cast<float2*>(halves_full + C::RING * 4);            // [RING][128]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = tc::cluster_rank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -386,14 +393,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
       tc::mbar_init(full + s, 1);
       tc::mbar_init(empty + s, 1);
     }
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < C::ACCS; ++s) {
       tc::mbar_init(acc_full + s, 1);
       tc::mbar_init(acc_empty + s, 16);
     }
     if (MODE == kStats)
-      for (int s = 0; s < 16; ++s) tc::mbar_init(halves_full + s, 1);
+      for (int s = 0; s < C::RING * 4; ++s) tc::mbar_init(halves_full + s, 1);
     *bad = 0;
     tc::mbar_fence_init();
+  }
+  if (threadIdx.x == 32) {
+    tc::tma_prefetch_map(&maps.a);
+    tc::tma_prefetch_map(&maps.b);
   }
   if (warp == 9) {
     tc::tmem_alloc_pair(tmem_slot, 512);
@@ -403,12 +414,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
   __syncthreads();
   tc::cluster_sync();
   tc::fence_after_sync();
+  begin_dependent();  // (nothing but this CTA's own memory is touched before)
   const uint32_t tmem = *tmem_slot;
   const Walk walk(p, MODE, C::BN, pairs);
   Item t;
   const Wait wait{bad};
   // blocks of K behind which an accumulator is handed over
-  constexpr int SEG = F32 ? kSegment : 1 << 30;
+  constexpr int SEG = F32 ? 2 : 1 << 30;
 
   if (warp == 8) {
     // ---- copies: each CTA its half of A and B, counted by the barrier of the CTA that issues the products
@@ -425,12 +437,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
 #pragma unroll
           for (int part = 0; part < C::PARTS; ++part, to += C::A) {
             const int m0 = t.m * 256 + (int)rank * 128;
-            if (C::A_MN) {
-              tc::tma_load_3d_pair(to, &maps.a, m0, kb * 64, part, bar);
-              tc::tma_load_3d_pair(to + 8192, &maps.a, m0 + 64, kb * 64, part, bar);
-            } else {
-              tc::tma_load_3d_pair(to, &maps.a, kb * 64, m0, part, bar);
-            }
+            if (MODE == kDx) tc::tma_load_4d_pair(to, &maps.a, 0, 0, kb * 8, part * p.blocks + m0 / 128, bar);
+            else if (MODE == kDw) tc::tma_load_4d_pair(to, &maps.a, 0, (kb & 1) * 2, m0 / 8, part * p.blocks + kb / 2, bar);
+            else tc::tma_load_3d_pair(to, &maps.a, kb * 64, m0, part, bar);
           }
 #pragma unroll
           for (int part = 0; part < C::PARTS; ++part, to += C::B) {
@@ -450,7 +459,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
     // ---- products, by one thread of the pair
     if (rank == 0 && tc::elect_one()) {
       constexpr uint32_t idesc = tc::make_idesc_bf16(256, C::BN, C::A_MN, C::B_MN);
-      constexpr uint32_t a_step = C::A_MN ? 2048 : 32, b_step = C::B_MN ? 2048 : 32;
+      constexpr uint32_t a_step = MODE == kDx ? 4096 : MODE == kDw ? 256 : 32, b_step = C::B_MN ? 2048 : 32;
       int s = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
@@ -459,33 +468,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
         for (int ks = t.k0; ok && ks < k1; ks += SEG) {
           if (!(ok = wait(acc_empty + acc, acc_phase ^ 1u))) break;
           tc::fence_after_sync();
-          const uint32_t d = tmem + acc * 256;
+          const uint32_t d = tmem + acc * BN;
           const int ke = min(ks + min(SEG, k1 - ks), k1);
           for (int kb = ks; kb < ke; ++kb) {
             if (!(ok = wait(full + s, phase))) break;
             tc::fence_after_sync();
             const uint32_t sa = base + s * C::STAGE, sb = sa + C::PARTS * C::A;
-            auto product = [&](int pa, int pb, uint32_t to, bool first) {
-              const uint64_t da = tc::make_smem_desc(sa + pa * C::A, C::A_MN ? 8192 : 16, 1024, tc::kSwizzle128);
+            auto product = [&](int pa, int pb, bool first) {
+              const uint64_t da = MODE == kDx   ? tc::make_smem_desc(sa + pa * C::A, 2048, 128, tc::kSwizzleNone)
+                                  : MODE == kDw ? tc::make_smem_desc(sa + pa * C::A, 128, 1024, tc::kSwizzleNone)
+                                                : tc::make_smem_desc(sa + pa * C::A, 16, 1024, tc::kSwizzle128);
               const uint64_t db = tc::make_smem_desc(sb + pb * C::B, C::B_MN ? 8192 : 16, 1024, tc::kSwizzle128);
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                tc::mma_pair(to, da + (uint64_t)((k * a_step) >> 4), db + (uint64_t)((k * b_step) >> 4), idesc, !(first && k == 0));
+                tc::mma_pair(d, da + (uint64_t)((k * a_step) >> 4), db + (uint64_t)((k * b_step) >> 4), idesc, !(first && k == 0));
             };
-            product(0, 0, d, kb == ks);
             if (F32) {
-              product(2, 0, d + 128, kb == ks);
-              product(0, 2, d + 128, false);
-              product(1, 1, d + 128, false);
-              product(1, 0, d + 128, false);
-              product(0, 1, d + 128, false);
+              product(2, 0, kb == ks);
+              product(0, 2, false);
+              product(1, 1, false);
+              product(1, 0, false);
+              product(0, 1, false);
             }
+            product(0, 0, !F32 && kb == ks);
             tc::mma_commit_pair(empty + s);
             if (++s == C::STAGES) { s = 0; phase ^= 1u; }
           }
           if (!ok) break;
           tc::mma_commit_pair(acc_full + acc);
-          if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+          if (++acc == C::ACCS) { acc = 0; acc_phase ^= 1u; }
         }
       }
     }
@@ -499,6 +510,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
     bool ok = true;
     for (int j = 0; ok && walk.item(pair, j, t); ++j) {
       const int m = t.m, n = t.n, k0 = t.k0, k1 = t.k1;
+      const int row = m * 256 + (int)rank * 128 + mine, c0 = n * C::BN + half * C::COLS;
+      int target = -1;  // what the epilogue needs of its row, under way beside the products
+      float both = 0.f, back = 0.f;
+      if constexpr (MODE == kStats) target = p.live ? p.tgt[row] : row < live ? target_at(p.targets, p.wide, p.V, row) : -1;
+      if constexpr (MODE == kGrad) {
+        target = p.tgt[row];
+        both = p.both[row];
+        back = -p.lse2[row];
+      }
       float v[C::COLS];
       if (k0 == k1 || F32)
 #pragma unroll
@@ -507,7 +527,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
         if (!(ok = wait(acc_full + acc, acc_phase))) break;
         __syncwarp();
         tc::fence_after_sync();
-        const uint32_t d = tmem + lanes + acc * 256 + half * C::COLS;
+        const uint32_t d = tmem + lanes + acc * BN + half * C::COLS;
         if constexpr (!F32) {
 #pragma unroll
           for (int c = 0; c < C::COLS; c += 32) {
@@ -518,24 +538,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
         } else {
 #pragma unroll
           for (int c = 0; c < C::COLS; c += 32) {
-            uint32_t big[32], small[32];
-            tc::tmem_ld_32x32b_x32(d + c, big);
-            tc::tmem_ld_32x32b_x32(d + 128 + c, small);
+            uint32_t sum[32];
+            tc::tmem_ld_32x32b_x32(d + c, sum);
             tc::tmem_ld_wait();
 #pragma unroll
-            for (int x = 0; x < 32; ++x) v[c + x] += __uint_as_float(big[x]) + __uint_as_float(small[x]);
+            for (int x = 0; x < 32; ++x) v[c + x] += __uint_as_float(sum[x]);
           }
         }
         tc::fence_before_sync();
         __syncwarp();
         if (lane == 0) tc::mbar_arrive_cluster(tc::in_cta(tc::smem_u32(acc_empty + acc), 0));
-        if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+        if (++acc == C::ACCS) { acc = 0; acc_phase ^= 1u; }
       }
       if (!ok) break;
-      const int row = m * 256 + (int)rank * 128 + mine, c0 = n * C::BN + half * C::COLS;
       if constexpr (MODE == kStats || MODE == kGrad) {
         const int here = p.V - p.v0 - c0;  // columns from c0 that are in the vocabulary
-        const int target = MODE != kStats || p.live ? p.tgt[row] : row < live ? target_at(p.targets, p.wide, p.V, row) : -1;
         const int at = target - p.v0 - c0;
         const bool hit = target >= 0 && at >= 0 && at < C::COLS;
         if constexpr (MODE == kStats) {
@@ -560,7 +577,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
             for (int c = 0; c < C::COLS; ++c) z = c == at ? v[c] : z;
             if (hit && row < live) p.hit[row] = z;
           }
-          const int slot = j & 3;
+          const int slot = j % C::RING;
           float2* buf = halves + slot * 128;
           uint64_t* there = halves_full + slot * 4 + quarter;
           if (half == 1) {
@@ -568,7 +585,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(there);
           } else {
-            if (!(ok = wait(there, (uint32_t)(j >> 2) & 1u))) break;
+            if (!(ok = wait(there, (uint32_t)(j / C::RING) & 1u))) break;
             const float2 o = buf[mine];
             if (row < live) {
               float2 both{shift, sum};
@@ -578,7 +595,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
           }
         } else {
           // (float32: the logit's distance from lse first, which leaves the exponent the error of that distance alone)
-          const float both = p.both[row], back = -p.lse2[row];
 #pragma unroll
           for (int c = 0; c < C::COLS; ++c) v[c] = both * ex2(F32 ? (v[c] + back) * kLog2e : fmaf(v[c], kLog2e, back));
           if (row >= live || here < C::COLS)
@@ -589,22 +605,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
 #pragma unroll
             for (int c = 0; c < C::COLS; ++c) v[c] = c == at ? v[c] - a : v[c];
           }
-          if constexpr (C::BOXES) {
-            leave_in_boxes<C::COLS>(&maps.g, staging + warp * 4096, v, c0, m * 256 + (int)rank * 128 + quarter * 32, lane);
-          } else {
-            bf16* to = p.g + (size_t)row * p.piece + n * C::BN + half * C::COLS;
+          bf16* to = p.g + g_at(p, m * 2 + rank, n * C::BN + half * C::COLS) + mine * 8;
 #pragma unroll
-            for (int part = 0; part < C::PARTS; ++part, to += p.pad * p.piece)
+          for (int part = 0; part < C::PARTS; ++part, to += p.pad * p.piece)
 #pragma unroll
-              for (int c = 0; c < C::COLS; c += 8) {  // what a part leaves of a value goes to the next
-                const uint4 w = tc::pack8(v + c);
-                *reinterpret_cast<uint4*>(to + c) = w;
-                float lo[8];
-                tc::unpack8(w, lo);
+            for (int c = 0; c < C::COLS; c += 8) {
+              const uint4 w = tc::pack8(v + c);
+              *reinterpret_cast<uint4*>(to + c * 128) = w;
+              if (part + 1 == C::PARTS) continue;
+              float lo[8];  // what a part leaves of a value goes to the next
+              tc::unpack8(w, lo);
 #pragma unroll
-                for (int y = 0; y < 8; ++y) v[c + y] -= lo[y];
-              }
-          }
+              for (int y = 0; y < 8; ++y) v[c + y] -= lo[y];
+            }
         }
       } else if (t.share >= 0 || (MODE == kDx && p.sums)) {
         const bool add = t.share < 0 && p.adds;
@@ -645,7 +658,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
   if (warp == 9) tc::tmem_dealloc_pair(tmem, 512);
 }
 
-// lse and loss of each row from its tiles' maxima and sums: eight warps take every eighth tile, then warp 0 theirs in order.
+// lse and loss of each row from its tiles' maxima and sums: 32 warps take every 32nd tile, then warp 0 theirs in order.
 struct JoinP {
   const float2* part;
   const float* hit;
@@ -657,9 +670,10 @@ struct JoinP {
   size_t pad;
   int tiles, rows, wide, V, blocks;
 };
-__global__ void __launch_bounds__(256) lce_join_kernel(JoinP p) {
+constexpr int kJoinWarps = 32;
+__global__ void __launch_bounds__(32 * kJoinWarps) lce_join_kernel(JoinP p) {
   begin_dependent();
-  __shared__ float2 red[8][32];
+  __shared__ float2 red[kJoinWarps][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row = blockIdx.x * 32 + lane;
   const bool in = row < (p.live ? *p.live : p.rows);
@@ -669,17 +683,17 @@ __global__ void __launch_bounds__(256) lce_join_kernel(JoinP p) {
   }
   float2 all{-INFINITY, 0.f};
   if (in)
-    for (int t0 = warp; t0 < p.tiles; t0 += 32) {
+    for (int t0 = warp; t0 < p.tiles; t0 += 4 * kJoinWarps) {
       float2 v[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = t0 + 8 * k < p.tiles ? p.part[(size_t)(t0 + 8 * k) * p.pad + row] : make_float2(-INFINITY, 0.f);
+      for (int k = 0; k < 4; ++k) v[k] = t0 + kJoinWarps * k < p.tiles ? p.part[(size_t)(t0 + kJoinWarps * k) * p.pad + row] : make_float2(-INFINITY, 0.f);
 #pragma unroll
       for (int k = 0; k < 4; ++k) add_sum(all, v[k]);
     }
   red[warp][lane] = all;
   __syncthreads();
   if (warp != 0 || !in) return;
-  for (int w = 1; w < 8; ++w) add_sum(all, red[w][lane]);
+  for (int w = 1; w < min(kJoinWarps, p.tiles); ++w) add_sum(all, red[w][lane]);
   const float lse = all.x + logf(all.y);
   const bool counts = p.live || target_at(p.targets, p.wide, p.V, row) >= 0;
   const int to = p.live ? p.idx[row] : row;
@@ -700,15 +714,8 @@ __global__ void __launch_bounds__(256) lce_shares_kernel(const GemmP px, const G
   Item t;
   walk.place(walk.whole + tile, t);
   const int rank = blockIdx.y & 1, mine = threadIdx.x & 127, c0 = (blockIdx.y >> 1) * 16 + (threadIdx.x >> 7) * 8;
-  // the pairs that have a unit of it: from the last that begins at or before its first unit on
-  const int64_t from = (int64_t)tile * walk.kblocks, to = from + walk.kblocks, all = (int64_t)walk.rest * walk.kblocks;
-  int pair = (int)(from * walk.sharers / all);
-  while (pair > 0 && walk.first_unit(pair) > from) --pair;
-  while (walk.first_unit(pair + 1) <= from) ++pair;
-  const int first_second = (int)(walk.first_unit(pair) / walk.kblocks) != tile;  // (only the first can have begun with another tile)
-  int end = (int)((to - 1) * walk.sharers / all);
-  while (end > 0 && walk.first_unit(end) >= to) --end;
-  while (end + 1 < walk.sharers && walk.first_unit(end + 1) < to) ++end;
+  const int from = tile * walk.kblocks, pair = from / walk.share, end = (from + walk.kblocks - 1) / walk.share;
+  const int first_second = pair * walk.share < from;  // (only the first pair can have begun with another tile)
   float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   const size_t in = tile_at<BN>(0, rank, mine, c0), stride = tile_at<BN>(1, 0, 0, 0);
   for (int q = pair; q <= end; q += 4) {
@@ -777,10 +784,9 @@ __global__ void __launch_bounds__(256) lce_finish_kernel(const GemmP p, int n_ti
 }
 
 // ------------------------------------------------------------------ host
-static bool make_map(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows, uint64_t parts, uint64_t pitch, uint64_t part_pitch,
-                     uint32_t box_rows) {
-  typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                             const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                           const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static Encode encode_fn() {
   static const Encode encode = []() -> Encode {
     void* f = nullptr;
     cudaDriverEntryPointQueryResult found;
@@ -788,10 +794,24 @@ static bool make_map(CUtensorMap* m, const void* base, uint64_t cols, uint64_t r
       return nullptr;
     return reinterpret_cast<Encode>(f);
   }();
+  return encode;
+}
+static bool make_map(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows, uint64_t parts, uint64_t pitch, uint64_t part_pitch,
+                     uint32_t box_rows) {
+  const Encode encode = encode_fn();
   const cuuint64_t dims[3] = {cols, rows, parts}, strides[2] = {pitch * 2, part_pitch * 2};
   const cuuint32_t box[3] = {64, box_rows, 1}, step[3] = {1, 1, 1};
   return encode && encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// g: boxes of 64 columns of 128 rows, or of 128 columns of 64 rows.
+static bool make_g_map(CUtensorMap* m, const void* g, uint64_t piece, uint64_t blocks, bool columns) {
+  const cuuint64_t dims[4] = {256, 4, piece / 8, blocks}, strides[3] = {512, 2048, piece * 256};
+  const cuuint32_t box[4] = {256, columns ? 2u : 4u, columns ? 16u : 8u, 1}, step[4] = {1, 1, 1, 1};
+  const Encode encode = encode_fn();
+  return encode && encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(g), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 constexpr int kPairs = 74;
@@ -802,7 +822,7 @@ constexpr size_t kPackBytes = (size_t)256 << 20;
 struct Plan {
   bool f32, pack_w, direct;
   int parts, Dp, piece, pieces;
-  int BN, BD;  // columns of a tile: of logits, of gradients
+  int BN, BD;             // columns of a tile: of logits, of gradients
   size_t N, pad;
   // workspace
   int32_t *status, *live, *counts, *idx, *tgt, *flags;
@@ -816,8 +836,7 @@ static Plan plan(const mxb_linear_ce_desc* d, const void* x, const void* weight,
   Plan q{};
   q.f32 = d->io_dtype == MXB_F32;
   q.parts = q.f32 ? 3 : 1;
-  q.BN = q.f32 ? 128 : 256;
-  q.BD = q.f32 || d->D <= 128 ? 128 : 256;
+  q.BD = d->D <= 128 ? 128 : 256;
   q.Dp = (d->D + 7) / 8 * 8;
   q.N = d->rows;
   q.pad = std::max<size_t>((q.N + 255) / 256 * 256, 256);
@@ -831,11 +850,19 @@ static Plan plan(const mxb_linear_ce_desc* d, const void* x, const void* weight,
   if (bwd && most < all && most / 256 >= round) most = most / 256 / round * round * 256;
   q.piece = (int)std::min<int64_t>(all, std::max<int64_t>(256, most / 256 * 256));
   // few tokens: a tile of 256 rows costs as much with all of them as with some (512 tokens, 32768 words of 1024: 46 us with their
-  // rows moved together first, PLACEHOLDER without)
+  // rows moved together first, 36 without)
   q.direct = !bwd && !q.pack_w && q.N <= 1024 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
   if (!bwd && !q.pack_w) q.piece = (int)all;
   q.pieces = (int)((d->V + (int64_t)q.piece - 1) / q.piece);
-  const int64_t m_tiles = q.pad / 256;
+  // float32, tiles of dx and dW: narrow ones start sooner (a third of the bytes before the first product), wide ones have fewer reads
+  // (2048 tokens, 5003 words of 448: gradients 154 us with narrow, 166 with wide ones; 4096, 32000 words: 1748 and 1560)
+  const int64_t words = std::min<int64_t>(q.piece, d->V);
+  if (q.f32 && (words + 255) / 256 * d_tiles < kPairs) q.BD = 128;
+  // float32, tiles of logits: those of 128 columns take a little over half as long as those of 256 (their operands' reads bound them), which pays
+  // where it saves as much of the last round
+  auto rounds = [&](int64_t columns) { return ((int64_t)q.pad / 256 * ((words + columns - 1) / columns) + kPairs - 1) / kPairs; };
+  q.BN = q.f32 && 115 * rounds(128) < 200 * rounds(256) ? 128 : 256;
+  const int64_t m_tiles = q.pad / 256, out_tiles = (d->D + q.BD - 1) / q.BD;
   Carver c(base);
   q.status = c.take<int32_t>(64);  // (the device's error word leads the workspace)
   q.live = c.take<int32_t>(1);
@@ -854,7 +881,7 @@ static Plan plan(const mxb_linear_ce_desc* d, const void* x, const void* weight,
     q.both = c.take<float>(q.pad);
     q.lse2 = c.take<float>(q.pad);
     q.g = c.take<bf16>((size_t)q.parts * q.pad * q.piece);
-    if (q.pieces > 1) q.sums = c.take<float>((size_t)m_tiles * d_tiles * 256 * q.BD);
+    if (q.pieces > 1) q.sums = c.take<float>((size_t)m_tiles * out_tiles * 256 * q.BD);
     for (float*& s : q.shares) s = c.take<float>((size_t)kPairs * 2 * 256 * q.BD);
   }
   q.bytes = c.bytes();
@@ -886,7 +913,7 @@ static mxb_status pack(PackP& p, int32_t* counts, cudaStream_t st) {
   return check_launch("lce_pack_kernel");
 }
 
-template <bool F32, int BD>
+template <bool F32, int BN, int BD>
 static mxb_status run(const mxb_linear_ce_desc* d, const Plan& q, PackP& pk, const void* weight, void* dweight, cudaStream_t st) {
   using T = std::conditional_t<F32, float, bf16>;
   const bool bwd = pk.d_loss != nullptr;
@@ -903,7 +930,6 @@ static mxb_status run(const mxb_linear_ce_desc* d, const Plan& q, PackP& pk, con
   }
   const size_t pad = q.pad;
   const int D = d->D;
-  constexpr int BN = F32 ? 128 : 256;
   GemmP last{};  // of the last piece's dx
   int blocks = 0;
   const int64_t m_tiles = pad / 256, d_tiles = (D + BD - 1) / BD;
@@ -931,6 +957,7 @@ static mxb_status run(const mxb_linear_ce_desc* d, const Plan& q, PackP& pk, con
     p.status = q.status;
     p.g = q.g;
     p.piece = q.piece;
+    p.blocks = (int)(pad / 128);
     p.tgt = q.tgt;
     p.idx = q.idx;
     p.v0 = v0;
@@ -941,7 +968,6 @@ static mxb_status run(const mxb_linear_ce_desc* d, const Plan& q, PackP& pk, con
     Maps maps;
     std::memset(&maps, 0, sizeof maps);
     bool ok = (q.direct ? make_map(&maps.a, pk.x, D, q.N, 1, D, q.N * D, 128) : make_map(&maps.a, q.xc, q.Dp, pad, q.parts, q.Dp, pad * q.Dp, 128)) && make_map(&maps.b, w, q.Dp, w_rows, q.parts, q.Dp, w_part, BN / 2);
-    if (bwd) ok = ok && make_map(&maps.g, q.g, q.piece, pad, q.parts, q.piece, pad * q.piece, 32);
     if (!ok) return MXB_ERR_UNSUPPORTED;
     p.N = rows;
     p.K = D;
@@ -967,7 +993,7 @@ static mxb_status run(const mxb_linear_ce_desc* d, const Plan& q, PackP& pk, con
       x.adds = piece > 0;
       x.out = pk.dx;
       x.whole = D % 8 == 0 && (reinterpret_cast<uintptr_t>(pk.dx) & 15) == 0;
-      if (!make_map(&maps.a, q.g, q.piece, pad, q.parts, q.piece, pad * q.piece, 128) || !make_map(&maps.b, w, q.Dp, w_rows, q.parts, q.Dp, w_part, 64))
+      if (!make_g_map(&maps.a, q.g, q.piece, pad / 128 * q.parts, false) || !make_map(&maps.b, w, q.Dp, w_rows, q.parts, q.Dp, w_part, 64))
         return MXB_ERR_UNSUPPORTED;
       const int64_t x_tiles = m_tiles * d_tiles, x_blocks = (rows + 63) / 64, y_tiles = (int64_t)((rows + 255) / 256) * d_tiles, y_blocks = (q.N + 63) / 64;
       const int x_pairs = pairs_for(x_tiles, x_blocks), y_pairs = pairs_for(y_tiles, y_blocks);
@@ -982,7 +1008,7 @@ static mxb_status run(const mxb_linear_ce_desc* d, const Plan& q, PackP& pk, con
       y.shares = q.shares[1];
       y.out = dweight;
       y.whole = D % 8 == 0 && (reinterpret_cast<uintptr_t>(dweight) & 15) == 0;
-      if (!make_map(&maps.a, q.g, q.piece, pad, q.parts, q.piece, pad * q.piece, 64) || !make_map(&maps.b, q.xc, q.Dp, pad, q.parts, q.Dp, pad * q.Dp, 64))
+      if (!make_g_map(&maps.a, q.g, q.piece, pad / 128 * q.parts, true) || !make_map(&maps.b, q.xc, q.Dp, pad, q.parts, q.Dp, pad * q.Dp, 64))
         return MXB_ERR_UNSUPPORTED;
       if (!F32 && y.whole && !make_map(&maps.g, dweight, D, d->V, 1, D, (uint64_t)d->V * D, 32)) return MXB_ERR_UNSUPPORTED;
       s = launch_gemm<kDw, F32, BD>(y, maps, y_pairs, st);
@@ -1002,12 +1028,19 @@ static mxb_status run(const mxb_linear_ce_desc* d, const Plan& q, PackP& pk, con
   }
   const JoinP j{q.part, q.hit, q.direct ? nullptr : q.live, q.idx, pk.targets, q.flags, q.status, pk.loss, pk.lse_out, pad, (d->V + BN - 1) / BN, (int)q.N,
                 pk.wide, d->V, blocks};
-  MXB_LAUNCH("lce_join_kernel", st, (launch_kernel(lce_join_kernel, (unsigned)(pad / 32), 256, 0, st, j)));
+  MXB_LAUNCH("lce_join_kernel", st, (launch_kernel(lce_join_kernel, (unsigned)(pad / 32), 32 * kJoinWarps, 0, st, j)));
   return check_launch("linear_ce_fwd");
 }
 static mxb_status by_shape(const mxb_linear_ce_desc* d, const Plan& q, PackP& p, const void* weight, void* dweight, cudaStream_t st) {
-  if (q.f32) return run<true, 128>(d, q, p, weight, dweight, st);
-  return q.BD == 128 ? run<false, 128>(d, q, p, weight, dweight, st) : run<false, 256>(d, q, p, weight, dweight, st);
+  auto by_width = [&](auto f32, auto bn) {
+    constexpr bool F = decltype(f32)::value;
+    constexpr int BN = decltype(bn)::value;
+    return q.BD == 128 ? run<F, BN, 128>(d, q, p, weight, dweight, st) : run<F, BN, 256>(d, q, p, weight, dweight, st);
+  };
+  constexpr std::integral_constant<int, 128> narrow;
+  constexpr std::integral_constant<int, 256> wide;
+  if (!q.f32) return by_width(std::false_type{}, wide);
+  return q.BN == 128 ? by_width(std::true_type{}, narrow) : by_width(std::true_type{}, wide);
 }
 static PackP pack_args(const mxb_linear_ce_desc* d, const Plan& q, const void* x, const void* targets) {
   PackP p{};
