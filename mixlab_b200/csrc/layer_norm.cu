@@ -53,22 +53,43 @@ __device__ __forceinline__ void centre(f2 (&h)[4], int base, int lane, int tpr, 
 // that the barrier of one sum stands between the reads of the last and the writes of the next.
 template <int TPR, int M>
 __device__ __forceinline__ void row_total(float (&v)[M], float* red) {
+  static_assert(M == 1 || M == 3, "");
+  if constexpr (TPR <= 32) {
 #pragma unroll
-  for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1)
+    for (int o = TPR / 2; o > 0; o >>= 1)
 #pragma unroll
-    for (int m = 0; m < M; ++m) v[m] += __shfl_xor_sync(0xffffffffu, v[m], o);
-  if constexpr (TPR > 32) {
-    constexpr int W = TPR / 32;
-    const int warp = threadIdx.x >> 5;
-    if ((threadIdx.x & 31) == 0)
+      for (int m = 0; m < M; ++m) v[m] += __shfl_xor_sync(0xffffffffu, v[m], o);
+  } else {
+    constexpr int W = TPR / 32, N = W * M;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if constexpr (M == 1) {
 #pragma unroll
-      for (int m = 0; m < M; ++m) red[warp * M + m] = v[m];
+      for (int o = 16; o > 0; o >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+      if (lane == 0) red[warp] = v[0];
+    } else {  // three sums in six exchanges instead of fifteen: two of them to each half of the warp, one to each quarter
+      const bool up = lane & 16, odd = lane & 8;
+      const float a = (up ? v[2] : v[0]) + __shfl_xor_sync(0xffffffffu, up ? v[0] : v[2], 16);
+      const float b = (up ? 0.f : v[1]) + __shfl_xor_sync(0xffffffffu, up ? v[1] : 0.f, 16);
+      float s = (odd ? b : a) + __shfl_xor_sync(0xffffffffu, odd ? a : b, 8);
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      if ((lane & 7) == 0 && lane < 24) red[warp * 3 + (lane >> 3)] = s;
+    }
     __syncthreads();
+    const float* from = red + warp / W * N;
+    float all[N];
+    if constexpr (N % 4 == 0) {  // (a warp of the row after the other, but read in whole pieces)
+#pragma unroll
+      for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(all + i) = *reinterpret_cast<const float4*>(from + i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) all[i] = from[i];
+    }
 #pragma unroll
     for (int m = 0; m < M; ++m) {
       float s = 0.f;
 #pragma unroll
-      for (int w = 0; w < W; ++w) s += red[(warp / W * W + w) * M + m];
+      for (int w = 0; w < W; ++w) s += all[w * M + m];
       v[m] = s;
     }
   }
@@ -78,7 +99,7 @@ __device__ __forceinline__ void row_total(float (&v)[M], float* red) {
 template <typename IO, typename RES, int TPR, int E, bool V>
 __global__ void __launch_bounds__(kThreads<TPR>) lnorm_fwd_kernel(NormP p) {
   begin_dependent();
-  __shared__ float red[2][kThreads<TPR> / 32];
+  __shared__ __align__(16) float red[2][kThreads<TPR> / 32 < 4 ? 4 : kThreads<TPR> / 32];
   constexpr int GROUPS = kThreads<TPR> / TPR;
   const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
   const float inv = 1.f / (float)p.D;
@@ -145,7 +166,7 @@ __global__ void __launch_bounds__(kThreads<TPR>) lnorm_fwd_kernel(NormP p) {
 template <typename IO, typename RES, int TPR, int E, bool V>
 __global__ void __launch_bounds__(kThreads<TPR>, TPR > 256 || E > 1 ? 1 : 2) lnorm_bwd_kernel(NormP p) {
   begin_dependent();
-  __shared__ float red[kThreads<TPR> / 32], red3[kThreads<TPR> / 32 * 3];
+  __shared__ __align__(16) float red[kThreads<TPR> / 32], red3[kThreads<TPR> / 32 * 3];
   constexpr int GROUPS = kThreads<TPR> / TPR;
   const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
   const float inv = 1.f / (float)p.D;
@@ -154,6 +175,8 @@ __global__ void __launch_bounds__(kThreads<TPR>, TPR > 256 || E > 1 ? 1 : 2) lno
   for (int e = 0; e < E; ++e)
 #pragma unroll
     for (int i = 0; i < 4; ++i) dw[e][i] = db[e][i] = 0;
+  f2 weight[4];  // (one piece of it stays in registers: read twice a row it is half of what the L1 cache delivers)
+  if (E == 1) load_cols<float, V>(p.weight, 0, lane, TPR, p.D, weight);
   Cols<RES, V> a_h[E], a_d[E];
   Cols<IO, V> a_g[E];
   auto offset = [&](size_t r0) { return (r0 + group < p.rows ? r0 + group : r0) * p.D; };
@@ -196,7 +219,12 @@ __global__ void __launch_bounds__(kThreads<TPR>, TPR > 256 || E > 1 ? 1 : 2) lno
       const int c = e * TPR * 8;
       centre<V>(h[e], c, lane, TPR, p.D, minus_m);
       f2 w[4];
-      load_cols<float, V>(p.weight, c, lane, TPR, p.D, w);
+      if constexpr (E == 1) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = weight[i];
+      } else {
+        load_cols<float, V>(p.weight, c, lane, TPR, p.D, w);
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const f2 t = mul2(g[e][i], w[i]);
@@ -213,7 +241,12 @@ __global__ void __launch_bounds__(kThreads<TPR>, TPR > 256 || E > 1 ? 1 : 2) lno
     for (int e = 0; e < E; ++e) {
       const int c = e * TPR * 8;
       f2 w[4];
-      load_cols<float, V>(p.weight, c, lane, TPR, p.D, w);
+      if constexpr (E == 1) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = weight[i];
+      } else {
+        load_cols<float, V>(p.weight, c, lane, TPR, p.D, w);
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (live) {
