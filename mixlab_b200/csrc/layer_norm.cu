@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(kThreads<TPR>) lnorm_fwd_kernel(NormP p) {
 }
 
 template <typename IO, typename RES, int TPR, int E, bool V>
-__global__ void __launch_bounds__(kThreads<TPR>, TPR > 256 || E > 1 ? 1 : 2) lnorm_bwd_kernel(NormP p) {
+__global__ void __launch_bounds__(kThreads<TPR>, TPR > 256 || E > 1 ? 1 : V && sizeof(RES) == 2 ? 3 : 2) lnorm_bwd_kernel(NormP p) {
   begin_dependent();
   __shared__ __align__(16) float red[kThreads<TPR> / 32], red3[kThreads<TPR> / 32 * 3];
   constexpr int GROUPS = kThreads<TPR> / TPR;
@@ -288,10 +288,12 @@ static RowShape row_shape(int D, bool bwd) {
   return {512, D > 8192 ? 4 : 2};
 }
 static int groups_of(int tpr) { return tpr > 256 ? 1 : 256 / tpr; }
-static int ctas(size_t rows, int D, bool bwd) {  // what the GPU holds at once
+// CTAs: what the GPU holds at once, by registers.  Forwards 4 an SM; backwards 2, or 3 where a bf16 stream comes in whole pieces (32768
+// rows of 2048 columns 105 us, with two 113), or one with two pieces a thread.
+static int ctas(size_t rows, int D, bool bwd, bool narrow) {
   const RowShape s = row_shape(D, bwd);
-  const int g = groups_of(s.tpr);
-  const size_t want = (rows + g - 1) / g, most = std::max(148, 148 * (!bwd ? 4 : s.e == 1 ? 2 : 1) * 256 / std::max(s.tpr, 256));
+  const int g = groups_of(s.tpr), each = !bwd ? 4 : s.e > 1 ? 1 : narrow && D % 8 == 0 ? 3 : 2;
+  const size_t want = (rows + g - 1) / g, most = std::max(148, 148 * each * 256 / std::max(s.tpr, 256));
   return (int)std::min(want, most);
 }
 template <typename F>
@@ -322,7 +324,7 @@ static void by_shape(int D, bool bwd, F&& f) {
 template <typename IO, typename RES, bool V>
 static mxb_status run(const NormP& p, float* dweight, float* dbias, cudaStream_t st) {
   const bool bwd = p.dn != nullptr;
-  const int n = ctas(p.rows, p.D, bwd);
+  const int n = ctas(p.rows, p.D, bwd, sizeof(RES) == 2);
   int parts = 0;
   by_shape(p.D, bwd, [&](auto tpr, auto e) {
     constexpr int TPR = decltype(tpr)::value, E = decltype(e)::value;
@@ -364,7 +366,7 @@ static mxb_status by_type(const mxb_layer_norm_desc* d, const NormP& p, float* d
 
 size_t layer_norm_scratch(const mxb_layer_norm_desc* d) {
   const int tpr = lnorm::row_shape(d->D, true).tpr;
-  return (size_t)lnorm::ctas(d->rows, d->D, true) * lnorm::groups_of(tpr) * 2 * d->D * sizeof(float);
+  return (size_t)lnorm::ctas(d->rows, d->D, true, d->resid_dtype == MXB_BF16) * lnorm::groups_of(tpr) * 2 * d->D * sizeof(float);
 }
 mxb_status layer_norm_fwd(const mxb_layer_norm_desc* d, const void* resid, const void* x, const float* weight, const float* bias, void* stream,
                           void* n, cudaStream_t st) {
