@@ -77,22 +77,34 @@ __global__ void __launch_bounds__(256) embedding_fwd_kernel(FwdP p, int tpr) {
 constexpr int kTile = 2048, kSortThreads = 256, kWarps = kSortThreads / 32, kEach = kTile / kSortThreads, kMaxDigits = 1024;
 struct SortP {
   const void* tokens;
-  const int32_t *key_in, *pos_in;  // null in the first pass
-  int32_t *key_out, *pos_out;
+  const int2* in;                  // tokens and their positions; null in the first pass
+  int2* out;
   int32_t* hist;                   // [digits][tiles]
   uint32_t* rows;                  // the first pass sets it to zero
-  int N, V, shift, digits, tiles;
+  int N, V, shift, digits, bits, tiles;
 };
 template <typename TOK>
 __device__ __forceinline__ int key_at(const SortP& p, int i) {
-  return p.key_in ? p.key_in[i] : token_of(static_cast<const TOK*>(p.tokens), i, p.V);
+  return p.in ? p.in[i].x : token_of(static_cast<const TOK*>(p.tokens), i, p.V);
+}
+// The lanes of the warp whose digits (of so many bits) are this lane's; in: which lanes have one.  (By __match_any_sync, which takes
+// the longer the more digits there are, 4096 entries' ranks take 7800 cycles, so 2600.)
+__device__ __forceinline__ uint32_t same_digit(int d, int bits, bool in) {
+  uint32_t peers = __ballot_sync(0xffffffffu, in);
+#pragma unroll
+  for (int b = 0; b < 10; ++b) {
+    if (b >= bits) break;
+    const uint32_t m = __ballot_sync(0xffffffffu, d >> b & 1);
+    peers &= d >> b & 1 ? m : ~m;
+  }
+  return peers;
 }
 template <typename TOK>
 __global__ void __launch_bounds__(kSortThreads) embedding_count_kernel(SortP p) {
   begin_dependent();
   __shared__ int32_t count[kMaxDigits];
   for (int d = threadIdx.x; d < p.digits; d += kSortThreads) count[d] = 0;
-  if (!p.key_in)
+  if (!p.in)
     for (int64_t w = (int64_t)blockIdx.x * kSortThreads + threadIdx.x; w <= p.V / 32; w += (int64_t)gridDim.x * kSortThreads) p.rows[w] = 0;
   __syncthreads();
 #pragma unroll
@@ -175,8 +187,8 @@ __global__ void __launch_bounds__(kSortThreads) embedding_place_kernel(SortP p, 
     const int64_t i = first + 32 * k;
     const bool in = i < p.N;
     key[k] = in ? key_at<TOK>(p, (int)i) : -1;
-    const int d = in ? (key[k] >> p.shift) & (p.digits - 1) : kMaxDigits;
-    const uint32_t peers = __match_any_sync(0xffffffffu, d);
+    const int d = in ? (key[k] >> p.shift) & (p.digits - 1) : 0;
+    const uint32_t peers = same_digit(d, p.bits, in);
     rank[k] = 0;
     if (in) rank[k] = mine[warp][d] + __popc(peers & ((1u << lane) - 1u));
     __syncwarp();
@@ -199,26 +211,26 @@ __global__ void __launch_bounds__(kSortThreads) embedding_place_kernel(SortP p, 
     const int64_t i = first + 32 * k;
     if (i >= p.N) continue;
     const int d = (key[k] >> p.shift) & (p.digits - 1), to = place[d] + mine[warp][d] + rank[k];
-    p.key_out[to] = key[k];
-    p.pos_out[to] = p.pos_in ? p.pos_in[i] : (int)i;
+    p.out[to] = make_int2(key[k], p.in ? p.in[i].y : (int)i);
   }
 }
 
 // A bit for each token that occurs, by its first entry in sorted order.  (By every entry, words of frequent tokens are updated so
 // often that the updates, one after the other, took 20 us of 32768 tokens.)
-__device__ __forceinline__ void mark_first(const int32_t* key, int i, uint32_t* rows) {
-  const int k = key[i];
-  if (i == 0 || key[i - 1] != k) atomicOr(rows + k / 32, 1u << (k & 31));
+__device__ __forceinline__ void mark_first(const int2* entry, int i, uint32_t* rows) {
+  const int k = entry[i].x;
+  if (i == 0 || entry[i - 1].x != k) atomicOr(rows + k / 32, 1u << (k & 31));
 }
-__global__ void __launch_bounds__(256) embedding_mark_kernel(const int32_t* key, int N, uint32_t* rows) {
+__global__ void __launch_bounds__(256) embedding_mark_kernel(const int2* entry, int N, uint32_t* rows) {
   begin_dependent();
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i < N) mark_first(key, (int)i, rows);
+  if (i < N) mark_first(entry, (int)i, rows);
 }
 
 // The whole sort in one launch for up to kClusterEntries entries: a cluster of CTAs, each with an equal share of the entries, that read
-// each other's digit counts through distributed shared memory.  (2047 entries, five launches: 19.8 us for the gradient, of which
-// 15 are the sort's three.)
+// each other's digit counts through distributed shared memory.  A CTA sorts its entries by the digit in its own memory first, so that
+// it writes runs of neighbours: entries written one by one from their places in the warps were 6 to 8 thousand of 27 thousand
+// cycles a pass of 32768 entries.  (The gradient of 2047 tokens with a sort of three launches 19.8 us, of 32768 155 us, so 16 and 139.)
 constexpr int kClusterThreads = 1024, kClusterEach = 8, kClusterMost = 8, kClusterEntries = kClusterThreads * kClusterEach * kClusterMost;
 __device__ __forceinline__ int32_t of_cta(const int32_t* p, uint32_t rank) {
   int32_t v;
@@ -227,47 +239,54 @@ __device__ __forceinline__ int32_t of_cta(const int32_t* p, uint32_t rank) {
 }
 struct ClusterP {
   const void* tokens;
-  int32_t *key[2], *pos[2];
+  int2* entry[2];
   uint32_t* rows;
   int N, V, bits, passes, share;  // share: entries of a CTA
 };
+__device__ __forceinline__ int warp_scan(int v, int lane) {  // inclusive
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
 template <typename TOK>
 __global__ void __launch_bounds__(kClusterThreads) embedding_sort_kernel(ClusterP p) {
   begin_dependent();
-  extern __shared__ uint16_t mine[];  // [32 warps][digits]
-  __shared__ int32_t hist[kMaxDigits], place[kMaxDigits], sums[32];
+  extern __shared__ int2 local[];  // [share] entries by digit, then counts of the warps [32][digits]
+  __shared__ int32_t hist[kMaxDigits], place[kMaxDigits], inside[kMaxDigits], sums[2][32];
+  uint16_t* mine = reinterpret_cast<uint16_t*>(local + p.share);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, digits = 1 << p.bits, ctas = gridDim.x, rank = tc::cluster_rank();
   const int each = (p.share + kClusterThreads - 1) / kClusterThreads;  // rounds of 32 consecutive entries a warp
-  const int begin = rank * p.share, end = min(begin + p.share, p.N), first = begin + warp * 32 * each + lane;
+  const int begin = min(rank * p.share, p.N), end = min(begin + p.share, p.N), first = begin + warp * 32 * each + lane;
   for (int64_t w = (int64_t)rank * kClusterThreads + threadIdx.x; w <= p.V / 32; w += (int64_t)ctas * kClusterThreads) p.rows[w] = 0;
   for (int pass = 0; pass < p.passes; ++pass) {
     const int shift = pass * p.bits;
     const bool odd = pass & 1;
-    const int32_t *key_in = odd ? p.key[0] : p.key[1], *pos_in = odd ? p.pos[0] : p.pos[1];
-    int32_t *key_out = odd ? p.key[1] : p.key[0], *pos_out = odd ? p.pos[1] : p.pos[0];
-    for (int d = threadIdx.x; d < 16 * digits; d += kClusterThreads) reinterpret_cast<uint32_t*>(mine)[d] = 0;
-    int key[kClusterEach], pos[kClusterEach], at[kClusterEach];
+    const int2* in = odd ? p.entry[0] : p.entry[1];
+    int2* out = odd ? p.entry[1] : p.entry[0];
+    int2 entry[kClusterEach];
+    int at[kClusterEach];
 #pragma unroll
     for (int k = 0; k < kClusterEach; ++k) {
       const int i = first + 32 * k;
-      key[k] = -1;
-      if (k < each && i < end) {
-        key[k] = pass ? key_in[i] : token_of(static_cast<const TOK*>(p.tokens), i, p.V);
-        pos[k] = pass ? pos_in[i] : i;
-      }
+      entry[k] = make_int2(-1, 0);
+      if (k < each && i < end) entry[k] = pass ? in[i] : make_int2(token_of(static_cast<const TOK*>(p.tokens), i, p.V), i);
     }
+    for (int d = threadIdx.x; d < 16 * digits; d += kClusterThreads) reinterpret_cast<uint32_t*>(mine)[d] = 0;
     __syncthreads();
     uint16_t* own = mine + warp * digits;
 #pragma unroll
     for (int k = 0; k < kClusterEach; ++k) {
       if (k >= each) break;
-      const bool in = key[k] >= 0;
-      const int d = in ? key[k] >> shift & digits - 1 : kMaxDigits;
-      const uint32_t peers = __match_any_sync(0xffffffffu, d);
+      const bool has = entry[k].x >= 0;
+      const int d = has ? entry[k].x >> shift & digits - 1 : 0;
+      const uint32_t peers = same_digit(d, p.bits, has);
       at[k] = 0;
-      if (in) at[k] = own[d] + __popc(peers & ((1u << lane) - 1u));
+      if (has) at[k] = own[d] + __popc(peers & ((1u << lane) - 1u));
       __syncwarp();
-      if (in && (peers >> lane) == 1u) own[d] = (uint16_t)(at[k] + 1);  // the last of its digit in the warp
+      if (has && (peers >> lane) == 1u) own[d] = (uint16_t)(at[k] + 1);  // the last of its digit in the warp
       __syncwarp();
     }
     __syncthreads();
@@ -287,8 +306,8 @@ __global__ void __launch_bounds__(kClusterThreads) embedding_sort_kernel(Cluster
       hist[d] = before;
     }
     tc::cluster_sync();
-    // places of the digits: those in front (an exclusive sum over the cluster's totals), CTAs in front
-    int before = 0, total = 0;
+    // places of the digits: those in front (an exclusive sum over the cluster's totals) and CTAs in front; likewise in this CTA alone
+    int before = 0, total = 0, here = 0;
     if ((int)threadIdx.x < digits) {
       int n[kClusterMost];
 #pragma unroll
@@ -298,44 +317,44 @@ __global__ void __launch_bounds__(kClusterThreads) embedding_sort_kernel(Cluster
         if (r < rank) before += n[r];
         total += n[r];
       }
+      here = hist[threadIdx.x];
     }
-    int s = total;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += u;
-    }
-    if (lane == 31) sums[warp] = s;
-    __syncthreads();
-    if (warp == 0) {
-      int v = sums[lane];
-      const int own_sum = v;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += u;
-      }
-      sums[lane] = v - own_sum;
+    const int all = warp_scan(total, lane), own_all = warp_scan(here, lane);
+    if (lane == 31) {
+      sums[0][warp] = all;
+      sums[1][warp] = own_all;
     }
     __syncthreads();
-    if ((int)threadIdx.x < digits) place[threadIdx.x] = sums[warp] + s - total + before;
+    if (warp < 2) {
+      const int v = sums[warp][lane];
+      sums[warp][lane] = warp_scan(v, lane) - v;
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < digits) {
+      inside[threadIdx.x] = sums[1][warp] + own_all - here;
+      place[threadIdx.x] = sums[0][warp] + all - total + before - inside[threadIdx.x];  // (of an entry's place in this CTA)
+    }
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kClusterEach; ++k) {
-      if (k >= each || key[k] < 0) continue;
-      const int d = key[k] >> shift & digits - 1, to = place[d] + own[d] + at[k];
-      key_out[to] = key[k];
-      pos_out[to] = pos[k];
+      if (k >= each || entry[k].x < 0) continue;
+      const int d = entry[k].x >> shift & digits - 1;
+      local[inside[d] + own[d] + at[k]] = entry[k];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < end - begin; i += kClusterThreads) {
+      const int2 e = local[i];
+      out[place[e.x >> shift & digits - 1] + i] = e;
+      // (a token's entries are neighbours now in every CTA that has some)
+      if (pass + 1 == p.passes) mark_first(local, i, p.rows);
     }
     tc::cluster_sync();  // (the entries are in place, the counts have been read)
   }
-  const int32_t* key = p.passes & 1 ? p.key[0] : p.key[1];
-  for (int i = rank * kClusterThreads + threadIdx.x; i < p.N; i += ctas * kClusterThreads) mark_first(key, i, p.rows);
 }
 
 // ------------------------------------------------------------------ sums
 struct SumP {
-  const int32_t *key, *pos;  // sorted; padding (key V) stands at the end
+  const int2* entry;         // tokens and positions, sorted; padding (token V) stands at the end
   const uint32_t* rows;      // a bit for each row of dW: its token occurs
   const void* d_out;
   void* dweight;
@@ -378,9 +397,9 @@ __global__ void __launch_bounds__(256, V ? 4 : 2) embedding_bwd_kernel(SumP p, i
   const int64_t begin = (int64_t)blockIdx.x * groups * p.run;
   for (int k = threadIdx.x; k < groups * (p.run + 2); k += 256) {
     const int64_t i = begin + (int64_t)(k / (p.run + 2)) * p.run + k % (p.run + 2) - 1;
-    entries[k] = i >= 0 && i < p.N ? p.key[i] : -1;
+    entries[k] = i >= 0 && i < p.N ? p.entry[i].x : -1;
   }
-  for (int k = threadIdx.x; k < groups * p.run; k += 256) entries[groups * (p.run + 2) + k] = begin + k < p.N ? p.pos[begin + k] : 0;
+  for (int k = threadIdx.x; k < groups * p.run; k += 256) entries[groups * (p.run + 2) + k] = begin + k < p.N ? p.entry[begin + k].y : 0;
   __syncthreads();
   const int64_t run = (int64_t)blockIdx.x * groups + group, i0 = run * p.run;
   if (i0 >= p.N) return;
@@ -454,14 +473,14 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(SumP p) {
   __syncthreads();
   const int64_t begin = (int64_t)run * p.run, end = begin + p.run;
   if (end < p.N) {
-    const int tok = p.key[end];
-    const bool starts = tok < p.V && p.key[end - 1] == tok && !(run > 0 && p.key[begin] == tok && p.key[begin - 1] == tok);
+    const int tok = p.entry[end].x;
+    const bool starts = tok < p.V && p.entry[end - 1].x == tok && !(run > 0 && p.entry[begin].x == tok && p.entry[begin - 1].x == tok);
     if (starts) {
       int lo = (int)end, hi = p.N;  // the first entry behind the token's
-      if (end + p.run < p.N && p.key[end + p.run] != tok) hi = (int)end + p.run;
+      if (end + p.run < p.N && p.entry[end + p.run].x != tok) hi = (int)end + p.run;
       while (lo < hi) {
         const int mid = lo + (hi - lo) / 2;
-        if (p.key[mid] <= tok) lo = mid + 1;
+        if (p.entry[mid].x <= tok) lo = mid + 1;
         else hi = mid;
       }
       const int n = (lo - 1) / p.run - run;  // partial rows besides the first
@@ -507,7 +526,8 @@ static int run_length(int64_t N, int D) {
   return (int)std::min<int64_t>(32, std::max<int64_t>(8, (want + 7) / 8 * 8));
 }
 struct Scratch {
-  int32_t *key[2], *pos[2], *hist, *total;
+  int2* entry[2];
+  int32_t *hist, *total;
   uint32_t* rows;
   float* part;
   size_t bytes;
@@ -524,10 +544,7 @@ static Scratch carve(const mxb_embedding_desc* d, void* base) {
   s.run = run_length(N, d->D);
   s.runs = (int)((N + s.run - 1) / s.run);
   s.tiles = (int)((N + kTile - 1) / kTile);
-  for (int i = 0; i < 2; ++i) {
-    s.key[i] = c.take<int32_t>(N);
-    s.pos[i] = c.take<int32_t>(N);
-  }
+  for (int2*& e : s.entry) e = c.take<int2>(N);
   s.rows = c.take<uint32_t>((size_t)d->V / 32 + 1);
   s.hist = c.take<int32_t>(((size_t)1 << s.bits) * s.tiles);
   s.total = c.take<int32_t>((size_t)1 << s.bits);
@@ -587,12 +604,12 @@ mxb_status embedding_bwd(const mxb_embedding_desc* d, const void* tokens, const 
     // about four entries a thread
     int ctas = 1;
     while (ctas < kClusterMost && (int64_t)ctas * kClusterThreads * 4 < d->tokens) ctas *= 2;
-    const ClusterP q{tokens, {s.key[0], s.key[1]}, {s.pos[0], s.pos[1]}, s.rows, (int)d->tokens, d->V, s.bits, s.passes, (int)((d->tokens + ctas - 1) / ctas)};
+    const ClusterP q{tokens, {s.entry[0], s.entry[1]}, s.rows, (int)d->tokens, d->V, s.bits, s.passes, (int)((d->tokens + ctas - 1) / ctas)};
     mxb_status st_ = MXB_OK;
     with_token(d, [&](auto tok) {
       using TOK = decltype(tok);
-      const int smem = 32 * 2 << s.bits;
-      st_ = MXB_ALLOW_SMEM(64 * kMaxDigits, embedding_sort_kernel<TOK>);
+      const int smem = q.share * (int)sizeof(int2) + (64 << s.bits);
+      st_ = MXB_ALLOW_SMEM(kClusterThreads * kClusterEach * (int)sizeof(int2) + 64 * kMaxDigits, embedding_sort_kernel<TOK>);
       if (st_ != MXB_OK) return;
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = ctas;
@@ -611,24 +628,22 @@ mxb_status embedding_bwd(const mxb_embedding_desc* d, const void* tokens, const 
     });
     if (st_ != MXB_OK) return st_;
   } else {
-    SortP q{tokens, nullptr, nullptr, nullptr, nullptr, s.hist, s.rows, (int)d->tokens, d->V, 0, 1 << s.bits, s.tiles};
+    SortP q{tokens, nullptr, nullptr, s.hist, s.rows, (int)d->tokens, d->V, 0, 1 << s.bits, s.bits, s.tiles};
     for (int pass = 0; pass < s.passes; ++pass) {
       q.shift = pass * s.bits;
-      q.key_out = s.key[pass & 1];
-      q.pos_out = s.pos[pass & 1];
+      q.out = s.entry[pass & 1];
       with_token(d, [&](auto tok) {
         using TOK = decltype(tok);
         MXB_LAUNCH("embedding_count_kernel", st, (launch_kernel(embedding_count_kernel<TOK>, s.tiles, kSortThreads, 0, st, q)));
         MXB_LAUNCH("embedding_scan_kernel", st, (launch_kernel(embedding_scan_kernel, 1 << s.bits, 256, 0, st, s.hist, s.total, s.tiles)));
         MXB_LAUNCH("embedding_place_kernel", st, (launch_kernel(embedding_place_kernel<TOK>, s.tiles, kSortThreads, 0, st, q, s.total)));
       });
-      q.key_in = q.key_out;
-      q.pos_in = q.pos_out;
+      q.in = q.out;
     }
     MXB_LAUNCH("embedding_mark_kernel", st,
-               (launch_kernel(embedding_mark_kernel, (unsigned)((d->tokens + 255) / 256), 256, 0, st, s.key[last], (int)d->tokens, s.rows)));
+               (launch_kernel(embedding_mark_kernel, (unsigned)((d->tokens + 255) / 256), 256, 0, st, s.entry[last], (int)d->tokens, s.rows)));
   }
-  const SumP p{s.key[last], s.pos[last], s.rows, d_out, dweight, s.part, (int)d->tokens, d->V, d->D, s.run, s.runs, adds, d->scale};
+  const SumP p{s.entry[last], s.rows, d_out, dweight, s.part, (int)d->tokens, d->V, d->D, s.run, s.runs, adds, d->scale};
   const int tpr = threads_per_row(d->D), groups = 256 / tpr, sums = (s.runs + groups - 1) / groups;
   const int zeros = adds ? 0 : (int)(((int64_t)d->V + kZeroRows - 1) / kZeroRows);
   with_type(d->io_dtype, [&](auto in) {

@@ -248,7 +248,7 @@ __device__ __forceinline__ int live_of(const GemmP& p) { return p.live ? *p.live
 struct Wait {
   volatile int32_t* bad;
   __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) const {
-    for (uint32_t i = 0; i < 1000000u; ++i) {
+    for (uint32_t i = 0; i < 4000000u; ++i) {
       if (tc::mbar_try_wait(bar, parity)) return true;
       if ((i & 63u) == 63u && *bad) return false;
     }
@@ -420,7 +420,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
   Item t;
   const Wait wait{bad};
   // blocks of K behind which an accumulator is handed over
-  constexpr int SEG = F32 ? 2 : 1 << 30;
+  // (bf16: 65536 terms, of which a cut accumulator may lose 4096 x 2^-23, half of the 2^-10 that a bf16 result's rounding takes)
+  constexpr int SEG = F32 ? 2 : 1024;
 
   if (warp == 8) {
     // ---- copies: each CTA its half of A and B, counted by the barrier of the CTA that issues the products
@@ -528,7 +529,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
         __syncwarp();
         tc::fence_after_sync();
         const uint32_t d = tmem + lanes + acc * BN + half * C::COLS;
-        if constexpr (!F32) {
+        if (!F32 && ks == k0) {
 #pragma unroll
           for (int c = 0; c < C::COLS; c += 32) {
             uint32_t(&r)[32] = reinterpret_cast<uint32_t(&)[32]>(v[c]);
