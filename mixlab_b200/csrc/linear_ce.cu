@@ -217,7 +217,7 @@ struct Cfg {
   static constexpr int ACCS = 512 / BN, RING = 2 * ACCS;  // accumulators in TMEM; kStats: slots for what halves of a tile exchange
   static constexpr int SMEM = 1024 + STAGES * STAGE + STAGING + 256 + (MODE == kStats ? RING * (4 * 8 + 128 * 8) : 0);
 };
-constexpr int kThreads = 320;
+constexpr int kThreads = 384;  // eight warps of the epilogue, one for copies, one for products, two that fill up their warpgroup
 struct GemmP {
   const int32_t* live;    // null: rows tokens, none left out
   const void* targets;    //   their targets (wide: of 64 bits)
@@ -423,85 +423,90 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
   // (bf16: 65536 terms, of which a cut accumulator may lose 4096 x 2^-23, half of the 2^-10 that a bf16 result's rounding takes)
   constexpr int SEG = F32 ? 2 : 1024;
 
-  if (warp == 8) {
-    // ---- copies: each CTA its half of A and B, counted by the barrier of the CTA that issues the products
-    if (tc::elect_one()) {
-      int s = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int j = 0; ok && walk.item(pair, j, t); ++j) {
-        for (int kb = t.k0; kb < t.k1; ++kb) {
-          if (!(ok = wait(empty + s, phase ^ 1u))) break;
-          if (rank == 0) tc::mbar_expect_tx(full + s, 2 * C::STAGE);
-          const uint32_t bar = tc::in_cta(tc::smem_u32(full + s), 0);
-          uint32_t to = base + s * C::STAGE;
-#pragma unroll
-          for (int part = 0; part < C::PARTS; ++part, to += C::A) {
-            const int m0 = t.m * 256 + (int)rank * 128;
-            if (MODE == kDx) tc::tma_load_4d_pair(to, &maps.a, 0, 0, kb * 8, part * p.blocks + m0 / 128, bar);
-            else if (MODE == kDw) tc::tma_load_4d_pair(to, &maps.a, 0, (kb & 1) * 2, m0 / 8, part * p.blocks + kb / 2, bar);
-            else tc::tma_load_3d_pair(to, &maps.a, kb * 64, m0, part, bar);
-          }
-#pragma unroll
-          for (int part = 0; part < C::PARTS; ++part, to += C::B) {
-            const int n0 = t.n * C::BN + (int)rank * (C::BN / 2);
-            if (C::B_MN) {
-#pragma unroll
-              for (int x = 0; x < C::BN / 128; ++x) tc::tma_load_3d_pair(to + x * 8192, &maps.b, n0 + 64 * x, p.b_row0 + kb * 64, part, bar);
-            } else {
-              tc::tma_load_3d_pair(to, &maps.b, kb * 64, p.b_row0 + n0, part, bar);
+  // Registers: the epilogue holds a row's 128 columns beside what it does with them; 256 x 232 + 128 x 40 are the 384 x 168 of the launch.
+  if (warp >= 8) {
+    tc::reg_dec<40>();
+    if (warp == 8) {
+      // ---- copies: each CTA its half of A and B, counted by the barrier of the CTA that issues the products
+      if (tc::elect_one()) {
+        int s = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int j = 0; ok && walk.item(pair, j, t); ++j) {
+          for (int kb = t.k0; kb < t.k1; ++kb) {
+            if (!(ok = wait(empty + s, phase ^ 1u))) break;
+            if (rank == 0) tc::mbar_expect_tx(full + s, 2 * C::STAGE);
+            const uint32_t bar = tc::in_cta(tc::smem_u32(full + s), 0);
+            uint32_t to = base + s * C::STAGE;
+  #pragma unroll
+            for (int part = 0; part < C::PARTS; ++part, to += C::A) {
+              const int m0 = t.m * 256 + (int)rank * 128;
+              if (MODE == kDx) tc::tma_load_4d_pair(to, &maps.a, 0, 0, kb * 8, part * p.blocks + m0 / 128, bar);
+              else if (MODE == kDw) tc::tma_load_4d_pair(to, &maps.a, 0, (kb & 1) * 2, m0 / 8, part * p.blocks + kb / 2, bar);
+              else tc::tma_load_3d_pair(to, &maps.a, kb * 64, m0, part, bar);
             }
-          }
-          if (++s == C::STAGES) { s = 0; phase ^= 1u; }
-        }
-      }
-    }
-  } else if (warp == 9) {
-    // ---- products, by one thread of the pair
-    if (rank == 0 && tc::elect_one()) {
-      constexpr uint32_t idesc = tc::make_idesc_bf16(256, C::BN, C::A_MN, C::B_MN);
-      constexpr uint32_t a_step = MODE == kDx ? 4096 : MODE == kDw ? 256 : 32, b_step = C::B_MN ? 2048 : 32;
-      int s = 0, acc = 0;
-      uint32_t phase = 0, acc_phase = 0;
-      bool ok = true;
-      for (int j = 0; ok && walk.item(pair, j, t); ++j) {
-        const int k1 = t.k1;
-        for (int ks = t.k0; ok && ks < k1; ks += SEG) {
-          if (!(ok = wait(acc_empty + acc, acc_phase ^ 1u))) break;
-          tc::fence_after_sync();
-          const uint32_t d = tmem + acc * BN;
-          const int ke = min(ks + min(SEG, k1 - ks), k1);
-          for (int kb = ks; kb < ke; ++kb) {
-            if (!(ok = wait(full + s, phase))) break;
-            tc::fence_after_sync();
-            const uint32_t sa = base + s * C::STAGE, sb = sa + C::PARTS * C::A;
-            auto product = [&](int pa, int pb, bool first) {
-              const uint64_t da = MODE == kDx   ? tc::make_smem_desc(sa + pa * C::A, 2048, 128, tc::kSwizzleNone)
-                                  : MODE == kDw ? tc::make_smem_desc(sa + pa * C::A, 128, 1024, tc::kSwizzleNone)
-                                                : tc::make_smem_desc(sa + pa * C::A, 16, 1024, tc::kSwizzle128);
-              const uint64_t db = tc::make_smem_desc(sb + pb * C::B, C::B_MN ? 8192 : 16, 1024, tc::kSwizzle128);
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                tc::mma_pair(d, da + (uint64_t)((k * a_step) >> 4), db + (uint64_t)((k * b_step) >> 4), idesc, !(first && k == 0));
-            };
-            if (F32) {
-              product(2, 0, kb == ks);
-              product(0, 2, false);
-              product(1, 1, false);
-              product(1, 0, false);
-              product(0, 1, false);
+  #pragma unroll
+            for (int part = 0; part < C::PARTS; ++part, to += C::B) {
+              const int n0 = t.n * C::BN + (int)rank * (C::BN / 2);
+              if (C::B_MN) {
+  #pragma unroll
+                for (int x = 0; x < C::BN / 128; ++x) tc::tma_load_3d_pair(to + x * 8192, &maps.b, n0 + 64 * x, p.b_row0 + kb * 64, part, bar);
+              } else {
+                tc::tma_load_3d_pair(to, &maps.b, kb * 64, p.b_row0 + n0, part, bar);
+              }
             }
-            product(0, 0, !F32 && kb == ks);
-            tc::mma_commit_pair(empty + s);
             if (++s == C::STAGES) { s = 0; phase ^= 1u; }
           }
-          if (!ok) break;
-          tc::mma_commit_pair(acc_full + acc);
-          if (++acc == C::ACCS) { acc = 0; acc_phase ^= 1u; }
+        }
+      }
+    } else if (warp == 9) {
+      // ---- products, by one thread of the pair
+      if (rank == 0 && tc::elect_one()) {
+        constexpr uint32_t idesc = tc::make_idesc_bf16(256, C::BN, C::A_MN, C::B_MN);
+        constexpr uint32_t a_step = MODE == kDx ? 4096 : MODE == kDw ? 256 : 32, b_step = C::B_MN ? 2048 : 32;
+        int s = 0, acc = 0;
+        uint32_t phase = 0, acc_phase = 0;
+        bool ok = true;
+        for (int j = 0; ok && walk.item(pair, j, t); ++j) {
+          const int k1 = t.k1;
+          for (int ks = t.k0; ok && ks < k1; ks += SEG) {
+            if (!(ok = wait(acc_empty + acc, acc_phase ^ 1u))) break;
+            tc::fence_after_sync();
+            const uint32_t d = tmem + acc * BN;
+            const int ke = min(ks + min(SEG, k1 - ks), k1);
+            for (int kb = ks; kb < ke; ++kb) {
+              if (!(ok = wait(full + s, phase))) break;
+              tc::fence_after_sync();
+              const uint32_t sa = base + s * C::STAGE, sb = sa + C::PARTS * C::A;
+              auto product = [&](int pa, int pb, bool first) {
+                const uint64_t da = MODE == kDx   ? tc::make_smem_desc(sa + pa * C::A, 2048, 128, tc::kSwizzleNone)
+                                    : MODE == kDw ? tc::make_smem_desc(sa + pa * C::A, 128, 1024, tc::kSwizzleNone)
+                                                  : tc::make_smem_desc(sa + pa * C::A, 16, 1024, tc::kSwizzle128);
+                const uint64_t db = tc::make_smem_desc(sb + pb * C::B, C::B_MN ? 8192 : 16, 1024, tc::kSwizzle128);
+  #pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  tc::mma_pair(d, da + (uint64_t)((k * a_step) >> 4), db + (uint64_t)((k * b_step) >> 4), idesc, !(first && k == 0));
+              };
+              if (F32) {
+                product(2, 0, kb == ks);
+                product(0, 2, false);
+                product(1, 1, false);
+                product(1, 0, false);
+                product(0, 1, false);
+              }
+              product(0, 0, !F32 && kb == ks);
+              tc::mma_commit_pair(empty + s);
+              if (++s == C::STAGES) { s = 0; phase ^= 1u; }
+            }
+            if (!ok) break;
+            tc::mma_commit_pair(acc_full + acc);
+            if (++acc == C::ACCS) { acc = 0; acc_phase ^= 1u; }
+          }
         }
       }
     }
   } else {
+    tc::reg_inc<232>();
     // ---- epilogue: a thread has a row of the CTA's 128 and half of the tile's columns
     const int half = warp >> 2, quarter = warp & 3, mine = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
