@@ -419,9 +419,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
   const Walk walk(p, MODE, C::BN, pairs);
   Item t;
   const Wait wait{bad};
-  // blocks of K behind which an accumulator is handed over
-  // (bf16: 65536 terms, of which a cut accumulator may lose 4096 x 2^-23, half of the 2^-10 that a bf16 result's rounding takes)
-  constexpr int SEG = F32 ? 2 : 1024;
+  // Blocks of K behind which an accumulator is handed over.  bf16: a cut accumulator loses up to 2^-23 of itself with every 16 terms,
+  // 2^-16 over the 2048 of a logit's part (which exponentials see as they are), 2^-11 over 65536 of a gradient's, which a rounding to
+  // bf16 (2^-9) follows.
+  constexpr int SEG = F32 ? 2 : MODE == kStats || MODE == kGrad ? 32 : 1024;
 
   // Registers: the epilogue holds a row's 128 columns beside what it does with them; 256 x 232 + 128 x 40 are the 384 x 168 of the launch.
   if (warp >= 8) {
