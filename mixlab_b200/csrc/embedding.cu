@@ -227,10 +227,50 @@ __global__ void __launch_bounds__(256) embedding_mark_kernel(const int2* entry, 
   if (i < N) mark_first(entry, (int)i, rows);
 }
 
+// Few entries: every block reads all tokens and counts, for 32 entries, those that stand in front, eight threads an entry; its part of
+// the bits that say which tokens occur likewise.  (Gradients of 2047 tokens, 257 words of
+// 448 columns 13.8 us, with the sort in a cluster 15.9; of 3000, 50000 words of 1024 columns 52 and 58; of 8000, 1000 words 34 and 23.)
+constexpr int kRankMost = 4096;
+template <typename TOK>
+__global__ void __launch_bounds__(256) embedding_rank_kernel(const void* tokens, int2* out, uint32_t* rows, int N, int V) {
+  begin_dependent();
+  __shared__ __align__(16) int32_t key[kRankMost];
+  __shared__ uint32_t bits[256];
+  const int most = (N + 31) / 32 * 32;
+  for (int i = threadIdx.x; i < most; i += 256) key[i] = i < N ? token_of(static_cast<const TOK*>(tokens), i, V) : INT32_MAX;
+  __syncthreads();
+  const int i = blockIdx.x * 32 + threadIdx.x / 8, sub = threadIdx.x & 7;
+  if (blockIdx.x * 32 < N) {
+    const int k = i < N ? key[i] : -1;
+    int before = 0;
+    for (int j = sub * 4; j < most; j += 32) {
+      const int4 o = *reinterpret_cast<const int4*>(key + j);
+      before += (o.x < k || (o.x == k && j < i)) + (o.y < k || (o.y == k && j + 1 < i)) + (o.z < k || (o.z == k && j + 2 < i)) +
+                (o.w < k || (o.w == k && j + 3 < i));
+    }
+    before += __shfl_xor_sync(0xffffffffu, before, 1);
+    before += __shfl_xor_sync(0xffffffffu, before, 2);
+    before += __shfl_xor_sync(0xffffffffu, before, 4);
+    if (sub == 0 && i < N) out[before] = make_int2(k, i);
+  }
+  const int64_t words = (int64_t)V / 32 + 1;
+  for (int64_t w0 = (int64_t)blockIdx.x * 256; w0 < words; w0 += (int64_t)gridDim.x * 256) {
+    __syncthreads();
+    bits[threadIdx.x] = 0;
+    __syncthreads();
+    for (int j = threadIdx.x; j < N; j += 256) {
+      const int64_t w = key[j] / 32 - w0;
+      if (w >= 0 && w < 256) atomicOr(&bits[w], 1u << (key[j] & 31));
+    }
+    __syncthreads();
+    if (w0 + threadIdx.x < words) rows[w0 + threadIdx.x] = bits[threadIdx.x];
+  }
+}
+
 // The whole sort in one launch for up to kClusterEntries entries: a cluster of CTAs, each with an equal share of the entries, that read
 // each other's digit counts through distributed shared memory.  A CTA sorts its entries by the digit in its own memory first, so that
 // it writes runs of neighbours: entries written one by one from their places in the warps were 6 to 8 thousand of 27 thousand
-// cycles a pass of 32768 entries.  (The gradient of 2047 tokens with a sort of three launches 19.8 us, of 32768 155 us, so 16 and 139.)
+// cycles a pass of 32768 entries.  (Their gradient, rows of 2048 columns: 155 us with a sort of three launches a pass, so 139.)
 constexpr int kClusterThreads = 1024, kClusterEach = 8, kClusterMost = 8, kClusterEntries = kClusterThreads * kClusterEach * kClusterMost;
 __device__ __forceinline__ int32_t of_cta(const int32_t* p, uint32_t rank) {
   int32_t v;
@@ -599,8 +639,14 @@ size_t embedding_bwd_scratch(const mxb_embedding_desc* d) { return carve(d, null
 mxb_status embedding_bwd(const mxb_embedding_desc* d, const void* tokens, const void* d_out, void* dweight, int adds, void* workspace,
                          cudaStream_t st) {
   const Scratch s = carve(d, workspace);
-  const int last = (s.passes - 1) & 1;  // where the sorted entries are
-  if (d->tokens <= kClusterEntries) {
+  const int last = d->tokens <= kRankMost ? 0 : (s.passes - 1) & 1;  // where the sorted entries are
+  if (d->tokens <= kRankMost) {
+    const int64_t blocks = std::max<int64_t>((d->tokens + 31) / 32, std::min<int64_t>(148, d->V / (32 * 256) + 1));
+    with_token(d, [&](auto tok) {
+      MXB_LAUNCH("embedding_rank_kernel", st, (launch_kernel(embedding_rank_kernel<decltype(tok)>, (unsigned)blocks, 256, 0, st, tokens, s.entry[0], s.rows,
+                                                             (int)d->tokens, d->V)));
+    });
+  } else if (d->tokens <= kClusterEntries) {
     // about four entries a thread
     int ctas = 1;
     while (ctas < kClusterMost && (int64_t)ctas * kClusterThreads * 4 < d->tokens) ctas *= 2;

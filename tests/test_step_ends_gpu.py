@@ -41,7 +41,7 @@ def words(g, n, V, skew):
     return tok
 
 
-ROWS = [(1, 1, 8), (5, 3, 1), (1, 70000, 16), (37, 5, 449), (300, 1, 64), (257, 1025, 24), (2047, 257, 448), (2049, 2, 40), (4100, 50001, 72),
+ROWS = [(1, 1, 8), (5, 3, 1), (1, 70000, 16), (37, 5, 449), (300, 1, 64), (257, 1025, 24), (2047, 257, 448), (2048, 9001, 24), (2049, 2, 40), (4096, 300, 16), (4097, 300, 16), (65536, 33, 8), (65537, 4000, 8), (4100, 50001, 72),
         (6000, 40, 2050), (70001, 700, 32), (131, 131, 2056)]
 
 
