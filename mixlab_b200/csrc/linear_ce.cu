@@ -420,10 +420,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
   Item t;
   const Wait wait{bad};
   // Blocks of K behind which an accumulator is handed over.  bf16: a cut accumulator loses up to 2^-23 of itself with every 16 terms,
-  // 2^-16 over the 2048 of a logit's part (which exponentials see as they are), 2^-11 over 65536 of a gradient's, which a rounding to
-  // bf16 (2^-9) follows.
-  constexpr int SEG = F32 ? 2 : MODE == kStats || MODE == kGrad ? 32 : 1024;
-
+  // 2^-17 over the 1024 of a loss's logits (32768 tokens, 65536 words: 2.84 ms; with 512, which halves the error, 2.91), 2^-16 over 2048
+  // of a gradient's, 2^-11 over the 65536 of its sums, which a rounding to bf16 (2^-9) follows.
+  constexpr int SEG = F32 ? 2 : MODE == kStats ? 16 : MODE == kGrad ? 32 : 1024;
   // Registers: the epilogue holds a row's 128 columns beside what it does with them; 256 x 232 + 128 x 40 are the 384 x 168 of the launch.
   if (warp >= 8) {
     tc::reg_dec<40>();
