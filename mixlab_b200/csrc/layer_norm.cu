@@ -4,10 +4,16 @@
 //     dh = dh' + k (t - mean t - u mean(t u)),   dw = sum dn u,   db = sum dn     over the rows
 // (dh' the gradient that reaches h from its other readers).
 //
-// HBM streams, built like the residual stage with its RMS norm: a row is read once and held by TPR threads in pieces of eight
-// columns, the next row is requested while one is worked on, narrow rows share a CTA.  The mean is taken first and the squares
-// of what is left after it, both from registers: no difference of two large sums.  Column sums: every group of TPR threads
-// walks over rows with its columns' sums in registers and leaves a partial row; a second launch adds those in a fixed order.
+// HBM streams: 32768 rows of 2048 columns in bf16 with the addition to the stream 88 us (537 MB: 93 % of the measured copy rate), their
+// gradients 106 (537 MB: 78 %), 5 of them in the column sums' own launch; 4001 rows of 449 columns in float32 9.7 us; one row 5.2,
+// the call on the host.  The gradients are bound by instructions and the sums across a row (62 % of the issue slots, 48 % of the
+// LSU pipe): two rows under way instead of one, and sums of each warp around its own mean, joined behind one barrier instead of two,
+// were no faster.
+//
+// A row is read once and held by TPR threads in pieces of eight columns, the next row is requested while one is worked on, narrow
+// rows share a CTA.  The mean is taken first and the squares of what is left after it, both from registers: no difference of two
+// large sums.  Column sums: every group of TPR threads walks over rows with its columns' sums in registers and leaves a partial
+// row; a second launch adds those in a fixed order.  Everything is computed in float32.
 #include <algorithm>
 #include <type_traits>
 
