@@ -628,7 +628,7 @@ static mxb_status check_linear_ce_desc(const mxb_linear_ce_desc* d) {
   if (!d || d->rows < 0 || d->V <= 0 || d->D <= 0 || (d->target_bytes != 4 && d->target_bytes != 8) || !element_type(d->io_dtype))
     return MXB_ERR_INVALID_ARGUMENT;
   // the kernels count tiles of 256 x 128 and rows of tiles in 32 bits
-  if (d->rows > INT32_MAX / 2 || d->V > INT32_MAX - 512 || d->D > INT32_MAX / 16) return MXB_ERR_UNSUPPORTED;
+  if (d->rows > INT32_MAX / 2 || d->V > INT32_MAX / 2 || d->D > INT32_MAX / 16) return MXB_ERR_UNSUPPORTED;
   const int64_t m = (d->rows + 255) / 256, n = ((int64_t)d->V + 127) / 128, k = ((int64_t)d->D + 127) / 128;
   if (m * n > INT32_MAX / 2 || m * k > INT32_MAX / 256 || n * k > INT32_MAX / 256) return MXB_ERR_UNSUPPORTED;
   return MXB_OK;

@@ -607,8 +607,6 @@ static void with_type(int32_t type, F&& f) {
   if (type == MXB_F32) f(float{});
   else f(bf16{});
 }
-static uintptr_t address(const void* p) { return reinterpret_cast<uintptr_t>(p); }
-
 }  // namespace embed
 
 using namespace embed;
@@ -623,7 +621,7 @@ mxb_status embedding_fwd(const mxb_embedding_desc* d, const void* tokens, const 
                (launch_kernel(embedding_fwd_kernel<decltype(tok), decltype(in), decltype(o), R, decltype(whole)::value>,
                               (unsigned)std::min<int64_t>(want, 148 * 8), 256, 0, st, p, tpr)));
   };
-  const bool whole = whole_pieces(address(weight) | address(out), d->D), many = d->tokens >= (int64_t)148 * 8 * groups;
+  const bool whole = whole_pieces(weight, d->io_dtype, d->D) && whole_pieces(out, d->out_dtype, d->D), many = d->tokens >= (int64_t)148 * 8 * groups;
   with_token(d, [&](auto tok) {
     with_type(d->io_dtype, [&](auto in) {
       with_type(d->out_dtype, [&](auto o) {
@@ -708,7 +706,7 @@ mxb_status embedding_bwd(const mxb_embedding_desc* d, const void* tokens, const 
           MXB_LAUNCH("embedding_join_kernel", st,
                      (launch_kernel(embedding_join_kernel<decltype(o), W>, dim3((s.runs + 6) / 8, (d->D + 255) / 256), 256, 0, st, p)));
       };
-      if (whole_pieces(address(d_out) | address(dweight), d->D)) launch(std::true_type{});
+      if (whole_pieces(d_out, d->io_dtype, d->D) && whole_pieces(dweight, d->out_dtype, d->D)) launch(std::true_type{});
       else launch(std::false_type{});
     });
   });

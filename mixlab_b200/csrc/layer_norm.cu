@@ -356,11 +356,11 @@ static mxb_status run(const NormP& p, float* dweight, float* dbias, cudaStream_t
 }
 template <typename IO, typename RES>
 static mxb_status by_alignment(const NormP& p, float* dweight, float* dbias, cudaStream_t st) {
-  uintptr_t at = 0;
-  for (const void* q : {p.resid, p.x, (const void*)p.weight, (const void*)p.bias, (const void*)p.stream, (const void*)p.n, p.d_resid, p.dn,
-                        (const void*)p.dx})
-    at |= reinterpret_cast<uintptr_t>(q);
-  return whole_pieces(at, p.D) ? run<IO, RES, true>(p, dweight, dbias, st) : run<IO, RES, false>(p, dweight, dbias, st);
+  constexpr int32_t io = sizeof(IO) == 4 ? MXB_F32 : MXB_BF16, res = sizeof(RES) == 4 ? MXB_F32 : MXB_BF16;
+  bool whole = whole_pieces(p.x, p.resid ? io : res, p.D) && whole_pieces(p.n, io, p.D) && whole_pieces(p.dn, io, p.D);
+  for (const void* q : {p.resid, (const void*)p.stream, p.d_resid, (const void*)p.dx}) whole = whole && whole_pieces(q, res, p.D);
+  for (const float* q : {p.weight, p.bias}) whole = whole && whole_pieces(q, MXB_F32, p.D);
+  return whole ? run<IO, RES, true>(p, dweight, dbias, st) : run<IO, RES, false>(p, dweight, dbias, st);
 }
 static mxb_status by_type(const mxb_layer_norm_desc* d, const NormP& p, float* dweight, float* dbias, cudaStream_t st) {
   if (d->io_dtype == MXB_F32) return by_alignment<float, float>(p, dweight, dbias, st);

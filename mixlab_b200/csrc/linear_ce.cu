@@ -659,6 +659,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
   }
   __syncwarp();
   __syncthreads();
+  if (*bad)  // a wait gave up: copies that are still under way get two milliseconds to land before this memory is given back
+    for (int i = 0; i < 2000; ++i) __nanosleep(1000);
   if (threadIdx.x == 0) {
     if (MODE == kStats && p.flags) p.flags[blockIdx.x] = *bad ? 11 : 0;
     else if (*bad) atomicExch(p.status, 11);

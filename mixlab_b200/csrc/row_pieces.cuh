@@ -100,8 +100,9 @@ __device__ __forceinline__ void load_floats(const float* p, uint32_t (&r)[8]) {
 __device__ __forceinline__ void store_floats(float* p, const f2 (&e)[4]) {
   asm volatile("st.global.v4.b64 [%0], {%1, %2, %3, %4};" ::"l"(p), "l"(e[0]), "l"(e[1]), "l"(e[2]), "l"(e[3]) : "memory");
 }
-// Whether every tensor of D columns may be read and written in such pieces, by the addresses' bits.
-inline bool whole_pieces(uintptr_t bits, int D) { return bits % 32 == 0 && D % 8 == 0; }
+// Whether a tensor of D columns may be read and written in whole pieces: of eight floats on 32 bytes, of eight bf16 on 16.  (No tensor:
+// nothing in the way.)
+inline bool whole_pieces(const void* p, int32_t type, int D) { return D % 8 == 0 && reinterpret_cast<uintptr_t>(p) % (type == MXB_F32 ? 32 : 16) == 0; }
 
 // Eight columns of a row by each of its `tpr` threads, from column `base` on.  Whole pieces (V): eight neighbours a thread.  Else
 // thread `lane` takes base + lane + j tpr, so that a warp's accesses lie side by side (eight neighbours a thread in single

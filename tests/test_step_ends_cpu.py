@@ -43,7 +43,7 @@ def test_linear_cross_entropy_refusals():
     fwd = lambda d, ws, n, w=FAKE, x=FAKE: lib.mxb_linear_ce_fwd(C.byref(d), x, w, FAKE, FAKE, FAKE, ws, n, None)  # noqa: E731
     bwd = lambda d, ws, n, w=FAKE, dw=FAKE: lib.mxb_linear_ce_bwd(C.byref(d), FAKE, w, FAKE, FAKE, FAKE, None, FAKE, dw, ws, n, None)  # noqa: E731
     for kw, want in [(dict(rows=-1), -1), (dict(V=0), -1), (dict(D=0), -1), (dict(target_bytes=1), -1), (dict(io=3), -1), (dict(rows=1 << 40), -2),
-                     (dict(rows=1 << 29, V=1 << 30), -2), (dict(D=1 << 30), -2)]:
+                     (dict(rows=1 << 29, V=1 << 29), -2), (dict(V=(1 << 30) + 8), -2), (dict(D=1 << 30), -2)]:
         assert fwd(desc(**kw), FAKE, 1 << 60) == want and bwd(desc(**kw), FAKE, 1 << 60) == want, kw
         assert lib.mxb_linear_ce_fwd_workspace_bytes(C.byref(desc(**kw))) == 0 == lib.mxb_linear_ce_bwd_workspace_bytes(C.byref(desc(**kw)))
     for call, n in ((fwd, lib.mxb_linear_ce_fwd_workspace_bytes(C.byref(desc()))), (bwd, lib.mxb_linear_ce_bwd_workspace_bytes(C.byref(desc())))):

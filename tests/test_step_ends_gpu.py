@@ -248,3 +248,23 @@ def test_layer_norm_at_any_element_and_in_place(D):
     ws, dw, db = torch.empty(lib.mxb_layer_norm_bwd_workspace_bytes(C.byref(d)), dtype=torch.uint8, device="cuda"), torch.empty_like(w), torch.empty_like(w)
     assert lib.mxb_layer_norm_bwd(C.byref(d), p(r), p(w), p(dr), p(y), p(dr), p(dw), p(db), p(ws), ws.numel(), st) == 0
     assert torch.equal(dr, want["dx"]) and torch.equal(dw, want["dweight"]) and torch.equal(db, want["dbias"])
+
+
+@pytest.mark.parametrize("D", [24, 40])
+def test_bf16_rows_on_sixteen_bytes(D):
+    """Views that begin in the middle of a matrix: whole pieces of bf16 on 16 bytes, float32 beside them on 32 or not."""
+    g = torch.Generator().manual_seed(8)
+    n, V = 300, 50
+    w, tok = rnd(g, V + 1, D).to(BF16), torch.randint(0, V, (n,), generator=g)
+    part = w.cuda()[1:]
+    for out in (BF16, F32):
+        y = ops.embedding(tok.cuda(), part, dtype=out)
+        assert torch.equal(y.cpu(), w[1:][tok].to(out))
+    d = rnd(g, n + 1, D).to(BF16)
+    want, size, terms = step_ends.embedding_backward(tok, d[1:].double(), V)
+    near(ops.embedding_backward(tok.cuda(), d.cuda()[1:], V, dtype=F32), want, (terms[:, None] + 2) * U * size, (F32, "gradient"))
+    stream = rnd(g, n + 1, D)
+    for x in (d, stream):
+        x64 = x[1:].double()
+        got = ops.layer_norm(x.cuda()[1:], torch.ones(D + 4, device="cuda")[4:], dtype=BF16)
+        near(got, step_ends.layer_norm(x64, torch.ones(D).double())[1], norm_slack(x64, torch.ones(D).double(), None, 1e-5), (BF16, "norm"))
