@@ -4,7 +4,7 @@
 //
 // Both are HBM streams.  32768 rows of 2048 columns, bf16 into float32: 60 us, 403 MB at the measured copy rate.  256 rows 4.8 us, of
 // which the call on the host is most.  Their gradient, float32 for 65536 words: 138 us (671 MB: 74 % of the copy rate), of which
-// the sort takes 20, the sums and the zeros between them 104 and the join 8; 2047 rows of 448 columns 13 us, three launches.
+// the sort takes 20 to 25, the sums and the zeros about 95 and the join 8; 2047 rows of 448 columns 13 us, three launches.
 //
 // The gradient sorts the positions by token (stable, so that a token's positions stand in their own order and the sums do not depend
 // on how blocks run), cuts the sorted list into runs of equal length, whatever the tokens' counts are, and adds up the rows of each
@@ -286,7 +286,8 @@ struct ClusterP {
   const void* tokens;
   int2* entry[2];
   uint32_t* rows;
-  int N, V, bits, passes, share;  // share: entries of a CTA
+  int N, V, bits, passes, share, ctas;  // share: entries of a CTA; ctas: of the cluster that sorts
+  char *zero_from, *zero_to;            // memory that the other clusters fill with zeros
 };
 __device__ __forceinline__ int warp_scan(int v, int lane) {  // inclusive
 #pragma unroll
@@ -299,10 +300,21 @@ __device__ __forceinline__ int warp_scan(int v, int lane) {  // inclusive
 template <typename TOK>
 __global__ void __launch_bounds__(kClusterThreads) embedding_sort_kernel(ClusterP p) {
   begin_dependent();
+  if ((int)blockIdx.x >= p.ctas) {  // zeros: whole pieces of 16 bytes, single pairs of bytes in front of and behind them
+    char* from = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(p.zero_from) + 15) & ~(uintptr_t)15);
+    char* to = reinterpret_cast<char*>(reinterpret_cast<uintptr_t>(p.zero_to) & ~(uintptr_t)15);
+    const size_t first = (size_t)(blockIdx.x - p.ctas) * kClusterThreads + threadIdx.x, step = (size_t)(gridDim.x - p.ctas) * kClusterThreads;
+    for (char* at = from + first * 16; at < to; at += step * 16) *reinterpret_cast<uint4*>(at) = make_uint4(0, 0, 0, 0);
+    if (first < 8) {
+      if (p.zero_from + first * 2 < (from < p.zero_to ? from : p.zero_to)) *reinterpret_cast<uint16_t*>(p.zero_from + first * 2) = 0;
+      if (to >= from && to + first * 2 < p.zero_to) *reinterpret_cast<uint16_t*>(to + first * 2) = 0;
+    }
+    return;
+  }
   extern __shared__ int2 local[];  // [share] entries by digit, then counts of the warps [32][digits]
   __shared__ int32_t hist[kMaxDigits], place[kMaxDigits], inside[kMaxDigits], sums[2][32];
   uint16_t* mine = reinterpret_cast<uint16_t*>(local + p.share);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, digits = 1 << p.bits, ctas = gridDim.x, rank = tc::cluster_rank();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, digits = 1 << p.bits, ctas = p.ctas, rank = tc::cluster_rank();
   const int each = (p.share + kClusterThreads - 1) / kClusterThreads;  // rounds of 32 consecutive entries a warp
   const int begin = min(rank * p.share, p.N), end = min(begin + p.share, p.N), first = begin + warp * 32 * each + lane;
   for (int64_t w = (int64_t)rank * kClusterThreads + threadIdx.x; w <= p.V / 32; w += (int64_t)ctas * kClusterThreads) p.rows[w] = 0;
@@ -405,6 +417,7 @@ struct SumP {
   void* dweight;
   float* part;               // [runs][2][D]: 0 of a token that began before the run, 1 of one that goes on behind it
   int N, V, D, run, runs, adds;
+  int zero_rows;             // rows from here on hold zeros already
   float scale;
 };
 template <typename OUT, bool V>
@@ -431,7 +444,7 @@ __global__ void __launch_bounds__(256, V ? 4 : 2) embedding_bwd_kernel(SumP p, i
     const uint32_t there = p.rows[word];
     f2 zero[4] = {0, 0, 0, 0};
     for (int r = group; r < kZeroRows; r += groups) {
-      if (there >> r & 1u || r0 + r >= p.V) continue;
+      if (there >> r & 1u || r0 + r >= p.zero_rows) continue;
       OUT* to = static_cast<OUT*>(p.dweight) + (size_t)(r0 + r) * p.D;
       for (int c = 0; c < p.D; c += tpr * 8) store_cols<OUT, V>(to, c, lane, tpr, p.D, zero);
     }
@@ -642,6 +655,7 @@ size_t embedding_bwd_scratch(const mxb_embedding_desc* d) { return carve(d, null
 mxb_status embedding_bwd(const mxb_embedding_desc* d, const void* tokens, const void* d_out, void* dweight, int adds, void* workspace,
                          cudaStream_t st) {
   const Scratch s = carve(d, workspace);
+  int zero_rows = d->V;
   const int last = d->tokens <= kRankMost ? 0 : (s.passes - 1) & 1;  // where the sorted entries are
   if (d->tokens <= kRankMost) {
     const int64_t blocks = std::max<int64_t>((d->tokens + 31) / 32, std::min<int64_t>(148, d->V / (32 * 256) + 1));
@@ -653,7 +667,13 @@ mxb_status embedding_bwd(const mxb_embedding_desc* d, const void* tokens, const 
     // about four entries a thread
     int ctas = 1;
     while (ctas < kClusterMost && (int64_t)ctas * kClusterThreads * 4 < d->tokens) ctas *= 2;
-    const ClusterP q{tokens, {s.entry[0], s.entry[1]}, s.rows, (int)d->tokens, d->V, s.bits, s.passes, (int)((d->tokens + ctas - 1) / ctas)};
+    // The sort leaves most SMs idle for 10 to 20 us: they write zeros to the last rows of dW meanwhile, those of the words that occur too
+    // (32768 rows of 2048 columns, 65536 words in float32: 138 us without, 134 with).
+    const size_t row = (size_t)d->D * (d->out_dtype == MXB_F32 ? 4 : 2);
+    if (!adds) zero_rows -= (int)std::min<size_t>(d->V, (((size_t)32 << 20) + (size_t)d->tokens * 2560) / row);
+    char* dw = static_cast<char*>(dweight);
+    const ClusterP q{tokens, {s.entry[0], s.entry[1]}, s.rows, (int)d->tokens, d->V, s.bits, s.passes, (int)((d->tokens + ctas - 1) / ctas), ctas,
+                     dw + zero_rows * row, dw + d->V * row};
     mxb_status st_ = MXB_OK;
     with_token(d, [&](auto tok) {
       using TOK = decltype(tok);
@@ -661,7 +681,7 @@ mxb_status embedding_bwd(const mxb_embedding_desc* d, const void* tokens, const 
       st_ = MXB_ALLOW_SMEM(kClusterThreads * kClusterEach * (int)sizeof(int2) + 64 * kMaxDigits, embedding_sort_kernel<TOK>);
       if (st_ != MXB_OK) return;
       cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = ctas;
+      cfg.gridDim = zero_rows < d->V ? 144 / ctas * ctas : ctas;
       cfg.blockDim = kClusterThreads;
       cfg.dynamicSmemBytes = smem;
       cfg.stream = st;
@@ -692,9 +712,9 @@ mxb_status embedding_bwd(const mxb_embedding_desc* d, const void* tokens, const 
     MXB_LAUNCH("embedding_mark_kernel", st,
                (launch_kernel(embedding_mark_kernel, (unsigned)((d->tokens + 255) / 256), 256, 0, st, s.entry[last], (int)d->tokens, s.rows)));
   }
-  const SumP p{s.entry[last], s.rows, d_out, dweight, s.part, (int)d->tokens, d->V, d->D, s.run, s.runs, adds, d->scale};
+  const SumP p{s.entry[last], s.rows, d_out, dweight, s.part, (int)d->tokens, d->V, d->D, s.run, s.runs, adds, zero_rows, d->scale};
   const int tpr = threads_per_row(d->D), groups = 256 / tpr, sums = (s.runs + groups - 1) / groups;
-  const int zeros = adds ? 0 : (int)(((int64_t)d->V + kZeroRows - 1) / kZeroRows);
+  const int zeros = adds ? 0 : (int)(((int64_t)zero_rows + kZeroRows - 1) / kZeroRows);
   with_type(d->io_dtype, [&](auto in) {
     with_type(d->out_dtype, [&](auto o) {
       auto launch = [&](auto whole) {
