@@ -3,14 +3,14 @@
 // A token outside 0 .. V-1 is padding: its row of y is zero and it has no part in dW.
 //
 // Both are HBM streams.  32768 rows of 2048 columns, bf16 into float32: 60 us, 403 MB at the measured copy rate.  256 rows 4.8 us, of
-// which the call on the host is most.  Their gradient, float32 for 65536 words: 138 us (671 MB: 74 % of the copy rate), of which
+// which the call on the host is most.  Their gradient, float32 for 65536 words: 134 us (671 MB: 76 % of the copy rate), of which
 // the sort takes 20 to 25, the sums and the zeros about 95 and the join 8; 2047 rows of 448 columns 13 us, three launches.
 //
 // The gradient sorts the positions by token (stable, so that a token's positions stand in their own order and the sums do not depend
 // on how blocks run), cuts the sorted list into runs of equal length, whatever the tokens' counts are, and adds up the rows of each
 // run, the next batch of rows under way beside them; a token that lies in several runs leaves a partial row in each, which a last
-// launch adds in the order of the runs.  Rows of words that do not occur are written by blocks of the same launch as the sums.  Sums
-// are float32 and rounded once.
+// launch adds in the order of the runs.  Rows of words that do not occur are written by blocks of the same launch as the sums, the last
+// of them beside the sort.  Sums are float32 and rounded once.
 #include <algorithm>
 #include <type_traits>
 

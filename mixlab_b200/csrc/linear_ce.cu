@@ -210,8 +210,7 @@ __global__ void __launch_bounds__(256) lce_pack_weight_kernel(const T* w, bf16* 
 
 // ------------------------------------------------------------------ the products
 enum Mode { kStats, kGrad, kDx, kDw };
-// A stage of the ring: PARTS tiles of A, 128 rows a CTA, and of B, BN / 2 rows a CTA, 64 deep.
-// BN, columns of a tile.
+// A stage of the ring: PARTS tiles of A, 128 rows a CTA, and of B, BN / 2 rows a CTA, 64 deep.  BN: columns of a tile.
 template <int MODE, bool F32, int BN_>
 struct Cfg {
   static constexpr int BN = BN_, PARTS = F32 ? 3 : 1, COLS = BN / 2;  // COLS: of a thread of the epilogue
@@ -444,18 +443,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
             if (rank == 0) tc::mbar_expect_tx(full + s, 2 * C::STAGE);
             const uint32_t bar = tc::in_cta(tc::smem_u32(full + s), 0);
             uint32_t to = base + s * C::STAGE;
-  #pragma unroll
+#pragma unroll
             for (int part = 0; part < C::PARTS; ++part, to += C::A) {
               const int m0 = t.m * 256 + (int)rank * 128;
               if (MODE == kDx) tc::tma_load_4d_pair(to, &maps.a, 0, 0, kb * 8, part * p.blocks + m0 / 128, bar);
               else if (MODE == kDw) tc::tma_load_4d_pair(to, &maps.a, 0, (kb & 1) * 2, m0 / 8, part * p.blocks + kb / 2, bar);
               else tc::tma_load_3d_pair(to, &maps.a, kb * 64, m0, part, bar);
             }
-  #pragma unroll
+#pragma unroll
             for (int part = 0; part < C::PARTS; ++part, to += C::B) {
               const int n0 = t.n * C::BN + (int)rank * (C::BN / 2);
               if (C::B_MN) {
-  #pragma unroll
+#pragma unroll
                 for (int x = 0; x < C::BN / 128; ++x) tc::tma_load_3d_pair(to + x * 8192, &maps.b, n0 + 64 * x, p.b_row0 + kb * 64, part, bar);
               } else {
                 tc::tma_load_3d_pair(to, &maps.b, kb * 64, p.b_row0 + n0, part, bar);
@@ -489,7 +488,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
                                     : MODE == kDw ? tc::make_smem_desc(sa + pa * C::A, 128, 1024, tc::kSwizzleNone)
                                                   : tc::make_smem_desc(sa + pa * C::A, 16, 1024, tc::kSwizzle128);
                 const uint64_t db = tc::make_smem_desc(sb + pb * C::B, C::B_MN ? 8192 : 16, 1024, tc::kSwizzle128);
-  #pragma unroll
+#pragma unroll
                 for (int k = 0; k < 4; ++k)
                   tc::mma_pair(d, da + (uint64_t)((k * a_step) >> 4), db + (uint64_t)((k * b_step) >> 4), idesc, !(first && k == 0));
               };
@@ -907,6 +906,12 @@ template <int MODE, bool F32, int BN>
 static mxb_status launch_gemm(const GemmP& p, const Maps& maps, int pairs, cudaStream_t st) {
   using C = Cfg<MODE, F32, BN>;
   if (MXB_ALLOW_SMEM(C::SMEM, lce_gemm_kernel<MODE, F32, BN>) != MXB_OK) return MXB_ERR_CUDA;
+  // (warps that ask for registers which the launch did not bring would wait for good)
+  static const bool fits = [] {
+    cudaFuncAttributes a;
+    return cudaFuncGetAttributes(&a, lce_gemm_kernel<MODE, F32, BN>) == cudaSuccess && a.numRegs * kThreads >= 256 * 232 + 128 * 40;
+  }();
+  if (!fits) return MXB_ERR_UNSUPPORTED;
   static const char* const names[] = {"lce_stats_kernel", "lce_grad_kernel", "lce_dx_kernel", "lce_dw_kernel"};
   MXB_LAUNCH(names[MODE], st, (launch_kernel(lce_gemm_kernel<MODE, F32, BN>, 2 * pairs, kThreads, C::SMEM, st, p, maps)));
   return check_launch(names[MODE]);
