@@ -35,6 +35,18 @@ __device__ __forceinline__ int token_of<int32_t>(const int32_t* tokens, size_t t
   return v >= 0 && v < V ? v : V;
 }
 
+// Zeros from one address to another, both multiples of two, by so many threads: whole pieces of 16 bytes, pairs of bytes in front of and
+// behind them.
+__device__ __forceinline__ void fill_zeros(char* begin, char* end, size_t thread, size_t threads) {
+  char* from = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(begin) + 15) & ~(uintptr_t)15);
+  char* to = reinterpret_cast<char*>(reinterpret_cast<uintptr_t>(end) & ~(uintptr_t)15);
+  for (char* at = from + thread * 16; at < to; at += threads * 16) *reinterpret_cast<uint4*>(at) = make_uint4(0, 0, 0, 0);
+  if (thread < 8) {
+    if (begin + thread * 2 < (from < end ? from : end)) *reinterpret_cast<uint16_t*>(begin + thread * 2) = 0;
+    if (to >= from && to + thread * 2 < end) *reinterpret_cast<uint16_t*>(to + thread * 2) = 0;
+  }
+}
+
 // ------------------------------------------------------------------ forward
 struct FwdP {
   const void* tokens;
@@ -300,15 +312,8 @@ __device__ __forceinline__ int warp_scan(int v, int lane) {  // inclusive
 template <typename TOK>
 __global__ void __launch_bounds__(kClusterThreads) embedding_sort_kernel(ClusterP p) {
   begin_dependent();
-  if ((int)blockIdx.x >= p.ctas) {  // zeros: whole pieces of 16 bytes, single pairs of bytes in front of and behind them
-    char* from = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(p.zero_from) + 15) & ~(uintptr_t)15);
-    char* to = reinterpret_cast<char*>(reinterpret_cast<uintptr_t>(p.zero_to) & ~(uintptr_t)15);
-    const size_t first = (size_t)(blockIdx.x - p.ctas) * kClusterThreads + threadIdx.x, step = (size_t)(gridDim.x - p.ctas) * kClusterThreads;
-    for (char* at = from + first * 16; at < to; at += step * 16) *reinterpret_cast<uint4*>(at) = make_uint4(0, 0, 0, 0);
-    if (first < 8) {
-      if (p.zero_from + first * 2 < (from < p.zero_to ? from : p.zero_to)) *reinterpret_cast<uint16_t*>(p.zero_from + first * 2) = 0;
-      if (to >= from && to + first * 2 < p.zero_to) *reinterpret_cast<uint16_t*>(to + first * 2) = 0;
-    }
+  if ((int)blockIdx.x >= p.ctas) {
+    fill_zeros(p.zero_from, p.zero_to, (size_t)(blockIdx.x - p.ctas) * kClusterThreads + threadIdx.x, (size_t)(gridDim.x - p.ctas) * kClusterThreads);
     return;
   }
   extern __shared__ int2 local[];  // [share] entries by digit, then counts of the warps [32][digits]
@@ -442,6 +447,13 @@ __global__ void __launch_bounds__(256, V ? 4 : 2) embedding_bwd_kernel(SumP p, i
   if ((int)blockIdx.x >= sum_blocks) {
     const int64_t word = blockIdx.x - sum_blocks, r0 = word * kZeroRows;
     const uint32_t there = p.rows[word];
+    // (rows side by side in one piece, in which their own alignment has no part: 3000 tokens, 50000 words of 699 columns in bf16 43 us row
+    // by row, 35 so)
+    if (there == 0 && r0 + kZeroRows <= p.zero_rows) {
+      char* at = static_cast<char*>(p.dweight) + (size_t)r0 * p.D * sizeof(OUT);
+      fill_zeros(at, at + (size_t)kZeroRows * p.D * sizeof(OUT), threadIdx.x, 256);
+      return;
+    }
     f2 zero[4] = {0, 0, 0, 0};
     for (int r = group; r < kZeroRows; r += groups) {
       if (there >> r & 1u || r0 + r >= p.zero_rows) continue;
