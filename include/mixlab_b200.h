@@ -462,7 +462,8 @@ MXB_API mxb_status mxb_layer_norm_bwd(const mxb_layer_norm_desc* d, const void* 
  * 8); loss, lse, d_loss, d_lse [rows] float32, d_lse may be NULL (zero), lse in the backward is what the
  * forward returned.  A row whose target is outside 0..V-1 has no part: its loss, lse and dx are zero and
  * its x may hold anything; the same holds in the backward for a row whose d_loss and d_lse are zero.
- * bf16: products of bf16 on the tensor cores added up in float32, g rounded to bf16 for the last two.  float32:
+ * bf16: products of bf16 on the tensor cores added up in float32, g rounded to bf16 for the last two as a multiple of the first
+ * weight's mantissa (equal weights d_loss are not rounded themselves).  float32:
  * finite operands in three bf16 parts, the error of float32 products.  The backward keeps g for a piece of the
  * vocabulary at a time, at most 640 MB or 256 columns.  bf16 weights with D a multiple of 8 must lie on
  * 16 bytes; everything else may start at any element.  The workspace's first word is the kernels'

@@ -8,7 +8,8 @@
 // Products on the tensor cores, 256 x 256 a pair of CTAs, fed by TMA through a ring of shared-memory stages; accumulators in TMEM by
 // turns, so that one is read while another is filled.  Forward: the accumulator is reduced to the maximum and the sum of
 // exponentials of each row over the tile's columns, 8 bytes a row and tile.  Backward, in pieces of the vocabulary: z again, g in
-// bf16 to a workspace of bounded size, then dx += g W and dW = g^T x from it.
+// bf16 to a workspace of bounded size, then dx += g W and dW = g^T x from it (a second part of g, which would leave the results' own
+// rounding alone, would be two products more beside three).
 //
 // What bounds it is the tensor pipe at the clock that the power limit leaves: 28672 tokens, 65536 words of 1024 columns 2.69 ms
 // (1430 TFLOP/s; cuBLAS's product alone runs at 1402 for seconds on end); the gradients for 50001 words 7.1 ms (1240), where g goes
@@ -248,6 +249,14 @@ struct GemmP {
 };
 struct Maps { CUtensorMap a, b, g; };
 __device__ __forceinline__ int live_of(const GemmP& p) { return p.live ? *p.live : p.rows; }
+// bf16: g is kept as a multiple of the first token's gradient's mantissa (1 .. 2; 1 of a zero, an infinity or a NaN), by which dx and dW are
+// multiplied before they are rounded.  Where all tokens weigh the same - a mean, a sum over some of them - what g is rounded from
+// is then 2^k (p - [v = i]).  Without it the rounding of the weight itself is in every token's largest element alike: 28672 tokens that
+// weigh 1 / 28672, off by 2e-3 as bf16, had gradients off by 2.3e-3, with it by 1.9e-3, of which their own rounding is 1.7e-3.
+__device__ __forceinline__ float unit_of(const GemmP& p) {
+  const uint32_t a = __float_as_uint(p.a[0]), v = a & 0x7fffffffu ? a : __float_as_uint(p.both[0]), e = v >> 23 & 255u;
+  return e == 0u || e == 255u ? 1.f : __uint_as_float((v & 0x7fffffu) | 0x3f800000u);
+}
 
 // A wait that gives up: on its own limit, or when another role of the CTA has.
 struct Wait {
@@ -527,7 +536,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
       if constexpr (MODE == kStats) target = p.live ? p.tgt[row] : row < live ? target_at(p.targets, p.wide, p.V, row) : -1;
       if constexpr (MODE == kGrad) {
         target = p.tgt[row];
-        both = p.both[row];
+        both = F32 ? p.both[row] : p.both[row] / unit_of(p);
         back = -p.lse2[row];
       }
       float v[C::COLS];
@@ -612,7 +621,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
 #pragma unroll
             for (int c = 0; c < C::COLS; ++c) v[c] = row < live && c < here ? v[c] : 0.f;
           if (__any_sync(0xffffffffu, hit)) {
-            const float a = hit ? p.a[row] : 0.f;
+            const float a = !hit ? 0.f : F32 ? p.a[row] : p.a[row] / unit_of(p);
 #pragma unroll
             for (int c = 0; c < C::COLS; ++c) v[c] = c == at ? v[c] - a : v[c];
           }
@@ -645,13 +654,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
             *reinterpret_cast<float4*>(to + (c / 4 + x) * 512) = make_float4(old[x].x + e[0], old[x].y + e[1], old[x].z + e[2], old[x].w + e[3]);
           }
         }
-      } else if (C::BOXES && p.whole) {
-        leave_in_boxes<C::COLS>(&maps.g, staging + warp * 4096, v, c0, p.v0 + m * 256 + (int)rank * 128 + quarter * 32, lane);
-      } else if (row < (MODE == kDx ? live : p.M)) {
-        using T = std::conditional_t<F32, float, bf16>;
-        T* to = static_cast<T*>(p.out) + (MODE == kDx ? (size_t)p.idx[row] : (size_t)p.v0 + row) * p.D;
+      } else {
+        const float unit = F32 ? 1.f : unit_of(p);
+        if (!F32)
 #pragma unroll
-        for (int c = 0; c < C::COLS; c += 8) store_row<T>(to, c0 + c, p.D, p.whole, v + c);
+          for (int c = 0; c < C::COLS; ++c) v[c] *= unit;
+        if (C::BOXES && p.whole) {
+          leave_in_boxes<C::COLS>(&maps.g, staging + warp * 4096, v, c0, p.v0 + m * 256 + (int)rank * 128 + quarter * 32, lane);
+        } else if (row < (MODE == kDx ? live : p.M)) {
+          using T = std::conditional_t<F32, float, bf16>;
+          T* to = static_cast<T*>(p.out) + (MODE == kDx ? (size_t)p.idx[row] : (size_t)p.v0 + row) * p.D;
+#pragma unroll
+          for (int c = 0; c < C::COLS; c += 8) store_row<T>(to, c0 + c, p.D, p.whole, v + c);
+        }
       }
     }
     if (C::BOXES && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
@@ -761,6 +776,11 @@ __global__ void __launch_bounds__(256) lce_shares_kernel(const GemmP px, const G
   }
   const int row = t.m * 256 + rank * 128 + mine;
   if (row >= (is_dx ? *p.live : p.M)) return;
+  if (!F32) {
+    const float unit = unit_of(p);
+#pragma unroll
+    for (int c = 0; c < 8; ++c) v[c] *= unit;
+  }
   T* out = static_cast<T*>(p.out) + (is_dx ? (size_t)p.idx[row] : (size_t)p.v0 + row) * p.D;
   store_row<T>(out, t.n * BN + c0, p.D, p.whole, v);
 }
@@ -773,12 +793,13 @@ __global__ void __launch_bounds__(256) lce_finish_kernel(const GemmP p, int n_ti
   const int m0 = blockIdx.x * 128, col = blockIdx.y * 64, live = *p.live;
   if (m0 >= live) return;
   const float* from = p.sums + tile_at<BN>((size_t)(blockIdx.x >> 1) * n_tiles + col / BN, blockIdx.x & 1, threadIdx.x & 127, col % BN);
+  const float unit = F32 ? 1.f : unit_of(p);
 #pragma unroll
   for (int x = 0; x < 8; ++x) {
     const int c4 = x * 2 + (threadIdx.x >> 7);
     const float4 v = *reinterpret_cast<const float4*>(from + c4 * 512);
     float* to = &box[threadIdx.x & 127][c4 * 4];
-    to[0] = v.x; to[1] = v.y; to[2] = v.z; to[3] = v.w;
+    to[0] = v.x * unit; to[1] = v.y * unit; to[2] = v.z * unit; to[3] = v.w * unit;
   }
   __syncthreads();
   const int lane = threadIdx.x & 31;

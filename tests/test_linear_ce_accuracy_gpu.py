@@ -1,0 +1,46 @@
+"""What the output head's loss and its gradients are off by, sum by sum, against float64.
+
+Tolerances are counted before the first run.  u = 2^-24; a bf16 is off by half of its eps, 2^-8, relative to the value."""
+import pytest
+import torch
+
+from mixlab_b200 import ops
+from oracle import step_ends
+
+pytestmark = pytest.mark.gpu
+F32, BF16 = torch.float32, torch.bfloat16
+U, HALF = 2.0 ** -24, 2.0 ** -8
+
+
+@pytest.mark.parametrize("weight", [1 / 28672, 0.3, -5.2])
+def test_equal_weights_have_no_part_in_the_rounding(weight):
+    """Gradients of a mean: what is left of got - want along want, element for element independent errors add up to little there, a
+    weight that is rounded does in full (0.0020, 0.0026 and 0.0018 for these weights)."""
+    n, V, D = 512, 8000, 64
+    g = torch.Generator().manual_seed(11)
+    w = torch.randn(V, D, generator=g).to(BF16).cuda()
+    x = (0.02 * torch.randn(n, D, generator=g)).to(BF16).cuda()
+    t = torch.randint(0, V, (n,), generator=g)
+    t[0] = -1  # (the first row has no part)
+    d = torch.full((n,), weight)
+    d[1::9] = 0.0
+    lse = ops.linear_cross_entropy(x, w, t.cuda())[1]
+    got = ops.linear_cross_entropy_backward(x, w, t.cuda(), lse, d.cuda())
+    t, d = t.cuda(), torch.where(t.cuda() >= 0, d.cuda(), 0.0).double()
+    xd, wd = x.double(), w.double()
+    want = step_ends.linear_cross_entropy_backward(xd, wd, t, lse.double(), d)
+    live = d != 0
+    p = live[:, None] * torch.exp(xd @ wd.T - lse.double()[:, None])
+    most = p.max().item()
+    grad = p * d.abs()[:, None]
+    grad[live.nonzero()[:, 0], t[live]] += d[live].abs()
+    for name, e, other in (("dx", grad, wd), ("dweight", grad.T, xd)):
+        need = want[name]
+        size = need.norm()
+        along = ((got[name].double() - need) * need).sum().abs() / size ** 2
+        last = 4 * HALF * need.square().norm() / size ** 2  # by chance, four deviations
+        hits = 1.5 * most  # 1 - p to the nearest bf16, 1 among them
+        others = 4 * HALF * most * abs(weight) * other.norm() / size  # by chance: |W need^T| <= |W| |need|
+        sums = 2 * U * (e.shape[1] / 16 + 2) * (e @ other.abs()).norm() / size  # accumulators that are cut
+        assert along <= last + hits + others + sums + 8 * U, (name, along.item(), last.item(), hits, others.item(), sums.item())
+        assert last + hits + others + sums < 1e-3, name  # (far below what a rounded weight leaves)
