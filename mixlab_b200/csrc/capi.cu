@@ -130,7 +130,7 @@ size_t embedding_bwd_scratch(const mxb_embedding_desc*);
 mxb_status embedding_bwd(const mxb_embedding_desc*, const void*, const void*, void*, int, void*, cudaStream_t);
 size_t layer_norm_scratch(const mxb_layer_norm_desc*);
 mxb_status layer_norm_fwd(const mxb_layer_norm_desc*, const void*, const void*, const float*, const float*, void*, void*, cudaStream_t);
-mxb_status layer_norm_bwd(const mxb_layer_norm_desc*, const void*, const float*, const void*, const void*, void*, float*, float*, float*,
+mxb_status layer_norm_bwd(const mxb_layer_norm_desc*, const void*, const float*, const void*, const void*, void*, float*, float*, void*,
                           cudaStream_t);
 size_t linear_ce_scratch(const mxb_linear_ce_desc*, bool bwd);
 mxb_status linear_ce_fwd(const mxb_linear_ce_desc*, const void*, const void*, const void*, float*, float*, void*, cudaStream_t);
@@ -621,7 +621,7 @@ mxb_status mxb_layer_norm_bwd(const mxb_layer_norm_desc* d, const void* x, const
   if (!x || !dn || !dx) return MXB_ERR_INVALID_ARGUMENT;
   if (!workspace || workspace_bytes < layer_norm_scratch(d)) return MXB_ERR_WORKSPACE;
   if (!aligned16(workspace)) return MXB_ERR_ALIGNMENT;
-  return layer_norm_bwd(d, x, weight, d_resid, dn, dx, dweight, dbias, static_cast<float*>(workspace), static_cast<cudaStream_t>(stream));
+  return layer_norm_bwd(d, x, weight, d_resid, dn, dx, dweight, dbias, workspace, static_cast<cudaStream_t>(stream));
 }
 
 static mxb_status check_linear_ce_desc(const mxb_linear_ce_desc* d) {

@@ -184,6 +184,9 @@ mxb_status allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>& done
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
 // Carves a caller-provided workspace into 256-byte aligned pieces.
+// Where scratch starts that is written in pieces of 32 bytes and whose base may lie on 16: up to kBaseRoom behind the base.
+constexpr size_t kBaseRoom = 256;
+inline void* round_base_up(void* base) { return reinterpret_cast<void*>(align_up(reinterpret_cast<uintptr_t>(base), kBaseRoom)); }
 struct Carver {
   char* base;
   size_t off = 0;

@@ -605,7 +605,7 @@ struct Scratch {
 };
 static Scratch carve(const mxb_embedding_desc* d, void* base) {
   Scratch s{};
-  Carver c(base);
+  Carver c(round_base_up(base));  // (partial rows are written in pieces of 32 bytes)
   const int64_t N = d->tokens;
   int bits = 1;
   while ((int64_t)1 << bits <= d->V) ++bits;  // keys are 0 .. V
@@ -619,7 +619,7 @@ static Scratch carve(const mxb_embedding_desc* d, void* base) {
   s.hist = c.take<int32_t>(((size_t)1 << s.bits) * s.tiles);
   s.total = c.take<int32_t>((size_t)1 << s.bits);
   s.part = c.take<float>((size_t)s.runs * 2 * d->D);
-  s.bytes = c.bytes();
+  s.bytes = c.bytes() + kBaseRoom;
   return s;
 }
 template <typename F>

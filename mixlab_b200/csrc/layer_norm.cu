@@ -372,7 +372,7 @@ static mxb_status by_type(const mxb_layer_norm_desc* d, const NormP& p, float* d
 
 size_t layer_norm_scratch(const mxb_layer_norm_desc* d) {
   const int tpr = lnorm::row_shape(d->D, true).tpr;
-  return (size_t)lnorm::ctas(d->rows, d->D, true, d->resid_dtype == MXB_BF16) * lnorm::groups_of(tpr) * 2 * d->D * sizeof(float);
+  return (size_t)lnorm::ctas(d->rows, d->D, true, d->resid_dtype == MXB_BF16) * lnorm::groups_of(tpr) * 2 * d->D * sizeof(float) + kBaseRoom;
 }
 mxb_status layer_norm_fwd(const mxb_layer_norm_desc* d, const void* resid, const void* x, const float* weight, const float* bias, void* stream,
                           void* n, cudaStream_t st) {
@@ -380,7 +380,8 @@ mxb_status layer_norm_fwd(const mxb_layer_norm_desc* d, const void* resid, const
   return lnorm::by_type(d, p, nullptr, nullptr, st);
 }
 mxb_status layer_norm_bwd(const mxb_layer_norm_desc* d, const void* x, const float* weight, const void* d_resid, const void* dn, void* dx,
-                          float* dweight, float* dbias, float* part, cudaStream_t st) {
+                          float* dweight, float* dbias, void* workspace, cudaStream_t st) {
+  float* part = static_cast<float*>(round_base_up(workspace));  // (written in pieces of 32 bytes)
   const lnorm::NormP p{(size_t)d->rows, d->D, d->eps, nullptr, x, weight, nullptr, nullptr, nullptr, d_resid, dn, dx, part};
   return lnorm::by_type(d, p, dweight, dbias, st);
 }
