@@ -164,7 +164,10 @@ MXB_API mxb_status mxb_gdn_fwd_static_scratch(const mxb_gdn_desc* d, const void*
 /* The tensor-core kernels bound every wait on an mbarrier; a wait that gives up
  * makes the kernel leave in an orderly way and write a nonzero code into the first
  * word of the workspace.  This BLOCKING call copies that word to *out (0 = no
- * device-side error).  Workspaces of the fp32 path never set it. */
+ * device-side error).  Calls that keep a word, and clear it first unless they go on from what
+ * a forward saved: the gated delta scans (chunk > 1) and their op records, the chunked Mamba-3
+ * scan (head dim 64, d_state 128, bf16) and the loss of the output head, forward and backward.
+ * Every other call leaves the workspace's first 256 bytes as they are. */
 MXB_API mxb_status mxb_gdn_device_status(const void* workspace, int32_t* out);
 
 /* One token of the recurrence on a persistent state: the loop body of

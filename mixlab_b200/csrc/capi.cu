@@ -317,7 +317,7 @@ static mxb_status check_block_desc(const mxb_gdn_desc* d) {
   return MXB_OK;
 }
 size_t mxb_gdn_block_workspace_bytes(const mxb_gdn_desc* d) {
-  return check_block_desc(d) == MXB_OK ? gdn_block_workspace_bytes(d) : 0;
+  return check_block_desc(d) == MXB_OK ? with_status(gdn_block_workspace_bytes(d)) : 0;
 }
 mxb_status mxb_gdn_block_pre_fwd(const mxb_gdn_desc* d, const void* q_proj, const void* k_proj, const void* v_proj,
                                  const float* conv_q, const float* conv_k, const float* conv_v, const float* a_raw,
@@ -351,10 +351,10 @@ mxb_status mxb_gdn_block_pre_bwd(const mxb_gdn_desc* d, const void* q_proj, cons
       !aligned16(dq_proj) || !aligned16(dk_proj) || !aligned16(dv_proj) || !aligned16(conv_q) || !aligned16(conv_k) ||
       !aligned16(conv_v) || !aligned16(workspace))
     return MXB_ERR_ALIGNMENT;
-  if (workspace_bytes < gdn_block_workspace_bytes(d)) return MXB_ERR_WORKSPACE;
+  if (workspace_bytes < with_status(gdn_block_workspace_bytes(d))) return MXB_ERR_WORKSPACE;
   return gdn_block_pre_bwd(d, q_proj, k_proj, v_proj, conv_q, conv_k, conv_v, a_raw, b_raw, a_log, dt_bias, dq, dk, dv, dbeta,
                            dgate, dq_proj, dk_proj, dv_proj, dconv_q, dconv_k, dconv_v, da_raw, db_raw, da_log, ddt_bias,
-                           workspace, static_cast<cudaStream_t>(stream));
+                           behind_status(workspace), static_cast<cudaStream_t>(stream));
 }
 mxb_status mxb_gdn_block_post_fwd(const mxb_gdn_desc* d, const void* o, const void* z, const float* o_norm, void* y,
                                   void* stream) {
@@ -373,8 +373,8 @@ mxb_status mxb_gdn_block_post_bwd(const mxb_gdn_desc* d, const void* o, const vo
   if (!aligned16(o) || !aligned16(z) || !aligned16(dy) || !aligned16(d_o) || !aligned16(dz) || !aligned16(o_norm) ||
       !aligned16(workspace))
     return MXB_ERR_ALIGNMENT;
-  if (workspace_bytes < gdn_block_workspace_bytes(d)) return MXB_ERR_WORKSPACE;
-  return gdn_block_post(d, o, z, o_norm, nullptr, dy, d_o, dz, do_norm, workspace, static_cast<cudaStream_t>(stream));
+  if (workspace_bytes < with_status(gdn_block_workspace_bytes(d))) return MXB_ERR_WORKSPACE;
+  return gdn_block_post(d, o, z, o_norm, nullptr, dy, d_o, dz, do_norm, behind_status(workspace), static_cast<cudaStream_t>(stream));
 }
 
 static mxb_status check_m3_desc(const mxb_mamba3_desc* d) {
@@ -451,7 +451,7 @@ static mxb_status serve_operands(ServeP* p, const void* x, const float* dt, cons
 }
 size_t mxb_mamba3_prefill_workspace_bytes(const mxb_mamba3_serve_desc* d) {
   ServeP p;
-  return serve_params(d, &p) == MXB_OK ? m3walk_scratch(p, d->io_dtype == MXB_F32, d->flags, nullptr) : 0;
+  return serve_params(d, &p) == MXB_OK ? with_status(m3walk_scratch(p, d->io_dtype == MXB_F32, d->flags, nullptr)) : 0;
 }
 mxb_status mxb_mamba3_prefill(const mxb_mamba3_serve_desc* d, const void* x, const float* dt, const float* lambda, const float* theta,
                               const float* a_log, const void* b, const void* c, const int32_t* cu_seqlens, const int32_t* slot,
@@ -467,11 +467,11 @@ mxb_status mxb_mamba3_prefill(const mxb_mamba3_serve_desc* d, const void* x, con
   p.cu = cu_seqlens;
   p.go = go_on;
   const bool f32 = d->io_dtype == MXB_F32;
-  const size_t need = m3walk_scratch(p, f32, d->flags, nullptr);
+  const size_t need = with_status(m3walk_scratch(p, f32, d->flags, nullptr));
   if (need) {
     if (!workspace || workspace_bytes < need) return MXB_ERR_WORKSPACE;
     if (!aligned16(workspace)) return MXB_ERR_ALIGNMENT;
-    m3walk_scratch(p, f32, d->flags, static_cast<char*>(workspace));
+    m3walk_scratch(p, f32, d->flags, static_cast<char*>(behind_status(workspace)));
   }
   return m3walk_prefill(p, f32, d->flags, static_cast<cudaStream_t>(stream));
 }
@@ -524,7 +524,7 @@ static mxb_status check_norm_desc(const mxb_residual_norm_desc* d) {
   return MXB_OK;
 }
 size_t mxb_residual_norm_workspace_bytes(const mxb_residual_norm_desc* d) {
-  return check_norm_desc(d) == MXB_OK ? residual_norm_scratch(d) : 0;
+  return check_norm_desc(d) == MXB_OK ? with_status(residual_norm_scratch(d)) : 0;
 }
 mxb_status mxb_residual_norm_fwd(const mxb_residual_norm_desc* d, const void* resid, const void* y, const float* norm,
                                  const float* post_norm, const void* z, const float* scale, void* resid_out, void* n, void* stream) {
@@ -550,10 +550,10 @@ mxb_status mxb_residual_norm_bwd(const mxb_residual_norm_desc* d, const void* re
     return MXB_OK;
   }
   if (!resid_out || !y || !dn || !d_resid || !dy) return MXB_ERR_INVALID_ARGUMENT;
-  if (!workspace || workspace_bytes < residual_norm_scratch(d)) return MXB_ERR_WORKSPACE;
+  if (!workspace || workspace_bytes < with_status(residual_norm_scratch(d))) return MXB_ERR_WORKSPACE;
   if (!aligned16(workspace)) return MXB_ERR_ALIGNMENT;
   return residual_norm_bwd(d, resid_out, y, norm, post_norm, z, scale, d_resid_out, dn, d_resid, dy, z ? dz : nullptr, dnorm,
-                           post_norm ? dpost_norm : nullptr, scale ? dscale : nullptr, static_cast<float*>(workspace),
+                           post_norm ? dpost_norm : nullptr, scale ? dscale : nullptr, static_cast<float*>(behind_status(workspace)),
                            static_cast<cudaStream_t>(stream));
 }
 
@@ -579,7 +579,7 @@ mxb_status mxb_embedding_fwd(const mxb_embedding_desc* d, const void* tokens, co
   return embedding_fwd(d, tokens, weight, out, static_cast<cudaStream_t>(stream));
 }
 size_t mxb_embedding_bwd_workspace_bytes(const mxb_embedding_desc* d) {
-  return check_embedding_desc(d, true) == MXB_OK ? embedding_bwd_scratch(d) : 0;
+  return check_embedding_desc(d, true) == MXB_OK ? with_status(embedding_bwd_scratch(d)) : 0;
 }
 mxb_status mxb_embedding_bwd(const mxb_embedding_desc* d, const void* tokens, const void* d_out, void* dweight, int32_t adds, void* workspace,
                              size_t workspace_bytes, void* stream) {
@@ -588,9 +588,9 @@ mxb_status mxb_embedding_bwd(const mxb_embedding_desc* d, const void* tokens, co
   if (!dweight) return MXB_ERR_INVALID_ARGUMENT;
   if (d->tokens == 0) return adds ? MXB_OK : zeros(dweight, (size_t)d->V * d->D * element_bytes(d->out_dtype), stream);
   if (!tokens || !d_out) return MXB_ERR_INVALID_ARGUMENT;
-  if (!workspace || workspace_bytes < embedding_bwd_scratch(d)) return MXB_ERR_WORKSPACE;
+  if (!workspace || workspace_bytes < with_status(embedding_bwd_scratch(d))) return MXB_ERR_WORKSPACE;
   if (!aligned16(workspace)) return MXB_ERR_ALIGNMENT;
-  return embedding_bwd(d, tokens, d_out, dweight, adds != 0, workspace, static_cast<cudaStream_t>(stream));
+  return embedding_bwd(d, tokens, d_out, dweight, adds != 0, behind_status(workspace), static_cast<cudaStream_t>(stream));
 }
 static mxb_status check_layer_norm_desc(const mxb_layer_norm_desc* d) {
   if (!d || d->rows < 0 || d->D <= 0 || !(d->eps >= 0.f) || !element_type(d->io_dtype)) return MXB_ERR_INVALID_ARGUMENT;
@@ -607,7 +607,7 @@ mxb_status mxb_layer_norm_fwd(const mxb_layer_norm_desc* d, const void* resid, c
   return layer_norm_fwd(d, resid, x, weight, bias, stream_out, n, static_cast<cudaStream_t>(stream));
 }
 size_t mxb_layer_norm_bwd_workspace_bytes(const mxb_layer_norm_desc* d) {
-  return check_layer_norm_desc(d) == MXB_OK ? layer_norm_scratch(d) : 0;
+  return check_layer_norm_desc(d) == MXB_OK ? with_status(layer_norm_scratch(d)) : 0;
 }
 mxb_status mxb_layer_norm_bwd(const mxb_layer_norm_desc* d, const void* x, const float* weight, const void* d_resid, const void* dn, void* dx,
                               float* dweight, float* dbias, void* workspace, size_t workspace_bytes, void* stream) {
@@ -619,9 +619,9 @@ mxb_status mxb_layer_norm_bwd(const mxb_layer_norm_desc* d, const void* x, const
     return s == MXB_OK ? zeros(dbias, d->D * sizeof(float), stream) : s;
   }
   if (!x || !dn || !dx) return MXB_ERR_INVALID_ARGUMENT;
-  if (!workspace || workspace_bytes < layer_norm_scratch(d)) return MXB_ERR_WORKSPACE;
+  if (!workspace || workspace_bytes < with_status(layer_norm_scratch(d))) return MXB_ERR_WORKSPACE;
   if (!aligned16(workspace)) return MXB_ERR_ALIGNMENT;
-  return layer_norm_bwd(d, x, weight, d_resid, dn, dx, dweight, dbias, workspace, static_cast<cudaStream_t>(stream));
+  return layer_norm_bwd(d, x, weight, d_resid, dn, dx, dweight, dbias, behind_status(workspace), static_cast<cudaStream_t>(stream));
 }
 
 static mxb_status check_linear_ce_desc(const mxb_linear_ce_desc* d) {
@@ -753,7 +753,7 @@ static mxb_status check_m3_block_desc(const mxb_mamba3_desc* d) {
   return MXB_OK;
 }
 size_t mxb_mamba3_block_workspace_bytes(const mxb_mamba3_desc* d) {
-  return check_m3_block_desc(d) == MXB_OK ? mamba3_block_workspace_bytes(d) : 0;
+  return check_m3_block_desc(d) == MXB_OK ? with_status(mamba3_block_workspace_bytes(d)) : 0;
 }
 mxb_status mxb_mamba3_block_conv_fwd(const mxb_mamba3_desc* d, int32_t K, const void* x, const float* w, void* y,
                                      void* stream) {
@@ -771,8 +771,8 @@ mxb_status mxb_mamba3_block_conv_bwd(const mxb_mamba3_desc* d, int32_t K, const 
   if (K < 1 || K > 4) return MXB_ERR_UNSUPPORTED;
   if (!x || !w || !dy || !dx || !dw || !workspace) return MXB_ERR_INVALID_ARGUMENT;
   if (!aligned16(x) || !aligned16(dy) || !aligned16(dx) || !aligned16(workspace)) return MXB_ERR_ALIGNMENT;
-  if (workspace_bytes < mamba3_block_workspace_bytes(d)) return MXB_ERR_WORKSPACE;
-  return mamba3_block_conv(d, K, x, w, nullptr, dy, dx, dw, workspace, static_cast<cudaStream_t>(stream));
+  if (workspace_bytes < with_status(mamba3_block_workspace_bytes(d))) return MXB_ERR_WORKSPACE;
+  return mamba3_block_conv(d, K, x, w, nullptr, dy, dx, dw, behind_status(workspace), static_cast<cudaStream_t>(stream));
 }
 mxb_status mxb_mamba3_block_bc_fwd(const mxb_mamba3_desc* d, float eps, const void* b_proj, const void* c_proj,
                                    const float* b_scale, const float* c_scale, const float* b_bias, const float* c_bias,
@@ -798,9 +798,9 @@ mxb_status mxb_mamba3_block_bc_bwd(const mxb_mamba3_desc* d, float eps, const vo
   if (!aligned16(b_proj) || !aligned16(c_proj) || !aligned16(db) || !aligned16(dc) || !aligned16(db_proj) ||
       !aligned16(dc_proj) || !aligned16(b_scale) || !aligned16(c_scale) || !aligned16(workspace))
     return MXB_ERR_ALIGNMENT;
-  if (workspace_bytes < mamba3_block_workspace_bytes(d)) return MXB_ERR_WORKSPACE;
+  if (workspace_bytes < with_status(mamba3_block_workspace_bytes(d))) return MXB_ERR_WORKSPACE;
   return mamba3_block_bc(d, eps, b_proj, c_proj, b_scale, c_scale, nullptr, nullptr, nullptr, nullptr, db, dc, db_proj,
-                         dc_proj, db_scale, dc_scale, db_bias, dc_bias, workspace, static_cast<cudaStream_t>(stream));
+                         dc_proj, db_scale, dc_scale, db_bias, dc_bias, behind_status(workspace), static_cast<cudaStream_t>(stream));
 }
 mxb_status mxb_mamba3_block_post_fwd(const mxb_mamba3_desc* d, float eps, const void* y, const void* z,
                                      const float* post_norm, void* out, void* stream) {
@@ -820,8 +820,8 @@ mxb_status mxb_mamba3_block_post_bwd(const mxb_mamba3_desc* d, float eps, const 
   if (!aligned16(y) || !aligned16(z) || !aligned16(dout) || !aligned16(dy) || !aligned16(dz) || !aligned16(post_norm) ||
       !aligned16(workspace))
     return MXB_ERR_ALIGNMENT;
-  if (workspace_bytes < mamba3_block_workspace_bytes(d)) return MXB_ERR_WORKSPACE;
-  return mamba3_block_post(d, eps, y, z, post_norm, nullptr, dout, dy, dz, dpost_norm, workspace,
+  if (workspace_bytes < with_status(mamba3_block_workspace_bytes(d))) return MXB_ERR_WORKSPACE;
+  return mamba3_block_post(d, eps, y, z, post_norm, nullptr, dout, dy, dz, dpost_norm, behind_status(workspace),
                            static_cast<cudaStream_t>(stream));
 }
 

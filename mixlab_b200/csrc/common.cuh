@@ -184,6 +184,12 @@ mxb_status allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>& done
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
 // Carves a caller-provided workspace into 256-byte aligned pieces.
+// A workspace leads with the status block, whose first word kernels with bounded waits raise.  A call that keeps no word leaves the block as it
+// is, so that what an earlier call on the same workspace reported stays readable: its scratch lies behind.
+constexpr size_t kStatusBytes = 256;
+inline void* behind_status(void* workspace) { return workspace ? static_cast<char*>(workspace) + kStatusBytes : nullptr; }
+inline size_t with_status(size_t scratch) { return scratch ? scratch + kStatusBytes : 0; }
+
 // Where scratch starts that is written in pieces of 32 bytes and whose base may lie on 16: up to kBaseRoom behind the base.
 constexpr size_t kBaseRoom = 256;
 inline void* round_base_up(void* base) { return reinterpret_cast<void*>(align_up(reinterpret_cast<uintptr_t>(base), kBaseRoom)); }

@@ -180,6 +180,7 @@ struct Workspace {
 // At most this many streams of a device keep a buffer; the one unused for longest goes back to the allocator (it was
 // allocated on the stream that used it, so its memory is handed on in that stream's order).
 constexpr size_t kStreamsPerDevice = 8;
+constexpr int64_t kStatusBytes = 256;  // of the status block that leads a buffer
 using Workspaces = std::map<std::pair<int, void*>, std::shared_ptr<Workspace>>;
 // The workspace of a stream.  The table is only touched under the interpreter lock.
 std::shared_ptr<Workspace> workspace_of(int device, void* stream) {
@@ -214,7 +215,8 @@ unsigned long long capture_of(void* stream) {
 // (allocating results, raising) stays outside the span.
 class Lease {
  public:
-  explicit Lease(const On& on) : w_(workspace_of(on.dev.index(), on.stream)), dev_(on.dev), capture_(capture_of(on.stream)) {
+  explicit Lease(const On& on)
+      : w_(workspace_of(on.dev.index(), on.stream)), dev_(on.dev), stream_(static_cast<cudaStream_t>(on.stream)), capture_(capture_of(on.stream)) {
     py::gil_scoped_release nogil;
     lock_ = std::unique_lock<std::mutex>(w_->busy);
   }
@@ -222,9 +224,19 @@ class Lease {
   void take(size_t nbytes) {
     w_->saved.kind = 0;
     if (!w_->buf.defined() || bytes() < nbytes || w_->capture != capture_) {
+      // (the status block goes along to a larger buffer and starts from zeros; nobody reads that of a capture)
+      Tensor status;
+      if (!capture_) {
+        status = make({kStatusBytes}, at::kByte, dev_);
+        if (w_->buf.defined() && !w_->capture)
+          C10_CUDA_CHECK(cudaMemcpyAsync(ptr(status), ptr(w_->buf), kStatusBytes, cudaMemcpyDeviceToDevice, stream_));
+        else
+          C10_CUDA_CHECK(cudaMemsetAsync(ptr(status), 0, kStatusBytes, stream_));
+      }
       w_->buf = Tensor();
-      w_->buf = make({static_cast<int64_t>(nbytes < 256 ? 256 : nbytes)}, at::kByte, dev_);
+      w_->buf = make({std::max(static_cast<int64_t>(nbytes), kStatusBytes)}, at::kByte, dev_);
       w_->capture = capture_;
+      if (!capture_) C10_CUDA_CHECK(cudaMemcpyAsync(ptr(w_->buf), ptr(status), kStatusBytes, cudaMemcpyDeviceToDevice, stream_));
     }
   }
   // the buffer of a use_saved backward, which still has to hold what the forward described by `want` left in it
@@ -244,6 +256,7 @@ class Lease {
   std::shared_ptr<Workspace> w_;  // (released after the lock: the last owner frees it)
   std::unique_lock<std::mutex> lock_;
   at::Device dev_;
+  cudaStream_t stream_;
   unsigned long long capture_;
 };
 // The current stream's buffer itself (its contents are the caller's from then on).

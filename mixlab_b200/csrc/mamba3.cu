@@ -423,6 +423,7 @@ static size_t carve_m3(M3P& p, void* ws, bool io_f32, size_t partial_floats = 0,
                        float** pc = nullptr, bool windows = false, bool bwd = true, size_t head_scalar_floats = 0,
                        float** hscal = nullptr) {
   Carver cv(ws);
+  cv.take<char>(kStatusBytes);
   if (partial_floats) {  // head-broadcast kernels
     float* a = cv.take<float>(partial_floats);
     float* b2 = cv.take<float>(partial_floats);

@@ -76,7 +76,11 @@ def ir_op_forward(op_type: int, inputs, int_params, *, out_shape, float_params=(
 
 
 def device_status(device=None) -> int:
-    """Blocking read of the device-side error word of the current stream's cached workspace (0 = ok)."""
+    """Blocking read of the device-side error word in the current stream's cached workspace: nonzero if a bounded wait of a kernel gave up
+    and results were left unwritten.  It is the word of the last call on the stream that keeps one - the gated delta scans (``chunk`` > 1) and
+    their op records, the Mamba-3 scan in chunks on the tensor cores, ``linear_cross_entropy``, each with its backward.  Every such call but
+    a ``use_saved`` backward clears it first, so ask behind each that matters; other calls leave it as it is.  0 = ok, also where there was none.
+    What a graph's replays report stays in the graph's own workspace and is not seen here."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else device
     ws = workspace(256, dev)
     torch.cuda.current_stream(dev).synchronize()
