@@ -276,10 +276,11 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// A maximum (-infinity: nothing yet) and the sum of exponentials from it, and another such pair.
+// A maximum (-infinity, 0: nothing yet; +infinity, +infinity: an infinite logit) and the sum of exponentials from it, and another such
+// pair.  The larger maximum's sum is not scaled, so that no infinity meets a difference of infinities or a zero.
 __device__ __forceinline__ void add_sum(float2& a, float2 b) {
   const float t = fmaxf(a.x, b.x);
-  a.y = (a.x == -INFINITY ? 0.f : a.y * ex2((a.x - t) * kLog2e)) + (b.x == -INFINITY ? 0.f : b.y * ex2((b.x - t) * kLog2e));
+  a.y = a.y * (a.x == t ? 1.f : ex2((a.x - t) * kLog2e)) + b.y * (b.x == t ? 1.f : ex2((b.x - t) * kLog2e));
   a.x = t;
 }
 
@@ -583,7 +584,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
 #pragma unroll
           for (int c = 1; c < C::COLS; ++c) top = fmaxf(top, v[c]);
           // (an infinite maximum would make NaNs of the infinities: the exponentials are then 0 or infinite)
-          const float back = fabsf(top) == INFINITY ? 0.f : -top * kLog2e, shift = top == INFINITY ? 0.f : top;
+          const float back = fabsf(top) == INFINITY ? 0.f : -top * kLog2e;
           float s0 = 0.f, s1 = 0.f;
 #pragma unroll
           for (int c = 0; c < C::COLS; c += 2) {
@@ -601,14 +602,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) lce_gem
           float2* buf = halves + slot * 128;
           uint64_t* there = halves_full + slot * 4 + quarter;
           if (half == 1) {
-            buf[mine] = make_float2(shift, sum);
+            buf[mine] = make_float2(top, sum);
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(there);
           } else {
             if (!(ok = wait(there, (uint32_t)(j / C::RING) & 1u))) break;
             const float2 o = buf[mine];
             if (row < live) {
-              float2 both{shift, sum};
+              float2 both{top, sum};
               add_sum(both, o);
               p.part[((size_t)(p.v0 / C::BN) + n) * p.pad + row] = both;
             }

@@ -44,3 +44,30 @@ def test_equal_weights_have_no_part_in_the_rounding(weight):
         sums = 2 * U * (e.shape[1] / 16 + 2) * (e @ other.abs()).norm() / size  # accumulators that are cut
         assert along <= last + hits + others + sums + 8 * U, (name, along.item(), last.item(), hits, others.item(), sums.item())
         assert last + hits + others + sums < 1e-3, name  # (far below what a rounded weight leaves)
+
+
+@pytest.mark.parametrize("n", [40, 1100])
+@pytest.mark.parametrize("D", [64, 63])
+def test_infinite_logits(n, D):
+    """lse of a logit of +infinity is +infinity, wherever its tile stands and however large the others are; one of -infinity has no part."""
+    g = torch.Generator().manual_seed(n)
+    V = 900
+    x = torch.randn(n, D, generator=g)
+    x[:, 0], x[:, 1] = 1.0, 1.0
+    x[1::2, 0] = -1.0
+    for word in (3, 130, 256, 511, 899):
+        for other in (5, 200, 700):
+            for large in (1.0, 250.0):
+                w = 0.1 * torch.randn(V, D, generator=g)
+                w[:, 0] = 0.0
+                w[word, 0], w[other, 1] = float("inf"), large
+                xb, wb = x.to(BF16).cuda(), w.to(BF16).cuda()
+                t = torch.full((n,), other, device="cuda")
+                loss, lse = ops.linear_cross_entropy(xb, wb, t)
+                assert (lse[::2] == float("inf")).all() and (loss[::2] == float("inf")).all(), (word, other, large)
+                rest = torch.cat([wb[:word], wb[word + 1:]]).double()
+                want, want_lse = step_ends.linear_cross_entropy(xb.double(), rest, t - int(word < other))
+                size = (xb.double().abs() @ rest.abs().T).amax(1)[1::2]
+                slack = (12 * size + 16 * size + 128 + V / 2048 + 16) * U  # the logits' sums (64 terms), exponents, the sum of exponentials
+                assert ((lse[1::2].double() - want_lse[1::2]).abs() <= slack).all(), (word, other, large)
+                assert ((loss[1::2].double() - want[1::2]).abs() <= 2 * slack).all(), (word, other, large)
