@@ -2,9 +2,11 @@
 //     y_t = s W[i_t],    dW_v = s sum over the t with i_t = v of dy_t, in the order of t
 // A token outside 0 .. V-1 is padding: its row of y is zero and it has no part in dW.
 //
-// Both are HBM streams.  32768 rows of 2048 columns, bf16 into float32: 60 us, 403 MB at the measured copy rate.  256 rows 4.8 us, of
-// which the call on the host is most.  Their gradient, float32 for 65536 words: 134 us (671 MB: 76 % of the copy rate), of which
-// the sort takes 20 to 25, the sums and the zeros about 95 and the join 8; 2047 rows of 448 columns 13 us, three launches.
+// Both are HBM streams.  32768 rows of 2048 columns, bf16 into float32: 60 us, 403 MB at the measured copy rate.  256 rows 4.6 us, of
+// which the call on the host is most.  Their gradient, float32 for 65536 words: 134 us (671 MB: 76 % of the copy rate); by the counters,
+// which time each launch alone and cold, the sort with zeros beside it takes 34, the sums and the other zeros 90, the join 13; 2047 rows of 448
+// columns 14 us, three launches.  Tokens above 65536, sorted in launches of their own: 131072 rows of 1024 columns 148 us for 82 of bytes.
+// Added to what is there, 32768 rows of 2048 of 11 thousand words: 98 us for 47 of bytes, 25 of them the sort.
 //
 // The gradient sorts the positions by token (stable, so that a token's positions stand in their own order and the sums do not depend
 // on how blocks run), cuts the sorted list into runs of equal length, whatever the tokens' counts are, and adds up the rows of each
@@ -679,8 +681,9 @@ mxb_status embedding_bwd(const mxb_embedding_desc* d, const void* tokens, const 
     // about four entries a thread
     int ctas = 1;
     while (ctas < kClusterMost && (int64_t)ctas * kClusterThreads * 4 < d->tokens) ctas *= 2;
-    // The sort leaves most SMs idle for 10 to 20 us: they write zeros to the last rows of dW meanwhile, those of the words that occur too
-    // (32768 rows of 2048 columns, 65536 words in float32: 138 us without, 134 with).
+    // The sort leaves most SMs idle: they write zeros to the last rows of dW meanwhile, those of the words that occur too - which a dW
+    // smaller than that gets twice - and about as many bytes as fit beside it: 54 MB of 8192 tokens (the launch 28 us for 24 without), 117 of
+    // 32768 (35 for 25), 201 of 65536 (55 for 37; all cold).  32768 rows of 2048 columns, 65536 words in float32: 138 us without, 134 with.
     const size_t row = (size_t)d->D * (d->out_dtype == MXB_F32 ? 4 : 2);
     if (!adds) zero_rows -= (int)std::min<size_t>(d->V, (((size_t)32 << 20) + (size_t)d->tokens * 2560) / row);
     char* dw = static_cast<char*>(dweight);

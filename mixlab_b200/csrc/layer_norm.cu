@@ -4,11 +4,12 @@
 //     dh = dh' + k (t - mean t - u mean(t u)),   dw = sum dn u,   db = sum dn     over the rows
 // (dh' the gradient that reaches h from its other readers).
 //
-// HBM streams: 32768 rows of 2048 columns in bf16 with the addition to the stream 88 us (537 MB: 93 % of the measured copy rate), their
+// HBM streams: 32768 rows of 2048 columns in bf16 with the addition to the stream 89 us (537 MB: 92 % of the measured copy rate), their
 // gradients 106 (537 MB: 78 %), 5 of them in the column sums' own launch; 4001 rows of 449 columns in float32 9.7 us; one row 5.2,
 // the call on the host.  The gradients are bound by instructions and the sums across a row (62 % of the issue slots, 48 % of the
 // LSU pipe): two rows under way instead of one, and sums of each warp around its own mean, joined behind one barrier instead of two,
-// were no faster.
+// were no faster.  Wide rows: 2048 of 8192 columns in bf16 33 us, their gradients 39 (134 MB: 21); of 16384 columns 49 and 187 (41).  The last
+// holds six arrays of 32 floats a thread in 128 registers and spills up to 2 KB of them; float32, 16384 columns: 111 and 295 (82).
 //
 // A row is read once and held by TPR threads in pieces of eight columns, the next row is requested while one is worked on, narrow
 // rows share a CTA.  The mean is taken first and the squares of what is left after it, both from registers: no difference of two

@@ -11,11 +11,12 @@
 // bf16 to a workspace of bounded size, then dx += g W and dW = g^T x from it (a second part of g, which would leave the results' own
 // rounding alone, would be two products more beside three).
 //
-// What bounds it is the tensor pipe at the clock that the power limit leaves: 28672 tokens, 65536 words of 1024 columns 2.69 ms
-// (1430 TFLOP/s; cuBLAS's product alone runs at 1402 for seconds on end); the gradients for 50001 words 7.1 ms (1240), where g goes
-// through HBM three times.  512 tokens, 32768 words: 36 us, of which four rounds of tiles take 18, the first copies and the last
-// tile's exponentials 5, the join and its launch 6.  2048 tokens, 5003 words of 448 columns in float32: 173 us for 96 of products; each of
-// the three products waits 4 us for its first stage and ends with an epilogue of 3.
+// What bounds it is the tensor pipe at the clock that the power limit leaves: 28672 tokens, 65536 words of 1024 columns 2.70 ms
+// (1425 TFLOP/s; cuBLAS's product alone runs at 1402 for seconds on end); the gradients for 50001 words 7.1 to 7.4 ms (1240 to 1190),
+// where g goes through HBM three times.  512 tokens, 32768 words: 36 us; by the counters, which time each launch alone and cold, the products
+// take 32 - four rounds of tiles 18 of them, the first copies and the last tile's exponentials 5, 9 not taken apart - and the join 7.
+// 2048 tokens, 5003 words of 448 columns in float32: 173 us for 96 of products; each of the three products waits 4 us for its first stage
+// and ends with an epilogue of 3; packing is 13 of it, the shares 10 (counters).  The loss of these 56 us for 33.
 // float32 tensors: every operand is split into three bf16 parts (24 bits and more), and six products of parts, those above
 // 2^-24, are added up.  An accumulator in TMEM is cut, not rounded, with every product added to it, so it takes the products
 // of 128 terms, small ones first, and is handed over: the sums of those are float32 in registers (2048 tokens, 5003 words of 448: gradients
@@ -890,7 +891,8 @@ static Plan plan(const mxb_linear_ce_desc* d, const void* x, const void* weight,
   if (!bwd && !q.pack_w) q.piece = (int)all;
   q.pieces = (int)((d->V + (int64_t)q.piece - 1) / q.piece);
   // float32, tiles of dx and dW: narrow ones start sooner (a third of the bytes before the first product), wide ones have fewer reads
-  // (2048 tokens, 5003 words of 448: gradients 154 us with narrow, 166 with wide ones; 4096, 32000 words: 1748 and 1560)
+  // (2048 tokens, 5003 words of 448: gradients 159 us with narrow, 165 with wide ones on one GPU, up to 173 on others; 4096, 32000 words:
+  // 1705 and 1537)
   const int64_t words = std::min<int64_t>(q.piece, d->V);
   if (q.f32 && (words + 255) / 256 * d_tiles < kPairs) q.BD = 128;
   // float32, tiles of logits: those of 128 columns take a little over half as long as those of 256 (their operands' reads bound them), which pays
@@ -1005,13 +1007,13 @@ static mxb_status run(const mxb_linear_ce_desc* d, const Plan& q, PackP& pk, con
     p.V = d->V;
     p.pad = pad;
     p.D = D;
-    // as many rows of tiles as keep their x in L2 (24 MB): W is read once for all of them (28672 tokens, 65536 words of 1024: loss 2.69 ms,
+    // as many rows of tiles as keep their x in L2 (24 MB): W is read once for all of them (28672 tokens, 65536 words of 1024: loss 2.70 ms,
     // by groups of eight 2.83)
     p.group = (int)std::min<int64_t>(64, std::max<int64_t>(8, (24 << 20) / (256 * 2 * (int64_t)q.Dp * q.parts)));
     Maps maps;
     std::memset(&maps, 0, sizeof maps);
-    bool ok = (q.direct ? make_map(&maps.a, pk.x, D, q.N, 1, D, q.N * D, 128) : make_map(&maps.a, q.xc, q.Dp, pad, q.parts, q.Dp, pad * q.Dp, 128)) && make_map(&maps.b, w, q.Dp, w_rows, q.parts, q.Dp, w_part, BN / 2);
-    if (!ok) return MXB_ERR_UNSUPPORTED;
+    const bool ok = q.direct ? make_map(&maps.a, pk.x, D, q.N, 1, D, q.N * D, 128) : make_map(&maps.a, q.xc, q.Dp, pad, q.parts, q.Dp, pad * q.Dp, 128);
+    if (!ok || !make_map(&maps.b, w, q.Dp, w_rows, q.parts, q.Dp, w_part, BN / 2)) return MXB_ERR_UNSUPPORTED;
     p.N = rows;
     p.K = D;
     p.b_row0 = w_row0;
